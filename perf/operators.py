@@ -152,8 +152,8 @@ def work(case) -> dict:
     hq, lens = case["hq"], _lens(case)
     if case["kind"] == "decode":
         total = sum(lens)
-        return {"bytes": 2 * row * hkv * total + 4 * D * hq * len(lens) + 4 * (-(-total // case["block_size"]) + len(lens)),
-                "flops": 4 * D * hq * total}
+        pages = -(-total // case["block_size"]) + len(lens)
+        return {"bytes": 2 * row * hkv * total + 4 * D * hq * len(lens) + 4 * pages, "flops": 4 * D * hq * total}
     cached = case["cached"]
     pairs = sum(n * cached + n * (n + 1) // 2 for n in lens)
     total = sum(lens)
@@ -183,11 +183,12 @@ def _pages(lens, bs, seed):
 
 
 def _empty_cache(blocks, case):
-    """codes and scales of keys and values, as bytes that no row has been written to."""
+    """Codes and scales of keys and values, as bytes that no row has been written to, and the codes' values."""
     def byte(width):
         return torch.zeros((blocks, case["hkv"], case["block_size"], width), dtype=torch.uint8, device="cuda")
 
-    return {"k_codes": byte(D // 2), "k_scales": byte(D // 32), "v_codes": byte(D // 2), "v_scales": byte(D // 32)}
+    return {"k_codes": byte(D // 2), "k_scales": byte(D // 32), "v_codes": byte(D // 2), "v_scales": byte(D // 32),
+            "grid": torch.tensor(GRID + tuple(-x for x in GRID), device="cuda")}
 
 
 def _channels(gen):
@@ -328,20 +329,21 @@ def _store(state, k, v, slots):
     vs[block, :, tile, :, t] = scale
 
 
-def _values(code, scale):
+def _values(grid, code, scale):
     """fp32 values [.., 4, 32] of codes and scale bytes."""
-    c = (code & 7).int()
-    x = torch.where(c < 2, 0.5 * c, torch.ldexp(1.0 + 0.5 * (c & 1), (c >> 1) - 1)) * (1.0 - 2.0 * (code >> 3))
-    return torch.where(scale[..., None] == 255, math.nan, torch.ldexp(x, scale[..., None].int() - 127))
+    one = torch.ones_like(scale, dtype=torch.float32)
+    step = torch.where(scale == 255, math.nan, torch.ldexp(one, scale.int() - 127))
+    return grid[code.int()] * step[..., None]
 
 
 def _load(state, slots):
     block, tile, t = _at(state, slots)
     kc, ks, vc, vs = _views(state)
     byte = kc[block, :, tile, t]
-    k = _values(torch.stack((byte & 15, byte >> 4), -1).unflatten(-2, (4, 16)).flatten(-2), ks[block, :, tile, t % 4, :, t // 4])
+    k = _values(state["grid"], torch.stack((byte & 15, byte >> 4), -1).unflatten(-2, (4, 16)).flatten(-2),
+                ks[block, :, tile, t % 4, :, t // 4])
     byte = vc[block, :, tile, :, t].unflatten(-1, (4, 16))
-    v = _values(torch.cat((byte & 15, byte >> 4), -1), vs[block, :, tile, :, t])
+    v = _values(state["grid"], torch.cat((byte & 15, byte >> 4), -1), vs[block, :, tile, :, t])
     live = (slots >= 0)[:, None, None]
     return torch.where(live, k.flatten(-2), 0.0), torch.where(live, v.flatten(-2), 0.0)
 
@@ -373,10 +375,10 @@ def _context(state):
     tables = state["tables"].long()
     n, hkv = tables.shape[0], kc.shape[1]
     byte = kc[tables]  # [n, blocks, hkv, tiles, 16, 64]
-    k = _values(torch.stack((byte & 15, byte >> 4), -1).unflatten(-2, (4, 16)).flatten(-2),
+    k = _values(state["grid"], torch.stack((byte & 15, byte >> 4), -1).unflatten(-2, (4, 16)).flatten(-2),
                 ks[tables].permute(0, 1, 2, 3, 6, 4, 5).flatten(4, 5)).flatten(-2)
     byte = vc[tables].unflatten(-2, (4, 16))  # [n, blocks, hkv, tiles, 4, 16, 16]
-    v = _values(torch.cat((byte & 15, byte >> 4), -2).permute(0, 1, 2, 3, 6, 4, 5),
+    v = _values(state["grid"], torch.cat((byte & 15, byte >> 4), -2).permute(0, 1, 2, 3, 6, 4, 5),
                 vs[tables].transpose(-1, -2)).flatten(-2)
     return (x.permute(0, 2, 1, 3, 4, 5).reshape(n, hkv, -1, D).contiguous() for x in (k, v))
 
