@@ -353,6 +353,12 @@ def _plain_store(state):
     return tuple(x.bfloat16() for x in _load(state, state["slots"]))
 
 
+def _rounded(x):
+    """bf16 of 64-bit values, rounded once (a cast by way of 32 bits rounds twice)."""
+    mantissa, exponent = torch.frexp(x)
+    return torch.ldexp((mantissa * 256).round(), exponent - 8).bfloat16()
+
+
 def _plain_rope(state):
     """In 64 bits: a key next to a border of the codes goes by its exact value."""
     angle = state["table"][state["positions"]].double()[:, None]
@@ -362,7 +368,7 @@ def _plain_rope(state):
         x = x.double()
         y = x / torch.sqrt((x * x).mean(-1, keepdim=True) + EPS) * weight.double()
         lo, hi = y[..., : D // 2], y[..., D // 2:]
-        return torch.cat((lo * cos - hi * sin, hi * cos + lo * sin), -1).bfloat16()
+        return _rounded(torch.cat((lo * cos - hi * sin, hi * cos + lo * sin), -1))
 
     q, k = rotated(state["q"], state["q_weight"]), rotated(state["k"], state["k_weight"])
     _store(state, k, state["v"], state["slots"])
@@ -439,6 +445,16 @@ def _nearest(row):
     return out
 
 
+def _bf16(x):
+    """The bf16 number nearest to each 64-bit value, of two as near the one of even bits: of the cast's and its neighbours."""
+    bits = x.bfloat16().view(torch.int16)
+    near = torch.stack((bits, bits - 1, bits + 1), -1)
+    off = (near.view(torch.bfloat16).double() - x[..., None]).abs()
+    nearest = off == off.min(-1, keepdim=True).values
+    pick = (2 * nearest.int() + (near % 2 == 0).int()).argmax(-1, keepdim=True)
+    return near.gather(-1, pick)[..., 0].contiguous().view(torch.bfloat16).double()
+
+
 def _cached(state, head, slots):
     """Keys and values [tokens, 128] of one kv head at the slots, in 64 bits, byte by byte."""
     bs, hkv = state["case"]["block_size"], state["case"]["hkv"]
@@ -475,7 +491,7 @@ def exact(case, seed):
 
             q, k = turned(q, state["q_weight"]), turned(k, state["k_weight"])
         none = state["slots"] < 0
-        rows = [_nearest(k.bfloat16().double()), _nearest(v)]  # what is stored is the bf16 key
+        rows = [_nearest(_bf16(k) if case["kind"] == "rope" else k), _nearest(v)]  # what is stored is the bf16 key
         for x in rows:
             x[none] = 0
         return tuple(rows) if case["kind"] == "store" else [q, *([k] if case["keys"] else []), *rows]
