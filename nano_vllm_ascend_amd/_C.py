@@ -11,6 +11,7 @@ from __future__ import annotations
 import ctypes
 import os
 from pathlib import Path
+from typing import NamedTuple
 
 import torch
 
@@ -85,6 +86,32 @@ _SIGNATURES = {
          _c_ptr]),
     "nvamd_embed_rows": (
         _c_int, [_c_ptr, _c_ptr, _c_i64, _c_int, _c_ptr, _c_i64, _c_int, _c_ptr, _c_int, _c_int, _c_ptr]),
+    "nvamd_kv_cache_write_fp4": (
+        _c_int,
+        [_c_ptr, _c_i64, _c_ptr, _c_i64, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_int, _c_ptr, _c_int, _c_int,
+         _c_int, _c_ptr],
+    ),
+    "nvamd_kv_cache_read_fp4": (
+        _c_int,
+        [_c_ptr, _c_i64, _c_ptr, _c_i64, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_int, _c_ptr, _c_int, _c_int,
+         _c_int, _c_ptr],
+    ),
+    "nvamd_qk_norm_rope_fp4": (
+        _c_int,
+        [_c_ptr, _c_i64, _c_ptr, _c_i64, _c_ptr, _c_i64, _c_ptr, _c_i64, _c_ptr, _c_i64, _c_ptr, _c_ptr, _c_ptr,
+         _c_ptr, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_int, _c_ptr, _c_int, _c_int, _c_int, _c_int,
+         _c_float, _c_ptr],
+    ),
+    "nvamd_paged_decode_fp4": (
+        _c_int,
+        [_c_ptr, _c_i64, _c_ptr, _c_i64, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_int, _c_ptr, _c_int, _c_int,
+         _c_ptr, _c_int, _c_int, _c_int, _c_int, _c_float, _c_int, _c_ptr, _c_size, _c_ptr],
+    ),
+    "nvamd_paged_prefill_fp4": (
+        _c_int,
+        [_c_ptr, _c_i64, _c_ptr, _c_i64, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_int, _c_ptr, _c_int, _c_int,
+         _c_ptr, _c_ptr, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_float, _c_ptr],
+    ),
     "nvamd_qk_norm_rope": (
         _c_int,
         [_c_ptr, _c_i64, _c_ptr, _c_i64, _c_ptr, _c_i64, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_ptr,
@@ -542,6 +569,214 @@ def paged_prefill(out: torch.Tensor, q: torch.Tensor, key_cache: torch.Tensor, v
         kv_lens.data_ptr(), n_seqs, int(max_q_len), q.shape[1], hkv, d, float(scale), _stream(),
     )
     _check(status, "nvamd_paged_prefill")
+    return out
+
+
+# ------------------------------------------------------------------ KV cache held in 4 bits
+# The same path over pages of FP4 codes with a power-of-two scale per 32 dims (format and layout: nvamd.h).
+FP4_ROW_BYTES, FP4_ROW_SCALES = 64, 4  # of a head vector
+
+
+class Fp4Pages(NamedTuple):
+    """The keys or the values of one layer in 4 bits: ``codes`` uint8 [blocks, kv heads, block_size, 64] and ``scales``
+    uint8 [blocks, kv heads, block_size, 4], contiguous.  Pages are opaque (``kv_cache_read_fp4`` gives their values)."""
+
+    codes: torch.Tensor
+    scales: torch.Tensor
+
+    @property
+    def shape(self) -> tuple[int, int, int, int]:
+        """[blocks, block_size, kv heads, head_dim], as a bf16 cache of these pages has it."""
+        nb, hkv, bs, width = self.codes.shape
+        return nb, bs, hkv, 2 * width
+
+
+def _fp4_pages(key_pages: Fp4Pages, value_pages: Fp4Pages) -> tuple[int, int, int, int]:
+    """Checks the pages of a layer; returns [blocks, block_size, kv heads, head_dim]."""
+    if not (isinstance(key_pages, Fp4Pages) and isinstance(value_pages, Fp4Pages)):
+        raise ValueError("key and value pages must be Fp4Pages")
+    shape = key_pages.codes.shape
+    if len(shape) != 4 or shape[3] != FP4_ROW_BYTES or value_pages.codes.shape != shape:
+        raise ValueError(f"codes must be [blocks, kv heads, block_size, {FP4_ROW_BYTES}] for keys and values, got "
+                         f"{tuple(shape)} and {tuple(value_pages.codes.shape)}")
+    scales = (*shape[:3], FP4_ROW_SCALES)
+    if key_pages.scales.shape != scales or value_pages.scales.shape != scales:
+        raise ValueError(f"scales must be {scales}, got {tuple(key_pages.scales.shape)} and "
+                         f"{tuple(value_pages.scales.shape)}")
+    for t in (*key_pages, *value_pages):
+        if t.dtype is not torch.uint8 or not t.is_contiguous():
+            raise ValueError("pages must be contiguous uint8 tensors")
+    return key_pages.shape
+
+
+def _on_current_device(*tensors: torch.Tensor | None) -> None:
+    """Every launch goes to the current device's current stream: its tensors have to live there."""
+    device = None
+    for t in tensors:
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise ValueError("every tensor must be on the GPU")
+        if device is None:
+            device = torch.cuda.current_device()
+        if t.get_device() != device:
+            raise ValueError(f"a tensor is on device {t.get_device()}, the current device is {device}")
+
+
+def _heads(name: str, t: torch.Tensor, rows: int, heads: int, d: int) -> int:
+    """Checks a [T, heads, D] bf16 view of dense rows; returns its row stride."""
+    if t.dtype is not torch.bfloat16:
+        raise ValueError(f"{name} must be bfloat16, got {t.dtype}")
+    if t.shape != (rows, heads, d):
+        raise ValueError(f"{name} must be {(rows, heads, d)}, got {tuple(t.shape)}")
+    stride = t.stride()
+    if rows and (stride[2] != 1 or (heads > 1 and stride[1] != d)):
+        raise ValueError(f"rows of {name} {tuple(t.shape)} are not dense")
+    return stride[0] if rows > 1 else max(stride[0], heads * d)
+
+
+def _page_slots(slot_mapping: torch.Tensor, rows: int, shape) -> None:
+    if (slot_mapping.dtype is not torch.int64 or slot_mapping.dim() != 1 or slot_mapping.numel() != rows
+            or not slot_mapping.is_contiguous()):
+        raise ValueError(f"slot_mapping must be contiguous int64 [{rows}], got {slot_mapping.dtype} "
+                         f"{tuple(slot_mapping.shape)}")
+    if _range_checks and _checking():
+        check_slots(slot_mapping, shape[0] * shape[1])
+
+
+def kv_cache_write_fp4(key_states: torch.Tensor, value_states: torch.Tensor, key_pages: Fp4Pages,
+                       value_pages: Fp4Pages, slot_mapping: torch.Tensor) -> None:
+    """Rows [T, Hkv, 128] of bf16 keys and values, quantised into the pages at their slots (-1: padding, skipped; no slot
+    twice in a call)."""
+    lib = load()
+    shape = nb, bs, hkv, d = _fp4_pages(key_pages, value_pages)
+    t = key_states.shape[0]
+    strides = _heads("key_states", key_states, t, hkv, d), _heads("value_states", value_states, t, hkv, d)
+    _page_slots(slot_mapping, t, shape)
+    _on_current_device(key_states, value_states, *key_pages, *value_pages, slot_mapping)
+    _check(lib.nvamd_kv_cache_write_fp4(
+        key_states.data_ptr(), strides[0], value_states.data_ptr(), strides[1], key_pages.codes.data_ptr(),
+        key_pages.scales.data_ptr(), value_pages.codes.data_ptr(), value_pages.scales.data_ptr(), nb, bs,
+        slot_mapping.data_ptr(), t, hkv, d, _stream()), "nvamd_kv_cache_write_fp4")
+
+
+def kv_cache_read_fp4(key_pages: Fp4Pages, value_pages: Fp4Pages, slot_mapping: torch.Tensor,
+                      k_out: torch.Tensor | None = None,
+                      v_out: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """The bf16 keys and values [T, Hkv, 128] that the pages hold at the slots (zeros for -1)."""
+    lib = load()
+    shape = nb, bs, hkv, d = _fp4_pages(key_pages, value_pages)
+    t = slot_mapping.numel()
+    _page_slots(slot_mapping, t, shape)
+    k, v = (torch.empty((t, hkv, d), dtype=torch.bfloat16, device=key_pages.codes.device) if out is None else out
+            for out in (k_out, v_out))
+    strides = _heads("k_out", k, t, hkv, d), _heads("v_out", v, t, hkv, d)
+    _on_current_device(k, v, *key_pages, *value_pages, slot_mapping)
+    _check(lib.nvamd_kv_cache_read_fp4(
+        k.data_ptr(), strides[0], v.data_ptr(), strides[1], key_pages.codes.data_ptr(), key_pages.scales.data_ptr(),
+        value_pages.codes.data_ptr(), value_pages.scales.data_ptr(), nb, bs, slot_mapping.data_ptr(), t, hkv, d,
+        _stream()), "nvamd_kv_cache_read_fp4")
+    return k, v
+
+
+def qk_norm_rope_fp4(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_weight: torch.Tensor,
+                     k_weight: torch.Tensor, positions: torch.Tensor, cos_sin: torch.Tensor, eps: float,
+                     key_pages: Fp4Pages, value_pages: Fp4Pages, slot_mapping: torch.Tensor, *,
+                     q_out: torch.Tensor | None = None, k_out: torch.Tensor | None = None) -> torch.Tensor:
+    """RoPE(RMSNorm_head(x) * w) of q and k in one pass that also stores the rotated k and the raw v in the pages.
+
+    Returns the rotated q: ``q_out``, which may be q itself, or a new tensor.  The rotated k is written
+    only to the pages unless ``k_out`` (which may be k itself) asks for it.  64-bit arithmetic, one rounding to bf16."""
+    lib = load()
+    shape = nb, bs, hkv, d = _fp4_pages(key_pages, value_pages)
+    if q.dim() != 3:
+        raise ValueError(f"q must be [T, heads, D], got {tuple(q.shape)}")
+    t, hq, _ = q.shape
+    if q_out is None:
+        q_out = torch.empty((t, hq, d), dtype=torch.bfloat16, device=q.device)
+    rows = [("q_out", q_out, hq), ("q", q, hq), ("k", k, hkv), ("v", v, hkv)]
+    qo_stride, q_stride, k_stride, v_stride = (_heads(name, x, t, h, d) for name, x, h in rows)
+    ko_stride = 0 if k_out is None else _heads("k_out", k_out, t, hkv, d)
+    for out, x, strides in ((q_out, q, (qo_stride, q_stride)), (k_out, k, (ko_stride, k_stride))):
+        if out is not None and out.data_ptr() == x.data_ptr() and strides[0] != strides[1]:
+            raise ValueError("an output in place of its input must have the input's row stride")
+    for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
+        if w.dtype is not torch.bfloat16 or w.numel() != d or not w.is_contiguous():
+            raise ValueError(f"{name} must be contiguous bf16 [{d}]")
+    if positions.dtype is not torch.int64 or positions.numel() != t or not positions.is_contiguous():
+        raise ValueError(f"positions must be contiguous int64 [{t}]")
+    if (cos_sin.dtype is not torch.float32 or cos_sin.dim() != 2 or cos_sin.shape[1] != d
+            or not cos_sin.is_contiguous()):
+        raise ValueError("cos_sin must be contiguous fp32 [max_positions, head_dim]")
+    _page_slots(slot_mapping, t, shape)
+    _on_current_device(q, k, v, q_out, k_out, q_weight, k_weight, positions, cos_sin, *key_pages, *value_pages,
+                       slot_mapping)
+    if _range_checks and _checking():
+        check_positions(positions, cos_sin.shape[0])
+    _check(lib.nvamd_qk_norm_rope_fp4(
+        q_out.data_ptr(), qo_stride, _ptr(k_out), ko_stride, q.data_ptr(), q_stride, k.data_ptr(), k_stride,
+        v.data_ptr(), v_stride, q_weight.data_ptr(), k_weight.data_ptr(), positions.data_ptr(), cos_sin.data_ptr(),
+        cos_sin.shape[0], key_pages.codes.data_ptr(), key_pages.scales.data_ptr(), value_pages.codes.data_ptr(),
+        value_pages.scales.data_ptr(), nb, bs, slot_mapping.data_ptr(), t, hq, hkv, d, float(eps), _stream()),
+        "nvamd_qk_norm_rope_fp4")
+    return q_out
+
+
+def _fp4_attention_args(out, q, key_pages, value_pages, block_tables, seqs: int):
+    """Checked arguments that decode and prefill share, up to the block tables."""
+    nb, bs, hkv, d = _fp4_pages(key_pages, value_pages)
+    if q.dim() != 3 or out.shape != q.shape:
+        raise ValueError(f"q/out shape mismatch: {tuple(q.shape)} vs {tuple(out.shape)}")
+    t, hq, _ = q.shape
+    out_stride, q_stride = _heads("out", out, t, hq, d), _heads("q", q, t, hq, d)
+    if block_tables.dtype is not torch.int32 or block_tables.dim() != 2 or block_tables.shape[0] < seqs:
+        raise ValueError(f"block_tables must be int32 [{seqs}, W]")
+    if block_tables.stride(1) != 1 and block_tables.shape[1] > 1:
+        raise ValueError("block_tables rows must be dense")
+    width = block_tables.shape[1]
+    return (out.data_ptr(), out_stride, q.data_ptr(), q_stride, key_pages.codes.data_ptr(),
+            key_pages.scales.data_ptr(), value_pages.codes.data_ptr(), value_pages.scales.data_ptr(), nb, bs,
+            block_tables.data_ptr(), max(block_tables.stride(0), width), width), (hq, hkv, d)
+
+
+def paged_decode_fp4(out: torch.Tensor, q: torch.Tensor, key_pages: Fp4Pages, value_pages: Fp4Pages,
+                     block_tables: torch.Tensor, context_lens: torch.Tensor, scale: float, max_context_len: int,
+                     workspace: torch.Tensor) -> torch.Tensor:
+    """``paged_decode`` over pages of 4 bits; the workspace is the same (``alloc_paged_decode_workspace``)."""
+    lib = load()
+    b = q.shape[0]
+    args, heads = _fp4_attention_args(out, q, key_pages, value_pages, block_tables, b)
+    if block_tables.shape[0] != b:
+        raise ValueError(f"block_tables must be int32 [{b}, W]")
+    if context_lens.dtype is not torch.int32 or context_lens.numel() != b or not context_lens.is_contiguous():
+        raise ValueError(f"context_lens must be contiguous int32 [{b}]")
+    if not workspace.is_contiguous():
+        raise ValueError("workspace must be contiguous")
+    _on_current_device(out, q, *key_pages, *value_pages, block_tables, context_lens, workspace)
+    if _range_checks and _checking():
+        check_paged_context(block_tables, context_lens, args[8], args[9], int(max_context_len))
+    _check(lib.nvamd_paged_decode_fp4(*args, context_lens.data_ptr(), b, *heads, float(scale), int(max_context_len),
+                                      workspace.data_ptr(), workspace.numel() * workspace.element_size(), _stream()),
+           "nvamd_paged_decode_fp4")
+    return out
+
+
+def paged_prefill_fp4(out: torch.Tensor, q: torch.Tensor, key_pages: Fp4Pages, value_pages: Fp4Pages,
+                      block_tables: torch.Tensor, cu_seqlens_q: torch.Tensor, kv_lens: torch.Tensor, max_q_len: int,
+                      scale: float) -> torch.Tensor:
+    """``paged_prefill`` over pages of 4 bits: queries are the last q_len of kv_len positions, all keys in the cache."""
+    lib = load()
+    if cu_seqlens_q.dtype is not torch.int32 or cu_seqlens_q.dim() != 1 or not cu_seqlens_q.is_contiguous():
+        raise ValueError("cu_seqlens_q must be contiguous int32 [n + 1]")
+    n = cu_seqlens_q.numel() - 1
+    args, heads = _fp4_attention_args(out, q, key_pages, value_pages, block_tables, n)
+    if n < 0 or kv_lens.dtype is not torch.int32 or kv_lens.numel() < n or not kv_lens.is_contiguous():
+        raise ValueError("kv_lens must be contiguous int32, one per sequence")
+    _on_current_device(out, q, *key_pages, *value_pages, block_tables, cu_seqlens_q, kv_lens)
+    if _range_checks and _checking():
+        check_paged_context(block_tables[:n], kv_lens[:n], args[8], args[9])
+    _check(lib.nvamd_paged_prefill_fp4(*args, cu_seqlens_q.data_ptr(), kv_lens.data_ptr(), n, q.shape[0],
+                                       int(max_q_len), *heads, float(scale), _stream()), "nvamd_paged_prefill_fp4")
     return out
 
 

@@ -7,6 +7,9 @@ and raise ValueError on the same shape mismatches:
 The ``Npu*`` names are kept as aliases so code written against the reference
 imports unchanged.  ``qk_norm_rope`` fuses q_norm, k_norm, RoPE and the KV
 store (nv/models/qwen3.py:83-96) into one kernel.
+
+Each takes either kind of cache: a PagedKVCache (bf16 tensors) or an
+Fp4PagedKVCache, whose layers are ``Fp4Pages`` of 4-bit codes and scales.
 """
 from __future__ import annotations
 
@@ -62,6 +65,10 @@ def qk_norm_rope(q, k, v, q_norm: RMSNorm, k_norm: RMSNorm, rotary: RotaryEmbedd
     kc = vc = None
     if kv_cache is not None:
         kc, vc = kv_cache.get_physical_cache(layer_idx)
+        if isinstance(kc, _C.Fp4Pages):
+            _C.qk_norm_rope_fp4(q, k, v, q_norm.weight, k_norm.weight, positions, rotary.cos_sin,
+                                q_norm.variance_epsilon, kc, vc, slot_mapping, q_out=q, k_out=k)
+            return
     _C.qk_norm_rope(q, k, q_norm.weight, k_norm.weight, positions, rotary.cos_sin, q_norm.variance_epsilon,
                     v=v if kc is not None else None, key_cache=kc, value_cache=vc,
                     slot_mapping=slot_mapping if kc is not None else None)
@@ -103,6 +110,9 @@ class HipPagedAttention(nn.Module):
         out = torch.empty_like(q) if out is None else out
         if context_lens.dtype is not torch.int32:
             context_lens = context_lens.to(torch.int32)
+        if isinstance(key_cache, _C.Fp4Pages):
+            return _C.paged_decode_fp4(out, q, key_cache, value_cache, block_tables, context_lens, self.scale,
+                                       max_context_len, workspace)
         return _C.paged_decode(out, q, key_cache, value_cache, block_tables, context_lens, self.scale,
                                max_context_len, workspace)
 
@@ -113,10 +123,15 @@ class HipPagedAttention(nn.Module):
                     workspace: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
         """One launch for a decode batch: q/k RMSNorm + RoPE, the KV store of post-RoPE k and raw v at
         slot_mapping, then this attention -- bit-identical to qk_norm_rope followed by forward().
-        q, k, v are the raw projection rows and are left unmodified."""
+        q, k, v are the raw projection rows and are left unmodified.  A 4-bit cache takes two launches."""
         total_tokens, num_heads, head_dim = q.shape
         if num_heads != self.num_heads or head_dim != self.head_dim:
             raise ValueError(f"query shape mismatch: got {tuple(q.shape)}")
+        if isinstance(key_cache, _C.Fp4Pages):
+            rotated = _C.qk_norm_rope_fp4(q, k, v, q_norm.weight, k_norm.weight, positions, rotary.cos_sin,
+                                          q_norm.variance_epsilon, key_cache, value_cache, slot_mapping)
+            return self.forward(rotated, key_cache, value_cache, block_tables, context_lens, max_context_len, workspace,
+                                out)
         if max_context_len is None:
             max_context_len = block_tables.shape[1] * key_cache.shape[1]
         if context_lens.device != q.device:
@@ -160,6 +175,9 @@ class HipBatchPrefillAttention(nn.Module):
         if attn_metadata.use_paged_prefill:
             if key_cache is None or value_cache is None:
                 raise ValueError("paged prefill requires physical key/value cache")
+            if isinstance(key_cache, _C.Fp4Pages):
+                return _C.paged_prefill_fp4(out, q, key_cache, value_cache, attn_metadata.block_tables,
+                                            attn_metadata.cu_seqlens_q, attn_metadata.context_lens, max_q, self.scale)
             return _C.paged_prefill(out, q, key_cache, value_cache, attn_metadata.block_tables,
                                     attn_metadata.cu_seqlens_q, attn_metadata.context_lens, max_q, self.scale)
         return _C.varlen_prefill(out, q, k, v, attn_metadata.cu_seqlens_q, max_q, self.scale)

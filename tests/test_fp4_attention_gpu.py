@@ -1,0 +1,417 @@
+"""Attention over the KV cache held in 4 bits, against the 64-bit oracle on the values that the pages hold.
+
+Tolerances are the bound that oracle.fp4_ref.attention derives for each element from the roundings that an evaluation with
+bf16 weights and results makes."""
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+from nano_vllm_ascend_amd import _C
+from nano_vllm_ascend_amd.block_manager import PagedKVCacheMetadata
+from nano_vllm_ascend_amd.layers import HipBatchPrefillAttention, HipPagedAttention, RMSNorm, RotaryEmbedding
+from nano_vllm_ascend_amd.paged_kv_cache import Fp4PagedKVCache
+from oracle import fp4_ref
+
+pytestmark = pytest.mark.gpu
+SCALE = 128 ** -0.5
+
+
+@pytest.fixture(autouse=True)
+def clean_word(device):
+    _C.clear_index_errors()
+    yield
+    _C.clear_index_errors()
+    torch.cuda.synchronize()
+
+
+class Batch:
+    """Sequences of the given contexts in pages of a seeded order; rows past a context and pages of nobody hold stale bytes,
+    scales of NaN among them."""
+
+    def __init__(self, device, lens, hq, hkv, bs, seed=0, spread=0.5, extra_width=0):
+        gen = torch.Generator().manual_seed(seed)
+        need = [-(-n // bs) for n in lens]
+        self.nb = sum(need) + 2
+        order = torch.randperm(self.nb, generator=gen)
+        self.tables = torch.zeros(len(lens), max(max(need), 1) + extra_width, dtype=torch.int32)
+        at = 0
+        for i, n in enumerate(need):
+            self.tables[i, :n] = order[at:at + n]
+            at += n
+        self.pages = tuple(torch.randint(0, 256, (self.nb, hkv, bs, w), generator=gen, dtype=torch.uint8)
+                           for w in (64, 4, 64, 4))
+        for p in self.pages[1::2]:
+            p[p > 200] = 255
+        self.slots = [self.tables[i, torch.arange(n) // bs].long() * bs + torch.arange(n) % bs
+                      for i, n in enumerate(lens)]
+        slots = torch.cat(self.slots)
+        k, v = (torch.randn(len(slots), hkv, 128, generator=gen) for _ in range(2))
+        k = k * torch.exp(spread * torch.randn(len(slots), hkv, 1, generator=gen))
+        fp4_ref.write(self.pages, k.bfloat16(), v.bfloat16(), slots)
+        self.lens, self.hq, self.hkv, self.bs, self.device, self.gen = lens, hq, hkv, bs, device, gen
+        self.upload()
+
+    def upload(self):
+        kc, ks, vc, vs = (p.to(self.device) for p in self.pages)
+        self.keys, self.values = _C.Fp4Pages(kc, ks), _C.Fp4Pages(vc, vs)
+
+    def queries(self, t, scale=1.0):
+        return (scale * torch.randn(t, self.hq, 128, generator=self.gen)).bfloat16()
+
+    def want(self, i, q, scale=SCALE):
+        """The last len(q) positions of sequence i."""
+        k, v = fp4_ref.read(self.pages, self.slots[i])
+        return fp4_ref.attention(q, k, v, scale)
+
+    def decode(self, q, bound=None, scale=SCALE, out=None, workspace=None):
+        bound = bound or max(max(self.lens), 1)
+        if workspace is None:
+            workspace = _C.alloc_paged_decode_workspace(len(self.lens), self.hq, self.hkv, bound, self.device)
+        out = torch.full(q.shape, 7.0, dtype=torch.bfloat16, device=self.device) if out is None else out
+        return _C.paged_decode_fp4(out, q.to(self.device), self.keys, self.values, self.tables.to(self.device),
+                                   torch.tensor(self.lens, dtype=torch.int32, device=self.device), scale, bound,
+                                   workspace)
+
+    def prefill(self, q, q_lens, out=None, max_q=None, scale=SCALE):
+        cu = torch.tensor([0] + q_lens).cumsum(0).to(torch.int32).to(self.device)
+        out = torch.full(q.shape, 7.0, dtype=torch.bfloat16, device=self.device) if out is None else out
+        return _C.paged_prefill_fp4(out, q.to(self.device), self.keys, self.values, self.tables.to(self.device), cu,
+                                    torch.tensor(self.lens, dtype=torch.int32, device=self.device),
+                                    max_q or max(q_lens), scale)
+
+
+def close(got, want, tol):
+    got = got.cpu().double()
+    assert torch.equal(got.isnan(), want.isnan())
+    off = ((got - want).abs() - tol).nan_to_num(-1.0)
+    assert off.max().item() <= 0, f"off by {off.max().item():.3g} over the bound at {off.argmax().item()}"
+
+
+def check_decode(batch, q, got, scale=SCALE):
+    for i, n in enumerate(batch.lens):
+        if n == 0:
+            assert not got[i].any()
+            continue
+        close(got[i:i + 1], *batch.want(i, q[i:i + 1], scale))
+
+
+# -------------------------------------------------------------------------------------------- decode
+@pytest.mark.parametrize("hq, hkv", [(1, 1), (2, 1), (16, 8), (6, 2), (4, 1), (5, 1), (16, 2), (15, 1), (16, 1), (17, 1),
+                                     (40, 2)])
+def test_decode_head_layouts(device, hq, hkv):
+    batch = Batch(device, [1, 300, 0, 77, 64], hq, hkv, 32, seed=hq)
+    q = batch.queries(5)
+    check_decode(batch, q, batch.decode(q))
+    assert _C.index_errors() == 0
+
+
+@pytest.mark.parametrize("bs", [16, 32, 64, 128, 256])
+def test_decode_contexts_around_tiles_pages_and_partitions(device, bs):
+    lens = [1, 2, 15, 16, 17, 31, 32, 33, 63, 64, 65, 127, 128, 129, 255, 256, 257, 511, 512, 513, 1023, 1024, 1025]
+    batch = Batch(device, lens, 4, 2, bs, seed=bs)
+    q = batch.queries(len(lens))
+    check_decode(batch, q, batch.decode(q))
+    check_decode(batch, q, batch.decode(q, bound=8192))  # a bound far past the contexts
+
+
+@pytest.mark.parametrize("lens, hq, hkv", [([5000, 3], 2, 1), ([9001, 1, 0, 4097], 4, 2), ([40960], 2, 1),
+                                           ([70000, 131072], 1, 1)])
+def test_decode_long_contexts(device, lens, hq, hkv):
+    batch = Batch(device, lens, hq, hkv, 128, seed=1)
+    q = batch.queries(len(lens))
+    check_decode(batch, q, batch.decode(q))
+
+
+def test_decode_many_sequences(device):
+    """More sequences than a wave's lanes, and enough partitions that they grow past the smallest."""
+    gen = torch.Generator().manual_seed(3)
+    lens = [int(x) for x in torch.randint(0, 700, (150,), generator=gen)]
+    batch = Batch(device, lens, 2, 2, 16, seed=4)
+    q = batch.queries(150)
+    check_decode(batch, q, batch.decode(q))
+    lens = [2600 + i for i in range(70)]
+    batch = Batch(device, lens, 4, 4, 128, seed=5)  # 70 x 11 x 4 partitions of 256 tokens, were they that small
+    q = batch.queries(70)
+    check_decode(batch, q, batch.decode(q, bound=4096))
+
+
+def test_decode_scores_far_apart(device):
+    """A few keys carry all of the weight, in whichever partition they are; large and negative scales."""
+    batch = Batch(device, [1500, 700], 4, 1, 64, seed=6, spread=1.5)
+    q = batch.queries(2, scale=8.0)
+    check_decode(batch, q, batch.decode(q))
+    check_decode(batch, q, batch.decode(q, scale=-0.05), scale=-0.05)
+
+
+def test_decode_nan_reaches_only_its_sequence_and_dims(device):
+    batch = Batch(device, [200, 300, 100], 2, 1, 32, seed=7)
+    v = torch.ones(1, 1, 128, dtype=torch.bfloat16)
+    bad_v, bad_k = v.clone(), v.clone()
+    bad_v[0, 0, 70], bad_k[0, 0, 5] = math.inf, math.nan
+    fp4_ref.write(batch.pages, v, bad_v, batch.slots[0][17:18])      # values of dims 64..95
+    fp4_ref.write(batch.pages, bad_k, v, batch.slots[1][299:300])    # a key: every weight
+    batch.upload()
+    q = batch.queries(3)
+    got = batch.decode(q)
+    check_decode(batch, q, got)
+    nan = got.isnan().cpu()
+    assert nan[0, :, 64:96].all() and not nan[0, :, :64].any() and not nan[0, :, 96:].any()
+    assert nan[1].all() and not nan[2].any()
+
+
+def test_decode_views_and_rows_behind_the_batch(device):
+    batch = Batch(device, [40, 500], 6, 2, 16, seed=8, extra_width=3)
+    fused = torch.zeros(2, 10, 128, dtype=torch.bfloat16)
+    q = batch.queries(2)
+    fused[:, 1:7] = q
+    wide = torch.full((4, 9, 128), 7.0, dtype=torch.bfloat16, device=device)
+    got = batch.decode(fused.to(device)[:, 1:7], out=wide[:2, 2:8])
+    check_decode(batch, q, got)
+    assert wide[2:].eq(7).all() and wide[:, :2].eq(7).all() and wide[:, 8:].eq(7).all()
+
+
+def test_decode_bad_pages_and_contexts_stay_in_the_pool_and_are_reported(device):
+    batch = Batch(device, [40, 500, 100], 2, 1, 16, seed=9)
+    q = batch.queries(3)
+    good = batch.decode(q)
+    for entry in (batch.nb, -1, 1 << 30):
+        batch.tables[1, 3] = entry
+        got = batch.decode(q)
+        assert _C.index_errors() == _C.ERR_BLOCK
+        assert torch.equal(got[[0, 2]], good[[0, 2]])
+        _C.clear_index_errors()
+    batch.tables[1, 3] = 0
+    for n in (-1, 513, 1 << 30):  # the table holds 512 tokens
+        batch.lens[1] = n
+        got = batch.decode(q, bound=1024)
+        assert _C.index_errors() == _C.ERR_CONTEXT
+        assert torch.equal(got[[0, 2]], good[[0, 2]])
+        _C.clear_index_errors()
+    batch.lens[1] = 500
+    batch.decode(q, bound=400)  # the launch's bound holds less
+    assert _C.index_errors() == _C.ERR_CONTEXT
+
+
+def test_decode_is_the_same_whatever_runs_beside_it(device):
+    """A replayed graph, a workspace that served other calls and repeated calls give the same bits."""
+    batch = Batch(device, [40, 3000, 900], 8, 2, 64, seed=10)
+    q = batch.queries(3).to(device)
+    first = batch.decode(q)
+    ws = _C.alloc_paged_decode_workspace(8, 16, 2, 8192, device)
+    other = Batch(device, [700, 5000], 16, 2, 32, seed=11)
+    for _ in range(3):
+        other.decode(other.queries(2), workspace=ws)
+        assert torch.equal(batch.decode(q, bound=4096, workspace=ws), first)
+    tables, lens = batch.tables.to(device), torch.tensor(batch.lens, dtype=torch.int32, device=device)
+    out = torch.empty_like(q)
+    attn = HipPagedAttention(8, 2, 128)
+
+    def call():
+        return _C.paged_decode_fp4(out, q, batch.keys, batch.values, tables, lens, SCALE, 4096, ws)
+
+    call()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call()
+    for n in (3000, 0, 17, 2999):
+        lens[1] = n
+        out.fill_(7.0)
+        graph.replay()
+        got = out.clone()
+        torch.cuda.synchronize()
+        batch.lens[1] = n
+        assert torch.equal(got, attn(q, batch.keys, batch.values, tables, lens))
+        check_decode(Window(batch, n), q.cpu(), got)
+
+
+class Window:
+    """A batch whose sequence 1 is cut to n tokens."""
+
+    def __init__(self, batch, n):
+        self.batch, self.lens = batch, [batch.lens[0], n, batch.lens[2]]
+
+    def want(self, i, q, scale):
+        k, v = fp4_ref.read(self.batch.pages, self.batch.slots[i][: self.lens[i]])
+        return fp4_ref.attention(q, k, v, scale)
+
+
+# -------------------------------------------------------------------------------------------- prefill
+def check_prefill(batch, q, q_lens, got, scale=SCALE):
+    at = 0
+    for i, n in enumerate(q_lens):
+        if n:
+            close(got[at:at + n], *batch.want(i, q[at:at + n], scale))
+        at += n
+
+
+@pytest.mark.parametrize("hq, hkv", [(1, 1), (2, 1), (3, 1), (4, 1), (5, 1), (16, 8), (8, 1), (14, 2)])
+def test_prefill_head_layouts(device, hq, hkv):
+    q_lens, cached = [1, 40, 0, 130], [200, 16, 33, 0]
+    batch = Batch(device, [a + b for a, b in zip(q_lens, cached)], hq, hkv, 32, seed=hq)
+    q = batch.queries(sum(q_lens))
+    check_prefill(batch, q, q_lens, batch.prefill(q, q_lens))
+    assert _C.index_errors() == 0
+
+
+@pytest.mark.parametrize("bs", [16, 32, 64, 128, 256])
+def test_prefill_lengths_around_tiles_and_pages(device, bs):
+    q_lens = [1, 2, 15, 16, 17, 31, 32, 33, 63, 64, 65, 127, 128, 129, 255, 257]
+    cached = [0, 1, 16, 31, 32, 5, 64, 100, 0, 128, 129, 1, 16, 300, 0, 255]
+    batch = Batch(device, [a + b for a, b in zip(q_lens, cached)], 4, 2, bs, seed=bs)
+    q = batch.queries(sum(q_lens))
+    check_prefill(batch, q, q_lens, batch.prefill(q, q_lens))
+    check_prefill(batch, q, q_lens, batch.prefill(q, q_lens, max_q=700))  # a bound past the lengths
+
+
+@pytest.mark.parametrize("q_len, cached", [(1, 9000), (600, 4096), (1500, 0)])
+def test_prefill_long(device, q_len, cached):
+    batch = Batch(device, [q_len + cached, 1], 2, 1, 128, seed=2)
+    q = batch.queries(q_len + 1)
+    check_prefill(batch, q, [q_len, 1], batch.prefill(q, [q_len, 1]))
+
+
+def test_prefill_scores_far_apart(device):
+    """Maxima that rise along the keys, so that the running reference moves again and again."""
+    batch = Batch(device, [400, 90], 2, 1, 16, seed=3, spread=1.5)
+    q = batch.queries(300 + 90, scale=8.0)
+    check_prefill(batch, q, [300, 90], batch.prefill(q, [300, 90]))
+
+
+def test_prefill_nan_reaches_the_rows_that_see_its_key_alone(device):
+    batch = Batch(device, [150, 150], 2, 1, 16, seed=4)
+    one = torch.ones(1, 1, 128, dtype=torch.bfloat16)
+    bad_v, bad_k = one.clone(), one.clone()
+    bad_v[0, 0, 40], bad_k[0, 0, 100] = -math.inf, math.inf
+    for at in (109, 115):
+        fp4_ref.write(batch.pages, one, bad_v, batch.slots[0][at:at + 1])
+    fp4_ref.write(batch.pages, bad_k, one, batch.slots[1][120:121])
+    batch.upload()
+    q = batch.queries(150)  # 50 rows of the first sequence, from position 100 on, and 100 of the second, from 50 on
+    got = batch.prefill(q, [50, 100])
+    check_prefill(batch, q, [50, 100], got)
+    nan = got.isnan().cpu()
+    assert not nan[:9].any() and nan[9:50, :, 32:64].all() and not nan[9:50, :, :32].any()
+    assert not nan[50:120].any() and nan[120:].all()
+
+
+def test_prefill_views_and_rows_behind_the_last_sequence(device):
+    batch = Batch(device, [40, 70], 3, 1, 16, seed=5)
+    fused = torch.zeros(60, 5, 128, dtype=torch.bfloat16)
+    q = batch.queries(50)
+    fused[:50, 1:4] = q
+    wide = torch.full((60, 5, 128), 7.0, dtype=torch.bfloat16, device=device)
+    batch.prefill(fused.to(device)[:, 1:4], [20, 30], out=wide[:, 2:])
+    check_prefill(batch, q, [20, 30], wide[:50, 2:])
+    assert wide[50:].eq(7).all() and wide[:, :2].eq(7).all()
+
+
+def test_prefill_faults_are_reported_and_leave_the_others_alone(device):
+    batch = Batch(device, [100, 60, 200], 2, 1, 16, seed=6)
+    q_lens = [20, 60, 100]
+    q = batch.queries(180)
+    good = batch.prefill(q, q_lens)
+    others = torch.cat([torch.arange(20), torch.arange(80, 180)])
+    batch.tables[1, 2] = batch.nb
+    got = batch.prefill(q, q_lens)
+    assert _C.index_errors() == _C.ERR_BLOCK and torch.equal(got[others], good[others])
+    _C.clear_index_errors()
+    batch.tables[1, 2] = 0
+    for n in (59, 0, -1, 1 << 20):  # fewer keys than rows; more than the table holds
+        batch.lens[1] = n
+        got = batch.prefill(q, q_lens)
+        assert _C.index_errors() == _C.ERR_CONTEXT and torch.equal(got[others], good[others])
+        if n <= 0:
+            assert not got[20:80].any()  # rows that see no key
+        _C.clear_index_errors()
+    batch.lens[1] = 60
+    cu = torch.tensor([0, 20, 80, 181], dtype=torch.int32, device=device)  # one row past the last
+    out = torch.full((180, 2, 128), 7.0, dtype=torch.bfloat16, device=device)
+    args = (batch.keys, batch.values, batch.tables.to(device), cu,
+            torch.tensor(batch.lens, dtype=torch.int32, device=device))
+    _C.paged_prefill_fp4(out, q.to(device), *args, 101, SCALE)
+    assert _C.index_errors() == _C.ERR_CONTEXT
+    assert torch.equal(out[:20], good[:20]) and out[80:].eq(7).all()
+
+
+def test_prefill_replays_from_a_graph(device):
+    batch = Batch(device, [100, 333], 4, 2, 16, seed=7)
+    q = batch.queries(130).to(device)
+    cu = torch.tensor([0, 30, 130], dtype=torch.int32, device=device)
+    lens, tables = torch.tensor(batch.lens, dtype=torch.int32, device=device), batch.tables.to(device)
+    out = torch.empty_like(q)
+
+    def call(out):
+        return _C.paged_prefill_fp4(out, q, batch.keys, batch.values, tables, cu, lens, 100, SCALE)
+
+    call(out)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call(out)
+    for seed in range(3):
+        q.copy_(batch.queries(130))
+        cu[1] = 10 + 20 * seed
+        graph.replay()
+        got = out.clone()
+        torch.cuda.synchronize()
+        assert torch.equal(got, call(torch.empty_like(q)))
+
+
+# -------------------------------------------------------------------------------------------- as they are used together
+def test_prompt_then_decode_steps(device):
+    """The layers as the model calls them: a prompt's rows are stored, a follow-up attends through the cache, decode steps
+    store their row and attend."""
+    hq, hkv, bs, nb = 8, 2, 16, 12
+    cache = Fp4PagedKVCache(2, nb, bs, hkv, 128, device)
+    pages = fp4_ref.empty_pages(nb, hkv, bs)
+    norms = [RMSNorm(128, 1e-6).to(device, torch.bfloat16) for _ in range(2)]
+    rotary = RotaryEmbedding(128, 512, 1e6).to(device)
+    prefill, decode = HipBatchPrefillAttention(hq, hkv, 128, bs, 512), HipPagedAttention(hq, hkv, 128)
+    gen = torch.Generator().manual_seed(1)
+    order = torch.randperm(nb, generator=gen)
+    tables = torch.stack([order[:6], order[6:]]).to(torch.int32)
+    done = [0, 0]
+
+    def step(new):
+        """The rows of `new[i]` more tokens of each sequence, as projected; returns what the oracle makes of them."""
+        pos = torch.cat([torch.arange(a, a + n) for a, n in zip(done, new)])
+        seq = torch.repeat_interleave(torch.arange(2), torch.tensor(new))
+        slots = tables[seq, pos // bs].long() * bs + pos % bs
+        qkv = torch.randn(sum(new), hq + 2 * hkv, 128, generator=gen).bfloat16()
+        q, k, v = qkv.split([hq, hkv, hkv], 1)
+        q, k = (fp4_ref.to_bf16(fp4_ref.norm_rope(x, m.weight.cpu(), pos, rotary.cos_sin.cpu(), 1e-6))
+                for x, m in zip((q, k), norms))
+        fp4_ref.write(pages, k, v, slots)
+        outs, tols, at = [], [], 0
+        for i, n in enumerate(new):
+            done[i] += n
+            seen = torch.arange(done[i])
+            kk, vv = fp4_ref.read(pages, tables[i, seen // bs].long() * bs + seen % bs)
+            out, tol = fp4_ref.attention(q[at:at + n], kk, vv, SCALE)
+            outs.append(out)
+            tols.append(tol)
+            at += n
+        return qkv.to(device).split([hq, hkv, hkv], 1), pos.to(device), slots.to(device), torch.cat(outs), torch.cat(tols)
+
+    from nano_vllm_ascend_amd.layers import qk_norm_rope
+    for new in ([20, 37], [33, 5]):
+        (q, k, v), pos, slots, want, tol = step(new)
+        qk_norm_rope(q, k, v, *norms, rotary, pos, cache, 1, slots)
+        md = PagedKVCacheMetadata(block_tables=tables.to(device), slot_mapping=slots, max_query_len=max(new),
+                                  context_lens=torch.tensor(done, dtype=torch.int32, device=device),
+                                  cu_seqlens_q=torch.tensor([0, new[0], sum(new)], dtype=torch.int32, device=device),
+                                  use_paged_prefill=True)
+        close(prefill(q, k, v, md, *cache.get_physical_cache(1)), want, tol)
+    for _ in range(4):
+        (q, k, v), pos, slots, want, tol = step([1, 1])
+        raw = q.clone(), k.clone()
+        got = decode.decode_step(q, k, v, *norms, rotary, pos, *cache.get_physical_cache(1), slots, tables.to(device),
+                                 torch.tensor(done, dtype=torch.int32, device=device))
+        close(got, want, tol)
+        assert torch.equal(q, raw[0]) and torch.equal(k, raw[1])
+    for a, b in zip((cache.key_codes, cache.key_scales, cache.value_codes, cache.value_scales), pages):
+        assert torch.equal(a[1].cpu(), b)
+    assert not cache.key_codes[0].any()
+    assert _C.index_errors() == 0
