@@ -591,36 +591,36 @@ class Fp4Pages(NamedTuple):
         return nb, bs, hkv, 2 * width
 
 
-def _fp4_pages(key_pages: Fp4Pages, value_pages: Fp4Pages) -> tuple[int, int, int, int]:
-    """Checks the pages of a layer; returns [blocks, block_size, kv heads, head_dim]."""
-    if not (isinstance(key_pages, Fp4Pages) and isinstance(value_pages, Fp4Pages)):
+def _fp4_pages(key_pages: Fp4Pages, value_pages: Fp4Pages) -> tuple[tuple[int, int, int, int], tuple]:
+    """Checks the pages of a layer; returns [blocks, block_size, kv heads, head_dim] and their addresses.  (Written out: a
+    small batch's eager call is bound by the host.)"""
+    if type(key_pages) is not Fp4Pages or type(value_pages) is not Fp4Pages:
         raise ValueError("key and value pages must be Fp4Pages")
-    shape = key_pages.codes.shape
-    if len(shape) != 4 or shape[3] != FP4_ROW_BYTES or value_pages.codes.shape != shape:
+    kc, ks = key_pages
+    vc, vs = value_pages
+    shape = kc.shape
+    if len(shape) != 4 or shape[3] != FP4_ROW_BYTES or vc.shape != shape:
         raise ValueError(f"codes must be [blocks, kv heads, block_size, {FP4_ROW_BYTES}] for keys and values, got "
-                         f"{tuple(shape)} and {tuple(value_pages.codes.shape)}")
-    scales = (*shape[:3], FP4_ROW_SCALES)
-    if key_pages.scales.shape != scales or value_pages.scales.shape != scales:
-        raise ValueError(f"scales must be {scales}, got {tuple(key_pages.scales.shape)} and "
-                         f"{tuple(value_pages.scales.shape)}")
-    for t in (*key_pages, *value_pages):
-        if t.dtype is not torch.uint8 or not t.is_contiguous():
-            raise ValueError("pages must be contiguous uint8 tensors")
-    return key_pages.shape
+                         f"{tuple(shape)} and {tuple(vc.shape)}")
+    nb, hkv, bs, _ = shape
+    scales = (nb, hkv, bs, FP4_ROW_SCALES)
+    if ks.shape != scales or vs.shape != scales:
+        raise ValueError(f"scales must be {scales}, got {tuple(ks.shape)} and {tuple(vs.shape)}")
+    u8 = torch.uint8
+    if not (kc.dtype is u8 and ks.dtype is u8 and vc.dtype is u8 and vs.dtype is u8 and kc.is_contiguous()
+            and ks.is_contiguous() and vc.is_contiguous() and vs.is_contiguous()):
+        raise ValueError("pages must be contiguous uint8 tensors")
+    return (nb, bs, hkv, 2 * FP4_ROW_BYTES), (kc.data_ptr(), ks.data_ptr(), vc.data_ptr(), vs.data_ptr())
 
 
-def _on_current_device(*tensors: torch.Tensor | None) -> None:
+def _on_current_device(*tensors: torch.Tensor) -> None:
     """Every launch goes to the current device's current stream: its tensors have to live there."""
-    device = None
+    device = tensors[0].get_device()
     for t in tensors:
-        if t is None:
-            continue
-        if not t.is_cuda:
-            raise ValueError("every tensor must be on the GPU")
-        if device is None:
-            device = torch.cuda.current_device()
-        if t.get_device() != device:
-            raise ValueError(f"a tensor is on device {t.get_device()}, the current device is {device}")
+        if t.get_device() != device or device < 0:
+            raise ValueError(f"every tensor must be on the GPU, and on the same one: got {[str(t.device) for t in tensors]}")
+    if device != torch.cuda.current_device():
+        raise ValueError(f"the tensors are on device {device}, the current device is {torch.cuda.current_device()}")
 
 
 def _heads(name: str, t: torch.Tensor, rows: int, heads: int, d: int) -> int:
@@ -635,13 +635,13 @@ def _heads(name: str, t: torch.Tensor, rows: int, heads: int, d: int) -> int:
     return stride[0] if rows > 1 else max(stride[0], heads * d)
 
 
-def _page_slots(slot_mapping: torch.Tensor, rows: int, shape) -> None:
+def _page_slots(slot_mapping: torch.Tensor, rows: int, num_slots: int) -> None:
     if (slot_mapping.dtype is not torch.int64 or slot_mapping.dim() != 1 or slot_mapping.numel() != rows
             or not slot_mapping.is_contiguous()):
         raise ValueError(f"slot_mapping must be contiguous int64 [{rows}], got {slot_mapping.dtype} "
                          f"{tuple(slot_mapping.shape)}")
     if _range_checks and _checking():
-        check_slots(slot_mapping, shape[0] * shape[1])
+        check_slots(slot_mapping, num_slots)
 
 
 def kv_cache_write_fp4(key_states: torch.Tensor, value_states: torch.Tensor, key_pages: Fp4Pages,
@@ -649,14 +649,13 @@ def kv_cache_write_fp4(key_states: torch.Tensor, value_states: torch.Tensor, key
     """Rows [T, Hkv, 128] of bf16 keys and values, quantised into the pages at their slots (-1: padding, skipped; no slot
     twice in a call)."""
     lib = load()
-    shape = nb, bs, hkv, d = _fp4_pages(key_pages, value_pages)
+    (nb, bs, hkv, d), pages = _fp4_pages(key_pages, value_pages)
     t = key_states.shape[0]
     strides = _heads("key_states", key_states, t, hkv, d), _heads("value_states", value_states, t, hkv, d)
-    _page_slots(slot_mapping, t, shape)
+    _page_slots(slot_mapping, t, nb * bs)
     _on_current_device(key_states, value_states, *key_pages, *value_pages, slot_mapping)
     _check(lib.nvamd_kv_cache_write_fp4(
-        key_states.data_ptr(), strides[0], value_states.data_ptr(), strides[1], key_pages.codes.data_ptr(),
-        key_pages.scales.data_ptr(), value_pages.codes.data_ptr(), value_pages.scales.data_ptr(), nb, bs,
+        key_states.data_ptr(), strides[0], value_states.data_ptr(), strides[1], *pages, nb, bs,
         slot_mapping.data_ptr(), t, hkv, d, _stream()), "nvamd_kv_cache_write_fp4")
 
 
@@ -665,16 +664,15 @@ def kv_cache_read_fp4(key_pages: Fp4Pages, value_pages: Fp4Pages, slot_mapping: 
                       v_out: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """The bf16 keys and values [T, Hkv, 128] that the pages hold at the slots (zeros for -1)."""
     lib = load()
-    shape = nb, bs, hkv, d = _fp4_pages(key_pages, value_pages)
+    (nb, bs, hkv, d), pages = _fp4_pages(key_pages, value_pages)
     t = slot_mapping.numel()
-    _page_slots(slot_mapping, t, shape)
+    _page_slots(slot_mapping, t, nb * bs)
     k, v = (torch.empty((t, hkv, d), dtype=torch.bfloat16, device=key_pages.codes.device) if out is None else out
             for out in (k_out, v_out))
     strides = _heads("k_out", k, t, hkv, d), _heads("v_out", v, t, hkv, d)
     _on_current_device(k, v, *key_pages, *value_pages, slot_mapping)
     _check(lib.nvamd_kv_cache_read_fp4(
-        k.data_ptr(), strides[0], v.data_ptr(), strides[1], key_pages.codes.data_ptr(), key_pages.scales.data_ptr(),
-        value_pages.codes.data_ptr(), value_pages.scales.data_ptr(), nb, bs, slot_mapping.data_ptr(), t, hkv, d,
+        k.data_ptr(), strides[0], v.data_ptr(), strides[1], *pages, nb, bs, slot_mapping.data_ptr(), t, hkv, d,
         _stream()), "nvamd_kv_cache_read_fp4")
     return k, v
 
@@ -688,7 +686,7 @@ def qk_norm_rope_fp4(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_weight
     Returns the rotated q: ``q_out``, which may be q itself, or a new tensor.  The rotated k is written
     only to the pages unless ``k_out`` (which may be k itself) asks for it.  64-bit arithmetic, one rounding to bf16."""
     lib = load()
-    shape = nb, bs, hkv, d = _fp4_pages(key_pages, value_pages)
+    (nb, bs, hkv, d), pages = _fp4_pages(key_pages, value_pages)
     if q.dim() != 3:
         raise ValueError(f"q must be [T, heads, D], got {tuple(q.shape)}")
     t, hq, _ = q.shape
@@ -708,42 +706,51 @@ def qk_norm_rope_fp4(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_weight
     if (cos_sin.dtype is not torch.float32 or cos_sin.dim() != 2 or cos_sin.shape[1] != d
             or not cos_sin.is_contiguous()):
         raise ValueError("cos_sin must be contiguous fp32 [max_positions, head_dim]")
-    _page_slots(slot_mapping, t, shape)
-    _on_current_device(q, k, v, q_out, k_out, q_weight, k_weight, positions, cos_sin, *key_pages, *value_pages,
-                       slot_mapping)
+    _page_slots(slot_mapping, t, nb * bs)
+    _on_current_device(q, k, v, q_out, q if k_out is None else k_out, q_weight, k_weight, positions, cos_sin,
+                       *key_pages, *value_pages, slot_mapping)
     if _range_checks and _checking():
         check_positions(positions, cos_sin.shape[0])
     _check(lib.nvamd_qk_norm_rope_fp4(
         q_out.data_ptr(), qo_stride, _ptr(k_out), ko_stride, q.data_ptr(), q_stride, k.data_ptr(), k_stride,
         v.data_ptr(), v_stride, q_weight.data_ptr(), k_weight.data_ptr(), positions.data_ptr(), cos_sin.data_ptr(),
-        cos_sin.shape[0], key_pages.codes.data_ptr(), key_pages.scales.data_ptr(), value_pages.codes.data_ptr(),
-        value_pages.scales.data_ptr(), nb, bs, slot_mapping.data_ptr(), t, hq, hkv, d, float(eps), _stream()),
+        cos_sin.shape[0], *pages, nb, bs, slot_mapping.data_ptr(), t, hq, hkv, d, float(eps), _stream()),
         "nvamd_qk_norm_rope_fp4")
     return q_out
 
 
 def _fp4_attention_args(out, q, key_pages, value_pages, block_tables, seqs: int):
-    """Checked arguments that decode and prefill share, up to the block tables."""
-    nb, bs, hkv, d = _fp4_pages(key_pages, value_pages)
-    if q.dim() != 3 or out.shape != q.shape:
-        raise ValueError(f"q/out shape mismatch: {tuple(q.shape)} vs {tuple(out.shape)}")
-    t, hq, _ = q.shape
-    out_stride, q_stride = _heads("out", out, t, hq, d), _heads("q", q, t, hq, d)
-    if block_tables.dtype is not torch.int32 or block_tables.dim() != 2 or block_tables.shape[0] < seqs:
+    """Checked arguments that decode and prefill share, up to the block tables, and [heads, kv heads, head_dim]."""
+    (nb, bs, hkv, d), pages = _fp4_pages(key_pages, value_pages)
+    shape = q.shape
+    if len(shape) != 3 or out.shape != shape:
+        raise ValueError(f"q/out shape mismatch: {tuple(shape)} vs {tuple(out.shape)}")
+    t, hq, dq = shape
+    if dq != d:
+        raise ValueError(f"head_dim mismatch {dq} vs {d}")
+    if q.dtype is not torch.bfloat16 or out.dtype is not torch.bfloat16:
+        raise ValueError(f"q and out must be bfloat16, got {q.dtype} and {out.dtype}")
+    q_stride, out_stride = q.stride(), out.stride()
+    for name, st in (("q", q_stride), ("out", out_stride)):
+        if t and (st[2] != 1 or (hq > 1 and st[1] != d)):
+            raise ValueError(f"rows of {name} {tuple(shape)} are not dense")
+    tables, bt_stride = block_tables.shape, block_tables.stride()
+    if block_tables.dtype is not torch.int32 or len(tables) != 2 or tables[0] < seqs:
         raise ValueError(f"block_tables must be int32 [{seqs}, W]")
-    if block_tables.stride(1) != 1 and block_tables.shape[1] > 1:
+    width = tables[1]
+    if bt_stride[1] != 1 and width > 1:
         raise ValueError("block_tables rows must be dense")
-    width = block_tables.shape[1]
-    return (out.data_ptr(), out_stride, q.data_ptr(), q_stride, key_pages.codes.data_ptr(),
-            key_pages.scales.data_ptr(), value_pages.codes.data_ptr(), value_pages.scales.data_ptr(), nb, bs,
-            block_tables.data_ptr(), max(block_tables.stride(0), width), width), (hq, hkv, d)
+    least = hq * d  # a single row's stride says nothing
+    return (out.data_ptr(), out_stride[0] if t > 1 else max(out_stride[0], least), q.data_ptr(),
+            q_stride[0] if t > 1 else max(q_stride[0], least), *pages, nb, bs, block_tables.data_ptr(),
+            max(bt_stride[0], width), width), (hq, hkv, d)
 
 
 def paged_decode_fp4(out: torch.Tensor, q: torch.Tensor, key_pages: Fp4Pages, value_pages: Fp4Pages,
                      block_tables: torch.Tensor, context_lens: torch.Tensor, scale: float, max_context_len: int,
                      workspace: torch.Tensor) -> torch.Tensor:
     """``paged_decode`` over pages of 4 bits; the workspace is the same (``alloc_paged_decode_workspace``)."""
-    lib = load()
+    lib = _lib or load()
     b = q.shape[0]
     args, heads = _fp4_attention_args(out, q, key_pages, value_pages, block_tables, b)
     if block_tables.shape[0] != b:
@@ -752,12 +759,13 @@ def paged_decode_fp4(out: torch.Tensor, q: torch.Tensor, key_pages: Fp4Pages, va
         raise ValueError(f"context_lens must be contiguous int32 [{b}]")
     if not workspace.is_contiguous():
         raise ValueError("workspace must be contiguous")
-    _on_current_device(out, q, *key_pages, *value_pages, block_tables, context_lens, workspace)
+    _on_current_device(q, out, *key_pages, *value_pages, block_tables, context_lens, workspace)
     if _range_checks and _checking():
         check_paged_context(block_tables, context_lens, args[8], args[9], int(max_context_len))
-    _check(lib.nvamd_paged_decode_fp4(*args, context_lens.data_ptr(), b, *heads, float(scale), int(max_context_len),
-                                      workspace.data_ptr(), workspace.numel() * workspace.element_size(), _stream()),
-           "nvamd_paged_decode_fp4")
+    status = lib.nvamd_paged_decode_fp4(*args, context_lens.data_ptr(), b, *heads, scale, max_context_len,
+                                        workspace.data_ptr(), workspace.nbytes, _stream())
+    if status:
+        _check(status, "nvamd_paged_decode_fp4")
     return out
 
 

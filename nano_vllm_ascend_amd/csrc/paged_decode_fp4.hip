@@ -1,23 +1,26 @@
 // GQA paged decode attention over the 4-bit KV cache (the counterpart of paged_decode.hip).
 //
 // For a query token of each sequence and its heads h of kv head g: out = softmax(q . K^T * scale) V over the cached
-// context, with K and V expanded from 4 bits on the way into the matrix cores (v_cvt_scalef32_pk_bf16_fp4: two values and
-// their scale in one instruction, exact).
+// context.
 //
-// Work: a unit (sequence, kv head) is cut into partitions of 256 * 2^shift tokens, a workgroup of 4 waves each.  Every
-// workgroup reads the context lengths and derives the same shift: the least that leaves at most `target` partitions.  So
-// the cut follows the contexts themselves and not the bound that the launch was made with.  A partition
-// leaves (max, sum, numerator) per head in the workspace and counts its arrival; the last one of a unit
-// joins them.
+// Work: a unit (sequence, kv head) is cut into partitions of equal length, a workgroup of 8 waves each.  Every workgroup
+// reads the context lengths and derives the same length from them (part_tokens), so the cut follows the contexts themselves
+// and not the bound that the launch was made with.  A partition leaves (max, sum, numerator) per head in the
+// workspace and counts its arrival; the last one of a unit joins them.
 //
 // A wave takes 64 tokens at a time, four 16-token tiles, one per 16 lanes (gq = lane / 16):
-//   S^T = K . Q^T  v_mfma_f32_16x16x32_bf16, A = 16 rows of K, B = the heads as 16 columns.  The contraction runs over
-//        dims 32 gq + 8 i + 0..7 in step i, so a lane's 16 bytes of codes are one block of a row, under one scale.
+//   S^T = K . Q^T  v_mfma_scale_f32_16x16x128_f8f6f4 on the codes as they lie in the cache, A = 16 rows of K: a lane's 16
+//        bytes are one block of a row, under one scale.  B = the heads as 16 columns, in 8 bits twice: a bf16 query is the sum
+//        of two e4m3 numbers under a common scale (split_query), so two products give the scores.  That takes the matrix
+//        cores as long as four bf16 products, and the vector ALUs no expansion of K.
 //        Row 4a + i of product t is token 4t + i of tile a: lane (h, gq) then finds the scores of tile gq's tokens
 //        4t .. 4t+3 of head h in its accumulator of product t, that is of all 16 tokens in the four products;
-//   O^T += V^T . P^T  A = 16 dims of V^T, B = P^T, whose 8 k-slots per lane are tokens 0..7 (8..15) of tile gq: just
+//   softmax  on up to 4 (8) heads the accumulators' 16 columns are mostly repeats: products 1..3 (2, 3) move into the idle
+//        columns by DPP, and one lane does 4 (8) scores instead of 16;
+//   O^T += V^T . P^T  v_mfma_f32_16x16x32_bf16, A = 16 dims of V^T expanded by v_cvt_scalef32_pk_bf16_fp4 (two values and
+//        their scale in one instruction, exact), B = P^T, whose 8 k-slots per lane are tokens 0..7 (8..15) of tile gq: just
 //        what the lane holds.  The cache keeps V with 16 tokens of a dim pair in consecutive bytes, so the lane's
-//        16 bytes give both products' operands of two dims: no lane movement anywhere.
+//        16 bytes give both products' operands of two dims: no lane movement.
 // The score of a token past the context is replaced by -inf and the scales of its values by zero, whatever bytes it holds.
 #include "fp4.h"
 
@@ -28,9 +31,13 @@ constexpr int kPartFloats = 132;  // a head's record: max, sum, 2 unused, 128 ac
 constexpr int kCounterSlots = 16384;
 constexpr size_t kCounterBytes = kCounterSlots * sizeof(int);
 constexpr int kMaxContext = 131072;  // largest context bound of a call
-constexpr int kMinPart = 256;        // tokens of the smallest partition: one 64-token chunk for each wave
-constexpr int kWaves = 4;
-constexpr int kTarget = 2048;  // partitions that a launch is cut into where the contexts allow
+constexpr int kWaves = 8;
+constexpr int kHalvesLog2 = 4, kHalves = 2 * kWaves;  // half-waves of a workgroup
+static_assert(kHalves == 1 << kHalvesLog2);
+constexpr int kMinPart = 64 * kWaves;  // tokens of the smallest partition: one step of each wave
+constexpr int kCus = 256;
+constexpr float kNoScore = -1e30f;   // reference of an empty softmax: finite, so that it needs no guard in exponents
+constexpr float kRescaleLog2 = 8.f;  // the reference moves when a score exceeds it by 2^8
 constexpr int kMaxHeads = 16;  // query heads of a kv head in one launch: the MFMA's columns
 
 struct DecodeFp4Args {
@@ -88,23 +95,118 @@ __device__ __forceinline__ float sum_over_quarters(float v) {
   return sum_xor32(__uint_as_float(r[0]) + __uint_as_float(r[1]));
 }
 
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+
+// S += K . q for 16 rows of codes (128 dims, a lane's block and its scale byte) and 16 columns of e4m3 under the scale
+// byte of a column.  Lane (row or column n, gq) gives block gq of its row; of its column, dims 16 gq .. +15 and 64 + 16 gq ..
+// +15 (checked on gfx950).
+__device__ __forceinline__ f32x4 mfma_fp4_fp8(u32x4 k, u32 k_scale, i32x8 q, u32 q_scale, f32x4 c) {
+  const i32x8 codes = {(int)k[0], (int)k[1], (int)k[2], (int)k[3], 0, 0, 0, 0};
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(codes, q, c, 4, 0, 0, (int)k_scale, 0, (int)q_scale);
+}
+
+// 32 bf16 values of a query row (16 lanes apart: 4 lanes hold the row) as hi + lo in e4m3 under 2^-s, s from the row's
+// largest value, which lands in [128, 256).  hi keeps 4 of the 8 significant bits and lo the rest: the sum is the value
+// itself down to 2^-10 of the largest one and off by at most 2^-17 of that below.  Returns the scale byte; 255, which makes
+// every score NaN, for a row with an infinity or a NaN.
+__device__ __forceinline__ u32 split_query(const u32x4 (&x)[4], i32x8 &hi, i32x8 &lo) {
+  u32 top = 0;
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const u32 w = x[j][e];
+      top = max(top, max(w & 0x7fffu, (w >> 16) & 0x7fffu));
+    }
+  top = (u32)max_over_quarters((float)top);  // 15 bits: exact
+  const int e = min(max((int)(top >> 7), 20), 254);  // biased exponent of the row's largest value
+  const float up = __uint_as_float((u32)(127 + 134 - e) << 23);  // 2^(7 - (e - 127))
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {  // 4 values to a word
+      const u32 w0 = x[j][2 * i], w1 = x[j][2 * i + 1];
+      const float a = bf16_lo(w0) * up, b = bf16_hi(w0) * up, c = bf16_lo(w1) * up, d = bf16_hi(w1) * up;
+      int h = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
+      h = __builtin_amdgcn_cvt_pk_fp8_f32(c, d, h, true);
+      int r = __builtin_amdgcn_cvt_pk_fp8_f32(a - __builtin_amdgcn_cvt_f32_fp8(h, 0),
+                                              b - __builtin_amdgcn_cvt_f32_fp8(h, 1), 0, false);
+      r = __builtin_amdgcn_cvt_pk_fp8_f32(c - __builtin_amdgcn_cvt_f32_fp8(h, 2),
+                                          d - __builtin_amdgcn_cvt_f32_fp8(h, 3), r, true);
+      hi[2 * j + i] = h;
+      lo[2 * j + i] = r;
+    }
+  return top >= 0x7f80u ? 255u : (u32)(e - 7);
+}
+
+// Byte B of a word of scales as a float scale: one instruction (the compiler takes two for bytes 0..2).
 template <int B>
 __device__ __forceinline__ float scale_of(u32 word) {
-  return __uint_as_float(((word >> (8 * B)) & 0xffu) << 23);
+  float r;
+  if constexpr (B == 0)
+    asm("v_lshlrev_b32_sdwa %0, %1, %2 dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:DWORD src1_sel:BYTE_0" : "=v"(r) : "v"(23), "v"(word));
+  else if constexpr (B == 1)
+    asm("v_lshlrev_b32_sdwa %0, %1, %2 dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:DWORD src1_sel:BYTE_1" : "=v"(r) : "v"(23), "v"(word));
+  else if constexpr (B == 2)
+    asm("v_lshlrev_b32_sdwa %0, %1, %2 dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:DWORD src1_sel:BYTE_2" : "=v"(r) : "v"(23), "v"(word));
+  else
+    asm("v_lshlrev_b32_sdwa %0, %1, %2 dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:DWORD src1_sel:BYTE_3" : "=v"(r) : "v"(23), "v"(word));
+  return r;
 }
 
-// Keeps the first n bytes (0 .. 16) of 16.
-__device__ __forceinline__ u32x4 keep_bytes(u32x4 v, int n) {
-#pragma unroll
-  for (int w = 0; w < 4; ++w) {
-    const int k = min(max(n - 4 * w, 0), 4);
-    v[w] &= k == 4 ? 0xffffffffu : (1u << (8 * k)) - 1u;
-  }
-  return v;
+// Lanes of the banks in MASK (4 lanes each, of 16) take src moved by the DPP control, the others keep `old`.
+template <int CTRL, int MASK>
+__device__ __forceinline__ float dpp_into(float old, float src) {
+  return __uint_as_float((u32)__builtin_amdgcn_update_dpp((int)__float_as_uint(old), (int)__float_as_uint(src), CTRL, 0xF,
+                                                          MASK, false));
+}
+template <int CTRL>
+__device__ __forceinline__ u32 dpp_u32(u32 v) {
+  return (u32)__builtin_amdgcn_mov_dpp((int)v, CTRL, 0xF, 0xF, true);
+}
+constexpr int kRowShl4 = 0x104, kRowShl8 = 0x108, kRowShl12 = 0x10C;  // lane n <- lane n + 4, 8, 12 of its 16
+constexpr int kRowShr4 = 0x114, kRowShr8 = 0x118, kRowShr12 = 0x11C;  // lane n <- lane n - 4, 8, 12
+constexpr int kRowRor4 = 0x124;
+constexpr int kRowBcast = 0x150;  // + n: every lane <- lane n of its 16
+
+// Codes are read once: past the caches' normal keeping.
+__device__ __forceinline__ u32x4 load16(const u8 *p) {
+  return __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(p));
 }
 
-template <int GP>
-__global__ void __launch_bounds__(kWaves * 64)
+// Keeps the first n bytes (any n) of a word.
+__device__ __forceinline__ u32 keep_bytes(u32 v, int n) {
+  return n >= 4 ? v : n <= 0 ? 0u : v & ((1u << (8 * n)) - 1u);
+}
+template <int N>
+struct Int {
+  static constexpr int value = N;
+};
+
+// Cutting units of `tokens` tokens in all every `length` tokens ends in tokens / length + units / 2 partitions on average,
+// and in a whole unit more than the quotient each at most.  The length is chosen for this quotient (share):
+//   few units: partitions fill the card once, with one workgroup on each CU while that leaves two per unit, else two.  Anything
+//     between one and two workgroups per CU has half of the CUs do double the work;
+//   many units: twice the mean context.  Units then go round by themselves, and only contexts far longer than the others
+//     are cut.
+// Measured (us): 4 x U[8192, 40960] at 8 kv heads 20.9 with one workgroup per CU, 22.8 with two, 25.8 where the length was the
+// next power of two; 16 x U[512, 4096] at 8 groups of 8 heads 13.9 either way (16.4); 32 x U[256, 2304] at 8 kv heads 21.7
+// uncut, 16.0 with two (16.7); 100 x U[2048, 4096] 63 uncut, 76 cut in two.
+__host__ __device__ constexpr int partition_share(int units) {
+  const int slots = units * 2 <= kCus ? kCus : 2 * kCus;
+  return slots - units / 2 > units / 2 ? slots - units / 2 : units / 2;
+}
+__device__ __forceinline__ int partition_tokens(u32 tokens, int units) {  // a multiple of 64
+  const u32 share = (u32)partition_share(units);
+  const u32 len = (tokens + share - 1) / share;
+  return max((int)((len + 63) & ~63u), kMinPart);
+}
+__host__ __device__ constexpr int max_partitions(int units) { return partition_share(units) + units; }
+
+// GP: heads that the registers and LDS are laid out for.  WIDE: pages of 64 tokens or more, so that the 64 tokens of a wave's
+// step lie in one page, whose id is a scalar.
+template <int GP, bool WIDE>
+__global__ void __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(WIDE ? 4 : 3)))
 paged_decode_fp4_kernel(DecodeFp4Args a) {
   constexpr int D = kHeadDim;
   constexpr int HS = kPartFloats;
@@ -121,22 +223,25 @@ paged_decode_fp4_kernel(DecodeFp4Args a) {
   // The cut, and this workgroup's place in it.
   const int ctx_cap = min(a.max_ctx, a.bt_width << a.bs_log2);
   u32 err_bits = 0;
-  int64_t total = 0;
+  u32 total = 0;  // tokens of one kv head, at most 2^31 with all of them
+  int ctx0 = 0;   // the context of this lane's sequence of the first 64
   for (int b0 = 0; b0 < a.batch; b0 += 64) {
     const int bi = b0 + lane;
     const int raw = bi < a.batch ? a.context_lens[bi] : 0;
     if (__ballot(raw < 0 || raw > ctx_cap)) err_bits |= NVAMD_ERR_CONTEXT;
-    const int units = bi < a.batch ? max(ceil_div(min(max(raw, 0), ctx_cap), kMinPart), 1) : 0;
-    total += __builtin_amdgcn_readlane(wave_scan(units, lane), 63);
+    const int ci = min(max(raw, 0), ctx_cap);
+    if (b0 == 0) ctx0 = ci;
+    total += (u32)__builtin_amdgcn_readlane(wave_scan(bi < a.batch ? max(ci, 1) : 0, lane), 63);
   }
-  int shift = 0;
-  while ((total * hkv >> shift) > kTarget) ++shift;
-  const int part_tokens = kMinPart << shift;
+  const int part_tokens = partition_tokens(total * (u32)hkv, a.batch * hkv);
+  const float per_part = 1.0f / (float)part_tokens;
   int b = -1, n_parts = 0, first = 0, ctx = 0;
   for (int b0 = 0, base = 0; b0 < a.batch; b0 += 64) {
     const int bi = b0 + lane;
-    const int ci = bi < a.batch ? min(max(a.context_lens[bi], 0), ctx_cap) : 0;
-    const int np = bi < a.batch ? max(ceil_div(ci, part_tokens), 1) : 0;
+    const int ci = b0 == 0 ? ctx0 : bi < a.batch ? min(max(a.context_lens[bi], 0), ctx_cap) : 0;
+    int np = (int)((float)(ci + part_tokens - 1) * per_part);  // off by one at most: both are below 2^24
+    np += np * part_tokens < ci ? 1 : (np - 1) * part_tokens >= ci ? -1 : 0;
+    np = bi < a.batch ? max(np, 1) : 0;
     const int incl = wave_scan(np, lane);
     const int sum = __builtin_amdgcn_readlane(incl, 63);
     if (item < (base + sum) * hkv) {
@@ -158,95 +263,171 @@ paged_decode_fp4_kernel(DecodeFp4Args a) {
   const int32_t *bt_row = a.block_tables + (int64_t)b * a.bt_stride;
   const int bs_mask = (1 << a.bs_log2) - 1;
 
-  // Query operand: dims 32 gq + 8 i .. +7 of head n (columns past the last head repeat it and are never read).
-  u32x4 qf[4];
+  // Query operand of head n (columns past the last head repeat it and are never read).
+  i32x8 q_hi, q_lo;
+  u32 q_scale;
   {
-    const u16 *qp = a.q + (int64_t)b * a.q_stride + (int64_t)(head0 + min(n, G - 1)) * D + 32 * gq;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) qf[i] = ld16(qp + 8 * i);
+    const u16 *qp = a.q + (int64_t)b * a.q_stride + (int64_t)(head0 + min(n, G - 1)) * D + 16 * gq;
+    const u32x4 x[4] = {ld16(qp), ld16(qp + 8), ld16(qp + 64), ld16(qp + 72)};
+    q_scale = split_query(x, q_hi, q_lo);
   }
 
-  float m = -INFINITY, l = 0.f;
+  // The exponent's reference, the threshold above which it moves; the sum and the numerators at that reference.
+  float m = kNoScore, m_thr = kNoScore, l = 0.f;
   f32x4 o[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) o[e] = f32x4{0.f, 0.f, 0.f, 0.f};
 
+  // A step's 64 tokens are the four tiles t0 .. t0+63.  The tile of each 16 lanes, as row owners of K (tile n / 4) and as token
+  // owners of V (tile gq); tiles past the context repeat its last one.
+  typedef const __attribute__((address_space(4))) int32_t const_i32;  // nothing writes the table: scalar loads
+  const_i32 *bt = (const_i32 *)bt_row;
   const int t_end = min((p + 1) * part_tokens, ctx);
-  for (int t0 = p * part_tokens + 64 * w; t0 < t_end; t0 += 64 * kWaves) {
-    // The tile of each 16 lanes, as row owners of K (a = n / 4) and as token owners of V (gq); tiles past the
-    // context repeat its last one.
-    const int last = (ctx - 1) & ~15;
-    auto tile_at = [&](int i) {
-      const int t = min(t0 + 16 * i, last);
-      int blk = bt_row[t >> a.bs_log2];
-      if ((unsigned)blk >= (unsigned)a.num_blocks) err_bits |= NVAMD_ERR_BLOCK;
-      blk = min(max(blk, 0), a.num_blocks - 1);  // never leave the pool
-      return fp4_tile(blk, t & bs_mask, g, hkv, a.bs_log2);
-    };
-    const int64_t kt = tile_at(n >> 2), vt = tile_at(gq);
-    const u8 *kp = a.cache.k_codes + kt * kFp4TileBytes + (n & 3) * kFp4RowBytes + 16 * gq;
-    const u8 *vp = a.cache.v_codes + vt * kFp4TileBytes + 16 * n;
-    u32x4 kc[4], vc[4], vs[4];
-#pragma unroll
-    for (int t = 0; t < 4; ++t) kc[t] = *reinterpret_cast<const u32x4 *>(kp + 4 * t * kFp4RowBytes);
-    const u32 ks = *reinterpret_cast<const u32 *>(a.cache.k_scales + kt * kFp4TileScales + fp4_key_scale_at(n & 3, gq));
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      vc[q] = *reinterpret_cast<const u32x4 *>(vp + 256 * q);
-      vs[q] = *reinterpret_cast<const u32x4 *>(a.cache.v_scales + vt * kFp4TileScales + 16 * q);
+  const int last = (ctx - 1) & ~15;
+  // The table's entries are asked for a step before their tiles.
+  int entry_k = 0, entry_v = 0;
+  auto look_up = [&](int t0) {
+    if constexpr (WIDE) {
+      entry_k = bt[min(t0, last) >> a.bs_log2];
+    } else {
+      entry_k = bt_row[min(t0 + 16 * (n >> 2), last) >> a.bs_log2];
+      entry_v = bt_row[min(t0 + 16 * gq, last) >> a.bs_log2];
     }
+  };
+  // Where the next tiles lie: a tile that the lanes share (a scalar, WIDE) and each lane's tiles past it.
+  int tile0 = 0;
+  u32 k_tile = 0, v_tile = 0;
+  auto locate = [&](int t0) {
+    auto page = [&](int t, int e) {
+      if ((unsigned)e >= (unsigned)a.num_blocks) err_bits |= NVAMD_ERR_BLOCK;
+      return (int)fp4_tile(min(max(e, 0), a.num_blocks - 1), t & bs_mask, g, hkv, a.bs_log2);  // never leave the pool
+    };
+    if constexpr (WIDE) {
+      tile0 = page(t0, entry_k);
+      const int tiles = (last - t0) >> 4;  // 0 .. 3, or more: the last tile that exists
+      k_tile = min(n >> 2, tiles);
+      v_tile = min(gq, tiles);
+    } else {
+      k_tile = page(min(t0 + 16 * (n >> 2), last), entry_k);
+      v_tile = page(min(t0 + 16 * gq, last), entry_v);
+    }
+  };
+  // Byte `at` of tile `tile0 + tile`: a 32-bit offset from a scalar address where the tiles lie in one page.
+  auto in_tiles = [&](const u8 *base, u32 tile, int tile_bytes, u32 at) {
+    if constexpr (WIDE) return base + (int64_t)tile0 * tile_bytes + (tile * tile_bytes + at);
+    else return base + (int64_t)tile * tile_bytes + at;
+  };
+  u32x4 kc[4], vc[4];
+  u32 ks, vs;
+  auto load_k = [&]() {
+    const u8 *kp = in_tiles(a.cache.k_codes, k_tile, kFp4TileBytes, (n & 3) * kFp4RowBytes + 16 * gq);
+#pragma unroll
+    for (int t = 0; t < 4; ++t) kc[t] = load16(kp + 4 * t * kFp4RowBytes);
+    ks = *reinterpret_cast<const u32 *>(in_tiles(a.cache.k_scales, k_tile, kFp4TileScales, fp4_key_scale_at(n & 3, gq)));
+  };
+  auto load_v = [&]() {
+    const u8 *vp = in_tiles(a.cache.v_codes, v_tile, kFp4TileBytes, 16 * n);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) vc[q] = load16(vp + 256 * q);
+    // the 16 lanes of a tile share its 64 scale bytes out: lane n has those of block n / 4, tokens 4 (n % 4) .. +3
+    vs = *reinterpret_cast<const u32 *>(in_tiles(a.cache.v_scales, v_tile, kFp4TileScales, 4 * n));
+  };
 
+  // K of the next step is asked for as soon as the scores have taken this step's, V as soon as the products have: each is in
+  // flight during the other half of the step, without registers of its own.
+  auto step = [&](const int t0, const int next) {
+    constexpr int NP = GP <= 4 ? 1 : GP <= 8 ? 2 : 4;  // accumulators that hold all scores once packed
     f32x4 s[4];
-    const float kscale[4] = {scale_of<0>(ks), scale_of<1>(ks), scale_of<2>(ks), scale_of<3>(ks)};
+    const u32 k_scale[4] = {ks & 0xffu, (ks >> 8) & 0xffu, (ks >> 16) & 0xffu, ks >> 24};
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
-      s[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int i = 0; i < 4; ++i) s[t] = mfma16(fp4_values(kc[t][i], kscale[t]), qf[i], s[t]);
+      s[t] = mfma_fp4_fp8(kc[t], k_scale[t], q_hi, q_scale, f32x4{0.f, 0.f, 0.f, 0.f});
+      s[t] = mfma_fp4_fp8(kc[t], k_scale[t], q_lo, q_scale, s[t]);
     }
+    __builtin_amdgcn_sched_barrier(0);
+    if (next < t_end) {
+      locate(next);
+      load_k();
+      look_up(next + 64 * kWaves);
+    }
+    __builtin_amdgcn_sched_barrier(0);
 
-    // Online softmax: one reference per head and wave.
-    const int live = t_end - t0 - 16 * gq;  // this lane's tokens that the partition holds
-    float cm = m;
+    // Score x * 4 + i of a lane: token 16 gq + 4 (x + NP * its column group) + i, the group being n / (4 NP).
 #pragma unroll
-    for (int t = 0; t < 4; ++t)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        s[t][i] = 4 * t + i < live ? s[t][i] * a.scale_log2e : -INFINITY;
-        cm = fmaxf(cm, s[t][i]);
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (NP == 1) {
+        s[0][i] = dpp_into<kRowShr4, 0x2>(s[0][i], s[1][i]);
+        s[0][i] = dpp_into<kRowShr8, 0x4>(s[0][i], s[2][i]);
+        s[0][i] = dpp_into<kRowShr12, 0x8>(s[0][i], s[3][i]);
+      } else if constexpr (NP == 2) {
+        s[0][i] = dpp_into<kRowShr8, 0xC>(s[0][i], s[2][i]);
+        s[1][i] = dpp_into<kRowShr8, 0xC>(s[1][i], s[3][i]);
       }
-    cm = max_over_quarters(cm);
-    const float ref = cm == -INFINITY ? 0.f : cm;
-    const float alpha = fast_exp2(m - ref);
-    m = cm;
-    l *= alpha;
+    }
+    const int group = NP == 4 ? 0 : n / (4 * NP);
+    const int live = t_end - t0 - 16 * gq;  // this lane's tile's tokens that the partition holds
+    float cm = kNoScore;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) o[e] *= alpha;
-    // P rounded to bf16 for the matrix cores; the sum takes the same rounded values.
+    for (int x = 0; x < NP; ++x)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s[x][i] *= a.scale_log2e;
+    if (t0 + 64 > t_end) {
+#pragma unroll
+      for (int x = 0; x < NP; ++x)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (4 * (x + NP * group) + i >= live) s[x][i] = -INFINITY;
+      vs = keep_bytes(vs, live - 4 * (n & 3));  // values past the partition's end weigh nothing, NaNs of stale rows too
+    }
+#pragma unroll
+    for (int x = 0; x < NP; ++x)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) cm = fmaxf(cm, s[x][i]);
+    if constexpr (NP == 1) cm = fmaxf(cm, dpp<kRowRor4>(cm));
+    if constexpr (NP <= 2) cm = fmaxf(cm, dpp<kDppRowRor8>(cm));
+    cm = max_over_quarters(cm);
+    // Lazy rescale: the weights stay below 2^8 and the numerators are scaled only where some head's reference moves.
+    if (__builtin_amdgcn_ballot_w64(cm > m_thr) != 0) {
+      const bool up = cm > m_thr;
+      const float alpha = up ? fast_exp2(m - cm) : 1.f;
+      if (up) {
+        m = cm;
+        m_thr = cm + kRescaleLog2;
+      }
+      l *= alpha;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) o[e] *= alpha;
+    }
+    // P rounded to bf16 for the matrix cores; the sum takes the same rounded values.  Back in the order of the products, the
+    // columns past the heads hold weights of other tokens and give numerators that are never read.
     u32x4 pf[2];
 #pragma unroll
-    for (int t = 0; t < 4; ++t)
+    for (int x = 0; x < NP; ++x)
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const u32 pr = pack_bf16x2(fast_exp2(s[t][2 * i] - ref), fast_exp2(s[t][2 * i + 1] - ref));
+        const u32 pr = pack_bf16x2(fast_exp2(s[x][2 * i] - m), fast_exp2(s[x][2 * i + 1] - m));
         l = dot2_bf16(pr, 0x3F803F80u, l);
-        pf[t >> 1][2 * (t & 1) + i] = pr;
+        pf[x >> 1][2 * (x & 1) + i] = pr;
+        if constexpr (NP == 1) {
+          pf[0][2 + i] = dpp_u32<kRowShl4>(pr);
+          pf[1][i] = dpp_u32<kRowShl8>(pr);
+          pf[1][2 + i] = dpp_u32<kRowShl12>(pr);
+        } else if constexpr (NP == 2) {
+          pf[1][2 * x + i] = dpp_u32<kRowShl8>(pr);
+        }
       }
-
-    if (t0 + 64 > t_end) {  // values past the partition's end weigh nothing, NaN scales of stale rows among them
-#pragma unroll
-      for (int q = 0; q < 4; ++q) vs[q] = keep_bytes(vs[q], live);
-    }
-#pragma unroll
-    for (int q = 0; q < 4; ++q)
+    auto products = [&](auto qq) {
+      constexpr int q = decltype(qq)::value;
+      const u32 sc[4] = {dpp_u32<kRowBcast + 4 * q>(vs), dpp_u32<kRowBcast + 4 * q + 1>(vs),
+                         dpp_u32<kRowBcast + 4 * q + 2>(vs), dpp_u32<kRowBcast + 4 * q + 3>(vs)};
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         u32x4 lo, hi;
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
-          const u32 c = vc[q][2 * h + x], sc = vs[q][2 * h + x];
-          const u32 v0 = fp4_pair<0>(c, scale_of<0>(sc)), v1 = fp4_pair<1>(c, scale_of<1>(sc));
-          const u32 v2 = fp4_pair<2>(c, scale_of<2>(sc)), v3 = fp4_pair<3>(c, scale_of<3>(sc));
+          const u32 c = vc[q][2 * h + x], w = sc[2 * h + x];
+          const u32 v0 = fp4_pair<0>(c, scale_of<0>(w)), v1 = fp4_pair<1>(c, scale_of<1>(w));
+          const u32 v2 = fp4_pair<2>(c, scale_of<2>(w)), v3 = fp4_pair<3>(c, scale_of<3>(w));
           lo[2 * x] = pair_lo(v0, v1);
           lo[2 * x + 1] = pair_lo(v2, v3);
           hi[2 * x] = pair_hi(v0, v1);
@@ -255,6 +436,25 @@ paged_decode_fp4_kernel(DecodeFp4Args a) {
         o[2 * q] = mfma16(lo, pf[h], o[2 * q]);
         o[2 * q + 1] = mfma16(hi, pf[h], o[2 * q + 1]);
       }
+    };
+    products(Int<0>{});
+    products(Int<1>{});
+    products(Int<2>{});
+    products(Int<3>{});
+    __builtin_amdgcn_sched_barrier(0);
+    if (next < t_end) load_v();
+  };
+  if (int t0 = p * part_tokens + 64 * w; t0 < t_end) {
+    look_up(t0);
+    locate(t0);
+    load_k();
+    load_v();
+    look_up(t0 + 64 * kWaves);
+#pragma unroll 1
+    do {
+      step(t0, t0 + 64 * kWaves);
+      t0 += 64 * kWaves;
+    } while (t0 < t_end);
   }
 
   {
@@ -265,6 +465,8 @@ paged_decode_fp4_kernel(DecodeFp4Args a) {
   }
 
   // Register i of o[e] is dim 16 e + 4 gq + i of head n.
+  if constexpr (GP <= 4) l += dpp<kRowRor4>(l);
+  if constexpr (GP <= 8) l += dpp<kDppRowRor8>(l);
   l = sum_over_quarters(l);
   if (n < G) {
 #pragma unroll
@@ -276,22 +478,22 @@ paged_decode_fp4_kernel(DecodeFp4Args a) {
   }
   __syncthreads();
 
-  // The waves' results meet: a half-wave takes heads hw, hw + 8, its lane dims 4 dl .. 4 dl + 3.
-  constexpr int HP = (GP + 7) / 8;
+  // The waves' results meet: a half-wave takes heads hw, hw + kHalves, its lane dims 4 dl .. 4 dl + 3.
+  constexpr int HP = (GP + kHalves - 1) / kHalves;
   const int hw = tid >> 5, dl = lane & 31;
   f32x4 acc[HP];
   float mx[HP], ls[HP];
 #pragma unroll
   for (int k = 0; k < HP; ++k) {
-    const int h = min(hw + 8 * k, G - 1);
-    float M = -INFINITY;
+    const int h = min(hw + kHalves * k, G - 1);
+    float M = s_m[0][h];
 #pragma unroll
-    for (int x = 0; x < kWaves; ++x) M = fmaxf(M, s_m[x][h]);
+    for (int x = 1; x < kWaves; ++x) M = fmaxf(M, s_m[x][h]);
     acc[k] = f32x4{0.f, 0.f, 0.f, 0.f};
     ls[k] = 0.f;
 #pragma unroll
     for (int x = 0; x < kWaves; ++x) {
-      const float f = s_m[x][h] == -INFINITY ? 0.f : fast_exp2(s_m[x][h] - M);
+      const float f = fast_exp2(s_m[x][h] - M);
       acc[k] += f * *reinterpret_cast<const f32x4 *>(&s_o[x][h * HS + 4 * dl]);
       ls[k] += f * s_l[x][h];
     }
@@ -305,7 +507,7 @@ paged_decode_fp4_kernel(DecodeFp4Args a) {
   if (n_parts == 1) {
 #pragma unroll
     for (int k = 0; k < HP; ++k)
-      if (hw + 8 * k < G) write_out(hw + 8 * k, acc[k], ls[k]);
+      if (hw + kHalves * k < G) write_out(hw + kHalves * k, acc[k], ls[k]);
     return;
   }
 
@@ -315,7 +517,7 @@ paged_decode_fp4_kernel(DecodeFp4Args a) {
   const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(base, 0, n_parts * rec_bytes, kBufferRsrcWord3);
 #pragma unroll
   for (int k = 0; k < HP; ++k) {
-    const int h = hw + 8 * k;
+    const int h = hw + kHalves * k;
     if (h < G) {
       const int off = p * rec_bytes + h * (HS * (int)sizeof(float));
       __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, acc[k]), rsrc, off + 16 + 16 * dl, 0,
@@ -334,34 +536,76 @@ paged_decode_fp4_kernel(DecodeFp4Args a) {
   __syncthreads();
   if (s_last != n_parts - 1) return;
 
-  // The last arriver joins the partitions, in their order.
+  // The last arriver joins the partitions.  The heads share out the half-waves: `split` of them take a head, each every
+  // split-th run of kRun partitions, whose records it loads together; their shares meet in LDS, in order.
+  constexpr int kRun = 8;
+  const int slots_log2 = min(G <= 1 ? 0 : 32 - __builtin_clz(G - 1), kHalvesLog2);
+  const int split = kHalves >> slots_log2;
+  const int sp = hw >> slots_log2;
+  float *so = &s_o[0][0];  // free: every wave has passed two barriers since it read them
 #pragma unroll 1
-  for (int h = hw; h < G; h += 8) {
+  for (int h = hw & ((1 << slots_log2) - 1); h < G; h += kHalves) {
     const int hoff = h * (HS * (int)sizeof(float));
-    float M = -INFINITY, den = 0.f;
+    float M = kNoScore, den = 0.f;
     f32x4 num = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 1
-    for (int y = 0; y < n_parts; ++y) {
-      const u32x2 ml = __builtin_amdgcn_raw_buffer_load_b64(rsrc, y * rec_bytes + hoff, 0, kCachePolicyAgent);
-      const u32x4 v = __builtin_amdgcn_raw_buffer_load_b128(rsrc, y * rec_bytes + hoff + 16 + 16 * dl, 0,
-                                                            kCachePolicyAgent);
-      const float pm = __uint_as_float(ml[0]);
-      const float up = fmaxf(M, pm);
-      const float f_old = M == -INFINITY ? 0.f : fast_exp2(M - up), f_new = pm == -INFINITY ? 0.f : fast_exp2(pm - up);
-      num = num * f_old + f_new * __builtin_bit_cast(f32x4, v);
-      den = den * f_old + f_new * __uint_as_float(ml[1]);
+    for (int y0 = sp * kRun; y0 < n_parts; y0 += split * kRun) {
+      u32x2 ml[kRun];
+      u32x4 v[kRun];
+#pragma unroll
+      for (int y = 0; y < kRun; ++y) {  // past n_parts: zeros without a memory access
+        ml[y] = __builtin_amdgcn_raw_buffer_load_b64(rsrc, (y0 + y) * rec_bytes + hoff, 0, kCachePolicyAgent);
+        v[y] = __builtin_amdgcn_raw_buffer_load_b128(rsrc, (y0 + y) * rec_bytes + hoff + 16 + 16 * dl, 0,
+                                                     kCachePolicyAgent);
+      }
+      float up = M;
+#pragma unroll
+      for (int y = 0; y < kRun; ++y)
+        if (y0 + y < n_parts) up = fmaxf(up, __uint_as_float(ml[y][0]));
+      const float f_old = fast_exp2(M - up);
+      num *= f_old;
+      den *= f_old;
+#pragma unroll
+      for (int y = 0; y < kRun; ++y) {
+        const float f = y0 + y < n_parts ? fast_exp2(__uint_as_float(ml[y][0]) - up) : 0.f;
+        num += f * __builtin_bit_cast(f32x4, v[y]);
+        den += f * __uint_as_float(ml[y][1]);
+      }
       M = up;
     }
-    write_out(h, num, den);
+    if (split > 1) {  // then every half-wave has one head at most
+      *reinterpret_cast<f32x4 *>(so + hw * HS + 4 + 4 * dl) = num;
+      if (dl == 0) *reinterpret_cast<u32x2 *>(so + hw * HS) = u32x2{__float_as_uint(M), __float_as_uint(den)};
+    } else {
+      write_out(h, num, den);
+    }
+  }
+  if (split > 1) {
+    __syncthreads();
+    if (sp == 0 && hw < G) {
+      float M = kNoScore, den = 0.f;
+      f32x4 num = {0.f, 0.f, 0.f, 0.f};
+      for (int x = 0; x < split; ++x) M = fmaxf(M, so[((x << slots_log2) + hw) * HS]);
+      for (int x = 0; x < split; ++x) {
+        const float *r = so + ((x << slots_log2) + hw) * HS;
+        const float f = fast_exp2(r[0] - M);
+        num += f * *reinterpret_cast<const f32x4 *>(r + 4 + 4 * dl);
+        den += f * r[1];
+      }
+      write_out(hw, num, den);
+    }
   }
 }
 
 template <int GP>
 int launch(const DecodeFp4Args &a, hipStream_t stream) {
-  const int64_t units = (int64_t)a.batch * a.num_kv_heads;
-  // partitions: one per unit at least, kTarget in all besides, and no more than the bound allows
-  const int64_t items = min(units * a.max_parts, units + kTarget);
-  hipLaunchKernelGGL((paged_decode_fp4_kernel<GP>), dim3((unsigned)items), dim3(kWaves * 64), 0, stream, a);
+  static_assert(kWaves * GP >= kHalves, "the shares of a join fit s_o");
+  const int units = a.batch * a.num_kv_heads;  // <= kCounterSlots
+  const int64_t items = min((int64_t)units * a.max_parts, (int64_t)max_partitions(units));
+  if (a.bs_log2 >= 6)
+    hipLaunchKernelGGL((paged_decode_fp4_kernel<GP, true>), dim3((unsigned)items), dim3(kWaves * 64), 0, stream, a);
+  else
+    hipLaunchKernelGGL((paged_decode_fp4_kernel<GP, false>), dim3((unsigned)items), dim3(kWaves * 64), 0, stream, a);
   return launch_status();
 }
 
@@ -389,7 +633,7 @@ extern "C" int nvamd_paged_decode_fp4(void *out, int64_t out_stride, const void 
       q_stride < (int64_t)num_heads * head_dim || out_stride < (int64_t)num_heads * head_dim)
     return NVAMD_EINVAL;
   if ((int64_t)batch * num_kv_heads > kCounterSlots || batch > 65535 || max_context_len > kMaxContext ||
-      ((int64_t)bt_width << bs_log2) > 0x7fffffff)
+      ((int64_t)bt_width << bs_log2) > 0x7fffffff || (((int64_t)num_blocks * num_kv_heads) << bs_log2) >> 4 > 0x7fffffff)
     return NVAMD_EUNSUPPORTED;
   if (!workspace ||
       workspace_bytes < nvamd_paged_decode_workspace_size(batch, num_heads, num_kv_heads, max_context_len))

@@ -244,7 +244,7 @@ def test_attention_refuses():
     def decode(out=q, q=q, bt=bt, lens=lens, ws=ws):
         _C.paged_decode_fp4(out, q, pages(), pages(), bt, lens, 0.1, 48, ws)
 
-    for match, over in (("shape mismatch", dict(out=heads(3, 16))), ("block_tables", dict(bt=bt.long())),
+    for match, over in (("shape mismatch", dict(out=heads(3, 16))), ("must be bfloat16", dict(q=heads(4, 16, dtype=torch.float32))), ("block_tables", dict(bt=bt.long())),
                         ("block_tables", dict(bt=bt[:3])), ("block_tables", dict(bt=torch.cat([bt, bt]))),
                         ("rows must be dense", dict(bt=torch.zeros(4, 6, dtype=torch.int32)[:, ::2])),
                         ("context_lens", dict(lens=lens.long())), ("context_lens", dict(lens=lens[:3])),
