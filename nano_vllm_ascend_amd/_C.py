@@ -591,9 +591,9 @@ class Fp4Pages(NamedTuple):
         return nb, bs, hkv, 2 * width
 
 
-def _fp4_pages(key_pages: Fp4Pages, value_pages: Fp4Pages) -> tuple[tuple[int, int, int, int], tuple]:
-    """Checks the pages of a layer; returns [blocks, block_size, kv heads, head_dim] and their addresses.  (Written out: a
-    small batch's eager call is bound by the host.)"""
+def _fp4_pages(key_pages: Fp4Pages, value_pages: Fp4Pages):
+    """Checks the pages of a layer; returns blocks, block_size, kv heads, their addresses and their device.  (The checks of
+    this section are written out: a small batch's eager call is bound by the host.)"""
     if type(key_pages) is not Fp4Pages or type(value_pages) is not Fp4Pages:
         raise ValueError("key and value pages must be Fp4Pages")
     kc, ks = key_pages
@@ -610,71 +610,83 @@ def _fp4_pages(key_pages: Fp4Pages, value_pages: Fp4Pages) -> tuple[tuple[int, i
     if not (kc.dtype is u8 and ks.dtype is u8 and vc.dtype is u8 and vs.dtype is u8 and kc.is_contiguous()
             and ks.is_contiguous() and vc.is_contiguous() and vs.is_contiguous()):
         raise ValueError("pages must be contiguous uint8 tensors")
-    return (nb, bs, hkv, 2 * FP4_ROW_BYTES), (kc.data_ptr(), ks.data_ptr(), vc.data_ptr(), vs.data_ptr())
+    device = kc.get_device()
+    if not device == ks.get_device() == vc.get_device() == vs.get_device():
+        raise ValueError("the pages of a layer must be on one device")
+    return nb, bs, hkv, (kc.data_ptr(), ks.data_ptr(), vc.data_ptr(), vs.data_ptr()), device
 
 
-def _on_current_device(*tensors: torch.Tensor) -> None:
-    """Every launch goes to the current device's current stream: its tensors have to live there."""
-    device = tensors[0].get_device()
+def _stream_of(device: int, *tensors: torch.Tensor) -> int:
+    """The current stream, which every launch goes to: the tensors and the pages have to be on its device."""
     for t in tensors:
-        if t.get_device() != device or device < 0:
-            raise ValueError(f"every tensor must be on the GPU, and on the same one: got {[str(t.device) for t in tensors]}")
+        if t.get_device() != device:
+            raise ValueError(f"every tensor must be on the GPU of the pages (device {device}), one is on {t.device}")
+    if device < 0:
+        raise ValueError("every tensor must be on the GPU")
     if device != torch.cuda.current_device():
         raise ValueError(f"the tensors are on device {device}, the current device is {torch.cuda.current_device()}")
+    return _raw_stream(device) if _raw_stream is not None else _stream()
 
 
 def _heads(name: str, t: torch.Tensor, rows: int, heads: int, d: int) -> int:
     """Checks a [T, heads, D] bf16 view of dense rows; returns its row stride."""
-    if t.dtype is not torch.bfloat16:
-        raise ValueError(f"{name} must be bfloat16, got {t.dtype}")
     if t.shape != (rows, heads, d):
         raise ValueError(f"{name} must be {(rows, heads, d)}, got {tuple(t.shape)}")
-    stride = t.stride()
-    if rows and (stride[2] != 1 or (heads > 1 and stride[1] != d)):
+    if t.dtype is not torch.bfloat16:
+        raise ValueError(f"{name} must be bfloat16, got {t.dtype}")
+    row, head, unit = t.stride()
+    if (unit != 1 or (head != d and heads > 1)) and rows:
         raise ValueError(f"rows of {name} {tuple(t.shape)} are not dense")
-    return stride[0] if rows > 1 else max(stride[0], heads * d)
+    return row if rows > 1 else max(row, heads * d)  # a single row's stride says nothing
 
 
-def _page_slots(slot_mapping: torch.Tensor, rows: int, num_slots: int) -> None:
-    if (slot_mapping.dtype is not torch.int64 or slot_mapping.dim() != 1 or slot_mapping.numel() != rows
-            or not slot_mapping.is_contiguous()):
+def _page_slots(slot_mapping: torch.Tensor, rows: int, num_slots: int) -> int:
+    if (slot_mapping.dtype is not torch.int64 or slot_mapping.shape != (rows,) or not slot_mapping.is_contiguous()):
         raise ValueError(f"slot_mapping must be contiguous int64 [{rows}], got {slot_mapping.dtype} "
                          f"{tuple(slot_mapping.shape)}")
     if _range_checks and _checking():
         check_slots(slot_mapping, num_slots)
+    return slot_mapping.data_ptr()
 
 
 def kv_cache_write_fp4(key_states: torch.Tensor, value_states: torch.Tensor, key_pages: Fp4Pages,
                        value_pages: Fp4Pages, slot_mapping: torch.Tensor) -> None:
     """Rows [T, Hkv, 128] of bf16 keys and values, quantised into the pages at their slots (-1: padding, skipped; no slot
     twice in a call)."""
-    lib = load()
-    (nb, bs, hkv, d), pages = _fp4_pages(key_pages, value_pages)
-    t = key_states.shape[0]
-    strides = _heads("key_states", key_states, t, hkv, d), _heads("value_states", value_states, t, hkv, d)
-    _page_slots(slot_mapping, t, nb * bs)
-    _on_current_device(key_states, value_states, *key_pages, *value_pages, slot_mapping)
-    _check(lib.nvamd_kv_cache_write_fp4(
-        key_states.data_ptr(), strides[0], value_states.data_ptr(), strides[1], *pages, nb, bs,
-        slot_mapping.data_ptr(), t, hkv, d, _stream()), "nvamd_kv_cache_write_fp4")
+    lib = _lib or load()
+    nb, bs, hkv, pages, device = _fp4_pages(key_pages, value_pages)
+    t, d = key_states.shape[0], 2 * FP4_ROW_BYTES
+    k_stride, v_stride = _heads("key_states", key_states, t, hkv, d), _heads("value_states", value_states, t, hkv, d)
+    slots = _page_slots(slot_mapping, t, nb * bs)
+    status = lib.nvamd_kv_cache_write_fp4(
+        key_states.data_ptr(), k_stride, value_states.data_ptr(), v_stride, *pages, nb, bs, slots, t, hkv, d,
+        _stream_of(device, key_states, value_states, slot_mapping))
+    if status:
+        _check(status, "nvamd_kv_cache_write_fp4")
 
 
 def kv_cache_read_fp4(key_pages: Fp4Pages, value_pages: Fp4Pages, slot_mapping: torch.Tensor,
                       k_out: torch.Tensor | None = None,
                       v_out: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """The bf16 keys and values [T, Hkv, 128] that the pages hold at the slots (zeros for -1)."""
-    lib = load()
-    (nb, bs, hkv, d), pages = _fp4_pages(key_pages, value_pages)
-    t = slot_mapping.numel()
-    _page_slots(slot_mapping, t, nb * bs)
-    k, v = (torch.empty((t, hkv, d), dtype=torch.bfloat16, device=key_pages.codes.device) if out is None else out
-            for out in (k_out, v_out))
-    strides = _heads("k_out", k, t, hkv, d), _heads("v_out", v, t, hkv, d)
-    _on_current_device(k, v, *key_pages, *value_pages, slot_mapping)
-    _check(lib.nvamd_kv_cache_read_fp4(
-        k.data_ptr(), strides[0], v.data_ptr(), strides[1], *pages, nb, bs, slot_mapping.data_ptr(), t, hkv, d,
-        _stream()), "nvamd_kv_cache_read_fp4")
-    return k, v
+    lib = _lib or load()
+    nb, bs, hkv, pages, device = _fp4_pages(key_pages, value_pages)
+    t, d = slot_mapping.shape[0], 2 * FP4_ROW_BYTES
+    slots = _page_slots(slot_mapping, t, nb * bs)
+    k_stride = v_stride = hkv * d
+    if k_out is None:
+        k_out = torch.empty((t, hkv, d), dtype=torch.bfloat16, device=key_pages.codes.device)
+    else:
+        k_stride = _heads("k_out", k_out, t, hkv, d)
+    if v_out is None:
+        v_out = torch.empty((t, hkv, d), dtype=torch.bfloat16, device=key_pages.codes.device)
+    else:
+        v_stride = _heads("v_out", v_out, t, hkv, d)
+    status = lib.nvamd_kv_cache_read_fp4(k_out.data_ptr(), k_stride, v_out.data_ptr(), v_stride, *pages, nb, bs, slots,
+                                         t, hkv, d, _stream_of(device, k_out, v_out, slot_mapping))
+    if status:
+        _check(status, "nvamd_kv_cache_read_fp4")
+    return k_out, v_out
 
 
 def qk_norm_rope_fp4(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_weight: torch.Tensor,
@@ -685,43 +697,48 @@ def qk_norm_rope_fp4(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_weight
 
     Returns the rotated q: ``q_out``, which may be q itself, or a new tensor.  The rotated k is written
     only to the pages unless ``k_out`` (which may be k itself) asks for it.  64-bit arithmetic, one rounding to bf16."""
-    lib = load()
-    (nb, bs, hkv, d), pages = _fp4_pages(key_pages, value_pages)
+    lib = _lib or load()
+    nb, bs, hkv, pages, device = _fp4_pages(key_pages, value_pages)
+    d = 2 * FP4_ROW_BYTES
     if q.dim() != 3:
         raise ValueError(f"q must be [T, heads, D], got {tuple(q.shape)}")
     t, hq, _ = q.shape
+    q_stride, k_stride, v_stride = _heads("q", q, t, hq, d), _heads("k", k, t, hkv, d), _heads("v", v, t, hkv, d)
     if q_out is None:
-        q_out = torch.empty((t, hq, d), dtype=torch.bfloat16, device=q.device)
-    rows = [("q_out", q_out, hq), ("q", q, hq), ("k", k, hkv), ("v", v, hkv)]
-    qo_stride, q_stride, k_stride, v_stride = (_heads(name, x, t, h, d) for name, x, h in rows)
-    ko_stride = 0 if k_out is None else _heads("k_out", k_out, t, hkv, d)
-    for out, x, strides in ((q_out, q, (qo_stride, q_stride)), (k_out, k, (ko_stride, k_stride))):
-        if out is not None and out.data_ptr() == x.data_ptr() and strides[0] != strides[1]:
-            raise ValueError("an output in place of its input must have the input's row stride")
+        q_out, qo_stride = torch.empty((t, hq, d), dtype=torch.bfloat16, device=q.device), hq * d
+    else:
+        qo_stride = _heads("q_out", q_out, t, hq, d)
+    q_ptr, k_ptr, qo_ptr, ko_ptr, ko_stride = q.data_ptr(), k.data_ptr(), q_out.data_ptr(), None, 0
+    if k_out is not None:
+        ko_stride, ko_ptr = _heads("k_out", k_out, t, hkv, d), k_out.data_ptr()
+    if (qo_ptr == q_ptr and qo_stride != q_stride) or (ko_ptr == k_ptr and ko_stride != k_stride):
+        raise ValueError("an output in place of its input must have the input's row stride")
     for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
-        if w.dtype is not torch.bfloat16 or w.numel() != d or not w.is_contiguous():
+        if w.dtype is not torch.bfloat16 or w.shape != (d,) or not w.is_contiguous():
             raise ValueError(f"{name} must be contiguous bf16 [{d}]")
-    if positions.dtype is not torch.int64 or positions.numel() != t or not positions.is_contiguous():
+    if positions.dtype is not torch.int64 or positions.shape != (t,) or not positions.is_contiguous():
         raise ValueError(f"positions must be contiguous int64 [{t}]")
-    if (cos_sin.dtype is not torch.float32 or cos_sin.dim() != 2 or cos_sin.shape[1] != d
-            or not cos_sin.is_contiguous()):
+    table = cos_sin.shape
+    if cos_sin.dtype is not torch.float32 or len(table) != 2 or table[1] != d or not cos_sin.is_contiguous():
         raise ValueError("cos_sin must be contiguous fp32 [max_positions, head_dim]")
-    _page_slots(slot_mapping, t, nb * bs)
-    _on_current_device(q, k, v, q_out, q if k_out is None else k_out, q_weight, k_weight, positions, cos_sin,
-                       *key_pages, *value_pages, slot_mapping)
+    slots = _page_slots(slot_mapping, t, nb * bs)
     if _range_checks and _checking():
-        check_positions(positions, cos_sin.shape[0])
-    _check(lib.nvamd_qk_norm_rope_fp4(
-        q_out.data_ptr(), qo_stride, _ptr(k_out), ko_stride, q.data_ptr(), q_stride, k.data_ptr(), k_stride,
-        v.data_ptr(), v_stride, q_weight.data_ptr(), k_weight.data_ptr(), positions.data_ptr(), cos_sin.data_ptr(),
-        cos_sin.shape[0], *pages, nb, bs, slot_mapping.data_ptr(), t, hq, hkv, d, float(eps), _stream()),
-        "nvamd_qk_norm_rope_fp4")
+        check_positions(positions, table[0])
+    status = lib.nvamd_qk_norm_rope_fp4(
+        qo_ptr, qo_stride, ko_ptr, ko_stride, q_ptr, q_stride, k_ptr, k_stride, v.data_ptr(), v_stride,
+        q_weight.data_ptr(), k_weight.data_ptr(), positions.data_ptr(), cos_sin.data_ptr(), table[0], *pages, nb, bs,
+        slots, t, hq, hkv, d, eps,
+        _stream_of(device, q, k, v, q_out, q if k_out is None else k_out, q_weight, k_weight, positions, cos_sin,
+                   slot_mapping))
+    if status:
+        _check(status, "nvamd_qk_norm_rope_fp4")
     return q_out
 
 
 def _fp4_attention_args(out, q, key_pages, value_pages, block_tables, seqs: int):
-    """Checked arguments that decode and prefill share, up to the block tables, and [heads, kv heads, head_dim]."""
-    (nb, bs, hkv, d), pages = _fp4_pages(key_pages, value_pages)
+    """Checked arguments that decode and prefill share, up to the block tables; [heads, kv heads, head_dim]; the device."""
+    nb, bs, hkv, pages, device = _fp4_pages(key_pages, value_pages)
+    d = 2 * FP4_ROW_BYTES
     shape = q.shape
     if len(shape) != 3 or out.shape != shape:
         raise ValueError(f"q/out shape mismatch: {tuple(shape)} vs {tuple(out.shape)}")
@@ -743,7 +760,7 @@ def _fp4_attention_args(out, q, key_pages, value_pages, block_tables, seqs: int)
     least = hq * d  # a single row's stride says nothing
     return (out.data_ptr(), out_stride[0] if t > 1 else max(out_stride[0], least), q.data_ptr(),
             q_stride[0] if t > 1 else max(q_stride[0], least), *pages, nb, bs, block_tables.data_ptr(),
-            max(bt_stride[0], width), width), (hq, hkv, d)
+            max(bt_stride[0], width), width), (hq, hkv, d), device
 
 
 def paged_decode_fp4(out: torch.Tensor, q: torch.Tensor, key_pages: Fp4Pages, value_pages: Fp4Pages,
@@ -752,18 +769,18 @@ def paged_decode_fp4(out: torch.Tensor, q: torch.Tensor, key_pages: Fp4Pages, va
     """``paged_decode`` over pages of 4 bits; the workspace is the same (``alloc_paged_decode_workspace``)."""
     lib = _lib or load()
     b = q.shape[0]
-    args, heads = _fp4_attention_args(out, q, key_pages, value_pages, block_tables, b)
+    args, heads, device = _fp4_attention_args(out, q, key_pages, value_pages, block_tables, b)
     if block_tables.shape[0] != b:
         raise ValueError(f"block_tables must be int32 [{b}, W]")
-    if context_lens.dtype is not torch.int32 or context_lens.numel() != b or not context_lens.is_contiguous():
+    if context_lens.dtype is not torch.int32 or context_lens.shape != (b,) or not context_lens.is_contiguous():
         raise ValueError(f"context_lens must be contiguous int32 [{b}]")
     if not workspace.is_contiguous():
         raise ValueError("workspace must be contiguous")
-    _on_current_device(q, out, *key_pages, *value_pages, block_tables, context_lens, workspace)
     if _range_checks and _checking():
         check_paged_context(block_tables, context_lens, args[8], args[9], int(max_context_len))
     status = lib.nvamd_paged_decode_fp4(*args, context_lens.data_ptr(), b, *heads, scale, max_context_len,
-                                        workspace.data_ptr(), workspace.nbytes, _stream())
+                                        workspace.data_ptr(), workspace.nbytes,
+                                        _stream_of(device, q, out, block_tables, context_lens, workspace))
     if status:
         _check(status, "nvamd_paged_decode_fp4")
     return out
@@ -777,14 +794,15 @@ def paged_prefill_fp4(out: torch.Tensor, q: torch.Tensor, key_pages: Fp4Pages, v
     if cu_seqlens_q.dtype is not torch.int32 or cu_seqlens_q.dim() != 1 or not cu_seqlens_q.is_contiguous():
         raise ValueError("cu_seqlens_q must be contiguous int32 [n + 1]")
     n = cu_seqlens_q.numel() - 1
-    args, heads = _fp4_attention_args(out, q, key_pages, value_pages, block_tables, n)
+    args, heads, device = _fp4_attention_args(out, q, key_pages, value_pages, block_tables, n)
     if n < 0 or kv_lens.dtype is not torch.int32 or kv_lens.numel() < n or not kv_lens.is_contiguous():
         raise ValueError("kv_lens must be contiguous int32, one per sequence")
-    _on_current_device(out, q, *key_pages, *value_pages, block_tables, cu_seqlens_q, kv_lens)
     if _range_checks and _checking():
         check_paged_context(block_tables[:n], kv_lens[:n], args[8], args[9])
-    _check(lib.nvamd_paged_prefill_fp4(*args, cu_seqlens_q.data_ptr(), kv_lens.data_ptr(), n, q.shape[0],
-                                       int(max_q_len), *heads, float(scale), _stream()), "nvamd_paged_prefill_fp4")
+    status = lib.nvamd_paged_prefill_fp4(*args, cu_seqlens_q.data_ptr(), kv_lens.data_ptr(), n, q.shape[0], max_q_len,
+                                         *heads, scale, _stream_of(device, q, out, block_tables, cu_seqlens_q, kv_lens))
+    if status:
+        _check(status, "nvamd_paged_prefill_fp4")
     return out
 
 

@@ -1,9 +1,11 @@
 // The 4-bit paged KV cache: writing rows, reading rows back, and the per-head QK-RMSNorm + RoPE that
 // writes them in the same pass (the 4-bit counterparts of kv_store.hip).
 //
-// Every kernel gives an aligned group of 8 lanes one head vector: lane c holds dims 8c..8c+7 and 64+8c..64+8c+7, so
-// a block of 32 dims is the low (or high) half of 4 consecutive lanes, its maximum two DPP steps away, and RoPE
-// needs no lane exchange.
+// The writing kernels give a wave 8 consecutive tokens, an aligned group of 8 lanes each, and a run of their heads one
+// after another: the rotation's table row, the weights and the slots are read once for the run, rows of a head that
+// follow one another in a page are written together, and the 8 tokens of a head's values meet in LDS so that bytes of
+// consecutive tokens leave as one store.  Of a head vector, lane c of a group holds dims 8c..8c+7 and 64+8c..64+8c+7: a block of
+// 32 dims is the low (or high) half of 4 consecutive lanes, its maximum two DPP steps away, and RoPE needs no lane exchange.
 #include "fp4.h"
 
 namespace nvamd {
@@ -27,6 +29,14 @@ __device__ __forceinline__ u32 quantise8(u32x4 x, u32 &scale) {
   scale = fp4_scale_byte(quad_max(m));
   return scale == kFp4Nan ? 0u : fp4_codes(x, fp4_scale(scale));
 }
+
+// A 64-bit value of one lane, as a scalar.
+__device__ __forceinline__ int64_t lane_value(int64_t v, int lane) {
+  const u32 lo = (u32)__builtin_amdgcn_readlane((int)(u32)v, lane);
+  const u32 hi = (u32)__builtin_amdgcn_readlane((int)(u32)((uint64_t)v >> 32), lane);
+  return (int64_t)(((uint64_t)hi << 32) | lo);
+}
+__device__ __forceinline__ int64_t uniform64(int64_t v) { return lane_value(v, 0); }
 
 struct Fp4Row {
   int64_t tile;  // 16-token tile of the row's page and head
@@ -54,24 +64,92 @@ __device__ __forceinline__ void store_key(const Fp4Cache &cache, const Fp4Row &r
 }
 
 // A byte of the values holds dims 32q + r and 32q + 16 + r: the two lanes of a quad that differ in bit 1 hold the two halves
-// of a block, and exchange so that the one builds the bytes of the low block, the other those of the high one.
-__device__ __forceinline__ void store_value(const Fp4Cache &cache, const Fp4Row &r, int c, u32x4 lo, u32x4 hi) {
+// of a block, and exchange so that the one builds the bytes of the low block, the other those of the high one.  The bytes go to
+// `tile` in LDS, [64 bytes of a row][8 tokens], at token `tok`.
+__device__ __forceinline__ void value_bytes(const Fp4Cache &cache, const Fp4Row &r, bool live, int c, int tok, u32x4 lo,
+                                            u32x4 hi, u8 *tile) {
   u32 s_lo, s_hi;
   const u32 w_lo = quantise8(lo, s_lo), w_hi = quantise8(hi, s_hi);
   const u32 o_lo = quad_xor2(w_lo), o_hi = quad_xor2(w_hi);
   const bool second = (c & 2) != 0;
   const u32 first16 = second ? o_hi : w_lo, last16 = second ? w_hi : o_lo;
+  // bytes j of even and of odd nibbles: (low nibble of the first half, low nibble of the second)
+  const u32 even = (first16 & 0x0f0f0f0fu) | ((last16 & 0x0f0f0f0fu) << 4);
+  const u32 odd = ((first16 >> 4) & 0x0f0f0f0fu) | (last16 & 0xf0f0f0f0u);
   const int q = (second ? 2 : 0) + (c >> 2);
-  u8 *p = cache.v_codes + r.tile * kFp4TileBytes + (16 * q + 8 * (c & 1)) * kFp4Tile + r.t;
+  u8 *p = tile + (16 * q + 8 * (c & 1)) * 8 + tok;
 #pragma unroll
-  for (int j = 0; j < 8; ++j)
-    p[j * kFp4Tile] = (u8)(((first16 >> (4 * j)) & 15) | (((last16 >> (4 * j)) & 15) << 4));
-  if ((c & 3) == 0) {
+  for (int j = 0; j < 4; ++j) {
+    p[(2 * j) * 8] = (u8)(even >> (8 * j));
+    p[(2 * j + 1) * 8] = (u8)(odd >> (8 * j));
+  }
+  if (live && (c & 3) == 0) {
     u8 *s = cache.v_scales + r.tile * kFp4TileScales;
     s[fp4_value_scale_at(r.t, c >> 2)] = (u8)s_lo;
     s[fp4_value_scale_at(r.t, 2 + (c >> 2))] = (u8)s_hi;
   }
 }
+
+// The 8 tokens' bytes of row byte `lane` to their slots.  Where the slots follow one another the bytes are turned to their
+// places in 8-byte half rows: one store if they fill one, else those of each side of the border, words where whole.
+__device__ __forceinline__ void store_values(const Fp4Cache &cache, const u8 *tile, int64_t slot, bool run, int head,
+                                             int num_kv_heads, int bs_log2, int lane) {
+  auto place = [&](int64_t s) {  // of the byte of slot s
+    const Fp4Row r = row_at(s, head, num_kv_heads, bs_log2);
+    return cache.v_codes + r.tile * kFp4TileBytes + lane * kFp4Tile + r.t;
+  };
+  const u32x2 w = *reinterpret_cast<const u32x2 *>(tile + lane * 8);
+  if (run) {
+    const int64_t s0 = uniform64(slot);
+    const int o = (int)(s0 & 7);
+    if (o == 0) {
+      *reinterpret_cast<u32x2 *>(place(s0)) = w;
+      return;
+    }
+    const uint64_t x = ((uint64_t)w[1] << 32) | w[0];
+    const uint64_t y = (x << (8 * o)) | (x >> (64 - 8 * o));  // byte i: the token of slot i mod 8
+    u8 *before = place(s0) - o, *after = place(s0 + 8 - o);   // the half rows that the run ends and begins
+    const int border = o >> 2;                                // the word that holds bytes of both, if o % 4
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const u32 v = (u32)(y >> (32 * k));
+      if (k != border || (o & 3) == 0) {
+        *reinterpret_cast<u32 *>((4 * k >= o ? before : after) + 4 * k) = v;
+      } else {
+#pragma unroll
+        for (int i = 4 * k; i < 4 * k + 4; ++i) (i >= o ? before : after)[i] = (u8)(v >> (8 * (i & 3)));
+      }
+    }
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int64_t s = lane_value(slot, 8 * i);
+    if (s >= 0) *place(s) = (u8)(w[i >> 2] >> (8 * (i & 3)));
+  }
+}
+
+// A wave's own LDS writes before its own reads: LDS serves a wave in order, so only the compiler has to keep it.
+__device__ __forceinline__ void wave_lds_fence() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); }
+
+// Rows too many for the caches until their next use go past them (32 MB a tensor: half of the 256 MB Infinity Cache for two
+// tensors in and out).  36,488 x 8 heads, plain / nontemporal: written from nontemporal loads 53.5 / 49 us, read back with
+// nontemporal stores 66 / 58.6; 12,345 x 8 heads both together 28.2 / 31.1.
+constexpr int64_t kStreamElems = 16 << 20;
+template <bool STREAM>
+__device__ __forceinline__ void put16(u16 *p, u32x4 v) {
+  if constexpr (STREAM)
+    __builtin_nontemporal_store(v, reinterpret_cast<u32x4 *>(p));
+  else
+    st16(p, v);
+}
+template <bool STREAM>
+__device__ __forceinline__ u32x4 get16(const u16 *p) {
+  if constexpr (STREAM) return ld16_stream(p);
+  else return ld16(p);
+}
+
+constexpr int kWantedWaves = 4096;  // four waves on each SIMD of 256 CUs
 
 struct WriteArgs {
   const u16 *k;
@@ -84,34 +162,9 @@ struct WriteArgs {
   int num_tokens;
   int num_kv_heads;
   int bs_log2;
+  int heads_per_wave;
   u32 *err;
 };
-
-// Vectors of a token: its key heads, then its value heads.
-__global__ void __launch_bounds__(256)
-kv_write_fp4_kernel(WriteArgs a) {
-  const int vecs = 2 * a.num_kv_heads;
-  const int64_t gv = (int64_t)blockIdx.x * 32 + (threadIdx.x >> 3);
-  if (gv >= (int64_t)a.num_tokens * vecs) return;  // whole 8-lane groups leave together
-  const int t = (int)(gv / vecs);
-  const int vec = (int)(gv % vecs);
-  const int c = threadIdx.x & 7;
-  const int64_t slot = a.slots[t];
-  if (slot >= a.num_slots || slot < -1) {
-    if (vec == 0 && c == 0) flag_index_error(a.err, NVAMD_ERR_SLOT);
-    return;
-  }
-  if (slot < 0) return;  // -1: a padding row
-  const bool is_k = vec < a.num_kv_heads;
-  const int h = is_k ? vec : vec - a.num_kv_heads;
-  const u16 *src = (is_k ? a.k + t * a.k_stride : a.v + t * a.v_stride) + h * kHeadDim + 8 * c;
-  const u32x4 lo = ld16(src), hi = ld16(src + 64);
-  const Fp4Row r = row_at(slot, h, a.num_kv_heads, a.bs_log2);
-  if (is_k)
-    store_key(a.cache, r, c, lo, hi);
-  else
-    store_value(a.cache, r, c, lo, hi);
-}
 
 struct ReadArgs {
   u16 *k;
@@ -124,57 +177,94 @@ struct ReadArgs {
   int num_tokens;
   int num_kv_heads;
   int bs_log2;
+  int heads_per_wave;
   u32 *err;
 };
 
-// As the write, the other way round; a row without a slot, or with one outside the cache, is zeros.
+// As the writes, the other way round: a wave takes 8 tokens and a run of their key and value heads.  A row without a slot, or
+// with one outside the cache, is zeros.
+template <bool STREAM>
 __global__ void __launch_bounds__(256)
 kv_read_fp4_kernel(ReadArgs a) {
-  const int vecs = 2 * a.num_kv_heads;
-  const int64_t gv = (int64_t)blockIdx.x * 32 + (threadIdx.x >> 3);
-  if (gv >= (int64_t)a.num_tokens * vecs) return;
-  const int t = (int)(gv / vecs);
-  const int vec = (int)(gv % vecs);
-  const int c = threadIdx.x & 7;
-  const int64_t slot = a.slots[t];
-  const bool bad = slot >= a.num_slots || slot < -1;
-  if (bad && vec == 0 && c == 0) flag_index_error(a.err, NVAMD_ERR_SLOT);
-  const bool live = !bad && slot >= 0;
-  const bool is_k = vec < a.num_kv_heads;
-  const int h = is_k ? vec : vec - a.num_kv_heads;
-  const Fp4Row r = row_at(live ? slot : 0, h, a.num_kv_heads, a.bs_log2);
+  __shared__ __attribute__((aligned(16))) u8 s_tile[4][2][512];
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int c = lane & 7, tok = lane >> 3;
+  const int hkv = a.num_kv_heads;
+  const int h_begin = (blockIdx.y * 4 + w) * a.heads_per_wave;
+  const int h_end = min(h_begin + a.heads_per_wave, 2 * hkv);
+  if (h_begin >= h_end) return;
+  const int t = blockIdx.x * 8 + tok;
+  const bool exists = t < a.num_tokens;
+  int64_t slot = exists ? a.slots[t] : -1;
+  if (slot >= a.num_slots || slot < -1) {
+    if (h_begin == 0 && c == 0) flag_index_error(a.err, NVAMD_ERR_SLOT);
+    slot = -1;
+  }
+  const bool live = slot >= 0;
+  const bool run = __all(live && slot == uniform64(slot) + tok);
   const u32x4 zero = {0u, 0u, 0u, 0u};
-  if (is_k) {
-    u32x4 lo = zero, hi = zero;
-    if (live) {
-      const u32 *row = reinterpret_cast<const u32 *>(a.cache.k_codes + r.tile * kFp4TileBytes + r.t * kFp4RowBytes);
-      const u8 *s = a.cache.k_scales + r.tile * kFp4TileScales;
-      lo = fp4_values(row[c], fp4_scale(s[fp4_key_scale_at(r.t, c >> 2)]));
-      hi = fp4_values(row[8 + c], fp4_scale(s[fp4_key_scale_at(r.t, 2 + (c >> 2))]));
+#pragma unroll 1
+  for (int v = h_begin; v < h_end; ++v) {
+    const int h = v < hkv ? v : v - hkv;
+    const Fp4Row r = row_at(live ? slot : 0, h, hkv, a.bs_log2);
+    if (v < hkv) {
+      u32x4 lo = zero, hi = zero;
+      if (live) {
+        const u32 *row = reinterpret_cast<const u32 *>(a.cache.k_codes + r.tile * kFp4TileBytes + r.t * kFp4RowBytes);
+        const u8 *s = a.cache.k_scales + r.tile * kFp4TileScales;
+        lo = fp4_values(row[c], fp4_scale(s[fp4_key_scale_at(r.t, c >> 2)]));
+        hi = fp4_values(row[8 + c], fp4_scale(s[fp4_key_scale_at(r.t, 2 + (c >> 2))]));
+      }
+      if (exists) {
+        u16 *dst = a.k + t * a.k_stride + h * kHeadDim + 8 * c;
+        put16<STREAM>(dst, lo);
+        put16<STREAM>(dst + 64, hi);
+      }
+      continue;
     }
-    u16 *dst = a.k + t * a.k_stride + h * kHeadDim + 8 * c;
-    st16(dst, lo);
-    st16(dst + 64, hi);
-  } else {
-    // lane c: bytes 8(c % 2) .. +7 of block c / 2, dims 8(c % 2) + j of the block's first and of its second half
+    // Row byte `lane` of the 8 tokens, then through LDS to lane c of each: bytes 8 (c % 2) .. +7 of block c / 2.
+    auto place = [&](int64_t s) {
+      const Fp4Row x = row_at(s, h, hkv, a.bs_log2);
+      return a.cache.v_codes + x.tile * kFp4TileBytes + lane * kFp4Tile + x.t;
+    };
+    u8 *tile = s_tile[w][v & 1];
+    uint64_t bytes = 0;
+    if (run) {
+      const int64_t s0 = uniform64(slot);
+      const int o = (int)(s0 & 7);
+      const u8 *first = place(s0) - o;
+      bytes = *reinterpret_cast<const uint64_t *>(first);
+      if (o != 0) bytes = (bytes >> (8 * o)) | (*reinterpret_cast<const uint64_t *>(place(s0 + 8 - o)) << (64 - 8 * o));
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int64_t s = lane_value(slot, 8 * i);
+        if (s >= 0) bytes |= (uint64_t)*place(s) << (8 * i);
+      }
+    }
+    *reinterpret_cast<uint64_t *>(tile + lane * 8) = bytes;
+    wave_lds_fence();
     u32x4 first = zero, last = zero;
     if (live) {
-      const u8 *p = a.cache.v_codes + r.tile * kFp4TileBytes + (16 * (c >> 1) + 8 * (c & 1)) * kFp4Tile + r.t;
+      const u8 *p = tile + (16 * (c >> 1) + 8 * (c & 1)) * 8 + tok;
       const float scale = fp4_scale(a.cache.v_scales[r.tile * kFp4TileScales + fp4_value_scale_at(r.t, c >> 1)]);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const u32 x = fp4_pair<0>(p[2 * j * kFp4Tile], scale), y = fp4_pair<0>(p[(2 * j + 1) * kFp4Tile], scale);
+        const u32 x = fp4_pair<0>(p[2 * j * 8], scale), y = fp4_pair<0>(p[(2 * j + 1) * 8], scale);
         first[j] = pair_lo(x, y);
         last[j] = pair_hi(x, y);
       }
     }
-    u16 *dst = a.v + t * a.v_stride + h * kHeadDim + 32 * (c >> 1) + 8 * (c & 1);
-    st16(dst, first);
-    st16(dst + 16, last);
+    if (exists) {
+      u16 *dst = a.v + t * a.v_stride + h * kHeadDim + 32 * (c >> 1) + 8 * (c & 1);
+      put16<STREAM>(dst, first);
+      put16<STREAM>(dst + 16, last);
+    }
   }
 }
 
 struct NormRopeFp4Args {
+  WriteArgs w;
   u16 *q_out;
   int64_t q_out_stride;
   u16 *k_out;  // or null
@@ -186,9 +276,8 @@ struct NormRopeFp4Args {
   const int64_t *positions;
   const float *cos_sin;
   int max_positions;
-  int num_heads;
+  int num_heads;  // 0: rows are only stored
   float eps;
-  WriteArgs w;
 };
 
 __device__ __forceinline__ double dpp_add(double v, int lo, int hi) {
@@ -204,97 +293,161 @@ __device__ __forceinline__ double dpp_sum8(double v) {
   return dpp_sum<kDppHalfMirror>(dpp_sum<kDppQuadXor2>(dpp_sum<kDppQuadXor1>(v)));
 }
 
+// A 32-bit value that rounds to bf16 as x does.  A plain cast rounds too, and may land on a border of bf16 that x is only close
+// to; here all but the top 20 bits of the fraction are cut off, and the last of these is set if any of the rest was.
+__device__ __forceinline__ float bf16_bound(double x) {
+  const uint64_t b = __builtin_bit_cast(uint64_t, x);
+  const uint64_t top = (uint64_t)((u32)(b >> 32) | ((u32)b != 0u ? 1u : 0u)) << 32;
+  return (float)__builtin_bit_cast(double, top);
+}
+
 // y = x * rsqrt(mean(x^2) + eps) * w, then the rotation out[d] = y[d] cos[d] - y[d+64] sin[d], out[d+64] = y[d+64]
 // cos[d] + y[d] sin[d], in 64 bits with one rounding to bf16 at the end.  A 4-bit code's step is a
 // third to a half of the value, so a key that 32-bit arithmetic puts on the other side of a rounding border is that far off;
-// in 64 bits the code is that of the exact value.  The fp64 units keep up with the stream.
+// in 64 bits the code is that of the exact value.  x w is a product of bf16 numbers, exact in 32 bits, and the
+// reciprocal root comes last: one multiplication for each result.
 __device__ __forceinline__ void norm_rope_f64(u32x4 &lo, u32x4 &hi, const u32x4 w_lo, const u32x4 w_hi,
-                                              const float *table_row, int c, float eps) {
-  double x[16];
-#pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    x[2 * e] = bf16_lo(lo[e]);
-    x[2 * e + 1] = bf16_hi(lo[e]);
-    x[8 + 2 * e] = bf16_lo(hi[e]);
-    x[8 + 2 * e + 1] = bf16_hi(hi[e]);
-  }
+                                              const float (&cs)[8], const float (&sn)[8], double eps) {
   double ss = 0.0;
 #pragma unroll
-  for (int e = 0; e < 16; ++e) ss += x[e] * x[e];
-  const double rstd = rsqrt(dpp_sum8(ss) * (1.0 / kHeadDim) + (double)eps);
-  const f32x4 c0 = *reinterpret_cast<const f32x4 *>(table_row + 8 * c);
-  const f32x4 c1 = *reinterpret_cast<const f32x4 *>(table_row + 8 * c + 4);
-  const f32x4 s0 = *reinterpret_cast<const f32x4 *>(table_row + 64 + 8 * c);
-  const f32x4 s1 = *reinterpret_cast<const f32x4 *>(table_row + 64 + 8 * c + 4);
-  float r_lo[8], r_hi[8];
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const u32 wl = w_lo[e >> 1], wh = w_hi[e >> 1];
-    const double y_lo = x[e] * rstd * (double)((e & 1) ? bf16_hi(wl) : bf16_lo(wl));
-    const double y_hi = x[8 + e] * rstd * (double)((e & 1) ? bf16_hi(wh) : bf16_lo(wh));
-    const double cs = e < 4 ? c0[e & 3] : c1[e & 3], sn = e < 4 ? s0[e & 3] : s1[e & 3];
-    r_lo[e] = (float)(y_lo * cs - y_hi * sn);
-    r_hi[e] = (float)(y_hi * cs + y_lo * sn);
+  for (int e = 0; e < 4; ++e) {
+    const double x0 = bf16_lo(lo[e]), x1 = bf16_hi(lo[e]), x2 = bf16_lo(hi[e]), x3 = bf16_hi(hi[e]);
+    ss += x0 * x0;
+    ss += x1 * x1;
+    ss += x2 * x2;
+    ss += x3 * x3;
   }
+  const double rstd = rsqrt(dpp_sum8(ss) * (1.0 / kHeadDim) + eps);
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
-    lo[e] = pack_bf16x2(r_lo[2 * e], r_lo[2 * e + 1]);
-    hi[e] = pack_bf16x2(r_hi[2 * e], r_hi[2 * e + 1]);
+    float r_lo[2], r_hi[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const double y_lo = i ? bf16_hi(lo[e]) * bf16_hi(w_lo[e]) : bf16_lo(lo[e]) * bf16_lo(w_lo[e]);
+      const double y_hi = i ? bf16_hi(hi[e]) * bf16_hi(w_hi[e]) : bf16_lo(hi[e]) * bf16_lo(w_hi[e]);
+      const double c = cs[2 * e + i], s = sn[2 * e + i];
+      r_lo[i] = bf16_bound((y_lo * c - y_hi * s) * rstd);
+      r_hi[i] = bf16_bound((y_hi * c + y_lo * s) * rstd);
+    }
+    lo[e] = pack_bf16x2(r_lo[0], r_lo[1]);
+    hi[e] = pack_bf16x2(r_hi[0], r_hi[1]);
   }
 }
 
-// Vectors of a token: its query heads, its key heads, its value heads.
+// A wave: 8 tokens, heads_per_wave of the vectors of each: its query heads, its key heads, its value heads.
+template <bool ROPE, bool STREAM>
 __global__ void __launch_bounds__(256)
-qk_norm_rope_fp4_kernel(NormRopeFp4Args a) {
-  const int hkv = a.w.num_kv_heads;
-  const int vecs = a.num_heads + 2 * hkv;
-  const int64_t gv = (int64_t)blockIdx.x * 32 + (threadIdx.x >> 3);
-  if (gv >= (int64_t)a.w.num_tokens * vecs) return;
-  const int t = (int)(gv / vecs);
-  const int vec = (int)(gv % vecs);
-  const int c = threadIdx.x & 7;
-  int64_t slot = a.w.slots[t];
-  if (slot >= a.w.num_slots || slot < -1) {
-    if (vec == 0 && c == 0) flag_index_error(a.w.err, NVAMD_ERR_SLOT);
+rows_fp4_kernel(NormRopeFp4Args a) {
+  __shared__ __attribute__((aligned(16))) u8 s_tile[4][2][512];
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int c = lane & 7, tok = lane >> 3;
+  const int hkv = a.w.num_kv_heads, hq = ROPE ? a.num_heads : 0;
+  const int h_begin = (blockIdx.y * 4 + w) * a.w.heads_per_wave;
+  const int h_end = min(h_begin + a.w.heads_per_wave, hq + 2 * hkv);
+  if (h_begin >= h_end) return;
+  const int t = blockIdx.x * 8 + tok;
+  const bool exists = t < a.w.num_tokens;
+  int64_t slot = exists ? a.w.slots[t] : -1;
+  if (slot >= a.w.num_slots || slot < -1) {  // skip the row, report it once per token
+    if (h_begin == 0 && c == 0) flag_index_error(a.w.err, NVAMD_ERR_SLOT);
     slot = -1;
   }
-  if (vec >= a.num_heads + hkv) {
-    if (slot < 0) return;
-    const int h = vec - a.num_heads - hkv;
-    const u16 *src = a.w.v + t * a.w.v_stride + h * kHeadDim + 8 * c;
-    store_value(a.w.cache, row_at(slot, h, hkv, a.w.bs_log2), c, ld16(src), ld16(src + 64));
-    return;
+  const bool run = __all(slot >= 0 && slot == uniform64(slot) + tok);
+
+  float cs[8], sn[8];
+  u32x4 qw_lo, qw_hi, kw_lo, kw_hi;
+  if constexpr (ROPE) {
+    if (h_begin < hq + hkv) {
+      int64_t pos = exists ? a.positions[t] : 0;
+      if (pos < 0 || pos >= a.max_positions) {  // clamp and report
+        if (h_begin == 0 && c == 0) flag_index_error(a.w.err, NVAMD_ERR_POSITION);
+        pos = pos < 0 ? 0 : a.max_positions - 1;
+      }
+      const float *row = a.cos_sin + pos * kHeadDim + 8 * c;
+      const f32x4 c0 = *reinterpret_cast<const f32x4 *>(row), c1 = *reinterpret_cast<const f32x4 *>(row + 4);
+      const f32x4 s0 = *reinterpret_cast<const f32x4 *>(row + 64), s1 = *reinterpret_cast<const f32x4 *>(row + 68);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        cs[e] = e < 4 ? c0[e & 3] : c1[e & 3];
+        sn[e] = e < 4 ? s0[e & 3] : s1[e & 3];
+      }
+      qw_lo = ld16(a.q_w + 8 * c);
+      qw_hi = ld16(a.q_w + 64 + 8 * c);
+      kw_lo = ld16(a.k_w + 8 * c);
+      kw_hi = ld16(a.k_w + 64 + 8 * c);
+    }
   }
-  const bool is_q = vec < a.num_heads;
-  const int h = is_q ? vec : vec - a.num_heads;
-  if (!is_q && slot < 0 && a.k_out == nullptr) return;
-  const u16 *src = (is_q ? a.q + t * a.q_stride : a.w.k + t * a.w.k_stride) + h * kHeadDim + 8 * c;
-  const u16 *wt = (is_q ? a.q_w : a.k_w) + 8 * c;
-  u32x4 lo = ld16(src), hi = ld16(src + 64);
-  const u32x4 w_lo = ld16(wt), w_hi = ld16(wt + 64);
-  int64_t pos = a.positions[t];
-  if (pos < 0 || pos >= a.max_positions) {
-    if (vec == 0 && c == 0) flag_index_error(a.w.err, NVAMD_ERR_POSITION);
-    pos = pos < 0 ? 0 : a.max_positions - 1;
+  const int64_t tt = exists ? t : 0;  // lanes without a token read the first one's rows and write nothing
+  auto source = [&](int v) {
+    const u16 *p = v < hq ? a.q + tt * a.q_stride + v * kHeadDim
+                 : v < hq + hkv ? a.w.k + tt * a.w.k_stride + (v - hq) * kHeadDim
+                                : a.w.v + tt * a.w.v_stride + (v - hq - hkv) * kHeadDim;
+    return p + 8 * c;
+  };
+  const u16 *src = source(h_begin);
+  u32x4 next_lo = get16<STREAM>(src), next_hi = get16<STREAM>(src + 64);
+#pragma unroll 1
+  for (int v = h_begin; v < h_end; ++v) {
+    u32x4 lo = next_lo, hi = next_hi;
+    if (v + 1 < h_end) {  // the next head's row is on its way during this one's work
+      src = source(v + 1);
+      next_lo = get16<STREAM>(src);
+      next_hi = get16<STREAM>(src + 64);
+    }
+    if (v >= hq + hkv) {
+      const int h = v - hq - hkv;
+      u8 *tile = s_tile[w][v & 1];  // the other one's reads are done: they have left as stores
+      const Fp4Row r = row_at(slot < 0 ? 0 : slot, h, hkv, a.w.bs_log2);
+      value_bytes(a.w.cache, r, slot >= 0, c, tok, lo, hi, tile);
+      wave_lds_fence();
+      store_values(a.w.cache, tile, slot, run, h, hkv, a.w.bs_log2, lane);
+      continue;
+    }
+    const bool is_q = v < hq;
+    if constexpr (ROPE) {
+      // Keeps the conversions of the row's 16 numbers and of the weights inside the loop: hoisted, they would hold 64 registers
+      // and with them a third of the waves.
+#pragma unroll
+      for (int e = 0; e < 8; ++e) asm volatile("" : "+v"(cs[e]), "+v"(sn[e]));
+      asm volatile("" : "+v"(qw_lo), "+v"(qw_hi), "+v"(kw_lo), "+v"(kw_hi));
+      norm_rope_f64(lo, hi, is_q ? qw_lo : kw_lo, is_q ? qw_hi : kw_hi, cs, sn, (double)a.eps);
+      u16 *dst = is_q ? a.q_out + tt * a.q_out_stride + v * kHeadDim
+                      : a.k_out ? a.k_out + tt * a.k_out_stride + (v - hq) * kHeadDim : nullptr;
+      if (dst != nullptr && exists) {
+        st16(dst + 8 * c, lo);
+        st16(dst + 8 * c + 64, hi);
+      }
+    }
+    if (!is_q && slot >= 0) store_key(a.w.cache, row_at(slot, v - hq, hkv, a.w.bs_log2), c, lo, hi);
   }
-  norm_rope_f64(lo, hi, w_lo, w_hi, a.cos_sin + pos * kHeadDim, c, a.eps);
-  u16 *dst = is_q ? a.q_out + t * a.q_out_stride : a.k_out ? a.k_out + t * a.k_out_stride : nullptr;
-  if (dst != nullptr) {
-    st16(dst + h * kHeadDim + 8 * c, lo);
-    st16(dst + h * kHeadDim + 8 * c + 64, hi);
-  }
-  if (!is_q && slot >= 0) store_key(a.w.cache, row_at(slot, h, hkv, a.w.bs_log2), c, lo, hi);
+}
+
+// A workgroup is 8 tokens x 4 waves' heads.  A wave takes up to 8 heads; fewer where that leaves too few waves to fill the card.
+int heads_per_wave(int num_tokens, int vecs, dim3 *grid) {
+  const int64_t octets = ((int64_t)num_tokens + 7) / 8;
+  int per_wave = 8;
+  while (per_wave > 1 && octets * ceil_div(vecs, per_wave) < kWantedWaves) per_wave >>= 1;
+  *grid = dim3((unsigned)octets, (unsigned)ceil_div(ceil_div(vecs, per_wave), 4));
+  return per_wave;
+}
+
+bool streams(int num_tokens, int num_kv_heads) { return (int64_t)num_tokens * num_kv_heads * kHeadDim >= kStreamElems; }
+
+template <bool ROPE>
+int launch_rows(NormRopeFp4Args &a, hipStream_t stream) {
+  dim3 grid;
+  a.w.heads_per_wave = heads_per_wave(a.w.num_tokens, (ROPE ? a.num_heads : 0) + 2 * a.w.num_kv_heads, &grid);
+  if (grid.y > 65535) return NVAMD_EUNSUPPORTED;
+  // (the rotation measured the same either way)
+  if (!ROPE && streams(a.w.num_tokens, a.w.num_kv_heads))
+    hipLaunchKernelGGL((rows_fp4_kernel<ROPE, !ROPE>), grid, dim3(256), 0, stream, a);
+  else
+    hipLaunchKernelGGL((rows_fp4_kernel<ROPE, false>), grid, dim3(256), 0, stream, a);
+  return launch_status();
 }
 
 bool rows_ok(const void *p, int64_t stride, int heads) {
   return p && aligned16(p) && stride % 8 == 0 && stride >= (int64_t)heads * kHeadDim;
-}
-
-int vector_blocks(int64_t vectors, unsigned *blocks) {
-  const int64_t n = (vectors + 31) / 32;
-  if (n > 0x7fffffff) return NVAMD_EINVAL;
-  *blocks = (unsigned)n;
-  return NVAMD_OK;
 }
 
 // Checks shared by the entry points; fills what they share.
@@ -338,10 +491,9 @@ extern "C" int nvamd_kv_cache_write_fp4(const void *k, int64_t k_stride, const v
   const int st = fill_write_args(w, k, k_stride, v, v_stride, k_codes, k_scales, v_codes, v_scales, slot_mapping,
                                  num_tokens, num_kv_heads, head_dim, num_blocks, block_size);
   if (st != NVAMD_OK) return st;
-  unsigned blocks;
-  if (vector_blocks((int64_t)num_tokens * 2 * num_kv_heads, &blocks) != NVAMD_OK) return NVAMD_EINVAL;
-  hipLaunchKernelGGL(kv_write_fp4_kernel, dim3(blocks), dim3(256), 0, stream, w);
-  return launch_status();
+  NormRopeFp4Args a = {};
+  a.w = w;
+  return launch_rows<false>(a, stream);
 }
 
 extern "C" int nvamd_kv_cache_read_fp4(void *k, int64_t k_stride, void *v, int64_t v_stride, const void *k_codes,
@@ -354,11 +506,15 @@ extern "C" int nvamd_kv_cache_read_fp4(void *k, int64_t k_stride, void *v, int64
                                  const_cast<void *>(v_codes), const_cast<void *>(v_scales), slot_mapping, num_tokens,
                                  num_kv_heads, head_dim, num_blocks, block_size);
   if (st != NVAMD_OK) return st;
-  unsigned blocks;
-  if (vector_blocks((int64_t)num_tokens * 2 * num_kv_heads, &blocks) != NVAMD_OK) return NVAMD_EINVAL;
+  dim3 grid;
+  const int per_wave = heads_per_wave(num_tokens, 2 * num_kv_heads, &grid);
+  if (grid.y > 65535) return NVAMD_EUNSUPPORTED;
   ReadArgs a{static_cast<u16 *>(k), k_stride, static_cast<u16 *>(v), v_stride, w.cache, w.slots, w.num_slots,
-             num_tokens, num_kv_heads, w.bs_log2, w.err};
-  hipLaunchKernelGGL(kv_read_fp4_kernel, dim3(blocks), dim3(256), 0, stream, a);
+             num_tokens, num_kv_heads, w.bs_log2, per_wave, w.err};
+  if (streams(num_tokens, num_kv_heads))
+    hipLaunchKernelGGL((kv_read_fp4_kernel<true>), grid, dim3(256), 0, stream, a);
+  else
+    hipLaunchKernelGGL((kv_read_fp4_kernel<false>), grid, dim3(256), 0, stream, a);
   return launch_status();
 }
 
@@ -391,8 +547,5 @@ extern "C" int nvamd_qk_norm_rope_fp4(void *q_out, int64_t q_out_stride, void *k
   a.max_positions = max_positions;
   a.num_heads = num_heads;
   a.eps = eps;
-  unsigned blocks;
-  if (vector_blocks((int64_t)num_tokens * (num_heads + 2 * num_kv_heads), &blocks) != NVAMD_OK) return NVAMD_EINVAL;
-  hipLaunchKernelGGL(qk_norm_rope_fp4_kernel, dim3(blocks), dim3(256), 0, stream, a);
-  return launch_status();
+  return launch_rows<true>(a, stream);
 }

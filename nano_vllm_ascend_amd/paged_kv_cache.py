@@ -80,7 +80,7 @@ class Fp4PagedKVCache:
         return 2 * num_layers * block_size * num_kv_heads * (head_dim // 2 + head_dim // 32)
 
     def _slots(self, slot_mapping: torch.Tensor) -> torch.Tensor:
-        return slot_mapping.to(device=self.key_codes.device, dtype=torch.int64).contiguous()
+        return slot_mapping.to(device=self.key_codes.device, dtype=torch.int64).reshape(-1).contiguous()
 
     def write(self, layer_idx: int, key_states: torch.Tensor, value_states: torch.Tensor,
               slot_mapping: torch.Tensor) -> None:
