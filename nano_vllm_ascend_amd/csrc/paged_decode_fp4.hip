@@ -11,7 +11,7 @@
 // A wave takes 64 tokens at a time, four 16-token tiles, one per 16 lanes (gq = lane / 16):
 //   S^T = K . Q^T  v_mfma_scale_f32_16x16x128_f8f6f4 on the codes as they lie in the cache, A = 16 rows of K: a lane's 16
 //        bytes are one block of a row, under one scale.  B = the heads as 16 columns, in 8 bits twice: a bf16 query is the sum
-//        of two e4m3 numbers under a common scale (split_query), so two products give the scores.  That takes the matrix
+//        of two e4m3 numbers under a common scale (QueryScale), so two products give the scores.  That takes the matrix
 //        cores as long as four bf16 products, and the vector ALUs no expansion of K.
 //        Row 4a + i of product t is token 4t + i of tile a: lane (h, gq) then finds the scores of tile gq's tokens
 //        4t .. 4t+3 of head h in its accumulator of product t, that is of all 16 tokens in the four products;
@@ -22,7 +22,7 @@
 //        what the lane holds.  The cache keeps V with 16 tokens of a dim pair in consecutive bytes, so the lane's
 //        16 bytes give both products' operands of two dims: no lane movement.
 // The score of a token past the context is replaced by -inf and the scales of its values by zero, whatever bytes it holds.
-#include "fp4.h"
+#include "fp4_attention.h"
 
 namespace nvamd {
 namespace {
@@ -36,8 +36,6 @@ constexpr int kHalvesLog2 = 4, kHalves = 2 * kWaves;  // half-waves of a workgro
 static_assert(kHalves == 1 << kHalvesLog2);
 constexpr int kMinPart = 64 * kWaves;  // tokens of the smallest partition: one step of each wave
 constexpr int kCus = 256;
-constexpr float kNoScore = -1e30f;   // reference of an empty softmax: finite, so that it needs no guard in exponents
-constexpr float kRescaleLog2 = 8.f;  // the reference moves when a score exceeds it by 2^8
 constexpr int kMaxHeads = 16;  // query heads of a kv head in one launch: the MFMA's columns
 
 struct DecodeFp4Args {
@@ -66,13 +64,6 @@ struct DecodeFp4Args {
   u32 *err;
 };
 
-__device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
-
-__device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c) {
-  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8v, a), __builtin_bit_cast(bf16x8v, b), c, 0,
-                                                 0, 0);
-}
-
 // Inclusive prefix sum over a wave (see paged_decode.hip).
 __device__ __forceinline__ int wave_scan(int v, int lane) {
   v += __builtin_amdgcn_mov_dpp(v, 0x111, 0xF, 0xF, true);
@@ -84,104 +75,6 @@ __device__ __forceinline__ int wave_scan(int v, int lane) {
   const int row = lane >> 4;
   return v + (row >= 1 ? r0 : 0) + (row >= 2 ? r1 : 0) + (row >= 3 ? r2 : 0);
 }
-
-// max / sum over lanes l, l ^ 16, l ^ 32, l ^ 48
-__device__ __forceinline__ float max_over_quarters(float v) {
-  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  return max_xor32(fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])));
-}
-__device__ __forceinline__ float sum_over_quarters(float v) {
-  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  return sum_xor32(__uint_as_float(r[0]) + __uint_as_float(r[1]));
-}
-
-typedef int i32x8 __attribute__((ext_vector_type(8)));
-
-// S += K . q for 16 rows of codes (128 dims, a lane's block and its scale byte) and 16 columns of e4m3 under the scale
-// byte of a column.  Lane (row or column n, gq) gives block gq of its row; of its column, dims 16 gq .. +15 and 64 + 16 gq ..
-// +15 (checked on gfx950).
-__device__ __forceinline__ f32x4 mfma_fp4_fp8(u32x4 k, u32 k_scale, i32x8 q, u32 q_scale, f32x4 c) {
-  const i32x8 codes = {(int)k[0], (int)k[1], (int)k[2], (int)k[3], 0, 0, 0, 0};
-  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(codes, q, c, 4, 0, 0, (int)k_scale, 0, (int)q_scale);
-}
-
-// 32 bf16 values of a query row (16 lanes apart: 4 lanes hold the row) as hi + lo in e4m3 under 2^-s, s from the row's
-// largest value, which lands in [128, 256).  hi keeps 4 of the 8 significant bits and lo the rest: the sum is the value
-// itself down to 2^-10 of the largest one and off by at most 2^-17 of that below.  Returns the scale byte; 255, which makes
-// every score NaN, for a row with an infinity or a NaN.
-__device__ __forceinline__ u32 split_query(const u32x4 (&x)[4], i32x8 &hi, i32x8 &lo) {
-  u32 top = 0;
-#pragma unroll
-  for (int j = 0; j < 4; ++j)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const u32 w = x[j][e];
-      top = max(top, max(w & 0x7fffu, (w >> 16) & 0x7fffu));
-    }
-  top = (u32)max_over_quarters((float)top);  // 15 bits: exact
-  const int e = min(max((int)(top >> 7), 20), 254);  // biased exponent of the row's largest value
-  const float up = __uint_as_float((u32)(127 + 134 - e) << 23);  // 2^(7 - (e - 127))
-#pragma unroll
-  for (int j = 0; j < 4; ++j)
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {  // 4 values to a word
-      const u32 w0 = x[j][2 * i], w1 = x[j][2 * i + 1];
-      const float a = bf16_lo(w0) * up, b = bf16_hi(w0) * up, c = bf16_lo(w1) * up, d = bf16_hi(w1) * up;
-      int h = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
-      h = __builtin_amdgcn_cvt_pk_fp8_f32(c, d, h, true);
-      int r = __builtin_amdgcn_cvt_pk_fp8_f32(a - __builtin_amdgcn_cvt_f32_fp8(h, 0),
-                                              b - __builtin_amdgcn_cvt_f32_fp8(h, 1), 0, false);
-      r = __builtin_amdgcn_cvt_pk_fp8_f32(c - __builtin_amdgcn_cvt_f32_fp8(h, 2),
-                                          d - __builtin_amdgcn_cvt_f32_fp8(h, 3), r, true);
-      hi[2 * j + i] = h;
-      lo[2 * j + i] = r;
-    }
-  return top >= 0x7f80u ? 255u : (u32)(e - 7);
-}
-
-// Byte B of a word of scales as a float scale: one instruction (the compiler takes two for bytes 0..2).
-template <int B>
-__device__ __forceinline__ float scale_of(u32 word) {
-  float r;
-  if constexpr (B == 0)
-    asm("v_lshlrev_b32_sdwa %0, %1, %2 dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:DWORD src1_sel:BYTE_0" : "=v"(r) : "v"(23), "v"(word));
-  else if constexpr (B == 1)
-    asm("v_lshlrev_b32_sdwa %0, %1, %2 dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:DWORD src1_sel:BYTE_1" : "=v"(r) : "v"(23), "v"(word));
-  else if constexpr (B == 2)
-    asm("v_lshlrev_b32_sdwa %0, %1, %2 dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:DWORD src1_sel:BYTE_2" : "=v"(r) : "v"(23), "v"(word));
-  else
-    asm("v_lshlrev_b32_sdwa %0, %1, %2 dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:DWORD src1_sel:BYTE_3" : "=v"(r) : "v"(23), "v"(word));
-  return r;
-}
-
-// Lanes of the banks in MASK (4 lanes each, of 16) take src moved by the DPP control, the others keep `old`.
-template <int CTRL, int MASK>
-__device__ __forceinline__ float dpp_into(float old, float src) {
-  return __uint_as_float((u32)__builtin_amdgcn_update_dpp((int)__float_as_uint(old), (int)__float_as_uint(src), CTRL, 0xF,
-                                                          MASK, false));
-}
-template <int CTRL>
-__device__ __forceinline__ u32 dpp_u32(u32 v) {
-  return (u32)__builtin_amdgcn_mov_dpp((int)v, CTRL, 0xF, 0xF, true);
-}
-constexpr int kRowShl4 = 0x104, kRowShl8 = 0x108, kRowShl12 = 0x10C;  // lane n <- lane n + 4, 8, 12 of its 16
-constexpr int kRowShr4 = 0x114, kRowShr8 = 0x118, kRowShr12 = 0x11C;  // lane n <- lane n - 4, 8, 12
-constexpr int kRowRor4 = 0x124;
-constexpr int kRowBcast = 0x150;  // + n: every lane <- lane n of its 16
-
-// Codes are read once: past the caches' normal keeping.
-__device__ __forceinline__ u32x4 load16(const u8 *p) {
-  return __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(p));
-}
-
-// Keeps the first n bytes (any n) of a word.
-__device__ __forceinline__ u32 keep_bytes(u32 v, int n) {
-  return n >= 4 ? v : n <= 0 ? 0u : v & ((1u << (8 * n)) - 1u);
-}
-template <int N>
-struct Int {
-  static constexpr int value = N;
-};
 
 // Cutting units of `tokens` tokens in all every `length` tokens ends in tokens / length + units / 2 partitions on average,
 // and in a whole unit more than the quotient each at most.  The length is chosen for this quotient (share):
@@ -269,7 +162,12 @@ paged_decode_fp4_kernel(DecodeFp4Args a) {
   {
     const u16 *qp = a.q + (int64_t)b * a.q_stride + (int64_t)(head0 + min(n, G - 1)) * D + 16 * gq;
     const u32x4 x[4] = {ld16(qp), ld16(qp + 8), ld16(qp + 64), ld16(qp + 72)};
-    q_scale = split_query(x, q_hi, q_lo);
+    u32 top = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) top = max(top, largest(x[j]));
+    const QueryScale scale = query_scale((u32)max_over_quarters((float)top));  // 15 bits: exact
+    split32(x, scale.up, q_hi, q_lo);
+    q_scale = scale.byte;
   }
 
   // The exponent's reference, the threshold above which it moves; the sum and the numerators at that reference.
@@ -406,7 +304,7 @@ paged_decode_fp4_kernel(DecodeFp4Args a) {
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const u32 pr = pack_bf16x2(fast_exp2(s[x][2 * i] - m), fast_exp2(s[x][2 * i + 1] - m));
-        l = dot2_bf16(pr, 0x3F803F80u, l);
+        l = dot2_bf16(pr, kBf16PairOne, l);
         pf[x >> 1][2 * (x & 1) + i] = pr;
         if constexpr (NP == 1) {
           pf[0][2 + i] = dpp_u32<kRowShl4>(pr);
@@ -416,31 +314,10 @@ paged_decode_fp4_kernel(DecodeFp4Args a) {
           pf[1][2 * x + i] = dpp_u32<kRowShl8>(pr);
         }
       }
-    auto products = [&](auto qq) {
-      constexpr int q = decltype(qq)::value;
-      const u32 sc[4] = {dpp_u32<kRowBcast + 4 * q>(vs), dpp_u32<kRowBcast + 4 * q + 1>(vs),
-                         dpp_u32<kRowBcast + 4 * q + 2>(vs), dpp_u32<kRowBcast + 4 * q + 3>(vs)};
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        u32x4 lo, hi;
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          const u32 c = vc[q][2 * h + x], w = sc[2 * h + x];
-          const u32 v0 = fp4_pair<0>(c, scale_of<0>(w)), v1 = fp4_pair<1>(c, scale_of<1>(w));
-          const u32 v2 = fp4_pair<2>(c, scale_of<2>(w)), v3 = fp4_pair<3>(c, scale_of<3>(w));
-          lo[2 * x] = pair_lo(v0, v1);
-          lo[2 * x + 1] = pair_lo(v2, v3);
-          hi[2 * x] = pair_hi(v0, v1);
-          hi[2 * x + 1] = pair_hi(v2, v3);
-        }
-        o[2 * q] = mfma16(lo, pf[h], o[2 * q]);
-        o[2 * q + 1] = mfma16(hi, pf[h], o[2 * q + 1]);
-      }
-    };
-    products(Int<0>{});
-    products(Int<1>{});
-    products(Int<2>{});
-    products(Int<3>{});
+    add_values<0>(o, vc, vs, pf);
+    add_values<1>(o, vc, vs, pf);
+    add_values<2>(o, vc, vs, pf);
+    add_values<3>(o, vc, vs, pf);
     __builtin_amdgcn_sched_barrier(0);
     if (next < t_end) load_v();
   };

@@ -1,31 +1,30 @@
 // Causal prefill attention over the 4-bit paged KV cache (the counterpart of prefill.hip's paged route): the queries are
 // the last q_len positions of a context of kv_len, query row r sees keys 0 .. kv_len - q_len + r, all of them in the cache.
 //
-// Workgroup = 4 waves = one kv head, 1, 2 or 4 of its query heads, and 128 / heads query tokens; wave w owns 32 query rows of
-// one head.  Per tile of 32 keys the workgroup expands K and V from 4 bits to bf16 once, into LDS, in the order in
-// which the MFMA operands are read (every operand read is 64 lanes x 16 consecutive bytes: no bank conflicts, no
-// swizzle), while the codes of the tile after the next are on their way into registers:
-//   waves 0, 1: thread (quarter, row) expands 16 bytes of codes, one block of a K row under one scale, to four chunks of
-//        8 dims;
-//   waves 2, 3: thread (dim pair) of a 16-token tile expands 16 bytes, the tile's tokens of two dims, each under its token's
-//        scale, and pairs tokens: four chunks of 8 keys of a dim.
-// Then, as in prefill.hip:
-//   S^T[32 keys x 32 queries] = K . Q^T        v_mfma_f32_32x32x16_bf16, Q in registers throughout;
-//   O^T[128 dims x 32 queries] += V^T . P^T    with the k-slots in the order in which the S^T accumulator holds its rows,
-//        so that P^T is a repack in registers.
+// The G query heads of a kv head and the q_len tokens make q_len * G rows, R = token * G + head, that share the keys; a
+// workgroup takes rows that follow one another, whatever G is.  Two kernels:
+//
+// Tiles (many rows).  Workgroup = 4 waves = 128 rows, a wave 32 of them; per tile of 32 keys
+//   S^T[32 keys x 32 rows] = K . Q^T   v_mfma_scale_f32_32x32x64_f8f6f4 on the codes as they lie in the cache: a lane loads 32
+//        dims of a key and their scale straight into the operand, and the row comes as two e4m3 numbers per value
+//        (fp4_attention.h).  No expansion of K, and none of it in LDS, whose bandwidth V alone takes half of;
+//   O^T[128 dims x 32 rows] += V^T . P^T   v_mfma_f32_32x32x16_bf16.  The workgroup expands a tile of V once, to bf16 operands
+//        in LDS (every access is 64 lanes x 16 consecutive bytes): a wave takes 8 tokens of a 16-token tile, a lane a dim
+//        pair of them.  The accumulator of S^T holds its rows in the order 8 (i / 4) + 4 half + i % 4, so key 16a + 8b + 4c + x sits in
+//        row 16a + 8c + 4b + x of K: then a lane's registers are 8 consecutive keys, and P^T a repack in registers.
+//   K of the next tile loads as the scores have taken this one's, V's codes are two tiles ahead, V's operands one (two stages, one
+//   barrier a tile).
+//
+// Few rows (a chat's next turn: nothing else would fill the card).  Workgroup = 8 waves = 16 rows, a wave every eighth 64 keys,
+// as in paged_decode_fp4.hip with rows in the place of heads and a last key for each row; the waves' results meet in LDS.
+//
 // A block of values that reads as NaN must reach the rows that see its key and no others, though masked rows
 // multiply it by a weight of zero: such values enter the products as zeros, and the rows that see
-// the key get the NaN added afterwards (a branch that no other tile takes).
-#include "fp4.h"
+// the key get the NaN afterwards (a branch that no other tile takes).
+#include "fp4_attention.h"
 
 namespace nvamd {
 namespace {
-
-constexpr int kBK = 32;               // keys per tile
-constexpr float kRescaleLog2 = 8.f;   // lazy-rescale threshold (log2 units)
-constexpr u32 kBf16PairOne = 0x3F803F80u;
-constexpr int kWaves = 4;
-constexpr int kThreads = kWaves * 64;
 
 struct PrefillFp4Args {
   u16 *out;
@@ -41,243 +40,299 @@ struct PrefillFp4Args {
   int num_blocks;
   int bs_log2;
   int num_kv_heads;
-  int max_q_tiles;
+  int group;  // query heads of a kv head
+  int max_tiles;
   int max_q_len;
   int num_tokens;
   float scale_log2e;
-  int q_group;  // query heads of kv head g: q_group * g + q_head0 + (0 .. GQA-1)
-  int q_head0;
   u32 *err;
 };
 
-__device__ __forceinline__ f32x16 mfma32(bf16x8v a, bf16x8v b, f32x16 c) {
-  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
-}
-
-template <int B>
-__device__ __forceinline__ float scale_of(u32 word) {
-  return __uint_as_float(((word >> (8 * B)) & 0xffu) << 23);
-}
-
-// One stage: the operands of a tile, each 64 lanes x 16 bytes, and a bit per (block, token) whose values read as NaN.
-struct Stage {
-  u32x4 k[8][64];     // [16-dim step][lane]
-  u32x4 v[2][4][64];  // [16-key step][32-dim block][lane]
-  u16 nan[2][4];      // [16-key step][32-dim block]: bit per token
+// A workgroup's sequence and rows.
+struct Rows {
+  int q_start;
+  int rows;    // q_len * group
+  int kv_len;
+  int offset;  // token t sees keys 0 .. offset + t
+  int first;   // the workgroup's first row
 };
-
-template <int GQA>
-__global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2)))
-prefill_fp4_kernel(PrefillFp4Args a) {
-  constexpr int D = kHeadDim;
-  constexpr int BQ = 32 * kWaves / GQA;  // query tokens per workgroup
-  constexpr int WPH = kWaves / GQA;      // waves per query head
-  __shared__ __attribute__((aligned(16))) Stage s_stage[2];
-
-  const int g = blockIdx.x;
-  const int qt = a.max_q_tiles - 1 - (int)blockIdx.y;
+// False if it has none.  Faults are reported once per sequence.
+__device__ __forceinline__ bool find_rows(const PrefillFp4Args &a, int per_group, Rows &r) {
   const int s = blockIdx.z;
-  const int q_start = a.cu_seqlens_q[s];
+  r.q_start = a.cu_seqlens_q[s];
   const int q_end = a.cu_seqlens_q[s + 1];
-  const int q_len = q_end - q_start;
+  const int q_len = q_end - r.q_start;
   const int cap = a.bt_width << a.bs_log2;
-  int kv_len = a.kv_lens[s];
-  const bool rows_in = q_start >= 0 && q_len >= 0 && q_end <= a.num_tokens;  // else no row is touched
-  if ((!rows_in || q_len > a.max_q_len || kv_len > cap || kv_len < q_len) && g == 0 && blockIdx.y == 0 &&
+  const int kv_len = a.kv_lens[s];
+  const bool rows_in = r.q_start >= 0 && q_len >= 0 && q_end <= a.num_tokens;  // else no row is touched
+  if ((!rows_in || q_len > a.max_q_len || kv_len > cap || kv_len < q_len) && blockIdx.x == 0 && blockIdx.y == 0 &&
       threadIdx.x == 0)
     flag_index_error(a.err, NVAMD_ERR_CONTEXT);
-  if (!rows_in || qt * BQ >= q_len) return;
-  kv_len = min(kv_len, cap);
-  const int offset = kv_len - q_len;  // query row r sees keys 0..offset+r
+  r.rows = q_len * a.group;
+  r.first = (a.max_tiles - 1 - (int)blockIdx.y) * per_group;  // the most keys first
+  r.kv_len = min(kv_len, cap);
+  r.offset = r.kv_len - q_len;
+  return rows_in && r.first < r.rows;
+}
 
-  const int tid = threadIdx.x;
-  const int lane = tid & 63;
-  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int hl = lane >> 5;
-  const int n = lane & 31;  // this lane's query column
-  const int head = g * a.q_group + a.q_head0 + w / WPH;
-  const int r0 = qt * BQ + (w % WPH) * 32;  // first query row of this wave
-  const int rq = r0 + n;
+__device__ __forceinline__ int tile_of(const PrefillFp4Args &a, int entry, int token, int g, bool report) {
+  if ((unsigned)entry >= (unsigned)a.num_blocks && report) flag_index_error(a.err, NVAMD_ERR_BLOCK);
+  entry = min(max(entry, 0), a.num_blocks - 1);  // never leave the pool
+  return (int)fp4_tile(entry, token & ((1 << a.bs_log2) - 1), g, a.num_kv_heads, a.bs_log2);
+}
 
-  bf16x8v qf[8];  // dims 16 kk + 8 hl .. +7 of the lane's query row
+// 0x80 in the bytes that are 255: only there do the low seven bits carry into a set top bit.
+__device__ __forceinline__ u32 nan_bytes(u32 scales) {
+  return ((scales & 0x7f7f7f7fu) + 0x01010101u) & scales & 0x80808080u;
+}
+__device__ __forceinline__ u32 without(u32 scales, u32 nans) { return scales & ~((nans >> 7) * 0xffu); }
+
+// ------------------------------------------------------------------------------------------ tiles
+constexpr int kBK = 32;  // keys per tile
+constexpr int kWaves = 4;
+constexpr int kTileRows = 32 * kWaves;
+
+__device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8v, a), __builtin_bit_cast(bf16x8v, b), c, 0,
+                                                 0, 0);
+}
+// 64 dims: lane (n, half) gives block `half` of them of row n; of column n, dims 16 half .. +15 and 32 + 16 half .. +15.
+__device__ __forceinline__ f32x16 mfma32_fp4_fp8(u32x4 k, u32 k_scale, i32x8 q, u32 q_scale, f32x16 c) {
+  const i32x8 codes = {(int)k[0], (int)k[1], (int)k[2], (int)k[3], 0, 0, 0, 0};
+  return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(codes, q, c, 4, 0, 0, (int)k_scale, 0, (int)q_scale);
+}
+
+struct Stage {
+  u32x4 v[2][4][64];  // [16-key step][32-dim block][lane]
+  u32 nan[4][2];      // [wave that expanded them][..]: a bit per (block, token) whose values read as NaN, 8 tokens a byte
+};
+constexpr int kRowPad = kHeadDim + 8;  // elements of a row in the output's turn: 16 bytes of padding spread the banks
+
+__global__ void __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(3)))
+prefill_fp4_kernel(PrefillFp4Args a) {
+  constexpr int D = kHeadDim;
+  constexpr size_t kTurn = (size_t)kWaves * 16 * kRowPad * sizeof(u16);
+  __shared__ __attribute__((aligned(16))) u8 s_mem[2 * sizeof(Stage) > kTurn ? 2 * sizeof(Stage) : kTurn];
+  Stage *stages = reinterpret_cast<Stage *>(s_mem);
+
+  Rows rows;
+  if (!find_rows(a, kTileRows, rows)) return;
+  const int g = blockIdx.x;
+  const int lane = threadIdx.x & 63;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int half = lane >> 5, n = lane & 31;
+  const int kv_len = rows.kv_len;
+  const int r0 = rows.first + 32 * w;  // the wave's first row
+  int row = min(r0 + n, rows.rows - 1);
+  const int last_seen = min(rows.offset + row / a.group, kv_len - 1);  // by this lane's row
+  const int wave_first = rows.offset + r0 / a.group;           // the last key that the wave's first row sees
+  const int wave_last = rows.offset + min(r0 + 31, rows.rows - 1) / a.group;
+  const int end_row = min(rows.first + kTileRows, rows.rows) - 1;
+  const int keys = min(kv_len, rows.offset + end_row / a.group + 1);  // that the workgroup needs
+  const int n_tiles = keys > 0 ? ceil_div(keys, kBK) : 0;
+
+  i32x8 q_hi[2], q_lo[2];
+  u32 q_scale;
   {
-    const u16 *qp = a.q + (int64_t)(q_start + min(rq, q_len - 1)) * a.q_stride + (int64_t)head * D + 8 * hl;
+    const int token = row / a.group, head = g * a.group + row - token * a.group;
+    const u16 *qp = a.q + (int64_t)(rows.q_start + token) * a.q_stride + (int64_t)head * D + 16 * half;
+    u32x4 x[2][4];
+    u32 top = 0;
 #pragma unroll
-    for (int kk = 0; kk < 8; ++kk) qf[kk] = __builtin_bit_cast(bf16x8v, ld16(qp + 16 * kk));
+    for (int s = 0; s < 2; ++s) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        x[s][j] = ld16(qp + 64 * s + 32 * (j >> 1) + 8 * (j & 1));
+        top = max(top, largest(x[s][j]));
+      }
+    }
+    const QueryScale scale = query_scale((u32)max_xor32((float)top));  // 15 bits: exact
+#pragma unroll
+    for (int s = 0; s < 2; ++s) split32(x[s], scale.up, q_hi[s], q_lo[s]);
+    q_scale = scale.byte;
   }
+
   f32x16 acc[4];
 #pragma unroll
   for (int db = 0; db < 4; ++db)
 #pragma unroll
     for (int i = 0; i < 16; ++i) acc[db][i] = 0.f;
-  float m_ref = -1e30f, m_thr = -1e30f, neg_ref = 1e30f, l_run = 0.f;
+  float neg_ref = -kNoScore, l_run = 0.f;  // minus the exponent's reference; the sum at that reference
 
-  // Keys this workgroup needs: up to the last visible key of its last valid row.
-  const int kv_hi = min(kv_len, offset + min((qt + 1) * BQ, q_len));
-  const int n_tiles = kv_hi > 0 ? ceil_div(kv_hi, kBK) : 0;
-  const int wave_last_key = offset + min(r0 + 31, q_len - 1);  // beyond: fully masked for this wave
-
-  const int32_t *bt_row = a.block_tables + (int64_t)s * a.bt_stride;
-  const int bs_mask = (1 << a.bs_log2) - 1;
-  // The 16-token tile of token t0 (the last one of the keys where t0 lies past them).
-  auto tile_at = [&](int t0) {
-    const int t = min(t0, (kv_len - 1) & ~15);
-    const int e = bt_row[t >> a.bs_log2];
-    if ((unsigned)e >= (unsigned)a.num_blocks && lane == 0) flag_index_error(a.err, NVAMD_ERR_BLOCK);
-    return fp4_tile(min(max(e, 0), a.num_blocks - 1), t & bs_mask, g, a.num_kv_heads, a.bs_log2);
+  // The two 16-token tiles of each tile of keys (past the keys: their last one), looked up a tile ahead.
+  typedef const __attribute__((address_space(4))) int32_t const_i32;  // nothing writes the table: scalar loads
+  const_i32 *bt = (const_i32 *)(a.block_tables + (int64_t)blockIdx.z * a.bt_stride);
+  const int last_tile = max(kv_len - 1, 0) & ~15;
+  int entry[2];
+  auto look_up = [&](int t) {
+#pragma unroll
+    for (int x = 0; x < 2; ++x) entry[x] = bt[min(t * kBK + 16 * x, last_tile) >> a.bs_log2];
   };
-
-  // What a thread expands: waves 0 and 1 row n of block 2w + hl of K, waves 2 and 3 the dim pair `lane` of tile w - 2.
-  u32x4 codes, scales;
-  auto fetch = [&](int t) {
-    if (w < 2) {
-      const int64_t t0 = tile_at(t * kBK), t1 = tile_at(t * kBK + 16);
-      const int64_t tile = n < 16 ? t0 : t1;
-      codes = *reinterpret_cast<const u32x4 *>(a.cache.k_codes + tile * kFp4TileBytes + (n & 15) * kFp4RowBytes +
-                                               16 * (2 * w + hl));
-      scales[0] = a.cache.k_scales[tile * kFp4TileScales + fp4_key_scale_at(n & 15, 2 * w + hl)];
-    } else {
-      const int64_t tile = tile_at(t * kBK + 16 * (w - 2));
-      codes = *reinterpret_cast<const u32x4 *>(a.cache.v_codes + tile * kFp4TileBytes + 16 * lane);
-      scales = *reinterpret_cast<const u32x4 *>(a.cache.v_scales + tile * kFp4TileScales + 16 * (lane >> 4));
+  int tile[2];  // of the latest tile that was located
+  auto locate = [&](int t) {
+#pragma unroll
+    for (int x = 0; x < 2; ++x)
+      tile[x] = tile_of(a, entry[x], min(t * kBK + 16 * x, last_tile), g, threadIdx.x == 0);
+  };
+  // K: key 16a + 8b + 4c + x of the tile in row n = 16a + 8c + 4b + x.
+  const int k_token = (n & 3) | ((n & 8) >> 1) | ((n & 4) << 1);  // of its 16-token tile, n / 16
+  u32x4 kc[2];
+  u32 ks[2];
+  auto load_k = [&](int t0, int t1) {
+    const int64_t t = n < 16 ? t0 : t1;
+    const u8 *kp = a.cache.k_codes + t * kFp4TileBytes + k_token * kFp4RowBytes + 16 * half;
+    const u8 *sp = a.cache.k_scales + t * kFp4TileScales + fp4_key_scale_at(k_token, half);
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      kc[s] = *reinterpret_cast<const u32x4 *>(kp + 32 * s);
+      ks[s] = sp[8 * s];
     }
+  };
+  // V: wave w expands tokens 8 (w % 2) .. +7 of 16-token tile w / 2, a lane one pair of dims.
+  u32x2 vc, vs;
+  auto load_v = [&]() {
+    const int64_t t = w < 2 ? tile[0] : tile[1];
+    vc = *reinterpret_cast<const u32x2 *>(a.cache.v_codes + t * kFp4TileBytes + 16 * lane + 8 * (w & 1));
+    vs = *reinterpret_cast<const u32x2 *>(a.cache.v_scales + t * kFp4TileScales + 16 * (lane >> 4) + 8 * (w & 1));
   };
   auto expand = [&](int t, Stage &st) {
-    if (w < 2) {
-      const float scale = fp4_scale(scales[0]);
-      const int q = 2 * w + hl;
+    const u32 bad0 = nan_bytes(vs[0]), bad1 = nan_bytes(vs[1]);
+    u32 seen0 = 0, seen1 = 0;
+    if (__builtin_expect(__builtin_amdgcn_ballot_w64((bad0 | bad1) != 0) != 0, 0)) {
+      vs[0] = without(vs[0], bad0);
+      vs[1] = without(vs[1], bad1);
+      const int left = kv_len - t * kBK - 8 * w;  // of the wave's 8 tokens
+      u32 bits = 0;
 #pragma unroll
-      for (int c = 0; c < 4; ++c) st.k[2 * q + (c >> 1)][32 * (c & 1) + n] = fp4_values(codes[c], scale);
-    } else {
-      // Blocks that read as NaN become zeros, and are noted where their token exists.
-      u32 seen = 0;
-#pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        // 0x80 in the bytes that are 255: only there do the low seven bits carry into a set top bit
-        const u32 bad = ((scales[x] & 0x7f7f7f7fu) + 0x01010101u) & scales[x] & 0x80808080u;
-        if (__builtin_expect(bad != 0, 0)) {
-          scales[x] &= ~((bad >> 7) * 0xffu);
-#pragma unroll
-          for (int b = 0; b < 4; ++b)
-            if ((bad >> (8 * b + 7)) & 1) seen |= 1u << (4 * x + b);
-        }
-      }
-      const int left = kv_len - t * kBK - 16 * (w - 2);
-      if (left < 16) seen &= (1u << max(left, 0)) - 1u;
-      if ((lane & 15) == 0) st.nan[w - 2][lane >> 4] = (u16)seen;
-      u32x4 lo[2], hi[2];  // [k-slot half of the operand] of dims r and r + 16
-#pragma unroll
-      for (int x = 0; x < 4; ++x) {  // word x: tokens 4x .. 4x+3, which half x % 2 of the lanes takes at place x / 2
-        const u32 v0 = fp4_pair<0>(codes[x], scale_of<0>(scales[x])), v1 = fp4_pair<1>(codes[x], scale_of<1>(scales[x]));
-        const u32 v2 = fp4_pair<2>(codes[x], scale_of<2>(scales[x])), v3 = fp4_pair<3>(codes[x], scale_of<3>(scales[x]));
-        lo[x & 1][2 * (x >> 1)] = pair_lo(v0, v1);
-        lo[x & 1][2 * (x >> 1) + 1] = pair_lo(v2, v3);
-        hi[x & 1][2 * (x >> 1)] = pair_hi(v0, v1);
-        hi[x & 1][2 * (x >> 1) + 1] = pair_hi(v2, v3);
-      }
-      u32x4 *dst = st.v[w - 2][lane >> 4];
-      const int r = lane & 15;
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        dst[32 * h + r] = lo[h];
-        dst[32 * h + 16 + r] = hi[h];
-      }
+      for (int i = 0; i < 4; ++i) bits |= ((bad0 >> (8 * i + 7)) & 1) << i | ((bad1 >> (8 * i + 7)) & 1) << (4 + i);
+      bits &= left >= 8 ? 0xffu : (1u << max(left, 0)) - 1u;
+      // blocks 0, 1 and 2, 3 in two words of 16 bits each
+      seen0 = (u32)__builtin_amdgcn_readlane((int)bits, 0) | (u32)__builtin_amdgcn_readlane((int)bits, 16) << 16;
+      seen1 = (u32)__builtin_amdgcn_readlane((int)bits, 32) | (u32)__builtin_amdgcn_readlane((int)bits, 48) << 16;
     }
+    if (lane == 0) *reinterpret_cast<u32x2 *>(st.nan[w]) = u32x2{seen0, seen1};
+    u32x4 lo, hi;
+    {
+      u32 x[8];
+      expand4(vc[0], vs[0], x[0], x[1], x[4], x[5]);
+      expand4(vc[1], vs[1], x[2], x[3], x[6], x[7]);
+      lo = u32x4{x[0], x[1], x[2], x[3]};
+      hi = u32x4{x[4], x[5], x[6], x[7]};
+    }
+    u32x4 *dst = st.v[w >> 1][lane >> 4] + 32 * (w & 1) + (lane & 15);
+    dst[0] = lo;
+    dst[16] = hi;
   };
 
-  auto compute = [&](int t, const Stage &st) {
-    const int base = t * kBK;
-    if (r0 >= q_len || base > wave_last_key) return;
-    f32x16 sc;
+  f32x16 sc;
+  auto score = [&]() {
 #pragma unroll
     for (int i = 0; i < 16; ++i) sc[i] = 0.f;
 #pragma unroll
-    for (int kk = 0; kk < 8; ++kk) sc = mfma32(__builtin_bit_cast(bf16x8v, st.k[kk][lane]), qf[kk], sc);
-    // Key of register i: base + 8(i/4) + 4hl + i%4.
-    const int lim = min(offset + rq, kv_len - 1) - base - 4 * hl;
-    const bool need_mask = (base + kBK - 1 > offset + r0) || (base + kBK > kv_len);
-    if (__builtin_expect(need_mask, 0)) {
+    for (int s = 0; s < 2; ++s) {
+      sc = mfma32_fp4_fp8(kc[s], ks[s], q_hi[s], q_scale, sc);
+      sc = mfma32_fp4_fp8(kc[s], ks[s], q_lo[s], q_scale, sc);
+    }
+  };
+  auto weigh = [&](int t, const Stage &st) {
+    const int base = t * kBK;
+    // Key of register i: base + 16 (i / 8) + 8 half + i % 8.
+    if (__builtin_expect(base + kBK - 1 > wave_first || base + kBK > kv_len, 0)) {
+      const int lim = last_seen - base - 8 * half;
 #pragma unroll
       for (int i = 0; i < 16; ++i)
-        if (8 * (i / 4) + (i % 4) > lim) sc[i] = -INFINITY;
+        if (16 * (i / 8) + (i % 8) > lim) sc[i] = -INFINITY;
     }
     float tmax = -INFINITY;
 #pragma unroll
     for (int i = 0; i < 16; ++i) tmax = fmaxf(tmax, sc[i]);
     tmax = max_xor32(tmax) * a.scale_log2e;
-    if (__builtin_amdgcn_ballot_w64(tmax > m_thr) != 0) {
-      const bool up = tmax > m_thr;
-      const float alpha = up ? __builtin_amdgcn_exp2f(m_ref - tmax) : 1.f;
-      if (up) {
-        m_ref = tmax;
-        m_thr = tmax + kRescaleLog2;
-        neg_ref = -tmax;
-      }
+    // Lazy rescale: the weights stay below 2^8, and O and l are scaled only where some row's reference moves.
+    const bool up = tmax + neg_ref > kRescaleLog2;
+    if (__builtin_amdgcn_ballot_w64(up) != 0) {
+      const float alpha = up ? fast_exp2(-neg_ref - tmax) : 1.f;
+      if (up) neg_ref = -tmax;
       l_run *= alpha;
 #pragma unroll
       for (int db = 0; db < 4; ++db)
 #pragma unroll
         for (int i = 0; i < 16; ++i) acc[db][i] *= alpha;
     }
-    bf16x8v pf[2];
-#pragma unroll
-    for (int hh = 0; hh < 2; ++hh) {
-      u32x4 packed;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const u32 pr = pack_bf16x2(__builtin_amdgcn_exp2f(fmaf(sc[8 * hh + 2 * e], a.scale_log2e, neg_ref)),
-                                   __builtin_amdgcn_exp2f(fmaf(sc[8 * hh + 2 * e + 1], a.scale_log2e, neg_ref)));
-        l_run = dot2_bf16(pr, kBf16PairOne, l_run);  // both rounded values of the pair
-        packed[e] = pr;
-      }
-      pf[hh] = __builtin_bit_cast(bf16x8v, packed);
-    }
+    u32x4 pf[2];
 #pragma unroll
     for (int hh = 0; hh < 2; ++hh)
 #pragma unroll
-      for (int db = 0; db < 4; ++db) acc[db] = mfma32(__builtin_bit_cast(bf16x8v, st.v[hh][db][lane]), pf[hh], acc[db]);
-    const u32x4 nan = *reinterpret_cast<const u32x4 *>(&st.nan[0][0]);
-    if (__builtin_expect(__builtin_amdgcn_readfirstlane(nan[0] | nan[1] | nan[2] | nan[3]) != 0, 0)) {
-      const int seen = min(offset + rq, kv_len - 1) - base;  // the last key of the tile that this lane's row sees
+      for (int e = 0; e < 4; ++e) {
+        const u32 pr = pack_bf16x2(fast_exp2(fmaf(sc[8 * hh + 2 * e], a.scale_log2e, neg_ref)),
+                                   fast_exp2(fmaf(sc[8 * hh + 2 * e + 1], a.scale_log2e, neg_ref)));
+        l_run = dot2_bf16(pr, kBf16PairOne, l_run);  // both rounded values of the pair
+        pf[hh][e] = pr;
+      }
+#pragma unroll
+    for (int hh = 0; hh < 2; ++hh)
+#pragma unroll
+      for (int db = 0; db < 4; ++db) acc[db] = mfma32(st.v[hh][db][lane], pf[hh], acc[db]);
+    const u32x4 n0 = *reinterpret_cast<const u32x4 *>(st.nan[0]), n1 = *reinterpret_cast<const u32x4 *>(st.nan[2]);
+    if (__builtin_expect(__builtin_amdgcn_readfirstlane(n0[0] | n0[1] | n0[2] | n0[3] | n1[0] | n1[1] | n1[2] | n1[3]) != 0,
+                         0)) {
+      const int seen = last_seen - base;  // the last key of the tile that this lane's row sees
+      const u32 mask = seen < 0 ? 0u : seen >= 31 ? 0xffffffffu : (2u << seen) - 1u;
 #pragma unroll
       for (int db = 0; db < 4; ++db) {
-        const u32 bits = (u32)st.nan[0][db] | ((u32)st.nan[1][db] << 16);
-        const bool hit = seen >= 0 && (bits & (seen >= 31 ? 0xffffffffu : (2u << seen) - 1u)) != 0;
-        if (hit) {
+        u32 bits = 0;  // a scalar
 #pragma unroll
-          for (int i = 0; i < 16; ++i) acc[db][i] = NAN;
+        for (int x = 0; x < 4; ++x) {
+          const u32 word = x < 2 ? n0[2 * x + (db >> 1)] : n1[2 * (x - 2) + (db >> 1)];
+          bits |= ((__builtin_amdgcn_readfirstlane(word) >> (16 * (db & 1))) & 0xffu) << (8 * x);
         }
+        const float poison = (bits & mask) != 0 ? NAN : 0.f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[db][i] += poison;
       }
     }
   };
 
-  // Tile t is computed from stage t % 2 while the other stage takes tile t + 1, whose codes were fetched during tile t - 1.
   if (n_tiles > 0) {
-    fetch(0);
-    expand(0, s_stage[0]);
-    if (n_tiles > 1) fetch(1);
-  }
-  __syncthreads();
-  for (int t = 0; t < n_tiles; ++t) {
-    if (t + 1 < n_tiles) {
-      expand(t + 1, s_stage[(t + 1) & 1]);
-      if (t + 2 < n_tiles) fetch(t + 2);
-    }
-    compute(t, s_stage[t & 1]);
+    look_up(0);
+    locate(0);
+    load_k(tile[0], tile[1]);
+    load_v();
+    look_up(1);
+    expand(0, stages[0]);
+    locate(1);
+    load_v();
+    look_up(2);
     __syncthreads();
+    // Here K holds tile t, V's registers tile t + 1, stage t % 2 V's operands of tile t; `tile` is t + 1's, `entry` t + 2's.
+#pragma unroll 1
+    for (int t = 0; t < n_tiles; ++t) {
+      const bool visible = r0 < rows.rows && t * kBK <= wave_last;
+      const int2 next = {tile[0], tile[1]};
+      if (t + 1 < n_tiles) {
+        expand(t + 1, stages[(t + 1) & 1]);
+        locate(t + 2);
+        load_v();
+        look_up(t + 3);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      if (visible) score();
+      __builtin_amdgcn_sched_barrier(0);
+      if (t + 1 < n_tiles) load_k(next.x, next.y);
+      if (visible) weigh(t, stages[t & 1]);
+      __syncthreads();
+    }
   }
 
-  // Normalise and write: the wave turns its 32 rows around in LDS and stores whole 256-byte rows.
+  // Normalise and write: the wave turns its rows around in LDS, 16 at a time, and stores whole 256-byte rows.
+  asm volatile("" : "+v"(row));  // token and head anew: they would hold registers through the loop
+  const int token = row / a.group, head = g * a.group + row - token * a.group;
   const float l_tot = sum_xor32(l_run);
   const float inv = l_tot > 0.f ? 1.f / l_tot : 0.f;
-  constexpr int kRow = D + 8;  // elements: 16 bytes of padding spread the rows over the banks
-  static_assert(sizeof(s_stage) >= (size_t)kWaves * 16 * kRow * sizeof(u16), "16 rows of every wave");
-  u16 *so = reinterpret_cast<u16 *>(&s_stage[0]) + w * 16 * kRow;
-  const int rows = min(q_len - r0, 32);
+  u16 *so = reinterpret_cast<u16 *>(s_mem) + w * 16 * kRowPad;
 #pragma unroll
-  for (int half = 0; half < 2; ++half) {  // 16 query rows at a time
+  for (int part = 0; part < 2; ++part) {
     __syncthreads();
-    if ((n >> 4) == half) {
+    if ((n >> 4) == part) {
 #pragma unroll
       for (int db = 0; db < 4; ++db)
 #pragma unroll
@@ -285,26 +340,210 @@ prefill_fp4_kernel(PrefillFp4Args a) {
           u32x2 pk;
           pk[0] = pack_bf16x2(acc[db][4 * i4] * inv, acc[db][4 * i4 + 1] * inv);
           pk[1] = pack_bf16x2(acc[db][4 * i4 + 2] * inv, acc[db][4 * i4 + 3] * inv);
-          *reinterpret_cast<u32x2 *>(so + (n & 15) * kRow + 32 * db + 8 * i4 + 4 * hl) = pk;
+          *reinterpret_cast<u32x2 *>(so + (n & 15) * kRowPad + 32 * db + 8 * i4 + 4 * half) = pk;
         }
     }
     __syncthreads();
-    u16 *op = a.out + (int64_t)(q_start + r0 + 16 * half) * a.out_stride + (int64_t)head * D + 8 * (lane & 15);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int r = 4 * i + (lane >> 4);
-      const u32x4 v = *reinterpret_cast<const u32x4 *>(so + r * kRow + 8 * (lane & 15));
-      if (16 * half + r < rows) st16(op + (int64_t)r * a.out_stride, v);
+      const int r = 4 * i + (lane >> 4);  // of the 16
+      const int t = __shfl(token, 16 * part + r), h = __shfl(head, 16 * part + r);
+      const u32x4 v = *reinterpret_cast<const u32x4 *>(so + r * kRowPad + 8 * (lane & 15));
+      if (r0 + 16 * part + r < rows.rows)
+        st16(a.out + (int64_t)(rows.q_start + t) * a.out_stride + (int64_t)h * D + 8 * (lane & 15), v);
     }
   }
 }
 
-template <int GQA>
-int launch(const PrefillFp4Args &a, int n_seqs, hipStream_t stream) {
-  hipLaunchKernelGGL((prefill_fp4_kernel<GQA>), dim3(a.num_kv_heads, a.max_q_tiles, n_seqs), dim3(kThreads), 0, stream,
-                     a);
-  return launch_status();
+// ------------------------------------------------------------------------------------------ few rows
+constexpr int kFewWaves = 8;
+constexpr int kFewRows = 16;
+constexpr int kRec = kHeadDim + 4;  // floats of a row in the waves' meeting
+
+__global__ void __launch_bounds__(kFewWaves * 64) __attribute__((amdgpu_waves_per_eu(3)))
+prefill_few_fp4_kernel(PrefillFp4Args a) {
+  constexpr int D = kHeadDim;
+  __shared__ __attribute__((aligned(16))) float s_o[kFewWaves][kFewRows * kRec];
+  __shared__ float s_m[kFewWaves][kFewRows];
+  __shared__ float s_l[kFewWaves][kFewRows];
+
+  Rows rows;
+  if (!find_rows(a, kFewRows, rows)) return;
+  const int g = blockIdx.x;
+  const int lane = threadIdx.x & 63;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int n = lane & 15, gq = lane >> 4;
+  const int row = min(rows.first + n, rows.rows - 1);
+  const int token = row / a.group, head = g * a.group + row - token * a.group;
+  const int last_seen = min(rows.offset + token, rows.kv_len - 1);
+  const int first_seen = rows.offset + rows.first / a.group;  // the last key that the first row sees
+  const int keys = min(rows.kv_len, rows.offset + (min(rows.first + kFewRows, rows.rows) - 1) / a.group + 1);
+
+  i32x8 q_hi, q_lo;
+  u32 q_scale;
+  {
+    const u16 *qp = a.q + (int64_t)(rows.q_start + token) * a.q_stride + (int64_t)head * D + 16 * gq;
+    const u32x4 x[4] = {ld16(qp), ld16(qp + 8), ld16(qp + 64), ld16(qp + 72)};
+    u32 top = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) top = max(top, largest(x[j]));
+    const QueryScale scale = query_scale((u32)max_over_quarters((float)top));
+    split32(x, scale.up, q_hi, q_lo);
+    q_scale = scale.byte;
+  }
+
+  float m = kNoScore, m_thr = kNoScore, l = 0.f;
+  f32x4 o[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) o[e] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+  const int32_t *bt = a.block_tables + (int64_t)blockIdx.z * a.bt_stride;
+  const int last_tile = max(rows.kv_len - 1, 0) & ~15;
+  int entry_k = 0, entry_v = 0;
+  auto look_up = [&](int t0) {
+    entry_k = bt[min(t0 + 16 * (n >> 2), last_tile) >> a.bs_log2];
+    entry_v = bt[min(t0 + 16 * gq, last_tile) >> a.bs_log2];
+  };
+  u32x4 kc[4], vc[4];
+  u32 ks, vs;
+  int64_t k_tile, v_tile;
+  auto locate = [&](int t0) {
+    k_tile = tile_of(a, entry_k, min(t0 + 16 * (n >> 2), last_tile), g, true);
+    v_tile = tile_of(a, entry_v, min(t0 + 16 * gq, last_tile), g, true);
+  };
+  auto load_k = [&]() {
+    const u8 *kp = a.cache.k_codes + k_tile * kFp4TileBytes + (n & 3) * kFp4RowBytes + 16 * gq;
+#pragma unroll
+    for (int t = 0; t < 4; ++t) kc[t] = *reinterpret_cast<const u32x4 *>(kp + 4 * t * kFp4RowBytes);
+    ks = *reinterpret_cast<const u32 *>(a.cache.k_scales + k_tile * kFp4TileScales + fp4_key_scale_at(n & 3, gq));
+  };
+  auto load_v = [&]() {
+    const u8 *vp = a.cache.v_codes + v_tile * kFp4TileBytes + 16 * n;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) vc[q] = *reinterpret_cast<const u32x4 *>(vp + 256 * q);
+    vs = *reinterpret_cast<const u32 *>(a.cache.v_scales + v_tile * kFp4TileScales + 4 * n);
+  };
+  auto step = [&](const int t0, const int next) {
+    f32x4 s[4];
+    const u32 k_scale[4] = {ks & 0xffu, (ks >> 8) & 0xffu, (ks >> 16) & 0xffu, ks >> 24};
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      s[t] = mfma_fp4_fp8(kc[t], k_scale[t], q_hi, q_scale, f32x4{0.f, 0.f, 0.f, 0.f});
+      s[t] = mfma_fp4_fp8(kc[t], k_scale[t], q_lo, q_scale, s[t]);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    if (next < keys) {
+      locate(next);
+      load_k();
+      look_up(next + 64 * kFewWaves);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    float cm = kNoScore;
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s[t][i] *= a.scale_log2e;
+    if (t0 + 63 > first_seen || t0 + 64 > rows.kv_len) {
+      const int lim = last_seen - t0 - 16 * gq;  // token 4 t + i of tile gq
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (4 * t + i > lim) s[t][i] = -INFINITY;
+      vs = keep_bytes(vs, rows.kv_len - t0 - 16 * gq - 4 * (n & 3));  // stale rows past the keys
+    }
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) cm = fmaxf(cm, s[t][i]);
+    cm = max_over_quarters(cm);
+    if (__builtin_amdgcn_ballot_w64(cm > m_thr) != 0) {
+      const bool up = cm > m_thr;
+      const float alpha = up ? fast_exp2(m - cm) : 1.f;
+      if (up) {
+        m = cm;
+        m_thr = cm + kRescaleLog2;
+      }
+      l *= alpha;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) o[e] *= alpha;
+    }
+    u32x4 pf[2];
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const u32 pr = pack_bf16x2(fast_exp2(s[t][2 * i] - m), fast_exp2(s[t][2 * i + 1] - m));
+        l = dot2_bf16(pr, kBf16PairOne, l);
+        pf[t >> 1][2 * (t & 1) + i] = pr;
+      }
+    const u32 bad = nan_bytes(vs);
+    vs = without(vs, bad);
+    add_values<0>(o, vc, vs, pf);
+    add_values<1>(o, vc, vs, pf);
+    add_values<2>(o, vc, vs, pf);
+    add_values<3>(o, vc, vs, pf);
+    if (__builtin_expect(__builtin_amdgcn_ballot_w64(bad != 0) != 0, 0)) {
+      float poison[4] = {0.f, 0.f, 0.f, 0.f};  // of each block, for this lane's row
+#pragma unroll 1
+      for (int x = 0; x < 64; ++x) {  // lane x noted tokens 4 (x % 4) .. of tile x / 16, block (x % 16) / 4
+        const u32 b = (u32)__builtin_amdgcn_readlane((int)bad, x);
+        if (b == 0) continue;
+        const int at = t0 + 16 * (x >> 4) + 4 * (x & 3) + (__ffs((int)b) >> 3) - 1;  // the first of them (bit 7 of a byte)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) poison[q] = last_seen >= at && (x & 15) >> 2 == q ? NAN : poison[q];
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) o[e] += poison[e >> 1];
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    if (next < keys) load_v();
+  };
+  if (int t0 = 64 * w; t0 < keys) {
+    look_up(t0);
+    locate(t0);
+    load_k();
+    load_v();
+    look_up(t0 + 64 * kFewWaves);
+#pragma unroll 1
+    do {
+      step(t0, t0 + 64 * kFewWaves);
+      t0 += 64 * kFewWaves;
+    } while (t0 < keys);
+  }
+
+  // Register i of o[e] is dim 16 e + 4 gq + i of row n.
+  l = sum_over_quarters(l);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) *reinterpret_cast<f32x4 *>(&s_o[w][n * kRec + 16 * e + 4 * gq]) = o[e];
+  if (gq == 0) {
+    s_m[w][n] = m;
+    s_l[w][n] = l;
+  }
+  __syncthreads();
+  // A half-wave takes a row, its lane dims 4 dl .. 4 dl + 3.
+  static_assert(2 * kFewWaves == kFewRows);
+  const int r = threadIdx.x >> 5, dl = lane & 31;
+  float M = s_m[0][r], den = 0.f;
+#pragma unroll
+  for (int x = 1; x < kFewWaves; ++x) M = fmaxf(M, s_m[x][r]);
+  f32x4 num = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int x = 0; x < kFewWaves; ++x) {
+    const float f = fast_exp2(s_m[x][r] - M);
+    num += f * *reinterpret_cast<const f32x4 *>(&s_o[x][r * kRec + 4 * dl]);
+    den += f * s_l[x][r];
+  }
+  if (rows.first + r < rows.rows) {
+    const float inv = den > 0.f ? 1.f / den : 0.f;
+    const int t = (rows.first + r) / a.group, h = g * a.group + rows.first + r - t * a.group;
+    *reinterpret_cast<u32x2 *>(a.out + (int64_t)(rows.q_start + t) * a.out_stride + (int64_t)h * D + 4 * dl) =
+        u32x2{pack_bf16x2(num[0] * inv, num[1] * inv), pack_bf16x2(num[2] * inv, num[3] * inv)};
+  }
 }
+
+// Workgroups of the tile kernel below which the few-rows kernel runs.
+constexpr int64_t kFewGroups = 256;
 
 }  // namespace
 }  // namespace nvamd
@@ -327,7 +566,8 @@ extern "C" int nvamd_paged_prefill_fp4(void *out, int64_t out_stride, const void
       !aligned16(out) || q_stride % 8 || out_stride % 8 || q_stride < (int64_t)num_heads * head_dim ||
       out_stride < (int64_t)num_heads * head_dim)
     return NVAMD_EINVAL;
-  if (((int64_t)bt_width << bs_log2) > 0x7fffffff) return NVAMD_EUNSUPPORTED;
+  if (((int64_t)bt_width << bs_log2) > 0x7fffffff || (((int64_t)num_blocks * num_kv_heads) << bs_log2) >> 4 > 0x7fffffff)
+    return NVAMD_EUNSUPPORTED;
   PrefillFp4Args a = {};
   a.out = static_cast<u16 *>(out);
   a.out_stride = out_stride;
@@ -349,17 +589,17 @@ extern "C" int nvamd_paged_prefill_fp4(void *out, int64_t out_stride, const void
   a.num_tokens = num_tokens;
   a.scale_log2e = scale * kLog2e;
   a.err = index_error_word();
-  a.q_group = num_heads / num_kv_heads;
-  // A workgroup takes 4, 2 or 1 heads of a group; other ratios run as consecutive launches over 4, then 2, then 1.
-  for (int rest = a.q_group; rest > 0;) {
-    const int sub = rest >= 4 ? 4 : rest >= 2 ? 2 : 1;
-    a.q_head0 = a.q_group - rest;
-    a.max_q_tiles = ceil_div(max_q_len, 32 * kWaves / sub);
-    if (a.max_q_tiles > 65535) return NVAMD_EUNSUPPORTED;
-    const int st = sub == 4 ? launch<4>(a, n_seqs, stream) : sub == 2 ? launch<2>(a, n_seqs, stream)
-                                                                      : launch<1>(a, n_seqs, stream);
-    if (st != NVAMD_OK) return st;
-    rest -= sub;
-  }
-  return NVAMD_OK;
+  a.group = num_heads / num_kv_heads;
+  const int64_t max_rows = (int64_t)max_q_len * a.group;
+  if (max_rows > 0x7fffffff) return NVAMD_EUNSUPPORTED;
+  const int64_t tiles = (max_rows + kTileRows - 1) / kTileRows;
+  const bool few = tiles * num_kv_heads * n_seqs <= kFewGroups;
+  a.max_tiles = (int)(few ? (max_rows + kFewRows - 1) / kFewRows : tiles);
+  if (a.max_tiles > 65535) return NVAMD_EUNSUPPORTED;
+  const dim3 grid(num_kv_heads, a.max_tiles, n_seqs);
+  if (few)
+    hipLaunchKernelGGL(prefill_few_fp4_kernel, grid, dim3(kFewWaves * 64), 0, stream, a);
+  else
+    hipLaunchKernelGGL(prefill_fp4_kernel, grid, dim3(kWaves * 64), 0, stream, a);
+  return launch_status();
 }

@@ -239,6 +239,11 @@ class Window:
 
 
 # -------------------------------------------------------------------------------------------- prefill
+# Launches whose bound gives few workgroups run another kernel than the rest: each test makes both, by a bound far past its
+# lengths.
+BOUNDS = pytest.mark.parametrize("bound", [None, 60_000], ids=["few", "tiles"])
+
+
 def check_prefill(batch, q, q_lens, got, scale=SCALE):
     at = 0
     for i, n in enumerate(q_lens):
@@ -247,40 +252,44 @@ def check_prefill(batch, q, q_lens, got, scale=SCALE):
         at += n
 
 
-@pytest.mark.parametrize("hq, hkv", [(1, 1), (2, 1), (3, 1), (4, 1), (5, 1), (16, 8), (8, 1), (14, 2)])
-def test_prefill_head_layouts(device, hq, hkv):
+@BOUNDS
+@pytest.mark.parametrize("hq, hkv", [(1, 1), (2, 1), (3, 1), (4, 1), (5, 1), (16, 8), (8, 1), (14, 2), (17, 1), (40, 1)])
+def test_prefill_head_layouts(device, hq, hkv, bound):
     q_lens, cached = [1, 40, 0, 130], [200, 16, 33, 0]
     batch = Batch(device, [a + b for a, b in zip(q_lens, cached)], hq, hkv, 32, seed=hq)
     q = batch.queries(sum(q_lens))
-    check_prefill(batch, q, q_lens, batch.prefill(q, q_lens))
+    check_prefill(batch, q, q_lens, batch.prefill(q, q_lens, max_q=bound))
     assert _C.index_errors() == 0
 
 
+@BOUNDS
 @pytest.mark.parametrize("bs", [16, 32, 64, 128, 256])
-def test_prefill_lengths_around_tiles_and_pages(device, bs):
+def test_prefill_lengths_around_tiles_and_pages(device, bs, bound):
     q_lens = [1, 2, 15, 16, 17, 31, 32, 33, 63, 64, 65, 127, 128, 129, 255, 257]
     cached = [0, 1, 16, 31, 32, 5, 64, 100, 0, 128, 129, 1, 16, 300, 0, 255]
     batch = Batch(device, [a + b for a, b in zip(q_lens, cached)], 4, 2, bs, seed=bs)
     q = batch.queries(sum(q_lens))
-    check_prefill(batch, q, q_lens, batch.prefill(q, q_lens))
-    check_prefill(batch, q, q_lens, batch.prefill(q, q_lens, max_q=700))  # a bound past the lengths
+    check_prefill(batch, q, q_lens, batch.prefill(q, q_lens, max_q=bound))
 
 
+@BOUNDS
 @pytest.mark.parametrize("q_len, cached", [(1, 9000), (600, 4096), (1500, 0)])
-def test_prefill_long(device, q_len, cached):
+def test_prefill_long(device, q_len, cached, bound):
     batch = Batch(device, [q_len + cached, 1], 2, 1, 128, seed=2)
     q = batch.queries(q_len + 1)
-    check_prefill(batch, q, [q_len, 1], batch.prefill(q, [q_len, 1]))
+    check_prefill(batch, q, [q_len, 1], batch.prefill(q, [q_len, 1], max_q=bound))
 
 
-def test_prefill_scores_far_apart(device):
+@BOUNDS
+def test_prefill_scores_far_apart(device, bound):
     """Maxima that rise along the keys, so that the running reference moves again and again."""
     batch = Batch(device, [400, 90], 2, 1, 16, seed=3, spread=1.5)
     q = batch.queries(300 + 90, scale=8.0)
-    check_prefill(batch, q, [300, 90], batch.prefill(q, [300, 90]))
+    check_prefill(batch, q, [300, 90], batch.prefill(q, [300, 90], max_q=bound))
 
 
-def test_prefill_nan_reaches_the_rows_that_see_its_key_alone(device):
+@BOUNDS
+def test_prefill_nan_reaches_the_rows_that_see_its_key_alone(device, bound):
     batch = Batch(device, [150, 150], 2, 1, 16, seed=4)
     one = torch.ones(1, 1, 128, dtype=torch.bfloat16)
     bad_v, bad_k = one.clone(), one.clone()
@@ -290,38 +299,40 @@ def test_prefill_nan_reaches_the_rows_that_see_its_key_alone(device):
     fp4_ref.write(batch.pages, bad_k, one, batch.slots[1][120:121])
     batch.upload()
     q = batch.queries(150)  # 50 rows of the first sequence, from position 100 on, and 100 of the second, from 50 on
-    got = batch.prefill(q, [50, 100])
+    got = batch.prefill(q, [50, 100], max_q=bound)
     check_prefill(batch, q, [50, 100], got)
     nan = got.isnan().cpu()
     assert not nan[:9].any() and nan[9:50, :, 32:64].all() and not nan[9:50, :, :32].any()
     assert not nan[50:120].any() and nan[120:].all()
 
 
-def test_prefill_views_and_rows_behind_the_last_sequence(device):
+@BOUNDS
+def test_prefill_views_and_rows_behind_the_last_sequence(device, bound):
     batch = Batch(device, [40, 70], 3, 1, 16, seed=5)
     fused = torch.zeros(60, 5, 128, dtype=torch.bfloat16)
     q = batch.queries(50)
     fused[:50, 1:4] = q
     wide = torch.full((60, 5, 128), 7.0, dtype=torch.bfloat16, device=device)
-    batch.prefill(fused.to(device)[:, 1:4], [20, 30], out=wide[:, 2:])
+    batch.prefill(fused.to(device)[:, 1:4], [20, 30], out=wide[:, 2:], max_q=bound)
     check_prefill(batch, q, [20, 30], wide[:50, 2:])
     assert wide[50:].eq(7).all() and wide[:, :2].eq(7).all()
 
 
-def test_prefill_faults_are_reported_and_leave_the_others_alone(device):
+@BOUNDS
+def test_prefill_faults_are_reported_and_leave_the_others_alone(device, bound):
     batch = Batch(device, [100, 60, 200], 2, 1, 16, seed=6)
     q_lens = [20, 60, 100]
     q = batch.queries(180)
-    good = batch.prefill(q, q_lens)
+    good = batch.prefill(q, q_lens, max_q=bound)
     others = torch.cat([torch.arange(20), torch.arange(80, 180)])
     batch.tables[1, 2] = batch.nb
-    got = batch.prefill(q, q_lens)
+    got = batch.prefill(q, q_lens, max_q=bound)
     assert _C.index_errors() == _C.ERR_BLOCK and torch.equal(got[others], good[others])
     _C.clear_index_errors()
     batch.tables[1, 2] = 0
     for n in (59, 0, -1, 1 << 20):  # fewer keys than rows; more than the table holds
         batch.lens[1] = n
-        got = batch.prefill(q, q_lens)
+        got = batch.prefill(q, q_lens, max_q=bound)
         assert _C.index_errors() == _C.ERR_CONTEXT and torch.equal(got[others], good[others])
         if n <= 0:
             assert not got[20:80].any()  # rows that see no key
@@ -331,9 +342,16 @@ def test_prefill_faults_are_reported_and_leave_the_others_alone(device):
     out = torch.full((180, 2, 128), 7.0, dtype=torch.bfloat16, device=device)
     args = (batch.keys, batch.values, batch.tables.to(device), cu,
             torch.tensor(batch.lens, dtype=torch.int32, device=device))
-    _C.paged_prefill_fp4(out, q.to(device), *args, 101, SCALE)
+    _C.paged_prefill_fp4(out, q.to(device), *args, bound or 101, SCALE)
     assert _C.index_errors() == _C.ERR_CONTEXT
     assert torch.equal(out[:20], good[:20]) and out[80:].eq(7).all()
+
+
+def test_prefill_bound_below_a_length_is_reported(device):
+    batch = Batch(device, [100], 2, 1, 16, seed=6)
+    q = batch.queries(50)
+    batch.prefill(q, [50], max_q=49)
+    assert _C.index_errors() == _C.ERR_CONTEXT
 
 
 def test_prefill_replays_from_a_graph(device):
@@ -344,7 +362,7 @@ def test_prefill_replays_from_a_graph(device):
     out = torch.empty_like(q)
 
     def call(out):
-        return _C.paged_prefill_fp4(out, q, batch.keys, batch.values, tables, cu, lens, 100, SCALE)
+        return _C.paged_prefill_fp4(out, q, batch.keys, batch.values, tables, cu, lens, 120, SCALE)  # 10 .. 120 rows
 
     call(out)
     graph = torch.cuda.CUDAGraph()
