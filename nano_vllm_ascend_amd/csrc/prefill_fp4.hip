@@ -104,10 +104,13 @@ __device__ __forceinline__ f32x16 mfma32_fp4_fp8(u32x4 k, u32 k_scale, i32x8 q, 
 
 struct Stage {
   u32x4 v[2][4][64];  // [16-key step][32-dim block][lane]
-  u32 nan[4][2];      // [wave that expanded them][..]: a bit per (block, token) whose values read as NaN, 8 tokens a byte
+  u32 any[4];         // [wave that expanded them]: whether any of its values read as NaN,
+  u32 nan[4][2];      // and which: two blocks of dims a word, a bit for each of the 8 tokens in its half
 };
 constexpr int kRowPad = kHeadDim + 8;  // elements of a row in the output's turn: 16 bytes of padding spread the banks
 
+// WIDE: pages of 32 tokens or more, so that a tile's keys lie in one page and K loads from a scalar address.
+template <bool WIDE>
 __global__ void __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(3)))
 prefill_fp4_kernel(PrefillFp4Args a) {
   constexpr int D = kHeadDim;
@@ -178,10 +181,19 @@ prefill_fp4_kernel(PrefillFp4Args a) {
   const int k_token = (n & 3) | ((n & 8) >> 1) | ((n & 4) << 1);  // of its 16-token tile, n / 16
   u32x4 kc[2];
   u32 ks[2];
+  const u32 k_at = k_token * kFp4RowBytes + 16 * half, ks_at = fp4_key_scale_at(k_token, half);
+  const u32 second = n < 16 ? 0u : ~0u;  // mask: the lane's key is in the second 16-token tile
   auto load_k = [&](int t0, int t1) {
-    const int64_t t = n < 16 ? t0 : t1;
-    const u8 *kp = a.cache.k_codes + t * kFp4TileBytes + k_token * kFp4RowBytes + 16 * half;
-    const u8 *sp = a.cache.k_scales + t * kFp4TileScales + fp4_key_scale_at(k_token, half);
+    const u8 *kp, *sp;
+    if constexpr (WIDE) {
+      const u32 d = (u32)(t1 - t0);  // 1, or 0 past the keys
+      kp = a.cache.k_codes + (int64_t)t0 * kFp4TileBytes + (k_at + (second & (d * kFp4TileBytes)));
+      sp = a.cache.k_scales + (int64_t)t0 * kFp4TileScales + (ks_at + (second & (d * kFp4TileScales)));
+    } else {
+      const int64_t t = second ? t1 : t0;
+      kp = a.cache.k_codes + t * kFp4TileBytes + k_at;
+      sp = a.cache.k_scales + t * kFp4TileScales + ks_at;
+    }
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
       kc[s] = *reinterpret_cast<const u32x4 *>(kp + 32 * s);
@@ -209,8 +221,9 @@ prefill_fp4_kernel(PrefillFp4Args a) {
       // blocks 0, 1 and 2, 3 in two words of 16 bits each
       seen0 = (u32)__builtin_amdgcn_readlane((int)bits, 0) | (u32)__builtin_amdgcn_readlane((int)bits, 16) << 16;
       seen1 = (u32)__builtin_amdgcn_readlane((int)bits, 32) | (u32)__builtin_amdgcn_readlane((int)bits, 48) << 16;
+      if (lane == 0) *reinterpret_cast<u32x2 *>(st.nan[w]) = u32x2{seen0, seen1};
     }
-    if (lane == 0) *reinterpret_cast<u32x2 *>(st.nan[w]) = u32x2{seen0, seen1};
+    if (lane == 0) st.any[w] = seen0 | seen1;
     u32x4 lo, hi;
     {
       u32 x[8];
@@ -272,22 +285,22 @@ prefill_fp4_kernel(PrefillFp4Args a) {
     for (int hh = 0; hh < 2; ++hh)
 #pragma unroll
       for (int db = 0; db < 4; ++db) acc[db] = mfma32(st.v[hh][db][lane], pf[hh], acc[db]);
-    const u32x4 n0 = *reinterpret_cast<const u32x4 *>(st.nan[0]), n1 = *reinterpret_cast<const u32x4 *>(st.nan[2]);
-    if (__builtin_expect(__builtin_amdgcn_readfirstlane(n0[0] | n0[1] | n0[2] | n0[3] | n1[0] | n1[1] | n1[2] | n1[3]) != 0,
-                         0)) {
+    const u32x4 any = *reinterpret_cast<const u32x4 *>(st.any);
+    if (__builtin_expect(__builtin_amdgcn_readfirstlane(any[0] | any[1] | any[2] | any[3]) != 0, 0)) {
       const int seen = last_seen - base;  // the last key of the tile that this lane's row sees
       const u32 mask = seen < 0 ? 0u : seen >= 31 ? 0xffffffffu : (2u << seen) - 1u;
+#pragma unroll 1
+      for (int x = 0; x < 4; ++x) {  // 8 tokens each
+        if (__builtin_amdgcn_readfirstlane(st.any[x]) == 0) continue;
+        const u32 word[2] = {(u32)__builtin_amdgcn_readfirstlane(st.nan[x][0]),
+                             (u32)__builtin_amdgcn_readfirstlane(st.nan[x][1])};
 #pragma unroll
-      for (int db = 0; db < 4; ++db) {
-        u32 bits = 0;  // a scalar
+        for (int db = 0; db < 4; ++db) {
+          const u32 bits = ((word[db >> 1] >> (16 * (db & 1))) & 0xffu) << (8 * x);
+          const float poison = (bits & mask) != 0 ? NAN : 0.f;
 #pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          const u32 word = x < 2 ? n0[2 * x + (db >> 1)] : n1[2 * (x - 2) + (db >> 1)];
-          bits |= ((__builtin_amdgcn_readfirstlane(word) >> (16 * (db & 1))) & 0xffu) << (8 * x);
+          for (int i = 0; i < 16; ++i) acc[db][i] += poison;
         }
-        const float poison = (bits & mask) != 0 ? NAN : 0.f;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) acc[db][i] += poison;
       }
     }
   };
@@ -599,7 +612,9 @@ extern "C" int nvamd_paged_prefill_fp4(void *out, int64_t out_stride, const void
   const dim3 grid(num_kv_heads, a.max_tiles, n_seqs);
   if (few)
     hipLaunchKernelGGL(prefill_few_fp4_kernel, grid, dim3(kFewWaves * 64), 0, stream, a);
+  else if (bs_log2 >= 5)
+    hipLaunchKernelGGL(prefill_fp4_kernel<true>, grid, dim3(kWaves * 64), 0, stream, a);
   else
-    hipLaunchKernelGGL(prefill_fp4_kernel, grid, dim3(kWaves * 64), 0, stream, a);
+    hipLaunchKernelGGL(prefill_fp4_kernel<false>, grid, dim3(kWaves * 64), 0, stream, a);
   return launch_status();
 }
