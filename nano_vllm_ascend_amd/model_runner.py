@@ -41,11 +41,12 @@ from .block_manager import BlockManager, PagedKVCacheMetadata
 from .config import load_config
 from .graph import DecodeGraphRunner
 from .layers import RotaryEmbedding, Sampler
-from .paged_kv_cache import PagedKVCache
+from .paged_kv_cache import Fp4PagedKVCache, PagedKVCache
 from .qwen3 import Qwen3ForCausalLM, load_safetensors_dir
 from .sequence import Sequence
 
 DEFAULT_DECODE_GRAPH_BATCH_SIZES = [1, 2, 4, 8, 16, 32]
+KV_CACHE_DTYPES = ("bf16", "fp4")
 
 
 class _TokenFetch:
@@ -111,7 +112,10 @@ class ModelRunner:
     def __init__(self, model_path, max_model_len: int, num_blocks: int | None, block_size: int, device_id: int,
                  npu_memory_utilization: float, enable_prefix_cache: bool = False, enable_decode_graph: bool = False,
                  decode_graph_batch_sizes: list[int] | None = None, seed: int = 0, max_num_seqs: int = 64,
-                 enable_overlap: bool = True, retain_logits: bool = False):
+                 enable_overlap: bool = True, retain_logits: bool = False, kv_cache_dtype: str = "bf16"):
+        if kv_cache_dtype not in KV_CACHE_DTYPES:
+            raise ValueError(f"kv_cache_dtype must be one of {KV_CACHE_DTYPES}, got {kv_cache_dtype!r}")
+        self.kv_cache_dtype = kv_cache_dtype
         torch.cuda.set_device(device_id)
         self.device = torch.device("cuda", device_id)
         self.model_path = model_path
@@ -131,8 +135,9 @@ class ModelRunner:
                                           max_seqs=max(max_num_seqs, 8),
                                           max_blocks_per_seq=max(1, -(-max_model_len // block_size)))
         cfg = self.config
-        self.kv_cache = PagedKVCache(cfg.num_hidden_layers, self.num_blocks, block_size, cfg.num_key_value_heads,
-                                     cfg.head_dim, self.dtype, self.device)
+        pool = cfg.num_hidden_layers, self.num_blocks, block_size, cfg.num_key_value_heads, cfg.head_dim
+        self.kv_cache = (Fp4PagedKVCache(*pool, self.device) if kv_cache_dtype == "fp4"
+                         else PagedKVCache(*pool, self.dtype, self.device))
         self.decode_graph_runner = None
         if enable_decode_graph:
             self.decode_graph_runner = DecodeGraphRunner(
@@ -187,8 +192,9 @@ class ModelRunner:
         free, total = torch.cuda.mem_get_info(self.device)
         budget = int(total * utilization) - (total - free)
         cfg = self.config
-        per_block = PagedKVCache.bytes_per_block(cfg.num_hidden_layers, self.block_size, cfg.num_key_value_heads,
-                                                 cfg.head_dim)
+        kind = Fp4PagedKVCache if self.kv_cache_dtype == "fp4" else PagedKVCache
+        per_block = kind.bytes_per_block(cfg.num_hidden_layers, self.block_size, cfg.num_key_value_heads,
+                                         cfg.head_dim)
         return max(1, budget // per_block)
 
     # -------------------------------------------------------------- prompts

@@ -74,6 +74,8 @@ class Fp4PagedKVCache:
                                             for _ in range(2))
         self.key_scales, self.value_scales = (
             torch.zeros((*rows, _C.FP4_ROW_SCALES), dtype=torch.uint8, device=device) for _ in range(2))
+        self._pages = [(_C.Fp4Pages(kc, ks), _C.Fp4Pages(vc, vs)) for kc, ks, vc, vs in
+                       zip(self.key_codes, self.key_scales, self.value_codes, self.value_scales)]
 
     @staticmethod
     def bytes_per_block(num_layers: int, block_size: int, num_kv_heads: int, head_dim: int) -> int:
@@ -96,5 +98,4 @@ class Fp4PagedKVCache:
         return _C.kv_cache_read_fp4(*self.get_physical_cache(layer_idx), self._slots(slot_mapping))
 
     def get_physical_cache(self, layer_idx: int) -> tuple[_C.Fp4Pages, _C.Fp4Pages]:
-        return (_C.Fp4Pages(self.key_codes[layer_idx], self.key_scales[layer_idx]),
-                _C.Fp4Pages(self.value_codes[layer_idx], self.value_scales[layer_idx]))
+        return self._pages[layer_idx]
