@@ -5,7 +5,7 @@
 
 namespace nvamd {
 
-constexpr float kNoScore = -1e30f;   // reference of an empty softmax: finite, so that it needs no guard in exponents
+constexpr float kNoScore = -3e38f;   // reference of an empty softmax: finite, so that it needs no guard in exponents
 constexpr float kRescaleLog2 = 8.f;  // the reference moves when a score exceeds it by 2^8
 constexpr u32 kBf16PairOne = 0x3F803F80u;
 
@@ -28,20 +28,20 @@ __device__ __forceinline__ float sum_over_quarters(float v) {
 
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 
-// S += K . q for 16 rows of codes (128 dims, a lane's block and its scale byte) and 16 columns of e4m3 under the scale
-// byte of a column.  Lane (row or column n, gq) gives block gq of its row; of its column, dims 16 gq .. +15 and 64 + 16 gq ..
-// +15 (checked on gfx950).
+// S += K . q for 16 rows of codes (128 dims) and 16 columns of e4m3, each block of 32 dims under its scale byte.  Lane (row
+// or column n, gq) gives block gq of its row, dims 16 gq .. +15 and 64 + 16 gq .. +15 of its column, and the scales of
+// block gq of either (checked on gfx950).
 __device__ __forceinline__ f32x4 mfma_fp4_fp8(u32x4 k, u32 k_scale, i32x8 q, u32 q_scale, f32x4 c) {
   const i32x8 codes = {(int)k[0], (int)k[1], (int)k[2], (int)k[3], 0, 0, 0, 0};
   return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(codes, q, c, 4, 0, 0, (int)k_scale, 0, (int)q_scale);
 }
 
-// A bf16 query row as hi + lo in e4m3 under 2^-s, s from the row's largest value, which lands in [128, 256).  hi keeps 4 of
-// the 8 significant bits and lo the rest: the sum is the value itself down to 2^-9 of the largest, and off by at most 2^-17 of the
-// largest below.
+// A block of 32 bf16 query values as hi + lo in e4m3 under 2^-s, s from its largest value, which lands in [128, 256).  hi
+// keeps 4 of the 8 significant bits and lo the rest: the sum is the value itself down to 2^-9 of the block's largest, and off
+// by at most 2^-17 of the largest below.
 struct QueryScale {
   float up;  // 2^s
-  u32 byte;  // of 2^-s; 255, which makes every score NaN, for a row with an infinity or a NaN
+  u32 byte;  // of 2^-s; 255, which makes every score NaN, for a block with an infinity or a NaN
 };
 __device__ __forceinline__ QueryScale query_scale(u32 top) {  // top: the largest value's bf16 bits, sign cleared
   const int e = min(max((int)(top >> 7), 20), 254);  // its biased exponent
@@ -67,17 +67,33 @@ __device__ __forceinline__ void split4(u32 w0, u32 w1, float up, int &hi, int &l
   lo = __builtin_amdgcn_cvt_pk_fp8_f32(c - __builtin_amdgcn_cvt_f32_fp8(h, 2),
                                        d - __builtin_amdgcn_cvt_f32_fp8(h, 3), r, true);
 }
-// A lane's 32 values, in the order of the operand.
-__device__ __forceinline__ void split32(const u32x4 (&x)[4], float up, i32x8 &hi, i32x8 &lo) {
+// A lane's 32 values, in the order of the operand: 16 of one block, then 16 of another.
+__device__ __forceinline__ void split32(const u32x4 (&x)[4], float up0, float up1, i32x8 &hi, i32x8 &lo) {
 #pragma unroll
   for (int j = 0; j < 4; ++j)
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       int h, l;
-      split4(x[j][2 * i], x[j][2 * i + 1], up, h, l);
+      split4(x[j][2 * i], x[j][2 * i + 1], j < 2 ? up0 : up1, h, l);
       hi[2 * j + i] = h;
       lo[2 * j + i] = l;
     }
+}
+
+// The operand of mfma_fp4_fp8 from a row's dims 16 gq .. +15 and 64 + 16 gq .. +15; returns its scale byte.
+__device__ __forceinline__ u32 query_operand(const u32x4 (&x)[4], int gq, i32x8 &hi, i32x8 &lo) {
+  // Lanes gq and gq ^ 1 hold the halves of blocks gq / 2 and 2 + gq / 2.
+  auto over_pair = [](u32 v) {
+    const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    return max((u32)r[0], (u32)r[1]);
+  };
+  const QueryScale s0 = query_scale(over_pair(max(largest(x[0]), largest(x[1]))));
+  const QueryScale s1 = query_scale(over_pair(max(largest(x[2]), largest(x[3]))));
+  split32(x, s0.up, s1.up, hi, lo);
+  // Lane gq gives block gq's: lanes 0 and 3 hold theirs, 1 and 2 take them from gq ^ 2.
+  const u32 mine = gq < 2 ? s0.byte : s1.byte, give = gq < 2 ? s1.byte : s0.byte;
+  const auto r = __builtin_amdgcn_permlane32_swap(give, give, false, false);
+  return gq == 0 || gq == 3 ? mine : gq == 1 ? (u32)r[1] : (u32)r[0];
 }
 
 // Byte B of a word of scales as a float scale: one instruction (the compiler takes two for bytes 0..2).

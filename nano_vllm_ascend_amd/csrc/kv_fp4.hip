@@ -423,12 +423,12 @@ rows_fp4_kernel(NormRopeFp4Args a) {
 }
 
 // A workgroup is 8 tokens x 4 waves' heads.  A wave takes up to 8 heads; fewer where that leaves too few waves to fill the card.
-int heads_per_wave(int num_tokens, int vecs, dim3 *grid) {
+int heads_per_wave(int num_tokens, int vecs, dim3 *grid) {  // 0: more than a launch takes
   const int64_t octets = ((int64_t)num_tokens + 7) / 8;
   int per_wave = 8;
   while (per_wave > 1 && octets * ceil_div(vecs, per_wave) < kWantedWaves) per_wave >>= 1;
   *grid = dim3((unsigned)octets, (unsigned)ceil_div(ceil_div(vecs, per_wave), 4));
-  return per_wave;
+  return octets < (1 << 24) && grid->y <= 65535 ? per_wave : 0;
 }
 
 bool streams(int num_tokens, int num_kv_heads) { return (int64_t)num_tokens * num_kv_heads * kHeadDim >= kStreamElems; }
@@ -437,7 +437,7 @@ template <bool ROPE>
 int launch_rows(NormRopeFp4Args &a, hipStream_t stream) {
   dim3 grid;
   a.w.heads_per_wave = heads_per_wave(a.w.num_tokens, (ROPE ? a.num_heads : 0) + 2 * a.w.num_kv_heads, &grid);
-  if (grid.y > 65535) return NVAMD_EUNSUPPORTED;
+  if (a.w.heads_per_wave == 0) return NVAMD_EUNSUPPORTED;
   // (the rotation measured the same either way)
   if (!ROPE && streams(a.w.num_tokens, a.w.num_kv_heads))
     hipLaunchKernelGGL((rows_fp4_kernel<ROPE, !ROPE>), grid, dim3(256), 0, stream, a);
@@ -508,7 +508,7 @@ extern "C" int nvamd_kv_cache_read_fp4(void *k, int64_t k_stride, void *v, int64
   if (st != NVAMD_OK) return st;
   dim3 grid;
   const int per_wave = heads_per_wave(num_tokens, 2 * num_kv_heads, &grid);
-  if (grid.y > 65535) return NVAMD_EUNSUPPORTED;
+  if (per_wave == 0) return NVAMD_EUNSUPPORTED;
   ReadArgs a{static_cast<u16 *>(k), k_stride, static_cast<u16 *>(v), v_stride, w.cache, w.slots, w.num_slots,
              num_tokens, num_kv_heads, w.bs_log2, per_wave, w.err};
   if (streams(num_tokens, num_kv_heads))

@@ -162,12 +162,7 @@ paged_decode_fp4_kernel(DecodeFp4Args a) {
   {
     const u16 *qp = a.q + (int64_t)b * a.q_stride + (int64_t)(head0 + min(n, G - 1)) * D + 16 * gq;
     const u32x4 x[4] = {ld16(qp), ld16(qp + 8), ld16(qp + 64), ld16(qp + 72)};
-    u32 top = 0;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) top = max(top, largest(x[j]));
-    const QueryScale scale = query_scale((u32)max_over_quarters((float)top));  // 15 bits: exact
-    split32(x, scale.up, q_hi, q_lo);
-    q_scale = scale.byte;
+    q_scale = query_operand(x, gq, q_hi, q_lo);
   }
 
   // The exponent's reference, the threshold above which it moves; the sum and the numerators at that reference.

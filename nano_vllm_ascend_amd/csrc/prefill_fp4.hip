@@ -61,10 +61,10 @@ __device__ __forceinline__ bool find_rows(const PrefillFp4Args &a, int per_group
   const int s = blockIdx.z;
   r.q_start = a.cu_seqlens_q[s];
   const int q_end = a.cu_seqlens_q[s + 1];
-  const int q_len = q_end - r.q_start;
+  const int q_len = (int)((unsigned)q_end - (unsigned)r.q_start);
   const int cap = a.bt_width << a.bs_log2;
   const int kv_len = a.kv_lens[s];
-  const bool rows_in = r.q_start >= 0 && q_len >= 0 && q_end <= a.num_tokens;  // else no row is touched
+  const bool rows_in = r.q_start >= 0 && r.q_start <= q_end && q_end <= a.num_tokens;  // else no row is touched
   if ((!rows_in || q_len > a.max_q_len || kv_len > cap || kv_len < q_len) && blockIdx.x == 0 && blockIdx.y == 0 &&
       threadIdx.x == 0)
     flag_index_error(a.err, NVAMD_ERR_CONTEXT);
@@ -96,7 +96,8 @@ __device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8v, a), __builtin_bit_cast(bf16x8v, b), c, 0,
                                                  0, 0);
 }
-// 64 dims: lane (n, half) gives block `half` of them of row n; of column n, dims 16 half .. +15 and 32 + 16 half .. +15.
+// 64 dims: lane (n, half) gives block `half` of them of row n, dims 16 half .. +15 and 32 + 16 half .. +15 of column n, and the
+// scales of block `half` of either (checked on gfx950).
 __device__ __forceinline__ f32x16 mfma32_fp4_fp8(u32x4 k, u32 k_scale, i32x8 q, u32 q_scale, f32x16 c) {
   const i32x8 codes = {(int)k[0], (int)k[1], (int)k[2], (int)k[3], 0, 0, 0, 0};
   return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(codes, q, c, 4, 0, 0, (int)k_scale, 0, (int)q_scale);
@@ -135,24 +136,24 @@ prefill_fp4_kernel(PrefillFp4Args a) {
   const int n_tiles = keys > 0 ? ceil_div(keys, kBK) : 0;
 
   i32x8 q_hi[2], q_lo[2];
-  u32 q_scale;
+  u32 q_scale[2];
   {
     const int token = row / a.group, head = g * a.group + row - token * a.group;
     const u16 *qp = a.q + (int64_t)(rows.q_start + token) * a.q_stride + (int64_t)head * D + 16 * half;
-    u32x4 x[2][4];
-    u32 top = 0;
+    auto over_halves = [](u32 v) {  // each has 16 dims of a block
+      const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+      return max((u32)r[0], (u32)r[1]);
+    };
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
+      u32x4 x[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        x[s][j] = ld16(qp + 64 * s + 32 * (j >> 1) + 8 * (j & 1));
-        top = max(top, largest(x[s][j]));
-      }
+      for (int j = 0; j < 4; ++j) x[j] = ld16(qp + 64 * s + 32 * (j >> 1) + 8 * (j & 1));
+      const QueryScale s0 = query_scale(over_halves(max(largest(x[0]), largest(x[1]))));
+      const QueryScale s1 = query_scale(over_halves(max(largest(x[2]), largest(x[3]))));
+      split32(x, s0.up, s1.up, q_hi[s], q_lo[s]);
+      q_scale[s] = half ? s1.byte : s0.byte;
     }
-    const QueryScale scale = query_scale((u32)max_xor32((float)top));  // 15 bits: exact
-#pragma unroll
-    for (int s = 0; s < 2; ++s) split32(x[s], scale.up, q_hi[s], q_lo[s]);
-    q_scale = scale.byte;
   }
 
   f32x16 acc[4];
@@ -243,8 +244,8 @@ prefill_fp4_kernel(PrefillFp4Args a) {
     for (int i = 0; i < 16; ++i) sc[i] = 0.f;
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
-      sc = mfma32_fp4_fp8(kc[s], ks[s], q_hi[s], q_scale, sc);
-      sc = mfma32_fp4_fp8(kc[s], ks[s], q_lo[s], q_scale, sc);
+      sc = mfma32_fp4_fp8(kc[s], ks[s], q_hi[s], q_scale[s], sc);
+      sc = mfma32_fp4_fp8(kc[s], ks[s], q_lo[s], q_scale[s], sc);
     }
   };
   auto weigh = [&](int t, const Stage &st) {
@@ -397,12 +398,7 @@ prefill_few_fp4_kernel(PrefillFp4Args a) {
   {
     const u16 *qp = a.q + (int64_t)(rows.q_start + token) * a.q_stride + (int64_t)head * D + 16 * gq;
     const u32x4 x[4] = {ld16(qp), ld16(qp + 8), ld16(qp + 64), ld16(qp + 72)};
-    u32 top = 0;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) top = max(top, largest(x[j]));
-    const QueryScale scale = query_scale((u32)max_over_quarters((float)top));
-    split32(x, scale.up, q_hi, q_lo);
-    q_scale = scale.byte;
+    q_scale = query_operand(x, gq, q_hi, q_lo);
   }
 
   float m = kNoScore, m_thr = kNoScore, l = 0.f;
@@ -579,7 +575,7 @@ extern "C" int nvamd_paged_prefill_fp4(void *out, int64_t out_stride, const void
       !aligned16(out) || q_stride % 8 || out_stride % 8 || q_stride < (int64_t)num_heads * head_dim ||
       out_stride < (int64_t)num_heads * head_dim)
     return NVAMD_EINVAL;
-  if (((int64_t)bt_width << bs_log2) > 0x7fffffff || (((int64_t)num_blocks * num_kv_heads) << bs_log2) >> 4 > 0x7fffffff)
+  if (((int64_t)bt_width << bs_log2) > 1 << 30 || (((int64_t)num_blocks * num_kv_heads) << bs_log2) >> 4 > 0x7fffffff)
     return NVAMD_EUNSUPPORTED;
   PrefillFp4Args a = {};
   a.out = static_cast<u16 *>(out);

@@ -85,11 +85,17 @@ class HipPagedAttention(nn.Module):
         self.scale = head_dim ** -0.5
         self._workspace: torch.Tensor | None = None
         self._ws_key = (0, 0)
+        self._outgrown: list[torch.Tensor] = []
 
     def workspace(self, batch: int, max_context_len: int, device) -> torch.Tensor:
-        """A zero-filled split-KV workspace large enough for (batch, max_context_len); grows on demand."""
+        """A zero-filled split-KV workspace large enough for (batch, max_context_len); grows on demand.  Calls that use
+        it must not overlap: give those of other streams, and of graphs that run beside others, one of their own.
+        One that was outgrown is kept, since a captured graph may still use it."""
         b, c = self._ws_key
         if self._workspace is None or batch > b or max_context_len > c or self._workspace.device != device:
+            if self._workspace is not None:  # powers of two from here on: few are outgrown
+                self._outgrown.append(self._workspace)
+                b, c = (max(old, 1 << (new - 1).bit_length()) for old, new in ((b, batch), (c, max_context_len)))
             b, c = max(batch, b), max(max_context_len, c)
             self._workspace = _C.alloc_paged_decode_workspace(b, self.num_heads, self.num_key_value_heads, c, device)
             self._ws_key = (b, c)

@@ -104,6 +104,8 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: float) -
       scores: 128 products and sums of 2^-24 of sum |q k| each, the product with the scale and the exponential's argument
         some 2^-22 of the largest score: an exponent off by d scales every weight by at most e^d, numerator and sum
         alike:                                                                    2 * (e^d - 1) * A
+      queries: of a block of 32 dims the values below 2^-9 of its largest are off by at most 2^-17 of that, which adds
+        2^-17 max |q| sum |k| over them to the error of a score
       result:                                                                     2^-8 * (|out| + the above)
     Rows that see no key are zero."""
     n, hq, _ = q.shape
@@ -122,7 +124,9 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: float) -
         out[:, h] = torch.where(hit > 0, math.nan, out[:, h])
         a = p.nan_to_num(0.0) @ vv.nan_to_num(0.0, 0.0, 0.0).abs()
         mass = (qq.abs() @ kk.nan_to_num(0.0).abs().T * abs(scale)).amax(-1, keepdim=True)
-        d = 2.0 * (130 * 2.0 ** -24 * mass + 2.0 ** -22 * mass)
+        top = qq.abs().unflatten(-1, (4, 32)).amax(-1, keepdim=True).expand(-1, -1, 32).flatten(1)
+        lost = torch.where(qq.abs() < 2.0 ** -9 * top, 2.0 ** -17 * top, 0.0) @ kk.nan_to_num(0.0).abs().T * abs(scale)
+        d = 2.0 * (130 * 2.0 ** -24 * mass + 2.0 ** -22 * mass + lost.amax(-1, keepdim=True))
         part = (2 * 2.0 ** -8 + 2 * torch.expm1(d)) * a
         tol[:, h] = part + 2.0 ** -8 * (out[:, h].abs() + part) + 1e-30
     return out, tol

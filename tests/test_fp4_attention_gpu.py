@@ -146,6 +146,128 @@ def test_decode_scores_far_apart(device):
     check_decode(batch, q, batch.decode(q, scale=-0.05), scale=-0.05)
 
 
+def outliers(q):
+    """A dim that is thousands of times the others, as some heads have."""
+    q = q.clone()
+    q[..., 5] *= 4000
+    q[..., 100] *= 70
+    return q
+
+
+def test_decode_queries_with_outliers(device):
+    """Keys without the outliers' dims: the scores come from what is left of the query."""
+    batch = Batch(device, [900, 70], 4, 1, 64, seed=16)
+    slots = torch.cat(batch.slots)
+    k, v = fp4_ref.read(batch.pages, slots)
+    k[..., 5] = k[..., 100] = 0
+    fp4_ref.write(batch.pages, k.bfloat16(), v.bfloat16(), slots)
+    batch.upload()
+    q = outliers(batch.queries(2))
+    check_decode(batch, q, batch.decode(q))
+
+
+def test_decode_scores_below_any_reference(device):
+    """Scores of about -1e31, all alike: every key weighs the same."""
+    batch = Batch(device, [700, 40], 2, 1, 16, seed=17)
+    slots = torch.cat(batch.slots)
+    _, v = fp4_ref.read(batch.pages, slots)
+    fp4_ref.write(batch.pages, torch.full((len(slots), 1, 128), -(2.0 ** 50)).bfloat16(), v.bfloat16(), slots)
+    batch.upload()
+    q = torch.full((2, 2, 128), 2.0 ** 50).bfloat16()
+    got = batch.decode(q).cpu().double()
+    for i, at in enumerate(batch.slots):
+        _, v = fp4_ref.read(batch.pages, at)
+        # equal weights are exact; 32-bit sums of up to 700 values, and one rounding
+        tol = 2.0 ** -8 * v.mean(0).abs() + 1e-4 * v.abs().mean(0)
+        assert ((got[i] - v.mean(0)).abs() <= tol).all()
+
+
+def test_decode_replays_from_a_graph(device):
+    """Contexts, tables and queries that change between the replays of a captured call."""
+    batch = Batch(device, [1500, 33, 700], 4, 2, 16, seed=18)
+    q = batch.queries(3).to(device)
+    lens, tables = torch.tensor(batch.lens, dtype=torch.int32, device=device), batch.tables.to(device)
+    out = torch.empty_like(q)
+    spaces = [_C.alloc_paged_decode_workspace(3, 4, 2, 1500, device) for _ in range(2)]
+
+    def call(out, space):
+        return _C.paged_decode_fp4(out, q, batch.keys, batch.values, tables, lens, SCALE, 1500, space)
+
+    call(out, spaces[0])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call(out, spaces[0])
+    for now in ([1500, 33, 700], [3, 0, 64], [512, 1, 1], [1400, 20, 513]):
+        q.copy_(batch.queries(3))
+        lens.copy_(torch.tensor(now, dtype=torch.int32))
+        for _ in range(2):
+            out.fill_(7.0)
+            graph.replay()
+            got = out.clone()
+            torch.cuda.synchronize()
+            assert torch.equal(got, call(torch.empty_like(q), spaces[1]))
+        batch.lens, full, slots = now, batch.lens, batch.slots
+        batch.slots = [s[:n] for s, n in zip(slots, now)]
+        check_decode(batch, q.cpu(), got)
+        batch.lens, batch.slots = full, slots
+
+
+def test_decode_layer_keeps_a_captured_workspace(device):
+    """A graph captured at a small batch replays right after the layer has served a larger one."""
+    batch = Batch(device, [2000, 33, 700, 1100], 4, 2, 16, seed=19)
+    layer = HipPagedAttention(4, 2, 128)
+    lens, tables = torch.tensor(batch.lens, dtype=torch.int32, device=device), batch.tables.to(device)
+    q = batch.queries(4).to(device)
+    out = torch.empty_like(q)
+
+    def call(n, out=None):
+        return layer(q[:n], batch.keys, batch.values, tables[:n], lens[:n], max_context_len=2000, out=out)
+
+    call(1)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call(1, out[:1])
+    for _ in range(3):
+        whole = call(4)
+        junk = [torch.full((1 << 20,), 255, dtype=torch.uint8, device=device) for _ in range(4)]  # takes what was freed
+        out.fill_(7.0)
+        graph.replay()
+        close(out[:1], *batch.want(0, q[:1].cpu()))
+        assert out[1:].eq(7).all()
+        del junk
+    check_decode(batch, q.cpu(), whole)
+
+
+def test_pages_past_32_bits(device):
+    """Pages whose codes lie past 4 GiB, and rows of them written, read and attended to."""
+    nb, bs, hkv = 4200, 256, 64
+    cache = Fp4PagedKVCache(1, nb, bs, hkv, 128, device)
+    assert cache.key_codes.nbytes > 1 << 32
+    gen = torch.Generator().manual_seed(20)
+    pages = torch.tensor([nb - 1, 0, nb // 2])
+    n = 600
+    slots = pages[torch.arange(n) // bs] * bs + torch.arange(n) % bs
+    k, v = (torch.randn(n, hkv, 128, generator=gen).bfloat16() for _ in range(2))
+    cache.write(0, k.to(device), v.to(device), slots.to(device))
+    small = fp4_ref.empty_pages(3, hkv, bs)
+    fp4_ref.write(small, k, v, torch.arange(n))
+    kk, vv = fp4_ref.read(small, torch.arange(n))
+    got = cache.read(0, slots.to(device))
+    assert torch.equal(got[0].cpu().double(), kk) and torch.equal(got[1].cpu().double(), vv)
+    q = torch.randn(n, hkv, 128, generator=gen).bfloat16()
+    tables = pages.to(torch.int32)[None].to(device)
+    lens = torch.tensor([n], dtype=torch.int32, device=device)
+    keys, values = cache.get_physical_cache(0)
+    for rows in (1, 20, 300):
+        want, tol = fp4_ref.attention(q[:rows], kk, vv, SCALE)
+        cu = torch.tensor([0, rows], dtype=torch.int32, device=device)
+        out = torch.empty(rows, hkv, 128, dtype=torch.bfloat16, device=device)
+        close(_C.paged_prefill_fp4(out, q[:rows].to(device), keys, values, tables, cu, lens, rows, SCALE), want, tol)
+    want, tol = fp4_ref.attention(q[:1], kk, vv, SCALE)
+    space = _C.alloc_paged_decode_workspace(1, hkv, hkv, n, device)
+    close(_C.paged_decode_fp4(out[:1], q[:1].to(device), keys, values, tables, lens, SCALE, n, space), want, tol)
+
+
 def test_decode_nan_reaches_only_its_sequence_and_dims(device):
     batch = Batch(device, [200, 300, 100], 2, 1, 32, seed=7)
     v = torch.ones(1, 1, 128, dtype=torch.bfloat16)
@@ -286,6 +408,18 @@ def test_prefill_scores_far_apart(device, bound):
     batch = Batch(device, [400, 90], 2, 1, 16, seed=3, spread=1.5)
     q = batch.queries(300 + 90, scale=8.0)
     check_prefill(batch, q, [300, 90], batch.prefill(q, [300, 90], max_q=bound))
+
+
+@BOUNDS
+def test_prefill_queries_with_outliers(device, bound):
+    batch = Batch(device, [300, 70], 4, 1, 64, seed=15)
+    slots = torch.cat(batch.slots)
+    k, v = fp4_ref.read(batch.pages, slots)
+    k[..., 5] = k[..., 100] = 0
+    fp4_ref.write(batch.pages, k.bfloat16(), v.bfloat16(), slots)
+    batch.upload()
+    q = outliers(batch.queries(150))
+    check_prefill(batch, q, [100, 50], batch.prefill(q, [100, 50], max_q=bound))
 
 
 @BOUNDS

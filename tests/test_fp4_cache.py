@@ -104,6 +104,7 @@ def test_write_and_read_argument_errors():
             assert call(**{name: 0}) == EINVAL and call(**{name: A + 8}) == EINVAL, name
         assert call(slots=0) == EINVAL
         assert call(k_stride=1016) == EINVAL and call(v_stride=1028) == EINVAL
+        assert call(t=1 << 27) == EUNSUPPORTED and call(t=2 ** 31 - 1) == EUNSUPPORTED
 
 
 def test_norm_rope_argument_errors():
@@ -164,6 +165,7 @@ def test_prefill_argument_errors():
     assert call(hq=12) == EINVAL and call(n=65536) == EINVAL and call(bt_width=16) == EINVAL
     assert call(d=64) == EUNSUPPORTED and call(bs=8) == EUNSUPPORTED
     assert call(bt_width=1 << 25, bt_stride=1 << 25) == EUNSUPPORTED
+    assert call(bt_width=(1 << 23) + 1, bt_stride=1 << 25) == EUNSUPPORTED  # past 2^30 tokens
 
 
 # -------------------------------------------------------------------------------------------- Python entry points
