@@ -1,11 +1,15 @@
 // The 4-bit paged KV cache: writing rows, reading rows back, and the per-head QK-RMSNorm + RoPE that
 // writes them in the same pass (the 4-bit counterparts of kv_store.hip).
 //
-// The writing kernels give a wave 8 consecutive tokens, an aligned group of 8 lanes each, and a run of their heads one
-// after another: the rotation's table row, the weights and the slots are read once for the run, rows of a head that
+// A wave takes 8 consecutive tokens, an aligned group of 8 lanes each, and one head or a run of them: rows of a head that
 // follow one another in a page are written together, and the 8 tokens of a head's values meet in LDS so that bytes of
-// consecutive tokens leave as one store.  Of a head vector, lane c of a group holds dims 8c..8c+7 and 64+8c..64+8c+7: a block of
-// 32 dims is the low (or high) half of 4 consecutive lanes, its maximum two DPP steps away, and RoPE needs no lane exchange.
+// consecutive tokens leave as one store.  Of a head vector, lane c of a group holds dims 8c..8c+7 and 64+8c..64+8c+7: a block
+// of 32 dims is the low (or high) half of 4 consecutive lanes, its maximum two DPP steps away, and RoPE needs no lane
+// exchange.
+//
+// All three are bound by memory: per head vector 256 bytes of bf16 and 68 of the cache, once.  36,488 tokens, 8 kv heads (and 16
+// query heads): write 189 MB in 40 us (4.7 TB/s), read 189 MB in 38 us (5.0 TB/s), norm + RoPE + write with the keys
+// returned 564 MB in 118 us (4.8 TB/s); a large copy reaches 5.0 TB/s.  One token: 3 us, the launch.
 #include "fp4.h"
 
 namespace nvamd {
@@ -133,8 +137,8 @@ __device__ __forceinline__ void store_values(const Fp4Cache &cache, const u8 *ti
 __device__ __forceinline__ void wave_lds_fence() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); }
 
 // Rows too many for the caches until their next use go past them (32 MB a tensor: half of the 256 MB Infinity Cache for two
-// tensors in and out).  36,488 x 8 heads, plain / nontemporal: written from nontemporal loads 53.5 / 49 us, read back with
-// nontemporal stores 66 / 58.6; 12,345 x 8 heads both together 28.2 / 31.1.
+// tensors in and out).  36,488 x 8 heads, plain / nontemporal: written 43.8 / 39.2 us, read 46.5 / 38.2; 12,345 x 8 heads
+// written and read back 27.6 / 31.9.
 constexpr int64_t kStreamElems = 16 << 20;
 template <bool STREAM>
 __device__ __forceinline__ void put16(u16 *p, u32x4 v) {
@@ -149,7 +153,11 @@ __device__ __forceinline__ u32x4 get16(const u16 *p) {
   else return ld16(p);
 }
 
-constexpr int kWantedWaves = 4096;  // four waves on each SIMD of 256 CUs
+// Heads that a wave of the rotation takes one after another: the table's row, the weights and the slots are read once for
+// them.  Fewer where that leaves less than four waves for each SIMD of 256 CUs.  (36,488 tokens: 118 us with 8 or 4, 142 with 2.)
+// Without the rotation a wave has one head (8: 42.2 us, 1: 40.1; 12,345 tokens 17.6, 16.7).
+constexpr int kRopeHeads = 8;
+constexpr int kWantedWaves = 4096;
 
 struct WriteArgs {
   const u16 *k;
@@ -177,89 +185,83 @@ struct ReadArgs {
   int num_tokens;
   int num_kv_heads;
   int bs_log2;
-  int heads_per_wave;
   u32 *err;
 };
 
-// As the writes, the other way round: a wave takes 8 tokens and a run of their key and value heads.  A row without a slot, or
-// with one outside the cache, is zeros.
+// The other way round.  A wave takes one key or value head of 8 tokens: it waits for its loads once, and more waves are all
+// that hides that (36,488 x 8 heads: 50 us with 8 heads one after another, 45 with 2, 37.4 so).  A row without a slot, or with one
+// outside the cache, is zeros.
 template <bool STREAM>
 __global__ void __launch_bounds__(256)
 kv_read_fp4_kernel(ReadArgs a) {
-  __shared__ __attribute__((aligned(16))) u8 s_tile[4][2][512];
+  __shared__ __attribute__((aligned(16))) u8 s_tile[4][512];
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int c = lane & 7, tok = lane >> 3;
   const int hkv = a.num_kv_heads;
-  const int h_begin = (blockIdx.y * 4 + w) * a.heads_per_wave;
-  const int h_end = min(h_begin + a.heads_per_wave, 2 * hkv);
-  if (h_begin >= h_end) return;
+  const int v = blockIdx.y * 4 + w;  // key heads, then value heads
+  if (v >= 2 * hkv) return;
   const int t = blockIdx.x * 8 + tok;
   const bool exists = t < a.num_tokens;
   int64_t slot = exists ? a.slots[t] : -1;
   if (slot >= a.num_slots || slot < -1) {
-    if (h_begin == 0 && c == 0) flag_index_error(a.err, NVAMD_ERR_SLOT);
+    if (v == 0 && c == 0) flag_index_error(a.err, NVAMD_ERR_SLOT);
     slot = -1;
   }
   const bool live = slot >= 0;
-  const bool run = __all(live && slot == uniform64(slot) + tok);
+  const int h = v < hkv ? v : v - hkv;
+  const Fp4Row r = row_at(live ? slot : 0, h, hkv, a.bs_log2);
   const u32x4 zero = {0u, 0u, 0u, 0u};
-#pragma unroll 1
-  for (int v = h_begin; v < h_end; ++v) {
-    const int h = v < hkv ? v : v - hkv;
-    const Fp4Row r = row_at(live ? slot : 0, h, hkv, a.bs_log2);
-    if (v < hkv) {
-      u32x4 lo = zero, hi = zero;
-      if (live) {
-        const u32 *row = reinterpret_cast<const u32 *>(a.cache.k_codes + r.tile * kFp4TileBytes + r.t * kFp4RowBytes);
-        const u8 *s = a.cache.k_scales + r.tile * kFp4TileScales;
-        lo = fp4_values(row[c], fp4_scale(s[fp4_key_scale_at(r.t, c >> 2)]));
-        hi = fp4_values(row[8 + c], fp4_scale(s[fp4_key_scale_at(r.t, 2 + (c >> 2))]));
-      }
-      if (exists) {
-        u16 *dst = a.k + t * a.k_stride + h * kHeadDim + 8 * c;
-        put16<STREAM>(dst, lo);
-        put16<STREAM>(dst + 64, hi);
-      }
-      continue;
-    }
-    // Row byte `lane` of the 8 tokens, then through LDS to lane c of each: bytes 8 (c % 2) .. +7 of block c / 2.
-    auto place = [&](int64_t s) {
-      const Fp4Row x = row_at(s, h, hkv, a.bs_log2);
-      return a.cache.v_codes + x.tile * kFp4TileBytes + lane * kFp4Tile + x.t;
-    };
-    u8 *tile = s_tile[w][v & 1];
-    uint64_t bytes = 0;
-    if (run) {
-      const int64_t s0 = uniform64(slot);
-      const int o = (int)(s0 & 7);
-      const u8 *first = place(s0) - o;
-      bytes = *reinterpret_cast<const uint64_t *>(first);
-      if (o != 0) bytes = (bytes >> (8 * o)) | (*reinterpret_cast<const uint64_t *>(place(s0 + 8 - o)) << (64 - 8 * o));
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int64_t s = lane_value(slot, 8 * i);
-        if (s >= 0) bytes |= (uint64_t)*place(s) << (8 * i);
-      }
-    }
-    *reinterpret_cast<uint64_t *>(tile + lane * 8) = bytes;
-    wave_lds_fence();
-    u32x4 first = zero, last = zero;
+  if (v < hkv) {
+    u32x4 lo = zero, hi = zero;
     if (live) {
-      const u8 *p = tile + (16 * (c >> 1) + 8 * (c & 1)) * 8 + tok;
-      const float scale = fp4_scale(a.cache.v_scales[r.tile * kFp4TileScales + fp4_value_scale_at(r.t, c >> 1)]);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const u32 x = fp4_pair<0>(p[2 * j * 8], scale), y = fp4_pair<0>(p[(2 * j + 1) * 8], scale);
-        first[j] = pair_lo(x, y);
-        last[j] = pair_hi(x, y);
-      }
+      const u32 *row = reinterpret_cast<const u32 *>(a.cache.k_codes + r.tile * kFp4TileBytes + r.t * kFp4RowBytes);
+      const u8 *s = a.cache.k_scales + r.tile * kFp4TileScales;
+      lo = fp4_values(row[c], fp4_scale(s[fp4_key_scale_at(r.t, c >> 2)]));
+      hi = fp4_values(row[8 + c], fp4_scale(s[fp4_key_scale_at(r.t, 2 + (c >> 2))]));
     }
     if (exists) {
-      u16 *dst = a.v + t * a.v_stride + h * kHeadDim + 32 * (c >> 1) + 8 * (c & 1);
-      put16<STREAM>(dst, first);
-      put16<STREAM>(dst + 16, last);
+      u16 *dst = a.k + t * a.k_stride + h * kHeadDim + 8 * c;
+      put16<STREAM>(dst, lo);
+      put16<STREAM>(dst + 64, hi);
     }
+    return;
+  }
+  // Row byte `lane` of the 8 tokens, then through LDS to lane c of each: bytes 8 (c % 2) .. +7 of block c / 2.
+  auto place = [&](int64_t s) {
+    const Fp4Row x = row_at(s, h, hkv, a.bs_log2);
+    return a.cache.v_codes + x.tile * kFp4TileBytes + lane * kFp4Tile + x.t;
+  };
+  u8 *tile = s_tile[w];
+  uint64_t bytes = 0;
+  if (__all(live && slot == uniform64(slot) + tok)) {
+    const int64_t s0 = uniform64(slot);
+    const int o = (int)(s0 & 7);
+    bytes = *reinterpret_cast<const uint64_t *>(place(s0) - o);
+    if (o != 0) bytes = (bytes >> (8 * o)) | (*reinterpret_cast<const uint64_t *>(place(s0 + 8 - o)) << (64 - 8 * o));
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int64_t s = lane_value(slot, 8 * i);
+      if (s >= 0) bytes |= (uint64_t)*place(s) << (8 * i);
+    }
+  }
+  *reinterpret_cast<uint64_t *>(tile + lane * 8) = bytes;
+  wave_lds_fence();
+  u32x4 first = zero, last = zero;
+  if (live) {
+    const u8 *p = tile + (16 * (c >> 1) + 8 * (c & 1)) * 8 + tok;
+    const float scale = fp4_scale(a.cache.v_scales[r.tile * kFp4TileScales + fp4_value_scale_at(r.t, c >> 1)]);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const u32 x = fp4_pair<0>(p[2 * j * 8], scale), y = fp4_pair<0>(p[(2 * j + 1) * 8], scale);
+      first[j] = pair_lo(x, y);
+      last[j] = pair_hi(x, y);
+    }
+  }
+  if (exists) {
+    u16 *dst = a.v + t * a.v_stride + h * kHeadDim + 32 * (c >> 1) + 8 * (c & 1);
+    put16<STREAM>(dst, first);
+    put16<STREAM>(dst + 16, last);
   }
 }
 
@@ -422,10 +424,10 @@ rows_fp4_kernel(NormRopeFp4Args a) {
   }
 }
 
-// A workgroup is 8 tokens x 4 waves' heads.  A wave takes up to 8 heads; fewer where that leaves too few waves to fill the card.
-int heads_per_wave(int num_tokens, int vecs, dim3 *grid) {  // 0: more than a launch takes
+// A workgroup is 8 tokens x 4 waves' heads.  A wave takes up to `per_wave` heads; fewer where that leaves too few waves to fill
+// the card.  0: more than a launch takes.
+int heads_per_wave(int num_tokens, int vecs, int per_wave, dim3 *grid) {
   const int64_t octets = ((int64_t)num_tokens + 7) / 8;
-  int per_wave = 8;
   while (per_wave > 1 && octets * ceil_div(vecs, per_wave) < kWantedWaves) per_wave >>= 1;
   *grid = dim3((unsigned)octets, (unsigned)ceil_div(ceil_div(vecs, per_wave), 4));
   return octets < (1 << 24) && grid->y <= 65535 ? per_wave : 0;
@@ -436,7 +438,8 @@ bool streams(int num_tokens, int num_kv_heads) { return (int64_t)num_tokens * nu
 template <bool ROPE>
 int launch_rows(NormRopeFp4Args &a, hipStream_t stream) {
   dim3 grid;
-  a.w.heads_per_wave = heads_per_wave(a.w.num_tokens, (ROPE ? a.num_heads : 0) + 2 * a.w.num_kv_heads, &grid);
+  a.w.heads_per_wave = heads_per_wave(a.w.num_tokens, (ROPE ? a.num_heads : 0) + 2 * a.w.num_kv_heads,
+                                      ROPE ? kRopeHeads : 1, &grid);
   if (a.w.heads_per_wave == 0) return NVAMD_EUNSUPPORTED;
   // (the rotation measured the same either way)
   if (!ROPE && streams(a.w.num_tokens, a.w.num_kv_heads))
@@ -507,10 +510,9 @@ extern "C" int nvamd_kv_cache_read_fp4(void *k, int64_t k_stride, void *v, int64
                                  num_kv_heads, head_dim, num_blocks, block_size);
   if (st != NVAMD_OK) return st;
   dim3 grid;
-  const int per_wave = heads_per_wave(num_tokens, 2 * num_kv_heads, &grid);
-  if (per_wave == 0) return NVAMD_EUNSUPPORTED;
+  if (heads_per_wave(num_tokens, 2 * num_kv_heads, 1, &grid) == 0) return NVAMD_EUNSUPPORTED;
   ReadArgs a{static_cast<u16 *>(k), k_stride, static_cast<u16 *>(v), v_stride, w.cache, w.slots, w.num_slots,
-             num_tokens, num_kv_heads, w.bs_log2, per_wave, w.err};
+             num_tokens, num_kv_heads, w.bs_log2, w.err};
   if (streams(num_tokens, num_kv_heads))
     hipLaunchKernelGGL((kv_read_fp4_kernel<true>), grid, dim3(256), 0, stream, a);
   else
