@@ -30,10 +30,11 @@ typedef int i32x8 __attribute__((ext_vector_type(8)));
 
 // S += K . q for 16 rows of codes (128 dims) and 16 columns of e4m3, each block of 32 dims under its scale byte.  Lane (row
 // or column n, gq) gives block gq of its row, dims 16 gq .. +15 and 64 + 16 gq .. +15 of its column, and the scales of
-// block gq of either (checked on gfx950).
-__device__ __forceinline__ f32x4 mfma_fp4_fp8(u32x4 k, u32 k_scale, i32x8 q, u32 q_scale, f32x4 c) {
+// block gq of either, the row's in byte B of a word (checked on gfx950).
+template <int B>
+__device__ __forceinline__ f32x4 mfma_fp4_fp8(u32x4 k, u32 k_scales, i32x8 q, u32 q_scale, f32x4 c) {
   const i32x8 codes = {(int)k[0], (int)k[1], (int)k[2], (int)k[3], 0, 0, 0, 0};
-  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(codes, q, c, 4, 0, 0, (int)k_scale, 0, (int)q_scale);
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(codes, q, c, 4, 0, B, (int)k_scales, 0, (int)q_scale);
 }
 
 // A block of 32 bf16 query values as hi + lo in e4m3 under 2^-s, s from its largest value, which lands in [128, 256).  hi
@@ -94,6 +95,12 @@ __device__ __forceinline__ u32 query_operand(const u32x4 (&x)[4], int gq, i32x8 
   const u32 mine = gq < 2 ? s0.byte : s1.byte, give = gq < 2 ? s1.byte : s0.byte;
   const auto r = __builtin_amdgcn_permlane32_swap(give, give, false, false);
   return gq == 0 || gq == 3 ? mine : gq == 1 ? (u32)r[1] : (u32)r[0];
+}
+
+template <int B>
+__device__ __forceinline__ void score(f32x4 &s, u32x4 k, u32 k_scales, i32x8 q_hi, i32x8 q_lo, u32 q_scale) {
+  s = mfma_fp4_fp8<B>(k, k_scales, q_hi, q_scale, f32x4{0.f, 0.f, 0.f, 0.f});
+  s = mfma_fp4_fp8<B>(k, k_scales, q_lo, q_scale, s);
 }
 
 // Byte B of a word of scales as a float scale: one instruction (the compiler takes two for bytes 0..2).

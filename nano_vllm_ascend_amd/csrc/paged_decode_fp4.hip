@@ -231,12 +231,10 @@ paged_decode_fp4_kernel(DecodeFp4Args a) {
   auto step = [&](const int t0, const int next) {
     constexpr int NP = GP <= 4 ? 1 : GP <= 8 ? 2 : 4;  // accumulators that hold all scores once packed
     f32x4 s[4];
-    const u32 k_scale[4] = {ks & 0xffu, (ks >> 8) & 0xffu, (ks >> 16) & 0xffu, ks >> 24};
-#pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      s[t] = mfma_fp4_fp8(kc[t], k_scale[t], q_hi, q_scale, f32x4{0.f, 0.f, 0.f, 0.f});
-      s[t] = mfma_fp4_fp8(kc[t], k_scale[t], q_lo, q_scale, s[t]);
-    }
+    score<0>(s[0], kc[0], ks, q_hi, q_lo, q_scale);
+    score<1>(s[1], kc[1], ks, q_hi, q_lo, q_scale);
+    score<2>(s[2], kc[2], ks, q_hi, q_lo, q_scale);
+    score<3>(s[3], kc[3], ks, q_hi, q_lo, q_scale);
     __builtin_amdgcn_sched_barrier(0);
     if (next < t_end) {
       locate(next);

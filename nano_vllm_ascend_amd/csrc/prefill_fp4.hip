@@ -2,21 +2,29 @@
 // the last q_len positions of a context of kv_len, query row r sees keys 0 .. kv_len - q_len + r, all of them in the cache.
 //
 // The G query heads of a kv head and the q_len tokens make q_len * G rows, R = token * G + head, that share the keys; a
-// workgroup takes rows that follow one another, whatever G is.  Two kernels:
+// workgroup takes rows that follow one another, whatever G is.  In all kernels
+//   S^T = K . Q^T   v_mfma_scale_f32_*_f8f6f4 on the codes as they lie in the cache: a lane loads 32 dims of a key and their
+//        scale straight into the operand, and the row comes as two e4m3 numbers per value (fp4_attention.h).  No expansion
+//        of K, and none of it in LDS;
+//   O^T += V^T . P^T   v_mfma_f32_*_bf16 on V expanded by v_cvt_scalef32_pk_bf16_fp4, exact.
+// The rows of K are taken in such an order that a lane's registers of S^T are the consecutive keys that its operand of P^T
+// needs: a repack in registers.  Three kernels, which differ in how many rows share an expansion of V:
 //
-// Tiles (many rows).  Workgroup = 4 waves = 128 rows, a wave 32 of them; per tile of 32 keys
-//   S^T[32 keys x 32 rows] = K . Q^T   v_mfma_scale_f32_32x32x64_f8f6f4 on the codes as they lie in the cache: a lane loads 32
-//        dims of a key and their scale straight into the operand, and the row comes as two e4m3 numbers per value
-//        (fp4_attention.h).  No expansion of K, and none of it in LDS, whose bandwidth V alone takes half of;
-//   O^T[128 dims x 32 rows] += V^T . P^T   v_mfma_f32_32x32x16_bf16.  The workgroup expands a tile of V once, to bf16 operands
-//        in LDS (every access is 64 lanes x 16 consecutive bytes): a wave takes 8 tokens of a 16-token tile, a lane a dim
-//        pair of them.  The accumulator of S^T holds its rows in the order 8 (i / 4) + 4 half + i % 4, so key 16a + 8b + 4c + x sits in
-//        row 16a + 8c + 4b + x of K: then a lane's registers are 8 consecutive keys, and P^T a repack in registers.
-//   K of the next tile loads as the scores have taken this one's, V's codes are two tiles ahead, V's operands one (two stages, one
-//   barrier a tile).
+// Tiles (the card is full).  Workgroup = 4 waves = 128 rows, a wave 32 of them, tiles of 32 keys.  The workgroup expands a
+//   tile of V once, to bf16 operands in LDS (every access is 64 lanes x 16 consecutive bytes): a wave takes 8 tokens of a
+//   16-token tile, a lane a dim pair of them.  Key 16a + 8b + 4c + x sits in row 16a + 8c + 4b + x of K.  K of the next tile
+//   loads as the scores have taken this one's, V's codes are two tiles ahead, V's operands one (two stages, one barrier a tile).
+//   Bound by issue: the matrix cores are busy 43.5% of the time and the vector ALUs (exponents, rounding, expansion) 55%, one or
+//   the other at 98.5% of it.  32 x U[512, 2048] rows on 1,152 cached keys 689 us (895 TFLOP/s), 2 x U[3000, 4000] rows of 40
+//   query heads on 4,096 972 us (1,022 TFLOP/s); a bf16 matrix product of 8,192^3 reaches 1,254.
 //
-// Few rows (a chat's next turn: nothing else would fill the card).  Workgroup = 8 waves = 16 rows, a wave every eighth 64 keys,
-// as in paged_decode_fp4.hip with rows in the place of heads and a last key for each row; the waves' results meet in LDS.
+// Strips (one long prompt, or several short ones).  Workgroup = 4 waves = 32 rows, a wave every fourth 32 keys; no barrier in the
+//   loop, the waves' results meet in LDS.  A lane expands 16 tokens of a dim pair straight into operands: four times the
+//   tile kernel's expansion for each row, for four times the workgroups.  1 x 4,000 rows on 4,096 keys 232 us (859 TFLOP/s).
+//
+// Few rows (a chat's next turn).  Workgroup = 8 waves = 16 rows, a wave every eighth 64 keys, as in paged_decode_fp4.hip with rows
+//   in the place of heads and a last key for each row.  Bound by the latency of a wave's steps: 1 x 20 rows on 4,096 keys
+//   20 us.
 //
 // A block of values that reads as NaN must reach the rows that see its key and no others, though masked rows
 // multiply it by a weight of zero: such values enter the products as zeros, and the rows that see
@@ -103,6 +111,28 @@ __device__ __forceinline__ f32x16 mfma32_fp4_fp8(u32x4 k, u32 k_scale, i32x8 q, 
   return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(codes, q, c, 4, 0, 0, (int)k_scale, 0, (int)q_scale);
 }
 
+// A row's operands: dims 64 s + 16 half .. +15 and 64 s + 32 + 16 half .. +15, the scales of block 2 s + half.
+__device__ __forceinline__ void load_query(const PrefillFp4Args &a, const Rows &rows, int row, int g, int half,
+                                           i32x8 (&hi)[2], i32x8 (&lo)[2], u32 (&scale)[2]) {
+  const int token = row / a.group, head = g * a.group + row - token * a.group;
+  const u16 *qp = a.q + (int64_t)(rows.q_start + token) * a.q_stride + (int64_t)head * kHeadDim + 16 * half;
+  auto over_halves = [](u32 v) {  // each has 16 dims of a block
+    const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return max((u32)r[0], (u32)r[1]);
+  };
+#pragma unroll
+  for (int s = 0; s < 2; ++s) {
+    u32x4 x[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x[j] = ld16(qp + 64 * s + 32 * (j >> 1) + 8 * (j & 1));
+    const QueryScale s0 = query_scale(over_halves(max(largest(x[0]), largest(x[1]))));
+    const QueryScale s1 = query_scale(over_halves(max(largest(x[2]), largest(x[3]))));
+    split32(x, s0.up, s1.up, hi[s], lo[s]);
+    scale[s] = half ? s1.byte : s0.byte;
+  }
+}
+typedef const __attribute__((address_space(4))) int32_t const_i32;  // block tables: nothing writes them, scalar loads
+
 struct Stage {
   u32x4 v[2][4][64];  // [16-key step][32-dim block][lane]
   u32 any[4];         // [wave that expanded them]: whether any of its values read as NaN,
@@ -137,24 +167,7 @@ prefill_fp4_kernel(PrefillFp4Args a) {
 
   i32x8 q_hi[2], q_lo[2];
   u32 q_scale[2];
-  {
-    const int token = row / a.group, head = g * a.group + row - token * a.group;
-    const u16 *qp = a.q + (int64_t)(rows.q_start + token) * a.q_stride + (int64_t)head * D + 16 * half;
-    auto over_halves = [](u32 v) {  // each has 16 dims of a block
-      const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
-      return max((u32)r[0], (u32)r[1]);
-    };
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      u32x4 x[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) x[j] = ld16(qp + 64 * s + 32 * (j >> 1) + 8 * (j & 1));
-      const QueryScale s0 = query_scale(over_halves(max(largest(x[0]), largest(x[1]))));
-      const QueryScale s1 = query_scale(over_halves(max(largest(x[2]), largest(x[3]))));
-      split32(x, s0.up, s1.up, q_hi[s], q_lo[s]);
-      q_scale[s] = half ? s1.byte : s0.byte;
-    }
-  }
+  load_query(a, rows, row, g, half, q_hi, q_lo, q_scale);
 
   f32x16 acc[4];
 #pragma unroll
@@ -164,7 +177,6 @@ prefill_fp4_kernel(PrefillFp4Args a) {
   float neg_ref = -kNoScore, l_run = 0.f;  // minus the exponent's reference; the sum at that reference
 
   // The two 16-token tiles of each tile of keys (past the keys: their last one), looked up a tile ahead.
-  typedef const __attribute__((address_space(4))) int32_t const_i32;  // nothing writes the table: scalar loads
   const_i32 *bt = (const_i32 *)(a.block_tables + (int64_t)blockIdx.z * a.bt_stride);
   const int last_tile = max(kv_len - 1, 0) & ~15;
   int entry[2];
@@ -369,10 +381,231 @@ prefill_fp4_kernel(PrefillFp4Args a) {
   }
 }
 
+// ------------------------------------------------------------------------------------------ strips
+constexpr int kStripWaves = 4;
+constexpr int kStripRows = 32;
+constexpr int kRec = kHeadDim + 4;  // floats of a row in the waves' meeting
+
+// acc[2 J], acc[2 J + 1] += V^T P^T for row bytes 32 J .. +31 and 32 tokens (lane (n, half): 16 tokens of tile `half`; scales in
+// lanes 4 J .. 4 J + 3 of each 16).
+template <int J>
+__device__ __forceinline__ void add_strip(f32x16 (&acc)[4], u32x4 codes, u32 v_scales, const u32x4 (&p)[2]) {
+  const u32 sc[4] = {dpp_u32<kRowBcast + 4 * J>(v_scales), dpp_u32<kRowBcast + 4 * J + 1>(v_scales),
+                     dpp_u32<kRowBcast + 4 * J + 2>(v_scales), dpp_u32<kRowBcast + 4 * J + 3>(v_scales)};
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    u32 x[4], y[4];
+    expand4(codes[2 * h], sc[2 * h], x[0], x[1], y[0], y[1]);
+    expand4(codes[2 * h + 1], sc[2 * h + 1], x[2], x[3], y[2], y[3]);
+    acc[2 * J] = mfma32(u32x4{x[0], x[1], x[2], x[3]}, p[h], acc[2 * J]);
+    acc[2 * J + 1] = mfma32(u32x4{y[0], y[1], y[2], y[3]}, p[h], acc[2 * J + 1]);
+  }
+}
+
+template <bool WIDE>
+__global__ void __launch_bounds__(kStripWaves * 64) __attribute__((amdgpu_waves_per_eu(3)))
+prefill_strip_fp4_kernel(PrefillFp4Args a) {
+  constexpr int D = kHeadDim;
+  __shared__ __attribute__((aligned(16))) float s_o[kStripWaves][kStripRows / 2][kRec];
+  __shared__ float s_m[kStripWaves][kStripRows];
+  __shared__ float s_l[kStripWaves][kStripRows];
+
+  Rows rows;
+  if (!find_rows(a, kStripRows, rows)) return;
+  const int g = blockIdx.x;
+  const int lane = threadIdx.x & 63;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int half = lane >> 5, n = lane & 31;
+  const int row = min(rows.first + n, rows.rows - 1);
+  const int last_seen = min(rows.offset + row / a.group, rows.kv_len - 1);
+  const int first_seen = rows.offset + rows.first / a.group;  // the last key that the first row sees
+  const int keys = min(rows.kv_len, rows.offset + (min(rows.first + kStripRows, rows.rows) - 1) / a.group + 1);
+
+  i32x8 q_hi[2], q_lo[2];
+  u32 q_scale[2];
+  load_query(a, rows, row, g, half, q_hi, q_lo, q_scale);
+
+  f32x16 acc[4];
+#pragma unroll
+  for (int db = 0; db < 4; ++db)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) acc[db][i] = 0.f;
+  float neg_ref = -kNoScore, l_run = 0.f;  // minus the exponent's reference; the sum at that reference
+
+  const_i32 *bt = (const_i32 *)(a.block_tables + (int64_t)blockIdx.z * a.bt_stride);
+  const int last_tile = max(rows.kv_len - 1, 0) & ~15;
+  int entry[2], tile[2];
+  auto look_up = [&](int t0) {
+#pragma unroll
+    for (int x = 0; x < 2; ++x) entry[x] = bt[min(t0 + 16 * x, last_tile) >> a.bs_log2];
+  };
+  auto locate = [&](int t0) {
+#pragma unroll
+    for (int x = 0; x < 2; ++x) tile[x] = tile_of(a, entry[x], min(t0 + 16 * x, last_tile), g, lane == 0);
+  };
+  // Byte `at` of the lane's one of the two tiles.
+  auto in_tile = [&](const u8 *base, u32 second, int tile_bytes, u32 at) {
+    if constexpr (WIDE) {
+      const u32 d = (u32)(tile[1] - tile[0]);  // 1, or 0 past the keys
+      return base + (int64_t)tile[0] * tile_bytes + (at + (second & (d * tile_bytes)));
+    } else {
+      return base + (int64_t)(second ? tile[1] : tile[0]) * tile_bytes + at;
+    }
+  };
+  // Row n of K is token 4 (n / 8) + n % 4 of tile (n / 4) % 2: then register i of the scores is token i of tile `half`.
+  const int k_token = 4 * (n >> 3) + (n & 3);
+  const u32 k_second = (n & 4) ? ~0u : 0u, v_second = half ? ~0u : 0u;
+  const u32 k_at = k_token * kFp4RowBytes + 16 * half, ks_at = fp4_key_scale_at(k_token, half);
+  // Row bytes n and 32 + n of V, 16 tokens of tile `half` each: the low nibbles are one operand's row, the high ones another's.
+  // Their scales: lane i of a row of 16 holds tokens 4 (i % 4) .. +3 of block 2 (i / 4 % 2) + n / 16.
+  const u32 vs_at = 16 * (2 * ((n >> 2) & 1) + (n >> 4)) + 4 * (n & 3);
+  u32x4 kc[2], vc[2];
+  u32 ks[2], vs;
+  auto load_k = [&]() {
+    const u8 *kp = in_tile(a.cache.k_codes, k_second, kFp4TileBytes, k_at);
+    const u8 *sp = in_tile(a.cache.k_scales, k_second, kFp4TileScales, ks_at);
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      kc[s] = *reinterpret_cast<const u32x4 *>(kp + 32 * s);
+      ks[s] = sp[8 * s];
+    }
+  };
+  auto load_v = [&]() {
+    const u8 *vp = in_tile(a.cache.v_codes, v_second, kFp4TileBytes, 16 * n);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) vc[j] = *reinterpret_cast<const u32x4 *>(vp + 512 * j);
+    vs = *reinterpret_cast<const u32 *>(in_tile(a.cache.v_scales, v_second, kFp4TileScales, vs_at));
+  };
+  auto step = [&](const int t0, const int next) {
+    f32x16 sc;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) sc[i] = 0.f;
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      sc = mfma32_fp4_fp8(kc[s], ks[s], q_hi[s], q_scale[s], sc);
+      sc = mfma32_fp4_fp8(kc[s], ks[s], q_lo[s], q_scale[s], sc);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    if (next < keys) {
+      locate(next);
+      load_k();
+      look_up(next + 32 * kStripWaves);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    if (t0 + 31 > first_seen || t0 + 32 > rows.kv_len) {
+      const int lim = last_seen - t0 - 16 * half;
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if (i > lim) sc[i] = -INFINITY;
+      vs = keep_bytes(vs, rows.kv_len - t0 - 16 * half - 4 * (n & 3));  // stale rows past the keys
+    }
+    float tmax = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) tmax = fmaxf(tmax, sc[i]);
+    tmax = max_xor32(tmax) * a.scale_log2e;
+    const bool up = tmax + neg_ref > kRescaleLog2;
+    if (__builtin_amdgcn_ballot_w64(up) != 0) {
+      const float alpha = up ? fast_exp2(-neg_ref - tmax) : 1.f;
+      if (up) neg_ref = -tmax;
+      l_run *= alpha;
+#pragma unroll
+      for (int db = 0; db < 4; ++db)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[db][i] *= alpha;
+    }
+    u32x4 pf[2];
+#pragma unroll
+    for (int hh = 0; hh < 2; ++hh)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const u32 pr = pack_bf16x2(fast_exp2(fmaf(sc[8 * hh + 2 * e], a.scale_log2e, neg_ref)),
+                                   fast_exp2(fmaf(sc[8 * hh + 2 * e + 1], a.scale_log2e, neg_ref)));
+        l_run = dot2_bf16(pr, kBf16PairOne, l_run);
+        pf[hh][e] = pr;
+      }
+    const u32 bad = nan_bytes(vs);
+    vs = without(vs, bad);
+    add_strip<0>(acc, vc[0], vs, pf);
+    add_strip<1>(acc, vc[1], vs, pf);
+    if (__builtin_expect(__builtin_amdgcn_ballot_w64(bad != 0) != 0, 0)) {
+      u32 hit = 0;  // a bit for each block that this lane's row sees a NaN of
+#pragma unroll 1
+      for (int x = 0; x < 64; ++x) {  // of lane x's scales
+        const u32 b = (u32)__builtin_amdgcn_readlane((int)bad, x);
+        if (b == 0) continue;
+        const int at = t0 + 16 * (x >> 5) + 4 * (x & 3) + (__ffs((int)b) >> 3) - 1;  // the first of them (bit 7 of a byte)
+        hit |= last_seen >= at ? 1u << (2 * ((x >> 2) & 1) + ((x >> 4) & 1)) : 0u;
+      }
+#pragma unroll
+      for (int db = 0; db < 4; ++db)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[db][i] += hit >> (2 * (db >> 1) + (i >> 3)) & 1 ? NAN : 0.f;
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    if (next < keys) load_v();
+  };
+  if (int t0 = 32 * w; t0 < keys) {
+    look_up(t0);
+    locate(t0);
+    load_k();
+    load_v();
+    look_up(t0 + 32 * kStripWaves);
+#pragma unroll 1
+    do {
+      step(t0, t0 + 32 * kStripWaves);
+      t0 += 32 * kStripWaves;
+    } while (t0 < keys);
+  }
+
+  // The waves' results meet, 16 rows at a time.  Register i of acc[2 j + x] is dim 64 j + 32 (i / 8) + 16 x + 8 (i / 4 % 2) +
+  // 4 half + i % 4 of row n.
+  l_run = sum_xor32(l_run);
+  if (half == 0) {
+    s_m[w][n] = -neg_ref;
+    s_l[w][n] = l_run;
+  }
+  constexpr int kDims = 8;  // of a thread
+  static_assert(kStripWaves * 64 * kDims == kStripRows / 2 * D);
+  const int r = threadIdx.x / (D / kDims), d0 = threadIdx.x % (D / kDims) * kDims;
+#pragma unroll 1
+  for (int part = 0; part < 2; ++part) {
+    if ((n >> 4) == part) {
+#pragma unroll
+      for (int db = 0; db < 4; ++db)
+#pragma unroll
+        for (int i = 0; i < 16; i += 4)
+          *reinterpret_cast<f32x4 *>(&s_o[w][n & 15][64 * (db >> 1) + 32 * (i >> 3) + 16 * (db & 1) + 2 * (i & 4) + 4 * half]) =
+              f32x4{acc[db][i], acc[db][i + 1], acc[db][i + 2], acc[db][i + 3]};
+    }
+    __syncthreads();
+    const int rr = 16 * part + r;
+    if (rows.first + rr < rows.rows) {
+      float M = s_m[0][rr], den = 0.f, num[kDims];
+#pragma unroll
+      for (int x = 1; x < kStripWaves; ++x) M = fmaxf(M, s_m[x][rr]);
+#pragma unroll
+      for (int d = 0; d < kDims; ++d) num[d] = 0.f;
+#pragma unroll
+      for (int x = 0; x < kStripWaves; ++x) {
+        const float f = fast_exp2(s_m[x][rr] - M);
+        den += f * s_l[x][rr];
+#pragma unroll
+        for (int d = 0; d < kDims; ++d) num[d] += f * s_o[x][r][d0 + d];
+      }
+      const float inv = den > 0.f ? 1.f / den : 0.f;
+      const int at = rows.first + rr, t = at / a.group, h = g * a.group + at - t * a.group;
+      u32x4 v;
+#pragma unroll
+      for (int d = 0; d < 4; ++d) v[d] = pack_bf16x2(num[2 * d] * inv, num[2 * d + 1] * inv);
+      st16(a.out + (int64_t)(rows.q_start + t) * a.out_stride + (int64_t)h * D + d0, v);
+    }
+    __syncthreads();
+  }
+}
+
 // ------------------------------------------------------------------------------------------ few rows
 constexpr int kFewWaves = 8;
 constexpr int kFewRows = 16;
-constexpr int kRec = kHeadDim + 4;  // floats of a row in the waves' meeting
 
 __global__ void __launch_bounds__(kFewWaves * 64) __attribute__((amdgpu_waves_per_eu(3)))
 prefill_few_fp4_kernel(PrefillFp4Args a) {
@@ -415,31 +648,29 @@ prefill_few_fp4_kernel(PrefillFp4Args a) {
   };
   u32x4 kc[4], vc[4];
   u32 ks, vs;
-  int64_t k_tile, v_tile;
+  int k_tile, v_tile;
   auto locate = [&](int t0) {
     k_tile = tile_of(a, entry_k, min(t0 + 16 * (n >> 2), last_tile), g, true);
     v_tile = tile_of(a, entry_v, min(t0 + 16 * gq, last_tile), g, true);
   };
   auto load_k = [&]() {
-    const u8 *kp = a.cache.k_codes + k_tile * kFp4TileBytes + (n & 3) * kFp4RowBytes + 16 * gq;
+    const u8 *kp = a.cache.k_codes + (int64_t)k_tile * kFp4TileBytes + (n & 3) * kFp4RowBytes + 16 * gq;
 #pragma unroll
     for (int t = 0; t < 4; ++t) kc[t] = *reinterpret_cast<const u32x4 *>(kp + 4 * t * kFp4RowBytes);
-    ks = *reinterpret_cast<const u32 *>(a.cache.k_scales + k_tile * kFp4TileScales + fp4_key_scale_at(n & 3, gq));
+    ks = *reinterpret_cast<const u32 *>(a.cache.k_scales + (int64_t)k_tile * kFp4TileScales + fp4_key_scale_at(n & 3, gq));
   };
   auto load_v = [&]() {
-    const u8 *vp = a.cache.v_codes + v_tile * kFp4TileBytes + 16 * n;
+    const u8 *vp = a.cache.v_codes + (int64_t)v_tile * kFp4TileBytes + 16 * n;
 #pragma unroll
     for (int q = 0; q < 4; ++q) vc[q] = *reinterpret_cast<const u32x4 *>(vp + 256 * q);
-    vs = *reinterpret_cast<const u32 *>(a.cache.v_scales + v_tile * kFp4TileScales + 4 * n);
+    vs = *reinterpret_cast<const u32 *>(a.cache.v_scales + (int64_t)v_tile * kFp4TileScales + 4 * n);
   };
   auto step = [&](const int t0, const int next) {
     f32x4 s[4];
-    const u32 k_scale[4] = {ks & 0xffu, (ks >> 8) & 0xffu, (ks >> 16) & 0xffu, ks >> 24};
-#pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      s[t] = mfma_fp4_fp8(kc[t], k_scale[t], q_hi, q_scale, f32x4{0.f, 0.f, 0.f, 0.f});
-      s[t] = mfma_fp4_fp8(kc[t], k_scale[t], q_lo, q_scale, s[t]);
-    }
+    score<0>(s[0], kc[0], ks, q_hi, q_lo, q_scale);
+    score<1>(s[1], kc[1], ks, q_hi, q_lo, q_scale);
+    score<2>(s[2], kc[2], ks, q_hi, q_lo, q_scale);
+    score<3>(s[3], kc[3], ks, q_hi, q_lo, q_scale);
     __builtin_amdgcn_sched_barrier(0);
     if (next < keys) {
       locate(next);
@@ -493,17 +724,16 @@ prefill_few_fp4_kernel(PrefillFp4Args a) {
     add_values<2>(o, vc, vs, pf);
     add_values<3>(o, vc, vs, pf);
     if (__builtin_expect(__builtin_amdgcn_ballot_w64(bad != 0) != 0, 0)) {
-      float poison[4] = {0.f, 0.f, 0.f, 0.f};  // of each block, for this lane's row
+      u32 hit = 0;  // a bit for each block that this lane's row sees a NaN of
 #pragma unroll 1
       for (int x = 0; x < 64; ++x) {  // lane x noted tokens 4 (x % 4) .. of tile x / 16, block (x % 16) / 4
         const u32 b = (u32)__builtin_amdgcn_readlane((int)bad, x);
         if (b == 0) continue;
         const int at = t0 + 16 * (x >> 4) + 4 * (x & 3) + (__ffs((int)b) >> 3) - 1;  // the first of them (bit 7 of a byte)
-#pragma unroll
-        for (int q = 0; q < 4; ++q) poison[q] = last_seen >= at && (x & 15) >> 2 == q ? NAN : poison[q];
+        hit |= last_seen >= at ? 1u << ((x & 15) >> 2) : 0u;
       }
 #pragma unroll
-      for (int e = 0; e < 8; ++e) o[e] += poison[e >> 1];
+      for (int e = 0; e < 8; ++e) o[e] += hit >> (e >> 1) & 1 ? NAN : 0.f;
     }
     __builtin_amdgcn_sched_barrier(0);
     if (next < keys) load_v();
@@ -551,8 +781,17 @@ prefill_few_fp4_kernel(PrefillFp4Args a) {
   }
 }
 
-// Workgroups of the tile kernel below which the few-rows kernel runs.
+// Which kernel, by the workgroups that the bounds of a call allow (few sequences are as long as the longest).  us, few rows /
+// strips / tiles, 16 query and 8 kv heads unless given:
+//   1 x 20 rows on 4,096 cached   20 /  32 / 132        1 x 1,000 on 4,096    87 /  60 / 163
+//   1 x 100 on 4,096              21 /  32 / 135        1 x 4,000 on none    171 /  96 / 151
+//   the same, 40 and 8 heads      21 /  34 / 134        4 x 2,000 on 1,152     - / 194 / 194 (1,000 workgroups of tiles)
+//   1 x 300 on none               10 / 8.7 /  16        3 x 3,000 on none      - / 163 / 146 (1,128)
+//   8 x 64 on 1,040               19 /  15 /  41        16 x 2,000 on 1,152    - / 698 / 642 (2,000)
+// Few rows: while one round over the CUs takes them all.  Tiles: from four workgroups a CU on; before, whole CUs wait
+// for the longest rows.
 constexpr int64_t kFewGroups = 256;
+constexpr int64_t kStripGroups = 1024;  // of the tile kernel
 
 }  // namespace
 }  // namespace nvamd
@@ -602,12 +841,18 @@ extern "C" int nvamd_paged_prefill_fp4(void *out, int64_t out_stride, const void
   const int64_t max_rows = (int64_t)max_q_len * a.group;
   if (max_rows > 0x7fffffff) return NVAMD_EUNSUPPORTED;
   const int64_t tiles = (max_rows + kTileRows - 1) / kTileRows;
-  const bool few = tiles * num_kv_heads * n_seqs <= kFewGroups;
-  a.max_tiles = (int)(few ? (max_rows + kFewRows - 1) / kFewRows : tiles);
+  const int64_t few_tiles = (max_rows + kFewRows - 1) / kFewRows, strips = (max_rows + kStripRows - 1) / kStripRows;
+  const int64_t units = (int64_t)num_kv_heads * n_seqs;
+  const bool few = few_tiles * units <= kFewGroups, strip = !few && tiles * units <= kStripGroups;
+  a.max_tiles = (int)(few ? few_tiles : strip ? strips : tiles);
   if (a.max_tiles > 65535) return NVAMD_EUNSUPPORTED;
   const dim3 grid(num_kv_heads, a.max_tiles, n_seqs);
   if (few)
     hipLaunchKernelGGL(prefill_few_fp4_kernel, grid, dim3(kFewWaves * 64), 0, stream, a);
+  else if (strip && bs_log2 >= 5)
+    hipLaunchKernelGGL((prefill_strip_fp4_kernel<true>), grid, dim3(kStripWaves * 64), 0, stream, a);
+  else if (strip)
+    hipLaunchKernelGGL((prefill_strip_fp4_kernel<false>), grid, dim3(kStripWaves * 64), 0, stream, a);
   else if (bs_log2 >= 5)
     hipLaunchKernelGGL(prefill_fp4_kernel<true>, grid, dim3(kWaves * 64), 0, stream, a);
   else

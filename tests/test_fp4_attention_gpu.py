@@ -78,6 +78,8 @@ class Batch:
     def prefill(self, q, q_lens, out=None, max_q=None, scale=SCALE):
         cu = torch.tensor([0] + q_lens).cumsum(0).to(torch.int32).to(self.device)
         out = torch.full(q.shape, 7.0, dtype=torch.bfloat16, device=self.device) if out is None else out
+        if max_q == "strips":
+            max_q = 65536 // (self.hq * len(self.lens))
         return _C.paged_prefill_fp4(out, q.to(self.device), self.keys, self.values, self.tables.to(self.device), cu,
                                     torch.tensor(self.lens, dtype=torch.int32, device=self.device),
                                     max_q or max(q_lens), scale)
@@ -361,9 +363,8 @@ class Window:
 
 
 # -------------------------------------------------------------------------------------------- prefill
-# Launches whose bound gives few workgroups run another kernel than the rest: each test makes both, by a bound far past its
-# lengths.
-BOUNDS = pytest.mark.parametrize("bound", [None, 60_000], ids=["few", "tiles"])
+# The kernel follows the rows that a call's bounds allow: as many as there are, those of a middle size, of a large one.
+BOUNDS = pytest.mark.parametrize("bound", [None, "strips", 60_000], ids=["exact", "strips", "tiles"])
 
 
 def check_prefill(batch, q, q_lens, got, scale=SCALE):
@@ -392,6 +393,16 @@ def test_prefill_lengths_around_tiles_and_pages(device, bs, bound):
     batch = Batch(device, [a + b for a, b in zip(q_lens, cached)], 4, 2, bs, seed=bs)
     q = batch.queries(sum(q_lens))
     check_prefill(batch, q, q_lens, batch.prefill(q, q_lens, max_q=bound))
+
+
+@pytest.mark.parametrize("bs", [16, 64])
+def test_prefill_few_rows(device, bs):
+    """Each alone, so that no call has more than a few rows."""
+    for q_len, cached in ((1, 0), (1, 1), (2, 15), (3, 16), (15, 17), (16, 63), (17, 64), (31, 33), (33, 500), (64, 511),
+                          (65, 512), (127, 3000), (256, 0), (300, 1)):
+        batch = Batch(device, [q_len + cached], 4, 2, bs, seed=q_len)
+        q = batch.queries(q_len)
+        check_prefill(batch, q, [q_len], batch.prefill(q, [q_len]))
 
 
 @BOUNDS
@@ -476,7 +487,7 @@ def test_prefill_faults_are_reported_and_leave_the_others_alone(device, bound):
     out = torch.full((180, 2, 128), 7.0, dtype=torch.bfloat16, device=device)
     args = (batch.keys, batch.values, batch.tables.to(device), cu,
             torch.tensor(batch.lens, dtype=torch.int32, device=device))
-    _C.paged_prefill_fp4(out, q.to(device), *args, bound or 101, SCALE)
+    _C.paged_prefill_fp4(out, q.to(device), *args, 65536 // 6 if bound == "strips" else bound or 101, SCALE)
     assert _C.index_errors() == _C.ERR_CONTEXT
     assert torch.equal(out[:20], good[:20]) and out[80:].eq(7).all()
 
