@@ -449,7 +449,10 @@ int nvamd_paged_decode_fp4(void *out, int64_t out_stride,
                            void *workspace, size_t workspace_bytes,
                            hipStream_t stream);
 
-/* paged_prefill_fp4: nvamd_paged_prefill over the 4-bit cache.  A NaN of the   */
+/* paged_prefill_fp4: nvamd_paged_prefill over the 4-bit cache.  workspace, of  */
+/* nvamd_paged_prefill_fp4_workspace_size(...) bytes (0: none needed), any      */
+/* contents, of this call's own while it runs, lets few rows on long contexts   */
+/* be cut along the keys; NULL runs them uncut.  |q . k| scale below 2^29.  A NaN of the */
 /* cache reaches the rows that see its key and no others.  A sequence whose    */
 /* rows leave [0, num_tokens) is skipped, and it, a q_len past max_q_len (whose */
 /* further rows are not written) and a kv_len below q_len are reported as       */
@@ -463,7 +466,11 @@ int nvamd_paged_prefill_fp4(void *out, int64_t out_stride,
                             int bt_width, const int32_t *cu_seqlens_q,
                             const int32_t *kv_lens, int n_seqs, int num_tokens,
                             int max_q_len, int num_heads, int num_kv_heads,
-                            int head_dim, float scale, hipStream_t stream);
+                            int head_dim, float scale, void *workspace,
+                            size_t workspace_bytes, hipStream_t stream);
+size_t nvamd_paged_prefill_fp4_workspace_size(int n_seqs, int max_q_len,
+                                              int num_heads, int num_kv_heads,
+                                              int block_size, int bt_width);
 
 #ifdef __cplusplus
 }

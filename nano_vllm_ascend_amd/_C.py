@@ -110,8 +110,9 @@ _SIGNATURES = {
     "nvamd_paged_prefill_fp4": (
         _c_int,
         [_c_ptr, _c_i64, _c_ptr, _c_i64, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_int, _c_ptr, _c_int, _c_int,
-         _c_ptr, _c_ptr, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_float, _c_ptr],
+         _c_ptr, _c_ptr, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_float, _c_ptr, _c_size, _c_ptr],
     ),
+    "nvamd_paged_prefill_fp4_workspace_size": (_c_size, [_c_int, _c_int, _c_int, _c_int, _c_int, _c_int]),
     "nvamd_qk_norm_rope": (
         _c_int,
         [_c_ptr, _c_i64, _c_ptr, _c_i64, _c_ptr, _c_i64, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_ptr,
@@ -799,8 +800,11 @@ def paged_prefill_fp4(out: torch.Tensor, q: torch.Tensor, key_pages: Fp4Pages, v
         raise ValueError("kv_lens must be contiguous int32, one per sequence")
     if _range_checks and _checking():
         check_paged_context(block_tables[:n], kv_lens[:n], args[8], args[9])
+    stream = _stream_of(device, q, out, block_tables, cu_seqlens_q, kv_lens)
+    need = lib.nvamd_paged_prefill_fp4_workspace_size(n, max_q_len, heads[0], heads[1], args[9], args[12])
+    space = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None  # until the stream has passed the call
     status = lib.nvamd_paged_prefill_fp4(*args, cu_seqlens_q.data_ptr(), kv_lens.data_ptr(), n, q.shape[0], max_q_len,
-                                         *heads, scale, _stream_of(device, q, out, block_tables, cu_seqlens_q, kv_lens))
+                                         *heads, scale, space.data_ptr() if need else None, need, stream)
     if status:
         _check(status, "nvamd_paged_prefill_fp4")
     return out

@@ -26,6 +26,7 @@ __device__ __forceinline__ float sum_over_quarters(float v) {
   return sum_xor32(__uint_as_float(r[0]) + __uint_as_float(r[1]));
 }
 
+typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 
 // S += K . q for 16 rows of codes (128 dims) and 16 columns of e4m3, each block of 32 dims under its scale byte.  Lane (row

@@ -23,8 +23,8 @@
 //   tile kernel's expansion for each row, for four times the workgroups.  1 x 4,000 rows on 4,096 keys 232 us (859 TFLOP/s).
 //
 // Few rows (a chat's next turn).  Workgroup = 8 waves = 16 rows, a wave every eighth 64 keys, as in paged_decode_fp4.hip with rows
-//   in the place of heads and a last key for each row.  Bound by the latency of a wave's steps: 1 x 20 rows on 4,096 keys
-//   20 us.
+//   in the place of heads and a last key for each row.  Bound by the latency of a launch and of a wave's steps: 8 x 20 rows on
+//   1,040 keys 10 us.  On long contexts the keys are cut as well.
 //
 // A block of values that reads as NaN must reach the rows that see its key and no others, though masked rows
 // multiply it by a weight of zero: such values enter the products as zeros, and the rows that see
@@ -53,6 +53,8 @@ struct PrefillFp4Args {
   int max_q_len;
   int num_tokens;
   float scale_log2e;
+  int splits;       // that the keys of a workgroup's rows are cut into at most
+  float *partials;  // [sequence][kv head][split][row][kRec]
   u32 *err;
 };
 
@@ -64,8 +66,9 @@ struct Rows {
   int offset;  // token t sees keys 0 .. offset + t
   int first;   // the workgroup's first row
 };
-// False if it has none.  Faults are reported once per sequence.
-__device__ __forceinline__ bool find_rows(const PrefillFp4Args &a, int per_group, Rows &r) {
+// The y-th group of rows from a sequence's end: those with the most keys start first.  False if it has none.  Faults are
+// reported once per sequence.
+__device__ __forceinline__ bool find_rows(const PrefillFp4Args &a, int per_group, int y, Rows &r) {
   const int s = blockIdx.z;
   r.q_start = a.cu_seqlens_q[s];
   const int q_end = a.cu_seqlens_q[s + 1];
@@ -76,11 +79,30 @@ __device__ __forceinline__ bool find_rows(const PrefillFp4Args &a, int per_group
   if ((!rows_in || q_len > a.max_q_len || kv_len > cap || kv_len < q_len) && blockIdx.x == 0 && blockIdx.y == 0 &&
       threadIdx.x == 0)
     flag_index_error(a.err, NVAMD_ERR_CONTEXT);
-  r.rows = q_len * a.group;
-  r.first = (a.max_tiles - 1 - (int)blockIdx.y) * per_group;  // the most keys first
+  r.rows = min(q_len, a.max_q_len) * a.group;
+  r.first = (a.max_tiles - 1 - y) * per_group;
   r.kv_len = min(kv_len, cap);
   r.offset = r.kv_len - q_len;
   return rows_in && r.first < r.rows;
+}
+
+// The keys that rows first .. first + per_group - 1 need, and their cut: pieces of a multiple of kMinSplit.
+constexpr int kMinSplit = 512;
+constexpr int kRec = kHeadDim + 4;  // floats of a row's record: max, sum, 2 unused, numerators
+struct Cut {
+  int keys;
+  int length;
+  int pieces;
+};
+__device__ __forceinline__ Cut find_cut(const PrefillFp4Args &a, const Rows &r, int per_group) {
+  const int keys = max(min(r.kv_len, r.offset + (min(r.first + per_group, r.rows) - 1) / a.group + 1), 0);
+  if (a.splits == 1) return {keys, keys, 1};
+  const int length = max(ceil_div(ceil_div(keys, a.splits), kMinSplit), 1) * kMinSplit;
+  return {keys, length, max(ceil_div(keys, length), 1)};
+}
+__device__ __forceinline__ float *record(const PrefillFp4Args &a, int per_group, int g, int piece, int row) {
+  const int64_t unit = ((int64_t)blockIdx.z * a.num_kv_heads + g) * a.splits + piece;
+  return a.partials + (unit * (a.max_tiles * per_group) + row) * kRec;
 }
 
 __device__ __forceinline__ int tile_of(const PrefillFp4Args &a, int entry, int token, int g, bool report) {
@@ -150,7 +172,7 @@ prefill_fp4_kernel(PrefillFp4Args a) {
   Stage *stages = reinterpret_cast<Stage *>(s_mem);
 
   Rows rows;
-  if (!find_rows(a, kTileRows, rows)) return;
+  if (!find_rows(a, kTileRows, blockIdx.y, rows)) return;
   const int g = blockIdx.x;
   const int lane = threadIdx.x & 63;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -384,7 +406,6 @@ prefill_fp4_kernel(PrefillFp4Args a) {
 // ------------------------------------------------------------------------------------------ strips
 constexpr int kStripWaves = 4;
 constexpr int kStripRows = 32;
-constexpr int kRec = kHeadDim + 4;  // floats of a row in the waves' meeting
 
 // acc[2 J], acc[2 J + 1] += V^T P^T for row bytes 32 J .. +31 and 32 tokens (lane (n, half): 16 tokens of tile `half`; scales in
 // lanes 4 J .. 4 J + 3 of each 16).
@@ -411,15 +432,17 @@ prefill_strip_fp4_kernel(PrefillFp4Args a) {
   __shared__ float s_l[kStripWaves][kStripRows];
 
   Rows rows;
-  if (!find_rows(a, kStripRows, rows)) return;
-  const int g = blockIdx.x;
+  if (!find_rows(a, kStripRows, blockIdx.y, rows)) return;
+  const int piece = blockIdx.x / a.num_kv_heads, g = blockIdx.x - piece * a.num_kv_heads;
+  const Cut cut = find_cut(a, rows, kStripRows);
+  if (piece >= cut.pieces) return;
+  const int begin = piece * cut.length, end = min(begin + cut.length, cut.keys);
   const int lane = threadIdx.x & 63;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int half = lane >> 5, n = lane & 31;
   const int row = min(rows.first + n, rows.rows - 1);
   const int last_seen = min(rows.offset + row / a.group, rows.kv_len - 1);
   const int first_seen = rows.offset + rows.first / a.group;  // the last key that the first row sees
-  const int keys = min(rows.kv_len, rows.offset + (min(rows.first + kStripRows, rows.rows) - 1) / a.group + 1);
 
   i32x8 q_hi[2], q_lo[2];
   u32 q_scale[2];
@@ -486,7 +509,7 @@ prefill_strip_fp4_kernel(PrefillFp4Args a) {
       sc = mfma32_fp4_fp8(kc[s], ks[s], q_lo[s], q_scale[s], sc);
     }
     __builtin_amdgcn_sched_barrier(0);
-    if (next < keys) {
+    if (next < end) {
       locate(next);
       load_k();
       look_up(next + 32 * kStripWaves);
@@ -542,9 +565,9 @@ prefill_strip_fp4_kernel(PrefillFp4Args a) {
         for (int i = 0; i < 16; ++i) acc[db][i] += hit >> (2 * (db >> 1) + (i >> 3)) & 1 ? NAN : 0.f;
     }
     __builtin_amdgcn_sched_barrier(0);
-    if (next < keys) load_v();
+    if (next < end) load_v();
   };
-  if (int t0 = 32 * w; t0 < keys) {
+  if (int t0 = begin + 32 * w; t0 < end) {
     look_up(t0);
     locate(t0);
     load_k();
@@ -554,7 +577,7 @@ prefill_strip_fp4_kernel(PrefillFp4Args a) {
     do {
       step(t0, t0 + 32 * kStripWaves);
       t0 += 32 * kStripWaves;
-    } while (t0 < keys);
+    } while (t0 < end);
   }
 
   // The waves' results meet, 16 rows at a time.  Register i of acc[2 j + x] is dim 64 j + 32 (i / 8) + 16 x + 8 (i / 4 % 2) +
@@ -592,18 +615,35 @@ prefill_strip_fp4_kernel(PrefillFp4Args a) {
 #pragma unroll
         for (int d = 0; d < kDims; ++d) num[d] += f * s_o[x][r][d0 + d];
       }
-      const float inv = den > 0.f ? 1.f / den : 0.f;
-      const int at = rows.first + rr, t = at / a.group, h = g * a.group + at - t * a.group;
-      u32x4 v;
+      if (cut.pieces > 1) {
+        float *rec = record(a, kStripRows, g, piece, rows.first + rr);
+        if (d0 == 0) *reinterpret_cast<f32x2 *>(rec) = f32x2{M, den};
 #pragma unroll
-      for (int d = 0; d < 4; ++d) v[d] = pack_bf16x2(num[2 * d] * inv, num[2 * d + 1] * inv);
-      st16(a.out + (int64_t)(rows.q_start + t) * a.out_stride + (int64_t)h * D + d0, v);
+        for (int d = 0; d < kDims; d += 4)
+          *reinterpret_cast<f32x4 *>(rec + 4 + d0 + d) = f32x4{num[d], num[d + 1], num[d + 2], num[d + 3]};
+      } else {
+        const float inv = den > 0.f ? 1.f / den : 0.f;
+        const int at = rows.first + rr, t = at / a.group, h = g * a.group + at - t * a.group;
+        u32x4 v;
+#pragma unroll
+        for (int d = 0; d < 4; ++d) v[d] = pack_bf16x2(num[2 * d] * inv, num[2 * d + 1] * inv);
+        st16(a.out + (int64_t)(rows.q_start + t) * a.out_stride + (int64_t)h * D + d0, v);
+      }
     }
     __syncthreads();
   }
 }
 
 // ------------------------------------------------------------------------------------------ few rows
+// Dims 4 dl .. 4 dl + 3 of the workgroup's row r.
+__device__ __forceinline__ void write_quad(const PrefillFp4Args &a, const Rows &rows, int g, int r, int dl, f32x4 num,
+                                           float den) {
+  const float inv = den > 0.f ? 1.f / den : 0.f;
+  const int t = (rows.first + r) / a.group, h = g * a.group + rows.first + r - t * a.group;
+  *reinterpret_cast<u32x2 *>(a.out + (int64_t)(rows.q_start + t) * a.out_stride + (int64_t)h * kHeadDim + 4 * dl) =
+      u32x2{pack_bf16x2(num[0] * inv, num[1] * inv), pack_bf16x2(num[2] * inv, num[3] * inv)};
+}
+
 constexpr int kFewWaves = 8;
 constexpr int kFewRows = 16;
 
@@ -615,8 +655,11 @@ prefill_few_fp4_kernel(PrefillFp4Args a) {
   __shared__ float s_l[kFewWaves][kFewRows];
 
   Rows rows;
-  if (!find_rows(a, kFewRows, rows)) return;
-  const int g = blockIdx.x;
+  if (!find_rows(a, kFewRows, blockIdx.y, rows)) return;
+  const int piece = blockIdx.x / a.num_kv_heads, g = blockIdx.x - piece * a.num_kv_heads;
+  const Cut cut = find_cut(a, rows, kFewRows);
+  if (piece >= cut.pieces) return;
+  const int begin = piece * cut.length, end = min(begin + cut.length, cut.keys);
   const int lane = threadIdx.x & 63;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n = lane & 15, gq = lane >> 4;
@@ -624,7 +667,6 @@ prefill_few_fp4_kernel(PrefillFp4Args a) {
   const int token = row / a.group, head = g * a.group + row - token * a.group;
   const int last_seen = min(rows.offset + token, rows.kv_len - 1);
   const int first_seen = rows.offset + rows.first / a.group;  // the last key that the first row sees
-  const int keys = min(rows.kv_len, rows.offset + (min(rows.first + kFewRows, rows.rows) - 1) / a.group + 1);
 
   i32x8 q_hi, q_lo;
   u32 q_scale;
@@ -672,7 +714,7 @@ prefill_few_fp4_kernel(PrefillFp4Args a) {
     score<2>(s[2], kc[2], ks, q_hi, q_lo, q_scale);
     score<3>(s[3], kc[3], ks, q_hi, q_lo, q_scale);
     __builtin_amdgcn_sched_barrier(0);
-    if (next < keys) {
+    if (next < end) {
       locate(next);
       load_k();
       look_up(next + 64 * kFewWaves);
@@ -736,9 +778,9 @@ prefill_few_fp4_kernel(PrefillFp4Args a) {
       for (int e = 0; e < 8; ++e) o[e] += hit >> (e >> 1) & 1 ? NAN : 0.f;
     }
     __builtin_amdgcn_sched_barrier(0);
-    if (next < keys) load_v();
+    if (next < end) load_v();
   };
-  if (int t0 = 64 * w; t0 < keys) {
+  if (int t0 = begin + 64 * w; t0 < end) {
     look_up(t0);
     locate(t0);
     load_k();
@@ -748,7 +790,7 @@ prefill_few_fp4_kernel(PrefillFp4Args a) {
     do {
       step(t0, t0 + 64 * kFewWaves);
       t0 += 64 * kFewWaves;
-    } while (t0 < keys);
+    } while (t0 < end);
   }
 
   // Register i of o[e] is dim 16 e + 4 gq + i of row n.
@@ -773,12 +815,59 @@ prefill_few_fp4_kernel(PrefillFp4Args a) {
     num += f * *reinterpret_cast<const f32x4 *>(&s_o[x][r * kRec + 4 * dl]);
     den += f * s_l[x][r];
   }
-  if (rows.first + r < rows.rows) {
-    const float inv = den > 0.f ? 1.f / den : 0.f;
-    const int t = (rows.first + r) / a.group, h = g * a.group + rows.first + r - t * a.group;
-    *reinterpret_cast<u32x2 *>(a.out + (int64_t)(rows.q_start + t) * a.out_stride + (int64_t)h * D + 4 * dl) =
-        u32x2{pack_bf16x2(num[0] * inv, num[1] * inv), pack_bf16x2(num[2] * inv, num[3] * inv)};
+  if (rows.first + r >= rows.rows) return;
+  if (cut.pieces > 1) {
+    float *rec = record(a, kFewRows, g, piece, rows.first + r);
+    if (dl == 0) *reinterpret_cast<f32x2 *>(rec) = f32x2{M, den};
+    *reinterpret_cast<f32x4 *>(rec + 4 + 4 * dl) = num;
+  } else {
+    write_quad(a, rows, g, r, dl, num, den);
   }
+}
+
+// ------------------------------------------------------------------------------------------ pieces
+// Joins the pieces of the rows whose keys were cut: 8 rows of a group a workgroup, a half-wave each, its lane dims 4 dl ..
+// 4 dl + 3.  The records of kRun pieces load together.
+constexpr int kRun = 8;
+
+__global__ void __launch_bounds__(256)
+prefill_join_fp4_kernel(PrefillFp4Args a, int per_group) {
+  Rows rows;
+  if (!find_rows(a, per_group, blockIdx.y / (per_group / 8), rows)) return;
+  const int g = blockIdx.x, dl = threadIdx.x & 31, r = blockIdx.y % (per_group / 8) * 8 + (threadIdx.x >> 5);
+  if (rows.first + r >= rows.rows) return;
+  const Cut cut = find_cut(a, rows, per_group);
+  if (cut.pieces == 1) return;
+  const int64_t stride = (int64_t)a.max_tiles * per_group * kRec;  // from a piece's record to the next one's
+  const float *rec = record(a, per_group, g, 0, rows.first + r);
+  float M = kNoScore, den = 0.f;
+  f32x4 num = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+  for (int y0 = 0; y0 < cut.pieces; y0 += kRun) {
+    f32x2 ml[kRun];
+    f32x4 v[kRun];
+#pragma unroll
+    for (int y = 0; y < kRun; ++y) {
+      const float *p = rec + min(y0 + y, cut.pieces - 1) * stride;
+      ml[y] = *reinterpret_cast<const f32x2 *>(p);
+      v[y] = *reinterpret_cast<const f32x4 *>(p + 4 + 4 * dl);
+    }
+    float up = M;
+#pragma unroll
+    for (int y = 0; y < kRun; ++y) up = fmaxf(up, ml[y][0]);  // the last piece's again past the end
+    const float f_old = fast_exp2(M - up);
+    num *= f_old;
+    den *= f_old;
+#pragma unroll
+    for (int y = 0; y < kRun; ++y) {
+      if (y0 + y >= cut.pieces) break;
+      const float f = fast_exp2(ml[y][0] - up);
+      num += f * v[y];
+      den += f * ml[y][1];
+    }
+    M = up;
+  }
+  write_quad(a, rows, g, r, dl, num, den);
 }
 
 // Which kernel, by the workgroups that the bounds of a call allow (few sequences are as long as the longest).  us, few rows /
@@ -787,23 +876,67 @@ prefill_few_fp4_kernel(PrefillFp4Args a) {
 //   1 x 100 on 4,096              21 /  32 / 135        1 x 4,000 on none    171 /  96 / 151
 //   the same, 40 and 8 heads      21 /  34 / 134        4 x 2,000 on 1,152     - / 194 / 194 (1,000 workgroups of tiles)
 //   1 x 300 on none               10 / 8.7 /  16        3 x 3,000 on none      - / 163 / 146 (1,128)
-//   8 x 64 on 1,040               19 /  15 /  41        16 x 2,000 on 1,152    - / 698 / 642 (2,000)
+//   8 x 64 on 1,040               19 /  15 /  41        16 x 2,000 on 1,152    - / 698 / 642 (4,096)
 // Few rows: while one round over the CUs takes them all.  Tiles: from four workgroups a CU on; before, whole CUs wait
 // for the longest rows.
 constexpr int64_t kFewGroups = 256;
 constexpr int64_t kStripGroups = 1024;  // of the tile kernel
+
+// Where few rows or strips leave the card idle and contexts may be long, the keys are cut until the workgroups fill it once, at
+// most kMaxSplits times, and a second kernel joins the pieces (some 3 us).  us, uncut / cut: 1 x 20 rows on 4,096 keys 20 /
+// 12.4, 2 x 20 on 8,192 35 / 17.6, 1 x 300 on 8,192 61 / 44, 1 x 600 on 8,192 93 / 79.  Few rows take a CU each, strips a
+// third of one (with half: 45 and 93).
+constexpr int kSplitFrom = 4096;  // keys that the block tables hold
+constexpr int kMaxSplits = 32;
+
+struct Plan {
+  int rows;  // of a workgroup: kFewRows, kStripRows or kTileRows
+  int64_t tiles;
+  int splits;
+  size_t workspace;
+};
+Plan plan_prefill(int64_t n_seqs, int64_t max_rows, int64_t num_kv_heads, int64_t cap) {
+  const int64_t units = n_seqs * num_kv_heads;
+  const auto tiles_of = [&](int rows) { return (max_rows + rows - 1) / rows; };
+  Plan p;
+  int64_t slots = 0;  // workgroups that the card holds at once
+  if (tiles_of(kFewRows) * units <= kFewGroups) {
+    p.rows = kFewRows;
+    slots = 256;
+  } else if (tiles_of(kTileRows) * units <= kStripGroups) {
+    p.rows = kStripRows;
+    slots = 3 * 256;
+  } else {
+    p.rows = kTileRows;
+  }
+  p.tiles = tiles_of(p.rows);
+  const int64_t wanted = cap < kSplitFrom ? 1 : min(slots / (p.tiles * units), min(cap / kMinSplit, (int64_t)kMaxSplits));
+  p.splits = (int)max(wanted, (int64_t)1);
+  p.workspace = p.splits == 1 ? 0 : (size_t)(units * p.splits * p.tiles * p.rows) * kRec * sizeof(float);
+  return p;
+}
 
 }  // namespace
 }  // namespace nvamd
 
 using namespace nvamd;
 
+extern "C" size_t nvamd_paged_prefill_fp4_workspace_size(int n_seqs, int max_q_len, int num_heads, int num_kv_heads,
+                                                         int block_size, int bt_width) {
+  if (n_seqs <= 0 || max_q_len <= 0 || num_kv_heads <= 0 || num_heads < num_kv_heads || block_size <= 0 || bt_width <= 0)
+    return 0;
+  return plan_prefill(n_seqs, (int64_t)max_q_len * (num_heads / num_kv_heads), num_kv_heads,
+                      (int64_t)bt_width * block_size)
+      .workspace;
+}
+
 extern "C" int nvamd_paged_prefill_fp4(void *out, int64_t out_stride, const void *q, int64_t q_stride,
                                        const void *k_codes, const void *k_scales, const void *v_codes,
                                        const void *v_scales, int num_blocks, int block_size,
                                        const int32_t *block_tables, int bt_stride, int bt_width,
                                        const int32_t *cu_seqlens_q, const int32_t *kv_lens, int n_seqs, int num_tokens,
-                                       int max_q_len, int num_heads, int num_kv_heads, int head_dim, float scale, hipStream_t stream) {
+                                       int max_q_len, int num_heads, int num_kv_heads, int head_dim, float scale,
+                                       void *workspace, size_t workspace_bytes, hipStream_t stream) {
   if (n_seqs == 0 || max_q_len == 0) return NVAMD_OK;
   const int bs_log2 = log2_exact(block_size);
   if (head_dim != kHeadDim || bs_log2 < 4) return NVAMD_EUNSUPPORTED;
@@ -840,14 +973,19 @@ extern "C" int nvamd_paged_prefill_fp4(void *out, int64_t out_stride, const void
   a.group = num_heads / num_kv_heads;
   const int64_t max_rows = (int64_t)max_q_len * a.group;
   if (max_rows > 0x7fffffff) return NVAMD_EUNSUPPORTED;
-  const int64_t tiles = (max_rows + kTileRows - 1) / kTileRows;
-  const int64_t few_tiles = (max_rows + kFewRows - 1) / kFewRows, strips = (max_rows + kStripRows - 1) / kStripRows;
-  const int64_t units = (int64_t)num_kv_heads * n_seqs;
-  const bool few = few_tiles * units <= kFewGroups, strip = !few && tiles * units <= kStripGroups;
-  a.max_tiles = (int)(few ? few_tiles : strip ? strips : tiles);
-  if (a.max_tiles > 65535) return NVAMD_EUNSUPPORTED;
-  const dim3 grid(num_kv_heads, a.max_tiles, n_seqs);
-  if (few)
+  const Plan plan = plan_prefill(n_seqs, max_rows, num_kv_heads, (int64_t)bt_width << bs_log2);
+  if (plan.tiles > 65535) return NVAMD_EUNSUPPORTED;
+  a.max_tiles = (int)plan.tiles;
+  a.splits = 1;
+  if (workspace != nullptr && plan.splits > 1) {
+    if (workspace_bytes < plan.workspace) return NVAMD_EWORKSPACE;
+    if (!aligned16(workspace)) return NVAMD_EINVAL;
+    a.splits = plan.splits;
+    a.partials = static_cast<float *>(workspace);
+  }
+  const dim3 grid(num_kv_heads * a.splits, a.max_tiles, n_seqs);
+  const bool strip = plan.rows == kStripRows;
+  if (plan.rows == kFewRows)
     hipLaunchKernelGGL(prefill_few_fp4_kernel, grid, dim3(kFewWaves * 64), 0, stream, a);
   else if (strip && bs_log2 >= 5)
     hipLaunchKernelGGL((prefill_strip_fp4_kernel<true>), grid, dim3(kStripWaves * 64), 0, stream, a);
@@ -857,5 +995,12 @@ extern "C" int nvamd_paged_prefill_fp4(void *out, int64_t out_stride, const void
     hipLaunchKernelGGL(prefill_fp4_kernel<true>, grid, dim3(kWaves * 64), 0, stream, a);
   else
     hipLaunchKernelGGL(prefill_fp4_kernel<false>, grid, dim3(kWaves * 64), 0, stream, a);
+  if (a.splits > 1) {
+    const int st = launch_status();
+    if (st != NVAMD_OK) return st;
+    a.err = nullptr;  // the faults have been reported
+    hipLaunchKernelGGL(prefill_join_fp4_kernel, dim3(num_kv_heads, a.max_tiles * (plan.rows / 8), n_seqs), dim3(256), 0,
+                       stream, a, plan.rows);
+  }
   return launch_status();
 }

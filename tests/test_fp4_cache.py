@@ -153,7 +153,7 @@ def test_prefill_argument_errors():
 
     def call(**over):
         args = dict(out=A, out_stride=2048, q=A, q_stride=2048, **CACHE, bt=A, bt_stride=8, bt_width=8, cu=A, kv=A,
-                    n=2, tokens=64, max_q=64, hq=16, hkv=8, d=128, scale=128 ** -0.5, stream=None)
+                    n=2, tokens=64, max_q=64, hq=16, hkv=8, d=128, scale=128 ** -0.5, ws=None, ws_bytes=0, stream=None)
         args.update(over)
         return lib.nvamd_paged_prefill_fp4(*args.values())
 
@@ -166,6 +166,17 @@ def test_prefill_argument_errors():
     assert call(d=64) == EUNSUPPORTED and call(bs=8) == EUNSUPPORTED
     assert call(bt_width=1 << 25, bt_stride=1 << 25) == EUNSUPPORTED
     assert call(bt_width=(1 << 23) + 1, bt_stride=1 << 25) == EUNSUPPORTED  # past 2^30 tokens
+    need = lib.nvamd_paged_prefill_fp4_workspace_size
+    size = need(2, 10, 16, 8, 128, 320)
+    # 2 x 8 units of 2 x 16 rows, the keys cut in 256 / 32 pieces, 528 bytes a row
+    assert size == 2 * 8 * 32 * 8 * 528
+    long = dict(max_q=10, bt_width=320, bt_stride=320)
+    assert call(**long, ws=A, ws_bytes=size - 1) == EWORKSPACE and call(**long, ws=A + 8, ws_bytes=size) == EINVAL
+    assert need(2, 10, 16, 8, 128, 31) == 0                        # short contexts
+    assert need(32, 2000, 16, 8, 128, 320) == 0                    # a full card
+    assert need(1, 1, 1, 1, 16, 1 << 20) == 16 * 32 * 528           # 32 pieces at most
+    for bad in ((0, 10, 16, 8, 128, 320), (2, 0, 16, 8, 128, 320), (2, 10, 4, 8, 128, 320), (2, 10, 16, 0, 128, 320)):
+        assert need(*bad) == 0
 
 
 # -------------------------------------------------------------------------------------------- Python entry points
