@@ -367,28 +367,32 @@ int nvamd_rms_norm_tiled(const void *x, int64_t x_stride, const void *weight,
 /* + write, paged decode, paged prefill -- over a cache of 68 instead of 256  */
 /* bytes per head vector, in the microscaling FP4 format:                     */
 /*   a head vector is 4 blocks of 32 consecutive dims.  A block's scale is    */
-/*   2^e with e the least integer for which max|x| <= 7 * 2^e, in [-125, 125]; */
-/*   its byte is e + 127, or 255 -- every value of the block reads as NaN -- if */
-/*   the block holds an infinity or a NaN.  A value's code is its sign (bit 3) */
-/*   and the nearest of 0, .5, 1, 1.5, 2, 3, 4, 6 (0..7) to |x| / 2^e, ties to */
-/*   the even code.  (A maximum between 6 and 7 steps is off by up to one step, */
-/*   as values between 4 and 6 are; the finer scale is worth more.)           */
+/*   2^e with e the least integer for which max|x| <= 7 * 2^e, in [-125,      */
+/*   125]; its byte is e + 127, or 255 -- every value of the block reads as   */
+/*   NaN -- if the block holds an infinity or a NaN.  A value's code is its   */
+/*   sign (bit 3) and the nearest of 0, .5, 1, 1.5, 2, 3, 4, 6 (0..7) to |x|  */
+/*   / 2^e, ties to the even code.  (A maximum between 6 and 7 steps is off   */
+/*   by up to one step, as values between 4 and 6 are; the finer scale is     */
+/*   worth more.)                                                             */
 /* One layer's cache is four byte arrays, 16-byte aligned:                    */
 /*   k_codes, v_codes   [num_blocks, num_kv_heads, block_size, 64]            */
 /*   k_scales, v_scales [num_blocks, num_kv_heads, block_size, 4]             */
 /* so a page of one head is contiguous.  Inside it every 16 tokens form a     */
-/* tile of 1024 bytes of codes and 64 of scales; with t = token % 16 and q the */
-/* block of 32 dims:                                                          */
+/* tile of 1024 bytes of codes and 64 of scales; with t = token % 16 and q    */
+/* the block of 32 dims:                                                      */
 /*   k_codes  byte 64 t + i: dims 2i (low nibble) and 2i + 1;                 */
 /*   k_scales byte 16 (t % 4) + 4 q + t / 4;                                  */
-/*   v_codes  byte 16 (16 q + r) + t: dims 32q + r (low) and 32q + 16 + r, r < 16; */
+/*   v_codes  byte 16 (16 q + r) + t: dims 32q + r (low) and 32q + 16 + r, r  */
+/*   < 16;                                                                    */
 /*   v_scales byte 16 q + t.                                                  */
-/* Slots, block tables, index errors, strides and alignments are as for the  */
-/* bf16 entry points; block_size a power of two >= 16.                        */
+/* Slots, block tables, index errors, strides and alignments are as for the   */
+/* bf16 entry points; block_size a power of two >= 16.  A write or read of    */
+/* 2^27 rows or more, a prefill table of more than 2^30 positions and a cache */
+/* of 2^31 tiles or more return NVAMD_EUNSUPPORTED.                           */
 /* ------------------------------------------------------------------------- */
 
-/* kv_cache_write_fp4: row t of k and v goes to slot_mapping[t] (-1: padding,  */
-/* skipped).  A call's slots are distinct: a slot named twice holds neither    */
+/* kv_cache_write_fp4: row t of k and v goes to slot_mapping[t] (-1: padding, */
+/* skipped).  A call's slots are distinct: a slot named twice holds neither   */
 /* row as a whole.                                                            */
 int nvamd_kv_cache_write_fp4(const void *k, int64_t k_stride,
                              const void *v, int64_t v_stride,
@@ -399,8 +403,9 @@ int nvamd_kv_cache_write_fp4(const void *k, int64_t k_stride,
                              int num_kv_heads, int head_dim,
                              hipStream_t stream);
 
-/* kv_cache_read_fp4: row t of k and v (bf16) = the values at slot_mapping[t];  */
-/* zeros for -1 and (reported) for a slot outside the cache.  Exact.           */
+/* kv_cache_read_fp4: row t of k and v (bf16) = the values at                 */
+/* slot_mapping[t]; zeros for -1 and (reported) for a slot outside the cache. */
+/* Exact.                                                                     */
 int nvamd_kv_cache_read_fp4(void *k, int64_t k_stride,
                             void *v, int64_t v_stride,
                             const void *k_codes, const void *k_scales,
@@ -410,14 +415,14 @@ int nvamd_kv_cache_read_fp4(void *k, int64_t k_stride,
                             int num_kv_heads, int head_dim,
                             hipStream_t stream);
 
-/* qk_norm_rope_fp4: per-head RMSNorm of q and k, then rotate-half RoPE (cos_sin */
-/* as for nvamd_qk_norm_rope), in 64-bit arithmetic with one rounding to bf16; */
-/* the rotated k (its bf16 value) and the raw v go into the cache at           */
-/* slot_mapping, the rotated q to q_out and, unless it is NULL, the rotated k  */
-/* to k_out.  q_out and k_out may be q and k themselves (same pointer and      */
-/* stride).  Padding rows (slot -1) are rotated too.  Unlike                  */
-/* nvamd_qk_norm_rope nothing is rounded on the way: not the normed value, not */
-/* cos and sin.                                                               */
+/* qk_norm_rope_fp4: per-head RMSNorm of q and k, then rotate-half RoPE       */
+/* (cos_sin as for nvamd_qk_norm_rope), in 64-bit arithmetic with one         */
+/* rounding to bf16; the rotated k (its bf16 value) and the raw v go into the */
+/* cache at slot_mapping, the rotated q to q_out and, unless it is NULL, the  */
+/* rotated k to k_out.  q_out and k_out may be q and k themselves (same       */
+/* pointer and stride).  Padding rows (slot -1) are rotated too.  Unlike      */
+/* nvamd_qk_norm_rope nothing is rounded on the way: not the normed value,    */
+/* not cos and sin.                                                           */
 int nvamd_qk_norm_rope_fp4(void *q_out, int64_t q_out_stride,
                            void *k_out, int64_t k_out_stride,
                            const void *q, int64_t q_stride,
@@ -433,10 +438,10 @@ int nvamd_qk_norm_rope_fp4(void *q_out, int64_t q_out_stride,
                            int num_heads, int num_kv_heads, int head_dim,
                            float eps, hipStream_t stream);
 
-/* paged_decode_fp4: nvamd_paged_decode over the 4-bit cache; workspace of      */
-/* nvamd_paged_decode_workspace_size bytes under the same rules (zero-filled    */
-/* once, any number of calls and replays of either kind one after another, none */
-/* that overlap).  max_context_len <= 131072.                                 */
+/* paged_decode_fp4: nvamd_paged_decode over the 4-bit cache; workspace of    */
+/* nvamd_paged_decode_workspace_size bytes under the same rules (zero-filled  */
+/* once, any number of calls and replays of either kind one after another,    */
+/* none that overlap).  max_context_len <= 131072.                            */
 int nvamd_paged_decode_fp4(void *out, int64_t out_stride,
                            const void *q, int64_t q_stride,
                            const void *k_codes, const void *k_scales,
@@ -449,14 +454,14 @@ int nvamd_paged_decode_fp4(void *out, int64_t out_stride,
                            void *workspace, size_t workspace_bytes,
                            hipStream_t stream);
 
-/* paged_prefill_fp4: nvamd_paged_prefill over the 4-bit cache.  workspace, of  */
-/* nvamd_paged_prefill_fp4_workspace_size(...) bytes (0: none needed), any      */
-/* contents, of this call's own while it runs, lets few rows on long contexts   */
-/* be cut along the keys; NULL runs them uncut.  |q . k| scale below 2^29.  A NaN of the */
-/* cache reaches the rows that see its key and no others.  A sequence whose    */
-/* rows leave [0, num_tokens) is skipped, and it, a q_len past max_q_len (whose */
-/* further rows are not written) and a kv_len below q_len are reported as       */
-/* NVAMD_ERR_CONTEXT.                                                         */
+/* paged_prefill_fp4: nvamd_paged_prefill over the 4-bit cache.  workspace,   */
+/* of nvamd_paged_prefill_fp4_workspace_size(...) bytes (0: none needed), any */
+/* contents, of this call's own while it runs, lets few rows on long contexts */
+/* be cut along the keys; NULL runs them uncut.  |q . k| scale below 2^29.  A */
+/* NaN of the cache reaches the rows that see its key and no others.  A       */
+/* sequence whose rows leave [0, num_tokens) is skipped, and it, a q_len past */
+/* max_q_len (whose further rows are not written) and a kv_len below q_len    */
+/* are reported as NVAMD_ERR_CONTEXT.                                         */
 int nvamd_paged_prefill_fp4(void *out, int64_t out_stride,
                             const void *q, int64_t q_stride,
                             const void *k_codes, const void *k_scales,

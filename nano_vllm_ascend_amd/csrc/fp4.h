@@ -17,16 +17,16 @@ constexpr int kFp4TileScales = kFp4Tile * kFp4Scales;
 constexpr u32 kFp4Nan = 255;                // scale byte of a block that holds an infinity or a NaN
 
 // Scale byte of a block whose largest |x| has the bf16 bits `amax` (sign cleared): the least e with
-// max <= 7 * 2^e is the maximum's own exponent - 2, or one more where its fraction is past 1.75 = 7 / 4.  Within [2, 252],
-// so that every value and its product with the largest code are normal, finite bf16 numbers.
+// max <= 7 * 2^e is the maximum's own exponent - 2, or one more where its fraction is past 1.75 = 7 / 4.  Within [2,
+// 252], so that every value and its product with the largest code are normal, finite bf16 numbers.
 __device__ __forceinline__ u32 fp4_scale_byte(u32 amax) {
   const int e = (int)(amax >> 7) - 2 + ((amax & 0x7f) > 0x60 ? 1 : 0);
   return amax >= 0x7f80u ? kFp4Nan : (u32)min(max(e, 2), 252);
 }
 __device__ __forceinline__ float fp4_scale(u32 byte) { return __uint_as_float(byte << 23); }
 
-// The codes of 8 bf16 values at a scale (element 0 in the low nibble): v_cvt_scalef32_pk_fp4_bf16 rounds to nearest, ties
-// to the even code, and saturates at 6 (checked on gfx950 over every bf16 value).
+// The codes of 8 bf16 values at a scale (element 0 in the low nibble): v_cvt_scalef32_pk_fp4_bf16 rounds to nearest,
+// ties to the even code, and saturates at 6 (checked on gfx950 over every bf16 value).
 template <int B>
 __device__ __forceinline__ u32 fp4_put_pair(u32 codes, u32 pair, float scale) {
   return __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(codes, __builtin_bit_cast(bf16x2v, pair), scale, B);

@@ -29,18 +29,18 @@ __device__ __forceinline__ float sum_over_quarters(float v) {
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 
-// S += K . q for 16 rows of codes (128 dims) and 16 columns of e4m3, each block of 32 dims under its scale byte.  Lane (row
-// or column n, gq) gives block gq of its row, dims 16 gq .. +15 and 64 + 16 gq .. +15 of its column, and the scales of
-// block gq of either, the row's in byte B of a word (checked on gfx950).
+// S += K . q for 16 rows of codes (128 dims) and 16 columns of e4m3, each block of 32 dims under its scale byte.  Lane
+// (row or column n, gq) gives block gq of its row, dims 16 gq .. +15 and 64 + 16 gq .. +15 of its column, and the
+// scales of block gq of either, the row's in byte B of a word (checked on gfx950).
 template <int B>
 __device__ __forceinline__ f32x4 mfma_fp4_fp8(u32x4 k, u32 k_scales, i32x8 q, u32 q_scale, f32x4 c) {
   const i32x8 codes = {(int)k[0], (int)k[1], (int)k[2], (int)k[3], 0, 0, 0, 0};
   return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(codes, q, c, 4, 0, B, (int)k_scales, 0, (int)q_scale);
 }
 
-// A block of 32 bf16 query values as hi + lo in e4m3 under 2^-s, s from its largest value, which lands in [128, 256).  hi
-// keeps 4 of the 8 significant bits and lo the rest: the sum is the value itself down to 2^-9 of the block's largest, and off
-// by at most 2^-17 of the largest below.
+// A block of 32 bf16 query values as hi + lo in e4m3 under 2^-s, s from its largest value, which lands in [128, 256).
+// hi keeps 4 of the 8 significant bits and lo the rest: the sum is the value itself down to 2^-9 of the block's
+// largest, and off by at most 2^-17 of the largest below.
 struct QueryScale {
   float up;  // 2^s
   u32 byte;  // of 2^-s; 255, which makes every score NaN, for a block with an infinity or a NaN
@@ -151,7 +151,8 @@ __device__ __forceinline__ u32x4 load16(const u8 *p) {
 __device__ __forceinline__ u32 keep_bytes(u32 v, int n) {
   return n >= 4 ? v : n <= 0 ? 0u : v & ((1u << (8 * n)) - 1u);
 }
-// The operands of V^T for 4 tokens (a word of codes) of a dim pair: bf16 pairs of tokens, of the first and of the second dim.
+// The operands of V^T for 4 tokens (a word of codes) of a dim pair: bf16 pairs of tokens, of the first and of the
+// second dim.
 __device__ __forceinline__ void expand4(u32 codes, u32 scales, u32 &a01, u32 &a23, u32 &b01, u32 &b23) {
   const u32 v0 = fp4_pair<0>(codes, scale_of<0>(scales)), v1 = fp4_pair<1>(codes, scale_of<1>(scales));
   const u32 v2 = fp4_pair<2>(codes, scale_of<2>(scales)), v3 = fp4_pair<3>(codes, scale_of<3>(scales));
@@ -161,8 +162,9 @@ __device__ __forceinline__ void expand4(u32 codes, u32 scales, u32 &a01, u32 &a2
   b23 = pair_hi(v2, v3);
 }
 
-// o[2q], o[2q + 1] += V^T P^T for dims 32q .. 32q+31 and the 64 tokens of a wave's step (lane (n, gq): codes of dims 32q + n and
-// 32q + 16 + n of the 16 tokens of tile gq, v_scales the scales of block n / 4, tokens 4 (n % 4) .. +3 of that tile).
+// o[2q], o[2q + 1] += V^T P^T for dims 32q .. 32q+31 and the 64 tokens of a wave's step (lane (n, gq): codes of dims
+// 32q + n and 32q + 16 + n of the 16 tokens of tile gq, v_scales the scales of block n / 4, tokens 4 (n % 4) .. +3 of
+// that tile).
 template <int Q>
 __device__ __forceinline__ void add_values(f32x4 (&o)[8], const u32x4 (&codes)[4], u32 v_scales, const u32x4 (&p)[2]) {
   const u32 sc[4] = {dpp_u32<kRowBcast + 4 * Q>(v_scales), dpp_u32<kRowBcast + 4 * Q + 1>(v_scales),

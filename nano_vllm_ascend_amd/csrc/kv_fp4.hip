@@ -1,15 +1,15 @@
 // The 4-bit paged KV cache: writing rows, reading rows back, and the per-head QK-RMSNorm + RoPE that
 // writes them in the same pass (the 4-bit counterparts of kv_store.hip).
 //
-// A wave takes 8 consecutive tokens, an aligned group of 8 lanes each, and one head or a run of them: rows of a head that
-// follow one another in a page are written together, and the 8 tokens of a head's values meet in LDS so that bytes of
-// consecutive tokens leave as one store.  Of a head vector, lane c of a group holds dims 8c..8c+7 and 64+8c..64+8c+7: a block
-// of 32 dims is the low (or high) half of 4 consecutive lanes, its maximum two DPP steps away, and RoPE needs no lane
-// exchange.
+// A wave takes 8 consecutive tokens, an aligned group of 8 lanes each, and one head or a run of them: rows of a head
+// that follow one another in a page are written together, and the 8 tokens of a head's values meet in LDS so that bytes
+// of consecutive tokens leave as one store.  Of a head vector, lane c of a group holds dims 8c..8c+7 and
+// 64+8c..64+8c+7: a block of 32 dims is the low (or high) half of 4 consecutive lanes, its maximum two DPP steps away,
+// and RoPE needs no lane exchange.
 //
-// All three are bound by memory: per head vector 256 bytes of bf16 and 68 of the cache, once.  36,488 tokens, 8 kv heads (and 16
-// query heads): write 189 MB in 40 us (4.7 TB/s), read 189 MB in 38 us (5.0 TB/s), norm + RoPE + write with the keys
-// returned 564 MB in 118 us (4.8 TB/s); a large copy reaches 5.0 TB/s.  One token: 3 us, the launch.
+// All three are bound by memory: per head vector 256 bytes of bf16 and 68 of the cache, once.  36,488 tokens, 8 kv
+// heads (and 16 query heads): write 189 MB in 40 us (4.7 TB/s), read 189 MB in 38 us (5.0 TB/s), norm + RoPE + write
+// with the keys returned 564 MB in 118 us (4.8 TB/s); a large copy reaches 5.0 TB/s.  One token: 3 us, the launch.
 #include "fp4.h"
 
 namespace nvamd {
@@ -67,9 +67,9 @@ __device__ __forceinline__ void store_key(const Fp4Cache &cache, const Fp4Row &r
   }
 }
 
-// A byte of the values holds dims 32q + r and 32q + 16 + r: the two lanes of a quad that differ in bit 1 hold the two halves
-// of a block, and exchange so that the one builds the bytes of the low block, the other those of the high one.  The bytes go to
-// `tile` in LDS, [64 bytes of a row][8 tokens], at token `tok`.
+// A byte of the values holds dims 32q + r and 32q + 16 + r: the two lanes of a quad that differ in bit 1 hold the two
+// halves of a block, and exchange so that the one builds the bytes of the low block, the other those of the high one.
+// The bytes go to `tile` in LDS, [64 bytes of a row][8 tokens], at token `tok`.
 __device__ __forceinline__ void value_bytes(const Fp4Cache &cache, const Fp4Row &r, bool live, int c, int tok, u32x4 lo,
                                             u32x4 hi, u8 *tile) {
   u32 s_lo, s_hi;
@@ -94,8 +94,9 @@ __device__ __forceinline__ void value_bytes(const Fp4Cache &cache, const Fp4Row 
   }
 }
 
-// The 8 tokens' bytes of row byte `lane` to their slots.  Where the slots follow one another the bytes are turned to their
-// places in 8-byte half rows: one store if they fill one, else those of each side of the border, words where whole.
+// The 8 tokens' bytes of row byte `lane` to their slots.  Where the slots follow one another the bytes are turned to
+// their places in 8-byte half rows: one store if they fill one, else those of each side of the border, words where
+// whole.
 __device__ __forceinline__ void store_values(const Fp4Cache &cache, const u8 *tile, int64_t slot, bool run, int head,
                                              int num_kv_heads, int bs_log2, int lane) {
   auto place = [&](int64_t s) {  // of the byte of slot s
@@ -136,9 +137,9 @@ __device__ __forceinline__ void store_values(const Fp4Cache &cache, const u8 *ti
 // A wave's own LDS writes before its own reads: LDS serves a wave in order, so only the compiler has to keep it.
 __device__ __forceinline__ void wave_lds_fence() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); }
 
-// Rows too many for the caches until their next use go past them (32 MB a tensor: half of the 256 MB Infinity Cache for two
-// tensors in and out).  36,488 x 8 heads, plain / nontemporal: written 43.8 / 39.2 us, read 46.5 / 38.2; 12,345 x 8 heads
-// written and read back 27.6 / 31.9.
+// Rows too many for the caches until their next use go past them (32 MB a tensor: half of the 256 MB Infinity Cache for
+// two tensors in and out).  36,488 x 8 heads, plain / nontemporal: written 43.8 / 39.2 us, read 46.5 / 38.2; 12,345 x 8
+// heads written and read back 27.6 / 31.9.
 constexpr int64_t kStreamElems = 16 << 20;
 template <bool STREAM>
 __device__ __forceinline__ void put16(u16 *p, u32x4 v) {
@@ -153,9 +154,9 @@ __device__ __forceinline__ u32x4 get16(const u16 *p) {
   else return ld16(p);
 }
 
-// Heads that a wave of the rotation takes one after another: the table's row, the weights and the slots are read once for
-// them.  Fewer where that leaves less than four waves for each SIMD of 256 CUs.  (36,488 tokens: 118 us with 8 or 4, 142 with 2.)
-// Without the rotation a wave has one head (8: 42.2 us, 1: 40.1; 12,345 tokens 17.6, 16.7).
+// Heads that a wave of the rotation takes one after another: the table's row, the weights and the slots are read once
+// for them.  Fewer where that leaves less than four waves for each SIMD of 256 CUs.  (36,488 tokens: 118 us with 8 or
+// 4, 142 with 2.) Without the rotation a wave has one head (8: 42.2 us, 1: 40.1; 12,345 tokens 17.6, 16.7).
 constexpr int kRopeHeads = 8;
 constexpr int kWantedWaves = 4096;
 
@@ -188,9 +189,9 @@ struct ReadArgs {
   u32 *err;
 };
 
-// The other way round.  A wave takes one key or value head of 8 tokens: it waits for its loads once, and more waves are all
-// that hides that (36,488 x 8 heads: 50 us with 8 heads one after another, 45 with 2, 37.4 so).  A row without a slot, or with one
-// outside the cache, is zeros.
+// The other way round.  A wave takes one key or value head of 8 tokens: it waits for its loads once, and more waves are
+// all that hides that (36,488 x 8 heads: 50 us with 8 heads one after another, 45 with 2, 37.4 so).  A row without a
+// slot, or with one outside the cache, is zeros.
 template <bool STREAM>
 __global__ void __launch_bounds__(256)
 kv_read_fp4_kernel(ReadArgs a) {
@@ -295,8 +296,9 @@ __device__ __forceinline__ double dpp_sum8(double v) {
   return dpp_sum<kDppHalfMirror>(dpp_sum<kDppQuadXor2>(dpp_sum<kDppQuadXor1>(v)));
 }
 
-// A 32-bit value that rounds to bf16 as x does.  A plain cast rounds too, and may land on a border of bf16 that x is only close
-// to; here all but the top 20 bits of the fraction are cut off, and the last of these is set if any of the rest was.
+// A 32-bit value that rounds to bf16 as x does.  A plain cast rounds too, and may land on a border of bf16 that x is
+// only close to; here all but the top 20 bits of the fraction are cut off, and the last of these is set if any of the
+// rest was.
 __device__ __forceinline__ float bf16_bound(double x) {
   const uint64_t b = __builtin_bit_cast(uint64_t, x);
   const uint64_t top = (uint64_t)((u32)(b >> 32) | ((u32)b != 0u ? 1u : 0u)) << 32;
@@ -305,8 +307,8 @@ __device__ __forceinline__ float bf16_bound(double x) {
 
 // y = x * rsqrt(mean(x^2) + eps) * w, then the rotation out[d] = y[d] cos[d] - y[d+64] sin[d], out[d+64] = y[d+64]
 // cos[d] + y[d] sin[d], in 64 bits with one rounding to bf16 at the end.  A 4-bit code's step is a
-// third to a half of the value, so a key that 32-bit arithmetic puts on the other side of a rounding border is that far off;
-// in 64 bits the code is that of the exact value.  x w is a product of bf16 numbers, exact in 32 bits, and the
+// third to a half of the value, so a key that 32-bit arithmetic puts on the other side of a rounding border is that far
+// off; in 64 bits the code is that of the exact value.  x w is a product of bf16 numbers, exact in 32 bits, and the
 // reciprocal root comes last: one multiplication for each result.
 __device__ __forceinline__ void norm_rope_f64(u32x4 &lo, u32x4 &hi, const u32x4 w_lo, const u32x4 w_hi,
                                               const float (&cs)[8], const float (&sn)[8], double eps) {
@@ -407,8 +409,8 @@ rows_fp4_kernel(NormRopeFp4Args a) {
     }
     const bool is_q = v < hq;
     if constexpr (ROPE) {
-      // Keeps the conversions of the row's 16 numbers and of the weights inside the loop: hoisted, they would hold 64 registers
-      // and with them a third of the waves.
+      // Keeps the conversions of the row's 16 numbers and of the weights inside the loop: hoisted, they would hold 64
+      // registers and with them a third of the waves.
 #pragma unroll
       for (int e = 0; e < 8; ++e) asm volatile("" : "+v"(cs[e]), "+v"(sn[e]));
       asm volatile("" : "+v"(qw_lo), "+v"(qw_hi), "+v"(kw_lo), "+v"(kw_hi));
@@ -424,8 +426,8 @@ rows_fp4_kernel(NormRopeFp4Args a) {
   }
 }
 
-// A workgroup is 8 tokens x 4 waves' heads.  A wave takes up to `per_wave` heads; fewer where that leaves too few waves to fill
-// the card.  0: more than a launch takes.
+// A workgroup is 8 tokens x 4 waves' heads.  A wave takes up to `per_wave` heads; fewer where that leaves too few waves
+// to fill the card.  0: more than a launch takes.
 int heads_per_wave(int num_tokens, int vecs, int per_wave, dim3 *grid) {
   const int64_t octets = ((int64_t)num_tokens + 7) / 8;
   while (per_wave > 1 && octets * ceil_div(vecs, per_wave) < kWantedWaves) per_wave >>= 1;

@@ -3,25 +3,31 @@
 // For a query token of each sequence and its heads h of kv head g: out = softmax(q . K^T * scale) V over the cached
 // context.
 //
-// Work: a unit (sequence, kv head) is cut into partitions of equal length, a workgroup of 8 waves each.  Every workgroup
-// reads the context lengths and derives the same length from them (part_tokens), so the cut follows the contexts themselves
-// and not the bound that the launch was made with.  A partition leaves (max, sum, numerator) per head in the
-// workspace and counts its arrival; the last one of a unit joins them.
+// Work: a unit (sequence, kv head) is cut into partitions of equal length, a workgroup of 8 waves each.  Every
+// workgroup reads the context lengths and derives the same length from them (partition_tokens), so the cut follows the
+// contexts themselves and not the bound that the launch was made with.  A partition leaves (max, sum, numerator) per
+// head in the workspace and counts its arrival; the last one of a unit joins them.
 //
 // A wave takes 64 tokens at a time, four 16-token tiles, one per 16 lanes (gq = lane / 16):
-//   S^T = K . Q^T  v_mfma_scale_f32_16x16x128_f8f6f4 on the codes as they lie in the cache, A = 16 rows of K: a lane's 16
-//        bytes are one block of a row, under one scale.  B = the heads as 16 columns, in 8 bits twice: a bf16 query is the sum
-//        of two e4m3 numbers under a common scale (QueryScale), so two products give the scores.  That takes the matrix
-//        cores as long as four bf16 products, and the vector ALUs no expansion of K.
+//   S^T = K . Q^T  v_mfma_scale_f32_16x16x128_f8f6f4 on the codes as they lie in the cache, A = 16 rows of K: a lane's
+//        16 bytes are one block of a row, under one scale.  B = the heads as 16 columns, in 8 bits twice: a bf16 query
+//        is the sum of two e4m3 numbers under a scale for each block (QueryScale), so two products give the scores.  That takes
+//        the matrix cores as long as four bf16 products, and the vector ALUs no expansion of K.
 //        Row 4a + i of product t is token 4t + i of tile a: lane (h, gq) then finds the scores of tile gq's tokens
 //        4t .. 4t+3 of head h in its accumulator of product t, that is of all 16 tokens in the four products;
-//   softmax  on up to 4 (8) heads the accumulators' 16 columns are mostly repeats: products 1..3 (2, 3) move into the idle
-//        columns by DPP, and one lane does 4 (8) scores instead of 16;
-//   O^T += V^T . P^T  v_mfma_f32_16x16x32_bf16, A = 16 dims of V^T expanded by v_cvt_scalef32_pk_bf16_fp4 (two values and
-//        their scale in one instruction, exact), B = P^T, whose 8 k-slots per lane are tokens 0..7 (8..15) of tile gq: just
-//        what the lane holds.  The cache keeps V with 16 tokens of a dim pair in consecutive bytes, so the lane's
-//        16 bytes give both products' operands of two dims: no lane movement.
-// The score of a token past the context is replaced by -inf and the scales of its values by zero, whatever bytes it holds.
+//   softmax  on up to 4 (8) heads the accumulators' 16 columns are mostly repeats: products 1..3 (2, 3) move into the
+//        idle columns by DPP, and one lane does 4 (8) scores instead of 16;
+//   O^T += V^T . P^T  v_mfma_f32_16x16x32_bf16, A = 16 dims of V^T expanded by v_cvt_scalef32_pk_bf16_fp4 (two values
+//        and their scale in one instruction, exact), B = P^T, whose 8 k-slots per lane are tokens 0..7 (8..15) of tile
+//        gq: just what the lane holds.  The cache keeps V with 16 tokens of a dim pair in consecutive bytes, so the
+//        lane's 16 bytes give both products' operands of two dims: no lane movement.
+// The score of a token past the context is replaced by -inf and the scales of its values by zero, whatever bytes it
+// holds.
+//
+// Bound by memory where contexts are long: 100 x U[2048, 4096] tokens of 8 kv heads, 330 MB, 59 .. 63 us (5.2 .. 5.6 TB/s,
+// part of it from the Infinity Cache; a large copy 5.0); 4 x U[8192, 40960], 91 MB, 21 us.  Below that by what every call
+// pays: some 2 us of launch, 1.3 to the first load (contexts, table, query) and 2 to 4 for the join: 32 x U[256, 2304],
+// 46 MB, 16 us, 4 x U[1, 512] 6.2.
 #include "fp4_attention.h"
 
 namespace nvamd {
@@ -76,15 +82,15 @@ __device__ __forceinline__ int wave_scan(int v, int lane) {
   return v + (row >= 1 ? r0 : 0) + (row >= 2 ? r1 : 0) + (row >= 3 ? r2 : 0);
 }
 
-// Cutting units of `tokens` tokens in all every `length` tokens ends in tokens / length + units / 2 partitions on average,
-// and in a whole unit more than the quotient each at most.  The length is chosen for this quotient (share):
-//   few units: partitions fill the card once, with one workgroup on each CU while that leaves two per unit, else two.  Anything
-//     between one and two workgroups per CU has half of the CUs do double the work;
-//   many units: twice the mean context.  Units then go round by themselves, and only contexts far longer than the others
-//     are cut.
-// Measured (us): 4 x U[8192, 40960] at 8 kv heads 20.9 with one workgroup per CU, 22.8 with two, 25.8 where the length was the
-// next power of two; 16 x U[512, 4096] at 8 groups of 8 heads 13.9 either way (16.4); 32 x U[256, 2304] at 8 kv heads 21.7
-// uncut, 16.0 with two (16.7); 100 x U[2048, 4096] 63 uncut, 76 cut in two.
+// Cutting units of `tokens` tokens in all every `length` tokens ends in tokens / length + units / 2 partitions on
+// average, and in a whole unit more than the quotient each at most.  The length is chosen for this quotient (share):
+//   few units: partitions fill the card once, with one workgroup on each CU while that leaves two per unit, else two.
+//     Anything between one and two workgroups per CU has half of the CUs do double the work;
+//   many units: twice the mean context.  Units then go round by themselves, and only contexts far longer than the
+//     others are cut.
+// Measured (us): 4 x U[8192, 40960] at 8 kv heads 20.9 with one workgroup per CU, 22.8 with two, 25.8 where the length
+// was the next power of two; 16 x U[512, 4096] at 8 groups of 8 heads 13.9 either way (16.4); 32 x U[256, 2304] at 8 kv
+// heads 21.7 uncut, 16.0 with two (16.7); 100 x U[2048, 4096] 63 uncut, 76 cut in two.
 __host__ __device__ constexpr int partition_share(int units) {
   const int slots = units * 2 <= kCus ? kCus : 2 * kCus;
   return slots - units / 2 > units / 2 ? slots - units / 2 : units / 2;
@@ -96,8 +102,9 @@ __device__ __forceinline__ int partition_tokens(u32 tokens, int units) {  // a m
 }
 __host__ __device__ constexpr int max_partitions(int units) { return partition_share(units) + units; }
 
-// GP: heads that the registers and LDS are laid out for.  WIDE: pages of 64 tokens or more, so that the 64 tokens of a wave's
-// step lie in one page, whose id is a scalar.
+// GP: heads that the registers and LDS are laid out for (2 heads at 4 x U[1, 512]: 6.2 us as 4, 6.5 as 16; at 100 x
+// U[2048, 4096] 63.2, 63.6).  WIDE: pages of 64 tokens or more, so that the 64 tokens of a wave's step lie in one page,
+// whose id is a scalar (pages of 128 at 32 x U[256, 2304]: 16.3 us, without 20.8; at 100 x U[2048, 4096] 63, 73).
 template <int GP, bool WIDE>
 __global__ void __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(WIDE ? 4 : 3)))
 paged_decode_fp4_kernel(DecodeFp4Args a) {
@@ -171,8 +178,8 @@ paged_decode_fp4_kernel(DecodeFp4Args a) {
 #pragma unroll
   for (int e = 0; e < 8; ++e) o[e] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-  // A step's 64 tokens are the four tiles t0 .. t0+63.  The tile of each 16 lanes, as row owners of K (tile n / 4) and as token
-  // owners of V (tile gq); tiles past the context repeat its last one.
+  // A step's 64 tokens are the four tiles t0 .. t0+63.  The tile of each 16 lanes, as row owners of K (tile n / 4) and
+  // as token owners of V (tile gq); tiles past the context repeat its last one.
   typedef const __attribute__((address_space(4))) int32_t const_i32;  // nothing writes the table: scalar loads
   const_i32 *bt = (const_i32 *)bt_row;
   const int t_end = min((p + 1) * part_tokens, ctx);
@@ -226,8 +233,8 @@ paged_decode_fp4_kernel(DecodeFp4Args a) {
     vs = *reinterpret_cast<const u32 *>(in_tiles(a.cache.v_scales, v_tile, kFp4TileScales, 4 * n));
   };
 
-  // K of the next step is asked for as soon as the scores have taken this step's, V as soon as the products have: each is in
-  // flight during the other half of the step, without registers of its own.
+  // K of the next step is asked for as soon as the scores have taken this step's, V as soon as the products have: each
+  // is in flight during the other half of the step, without registers of its own.
   auto step = [&](const int t0, const int next) {
     constexpr int NP = GP <= 4 ? 1 : GP <= 8 ? 2 : 4;  // accumulators that hold all scores once packed
     f32x4 s[4];
@@ -289,8 +296,8 @@ paged_decode_fp4_kernel(DecodeFp4Args a) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) o[e] *= alpha;
     }
-    // P rounded to bf16 for the matrix cores; the sum takes the same rounded values.  Back in the order of the products, the
-    // columns past the heads hold weights of other tokens and give numerators that are never read.
+    // P rounded to bf16 for the matrix cores; the sum takes the same rounded values.  Back in the order of the
+    // products, the columns past the heads hold weights of other tokens and give numerators that are never read.
     u32x4 pf[2];
 #pragma unroll
     for (int x = 0; x < NP; ++x)

@@ -1,30 +1,33 @@
-// Causal prefill attention over the 4-bit paged KV cache (the counterpart of prefill.hip's paged route): the queries are
-// the last q_len positions of a context of kv_len, query row r sees keys 0 .. kv_len - q_len + r, all of them in the cache.
+// Causal prefill attention over the 4-bit paged KV cache (the counterpart of prefill.hip's paged route): the queries
+// are the last q_len positions of a context of kv_len, query row r sees keys 0 .. kv_len - q_len + r, all of them in
+// the cache.
 //
 // The G query heads of a kv head and the q_len tokens make q_len * G rows, R = token * G + head, that share the keys; a
 // workgroup takes rows that follow one another, whatever G is.  In all kernels
 //   S^T = K . Q^T   v_mfma_scale_f32_*_f8f6f4 on the codes as they lie in the cache: a lane loads 32 dims of a key and their
-//        scale straight into the operand, and the row comes as two e4m3 numbers per value (fp4_attention.h).  No expansion
-//        of K, and none of it in LDS;
+//        scale straight into the operand, and the row comes as two e4m3 numbers per value (fp4_attention.h).  No
+//        expansion of K, and none of it in LDS;
 //   O^T += V^T . P^T   v_mfma_f32_*_bf16 on V expanded by v_cvt_scalef32_pk_bf16_fp4, exact.
-// The rows of K are taken in such an order that a lane's registers of S^T are the consecutive keys that its operand of P^T
-// needs: a repack in registers.  Three kernels, which differ in how many rows share an expansion of V:
+// The rows of K are taken in such an order that a lane's registers of S^T are the consecutive keys that its operand of
+// P^T needs: a repack in registers.  Three kernels, which differ in how many rows share an expansion of V:
 //
-// Tiles (the card is full).  Workgroup = 4 waves = 128 rows, a wave 32 of them, tiles of 32 keys.  The workgroup expands a
-//   tile of V once, to bf16 operands in LDS (every access is 64 lanes x 16 consecutive bytes): a wave takes 8 tokens of a
-//   16-token tile, a lane a dim pair of them.  Key 16a + 8b + 4c + x sits in row 16a + 8c + 4b + x of K.  K of the next tile
-//   loads as the scores have taken this one's, V's codes are two tiles ahead, V's operands one (two stages, one barrier a tile).
-//   Bound by issue: the matrix cores are busy 43.5% of the time and the vector ALUs (exponents, rounding, expansion) 55%, one or
-//   the other at 98.5% of it.  32 x U[512, 2048] rows on 1,152 cached keys 689 us (895 TFLOP/s), 2 x U[3000, 4000] rows of 40
-//   query heads on 4,096 972 us (1,022 TFLOP/s); a bf16 matrix product of 8,192^3 reaches 1,254.
+// Tiles (the card is full).  Workgroup = 4 waves = 128 rows, a wave 32 of them, tiles of 32 keys.  The workgroup
+//   expands a tile of V once, to bf16 operands in LDS (every access is 64 lanes x 16 consecutive bytes): a wave takes 8
+//   tokens of a 16-token tile, a lane a dim pair of them.  Key 16a + 8b + 4c + x sits in row 16a + 8c + 4b + x of K.  K
+//   of the next tile loads as the scores have taken this one's, V's codes are two tiles ahead, V's operands one (two
+//   stages, one barrier a tile). Bound by issue: the matrix cores are busy 43.5% of the time and the vector ALUs
+//   (exponents, rounding, expansion) 55%, one or the other at 98.5% of it.  32 x U[512, 2048] rows on 1,152 cached keys
+//   689 us (895 TFLOP/s), 2 x U[3000, 4000] rows of 40 query heads on 4,096 972 us (1,022 TFLOP/s); a bf16 matrix
+//   product of 8,192^3 reaches 1,254.
 //
-// Strips (one long prompt, or several short ones).  Workgroup = 4 waves = 32 rows, a wave every fourth 32 keys; no barrier in the
-//   loop, the waves' results meet in LDS.  A lane expands 16 tokens of a dim pair straight into operands: four times the
-//   tile kernel's expansion for each row, for four times the workgroups.  1 x 4,000 rows on 4,096 keys 232 us (859 TFLOP/s).
+// Strips (one long prompt, or several short ones).  Workgroup = 4 waves = 32 rows, a wave every fourth 32 keys; no
+//   barrier in the loop, the waves' results meet in LDS.  A lane expands 16 tokens of a dim pair straight into
+//   operands: four times the tile kernel's expansion for each row, for four times the workgroups.  1 x 4,000 rows on
+//   4,096 keys 232 us (859 TFLOP/s).
 //
-// Few rows (a chat's next turn).  Workgroup = 8 waves = 16 rows, a wave every eighth 64 keys, as in paged_decode_fp4.hip with rows
-//   in the place of heads and a last key for each row.  Bound by the latency of a launch and of a wave's steps: 8 x 20 rows on
-//   1,040 keys 10 us.  On long contexts the keys are cut as well.
+// Few rows (a chat's next turn).  Workgroup = 8 waves = 16 rows, a wave every eighth 64 keys, as in
+//   paged_decode_fp4.hip with rows in the place of heads and a last key for each row.  Bound by the latency of a launch
+//   and of a wave's steps: 8 x 20 rows on 1,040 keys 10 us.  On long contexts the keys are cut as well.
 //
 // A block of values that reads as NaN must reach the rows that see its key and no others, though masked rows
 // multiply it by a weight of zero: such values enter the products as zeros, and the rows that see
@@ -66,8 +69,8 @@ struct Rows {
   int offset;  // token t sees keys 0 .. offset + t
   int first;   // the workgroup's first row
 };
-// The y-th group of rows from a sequence's end: those with the most keys start first.  False if it has none.  Faults are
-// reported once per sequence.
+// The y-th group of rows from a sequence's end: those with the most keys start first.  False if it has none.  Faults
+// are reported once per sequence.
 __device__ __forceinline__ bool find_rows(const PrefillFp4Args &a, int per_group, int y, Rows &r) {
   const int s = blockIdx.z;
   r.q_start = a.cu_seqlens_q[s];
@@ -126,8 +129,8 @@ __device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8v, a), __builtin_bit_cast(bf16x8v, b), c, 0,
                                                  0, 0);
 }
-// 64 dims: lane (n, half) gives block `half` of them of row n, dims 16 half .. +15 and 32 + 16 half .. +15 of column n, and the
-// scales of block `half` of either (checked on gfx950).
+// 64 dims: lane (n, half) gives block `half` of them of row n, dims 16 half .. +15 and 32 + 16 half .. +15 of column n,
+// and the scales of block `half` of either (checked on gfx950).
 __device__ __forceinline__ f32x16 mfma32_fp4_fp8(u32x4 k, u32 k_scale, i32x8 q, u32 q_scale, f32x16 c) {
   const i32x8 codes = {(int)k[0], (int)k[1], (int)k[2], (int)k[3], 0, 0, 0, 0};
   return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(codes, q, c, 4, 0, 0, (int)k_scale, 0, (int)q_scale);
@@ -162,7 +165,8 @@ struct Stage {
 };
 constexpr int kRowPad = kHeadDim + 8;  // elements of a row in the output's turn: 16 bytes of padding spread the banks
 
-// WIDE: pages of 32 tokens or more, so that a tile's keys lie in one page and K loads from a scalar address.
+// WIDE: pages of 32 tokens or more, so that a tile's keys lie in one page and K loads from a scalar address (702 us, 705
+// without, where the header counts 689; the strips gain nothing by it).
 template <bool WIDE>
 __global__ void __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(3)))
 prefill_fp4_kernel(PrefillFp4Args a) {
@@ -351,7 +355,8 @@ prefill_fp4_kernel(PrefillFp4Args a) {
     load_v();
     look_up(2);
     __syncthreads();
-    // Here K holds tile t, V's registers tile t + 1, stage t % 2 V's operands of tile t; `tile` is t + 1's, `entry` t + 2's.
+    // Here K holds tile t, V's registers tile t + 1, stage t % 2 V's operands of tile t; `tile` is t + 1's, `entry` t +
+    // 2's.
 #pragma unroll 1
     for (int t = 0; t < n_tiles; ++t) {
       const bool visible = r0 < rows.rows && t * kBK <= wave_last;
@@ -407,8 +412,8 @@ prefill_fp4_kernel(PrefillFp4Args a) {
 constexpr int kStripWaves = 4;
 constexpr int kStripRows = 32;
 
-// acc[2 J], acc[2 J + 1] += V^T P^T for row bytes 32 J .. +31 and 32 tokens (lane (n, half): 16 tokens of tile `half`; scales in
-// lanes 4 J .. 4 J + 3 of each 16).
+// acc[2 J], acc[2 J + 1] += V^T P^T for row bytes 32 J .. +31 and 32 tokens (lane (n, half): 16 tokens of tile `half`;
+// scales in lanes 4 J .. 4 J + 3 of each 16).
 template <int J>
 __device__ __forceinline__ void add_strip(f32x16 (&acc)[4], u32x4 codes, u32 v_scales, const u32x4 (&p)[2]) {
   const u32 sc[4] = {dpp_u32<kRowBcast + 4 * J>(v_scales), dpp_u32<kRowBcast + 4 * J + 1>(v_scales),
@@ -423,7 +428,6 @@ __device__ __forceinline__ void add_strip(f32x16 (&acc)[4], u32x4 codes, u32 v_s
   }
 }
 
-template <bool WIDE>
 __global__ void __launch_bounds__(kStripWaves * 64) __attribute__((amdgpu_waves_per_eu(3)))
 prefill_strip_fp4_kernel(PrefillFp4Args a) {
   constexpr int D = kHeadDim;
@@ -467,20 +471,15 @@ prefill_strip_fp4_kernel(PrefillFp4Args a) {
     for (int x = 0; x < 2; ++x) tile[x] = tile_of(a, entry[x], min(t0 + 16 * x, last_tile), g, lane == 0);
   };
   // Byte `at` of the lane's one of the two tiles.
-  auto in_tile = [&](const u8 *base, u32 second, int tile_bytes, u32 at) {
-    if constexpr (WIDE) {
-      const u32 d = (u32)(tile[1] - tile[0]);  // 1, or 0 past the keys
-      return base + (int64_t)tile[0] * tile_bytes + (at + (second & (d * tile_bytes)));
-    } else {
-      return base + (int64_t)(second ? tile[1] : tile[0]) * tile_bytes + at;
-    }
+  auto in_tile = [&](const u8 *base, int second, int tile_bytes, u32 at) {  // (second as a bool: 25 us for 14)
+    return base + (int64_t)(second ? tile[1] : tile[0]) * tile_bytes + at;
   };
   // Row n of K is token 4 (n / 8) + n % 4 of tile (n / 4) % 2: then register i of the scores is token i of tile `half`.
   const int k_token = 4 * (n >> 3) + (n & 3);
-  const u32 k_second = (n & 4) ? ~0u : 0u, v_second = half ? ~0u : 0u;
+  const int k_second = (n & 4) ? -1 : 0, v_second = -half;
   const u32 k_at = k_token * kFp4RowBytes + 16 * half, ks_at = fp4_key_scale_at(k_token, half);
-  // Row bytes n and 32 + n of V, 16 tokens of tile `half` each: the low nibbles are one operand's row, the high ones another's.
-  // Their scales: lane i of a row of 16 holds tokens 4 (i % 4) .. +3 of block 2 (i / 4 % 2) + n / 16.
+  // Row bytes n and 32 + n of V, 16 tokens of tile `half` each: the low nibbles are one operand's row, the high ones
+  // another's. Their scales: lane i of a row of 16 holds tokens 4 (i % 4) .. +3 of block 2 (i / 4 % 2) + n / 16.
   const u32 vs_at = 16 * (2 * ((n >> 2) & 1) + (n >> 4)) + 4 * (n & 3);
   u32x4 kc[2], vc[2];
   u32 ks[2], vs;
@@ -580,8 +579,8 @@ prefill_strip_fp4_kernel(PrefillFp4Args a) {
     } while (t0 < end);
   }
 
-  // The waves' results meet, 16 rows at a time.  Register i of acc[2 j + x] is dim 64 j + 32 (i / 8) + 16 x + 8 (i / 4 % 2) +
-  // 4 half + i % 4 of row n.
+  // The waves' results meet, 16 rows at a time.  Register i of acc[2 j + x] is dim 64 j + 32 (i / 8) + 16 x + 8 (i / 4
+  // % 2) + 4 half + i % 4 of row n.
   l_run = sum_xor32(l_run);
   if (half == 0) {
     s_m[w][n] = -neg_ref;
@@ -826,8 +825,8 @@ prefill_few_fp4_kernel(PrefillFp4Args a) {
 }
 
 // ------------------------------------------------------------------------------------------ pieces
-// Joins the pieces of the rows whose keys were cut: 8 rows of a group a workgroup, a half-wave each, its lane dims 4 dl ..
-// 4 dl + 3.  The records of kRun pieces load together.
+// Joins the pieces of the rows whose keys were cut: 8 rows of a group a workgroup, a half-wave each, its lane dims 4 dl
+// .. 4 dl + 3.  The records of kRun pieces load together.
 constexpr int kRun = 8;
 
 __global__ void __launch_bounds__(256)
@@ -870,8 +869,8 @@ prefill_join_fp4_kernel(PrefillFp4Args a, int per_group) {
   write_quad(a, rows, g, r, dl, num, den);
 }
 
-// Which kernel, by the workgroups that the bounds of a call allow (few sequences are as long as the longest).  us, few rows /
-// strips / tiles, 16 query and 8 kv heads unless given:
+// Which kernel, by the workgroups that the bounds of a call allow (few sequences are as long as the longest).  us, few
+// rows / strips / tiles, 16 query and 8 kv heads unless given:
 //   1 x 20 rows on 4,096 cached   20 /  32 / 132        1 x 1,000 on 4,096    87 /  60 / 163
 //   1 x 100 on 4,096              21 /  32 / 135        1 x 4,000 on none    171 /  96 / 151
 //   the same, 40 and 8 heads      21 /  34 / 134        4 x 2,000 on 1,152     - / 194 / 194 (1,000 workgroups of tiles)
@@ -882,10 +881,10 @@ prefill_join_fp4_kernel(PrefillFp4Args a, int per_group) {
 constexpr int64_t kFewGroups = 256;
 constexpr int64_t kStripGroups = 1024;  // of the tile kernel
 
-// Where few rows or strips leave the card idle and contexts may be long, the keys are cut until the workgroups fill it once, at
-// most kMaxSplits times, and a second kernel joins the pieces (some 3 us).  us, uncut / cut: 1 x 20 rows on 4,096 keys 20 /
-// 12.4, 2 x 20 on 8,192 35 / 17.6, 1 x 300 on 8,192 61 / 44, 1 x 600 on 8,192 93 / 79.  Few rows take a CU each, strips a
-// third of one (with half: 45 and 93).
+// Where few rows or strips leave the card idle and contexts may be long, the keys are cut until the workgroups fill it
+// once, at most kMaxSplits times, and a second kernel joins the pieces (some 3 us).  us, uncut / cut: 1 x 20 rows on
+// 4,096 keys 20 / 12.4, 2 x 20 on 8,192 35 / 17.6, 1 x 300 on 8,192 61 / 44, 1 x 600 on 8,192 93 / 79.  Few rows take a
+// CU each, strips a third of one (with half: 45 and 93).
 constexpr int kSplitFrom = 4096;  // keys that the block tables hold
 constexpr int kMaxSplits = 32;
 
@@ -984,13 +983,10 @@ extern "C" int nvamd_paged_prefill_fp4(void *out, int64_t out_stride, const void
     a.partials = static_cast<float *>(workspace);
   }
   const dim3 grid(num_kv_heads * a.splits, a.max_tiles, n_seqs);
-  const bool strip = plan.rows == kStripRows;
   if (plan.rows == kFewRows)
     hipLaunchKernelGGL(prefill_few_fp4_kernel, grid, dim3(kFewWaves * 64), 0, stream, a);
-  else if (strip && bs_log2 >= 5)
-    hipLaunchKernelGGL((prefill_strip_fp4_kernel<true>), grid, dim3(kStripWaves * 64), 0, stream, a);
-  else if (strip)
-    hipLaunchKernelGGL((prefill_strip_fp4_kernel<false>), grid, dim3(kStripWaves * 64), 0, stream, a);
+  else if (plan.rows == kStripRows)
+    hipLaunchKernelGGL(prefill_strip_fp4_kernel, grid, dim3(kStripWaves * 64), 0, stream, a);
   else if (bs_log2 >= 5)
     hipLaunchKernelGGL(prefill_fp4_kernel<true>, grid, dim3(kWaves * 64), 0, stream, a);
   else
