@@ -936,7 +936,7 @@ extern "C" int nvamd_paged_prefill_fp4(void *out, int64_t out_stride, const void
                                        const int32_t *cu_seqlens_q, const int32_t *kv_lens, int n_seqs, int num_tokens,
                                        int max_q_len, int num_heads, int num_kv_heads, int head_dim, float scale,
                                        void *workspace, size_t workspace_bytes, hipStream_t stream) {
-  if (n_seqs == 0 || max_q_len == 0) return NVAMD_OK;
+  if (n_seqs == 0 || max_q_len == 0 || num_tokens == 0) return NVAMD_OK;
   const int bs_log2 = log2_exact(block_size);
   if (head_dim != kHeadDim || bs_log2 < 4) return NVAMD_EUNSUPPORTED;
   if (!(scale > 0.f)) return NVAMD_EINVAL;  // the softmax keeps its running max on raw scores

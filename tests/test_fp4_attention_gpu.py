@@ -5,6 +5,7 @@ bf16 weights and results makes."""
 from __future__ import annotations
 
 import math
+import random
 
 import pytest
 import torch
@@ -568,6 +569,40 @@ def test_prefill_replays_from_a_graph(device):
         got = out.clone()
         torch.cuda.synchronize()
         assert torch.equal(got, call(torch.empty_like(q)))
+
+
+# -------------------------------------------------------------------------------------------- drawn calls
+HEADS = [(1, 1), (16, 8), (14, 2), (12, 4), (40, 8), (32, 4), (7, 7), (33, 1)]
+
+
+def some_length(rng, most):
+    return rng.choice([0, 1, 16, rng.randint(1, 40), int(2 ** rng.uniform(0, math.log2(most)))])
+
+
+@pytest.mark.parametrize("seed", range(10))
+def test_decode_of_a_drawn_batch(device, seed):
+    rng = random.Random(seed)
+    hq, hkv = rng.choice(HEADS)
+    batch = Batch(device, [some_length(rng, 6000) for _ in range(rng.randint(1, 20))], hq, hkv,
+                  rng.choice([16, 32, 64, 128, 256]), seed=seed, extra_width=rng.choice([0, 5]))
+    q = batch.queries(len(batch.lens))
+    check_decode(batch, q, batch.decode(q, bound=rng.choice([None, 8192, 131072])))
+    assert _C.index_errors() == 0
+
+
+@pytest.mark.parametrize("seed", range(12))
+def test_prefill_of_a_drawn_batch(device, seed):
+    rng = random.Random(100 + seed)
+    hq, hkv = rng.choice(HEADS)
+    most = 2000 // hq + 20
+    q_lens = [some_length(rng, most) for _ in range(rng.randint(1, 6))]
+    lens = [n + some_length(rng, 3000) for n in q_lens]
+    bs = rng.choice([16, 32, 64, 128, 256])
+    batch = Batch(device, lens, hq, hkv, bs, seed=seed, extra_width=rng.choice([0, 8192 // bs]))
+    q = batch.queries(sum(q_lens))
+    bound = max(max(q_lens), 1)
+    check_prefill(batch, q, q_lens, batch.prefill(q, q_lens, max_q=rng.choice([bound, bound, 4 * bound, bound + 1000, 20_000])))
+    assert _C.index_errors() == 0
 
 
 # -------------------------------------------------------------------------------------------- as they are used together

@@ -157,7 +157,7 @@ def test_prefill_argument_errors():
         args.update(over)
         return lib.nvamd_paged_prefill_fp4(*args.values())
 
-    assert call(n=0) == 0 and call(max_q=0) == 0
+    assert call(n=0) == 0 and call(max_q=0) == 0 and call(tokens=0) == 0
     for name in ("out", "q", "kc", "ks", "vc", "vs"):
         assert call(**{name: 0}) == EINVAL and call(**{name: A + 8}) == EINVAL, name
     assert call(bt=0) == EINVAL and call(cu=0) == EINVAL and call(kv=0) == EINVAL
