@@ -143,8 +143,25 @@ def load() -> ctypes.CDLL:
         fn = getattr(lib, name)
         fn.restype = restype
         fn.argtypes = argtypes
+    _bind_calls(lib)
     _lib = lib
     return lib
+
+
+_calls = None  # csrc/calls.cpp: eager calls of the 4-bit cache, checked and made in one step
+
+
+def _bind_calls(lib: ctypes.CDLL) -> None:
+    global _calls
+    try:
+        from . import _calls as calls
+    except ImportError as e:
+        raise RuntimeError("nano_vllm_ascend_amd/_calls.so is missing: build it with "
+                           "`python -m nano_vllm_ascend_amd.build` (or __graft_entry__.build())") from e
+    names = ("kv_cache_write_fp4", "kv_cache_read_fp4", "qk_norm_rope_fp4", "paged_decode_fp4", "paged_prefill_fp4",
+             "paged_prefill_fp4_workspace_size")
+    calls.bind(Fp4Pages, *(ctypes.cast(getattr(lib, f"nvamd_{n}"), ctypes.c_void_p).value for n in names))
+    _calls = calls
 
 
 def _check(status: int, name: str) -> None:
@@ -578,6 +595,10 @@ def paged_prefill(out: torch.Tensor, q: torch.Tensor, key_cache: torch.Tensor, v
 FP4_ROW_BYTES, FP4_ROW_SCALES = 64, 4  # of a head vector
 
 
+# The functions below hand a call to csrc/calls.cpp first, which makes it if every argument is plainly right.  Else, and
+# with range checks on, the checks here name what is wrong, or make the call.
+
+
 class Fp4Pages(NamedTuple):
     """The keys or the values of one layer in 4 bits: ``codes`` uint8 [blocks, kv heads, block_size, 64] and ``scales``
     uint8 [blocks, kv heads, block_size, 4], contiguous.  Pages are opaque (``kv_cache_read_fp4`` gives their values)."""
@@ -593,8 +614,7 @@ class Fp4Pages(NamedTuple):
 
 
 def _fp4_pages(key_pages: Fp4Pages, value_pages: Fp4Pages):
-    """Checks the pages of a layer; returns blocks, block_size, kv heads, their addresses and their device.  (The checks of
-    this section are written out: a small batch's eager call is bound by the host.)"""
+    """Checks the pages of a layer; returns blocks, block_size, kv heads, their addresses and their device."""
     if type(key_pages) is not Fp4Pages or type(value_pages) is not Fp4Pages:
         raise ValueError("key and value pages must be Fp4Pages")
     kc, ks = key_pages
@@ -650,11 +670,23 @@ def _page_slots(slot_mapping: torch.Tensor, rows: int, num_slots: int) -> int:
     return slot_mapping.data_ptr()
 
 
+def _made(answer, name: str) -> bool:
+    """Whether calls.cpp has made the call; raises for what the library answered."""
+    if answer is None:
+        return False
+    if type(answer) is int:
+        _check(answer, name)
+    return True
+
+
 def kv_cache_write_fp4(key_states: torch.Tensor, value_states: torch.Tensor, key_pages: Fp4Pages,
                        value_pages: Fp4Pages, slot_mapping: torch.Tensor) -> None:
     """Rows [T, Hkv, 128] of bf16 keys and values, quantised into the pages at their slots (-1: padding, skipped; no slot
     twice in a call)."""
     lib = _lib or load()
+    if not _range_checks and _made(_calls.write(key_states, value_states, key_pages, value_pages, slot_mapping),
+                                   "nvamd_kv_cache_write_fp4"):
+        return
     nb, bs, hkv, pages, device = _fp4_pages(key_pages, value_pages)
     t, d = key_states.shape[0], 2 * FP4_ROW_BYTES
     k_stride, v_stride = _heads("key_states", key_states, t, hkv, d), _heads("value_states", value_states, t, hkv, d)
@@ -671,6 +703,10 @@ def kv_cache_read_fp4(key_pages: Fp4Pages, value_pages: Fp4Pages, slot_mapping: 
                       v_out: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """The bf16 keys and values [T, Hkv, 128] that the pages hold at the slots (zeros for -1)."""
     lib = _lib or load()
+    if not _range_checks and k_out is None and v_out is None:
+        rows = _calls.read(key_pages, value_pages, slot_mapping)
+        if _made(rows, "nvamd_kv_cache_read_fp4"):
+            return rows
     nb, bs, hkv, pages, device = _fp4_pages(key_pages, value_pages)
     t, d = slot_mapping.shape[0], 2 * FP4_ROW_BYTES
     slots = _page_slots(slot_mapping, t, nb * bs)
@@ -699,6 +735,11 @@ def qk_norm_rope_fp4(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_weight
     Returns the rotated q: ``q_out``, which may be q itself, or a new tensor.  The rotated k is written
     only to the pages unless ``k_out`` (which may be k itself) asks for it.  64-bit arithmetic, one rounding to bf16."""
     lib = _lib or load()
+    if not _range_checks:
+        rotated = _calls.rope(q, k, v, q_weight, k_weight, positions, cos_sin, eps, key_pages, value_pages, slot_mapping,
+                              q_out, k_out)
+        if _made(rotated, "nvamd_qk_norm_rope_fp4"):
+            return rotated
     nb, bs, hkv, pages, device = _fp4_pages(key_pages, value_pages)
     d = 2 * FP4_ROW_BYTES
     if q.dim() != 3:
@@ -764,11 +805,18 @@ def _fp4_attention_args(out, q, key_pages, value_pages, block_tables, seqs: int)
             max(bt_stride[0], width), width), (hq, hkv, d), device
 
 
-def paged_decode_fp4(out: torch.Tensor, q: torch.Tensor, key_pages: Fp4Pages, value_pages: Fp4Pages,
+def paged_decode_fp4(out: torch.Tensor | None, q: torch.Tensor, key_pages: Fp4Pages, value_pages: Fp4Pages,
                      block_tables: torch.Tensor, context_lens: torch.Tensor, scale: float, max_context_len: int,
                      workspace: torch.Tensor) -> torch.Tensor:
-    """``paged_decode`` over pages of 4 bits; the workspace is the same (``alloc_paged_decode_workspace``)."""
+    """``paged_decode`` over pages of 4 bits; the workspace is the same (``alloc_paged_decode_workspace``).  Without
+    ``out`` the result is a new tensor."""
     lib = _lib or load()
+    if not _range_checks:
+        made = _calls.decode(out, q, key_pages, value_pages, block_tables, context_lens, scale, max_context_len, workspace)
+        if _made(made, "nvamd_paged_decode_fp4"):
+            return made
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     b = q.shape[0]
     args, heads, device = _fp4_attention_args(out, q, key_pages, value_pages, block_tables, b)
     if block_tables.shape[0] != b:
@@ -791,7 +839,11 @@ def paged_prefill_fp4(out: torch.Tensor, q: torch.Tensor, key_pages: Fp4Pages, v
                       block_tables: torch.Tensor, cu_seqlens_q: torch.Tensor, kv_lens: torch.Tensor, max_q_len: int,
                       scale: float) -> torch.Tensor:
     """``paged_prefill`` over pages of 4 bits: queries are the last q_len of kv_len positions, all keys in the cache."""
-    lib = load()
+    lib = _lib or load()
+    if not _range_checks and _made(
+            _calls.prefill(out, q, key_pages, value_pages, block_tables, cu_seqlens_q, kv_lens, max_q_len, scale),
+            "nvamd_paged_prefill_fp4"):
+        return out
     if cu_seqlens_q.dtype is not torch.int32 or cu_seqlens_q.dim() != 1 or not cu_seqlens_q.is_contiguous():
         raise ValueError("cu_seqlens_q must be contiguous int32 [n + 1]")
     n = cu_seqlens_q.numel() - 1

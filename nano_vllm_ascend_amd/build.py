@@ -4,6 +4,8 @@
 hipcc for gfx950 and links them into ``nano_vllm_ascend_amd/libnvamd.so``.
 The library exports the C ABI declared in ``include/nvamd.h`` and nothing that
 depends on torch, so the same file serves ctypes, a C harness or any FFI.
+``csrc/calls.cpp``, host code that makes some of its calls for Python, becomes the
+extension module ``nano_vllm_ascend_amd/_calls.so``.
 """
 from __future__ import annotations
 
@@ -12,6 +14,7 @@ import re
 import shutil
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
@@ -20,6 +23,7 @@ REPO_DIR = PKG_DIR.parent
 CSRC_DIR = PKG_DIR / "csrc"
 INCLUDE_DIR = REPO_DIR / "include"
 LIB_PATH = PKG_DIR / "libnvamd.so"
+CALLS_PATH = PKG_DIR / "_calls.so"
 OBJ_DIR = PKG_DIR / "_build"
 
 ARCH = "gfx950"
@@ -77,6 +81,22 @@ def _compile(src: Path) -> Path:
     return obj
 
 
+def _build_calls() -> None:
+    import torch
+
+    root = Path(torch.__file__).resolve().parent
+    tmp = CALLS_PATH.with_suffix(".so.tmp")
+    cmd = [HIPCC, "-x", "c++", str(CSRC_DIR / "calls.cpp"), "-O2", "-std=c++17", "-shared", "-fPIC", "-Wall",
+           "-D__HIP_PLATFORM_AMD__", "-DUSE_ROCM", f"-I{INCLUDE_DIR}", f"-isystem{root / 'include'}",
+           f"-isystem{Path(shutil.which(HIPCC) or HIPCC).resolve().parents[1] / 'include'}",
+           f"-isystem{root / 'include/torch/csrc/api/include'}", f"-I{sysconfig.get_path('include')}",
+           f"-L{root / 'lib'}", "-ltorch_python", "-ltorch_cpu", "-ltorch_hip", "-lc10", "-lc10_hip", "-o", str(tmp)]
+    proc = subprocess.run(cmd, capture_output=True, text=True)
+    if proc.returncode != 0:
+        raise RuntimeError(f"calls.cpp failed:\n{proc.stdout}\n{proc.stderr}")
+    os.replace(tmp, CALLS_PATH)
+
+
 def build(verbose: bool = True) -> Path:
     """Compile all sources and link the shared library; returns its path."""
     if not Path(HIPCC).exists() and shutil.which(HIPCC) is None:
@@ -87,7 +107,9 @@ def build(verbose: bool = True) -> Path:
         raise RuntimeError(f"no HIP sources in {CSRC_DIR}")
     workers = max(1, min(len(srcs), int(os.environ.get("MAX_JOBS", "8"))))
     with ThreadPoolExecutor(max_workers=workers) as pool:
+        calls = pool.submit(_build_calls)
         objs = list(pool.map(_compile, srcs))
+        calls.result()
     tmp = LIB_PATH.with_suffix(".so.tmp")
     cmd = [HIPCC, f"--offload-arch={ARCH}", "-shared", "-fPIC", *map(str, objs), "-o", str(tmp)]
     proc = subprocess.run(cmd, capture_output=True, text=True)

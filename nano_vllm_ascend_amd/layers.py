@@ -113,12 +113,12 @@ class HipPagedAttention(nn.Module):
             context_lens = context_lens.to(q.device, non_blocking=True)
         if workspace is None:
             workspace = self.workspace(total_tokens, max_context_len, q.device)
-        out = torch.empty_like(q) if out is None else out
         if context_lens.dtype is not torch.int32:
             context_lens = context_lens.to(torch.int32)
         if isinstance(key_cache, _C.Fp4Pages):
             return _C.paged_decode_fp4(out, q, key_cache, value_cache, block_tables, context_lens, self.scale,
                                        max_context_len, workspace)
+        out = torch.empty_like(q) if out is None else out
         return _C.paged_decode(out, q, key_cache, value_cache, block_tables, context_lens, self.scale,
                                max_context_len, workspace)
 

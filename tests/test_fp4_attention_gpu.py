@@ -571,6 +571,61 @@ def test_prefill_replays_from_a_graph(device):
         assert torch.equal(got, call(torch.empty_like(q)))
 
 
+# -------------------------------------------------------------------------------------------- the two routes of a call
+def test_a_call_made_at_once_equals_one_that_python_checks(device):
+    """Range checks send the calls through the checks of _C.py; without them csrc/calls.cpp makes those that are plain."""
+    batch = Batch(device, [300, 5000, 20], 4, 2, 16, seed=21, extra_width=300)
+    gen = torch.Generator().manual_seed(22)
+    qkv = torch.randn(9, 8, 128, generator=gen).bfloat16().to(device)
+    q, k, v = qkv.split([4, 2, 2], 1)
+    weights = [torch.rand(128, generator=gen).bfloat16().to(device) for _ in range(2)]
+    table = torch.randn(64, 128, generator=gen).to(device)
+    pos = torch.arange(9, device=device)
+    slots = batch.slots[0][:9].to(device)
+    slots[3] = -1
+    lens = torch.tensor(batch.lens, dtype=torch.int32, device=device)
+    tables = batch.tables.to(device)
+    cu = torch.tensor([0, 4, 8, 9], dtype=torch.int32, device=device)
+    space = _C.alloc_paged_decode_workspace(3, 4, 2, 5000, device)
+
+    def results():
+        batch.upload()
+        pages = batch.keys, batch.values
+        got = [_C.paged_decode_fp4(None, q[:3], *pages, tables, lens, SCALE, 5000, space),
+               _C.paged_decode_fp4(torch.empty(3, 4, 128, dtype=torch.bfloat16, device=device), q[:3], *pages, tables, lens,
+                                   SCALE, 5000, space),
+               _C.paged_prefill_fp4(torch.empty(9, 4, 128, dtype=torch.bfloat16, device=device), q, *pages, tables, cu, lens,
+                                    4, SCALE)]
+        _C.kv_cache_write_fp4(k, v, *pages, slots)
+        got += [*pages[0], *pages[1], *_C.kv_cache_read_fp4(*pages, slots)]
+        k_out = torch.zeros(9, 2, 128, dtype=torch.bfloat16, device=device)
+        got.append(_C.qk_norm_rope_fp4(q, k, v, *weights, pos, table, 1e-6, *pages, slots, k_out=k_out))
+        got.append(_C.qk_norm_rope_fp4(q, k, v, *weights, pos, table, 1e-6, *pages, slots, q_out=torch.empty_like(got[-1])))
+        return [t.clone() for t in (*got, k_out, *pages[0], *pages[1])]
+
+    at_once = results()
+    before = _C.set_range_checks(True)
+    try:
+        checked = results()
+    finally:
+        _C.set_range_checks(before)
+    assert len(at_once) == len(checked) and all(torch.equal(a, b) for a, b in zip(at_once, checked))
+
+
+def test_what_the_library_refuses_raises(device):
+    batch = Batch(device, [30], 2, 1, 16, seed=23)
+    q = batch.queries(1).to(device)
+    with pytest.raises(ValueError, match="workspace"):
+        batch.decode(q, workspace=torch.zeros(64, dtype=torch.uint8, device=device))
+    with pytest.raises(ValueError, match="invalid argument"):
+        batch.prefill(q, [1], scale=-1.0)
+    with pytest.raises(ValueError, match="invalid argument"):
+        _C.kv_cache_write_fp4(q[:, :1].expand(4, 1, 128), q[:, :1].expand(4, 1, 128), batch.keys, batch.values,
+                              torch.arange(4, device=device))
+    with pytest.raises(ValueError, match="on one device|GPU"):
+        _C.kv_cache_write_fp4(q[:, :1].cpu(), q[:, :1].cpu(), batch.keys, batch.values, torch.arange(1, device=device))
+
+
 # -------------------------------------------------------------------------------------------- drawn calls
 HEADS = [(1, 1), (16, 8), (14, 2), (12, 4), (40, 8), (32, 4), (7, 7), (33, 1)]
 
