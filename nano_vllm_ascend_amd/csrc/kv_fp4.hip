@@ -8,8 +8,8 @@
 // and RoPE needs no lane exchange.
 //
 // All three are bound by memory: per head vector 256 bytes of bf16 and 68 of the cache, once.  36,488 tokens, 8 kv
-// heads (and 16 query heads): write 189 MB in 40 us (4.7 TB/s), read 189 MB in 38 us (5.0 TB/s), norm + RoPE + write
-// with the keys returned 564 MB in 118 us (4.8 TB/s); a large copy reaches 5.0 TB/s.  One token: 3 us, the launch.
+// heads (and 16 query heads): write 189 MB in 37 us (5.2 TB/s), read 189 MB in 38 us (5.0 TB/s), norm + RoPE + write
+// with the keys returned 564 MB in 117 us (4.8 TB/s); a large copy reaches 5.0 TB/s.  One token: 3 us, the launch.
 #include "fp4.h"
 
 namespace nvamd {
@@ -199,9 +199,9 @@ kv_read_fp4_kernel(ReadArgs a) {
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int c = lane & 7, tok = lane >> 3;
   const int hkv = a.num_kv_heads;
-  const int v = blockIdx.y * 4 + w;  // key heads, then value heads
-  if (v >= 2 * hkv) return;
-  const int t = blockIdx.x * 8 + tok;
+  const int v = blockIdx.y * 2 + (w >> 1);  // key heads, then value heads
+  if (v >= 2 * hkv || blockIdx.x * 16 + (w & 1) * 8 >= a.num_tokens) return;
+  const int t = blockIdx.x * 16 + (w & 1) * 8 + tok;
   const bool exists = t < a.num_tokens;
   int64_t slot = exists ? a.slots[t] : -1;
   if (slot >= a.num_slots || slot < -1) {
@@ -346,10 +346,10 @@ rows_fp4_kernel(NormRopeFp4Args a) {
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int c = lane & 7, tok = lane >> 3;
   const int hkv = a.w.num_kv_heads, hq = ROPE ? a.num_heads : 0;
-  const int h_begin = (blockIdx.y * 4 + w) * a.w.heads_per_wave;
+  const int h_begin = (blockIdx.y * 2 + (w >> 1)) * a.w.heads_per_wave;
   const int h_end = min(h_begin + a.w.heads_per_wave, hq + 2 * hkv);
-  if (h_begin >= h_end) return;
-  const int t = blockIdx.x * 8 + tok;
+  if (h_begin >= h_end || blockIdx.x * 16 + (w & 1) * 8 >= a.w.num_tokens) return;
+  const int t = blockIdx.x * 16 + (w & 1) * 8 + tok;
   const bool exists = t < a.w.num_tokens;
   int64_t slot = exists ? a.w.slots[t] : -1;
   if (slot >= a.w.num_slots || slot < -1) {  // skip the row, report it once per token
@@ -426,12 +426,13 @@ rows_fp4_kernel(NormRopeFp4Args a) {
   }
 }
 
-// A workgroup is 8 tokens x 4 waves' heads.  A wave takes up to `per_wave` heads; fewer where that leaves too few waves
-// to fill the card.  0: more than a launch takes.
+// A workgroup is 2 x 8 tokens x 2 waves' heads: the two halves of a tile's value bytes share lines, and meet in one L2
+// (8 tokens x 4 waves': 12,345 rows read in 17.8 us, so 15.0; 36,488 written in 39.9, so 36.6).  A wave takes up to
+// `per_wave` heads; fewer where that leaves too few waves to fill the card.  0: more than a launch takes.
 int heads_per_wave(int num_tokens, int vecs, int per_wave, dim3 *grid) {
   const int64_t octets = ((int64_t)num_tokens + 7) / 8;
   while (per_wave > 1 && octets * ceil_div(vecs, per_wave) < kWantedWaves) per_wave >>= 1;
-  *grid = dim3((unsigned)octets, (unsigned)ceil_div(ceil_div(vecs, per_wave), 4));
+  *grid = dim3((unsigned)((octets + 1) / 2), (unsigned)ceil_div(ceil_div(vecs, per_wave), 2));
   return octets < (1 << 24) && grid->y <= 65535 ? per_wave : 0;
 }
 
