@@ -11,6 +11,8 @@ attention_ref      fp32 torch-CPU paged decode, dense and paged causal varlen
                    prefill, KV store, per-head RMSNorm + rotate-half RoPE.
 block_manager_ref  plain-Python restatement of the reference BlockManager,
                    including the per-token slot loop the GPU packing replaces.
+fp4_ref            the KV cache in 4 bits: quantised rows, page layout, norm and
+                   rotation, attention in 64 bits with a bound of the error.
 qwen3_ref          torch restatement of the reference Qwen3 forward (fp32, or
                    bf16 at the reference's rounding points) for greedy-token
                    and logits parity of the whole model.
