@@ -8,8 +8,8 @@
 // and RoPE needs no lane exchange.
 //
 // All three are bound by memory: per head vector 256 bytes of bf16 and 68 of the cache, once.  36,488 tokens, 8 kv
-// heads (and 16 query heads): write 189 MB in 37 us (5.2 TB/s), read 189 MB in 38 us (5.0 TB/s), norm + RoPE + write
-// with the keys returned 564 MB in 117 us (4.8 TB/s); a large copy reaches 5.0 TB/s.  One token: 3 us, the launch.
+// heads (and 16 query heads): write 189 MB in 37 us (5.2 TB/s), read 189 MB in 34 us (5.6 TB/s), norm + RoPE + write
+// with the keys returned 564 MB in 115 us (4.9 TB/s); a large copy reaches 5.0 TB/s.  One token: 3 us, the launch.
 #include "fp4.h"
 
 namespace nvamd {
@@ -190,7 +190,8 @@ struct ReadArgs {
 };
 
 // The other way round.  A wave takes one key or value head of 8 tokens: it waits for its loads once, and more waves are
-// all that hides that (36,488 x 8 heads: 50 us with 8 heads one after another, 45 with 2, 37.4 so).  A row without a
+// all that hides that (36,488 x 8 heads: 50 us with 8 heads one after another, 45 with 2, 37.4 so; 34 since the scale
+// loads with the bytes).  A row without a
 // slot, or with one outside the cache, is zeros.
 template <bool STREAM>
 __global__ void __launch_bounds__(256)
@@ -233,6 +234,7 @@ kv_read_fp4_kernel(ReadArgs a) {
     return a.cache.v_codes + x.tile * kFp4TileBytes + lane * kFp4Tile + x.t;
   };
   u8 *tile = s_tile[w];
+  const u32 scale_byte = live ? a.cache.v_scales[r.tile * kFp4TileScales + fp4_value_scale_at(r.t, c >> 1)] : 0u;
   uint64_t bytes = 0;
   if (__all(live && slot == uniform64(slot) + tok)) {
     const int64_t s0 = uniform64(slot);
@@ -251,7 +253,7 @@ kv_read_fp4_kernel(ReadArgs a) {
   u32x4 first = zero, last = zero;
   if (live) {
     const u8 *p = tile + (16 * (c >> 1) + 8 * (c & 1)) * 8 + tok;
-    const float scale = fp4_scale(a.cache.v_scales[r.tile * kFp4TileScales + fp4_value_scale_at(r.t, c >> 1)]);
+    const float scale = fp4_scale(scale_byte);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const u32 x = fp4_pair<0>(p[2 * j * 8], scale), y = fp4_pair<0>(p[(2 * j + 1) * 8], scale);
