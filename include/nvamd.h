@@ -454,6 +454,28 @@ int nvamd_paged_decode_fp4(void *out, int64_t out_stride,
                            void *workspace, size_t workspace_bytes,
                            hipStream_t stream);
 
+/* paged_decode_fused_fp4: nvamd_qk_norm_rope_fp4 (q, k and v as they are     */
+/* projected, left as they are) and nvamd_paged_decode_fp4 in one launch, with */
+/* the same bits.  slot_mapping[b] is the slot of sequence b's last position, */
+/* or -1: then nothing is stored.  out may be q.                              */
+int nvamd_paged_decode_fused_fp4(void *out, int64_t out_stride,
+                                 const void *q, int64_t q_stride,
+                                 const void *k, int64_t k_stride,
+                                 const void *v, int64_t v_stride,
+                                 const void *q_weight, const void *k_weight,
+                                 const int64_t *positions,
+                                 const float *cos_sin, int max_positions,
+                                 float eps, void *k_codes, void *k_scales,
+                                 void *v_codes, void *v_scales,
+                                 int num_blocks, int block_size,
+                                 const int64_t *slot_mapping,
+                                 const int32_t *block_tables, int bt_stride,
+                                 int bt_width, const int32_t *context_lens,
+                                 int batch, int num_heads, int num_kv_heads,
+                                 int head_dim, float scale,
+                                 int max_context_len, void *workspace,
+                                 size_t workspace_bytes, hipStream_t stream);
+
 /* paged_prefill_fp4: nvamd_paged_prefill over the 4-bit cache.  workspace,   */
 /* of nvamd_paged_prefill_fp4_workspace_size(...) bytes (0: none needed), any */
 /* contents, of this call's own while it runs, lets few rows on long contexts */

@@ -107,6 +107,12 @@ _SIGNATURES = {
         [_c_ptr, _c_i64, _c_ptr, _c_i64, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_int, _c_ptr, _c_int, _c_int,
          _c_ptr, _c_int, _c_int, _c_int, _c_int, _c_float, _c_int, _c_ptr, _c_size, _c_ptr],
     ),
+    "nvamd_paged_decode_fused_fp4": (
+        _c_int,
+        [_c_ptr, _c_i64, _c_ptr, _c_i64, _c_ptr, _c_i64, _c_ptr, _c_i64, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int,
+         _c_float, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_int, _c_ptr, _c_ptr, _c_int, _c_int, _c_ptr, _c_int,
+         _c_int, _c_int, _c_int, _c_float, _c_int, _c_ptr, _c_size, _c_ptr],
+    ),
     "nvamd_paged_prefill_fp4": (
         _c_int,
         [_c_ptr, _c_i64, _c_ptr, _c_i64, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_int, _c_ptr, _c_int, _c_int,
@@ -158,8 +164,8 @@ def _bind_calls(lib: ctypes.CDLL) -> None:
     except ImportError as e:
         raise RuntimeError("nano_vllm_ascend_amd/_calls.so is missing: build it with "
                            "`python -m nano_vllm_ascend_amd.build` (or __graft_entry__.build())") from e
-    names = ("kv_cache_write_fp4", "kv_cache_read_fp4", "qk_norm_rope_fp4", "paged_decode_fp4", "paged_prefill_fp4",
-             "paged_prefill_fp4_workspace_size")
+    names = ("kv_cache_write_fp4", "kv_cache_read_fp4", "qk_norm_rope_fp4", "paged_decode_fp4",
+             "paged_decode_fused_fp4", "paged_prefill_fp4", "paged_prefill_fp4_workspace_size")
     calls.bind(Fp4Pages, *(ctypes.cast(getattr(lib, f"nvamd_{n}"), ctypes.c_void_p).value for n in names))
     _calls = calls
 
@@ -726,6 +732,17 @@ def kv_cache_read_fp4(key_pages: Fp4Pages, value_pages: Fp4Pages, slot_mapping: 
     return k_out, v_out
 
 
+def _rope_args(q_weight, k_weight, positions, cos_sin, t: int, d: int) -> None:
+    for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
+        if w.dtype is not torch.bfloat16 or w.shape != (d,) or not w.is_contiguous():
+            raise ValueError(f"{name} must be contiguous bf16 [{d}]")
+    if positions.dtype is not torch.int64 or positions.shape != (t,) or not positions.is_contiguous():
+        raise ValueError(f"positions must be contiguous int64 [{t}]")
+    table = cos_sin.shape
+    if cos_sin.dtype is not torch.float32 or len(table) != 2 or table[1] != d or not cos_sin.is_contiguous():
+        raise ValueError("cos_sin must be contiguous fp32 [max_positions, head_dim]")
+
+
 def qk_norm_rope_fp4(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_weight: torch.Tensor,
                      k_weight: torch.Tensor, positions: torch.Tensor, cos_sin: torch.Tensor, eps: float,
                      key_pages: Fp4Pages, value_pages: Fp4Pages, slot_mapping: torch.Tensor, *,
@@ -755,21 +772,14 @@ def qk_norm_rope_fp4(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_weight
         ko_stride, ko_ptr = _heads("k_out", k_out, t, hkv, d), k_out.data_ptr()
     if (qo_ptr == q_ptr and qo_stride != q_stride) or (ko_ptr == k_ptr and ko_stride != k_stride):
         raise ValueError("an output in place of its input must have the input's row stride")
-    for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
-        if w.dtype is not torch.bfloat16 or w.shape != (d,) or not w.is_contiguous():
-            raise ValueError(f"{name} must be contiguous bf16 [{d}]")
-    if positions.dtype is not torch.int64 or positions.shape != (t,) or not positions.is_contiguous():
-        raise ValueError(f"positions must be contiguous int64 [{t}]")
-    table = cos_sin.shape
-    if cos_sin.dtype is not torch.float32 or len(table) != 2 or table[1] != d or not cos_sin.is_contiguous():
-        raise ValueError("cos_sin must be contiguous fp32 [max_positions, head_dim]")
+    _rope_args(q_weight, k_weight, positions, cos_sin, t, d)
     slots = _page_slots(slot_mapping, t, nb * bs)
     if _range_checks and _checking():
-        check_positions(positions, table[0])
+        check_positions(positions, cos_sin.shape[0])
     status = lib.nvamd_qk_norm_rope_fp4(
         qo_ptr, qo_stride, ko_ptr, ko_stride, q_ptr, q_stride, k_ptr, k_stride, v.data_ptr(), v_stride,
-        q_weight.data_ptr(), k_weight.data_ptr(), positions.data_ptr(), cos_sin.data_ptr(), table[0], *pages, nb, bs,
-        slots, t, hq, hkv, d, eps,
+        q_weight.data_ptr(), k_weight.data_ptr(), positions.data_ptr(), cos_sin.data_ptr(), cos_sin.shape[0], *pages, nb,
+        bs, slots, t, hq, hkv, d, eps,
         _stream_of(device, q, k, v, q_out, q if k_out is None else k_out, q_weight, k_weight, positions, cos_sin,
                    slot_mapping))
     if status:
@@ -805,6 +815,15 @@ def _fp4_attention_args(out, q, key_pages, value_pages, block_tables, seqs: int)
             max(bt_stride[0], width), width), (hq, hkv, d), device
 
 
+def _fp4_decode_args(block_tables, context_lens, workspace, b: int) -> None:
+    if block_tables.shape[0] != b:
+        raise ValueError(f"block_tables must be int32 [{b}, W]")
+    if context_lens.dtype is not torch.int32 or context_lens.shape != (b,) or not context_lens.is_contiguous():
+        raise ValueError(f"context_lens must be contiguous int32 [{b}]")
+    if not workspace.is_contiguous():
+        raise ValueError("workspace must be contiguous")
+
+
 def paged_decode_fp4(out: torch.Tensor | None, q: torch.Tensor, key_pages: Fp4Pages, value_pages: Fp4Pages,
                      block_tables: torch.Tensor, context_lens: torch.Tensor, scale: float, max_context_len: int,
                      workspace: torch.Tensor) -> torch.Tensor:
@@ -819,12 +838,7 @@ def paged_decode_fp4(out: torch.Tensor | None, q: torch.Tensor, key_pages: Fp4Pa
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     b = q.shape[0]
     args, heads, device = _fp4_attention_args(out, q, key_pages, value_pages, block_tables, b)
-    if block_tables.shape[0] != b:
-        raise ValueError(f"block_tables must be int32 [{b}, W]")
-    if context_lens.dtype is not torch.int32 or context_lens.shape != (b,) or not context_lens.is_contiguous():
-        raise ValueError(f"context_lens must be contiguous int32 [{b}]")
-    if not workspace.is_contiguous():
-        raise ValueError("workspace must be contiguous")
+    _fp4_decode_args(block_tables, context_lens, workspace, b)
     if _range_checks and _checking():
         check_paged_context(block_tables, context_lens, args[8], args[9], int(max_context_len))
     status = lib.nvamd_paged_decode_fp4(*args, context_lens.data_ptr(), b, *heads, scale, max_context_len,
@@ -832,6 +846,42 @@ def paged_decode_fp4(out: torch.Tensor | None, q: torch.Tensor, key_pages: Fp4Pa
                                         _stream_of(device, q, out, block_tables, context_lens, workspace))
     if status:
         _check(status, "nvamd_paged_decode_fp4")
+    return out
+
+
+def paged_decode_fused_fp4(out: torch.Tensor | None, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+                           q_weight: torch.Tensor, k_weight: torch.Tensor, positions: torch.Tensor,
+                           cos_sin: torch.Tensor, eps: float, key_pages: Fp4Pages, value_pages: Fp4Pages,
+                           slot_mapping: torch.Tensor, block_tables: torch.Tensor, context_lens: torch.Tensor,
+                           scale: float, max_context_len: int, workspace: torch.Tensor) -> torch.Tensor:
+    """``qk_norm_rope_fp4`` and ``paged_decode_fp4`` in one launch, with the same bits: the step's k and v go to the slots
+    of their sequences' last positions (-1: not stored), q, k and v stay as they are."""
+    lib = _lib or load()
+    if not _range_checks:
+        made = _calls.decode_fused(out, q, k, v, q_weight, k_weight, positions, cos_sin, eps, key_pages, value_pages,
+                                   slot_mapping, block_tables, context_lens, scale, max_context_len, workspace)
+        if _made(made, "nvamd_paged_decode_fused_fp4"):
+            return made
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    b = q.shape[0]
+    args, heads, device = _fp4_attention_args(out, q, key_pages, value_pages, block_tables, b)
+    _fp4_decode_args(block_tables, context_lens, workspace, b)
+    nb, bs, (hq, hkv, d) = args[8], args[9], heads
+    k_stride, v_stride = _heads("k", k, b, hkv, d), _heads("v", v, b, hkv, d)
+    _rope_args(q_weight, k_weight, positions, cos_sin, b, d)
+    slots = _page_slots(slot_mapping, b, nb * bs)
+    if _range_checks and _checking():
+        check_positions(positions, cos_sin.shape[0])
+        check_paged_context(block_tables, context_lens, nb, bs, int(max_context_len))
+    status = lib.nvamd_paged_decode_fused_fp4(
+        *args[:4], k.data_ptr(), k_stride, v.data_ptr(), v_stride, q_weight.data_ptr(), k_weight.data_ptr(),
+        positions.data_ptr(), cos_sin.data_ptr(), cos_sin.shape[0], eps, *args[4:10], slots, *args[10:],
+        context_lens.data_ptr(), b, hq, hkv, d, scale, max_context_len, workspace.data_ptr(), workspace.nbytes,
+        _stream_of(device, q, k, v, out, q_weight, k_weight, positions, cos_sin, slot_mapping, block_tables,
+                   context_lens, workspace))
+    if status:
+        _check(status, "nvamd_paged_decode_fused_fp4")
     return out
 
 

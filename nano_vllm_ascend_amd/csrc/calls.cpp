@@ -1,7 +1,7 @@
-// The eager calls of the 4-bit cache from Python: arguments checked and read, outputs made and the C ABI called in one step.
-// A small batch's eager call is bound by the host: a launch costs it some 3.6 us, and checking 5 to 15 tensors attribute by
-// attribute from Python another 4 to 5, with 1 for ctypes (decode of 4 x U[1, 512] through the layer: 12.7 us, so 8.1; a row
-// written and read back 18.5, 9.0).
+// The eager calls of the 4-bit cache from Python: arguments checked and read, outputs made and the C ABI called in one
+// step. A small batch's eager call is bound by the host: a launch costs it some 3.6 us, and checking 5 to 15 tensors
+// attribute by attribute from Python another 4 to 5, with 1 for ctypes (decode of 4 x U[1, 512] through the layer: 12.7
+// us, so 8.1; a row written and read back 18.5, 9.0).
 //
 // Every function answers
 //   its result   the call was made;
@@ -24,6 +24,7 @@ decltype(&nvamd_kv_cache_write_fp4) f_write;
 decltype(&nvamd_kv_cache_read_fp4) f_read;
 decltype(&nvamd_qk_norm_rope_fp4) f_rope;
 decltype(&nvamd_paged_decode_fp4) f_decode;
+decltype(&nvamd_paged_decode_fused_fp4) f_fused;
 decltype(&nvamd_paged_prefill_fp4) f_prefill;
 decltype(&nvamd_paged_prefill_fp4_workspace_size) f_prefill_space;
 PyTypeObject *pages_type;  // _C.Fp4Pages
@@ -129,6 +130,30 @@ at::Tensor empty(at::IntArrayRef sizes, at::ScalarType type, int device) {
   return at::empty(sizes, at::TensorOptions().dtype(type).device(at::kCUDA, (c10::DeviceIndex)device));
 }
 
+// The rows given for a result, or new ones like q's.
+Rows result(PyObject *o, int device, const Rows &q, at::Tensor &made) {
+  if (o != Py_None) return rows_of(o, device, q.rows, q.heads);
+  made = empty({q.rows, q.heads, kHeadDim}, at::kBFloat16, device);
+  return {made.data_ptr(), q.heads * kHeadDim, q.rows, q.heads};
+}
+
+struct Rope {
+  const void *qw, *kw;
+  const int64_t *positions;
+  const float *table;
+  int rows;
+  float eps;
+};
+// q_weight, k_weight, positions, cos_sin, eps
+Rope rope_of(PyObject *const *a, int &device, int64_t rows) {
+  const at::Tensor &qw = dense(a[0], device, at::kBFloat16), &kw = dense(a[1], device, at::kBFloat16);
+  need(qw.dim() == 1 && qw.size(0) == kHeadDim && kw.dim() == 1 && kw.size(0) == kHeadDim);
+  const int64_t *positions = indices(a[2], device, rows);
+  const at::Tensor &table = dense(a[3], device, at::kFloat);
+  need(table.dim() == 2 && table.size(1) == kHeadDim);
+  return {qw.data_ptr(), kw.data_ptr(), positions, table.data_ptr<float>(), narrow(table.size(0)), number(a[4])};
+}
+
 template <typename F>
 int call(F &&f) {  // other threads run meanwhile: a full queue makes a launch wait
   PyThreadState *state = PyEval_SaveThread();
@@ -173,44 +198,34 @@ PyObject *read(PyObject *const *a) {
   return Py_BuildValue("(NN)", THPVariable_Wrap(std::move(k)), THPVariable_Wrap(std::move(v)));
 }
 
-// (q, k, v, q_weight, k_weight, positions, cos_sin, eps, key_pages, value_pages, slot_mapping, q_out, k_out) -> q_out; q_out
-// None: a new one, k_out None: none
+// (q, k, v, q_weight, k_weight, positions, cos_sin, eps, key_pages, value_pages, slot_mapping, q_out, k_out) -> q_out;
+// q_out None: a new one, k_out None: none
 PyObject *rope(PyObject *const *a) {
   int dev = -1;
   const Pages c = pages(a[8], a[9], dev);
   const Rows q = rows_of(a[0], dev, -1, -1), k = rows_of(a[1], dev, q.rows, c.hkv), v = rows_of(a[2], dev, q.rows, c.hkv);
-  const at::Tensor &qw = dense(a[3], dev, at::kBFloat16), &kw = dense(a[4], dev, at::kBFloat16);
-  need(qw.dim() == 1 && qw.size(0) == kHeadDim && kw.dim() == 1 && kw.size(0) == kHeadDim);
-  const int64_t *positions = indices(a[5], dev, q.rows), *slots = indices(a[10], dev, q.rows);
-  const at::Tensor &table = dense(a[6], dev, at::kFloat);
-  need(table.dim() == 2 && table.size(1) == kHeadDim);
-  const float eps = number(a[7]);
-  Rows ko = {nullptr, 0, 0, 0}, qo;
+  const Rope r = rope_of(a + 3, dev, q.rows);
+  const int64_t *slots = indices(a[10], dev, q.rows);
+  Rows ko = {nullptr, 0, 0, 0};
   if (a[12] != Py_None) {
     ko = rows_of(a[12], dev, q.rows, c.hkv);
     need(ko.p != k.p || ko.stride == k.stride);
   }
   const int nb = narrow(c.nb), bs = narrow(c.bs), t = narrow(q.rows), hq = narrow(q.heads), hkv = narrow(c.hkv);
-  const int table_rows = narrow(table.size(0));
   hipStream_t s = stream_on(dev);
   at::Tensor made;
-  if (a[11] != Py_None) {
-    qo = rows_of(a[11], dev, q.rows, q.heads);
-    need(qo.p != q.p || qo.stride == q.stride);
-  } else {
-    made = empty({q.rows, q.heads, kHeadDim}, at::kBFloat16, dev);
-    qo = {made.data_ptr(), q.heads * kHeadDim, q.rows, q.heads};
-  }
+  const Rows qo = result(a[11], dev, q, made);
+  need(qo.p != q.p || qo.stride == q.stride);
   const int status = call([&] {
-    return f_rope(qo.p, qo.stride, ko.p, ko.stride, q.p, q.stride, k.p, k.stride, v.p, v.stride, qw.data_ptr(),
-                  kw.data_ptr(), positions, table.data_ptr<float>(), table_rows, c.kc, c.ks, c.vc, c.vs, nb, bs, slots, t,
-                  hq, hkv, kHeadDim, eps, s);
+    return f_rope(qo.p, qo.stride, ko.p, ko.stride, q.p, q.stride, k.p, k.stride, v.p, v.stride, r.qw, r.kw,
+                  r.positions, r.table, r.rows, c.kc, c.ks, c.vc, c.vs, nb, bs, slots, t, hq, hkv, kHeadDim, r.eps, s);
   });
   if (status) return PyLong_FromLong(status);
   return made.defined() ? THPVariable_Wrap(std::move(made)) : same(a[11]);
 }
 
-// (out, q, key_pages, value_pages, block_tables, context_lens, scale, max_context_len, workspace) -> out; out None: a new one
+// (out, q, key_pages, value_pages, block_tables, context_lens, scale, max_context_len, workspace) -> out; out None: a
+// new one
 PyObject *decode(PyObject *const *a) {
   int dev = -1;
   const Pages c = pages(a[2], a[3], dev);
@@ -224,16 +239,37 @@ PyObject *decode(PyObject *const *a) {
   const int nb = narrow(c.nb), bs = narrow(c.bs), t = narrow(q.rows), hq = narrow(q.heads), hkv = narrow(c.hkv);
   hipStream_t s = stream_on(dev);
   at::Tensor made;
-  Rows out;
-  if (a[0] != Py_None) {
-    out = rows_of(a[0], dev, q.rows, q.heads);
-  } else {
-    made = empty({q.rows, q.heads, kHeadDim}, at::kBFloat16, dev);
-    out = {made.data_ptr(), q.heads * kHeadDim, q.rows, q.heads};
-  }
+  const Rows out = result(a[0], dev, q, made);
   const int status = call([&] {
     return f_decode(out.p, out.stride, q.p, q.stride, c.kc, c.ks, c.vc, c.vs, nb, bs, bt.p, bt.stride, bt.width, lens, t,
                     hq, hkv, kHeadDim, scale, most, space.data_ptr(), space.nbytes(), s);
+  });
+  if (status) return PyLong_FromLong(status);
+  return made.defined() ? THPVariable_Wrap(std::move(made)) : same(a[0]);
+}
+
+// (out, q, k, v, q_weight, k_weight, positions, cos_sin, eps, key_pages, value_pages, slot_mapping, block_tables,
+// context_lens, scale, max_context_len, workspace) -> out; out None: a new one
+PyObject *decode_fused(PyObject *const *a) {
+  int dev = -1;
+  const Pages c = pages(a[9], a[10], dev);
+  const Rows q = rows_of(a[1], dev, -1, -1), k = rows_of(a[2], dev, q.rows, c.hkv), v = rows_of(a[3], dev, q.rows, c.hkv);
+  const Rope r = rope_of(a + 4, dev, q.rows);
+  const int64_t *slots = indices(a[11], dev, q.rows);
+  const Table bt = table_of(a[12], dev, q.rows, true);
+  const int32_t *lens = lengths(a[13], dev, q.rows, true);
+  const float scale = number(a[14]);
+  const int most = integer(a[15]);
+  const at::Tensor &space = tensor(a[16], dev);
+  need(space.is_contiguous());
+  const int nb = narrow(c.nb), bs = narrow(c.bs), t = narrow(q.rows), hq = narrow(q.heads), hkv = narrow(c.hkv);
+  hipStream_t s = stream_on(dev);
+  at::Tensor made;
+  const Rows out = result(a[0], dev, q, made);
+  const int status = call([&] {
+    return f_fused(out.p, out.stride, q.p, q.stride, k.p, k.stride, v.p, v.stride, r.qw, r.kw, r.positions, r.table, r.rows,
+                   r.eps, c.kc, c.ks, c.vc, c.vs, nb, bs, slots, bt.p, bt.stride, bt.width, lens, t, hq, hkv, kHeadDim,
+                   scale, most, space.data_ptr(), space.nbytes(), s);
   });
   if (status) return PyLong_FromLong(status);
   return made.defined() ? THPVariable_Wrap(std::move(made)) : same(a[0]);
@@ -276,27 +312,31 @@ PyObject *entry(PyObject *, PyObject *const *args, Py_ssize_t n) {
   }
 }
 
-// (Fp4Pages, addresses of the six functions above)
+// (Fp4Pages, addresses of the functions above)
 PyObject *bind(PyObject *, PyObject *args) {
   PyObject *type;
-  unsigned long long p[6];
-  if (!PyArg_ParseTuple(args, "O!KKKKKK", &PyType_Type, &type, &p[0], &p[1], &p[2], &p[3], &p[4], &p[5])) return nullptr;
+  unsigned long long p[7];
+  if (!PyArg_ParseTuple(args, "O!KKKKKKK", &PyType_Type, &type, &p[0], &p[1], &p[2], &p[3], &p[4], &p[5], &p[6]))
+    return nullptr;
   f_write = reinterpret_cast<decltype(f_write)>(p[0]);
   f_read = reinterpret_cast<decltype(f_read)>(p[1]);
   f_rope = reinterpret_cast<decltype(f_rope)>(p[2]);
   f_decode = reinterpret_cast<decltype(f_decode)>(p[3]);
-  f_prefill = reinterpret_cast<decltype(f_prefill)>(p[4]);
-  f_prefill_space = reinterpret_cast<decltype(f_prefill_space)>(p[5]);
+  f_fused = reinterpret_cast<decltype(f_fused)>(p[4]);
+  f_prefill = reinterpret_cast<decltype(f_prefill)>(p[5]);
+  f_prefill_space = reinterpret_cast<decltype(f_prefill_space)>(p[6]);
   Py_INCREF(type);
   Py_XDECREF(reinterpret_cast<PyObject *>(pages_type));
   pages_type = reinterpret_cast<PyTypeObject *>(type);
   Py_RETURN_NONE;
 }
 
-#define ENTRY(name, args) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&entry<name, args>)), METH_FASTCALL, nullptr}
+#define ENTRY(name, args) \
+  { #name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&entry<name, args>)), METH_FASTCALL, nullptr }
 PyMethodDef methods[] = {
     {"bind", bind, METH_VARARGS, nullptr},
-    ENTRY(write, 5), ENTRY(read, 3), ENTRY(rope, 13), ENTRY(decode, 9), ENTRY(prefill, 9),
+    ENTRY(write, 5), ENTRY(read, 3), ENTRY(rope, 13), ENTRY(decode, 9), ENTRY(decode_fused, 17),
+    ENTRY(prefill, 9),
     {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_calls", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

@@ -10,29 +10,10 @@
 // All three are bound by memory: per head vector 256 bytes of bf16 and 68 of the cache, once.  36,488 tokens, 8 kv
 // heads (and 16 query heads): write 189 MB in 37 us (5.2 TB/s), read 189 MB in 34 us (5.6 TB/s), norm + RoPE + write
 // with the keys returned 564 MB in 115 us (4.9 TB/s); a large copy reaches 5.0 TB/s.  One token: 3 us, the launch.
-#include "fp4.h"
+#include "fp4_rows.h"
 
 namespace nvamd {
 namespace {
-
-// max over the 4 lanes of an aligned quad, of non-negative integers
-__device__ __forceinline__ u32 quad_max(u32 v) {
-  v = max(v, (u32)__builtin_amdgcn_mov_dpp((int)v, kDppQuadXor1, 0xF, 0xF, true));
-  v = max(v, (u32)__builtin_amdgcn_mov_dpp((int)v, kDppQuadXor2, 0xF, 0xF, true));
-  return v;
-}
-__device__ __forceinline__ u32 quad_xor2(u32 v) {
-  return (u32)__builtin_amdgcn_mov_dpp((int)v, kDppQuadXor2, 0xF, 0xF, true);
-}
-
-// Scale byte and codes of a lane's 8 values of a block that a quad shares.
-__device__ __forceinline__ u32 quantise8(u32x4 x, u32 &scale) {
-  u32 m = 0;
-#pragma unroll
-  for (int e = 0; e < 4; ++e) m = max(m, max(x[e] & 0x7fffu, (x[e] >> 16) & 0x7fffu));
-  scale = fp4_scale_byte(quad_max(m));
-  return scale == kFp4Nan ? 0u : fp4_codes(x, fp4_scale(scale));
-}
 
 // A 64-bit value of one lane, as a scalar.
 __device__ __forceinline__ int64_t lane_value(int64_t v, int lane) {
@@ -41,58 +22,6 @@ __device__ __forceinline__ int64_t lane_value(int64_t v, int lane) {
   return (int64_t)(((uint64_t)hi << 32) | lo);
 }
 __device__ __forceinline__ int64_t uniform64(int64_t v) { return lane_value(v, 0); }
-
-struct Fp4Row {
-  int64_t tile;  // 16-token tile of the row's page and head
-  int t;         // token of the tile
-};
-
-__device__ __forceinline__ Fp4Row row_at(int64_t slot, int head, int num_kv_heads, int bs_log2) {
-  const int64_t block = slot >> bs_log2;
-  const int token = (int)(slot & ((1 << bs_log2) - 1));
-  return {fp4_tile(block, token, head, num_kv_heads, bs_log2), token & 15};
-}
-
-// lo / hi: dims 8c.. and 64 + 8c.. of the row, c = lane of the 8.
-__device__ __forceinline__ void store_key(const Fp4Cache &cache, const Fp4Row &r, int c, u32x4 lo, u32x4 hi) {
-  u32 s_lo, s_hi;
-  const u32 w_lo = quantise8(lo, s_lo), w_hi = quantise8(hi, s_hi);
-  u32 *row = reinterpret_cast<u32 *>(cache.k_codes + r.tile * kFp4TileBytes + r.t * kFp4RowBytes);
-  row[c] = w_lo;
-  row[8 + c] = w_hi;
-  if ((c & 3) == 0) {
-    u8 *s = cache.k_scales + r.tile * kFp4TileScales;
-    s[fp4_key_scale_at(r.t, c >> 2)] = (u8)s_lo;
-    s[fp4_key_scale_at(r.t, 2 + (c >> 2))] = (u8)s_hi;
-  }
-}
-
-// A byte of the values holds dims 32q + r and 32q + 16 + r: the two lanes of a quad that differ in bit 1 hold the two
-// halves of a block, and exchange so that the one builds the bytes of the low block, the other those of the high one.
-// The bytes go to `tile` in LDS, [64 bytes of a row][8 tokens], at token `tok`.
-__device__ __forceinline__ void value_bytes(const Fp4Cache &cache, const Fp4Row &r, bool live, int c, int tok, u32x4 lo,
-                                            u32x4 hi, u8 *tile) {
-  u32 s_lo, s_hi;
-  const u32 w_lo = quantise8(lo, s_lo), w_hi = quantise8(hi, s_hi);
-  const u32 o_lo = quad_xor2(w_lo), o_hi = quad_xor2(w_hi);
-  const bool second = (c & 2) != 0;
-  const u32 first16 = second ? o_hi : w_lo, last16 = second ? w_hi : o_lo;
-  // bytes j of even and of odd nibbles: (low nibble of the first half, low nibble of the second)
-  const u32 even = (first16 & 0x0f0f0f0fu) | ((last16 & 0x0f0f0f0fu) << 4);
-  const u32 odd = ((first16 >> 4) & 0x0f0f0f0fu) | (last16 & 0xf0f0f0f0u);
-  const int q = (second ? 2 : 0) + (c >> 2);
-  u8 *p = tile + (16 * q + 8 * (c & 1)) * 8 + tok;
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    p[(2 * j) * 8] = (u8)(even >> (8 * j));
-    p[(2 * j + 1) * 8] = (u8)(odd >> (8 * j));
-  }
-  if (live && (c & 3) == 0) {
-    u8 *s = cache.v_scales + r.tile * kFp4TileScales;
-    s[fp4_value_scale_at(r.t, c >> 2)] = (u8)s_lo;
-    s[fp4_value_scale_at(r.t, 2 + (c >> 2))] = (u8)s_hi;
-  }
-}
 
 // The 8 tokens' bytes of row byte `lane` to their slots.  Where the slots follow one another the bytes are turned to
 // their places in 8-byte half rows: one store if they fill one, else those of each side of the border, words where
@@ -133,9 +62,6 @@ __device__ __forceinline__ void store_values(const Fp4Cache &cache, const u8 *ti
     if (s >= 0) *place(s) = (u8)(w[i >> 2] >> (8 * (i & 3)));
   }
 }
-
-// A wave's own LDS writes before its own reads: LDS serves a wave in order, so only the compiler has to keep it.
-__device__ __forceinline__ void wave_lds_fence() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); }
 
 // Rows too many for the caches until their next use go past them (32 MB a tensor: half of the 256 MB Infinity Cache for
 // two tensors in and out).  36,488 x 8 heads, plain / nontemporal: written 43.8 / 39.2 us, read 46.5 / 38.2; 12,345 x 8
@@ -285,61 +211,6 @@ struct NormRopeFp4Args {
   float eps;
 };
 
-__device__ __forceinline__ double dpp_add(double v, int lo, int hi) {
-  return v + __builtin_bit_cast(double, ((uint64_t)(u32)hi << 32) | (u32)lo);
-}
-template <int CTRL>
-__device__ __forceinline__ double dpp_sum(double v) {
-  const uint64_t b = __builtin_bit_cast(uint64_t, v);
-  return dpp_add(v, __builtin_amdgcn_mov_dpp((int)(u32)b, CTRL, 0xF, 0xF, true),
-                 __builtin_amdgcn_mov_dpp((int)(u32)(b >> 32), CTRL, 0xF, 0xF, true));
-}
-__device__ __forceinline__ double dpp_sum8(double v) {
-  return dpp_sum<kDppHalfMirror>(dpp_sum<kDppQuadXor2>(dpp_sum<kDppQuadXor1>(v)));
-}
-
-// A 32-bit value that rounds to bf16 as x does.  A plain cast rounds too, and may land on a border of bf16 that x is
-// only close to; here all but the top 20 bits of the fraction are cut off, and the last of these is set if any of the
-// rest was.
-__device__ __forceinline__ float bf16_bound(double x) {
-  const uint64_t b = __builtin_bit_cast(uint64_t, x);
-  const uint64_t top = (uint64_t)((u32)(b >> 32) | ((u32)b != 0u ? 1u : 0u)) << 32;
-  return (float)__builtin_bit_cast(double, top);
-}
-
-// y = x * rsqrt(mean(x^2) + eps) * w, then the rotation out[d] = y[d] cos[d] - y[d+64] sin[d], out[d+64] = y[d+64]
-// cos[d] + y[d] sin[d], in 64 bits with one rounding to bf16 at the end.  A 4-bit code's step is a
-// third to a half of the value, so a key that 32-bit arithmetic puts on the other side of a rounding border is that far
-// off; in 64 bits the code is that of the exact value.  x w is a product of bf16 numbers, exact in 32 bits, and the
-// reciprocal root comes last: one multiplication for each result.
-__device__ __forceinline__ void norm_rope_f64(u32x4 &lo, u32x4 &hi, const u32x4 w_lo, const u32x4 w_hi,
-                                              const float (&cs)[8], const float (&sn)[8], double eps) {
-  double ss = 0.0;
-#pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    const double x0 = bf16_lo(lo[e]), x1 = bf16_hi(lo[e]), x2 = bf16_lo(hi[e]), x3 = bf16_hi(hi[e]);
-    ss += x0 * x0;
-    ss += x1 * x1;
-    ss += x2 * x2;
-    ss += x3 * x3;
-  }
-  const double rstd = rsqrt(dpp_sum8(ss) * (1.0 / kHeadDim) + eps);
-#pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    float r_lo[2], r_hi[2];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const double y_lo = i ? bf16_hi(lo[e]) * bf16_hi(w_lo[e]) : bf16_lo(lo[e]) * bf16_lo(w_lo[e]);
-      const double y_hi = i ? bf16_hi(hi[e]) * bf16_hi(w_hi[e]) : bf16_lo(hi[e]) * bf16_lo(w_hi[e]);
-      const double c = cs[2 * e + i], s = sn[2 * e + i];
-      r_lo[i] = bf16_bound((y_lo * c - y_hi * s) * rstd);
-      r_hi[i] = bf16_bound((y_hi * c + y_lo * s) * rstd);
-    }
-    lo[e] = pack_bf16x2(r_lo[0], r_lo[1]);
-    hi[e] = pack_bf16x2(r_hi[0], r_hi[1]);
-  }
-}
-
 // A wave: 8 tokens, heads_per_wave of the vectors of each: its query heads, its key heads, its value heads.
 template <bool ROPE, bool STREAM>
 __global__ void __launch_bounds__(256)
@@ -416,7 +287,8 @@ rows_fp4_kernel(NormRopeFp4Args a) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) asm volatile("" : "+v"(cs[e]), "+v"(sn[e]));
       asm volatile("" : "+v"(qw_lo), "+v"(qw_hi), "+v"(kw_lo), "+v"(kw_hi));
-      norm_rope_f64(lo, hi, is_q ? qw_lo : kw_lo, is_q ? qw_hi : kw_hi, cs, sn, (double)a.eps);
+      const double rstd = norm_factor(dpp_sum8(sum_squares(lo, hi)), (double)a.eps);
+      norm_rope_f64(lo, hi, is_q ? qw_lo : kw_lo, is_q ? qw_hi : kw_hi, cs, sn, rstd);
       u16 *dst = is_q ? a.q_out + tt * a.q_out_stride + v * kHeadDim
                       : a.k_out ? a.k_out + tt * a.k_out_stride + (v - hq) * kHeadDim : nullptr;
       if (dst != nullptr && exists) {

@@ -11,8 +11,8 @@
 // A wave takes 64 tokens at a time, four 16-token tiles, one per 16 lanes (gq = lane / 16):
 //   S^T = K . Q^T  v_mfma_scale_f32_16x16x128_f8f6f4 on the codes as they lie in the cache, A = 16 rows of K: a lane's
 //        16 bytes are one block of a row, under one scale.  B = the heads as 16 columns, in 8 bits twice: a bf16 query
-//        is the sum of two e4m3 numbers under a scale for each block (QueryScale), so two products give the scores.  That takes
-//        the matrix cores as long as four bf16 products, and the vector ALUs no expansion of K.
+//        is the sum of two e4m3 numbers under a scale for each block (QueryScale), so two products give the scores.
+//        That takes the matrix cores as long as four bf16 products, and the vector ALUs no expansion of K.
 //        Row 4a + i of product t is token 4t + i of tile a: lane (h, gq) then finds the scores of tile gq's tokens
 //        4t .. 4t+3 of head h in its accumulator of product t, that is of all 16 tokens in the four products;
 //   softmax  on up to 4 (8) heads the accumulators' 16 columns are mostly repeats: products 1..3 (2, 3) move into the
@@ -24,11 +24,14 @@
 // The score of a token past the context is replaced by -inf and the scales of its values by zero, whatever bytes it
 // holds.
 //
-// Bound by memory where contexts are long: 100 x U[2048, 4096] tokens of 8 kv heads, 330 MB, 59 .. 63 us (5.2 .. 5.6 TB/s,
-// part of it from the Infinity Cache; a large copy 5.0); 4 x U[8192, 40960], 91 MB, 21 us.  Below that by what every call
-// pays: some 2 us of launch, 1.3 to the first load (contexts, table, query) and 2 to 4 for the join: 32 x U[256, 2304],
-// 46 MB, 16 us, 4 x U[1, 512] 6.2.
+// Bound by memory where contexts are long: 100 x U[2048, 4096] tokens of 8 kv heads, 330 MB, 59 .. 63 us (5.2 .. 5.6
+// TB/s, part of it from the Infinity Cache; a large copy 5.0); 4 x U[8192, 40960], 91 MB, 21 us.  Below that by what
+// every call pays: some 2 us of launch, 1.3 to the first load (contexts, table, query) and 2 to 4 for the join: 32 x
+// U[256, 2304], 46 MB, 16 us, 4 x U[1, 512] 6.2.
 #include "fp4_attention.h"
+#include "fp4_rows.h"
+
+#include <type_traits>
 
 namespace nvamd {
 namespace {
@@ -70,6 +73,83 @@ struct DecodeFp4Args {
   u32 *err;
 };
 
+// The step before the attention, where the kernel makes it too: q, k and v as they are projected.
+struct StepArgs {
+  const u16 *k;
+  int64_t k_stride;
+  const u16 *v;
+  int64_t v_stride;
+  const u16 *q_w;
+  const u16 *k_w;
+  const int64_t *positions;
+  const float *cos_sin;
+  const int64_t *slots;
+  int64_t num_slots;
+  int max_positions;
+  float eps;
+};
+struct Nothing {};
+
+__device__ __forceinline__ double swap_sum16(double v) {  // over lanes l and l ^ 16
+  const uint64_t b = __builtin_bit_cast(uint64_t, v);
+  const auto lo = __builtin_amdgcn_permlane16_swap((u32)b, (u32)b, false, false);
+  const auto hi = __builtin_amdgcn_permlane16_swap((u32)(b >> 32), (u32)(b >> 32), false, false);
+  return __builtin_bit_cast(double, (uint64_t)(u32)hi[0] << 32 | (u32)lo[0]) +
+         __builtin_bit_cast(double, (uint64_t)(u32)hi[1] << 32 | (u32)lo[1]);
+}
+__device__ __forceinline__ double swap_sum32(double v) {  // over lanes l and l ^ 32
+  const uint64_t b = __builtin_bit_cast(uint64_t, v);
+  const auto lo = __builtin_amdgcn_permlane32_swap((u32)b, (u32)b, false, false);
+  const auto hi = __builtin_amdgcn_permlane32_swap((u32)(b >> 32), (u32)(b >> 32), false, false);
+  return __builtin_bit_cast(double, (uint64_t)(u32)hi[0] << 32 | (u32)lo[0]) +
+         __builtin_bit_cast(double, (uint64_t)(u32)hi[1] << 32 | (u32)lo[1]);
+}
+__device__ __forceinline__ void load8(const float *p, float (&x)[8]) {
+  const f32x4 a = *reinterpret_cast<const f32x4 *>(p), b = *reinterpret_cast<const f32x4 *>(p + 4);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) x[e] = e < 4 ? a[e & 3] : b[e & 3];
+}
+
+// Norm and rotation of a query row whose lane gq holds dims 16 gq .. +15 and 64 + 16 gq .. +15: what two lanes of 8
+// hold elsewhere, summed in the same order, so that the bits are the same.
+__device__ __forceinline__ void norm_rope_row(u32x4 (&x)[4], const u16 *weight, const float *row, int gq, double eps) {
+  const double pair = sum_squares(x[0], x[2]) + sum_squares(x[1], x[3]);
+  const double rstd = norm_factor(swap_sum32(swap_sum16(pair)), eps);
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const int at = 16 * gq + 8 * j;
+    float cs[8], sn[8];
+    load8(row + at, cs);
+    load8(row + 64 + at, sn);
+    norm_rope_f64(x[j], x[2 + j], ld16(weight + at), ld16(weight + 64 + at), cs, sn, rstd);
+  }
+}
+
+// The new token's k (normed and rotated) and v of a kv head into its slot: lanes 0 .. 7 of a wave the key, 8 .. 15 the
+// value, whose bytes go through 512 bytes of LDS.
+__device__ __forceinline__ void store_row(const Fp4Cache &cache, const StepArgs &s, int b, int g, int64_t slot,
+                                          const float *row, int num_kv_heads, int bs_log2, int lane, u8 *tile) {
+  const int c = lane & 7;
+  const bool is_key = lane < 8;
+  const Fp4Row at = row_at(slot, g, num_kv_heads, bs_log2);
+  if (lane < 16) {
+    const u16 *p = (is_key ? s.k + b * s.k_stride : s.v + b * s.v_stride) + g * kHeadDim + 8 * c;
+    u32x4 lo = ld16(p), hi = ld16(p + 64);
+    if (is_key) {
+      float cs[8], sn[8];
+      load8(row + 8 * c, cs);
+      load8(row + 64 + 8 * c, sn);
+      const double rstd = norm_factor(dpp_sum8(sum_squares(lo, hi)), (double)s.eps);
+      norm_rope_f64(lo, hi, ld16(s.k_w + 8 * c), ld16(s.k_w + 64 + 8 * c), cs, sn, rstd);
+      store_key(cache, at, c, lo, hi);
+    } else {
+      value_bytes(cache, at, true, c, 0, lo, hi, tile);
+    }
+  }
+  wave_lds_fence();
+  cache.v_codes[at.tile * kFp4TileBytes + lane * kFp4Tile + at.t] = tile[lane * 8];
+}
+
 // Inclusive prefix sum over a wave (see paged_decode.hip).
 __device__ __forceinline__ int wave_scan(int v, int lane) {
   v += __builtin_amdgcn_mov_dpp(v, 0x111, 0xF, 0xF, true);
@@ -105,9 +185,13 @@ __host__ __device__ constexpr int max_partitions(int units) { return partition_s
 // GP: heads that the registers and LDS are laid out for (2 heads at 4 x U[1, 512]: 6.2 us as 4, 6.5 as 16; at 100 x
 // U[2048, 4096] 63.2, 63.6).  WIDE: pages of 64 tokens or more, so that the 64 tokens of a wave's step lie in one page,
 // whose id is a scalar (pages of 128 at 32 x U[256, 2304]: 16.3 us, without 20.8; at 100 x U[2048, 4096] 63, 73).
-template <int GP, bool WIDE>
+// FUSED: the norm, the rotation and the store of the step's rows first.  Every workgroup makes its own queries; the one
+// whose partition ends the context stores the new row and waits for it, so that its loads find it.  Bits as of
+// nvamd_qk_norm_rope_fp4 and this kernel after it, in less time: 32 x U[256, 2304] 17.3 us for 19.9 (this kernel alone
+// 15.9), 16 x U[512, 4096] at 64 heads 15.6 for 17.8, 100 x U[2048, 4096] 66.6 for 67.8, 4 x U[1, 512] 6.8 for 8.0.
+template <int GP, bool WIDE, bool FUSED>
 __global__ void __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(WIDE ? 4 : 3)))
-paged_decode_fp4_kernel(DecodeFp4Args a) {
+paged_decode_fp4_kernel(DecodeFp4Args a, std::conditional_t<FUSED, StepArgs, Nothing> step_args) {
   constexpr int D = kHeadDim;
   constexpr int HS = kPartFloats;
   __shared__ __attribute__((aligned(16))) float s_o[kWaves][GP * HS];
@@ -166,9 +250,58 @@ paged_decode_fp4_kernel(DecodeFp4Args a) {
   // Query operand of head n (columns past the last head repeat it and are never read).
   i32x8 q_hi, q_lo;
   u32 q_scale;
-  {
+  auto load_query = [&](u32x4 (&x)[4]) {
     const u16 *qp = a.q + (int64_t)b * a.q_stride + (int64_t)(head0 + min(n, G - 1)) * D + 16 * gq;
-    const u32x4 x[4] = {ld16(qp), ld16(qp + 8), ld16(qp + 64), ld16(qp + 72)};
+    x[0] = ld16(qp);
+    x[1] = ld16(qp + 8);
+    x[2] = ld16(qp + 64);
+    x[3] = ld16(qp + 72);
+  };
+  if constexpr (FUSED) {
+    // One wave makes the operand for all (the 64-bit arithmetic of 8 waves at once takes 3 us more), another stores the
+    // row.
+    __shared__ __attribute__((aligned(16))) u32x4 s_q[4][64];
+    __shared__ u32 s_q_scale[64];
+    int64_t pos = step_args.positions[b];
+    if (pos < 0 || pos >= step_args.max_positions) {  // clamp and report
+      err_bits |= NVAMD_ERR_POSITION;
+      pos = pos < 0 ? 0 : step_args.max_positions - 1;
+    }
+    const float *row = step_args.cos_sin + pos * D;
+    if (w == 1) {
+      u32x4 x[4];
+      load_query(x);
+      norm_rope_row(x, step_args.q_w, row, gq, (double)step_args.eps);
+      s_q_scale[lane] = query_operand(x, gq, q_hi, q_lo);
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        s_q[j][lane] = u32x4{(u32)q_hi[4 * j], (u32)q_hi[4 * j + 1], (u32)q_hi[4 * j + 2], (u32)q_hi[4 * j + 3]};
+        s_q[2 + j][lane] = u32x4{(u32)q_lo[4 * j], (u32)q_lo[4 * j + 1], (u32)q_lo[4 * j + 2], (u32)q_lo[4 * j + 3]};
+      }
+    } else if (w == 0 && p == n_parts - 1 && a.q_head0 == 0) {
+      const int64_t slot = step_args.slots[b];
+      if (slot < -1 || slot >= step_args.num_slots) {
+        err_bits |= NVAMD_ERR_SLOT;
+      } else if (slot >= 0) {
+        store_row(a.cache, step_args, b, g, slot, row, hkv, a.bs_log2, lane, reinterpret_cast<u8 *>(&s_o[0][0]));
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
+        __builtin_amdgcn_s_waitcnt(0);  // before this workgroup's loads of the row
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const u32x4 h = s_q[j][lane], l = s_q[2 + j][lane];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        q_hi[4 * j + i] = (int)h[i];
+        q_lo[4 * j + i] = (int)l[i];
+      }
+    }
+    q_scale = s_q_scale[lane];
+  } else {
+    u32x4 x[4];
+    load_query(x);
     q_scale = query_operand(x, gq, q_hi, q_lo);
   }
 
@@ -474,31 +607,39 @@ paged_decode_fp4_kernel(DecodeFp4Args a) {
   }
 }
 
-template <int GP>
-int launch(const DecodeFp4Args &a, hipStream_t stream) {
+template <int GP, typename Step>
+int launch(const DecodeFp4Args &a, const Step &s, hipStream_t stream) {
+  constexpr bool FUSED = std::is_same_v<Step, StepArgs>;
   static_assert(kWaves * GP >= kHalves, "the shares of a join fit s_o");
   const int units = a.batch * a.num_kv_heads;  // <= kCounterSlots
   const int64_t items = min((int64_t)units * a.max_parts, (int64_t)max_partitions(units));
+  const dim3 grid((unsigned)items), block(kWaves * 64);
   if (a.bs_log2 >= 6)
-    hipLaunchKernelGGL((paged_decode_fp4_kernel<GP, true>), dim3((unsigned)items), dim3(kWaves * 64), 0, stream, a);
+    hipLaunchKernelGGL((paged_decode_fp4_kernel<GP, true, FUSED>), grid, block, 0, stream, a, s);
   else
-    hipLaunchKernelGGL((paged_decode_fp4_kernel<GP, false>), dim3((unsigned)items), dim3(kWaves * 64), 0, stream, a);
+    hipLaunchKernelGGL((paged_decode_fp4_kernel<GP, false, FUSED>), grid, block, 0, stream, a, s);
   return launch_status();
 }
 
-}  // namespace
-}  // namespace nvamd
+template <typename Step>
+int launch_groups(DecodeFp4Args &a, const Step &s, hipStream_t stream) {
+  for (a.q_head0 = 0; a.q_head0 < a.q_group; a.q_head0 += a.q_sub) {
+    a.q_sub = min(a.q_group - a.q_head0, kMaxHeads);
+    const int st = a.q_sub <= 4   ? launch<4>(a, s, stream)
+                   : a.q_sub <= 8 ? launch<8>(a, s, stream)
+                                  : launch<16>(a, s, stream);
+    if (st != NVAMD_OK) return st;
+  }
+  return NVAMD_OK;
+}
 
-using namespace nvamd;
-
-extern "C" int nvamd_paged_decode_fp4(void *out, int64_t out_stride, const void *q, int64_t q_stride,
-                                      const void *k_codes, const void *k_scales, const void *v_codes,
-                                      const void *v_scales, int num_blocks, int block_size,
-                                      const int32_t *block_tables, int bt_stride, int bt_width,
-                                      const int32_t *context_lens, int batch, int num_heads, int num_kv_heads,
-                                      int head_dim, float scale, int max_context_len, void *workspace,
-                                      size_t workspace_bytes, hipStream_t stream) {
-  if (batch == 0) return NVAMD_OK;
+// Checks shared by the entry points; fills what they share.
+int fill_decode_args(DecodeFp4Args &a, void *out, int64_t out_stride, const void *q, int64_t q_stride,
+                     const void *k_codes, const void *k_scales, const void *v_codes, const void *v_scales,
+                     int num_blocks, int block_size,
+                     const int32_t *block_tables, int bt_stride, int bt_width, const int32_t *context_lens, int batch,
+                     int num_heads, int num_kv_heads, int head_dim, float scale, int max_context_len, void *workspace,
+                     size_t workspace_bytes) {
   if (!out || !q || !fp4_cache_ok(k_codes, k_scales, v_codes, v_scales) || !block_tables || !context_lens)
     return NVAMD_EINVAL;
   if (batch < 0 || num_blocks <= 0 || num_kv_heads <= 0 || num_heads <= 0 || bt_width <= 0 || bt_stride < bt_width ||
@@ -517,7 +658,7 @@ extern "C" int nvamd_paged_decode_fp4(void *out, int64_t out_stride, const void 
     return NVAMD_EWORKSPACE;
   if (!aligned16(workspace)) return NVAMD_EINVAL;
 
-  DecodeFp4Args a = {};
+  a = {};
   a.out = static_cast<u16 *>(out);
   a.out_stride = out_stride;
   a.q = static_cast<const u16 *>(q);
@@ -541,10 +682,63 @@ extern "C" int nvamd_paged_decode_fp4(void *out, int64_t out_stride, const void 
   a.scale_log2e = scale * kLog2e;
   a.q_group = num_heads / num_kv_heads;
   a.err = index_error_word();
-  for (a.q_head0 = 0; a.q_head0 < a.q_group; a.q_head0 += a.q_sub) {
-    a.q_sub = min(a.q_group - a.q_head0, kMaxHeads);
-    const int st = a.q_sub <= 4 ? launch<4>(a, stream) : a.q_sub <= 8 ? launch<8>(a, stream) : launch<16>(a, stream);
-    if (st != NVAMD_OK) return st;
-  }
   return NVAMD_OK;
+}
+
+}  // namespace
+}  // namespace nvamd
+
+using namespace nvamd;
+
+extern "C" int nvamd_paged_decode_fp4(void *out, int64_t out_stride, const void *q, int64_t q_stride,
+                                      const void *k_codes, const void *k_scales, const void *v_codes,
+                                      const void *v_scales, int num_blocks, int block_size,
+                                      const int32_t *block_tables, int bt_stride, int bt_width,
+                                      const int32_t *context_lens, int batch, int num_heads, int num_kv_heads,
+                                      int head_dim, float scale, int max_context_len, void *workspace,
+                                      size_t workspace_bytes, hipStream_t stream) {
+  if (batch == 0) return NVAMD_OK;
+  DecodeFp4Args a;
+  const int st = fill_decode_args(a, out, out_stride, q, q_stride, k_codes, k_scales, v_codes, v_scales, num_blocks,
+                                  block_size, block_tables, bt_stride, bt_width, context_lens, batch, num_heads,
+                                  num_kv_heads, head_dim, scale, max_context_len, workspace, workspace_bytes);
+  if (st != NVAMD_OK) return st;
+  return launch_groups(a, Nothing{}, stream);
+}
+
+extern "C" int nvamd_paged_decode_fused_fp4(void *out, int64_t out_stride, const void *q, int64_t q_stride,
+                                            const void *k, int64_t k_stride, const void *v, int64_t v_stride,
+                                            const void *q_weight, const void *k_weight, const int64_t *positions,
+                                            const float *cos_sin, int max_positions, float eps, void *k_codes,
+                                            void *k_scales, void *v_codes, void *v_scales, int num_blocks,
+                                            int block_size, const int64_t *slot_mapping, const int32_t *block_tables,
+                                            int bt_stride, int bt_width, const int32_t *context_lens, int batch,
+                                            int num_heads, int num_kv_heads, int head_dim, float scale,
+                                            int max_context_len, void *workspace, size_t workspace_bytes,
+                                            hipStream_t stream) {
+  if (batch == 0) return NVAMD_OK;
+  DecodeFp4Args a;
+  const int st = fill_decode_args(a, out, out_stride, q, q_stride, k_codes, k_scales, v_codes, v_scales, num_blocks,
+                                  block_size, block_tables, bt_stride, bt_width, context_lens, batch, num_heads,
+                                  num_kv_heads, head_dim, scale, max_context_len, workspace, workspace_bytes);
+  if (st != NVAMD_OK) return st;
+  const int64_t row = (int64_t)num_kv_heads * kHeadDim;
+  if (!k || !v || !aligned16(k) || !aligned16(v) || k_stride % 8 || v_stride % 8 || k_stride < row || v_stride < row ||
+      !q_weight || !k_weight || !aligned16(q_weight) || !aligned16(k_weight) || !positions || !cos_sin ||
+      !aligned16(cos_sin) || max_positions <= 0 || !slot_mapping)
+    return NVAMD_EINVAL;
+  StepArgs s;
+  s.k = static_cast<const u16 *>(k);
+  s.k_stride = k_stride;
+  s.v = static_cast<const u16 *>(v);
+  s.v_stride = v_stride;
+  s.q_w = static_cast<const u16 *>(q_weight);
+  s.k_w = static_cast<const u16 *>(k_weight);
+  s.positions = positions;
+  s.cos_sin = cos_sin;
+  s.slots = slot_mapping;
+  s.num_slots = (int64_t)num_blocks * block_size;
+  s.max_positions = max_positions;
+  s.eps = eps;
+  return launch_groups(a, s, stream);
 }

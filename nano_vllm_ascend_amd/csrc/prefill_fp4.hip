@@ -165,8 +165,8 @@ struct Stage {
 };
 constexpr int kRowPad = kHeadDim + 8;  // elements of a row in the output's turn: 16 bytes of padding spread the banks
 
-// WIDE: pages of 32 tokens or more, so that a tile's keys lie in one page and K loads from a scalar address (702 us, 705
-// without, where the header counts 689; the strips gain nothing by it).
+// WIDE: pages of 32 tokens or more, so that a tile's keys lie in one page and K loads from a scalar address (702 us,
+// 705 without, where the header counts 689; the strips gain nothing by it).
 template <bool WIDE>
 __global__ void __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(3)))
 prefill_fp4_kernel(PrefillFp4Args a) {

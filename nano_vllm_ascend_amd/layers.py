@@ -129,24 +129,23 @@ class HipPagedAttention(nn.Module):
                     workspace: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
         """One launch for a decode batch: q/k RMSNorm + RoPE, the KV store of post-RoPE k and raw v at
         slot_mapping, then this attention -- bit-identical to qk_norm_rope followed by forward().
-        q, k, v are the raw projection rows and are left unmodified.  A 4-bit cache takes two launches."""
+        q, k, v are the raw projection rows and are left unmodified."""
         total_tokens, num_heads, head_dim = q.shape
         if num_heads != self.num_heads or head_dim != self.head_dim:
             raise ValueError(f"query shape mismatch: got {tuple(q.shape)}")
-        if isinstance(key_cache, _C.Fp4Pages):
-            rotated = _C.qk_norm_rope_fp4(q, k, v, q_norm.weight, k_norm.weight, positions, rotary.cos_sin,
-                                          q_norm.variance_epsilon, key_cache, value_cache, slot_mapping)
-            return self.forward(rotated, key_cache, value_cache, block_tables, context_lens, max_context_len, workspace,
-                                out)
         if max_context_len is None:
             max_context_len = block_tables.shape[1] * key_cache.shape[1]
         if context_lens.device != q.device:
             context_lens = context_lens.to(q.device, non_blocking=True)
         if workspace is None:
             workspace = self.workspace(total_tokens, max_context_len, q.device)
-        out = torch.empty_like(q) if out is None else out
         if context_lens.dtype is not torch.int32:
             context_lens = context_lens.to(torch.int32)
+        if isinstance(key_cache, _C.Fp4Pages):
+            return _C.paged_decode_fused_fp4(out, q, k, v, q_norm.weight, k_norm.weight, positions, rotary.cos_sin,
+                                             q_norm.variance_epsilon, key_cache, value_cache, slot_mapping,
+                                             block_tables, context_lens, self.scale, max_context_len, workspace)
+        out = torch.empty_like(q) if out is None else out
         return _C.paged_decode_fused(out, q, k, v, q_norm.weight, k_norm.weight, positions, rotary.cos_sin,
                                      q_norm.variance_epsilon, key_cache, value_cache, slot_mapping, block_tables,
                                      context_lens, self.scale, max_context_len, workspace)

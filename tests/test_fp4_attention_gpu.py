@@ -571,6 +571,68 @@ def test_prefill_replays_from_a_graph(device):
         assert torch.equal(got, call(torch.empty_like(q)))
 
 
+# -------------------------------------------------------------------------------------------- a whole decode step
+def step_of(batch, seed, slots=None):
+    """Projected rows of a new token for each sequence of the batch, whose last position is the token's."""
+    gen = torch.Generator().manual_seed(seed)
+    b = len(batch.lens)
+    qkv = torch.randn(b, batch.hq + 2 * batch.hkv, 128, generator=gen).bfloat16().to(batch.device)
+    q, k, v = qkv.split([batch.hq, batch.hkv, batch.hkv], 1)
+    weights = [(1 + 0.1 * torch.randn(128, generator=gen)).bfloat16().to(batch.device) for _ in range(2)]
+    angle = torch.rand(64, 64, generator=gen) * 7
+    table = torch.cat((angle.cos(), angle.sin()), 1).to(batch.device)
+    pos = torch.randint(0, 64, (b,), generator=gen).to(batch.device)
+    if slots is None:
+        slots = torch.stack([s[-1] if len(s) else torch.tensor(-1) for s in batch.slots])
+    return q, k, v, *weights, pos, table, 1e-6, batch.keys, batch.values, slots.to(batch.device)
+
+
+def attend(batch, q, bound, workspace, fused=None):
+    tables, lens = batch.tables.to(batch.device), torch.tensor(batch.lens, dtype=torch.int32, device=batch.device)
+    if fused is None:
+        return _C.paged_decode_fp4(None, q, batch.keys, batch.values, tables, lens, SCALE, bound, workspace)
+    return _C.paged_decode_fused_fp4(q, *fused, tables, lens, SCALE, bound, workspace)
+
+
+def in_pages(batch):
+    return [t.clone() for t in (*batch.keys, *batch.values)]
+
+
+@pytest.mark.parametrize("hq, hkv, bs", [(16, 8, 128), (1, 1, 16), (12, 4, 32), (8, 1, 64), (40, 8, 16), (17, 1, 256),
+                                         (34, 2, 128)])
+def test_fused_step_has_the_bits_of_the_two_launches(device, hq, hkv, bs):
+    batch = Batch(device, [1, 16, 17, 300, 0, 512, 513, 1100, 4097], hq, hkv, bs, seed=hq + bs)
+    space = _C.alloc_paged_decode_workspace(9, hq, hkv, 8192, device)
+    for bound in (4097, 8192):
+        batch.upload()
+        args = step_of(batch, seed=bound)
+        raw = [t.clone() for t in args[:3]]
+        want = attend(batch, _C.qk_norm_rope_fp4(*args), bound, space)
+        stored = in_pages(batch)
+        batch.upload()
+        got = attend(batch, None, bound, space, fused=step_of(batch, seed=bound))
+        assert torch.equal(got, want) and all(torch.equal(a, b) for a, b in zip(in_pages(batch), stored))
+        assert all(torch.equal(a, b) for a, b in zip(args[:3], raw))
+    assert _C.index_errors() == 0
+
+
+def test_fused_step_reports_what_it_skips_and_clamps(device):
+    batch = Batch(device, [30, 40, 50], 4, 2, 16, seed=24)
+    space = _C.alloc_paged_decode_workspace(3, 4, 2, 64, device)
+    slots = torch.stack([s[-1] for s in batch.slots])
+    before = in_pages(batch)
+    for bad, word in ((torch.tensor(-1), 0), (torch.tensor(-2), _C.ERR_SLOT), (torch.tensor(batch.nb * 16), _C.ERR_SLOT)):
+        attend(batch, None, 64, space, fused=step_of(batch, 25, slots=torch.stack([bad] * 3)))
+        assert _C.index_errors() == word and all(torch.equal(a, b) for a, b in zip(in_pages(batch), before))
+        _C.clear_index_errors()
+    args = list(step_of(batch, 26, slots=slots))
+    good = attend(batch, None, 64, space, fused=args)
+    args[5] = args[5].clone()
+    args[5][1] = 64
+    got = attend(batch, None, 64, space, fused=args)
+    assert _C.index_errors() == _C.ERR_POSITION and torch.equal(got[::2], good[::2])
+
+
 # -------------------------------------------------------------------------------------------- the two routes of a call
 def test_a_call_made_at_once_equals_one_that_python_checks(device):
     """Range checks send the calls through the checks of _C.py; without them csrc/calls.cpp makes those that are plain."""
@@ -601,6 +663,9 @@ def test_a_call_made_at_once_equals_one_that_python_checks(device):
         k_out = torch.zeros(9, 2, 128, dtype=torch.bfloat16, device=device)
         got.append(_C.qk_norm_rope_fp4(q, k, v, *weights, pos, table, 1e-6, *pages, slots, k_out=k_out))
         got.append(_C.qk_norm_rope_fp4(q, k, v, *weights, pos, table, 1e-6, *pages, slots, q_out=torch.empty_like(got[-1])))
+        last = torch.stack([s[-1] for s in batch.slots]).to(device)
+        fused = q[:3], k[:3], v[:3], *weights, pos[:3], table, 1e-6, *pages, last, tables, lens, SCALE, 5000, space
+        got += [_C.paged_decode_fused_fp4(None, *fused), _C.paged_decode_fused_fp4(torch.empty_like(got[0]), *fused)]
         return [t.clone() for t in (*got, k_out, *pages[0], *pages[1])]
 
     at_once = results()
