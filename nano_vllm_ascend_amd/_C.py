@@ -779,7 +779,7 @@ def qk_norm_rope_fp4(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_weight
     status = lib.nvamd_qk_norm_rope_fp4(
         qo_ptr, qo_stride, ko_ptr, ko_stride, q_ptr, q_stride, k_ptr, k_stride, v.data_ptr(), v_stride,
         q_weight.data_ptr(), k_weight.data_ptr(), positions.data_ptr(), cos_sin.data_ptr(), cos_sin.shape[0], *pages, nb,
-        bs, slots, t, hq, hkv, d, eps,
+        bs, slots, t, hq, hkv, d, float(eps),
         _stream_of(device, q, k, v, q_out, q if k_out is None else k_out, q_weight, k_weight, positions, cos_sin,
                    slot_mapping))
     if status:
@@ -841,7 +841,7 @@ def paged_decode_fp4(out: torch.Tensor | None, q: torch.Tensor, key_pages: Fp4Pa
     _fp4_decode_args(block_tables, context_lens, workspace, b)
     if _range_checks and _checking():
         check_paged_context(block_tables, context_lens, args[8], args[9], int(max_context_len))
-    status = lib.nvamd_paged_decode_fp4(*args, context_lens.data_ptr(), b, *heads, scale, max_context_len,
+    status = lib.nvamd_paged_decode_fp4(*args, context_lens.data_ptr(), b, *heads, float(scale), int(max_context_len),
                                         workspace.data_ptr(), workspace.nbytes,
                                         _stream_of(device, q, out, block_tables, context_lens, workspace))
     if status:
@@ -876,8 +876,9 @@ def paged_decode_fused_fp4(out: torch.Tensor | None, q: torch.Tensor, k: torch.T
         check_paged_context(block_tables, context_lens, nb, bs, int(max_context_len))
     status = lib.nvamd_paged_decode_fused_fp4(
         *args[:4], k.data_ptr(), k_stride, v.data_ptr(), v_stride, q_weight.data_ptr(), k_weight.data_ptr(),
-        positions.data_ptr(), cos_sin.data_ptr(), cos_sin.shape[0], eps, *args[4:10], slots, *args[10:],
-        context_lens.data_ptr(), b, hq, hkv, d, scale, max_context_len, workspace.data_ptr(), workspace.nbytes,
+        positions.data_ptr(), cos_sin.data_ptr(), cos_sin.shape[0], float(eps), *args[4:10], slots,
+        *args[10:], context_lens.data_ptr(), b, hq, hkv, d, float(scale), int(max_context_len), workspace.data_ptr(),
+        workspace.nbytes,
         _stream_of(device, q, k, v, out, q_weight, k_weight, positions, cos_sin, slot_mapping, block_tables,
                    context_lens, workspace))
     if status:
@@ -903,10 +904,11 @@ def paged_prefill_fp4(out: torch.Tensor, q: torch.Tensor, key_pages: Fp4Pages, v
     if _range_checks and _checking():
         check_paged_context(block_tables[:n], kv_lens[:n], args[8], args[9])
     stream = _stream_of(device, q, out, block_tables, cu_seqlens_q, kv_lens)
+    max_q_len = int(max_q_len)
     need = lib.nvamd_paged_prefill_fp4_workspace_size(n, max_q_len, heads[0], heads[1], args[9], args[12])
-    space = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None  # until the stream has passed the call
+    space = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None  # freed behind the call
     status = lib.nvamd_paged_prefill_fp4(*args, cu_seqlens_q.data_ptr(), kv_lens.data_ptr(), n, q.shape[0], max_q_len,
-                                         *heads, scale, space.data_ptr() if need else None, need, stream)
+                                         *heads, float(scale), space.data_ptr() if need else None, need, stream)
     if status:
         _check(status, "nvamd_paged_prefill_fp4")
     return out

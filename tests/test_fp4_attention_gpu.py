@@ -287,6 +287,25 @@ def test_decode_nan_reaches_only_its_sequence_and_dims(device):
     assert nan[1].all() and not nan[2].any()
 
 
+def test_a_nan_of_a_query_stays_in_its_row(device):
+    batch = Batch(device, [150, 400], 4, 1, 16, seed=27)
+    q = batch.queries(2)
+    clean = batch.decode(q)
+    q[1, 2, 77] = math.nan
+    got = batch.decode(q)
+    assert got[1, 2].isnan().all() and torch.equal(got[0], clean[0]) and torch.equal(got[1, :2], clean[1, :2])
+    assert torch.equal(got[1, 3], clean[1, 3])
+    q = batch.queries(200)
+    for bound in (None, "strips", 60_000):
+        clean = batch.prefill(q, [100, 100], max_q=bound)
+        bad = q.clone()
+        bad[130, 1, 3] = math.inf
+        got = batch.prefill(bad, [100, 100], max_q=bound)
+        assert got[130, 1].isnan().all()
+        got[130, 1] = clean[130, 1]
+        assert torch.equal(got, clean)
+
+
 def test_decode_views_and_rows_behind_the_batch(device):
     batch = Batch(device, [40, 500], 6, 2, 16, seed=8, extra_width=3)
     fused = torch.zeros(2, 10, 128, dtype=torch.bfloat16)
