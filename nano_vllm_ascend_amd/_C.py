@@ -601,9 +601,6 @@ def paged_prefill(out: torch.Tensor, q: torch.Tensor, key_cache: torch.Tensor, v
 FP4_ROW_BYTES, FP4_ROW_SCALES = 64, 4  # of a head vector
 
 
-# The functions below hand a call to csrc/calls.cpp first, which makes it if every argument is plainly right.  Else, and
-# with range checks on, the checks here name what is wrong, or make the call.
-
 
 class Fp4Pages(NamedTuple):
     """The keys or the values of one layer in 4 bits: ``codes`` uint8 [blocks, kv heads, block_size, 64] and ``scales``
@@ -677,7 +674,8 @@ def _page_slots(slot_mapping: torch.Tensor, rows: int, num_slots: int) -> int:
 
 
 def _made(answer, name: str) -> bool:
-    """Whether calls.cpp has made the call; raises for what the library answered."""
+    """Whether csrc/calls.cpp has made the call, as it does if every argument is plainly right; raises for what the library
+    answered.  If not, and with range checks on, the checks of the functions below name what is wrong, or they call."""
     if answer is None:
         return False
     if type(answer) is int:
