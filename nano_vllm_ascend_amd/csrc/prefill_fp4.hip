@@ -247,16 +247,19 @@ prefill_fp4_kernel(PrefillFp4Args a) {
     vs = *reinterpret_cast<const u32x2 *>(a.cache.v_scales + t * kFp4TileScales + 16 * (lane >> 4) + 8 * (w & 1));
   };
   auto expand = [&](int t, Stage &st) {
+    const int left = kv_len - t * kBK - 8 * w;  // of the wave's 8 tokens
+    if (__builtin_expect(left < 8, 0)) {  // stale rows past the keys: under some scales a code is past bf16, and a weight
+      vs[0] = keep_bytes(vs[0], left);    // of zero does not cancel it
+      vs[1] = keep_bytes(vs[1], left - 4);
+    }
     const u32 bad0 = nan_bytes(vs[0]), bad1 = nan_bytes(vs[1]);
     u32 seen0 = 0, seen1 = 0;
     if (__builtin_expect(__builtin_amdgcn_ballot_w64((bad0 | bad1) != 0) != 0, 0)) {
       vs[0] = without(vs[0], bad0);
       vs[1] = without(vs[1], bad1);
-      const int left = kv_len - t * kBK - 8 * w;  // of the wave's 8 tokens
       u32 bits = 0;
 #pragma unroll
       for (int i = 0; i < 4; ++i) bits |= ((bad0 >> (8 * i + 7)) & 1) << i | ((bad1 >> (8 * i + 7)) & 1) << (4 + i);
-      bits &= left >= 8 ? 0xffu : (1u << max(left, 0)) - 1u;
       // blocks 0, 1 and 2, 3 in two words of 16 bits each
       seen0 = (u32)__builtin_amdgcn_readlane((int)bits, 0) | (u32)__builtin_amdgcn_readlane((int)bits, 16) << 16;
       seen1 = (u32)__builtin_amdgcn_readlane((int)bits, 32) | (u32)__builtin_amdgcn_readlane((int)bits, 48) << 16;

@@ -590,6 +590,35 @@ def test_prefill_replays_from_a_graph(device):
         assert torch.equal(got, call(torch.empty_like(q)))
 
 
+# -------------------------------------------------------------------------------------------- bytes that nobody wrote
+def with_stale_scales(batch, byte):
+    """The batch's rows in pages whose other scale bytes are all `byte`, over random codes."""
+    k, v = fp4_ref.read(batch.pages, torch.cat(batch.slots))
+    for p in batch.pages[1::2]:
+        p.fill_(byte)
+    fp4_ref.write(batch.pages, k.bfloat16(), v.bfloat16(), torch.cat(batch.slots))
+    batch.upload()
+
+
+@BOUNDS
+@pytest.mark.parametrize("byte", [0, 201, 252, 253, 254, 255])
+def test_prefill_reads_no_value_past_the_keys(device, byte, bound):
+    """Scales that the writer never makes (under 253 and 254 a code is past bf16): a weight of zero does not cancel them."""
+    q_lens, cached = [1, 40, 130, 20], [200, 17, 1, 0]
+    batch = Batch(device, [a + b for a, b in zip(q_lens, cached)], 4, 2, 32, seed=28)
+    with_stale_scales(batch, byte)
+    q = batch.queries(sum(q_lens))
+    check_prefill(batch, q, q_lens, batch.prefill(q, q_lens, max_q=bound))
+
+
+@pytest.mark.parametrize("byte", [0, 201, 252, 253, 254, 255])
+def test_decode_reads_no_value_past_the_context(device, byte):
+    batch = Batch(device, [1, 40, 131, 530, 0, 65], 4, 2, 32, seed=29)
+    with_stale_scales(batch, byte)
+    q = batch.queries(6)
+    check_decode(batch, q, batch.decode(q))
+
+
 # -------------------------------------------------------------------------------------------- a whole decode step
 def step_of(batch, seed, slots=None):
     """Projected rows of a new token for each sequence of the batch, whose last position is the token's."""
