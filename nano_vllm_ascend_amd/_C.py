@@ -807,6 +807,8 @@ def _fp4_attention_args(out, q, key_pages, value_pages, block_tables, seqs: int)
     width = tables[1]
     if bt_stride[1] != 1 and width > 1:
         raise ValueError("block_tables rows must be dense")
+    if tables[0] > 1 and bt_stride[0] < width:
+        raise ValueError(f"rows of block_tables overlap: {tuple(tables)} with a row stride of {bt_stride[0]}")
     least = hq * d  # a single row's stride says nothing
     return (out.data_ptr(), out_stride[0] if t > 1 else max(out_stride[0], least), q.data_ptr(),
             q_stride[0] if t > 1 else max(q_stride[0], least), *pages, nb, bs, block_tables.data_ptr(),

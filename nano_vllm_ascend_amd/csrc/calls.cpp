@@ -105,6 +105,8 @@ Table table_of(PyObject *o, int &device, int64_t least, bool exact) {
   const at::Tensor &t = tensor(o, device);
   need(t.scalar_type() == at::kInt && t.dim() == 2 && (exact ? t.size(0) == least : t.size(0) >= least));
   need(t.size(1) > 0 && (t.stride(1) == 1 || t.size(1) == 1));
+  need(t.size(0) <= 1 || t.stride(0) >= t.size(1));
+  // a single row's stride says nothing
   return {t.data_ptr<int32_t>(), narrow(t.stride(0) > t.size(1) ? t.stride(0) : t.size(1)), narrow(t.size(1))};
 }
 

@@ -739,6 +739,33 @@ def test_what_the_library_refuses_raises(device):
         _C.kv_cache_write_fp4(q[:, :1].cpu(), q[:, :1].cpu(), batch.keys, batch.values, torch.arange(1, device=device))
 
 
+def test_block_tables_whose_rows_overlap_are_refused_on_either_route(device):
+    batch = Batch(device, [40, 33, 20], 4, 2, 16, seed=30)
+    q, step = batch.queries(3).to(device), step_of(batch, 31)
+    lens = torch.tensor(batch.lens, dtype=torch.int32, device=device)
+    cu = torch.arange(4, dtype=torch.int32, device=device)
+    space = _C.alloc_paged_decode_workspace(3, 4, 2, 64, device)
+    pages = batch.keys, batch.values
+    shared = batch.tables[:1].to(device).expand(3, -1)
+    calls = {
+        "decode": (_C.paged_decode_fp4, (None, q, *pages, shared, lens, SCALE, 64, space)),
+        "decode_fused": (_C.paged_decode_fused_fp4, (None, *step, shared, lens, SCALE, 64, space)),
+        "prefill": (_C.paged_prefill_fp4, (torch.empty_like(q), q, *pages, shared, cu, lens, 1, SCALE)),
+    }
+    for name, (call, args) in calls.items():
+        assert getattr(_C._calls, name)(*args) is None  # left to the checks, which name what is wrong
+        for checks in (False, True):
+            before = _C.set_range_checks(checks)
+            try:
+                with pytest.raises(ValueError, match="block_tables overlap"):
+                    call(*args)
+            finally:
+                _C.set_range_checks(before)
+    whole = _C.paged_decode_fp4(None, q, *pages, shared.contiguous(), lens, SCALE, 64, space)
+    one = batch.tables[0].to(device).expand(1, -1)  # a single row, whatever its stride
+    assert torch.equal(_C.paged_decode_fp4(None, q[:1], *pages, one, lens[:1], SCALE, 64, space), whole[:1])
+
+
 # -------------------------------------------------------------------------------------------- drawn calls
 HEADS = [(1, 1), (16, 8), (14, 2), (12, 4), (40, 8), (32, 4), (7, 7), (33, 1)]
 

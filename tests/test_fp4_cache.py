@@ -292,3 +292,33 @@ def test_attention_refuses():
                         ("block_tables", dict(bt=bt[:1])), ("on the GPU", {})):
         with pytest.raises(ValueError, match=match):
             prefill(**over)
+
+
+def test_block_tables_whose_rows_overlap_are_refused():
+    """One table for several sequences by a stride of 0, or windows of one list: a row at the table's width from the one
+    before would lie outside its memory."""
+    q, kv, w = heads(4, 16), heads(4, 8), torch.ones(128, dtype=torch.bfloat16)
+    lens, pos, ws = torch.ones(4, dtype=torch.int32), torch.arange(4), torch.zeros(64)
+    cu = torch.arange(5, dtype=torch.int32)
+    one = torch.zeros(1, 3, dtype=torch.int32)
+
+    def decode(bt, n=4):
+        _C.paged_decode_fp4(None, q[:n], pages(), pages(), bt, lens[:n], 0.1, 48, ws)
+
+    def fused(bt, n=4):
+        _C.paged_decode_fused_fp4(None, q[:n], kv[:n], kv[:n], w, w, pos[:n], torch.zeros(64, 128), 1e-6, pages(), pages(),
+                                  pos[:n], bt, lens[:n], 0.1, 48, ws)
+
+    def prefill(bt, n=4):
+        _C.paged_prefill_fp4(q[:n], q[:n], pages(), pages(), bt, cu[:n + 1], lens, 1, 0.1)
+
+    for call in (decode, fused, prefill):
+        for bt in (one.expand(4, 3), torch.zeros(6, dtype=torch.int32).as_strided((4, 3), (1, 1)),
+                   torch.zeros(9, dtype=torch.int32).as_strided((4, 3), (2, 1))):
+            with pytest.raises(ValueError, match="block_tables overlap"):
+                call(bt)
+        for bt in (one, one[0].expand(1, 3)):  # a single row's stride says nothing
+            with pytest.raises(ValueError, match="on the GPU"):
+                call(bt, 1)
+        with pytest.raises(ValueError, match="on the GPU"):
+            call(torch.zeros(12, dtype=torch.int32).as_strided((4, 3), (3, 1)))
