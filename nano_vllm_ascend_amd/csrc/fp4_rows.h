@@ -95,7 +95,7 @@ __device__ __forceinline__ double dpp_sum8(double v) {
 
 // A 32-bit value that rounds to bf16 as x does.  A plain cast rounds too, and may land on a border of bf16 that x is
 // only close to; here all but the top 20 bits of the fraction are cut off, and the last of these is set if any of the
-// rest was.
+// rest was.  (From 2^-129 on; below that the cast rounds at 2^-149, 2^-16 of bf16's step there.)
 __device__ __forceinline__ float bf16_bound(double x) {
   const uint64_t b = __builtin_bit_cast(uint64_t, x);
   const uint64_t top = (uint64_t)((u32)(b >> 32) | ((u32)b != 0u ? 1u : 0u)) << 32;
@@ -122,8 +122,8 @@ __device__ __forceinline__ double norm_factor(double squares, double eps) {
 // y = x * rsqrt(mean(x^2) + eps) * w, then the rotation out[d] = y[d] cos[d] - y[d+64] sin[d], out[d+64] = y[d+64]
 // cos[d] + y[d] sin[d], in 64 bits with one rounding to bf16 at the end.  A 4-bit code's step is a
 // third to a half of the value, so a key that 32-bit arithmetic puts on the other side of a rounding border is that far
-// off; in 64 bits the code is that of the exact value.  x w is a product of bf16 numbers, exact in 32 bits, and the
-// reciprocal root comes last: one multiplication for each result.
+// off; in 64 bits the code is that of the exact value.  x w is exact in 64 bits (in 32 its bits would fit, its exponent not
+// always), and the reciprocal root comes last: one multiplication for each result.
 __device__ __forceinline__ void norm_rope_f64(u32x4 &lo, u32x4 &hi, const u32x4 w_lo, const u32x4 w_hi,
                                               const float (&cs)[8], const float (&sn)[8], double rstd) {
 #pragma unroll
@@ -131,8 +131,9 @@ __device__ __forceinline__ void norm_rope_f64(u32x4 &lo, u32x4 &hi, const u32x4 
     float r_lo[2], r_hi[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const double y_lo = i ? bf16_hi(lo[e]) * bf16_hi(w_lo[e]) : bf16_lo(lo[e]) * bf16_lo(w_lo[e]);
-      const double y_hi = i ? bf16_hi(hi[e]) * bf16_hi(w_hi[e]) : bf16_lo(hi[e]) * bf16_lo(w_hi[e]);
+      const double x_lo = i ? bf16_hi(lo[e]) : bf16_lo(lo[e]), x_hi = i ? bf16_hi(hi[e]) : bf16_lo(hi[e]);
+      const double y_lo = x_lo * (i ? bf16_hi(w_lo[e]) : bf16_lo(w_lo[e]));
+      const double y_hi = x_hi * (i ? bf16_hi(w_hi[e]) : bf16_lo(w_hi[e]));
       const double c = cs[2 * e + i], s = sn[2 * e + i];
       r_lo[i] = bf16_bound((y_lo * c - y_hi * s) * rstd);
       r_hi[i] = bf16_bound((y_hi * c + y_lo * s) * rstd);

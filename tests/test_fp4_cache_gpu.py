@@ -200,6 +200,37 @@ def test_norm_rope_stores_the_code_of_the_exact_key(device, t, hq, hkv, bs, orde
     assert _C.index_errors() == 0
 
 
+def spread_out(gen, *shape, low, high):
+    """Normal numbers times powers of two of exponents low .. high, within bf16's largest."""
+    e = torch.randint(low, high + 1, shape[:-1] + (1,), generator=gen).double()
+    return (torch.randn(*shape, generator=gen).double() * torch.pow(2.0, e)).clamp(-3.38e38, 3.38e38).bfloat16()
+
+
+@pytest.mark.parametrize("low, high, weight_low, weight_high, eps", [
+    (118, 126, 8, 8, 1e-6),         # x w is past 32 bits' largest, the normed value is not
+    (-120, 126, -60, 60, 1e-6),
+    (-104, -90, -50, -36, 2e-38),   # x w is below their least normal one
+    (-133, 126, -100, 100, 2e-38),  # results past bf16's largest, and below its least, among them
+])
+def test_norm_rope_over_the_whole_range_of_bf16(device, low, high, weight_low, weight_high, eps):
+    t, hq, hkv, bs, table = 200, 4, 2, 32, table_of(4096)
+    gen = torch.Generator().manual_seed(high - low)
+    qkv = spread_out(gen, t, hq + 2 * hkv, 128, low=low, high=high)
+    qw, kw = (spread_out(gen, 128, 1, low=weight_low, high=weight_high)[:, 0].contiguous() for _ in range(2))
+    pos, slots = torch.randint(0, 4096, (t,), generator=gen), some_slots(t, 8, bs, "odd", 1)
+    q, k, v = qkv.split([hq, hkv, hkv], 1)
+    want_q, want_k = (fp4_ref.to_bf16(fp4_ref.norm_rope(x, w, pos, table, eps)) for x, w in ((q, qw), (k, kw)))
+    pages = filled(8, hkv, bs, 2)
+    got = on(device, pages)
+    fp4_ref.write(pages, want_k, v, slots)
+    dq, dk, dv = qkv.to(device).split([hq, hkv, hkv], 1)
+    k_out = torch.empty(t, hkv, 128, dtype=torch.bfloat16, device=device)
+    q_out = _C.qk_norm_rope_fp4(dq, dk, dv, qw.to(device), kw.to(device), pos.to(device), table.to(device), eps, *got,
+                                slots.to(device), k_out=k_out)
+    assert torch.equal(q_out.cpu(), want_q) and torch.equal(k_out.cpu(), want_k)
+    same(got, pages)
+
+
 def test_norm_rope_in_place_through_the_layer_equals_the_two_steps(device):
     """qk_norm_rope with a 4-bit cache rewrites q and k, as with a bf16 one; what it stored is what a write of that k stores."""
     t, hq, hkv = 50, 16, 8
