@@ -12,6 +12,7 @@
 #include <ATen/ops/empty.h>
 #include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPStream.h>
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include "nvamd.h"
@@ -308,8 +309,8 @@ PyObject *entry(PyObject *, PyObject *const *args, Py_ssize_t n) {
     return F(args);
   } catch (const Irregular &) {
     Py_RETURN_NONE;
-  } catch (const std::exception &e) {  // of an allocation or a device query
-    if (!PyErr_Occurred()) PyErr_SetString(PyExc_RuntimeError, e.what());
+  } catch (const std::exception &) {  // of an allocation or a device query: raised as torch raises it
+    torch::translate_exception_to_python(std::current_exception());
     return nullptr;
   }
 }

@@ -301,3 +301,20 @@ def test_calls_go_to_the_current_stream_and_replay_from_a_graph(device):
         assert torch.equal(replayed[1], k_back) and torch.equal(replayed[2], v_back)
         want_k, want_v = fp4_ref.read(tuple(p.cpu() for p in (*want[0], *want[1])), slots.cpu())
         assert torch.equal(k_back.cpu().double(), want_k) and torch.equal(v_back.cpu().double(), want_v)
+
+
+@pytest.mark.parametrize("checks", [False, True])
+def test_no_memory_raises_as_torch_does(device, checks):
+    """Results of 2 x 4 GiB under a limit on torch's allocator of about 1 GiB: the allocation fails, nothing is launched."""
+    got = on(device, filled(2, 8, 16, 0))
+    slots = torch.zeros(1 << 21, dtype=torch.int64, device=device)
+    torch.cuda.empty_cache()
+    total = torch.cuda.get_device_properties(device).total_memory
+    before = _C.set_range_checks(checks)
+    torch.cuda.set_per_process_memory_fraction((torch.cuda.memory_reserved() + (1 << 30)) / total)
+    try:
+        with pytest.raises(torch.OutOfMemoryError):
+            _C.kv_cache_read_fp4(*got, slots)
+    finally:
+        torch.cuda.set_per_process_memory_fraction(1.0)
+        _C.set_range_checks(before)
