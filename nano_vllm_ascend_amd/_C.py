@@ -9,7 +9,9 @@ passes has run the HIP kernels.
 from __future__ import annotations
 
 import ctypes
+import importlib
 import os
+import warnings
 from pathlib import Path
 from typing import NamedTuple
 
@@ -154,18 +156,24 @@ def load() -> ctypes.CDLL:
     return lib
 
 
-_calls = None  # csrc/calls.cpp: eager calls of the 4-bit cache, checked and made in one step
+_calls = None  # csrc/calls.cpp: eager calls of the 4-bit cache, checked and made in one step; None: not usable here
 
 
 def _bind_calls(lib: ctypes.CDLL) -> None:
+    """The library needs nothing of torch, the extension is tied to the torch that it was built with: without it the calls
+    go through the checks in this file, with the same results."""
     global _calls
-    try:
-        from . import _calls as calls
-    except ImportError as e:
-        raise RuntimeError("nano_vllm_ascend_amd/_calls.so is missing: build it with "
-                           "`python -m nano_vllm_ascend_amd.build` (or __graft_entry__.build())") from e
     names = ("kv_cache_write_fp4", "kv_cache_read_fp4", "qk_norm_rope_fp4", "paged_decode_fp4",
              "paged_decode_fused_fp4", "paged_prefill_fp4", "paged_prefill_fp4_workspace_size")
+    try:
+        calls = importlib.import_module("._calls", __package__)
+        if calls.ABI_VERSION != lib.nvamd_version():
+            raise ImportError(f"built for version {calls.ABI_VERSION} of the C ABI, the library has {lib.nvamd_version()}")
+    except ImportError as e:
+        _calls = None
+        warnings.warn(f"eager calls of the 4-bit KV cache take some 5 us more each: {LIB_PATH.with_name('_calls.so')} cannot "
+                      f"be used ({e}); `python -m nano_vllm_ascend_amd.build` builds it", RuntimeWarning, stacklevel=3)
+        return
     calls.bind(Fp4Pages, *(ctypes.cast(getattr(lib, f"nvamd_{n}"), ctypes.c_void_p).value for n in names))
     _calls = calls
 
@@ -688,8 +696,8 @@ def kv_cache_write_fp4(key_states: torch.Tensor, value_states: torch.Tensor, key
     """Rows [T, Hkv, 128] of bf16 keys and values, quantised into the pages at their slots (-1: padding, skipped; no slot
     twice in a call)."""
     lib = _lib or load()
-    if not _range_checks and _made(_calls.write(key_states, value_states, key_pages, value_pages, slot_mapping),
-                                   "nvamd_kv_cache_write_fp4"):
+    if _calls and not _range_checks and _made(
+            _calls.write(key_states, value_states, key_pages, value_pages, slot_mapping), "nvamd_kv_cache_write_fp4"):
         return
     nb, bs, hkv, pages, device = _fp4_pages(key_pages, value_pages)
     t, d = key_states.shape[0], 2 * FP4_ROW_BYTES
@@ -707,7 +715,7 @@ def kv_cache_read_fp4(key_pages: Fp4Pages, value_pages: Fp4Pages, slot_mapping: 
                       v_out: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """The bf16 keys and values [T, Hkv, 128] that the pages hold at the slots (zeros for -1)."""
     lib = _lib or load()
-    if not _range_checks and k_out is None and v_out is None:
+    if _calls and not _range_checks and k_out is None and v_out is None:
         rows = _calls.read(key_pages, value_pages, slot_mapping)
         if _made(rows, "nvamd_kv_cache_read_fp4"):
             return rows
@@ -750,7 +758,7 @@ def qk_norm_rope_fp4(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_weight
     Returns the rotated q: ``q_out``, which may be q itself, or a new tensor.  The rotated k is written
     only to the pages unless ``k_out`` (which may be k itself) asks for it.  64-bit arithmetic, one rounding to bf16."""
     lib = _lib or load()
-    if not _range_checks:
+    if _calls and not _range_checks:
         rotated = _calls.rope(q, k, v, q_weight, k_weight, positions, cos_sin, eps, key_pages, value_pages, slot_mapping,
                               q_out, k_out)
         if _made(rotated, "nvamd_qk_norm_rope_fp4"):
@@ -830,7 +838,7 @@ def paged_decode_fp4(out: torch.Tensor | None, q: torch.Tensor, key_pages: Fp4Pa
     """``paged_decode`` over pages of 4 bits; the workspace is the same (``alloc_paged_decode_workspace``).  Without
     ``out`` the result is a new tensor."""
     lib = _lib or load()
-    if not _range_checks:
+    if _calls and not _range_checks:
         made = _calls.decode(out, q, key_pages, value_pages, block_tables, context_lens, scale, max_context_len, workspace)
         if _made(made, "nvamd_paged_decode_fp4"):
             return made
@@ -857,7 +865,7 @@ def paged_decode_fused_fp4(out: torch.Tensor | None, q: torch.Tensor, k: torch.T
     """``qk_norm_rope_fp4`` and ``paged_decode_fp4`` in one launch, with the same bits: the step's k and v go to the slots
     of their sequences' last positions (-1: not stored), q, k and v stay as they are."""
     lib = _lib or load()
-    if not _range_checks:
+    if _calls and not _range_checks:
         made = _calls.decode_fused(out, q, k, v, q_weight, k_weight, positions, cos_sin, eps, key_pages, value_pages,
                                    slot_mapping, block_tables, context_lens, scale, max_context_len, workspace)
         if _made(made, "nvamd_paged_decode_fused_fp4"):
@@ -891,7 +899,7 @@ def paged_prefill_fp4(out: torch.Tensor, q: torch.Tensor, key_pages: Fp4Pages, v
                       scale: float) -> torch.Tensor:
     """``paged_prefill`` over pages of 4 bits: queries are the last q_len of kv_len positions, all keys in the cache."""
     lib = _lib or load()
-    if not _range_checks and _made(
+    if _calls and not _range_checks and _made(
             _calls.prefill(out, q, key_pages, value_pages, block_tables, cu_seqlens_q, kv_lens, max_q_len, scale),
             "nvamd_paged_prefill_fp4"):
         return out

@@ -5,7 +5,9 @@ hipcc for gfx950 and links them into ``nano_vllm_ascend_amd/libnvamd.so``.
 The library exports the C ABI declared in ``include/nvamd.h`` and nothing that
 depends on torch, so the same file serves ctypes, a C harness or any FFI.
 ``csrc/calls.cpp``, host code that makes some of its calls for Python, becomes the
-extension module ``nano_vllm_ascend_amd/_calls.so``.
+extension module ``nano_vllm_ascend_amd/_calls.so``, which needs the headers of Python
+and of the torch that it runs with; where it cannot be built the library is complete
+without it, and the package makes those calls from Python.
 """
 from __future__ import annotations
 
@@ -15,6 +17,7 @@ import shutil
 import subprocess
 import sys
 import sysconfig
+import warnings
 from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
@@ -109,13 +112,15 @@ def build(verbose: bool = True) -> Path:
     with ThreadPoolExecutor(max_workers=workers) as pool:
         calls = pool.submit(_build_calls)
         objs = list(pool.map(_compile, srcs))
-        calls.result()
     tmp = LIB_PATH.with_suffix(".so.tmp")
     cmd = [HIPCC, f"--offload-arch={ARCH}", "-shared", "-fPIC", *map(str, objs), "-o", str(tmp)]
     proc = subprocess.run(cmd, capture_output=True, text=True)
     if proc.returncode != 0:
         raise RuntimeError(f"link failed:\n{proc.stdout}\n{proc.stderr}")
     os.replace(tmp, LIB_PATH)
+    if (problem := calls.exception()) is not None:
+        CALLS_PATH.unlink(missing_ok=True)  # one of other sources would not fit the library
+        warnings.warn(f"{CALLS_PATH.name} was not built, {LIB_PATH.name} was: {problem}", RuntimeWarning)
     if verbose:
         print(f"[nvamd] built {LIB_PATH} from {len(srcs)} sources for {ARCH}")
     return LIB_PATH

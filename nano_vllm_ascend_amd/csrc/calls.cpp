@@ -346,4 +346,8 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_calls", nullptr, -1, methods, nul
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__calls() { return PyModule_Create(&module); }
+PyMODINIT_FUNC PyInit__calls() {
+  PyObject *m = PyModule_Create(&module);
+  if (m != nullptr && PyModule_AddIntConstant(m, "ABI_VERSION", NVAMD_ABI_VERSION) < 0) Py_CLEAR(m);
+  return m;
+}

@@ -739,6 +739,30 @@ def test_what_the_library_refuses_raises(device):
         _C.kv_cache_write_fp4(q[:, :1].cpu(), q[:, :1].cpu(), batch.keys, batch.values, torch.arange(1, device=device))
 
 
+def test_calls_without_the_extension(device, monkeypatch):
+    """Where csrc/calls.cpp cannot be used the same calls are made from Python."""
+    batch = Batch(device, [300, 20], 4, 2, 16, seed=32)
+    q = batch.queries(2)
+    step = step_of(batch, 33)
+    space = _C.alloc_paged_decode_workspace(2, 4, 2, 512, device)
+    slots = torch.stack([s[-1] for s in batch.slots]).to(device)
+
+    def results():
+        batch.upload()
+        args = (*step[:8], batch.keys, batch.values, slots)
+        got = [batch.decode(q, bound=512), batch.prefill(q, [1, 1]), attend(batch, None, 512, space, fused=args)]
+        batch.upload()
+        args = (*step[:8], batch.keys, batch.values, slots)
+        got.append(_C.qk_norm_rope_fp4(*args))
+        got += _C.kv_cache_read_fp4(batch.keys, batch.values, slots)
+        _C.kv_cache_write_fp4(step[1], step[2], batch.keys, batch.values, slots)
+        return got + in_pages(batch)
+
+    want = results()
+    monkeypatch.setattr(_C, "_calls", None)
+    assert all(torch.equal(a, b) for a, b in zip(results(), want))
+
+
 def test_block_tables_whose_rows_overlap_are_refused_on_either_route(device):
     batch = Batch(device, [40, 33, 20], 4, 2, 16, seed=30)
     q, step = batch.queries(3).to(device), step_of(batch, 31)

@@ -2,12 +2,16 @@
 of the C ABI and the refusals of the Python entry points."""
 from __future__ import annotations
 
+import importlib
 import math
+import subprocess
+import sys
+import warnings
 
 import pytest
 import torch
 
-from nano_vllm_ascend_amd import _C
+from nano_vllm_ascend_amd import _C, build
 from nano_vllm_ascend_amd.paged_kv_cache import Fp4PagedKVCache
 from oracle import fp4_ref
 
@@ -322,3 +326,60 @@ def test_block_tables_whose_rows_overlap_are_refused():
                 call(bt, 1)
         with pytest.raises(ValueError, match="on the GPU"):
             call(torch.zeros(12, dtype=torch.int32).as_strided((4, 3), (3, 1)))
+
+
+# -------------------------------------------------------------------------------------------- without csrc/calls.cpp
+CALLS = "nano_vllm_ascend_amd._calls"
+
+
+@pytest.fixture
+def unloaded(monkeypatch):
+    monkeypatch.setattr(_C, "_lib", None)
+    monkeypatch.setattr(_C, "_calls", None)
+
+
+def test_the_library_loads_without_the_extension(unloaded, monkeypatch):
+    monkeypatch.setitem(sys.modules, CALLS, None)  # an import of it fails
+    with pytest.warns(RuntimeWarning, match="_calls.so cannot be used"):
+        _C.load()
+    assert _C._calls is None and _C.version() > 0 and _C.paged_decode_workspace_size(4, 16, 8, 1024) > 0
+    for call in (lambda: _C.kv_cache_write_fp4(heads(4, 8), heads(4, 8), pages(), pages(), torch.arange(4)),
+                 lambda: _C.kv_cache_read_fp4(pages(), pages(), torch.arange(4))):
+        with pytest.raises(ValueError, match="on the GPU"):
+            call()
+
+
+def test_an_extension_of_another_abi_is_not_used(unloaded, monkeypatch):
+    other = type(sys)(CALLS)
+    other.ABI_VERSION, other.bind = _C.load().nvamd_version() + 1, None
+    monkeypatch.setattr(_C, "_lib", None)
+    monkeypatch.setitem(sys.modules, CALLS, other)
+    with pytest.warns(RuntimeWarning, match="version .* of the C ABI"):
+        _C.load()
+    assert _C._calls is None
+
+
+def test_the_extension_is_used_where_it_is_built(unloaded):
+    with warnings.catch_warnings():
+        warnings.simplefilter("error")
+        _C.load()
+    assert _C._calls is importlib.import_module(CALLS)
+
+
+def test_the_library_is_built_without_the_extension(monkeypatch, tmp_path):
+    def no_torch():
+        raise ImportError("no module named torch")
+
+    def link(cmd, **_):
+        open(cmd[-1], "w").close()
+        return subprocess.CompletedProcess(cmd, 0, "", "")
+
+    stale = tmp_path / "_calls.so"
+    stale.touch()
+    for name, value in (("LIB_PATH", tmp_path / "libnvamd.so"), ("CALLS_PATH", stale), ("OBJ_DIR", tmp_path / "obj"),
+                        ("_compile", lambda src: tmp_path / src.name), ("_build_calls", no_torch)):
+        monkeypatch.setattr(build, name, value)
+    monkeypatch.setattr(build.subprocess, "run", link)
+    with pytest.warns(RuntimeWarning, match="no module named torch"):
+        build.build(verbose=False)
+    assert (tmp_path / "libnvamd.so").exists() and not stale.exists()
