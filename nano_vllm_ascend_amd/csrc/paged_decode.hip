@@ -47,21 +47,13 @@
 // The wave whose chunk holds the new token's row stores it before loading its chunk.
 #include <mutex>
 
-#include "common.h"
+#include "decode_workspace.h"
 
 namespace nvamd {
 namespace {
 
-constexpr int kPartFloats = 132;  // max, sum, 128 accumulators, 2 pad (16-byte rows)
-// Arrival counters live in a fixed-size region at the front of the workspace so
-// calls with different batch sizes or context bounds never place partial
-// results where another call expects a zero counter.
-constexpr int kCounterSlots = 16384;
-constexpr size_t kCounterBytes = kCounterSlots * sizeof(int);
 constexpr int kMaxGroups = 4096;  // workgroups of an MFMA launch; each takes every kMaxGroups-th item
 constexpr int kMaxDots = 32768;  // largest context bound of the dot-product kernel: 64 partitions of 512 tokens
-constexpr int kMaxContext = 131072;  // largest context bound of a call
-constexpr int kMinPart = 256;  // smallest partition of a split launch (sizes the workspace)
 
 struct DecodeArgs {
   u16 *out;
@@ -112,20 +104,6 @@ struct KVTile {
 };
 
 __device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
-
-// Inclusive prefix sum over the 64 lanes of a wave, in registers: a Hillis-Steele scan inside
-// each 16-lane row by DPP row shifts (lanes shifted in from outside the row read 0), then each
-// row adds the totals of the rows before it (lane 15 of each row, read into scalar registers).
-__device__ __forceinline__ int wave_incl_scan(int v, int lane) {
-  v += __builtin_amdgcn_mov_dpp(v, 0x111, 0xF, 0xF, true);  // row_shr:1
-  v += __builtin_amdgcn_mov_dpp(v, 0x112, 0xF, 0xF, true);  // row_shr:2
-  v += __builtin_amdgcn_mov_dpp(v, 0x114, 0xF, 0xF, true);  // row_shr:4
-  v += __builtin_amdgcn_mov_dpp(v, 0x118, 0xF, 0xF, true);  // row_shr:8
-  const int r0 = __builtin_amdgcn_readlane(v, 15), r1 = __builtin_amdgcn_readlane(v, 31);
-  const int r2 = __builtin_amdgcn_readlane(v, 47);
-  const int row = lane >> 4;
-  return v + (row >= 1 ? r0 : 0) + (row >= 2 ? r1 : 0) + (row >= 3 ? r2 : 0);
-}
 
 // 2 * GQA consecutive floats of a partial record through an agent-coherent buffer range
 // (write-through stores, loads that bypass the non-coherent caches): 8 bytes for one head, 16 for two.
@@ -647,6 +625,7 @@ paged_decode_kernel(DecodeArgs a) {
 template <int GQA, int NW, int CPW, bool WHOLE, bool FUSED>
 int launch(DecodeArgs a, int batch, hipStream_t stream) {
   constexpr int PART = NW * CPW * 64;
+  static_assert(WHOLE || PART >= kMinPart, "the workspace has records for these partitions");
   a.max_parts = ceil_div(a.max_ctx, PART);
   if (a.max_parts > 64) return NVAMD_EUNSUPPORTED;  // merge stage holds <= 64 partitions
   if (WHOLE && a.max_parts != 1) return NVAMD_EINVAL;
@@ -1242,6 +1221,7 @@ paged_decode_mfma_kernel(DecodeArgs a) {
 
 template <int GP, int NW, int CPW, bool WHOLE, bool FUSED>
 int launch_mfma(DecodeArgs a, int batch, hipStream_t stream) {
+  static_assert(WHOLE || NW * CPW * 64 >= kMinPart, "the workspace has records for these partitions");
   a.max_parts = ceil_div(a.max_ctx, NW * CPW * 64);
   if (WHOLE && a.max_parts != 1) return NVAMD_EINVAL;
   a.batch = batch;
@@ -1338,10 +1318,7 @@ using namespace nvamd;
 extern "C" size_t nvamd_paged_decode_workspace_size(int max_batch, int num_heads, int num_kv_heads,
                                                     int max_context_len) {
   if (max_batch <= 0 || num_kv_heads <= 0 || num_heads <= 0 || max_context_len <= 0) return 0;
-  const int gqa = num_heads / num_kv_heads;
-  const size_t parts = (size_t)ceil_div(max_context_len, kMinPart);
-  const size_t units = (size_t)max_batch * num_kv_heads;
-  return kCounterBytes + units * parts * gqa * kPartFloats * sizeof(float);
+  return decode_workspace_bytes(max_batch, num_heads, num_kv_heads, max_context_len);
 }
 
 namespace {

@@ -28,6 +28,7 @@
 // TB/s, part of it from the Infinity Cache; a large copy 5.0); 4 x U[8192, 40960], 91 MB, 21 us.  Below that by what
 // every call pays: some 2 us of launch, 1.3 to the first load (contexts, table, query) and 2 to 4 for the join: 32 x
 // U[256, 2304], 46 MB, 16 us, 4 x U[1, 512] 6.2.
+#include "decode_workspace.h"
 #include "fp4_attention.h"
 #include "fp4_rows.h"
 
@@ -36,14 +37,11 @@
 namespace nvamd {
 namespace {
 
-constexpr int kPartFloats = 132;  // a head's record: max, sum, 2 unused, 128 accumulators
-constexpr int kCounterSlots = 16384;
-constexpr size_t kCounterBytes = kCounterSlots * sizeof(int);
-constexpr int kMaxContext = 131072;  // largest context bound of a call
 constexpr int kWaves = 8;
 constexpr int kHalvesLog2 = 4, kHalves = 2 * kWaves;  // half-waves of a workgroup
 static_assert(kHalves == 1 << kHalvesLog2);
-constexpr int kMinPart = 64 * kWaves;  // tokens of the smallest partition: one step of each wave
+constexpr int kLeastPart = 64 * kWaves;  // tokens of the smallest partition: one step of each wave
+static_assert(kLeastPart >= kMinPart, "the workspace has records for these partitions");
 constexpr int kCus = 256;
 constexpr int kMaxHeads = 16;  // query heads of a kv head in one launch: the MFMA's columns
 
@@ -150,18 +148,6 @@ __device__ __forceinline__ void store_row(const Fp4Cache &cache, const StepArgs 
   cache.v_codes[at.tile * kFp4TileBytes + lane * kFp4Tile + at.t] = tile[lane * 8];
 }
 
-// Inclusive prefix sum over a wave (see paged_decode.hip).
-__device__ __forceinline__ int wave_scan(int v, int lane) {
-  v += __builtin_amdgcn_mov_dpp(v, 0x111, 0xF, 0xF, true);
-  v += __builtin_amdgcn_mov_dpp(v, 0x112, 0xF, 0xF, true);
-  v += __builtin_amdgcn_mov_dpp(v, 0x114, 0xF, 0xF, true);
-  v += __builtin_amdgcn_mov_dpp(v, 0x118, 0xF, 0xF, true);
-  const int r0 = __builtin_amdgcn_readlane(v, 15), r1 = __builtin_amdgcn_readlane(v, 31);
-  const int r2 = __builtin_amdgcn_readlane(v, 47);
-  const int row = lane >> 4;
-  return v + (row >= 1 ? r0 : 0) + (row >= 2 ? r1 : 0) + (row >= 3 ? r2 : 0);
-}
-
 // Cutting units of `tokens` tokens in all every `length` tokens ends in tokens / length + units / 2 partitions on
 // average, and in a whole unit more than the quotient each at most.  The length is chosen for this quotient (share):
 //   few units: partitions fill the card once, with one workgroup on each CU while that leaves two per unit, else two.
@@ -178,7 +164,7 @@ __host__ __device__ constexpr int partition_share(int units) {
 __device__ __forceinline__ int partition_tokens(u32 tokens, int units) {  // a multiple of 64
   const u32 share = (u32)partition_share(units);
   const u32 len = (tokens + share - 1) / share;
-  return max((int)((len + 63) & ~63u), kMinPart);
+  return max((int)((len + 63) & ~63u), kLeastPart);
 }
 __host__ __device__ constexpr int max_partitions(int units) { return partition_share(units) + units; }
 
@@ -215,7 +201,7 @@ paged_decode_fp4_kernel(DecodeFp4Args a, std::conditional_t<FUSED, StepArgs, Not
     if (__ballot(raw < 0 || raw > ctx_cap)) err_bits |= NVAMD_ERR_CONTEXT;
     const int ci = min(max(raw, 0), ctx_cap);
     if (b0 == 0) ctx0 = ci;
-    total += (u32)__builtin_amdgcn_readlane(wave_scan(bi < a.batch ? max(ci, 1) : 0, lane), 63);
+    total += (u32)__builtin_amdgcn_readlane(wave_incl_scan(bi < a.batch ? max(ci, 1) : 0, lane), 63);
   }
   const int part_tokens = partition_tokens(total * (u32)hkv, a.batch * hkv);
   const float per_part = 1.0f / (float)part_tokens;
@@ -226,7 +212,7 @@ paged_decode_fp4_kernel(DecodeFp4Args a, std::conditional_t<FUSED, StepArgs, Not
     int np = (int)((float)(ci + part_tokens - 1) * per_part);  // off by one at most: both are below 2^24
     np += np * part_tokens < ci ? 1 : (np - 1) * part_tokens >= ci ? -1 : 0;
     np = bi < a.batch ? max(np, 1) : 0;
-    const int incl = wave_scan(np, lane);
+    const int incl = wave_incl_scan(np, lane);
     const int sum = __builtin_amdgcn_readlane(incl, 63);
     if (item < (base + sum) * hkv) {
       const int sel = __ffsll((unsigned long long)__ballot((base + incl) * hkv > item)) - 1;
@@ -654,7 +640,7 @@ int fill_decode_args(DecodeFp4Args &a, void *out, int64_t out_stride, const void
       ((int64_t)bt_width << bs_log2) > 0x7fffffff || (((int64_t)num_blocks * num_kv_heads) << bs_log2) >> 4 > 0x7fffffff)
     return NVAMD_EUNSUPPORTED;
   if (!workspace ||
-      workspace_bytes < nvamd_paged_decode_workspace_size(batch, num_heads, num_kv_heads, max_context_len))
+      workspace_bytes < decode_workspace_bytes(batch, num_heads, num_kv_heads, max_context_len))
     return NVAMD_EWORKSPACE;
   if (!aligned16(workspace)) return NVAMD_EINVAL;
 
@@ -677,7 +663,7 @@ int fill_decode_args(DecodeFp4Args &a, void *out, int64_t out_stride, const void
   a.num_kv_heads = num_kv_heads;
   a.bs_log2 = bs_log2;
   a.max_ctx = max_context_len;
-  a.max_parts = ceil_div(max_context_len, kMinPart);
+  a.max_parts = ceil_div(max_context_len, kLeastPart);
   a.batch = batch;
   a.scale_log2e = scale * kLog2e;
   a.q_group = num_heads / num_kv_heads;

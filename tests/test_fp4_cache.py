@@ -152,6 +152,14 @@ def test_decode_argument_errors():
     assert call(ws_bytes=need - 1) == EWORKSPACE and call(ws=0) == EWORKSPACE and call(ws=A + 8) == EINVAL
 
 
+@pytest.mark.parametrize("batch, hq, hkv, bound", [(1, 1, 1, 1), (4, 16, 8, 512), (4, 16, 8, 513), (100, 40, 8, 40960),
+                                                   (7, 17, 1, 131072)])
+def test_the_shared_workspace_holds_the_partitions_of_4_bit_decode(batch, hq, hkv, bound):
+    """A counter for each of 16,384 units; records of 132 floats a head for partitions of 512 tokens or more."""
+    records = batch * hkv * -(-bound // 512) * (hq // hkv)
+    assert _C.paged_decode_workspace_size(batch, hq, hkv, bound) >= 4 * 16384 + 4 * 132 * records
+
+
 def test_fused_decode_argument_errors():
     lib = _C.load()
 
