@@ -83,23 +83,25 @@ class HipPagedAttention(nn.Module):
         self.num_key_value_heads = num_key_value_heads
         self.head_dim = head_dim
         self.scale = head_dim ** -0.5
-        self._workspace: torch.Tensor | None = None
-        self._ws_key = (0, 0)
+        self._workspaces: dict[torch.device, tuple[torch.Tensor, int, int]] = {}  # with the batch and bound they hold
         self._outgrown: list[torch.Tensor] = []
 
     def workspace(self, batch: int, max_context_len: int, device) -> torch.Tensor:
         """A zero-filled split-KV workspace large enough for (batch, max_context_len); grows on demand.  Calls that use
         it must not overlap: give those of other streams, and of graphs that run beside others, one of their own.
         One that was outgrown is kept, since a captured graph may still use it."""
-        b, c = self._ws_key
-        if self._workspace is None or batch > b or max_context_len > c or self._workspace.device != device:
-            if self._workspace is not None:  # powers of two from here on: few are outgrown
-                self._outgrown.append(self._workspace)
+        device = torch.device(device)
+        if device.type == "cuda" and device.index is None:
+            device = torch.device("cuda", torch.cuda.current_device())
+        space, b, c = self._workspaces.get(device, (None, 0, 0))
+        if space is None or batch > b or max_context_len > c:
+            if space is not None:  # powers of two from here on: few are outgrown
+                self._outgrown.append(space)
                 b, c = (max(old, 1 << (new - 1).bit_length()) for old, new in ((b, batch), (c, max_context_len)))
             b, c = max(batch, b), max(max_context_len, c)
-            self._workspace = _C.alloc_paged_decode_workspace(b, self.num_heads, self.num_key_value_heads, c, device)
-            self._ws_key = (b, c)
-        return self._workspace
+            space = _C.alloc_paged_decode_workspace(b, self.num_heads, self.num_key_value_heads, c, device)
+            self._workspaces[device] = space, b, c
+        return space
 
     def forward(self, q: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor,
                 block_tables: torch.Tensor, context_lens: torch.Tensor, max_context_len: int | None = None,

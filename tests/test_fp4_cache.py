@@ -391,3 +391,19 @@ def test_the_library_is_built_without_the_extension(monkeypatch, tmp_path):
     with pytest.warns(RuntimeWarning, match="no module named torch"):
         build.build(verbose=False)
     assert (tmp_path / "libnvamd.so").exists() and not stale.exists()
+
+
+def test_the_attention_layer_keeps_one_workspace_for_each_device():
+    """Calls that go to and fro between devices find the workspace that they left; only one that was outgrown is kept beside it."""
+    from nano_vllm_ascend_amd.layers import HipPagedAttention
+    layer = HipPagedAttention(4, 2, 128)
+    first = {d: layer.workspace(2, 600, torch.device(d)) for d in ("cpu", "meta")}
+    assert all(space.device.type == d for d, space in first.items())
+    for _ in range(3):
+        for d, space in first.items():
+            assert layer.workspace(1, 512, torch.device(d)) is space
+    assert layer._outgrown == []
+    grown = layer.workspace(3, 512, torch.device("cpu"))
+    assert grown is not first["cpu"] and len(layer._outgrown) == 1 and layer._outgrown[0] is first["cpu"]
+    assert layer.workspace(4, 600, torch.device("cpu")) is grown  # to a power of two
+    assert layer.workspace(2, 600, torch.device("meta")) is first["meta"]
