@@ -165,9 +165,6 @@ struct Stage {
 };
 constexpr int kRowPad = kHeadDim + 8;  // elements of a row in the output's turn: 16 bytes of padding spread the banks
 
-// WIDE: pages of 32 tokens or more, so that a tile's keys lie in one page and K loads from a scalar address (702 us,
-// 705 without, where the header counts 689; the strips gain nothing by it).
-template <bool WIDE>
 __global__ void __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(3)))
 prefill_fp4_kernel(PrefillFp4Args a) {
   constexpr int D = kHeadDim;
@@ -221,18 +218,9 @@ prefill_fp4_kernel(PrefillFp4Args a) {
   u32x4 kc[2];
   u32 ks[2];
   const u32 k_at = k_token * kFp4RowBytes + 16 * half, ks_at = fp4_key_scale_at(k_token, half);
-  const u32 second = n < 16 ? 0u : ~0u;  // mask: the lane's key is in the second 16-token tile
   auto load_k = [&](int t0, int t1) {
-    const u8 *kp, *sp;
-    if constexpr (WIDE) {
-      const u32 d = (u32)(t1 - t0);  // 1, or 0 past the keys
-      kp = a.cache.k_codes + (int64_t)t0 * kFp4TileBytes + (k_at + (second & (d * kFp4TileBytes)));
-      sp = a.cache.k_scales + (int64_t)t0 * kFp4TileScales + (ks_at + (second & (d * kFp4TileScales)));
-    } else {
-      const int64_t t = second ? t1 : t0;
-      kp = a.cache.k_codes + t * kFp4TileBytes + k_at;
-      sp = a.cache.k_scales + t * kFp4TileScales + ks_at;
-    }
+    const int64_t t = n < 16 ? t0 : t1;
+    const u8 *kp = a.cache.k_codes + t * kFp4TileBytes + k_at, *sp = a.cache.k_scales + t * kFp4TileScales + ks_at;
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
       kc[s] = *reinterpret_cast<const u32x4 *>(kp + 32 * s);
@@ -990,10 +978,8 @@ extern "C" int nvamd_paged_prefill_fp4(void *out, int64_t out_stride, const void
     hipLaunchKernelGGL(prefill_few_fp4_kernel, grid, dim3(kFewWaves * 64), 0, stream, a);
   else if (plan.rows == kStripRows)
     hipLaunchKernelGGL(prefill_strip_fp4_kernel, grid, dim3(kStripWaves * 64), 0, stream, a);
-  else if (bs_log2 >= 5)
-    hipLaunchKernelGGL(prefill_fp4_kernel<true>, grid, dim3(kWaves * 64), 0, stream, a);
   else
-    hipLaunchKernelGGL(prefill_fp4_kernel<false>, grid, dim3(kWaves * 64), 0, stream, a);
+    hipLaunchKernelGGL(prefill_fp4_kernel, grid, dim3(kWaves * 64), 0, stream, a);
   if (a.splits > 1) {
     const int st = launch_status();
     if (st != NVAMD_OK) return st;
