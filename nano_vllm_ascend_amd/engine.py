@@ -61,9 +61,9 @@ class LLM:
     readable as ``runner.last_logits``, at one logits-sized copy per overlapped
     step.  ``kv_cache_dtype="fp4"`` (not in the reference) holds the KV cache in
     4 bits: 3.76 times the tokens in the same memory, at the precision of 4-bit
-    keys and values.  A batch of prompts none of which has a cached prefix attends
-    to its own keys as they are; any other batch, and every decode step, to what
-    the cache holds.
+    keys and values.  A prompt without a cached prefix attends to its own keys as
+    they are; one with a cached prefix, and every decode step, to what the cache
+    holds.  (Prompts of both kinds admitted together run as two batches.)
     """
 
     def __init__(self, model_path, max_model_len: int = 2048, block_size: int = 128, num_blocks: int | None = None,

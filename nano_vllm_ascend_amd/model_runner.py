@@ -278,6 +278,26 @@ class ModelRunner:
             return
         self._drop_in_flight()
         self._prefilled_since_decode = True
+        batches = self._by_route(seqs)
+        if len(batches) == 1:
+            return self._prefill(seqs)
+        rows = {}
+        for batch in batches:
+            self._prefill(batch)
+            rows.update(zip((s.seq_id for s in batch), self.last_logits))
+        self.last_logits = torch.stack([rows[s.seq_id] for s in seqs])
+
+    def _by_route(self, seqs: list[Sequence]) -> list[list[Sequence]]:
+        """The batches that prompts run in.  A batch takes one route: the paged one, over what the cache holds, if any of
+        its prompts has a cached prefix, else the dense one, over the prompts' own keys.  In a 4-bit cache the two differ by
+        the precision of the cache, and prompts with a prefix run apart from those without, so that none of them
+        depends on what the others hit.  (Those with a prefix first: new prompts may take unused cached blocks.)"""
+        hits = [s for s in seqs if s.cached_prefix_len > 0]
+        if not isinstance(self.kv_cache, Fp4PagedKVCache) or len(hits) in (0, len(seqs)):
+            return [seqs]
+        return [hits, [s for s in seqs if s.cached_prefix_len == 0]]
+
+    def _prefill(self, seqs: list[Sequence]) -> None:
         md = self.block_manager.prepare_prefill_metadata(
             slots=[s.seq_id for s in seqs], seq_lens=[s.runtime_prompt_len for s in seqs],
             start_positions=[s.cached_prefix_len for s in seqs], prefix_block_ids=[s.cached_block_ids for s in seqs],

@@ -109,6 +109,46 @@ def test_prefix_hits_read_the_4_bit_pages(device):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("beside", [[], [90, 5]], ids=["alone", "beside_prompts_without_a_hit"])
+def test_a_prompt_takes_the_route_of_its_own_prefix(device, beside):
+    """The logits of a prompt with cached blocks are the oracle's on the keys and values that the cache holds; those of
+    prompts without any, in the same step, the oracle's on its own keys and values, as if they ran alone."""
+    llm = make_llm(enable_prefix_cache=True)
+    ref = Qwen3Ref(dict(llm.runner.model.state_dict()), SMALL, round_bf16=True, max_positions=512)
+    shared = prompts_for([300], seed=5)[0]
+    llm.generate([shared + [1, 2, 3]], max_new_tokens=2)
+    prompts = prompts_for(beside, seed=6)
+    prompts.insert(1, shared + [7, 8])  # between the others
+    seen = {}
+
+    def hook(kind, slots, md):
+        assert kind == "prefill"
+        seen.update((slot, (md.block_tables[row], int(md.context_lens[row]))) for row, slot in enumerate(slots))
+
+    llm.runner.metadata_hook = hook
+    ids = [llm.submit(p, max_new_tokens=6) for p in prompts]
+    llm.step()
+    llm.runner.metadata_hook = None
+    assert list(llm.scheduler.running) == ids and llm.runner.last_logits.shape[0] == len(prompts)
+    bs, cache = llm.runner.block_size, llm.runner.kv_cache
+    for row, (seq_id, prompt) in enumerate(zip(ids, prompts)):
+        seq = llm.scheduler.running[seq_id]
+        table, n = seen[seq_id]
+        assert n == len(prompt) and (seq.cached_prefix_len == 256) == (len(prompt) == 302)
+        if seq.cached_prefix_len:
+            pos = torch.arange(n)
+            where = (table.long()[pos // bs] * bs + pos % bs).to(device)
+            history = [tuple(x.cpu() for x in cache.read(layer, where)) for layer in range(SMALL.num_hidden_layers)]
+            want = logits_after(ref, history, prompt[-1], n - 1)
+        else:
+            ref.reset()
+            want = ref.forward(prompt).reshape(-1)
+        got = llm.runner.last_logits[row].float().cpu()
+        assert (got - want).abs().max().item() <= LOGIT_TOL, (row, (got - want).abs().max().item())
+        assert seq.next_token_id == int(got.argmax())
+
+
+@pytest.mark.gpu
 def test_the_pool_holds_as_many_more_tokens(device):
     llm = make_llm(num_blocks=None, npu_memory_utilization=0.2)
     args = (SMALL.num_hidden_layers, llm.runner.block_size, SMALL.num_key_value_heads, SMALL.head_dim)
