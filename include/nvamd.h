@@ -441,7 +441,11 @@ int nvamd_qk_norm_rope_fp4(void *q_out, int64_t q_out_stride,
 /* paged_decode_fp4: nvamd_paged_decode over the 4-bit cache; workspace of    */
 /* nvamd_paged_decode_workspace_size bytes under the same rules (zero-filled  */
 /* once, any number of calls and replays of either kind one after another,    */
-/* none that overlap).  max_context_len <= 131072.                            */
+/* none that overlap).  max_context_len <= 131072.  A sequence's bits do not  */
+/* depend on that bound or on the table's width.  Past 512 tokens they depend */
+/* on the batch: a context is cut where the contexts of the whole call put    */
+/* it, and the order of its sums follows (nvamd_paged_decode cuts every       */
+/* sequence alike).  Every order is within the same error.                    */
 int nvamd_paged_decode_fp4(void *out, int64_t out_stride,
                            const void *q, int64_t q_stride,
                            const void *k_codes, const void *k_scales,
@@ -483,7 +487,9 @@ int nvamd_paged_decode_fused_fp4(void *out, int64_t out_stride,
 /* NaN of the cache reaches the rows that see its key and no others.  A       */
 /* sequence whose rows leave [0, num_tokens) is skipped, and it, a q_len past */
 /* max_q_len (whose further rows are not written) and a kv_len below q_len    */
-/* are reported as NVAMD_ERR_CONTEXT.                                         */
+/* are reported as NVAMD_ERR_CONTEXT.  The order of a row's sums follows from */
+/* n_seqs, max_q_len, the heads and the table's positions (which kernel, and  */
+/* whether the keys are cut), not from the other sequences' lengths.          */
 int nvamd_paged_prefill_fp4(void *out, int64_t out_stride,
                             const void *q, int64_t q_stride,
                             const void *k_codes, const void *k_scales,

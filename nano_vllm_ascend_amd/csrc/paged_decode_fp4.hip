@@ -5,8 +5,9 @@
 //
 // Work: a unit (sequence, kv head) is cut into partitions of equal length, a workgroup of 8 waves each.  Every
 // workgroup reads the context lengths and derives the same length from them (partition_tokens), so the cut follows the
-// contexts themselves and not the bound that the launch was made with.  A partition leaves (max, sum, numerator) per
-// head in the workspace and counts its arrival; the last one of a unit joins them.
+// contexts themselves and not the bound that the launch was made with.  (A sequence of more than kLeastPart tokens is so
+// summed in an order that depends on the sequences beside it.)  A partition leaves (max, sum, numerator) per head in the
+// workspace and counts its arrival; the last one of a unit joins them.
 //
 // A wave takes 64 tokens at a time, four 16-token tiles, one per 16 lanes (gq = lane / 16):
 //   S^T = K . Q^T  v_mfma_scale_f32_16x16x128_f8f6f4 on the codes as they lie in the cache, A = 16 rows of K: a lane's
@@ -415,8 +416,11 @@ paged_decode_fp4_kernel(DecodeFp4Args a, std::conditional_t<FUSED, StepArgs, Not
 #pragma unroll
       for (int e = 0; e < 8; ++e) o[e] *= alpha;
     }
-    // P rounded to bf16 for the matrix cores; the sum takes the same rounded values.  Back in the order of the
-    // products, the columns past the heads hold weights of other tokens and give numerators that are never read.
+    // P rounded to bf16 for the matrix cores; the sum takes the same rounded values.  The result is then off by 1.9e-3 to
+    // 2.3e-3 of its size where its own rounding is 1.65e-3.  A second bf16 term of P, which the bf16 cache's kernel has
+    // at no cost, takes 20 registers more here, with them one of the two workgroups of a CU, and the products twice:
+    // 100 x U[2048, 4096] 73 us for 62, 32 x U[256, 2304] 20.8 for 16.2.  Back in the order of the products, the columns
+    // past the heads hold weights of other tokens and give numerators that are never read.
     u32x4 pf[2];
 #pragma unroll
     for (int x = 0; x < NP; ++x)

@@ -29,6 +29,10 @@
 //   paged_decode_fp4.hip with rows in the place of heads and a last key for each row.  Bound by the latency of a launch
 //   and of a wave's steps: 8 x 20 rows on 1,040 keys 10 us.  On long contexts the keys are cut as well.
 //
+// Weights are rounded to bf16 once for the matrix cores, and the sums take the rounded values, as in the bf16 cache's
+// prefill: a second term would double the products with V, where the matrix cores' and the vector ALUs' issue already
+// fills the time.
+//
 // A block of values that reads as NaN must reach the rows that see its key and no others, though masked rows
 // multiply it by a weight of zero: such values enter the products as zeros, and the rows that see
 // the key get the NaN afterwards (a branch that no other tile takes).

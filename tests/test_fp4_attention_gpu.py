@@ -141,6 +141,25 @@ def test_decode_many_sequences(device):
     check_decode(batch, q, batch.decode(q, bound=4096))
 
 
+@pytest.mark.parametrize("hq, hkv", [(2, 1), (16, 8), (12, 2)])
+def test_decode_beside_other_sequences(device, hq, hkv):
+    """Contexts of up to 512 tokens give the same bits whatever runs beside them; of longer ones the cut, and with it the
+    order of the sums, follows from all contexts of the call, within the bound."""
+    lens = [512, 1, 3000, 200, 513, 5000] + [700] * 40
+    batch = Batch(device, lens, hq, hkv, 64, seed=36)
+    q = batch.queries(len(lens))
+    whole = batch.decode(q)
+    check_decode(batch, q, whole)
+    tables, dq = batch.tables.to(device), q.to(device)
+    for i in range(6):
+        n = torch.tensor(lens[i:i + 1], dtype=torch.int32, device=device)
+        space = _C.alloc_paged_decode_workspace(1, hq, hkv, 5000, device)
+        alone = _C.paged_decode_fp4(None, dq[i:i + 1], batch.keys, batch.values, tables[i:i + 1], n, SCALE, 5000, space)
+        close(alone, *batch.want(i, q[i:i + 1]))
+        if lens[i] <= 512:
+            assert torch.equal(alone[0], whole[i])
+
+
 def test_decode_scores_far_apart(device):
     """A few keys carry all of the weight, in whichever partition they are; large and negative scales."""
     batch = Batch(device, [1500, 700], 4, 1, 64, seed=6, spread=1.5)
@@ -737,6 +756,62 @@ def test_what_the_library_refuses_raises(device):
                               torch.arange(4, device=device))
     with pytest.raises(ValueError, match="on one device|GPU"):
         _C.kv_cache_write_fp4(q[:, :1].cpu(), q[:, :1].cpu(), batch.keys, batch.values, torch.arange(1, device=device))
+
+
+def irregular(name, x):
+    """What an argument must not be: on the host, of another type, a row short, not dense."""
+    if isinstance(x, _C.Fp4Pages):
+        for i, t in enumerate(x):
+            for how, bad in irregular(name, t):
+                yield f"{x._fields[i]} {how}", x._replace(**{x._fields[i]: bad})
+        yield "a plain tuple", tuple(x)
+        return
+    yield "on the host", x.cpu()
+    if name != "workspace":
+        yield "of another type", x.to(torch.float64)
+        if name not in ("cos_sin", "cu_seqlens_q"):
+            yield "a row short", x[:-1]
+    if x.dim() == 1:
+        yield "with gaps", x.repeat_interleave(2)[::2]
+    else:
+        yield "with gaps", x.repeat_interleave(2, -1)[..., ::2]
+
+
+@pytest.mark.parametrize("name", ["write", "read", "rope", "decode", "decode_fused", "prefill"])
+def test_what_the_checks_refuse_is_not_called_at_once(device, name):
+    """csrc/calls.cpp leaves each call that _C.py refuses to it."""
+    batch = Batch(device, [40, 33, 20], 4, 2, 16, seed=34)
+    q, k, v, qw, kw, pos, table, eps, keys, values, slots = step_of(batch, 35)
+    lens = torch.tensor(batch.lens, dtype=torch.int32, device=device)
+    tables = batch.tables.to(device)
+    cu = torch.arange(4, dtype=torch.int32, device=device)
+    space = _C.alloc_paged_decode_workspace(3, 4, 2, 64, device)
+    out = torch.empty_like(q)
+    rope = dict(q=q, k=k, v=v, q_weight=qw, k_weight=kw, positions=pos, cos_sin=table, eps=eps)
+    pages = dict(key_pages=keys, value_pages=values)
+    where = dict(block_tables=tables, context_lens=lens, scale=SCALE, max_context_len=64, workspace=space)
+    call, args = {
+        "write": (_C.kv_cache_write_fp4, dict(key_states=k, value_states=v, **pages, slot_mapping=slots)),
+        "read": (_C.kv_cache_read_fp4, dict(**pages, slot_mapping=slots)),
+        "rope": (_C.qk_norm_rope_fp4, dict(**rope, **pages, slot_mapping=slots, q_out=out, k_out=torch.empty_like(k))),
+        "decode": (_C.paged_decode_fp4, dict(out=out, q=q, **pages, **where)),
+        "decode_fused": (_C.paged_decode_fused_fp4, dict(out=out, **rope, **pages, slot_mapping=slots, **where)),
+        "prefill": (_C.paged_prefill_fp4, dict(out=out, q=q, **pages, block_tables=tables, cu_seqlens_q=cu, kv_lens=lens,
+                                               max_q_len=1, scale=SCALE)),
+    }[name]
+    at_once = getattr(_C._calls, name)
+    assert type(at_once(*args.values())) not in (type(None), int)
+    for arg, x in args.items():
+        if name == "read" and arg == "slot_mapping":
+            cases = [c for c in irregular(arg, x) if c[0] != "a row short"]  # as many rows as there are slots
+        else:
+            cases = irregular(arg, x) if isinstance(x, (torch.Tensor, _C.Fp4Pages)) else ()
+        for how, bad in cases:
+            changed = {**args, arg: bad}
+            assert at_once(*changed.values()) is None, (arg, how)
+            with pytest.raises(ValueError):
+                call(**changed)
+    assert _C.index_errors() == 0
 
 
 def test_calls_without_the_extension(device, monkeypatch):
