@@ -385,6 +385,8 @@ int nvamd_rms_norm_tiled(const void *x, int64_t x_stride, const void *weight,
 /*   v_codes  byte 16 (16 q + r) + t: dims 32q + r (low) and 32q + 16 + r, r  */
 /*   < 16;                                                                    */
 /*   v_scales byte 16 q + t.                                                  */
+/* Bytes that no write has filled may be anything: past a sequence's length   */
+/* they reach no result.                                                      */
 /* Slots, block tables, index errors, strides and alignments are as for the   */
 /* bf16 entry points; block_size a power of two >= 16.  A write or read of    */
 /* 2^27 rows or more, a prefill table of more than 2^30 positions and a cache */

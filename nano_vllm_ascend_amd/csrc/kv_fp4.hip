@@ -9,7 +9,7 @@
 //
 // All three are bound by memory: per head vector 256 bytes of bf16 and 68 of the cache, once.  36,488 tokens, 8 kv
 // heads (and 16 query heads): write 189 MB in 37 us (5.2 TB/s), read 189 MB in 34 us (5.6 TB/s), norm + RoPE + write
-// with the keys returned 564 MB in 115 us (4.9 TB/s); a large copy reaches 5.0 TB/s.  One token: 3 us, the launch.
+// with the keys returned 564 MB in 117 us (4.8 TB/s); a large copy reaches 5.0 TB/s.  One token: 3 us, the launch.
 #include "fp4_rows.h"
 
 namespace nvamd {

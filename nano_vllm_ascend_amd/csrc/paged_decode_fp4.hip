@@ -174,8 +174,9 @@ __host__ __device__ constexpr int max_partitions(int units) { return partition_s
 // whose id is a scalar (pages of 128 at 32 x U[256, 2304]: 16.3 us, without 20.8; at 100 x U[2048, 4096] 63, 73).
 // FUSED: the norm, the rotation and the store of the step's rows first.  Every workgroup makes its own queries; the one
 // whose partition ends the context stores the new row and waits for it, so that its loads find it.  Bits as of
-// nvamd_qk_norm_rope_fp4 and this kernel after it, in less time: 32 x U[256, 2304] 17.3 us for 19.9 (this kernel alone
-// 15.9), 16 x U[512, 4096] at 64 heads 15.6 for 17.8, 100 x U[2048, 4096] 66.6 for 67.8, 4 x U[1, 512] 6.8 for 8.0.
+// nvamd_qk_norm_rope_fp4 and this kernel after it, in less time (from a graph over three caches in turn; in brackets this
+// kernel alone): 32 x U[256, 2304] 17.4 us for 19.7 (15.8), 16 x U[512, 4096] at 64 heads 15.5 for 17.8 (14.1), 100 x
+// U[2048, 4096] 66.2 for 67.4 (62.3), 4 x U[1, 512] 6.8 for 8.0 (4.9).
 template <int GP, bool WIDE, bool FUSED>
 __global__ void __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(WIDE ? 4 : 3)))
 paged_decode_fp4_kernel(DecodeFp4Args a, std::conditional_t<FUSED, StepArgs, Nothing> step_args) {

@@ -17,8 +17,8 @@
 //   of the next tile loads as the scores have taken this one's, V's codes are two tiles ahead, V's operands one (two
 //   stages, one barrier a tile). Bound by issue: the matrix cores are busy 43.5% of the time and the vector ALUs
 //   (exponents, rounding, expansion) 55%, one or the other at 98.5% of it.  32 x U[512, 2048] rows on 1,152 cached keys
-//   689 us (895 TFLOP/s), 2 x U[3000, 4000] rows of 40 query heads on 4,096 972 us (1,022 TFLOP/s); a bf16 matrix
-//   product of 8,192^3 reaches 1,254.
+//   695 us (887 TFLOP/s), 2 x U[3000, 4000] rows of 40 query heads on 4,096 1,004 us (990 TFLOP/s), on a card whose bf16
+//   matrix product of 8,192^3 reaches 1,252 (where it reaches 1,185, 754 and 1,113 us).
 //
 // Strips (one long prompt, or several short ones).  Workgroup = 4 waves = 32 rows, a wave every fourth 32 keys; no
 //   barrier in the loop, the waves' results meet in LDS.  A lane expands 16 tokens of a dim pair straight into
