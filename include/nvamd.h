@@ -387,6 +387,8 @@ int nvamd_rms_norm_tiled(const void *x, int64_t x_stride, const void *weight,
 /*   v_scales byte 16 q + t.                                                  */
 /* Bytes that no write has filled may be anything: past a sequence's length   */
 /* they reach no result.                                                      */
+/* Attention sums weights of up to 2^8, and their products with v, in 32      */
+/* bits: |v| * 2^8 * (keys of the row) has to stay below 2^128.               */
 /* Slots, block tables, index errors, strides and alignments are as for the   */
 /* bf16 entry points; block_size a power of two >= 16.  A write or read of    */
 /* 2^27 rows or more, a prefill table of more than 2^30 positions and a cache */

@@ -141,6 +141,44 @@ def test_decode_many_sequences(device):
     check_decode(batch, q, batch.decode(q, bound=4096))
 
 
+def test_decode_of_the_largest_batches(device):
+    """16,384 units of a sequence and a kv head: each sequence's bits are those of a small batch."""
+    gen = torch.Generator().manual_seed(39)
+    lens = [int(x) for x in torch.randint(0, 40, (2048,), generator=gen)]
+    batch = Batch(device, lens, 8, 8, 16, seed=40)
+    q = batch.queries(2048)
+    got = batch.decode(q, bound=4096)
+    tables, dq, n = batch.tables.to(device), q.to(device), torch.tensor(lens, dtype=torch.int32, device=device)
+    space = _C.alloc_paged_decode_workspace(100, 8, 8, 64, device)
+    for at in (0, 1000, 1948):
+        rows = slice(at, at + 100)
+        few = _C.paged_decode_fp4(None, dq[rows], batch.keys, batch.values, tables[rows], n[rows], SCALE, 64, space)
+        assert torch.equal(few, got[rows])
+    for i in (0, 1, 1023, 2047):
+        if lens[i]:
+            close(got[i:i + 1], *batch.want(i, q[i:i + 1]))
+    assert not got[n == 0].any() and _C.index_errors() == 0
+
+
+def at_scale(batch, k_exp, v_exp):
+    """The batch's rows with keys and values of about 2^k_exp and 2^v_exp."""
+    slots = torch.cat(batch.slots)
+    k, v = fp4_ref.read(batch.pages, slots)
+    fp4_ref.write(batch.pages, (k * 2.0 ** k_exp).bfloat16(), (v * 2.0 ** v_exp).bfloat16(), slots)
+    batch.upload()
+
+
+EXPONENTS = pytest.mark.parametrize("q_exp, k_exp, v_exp", [(100, -100, 0), (-90, 90, 90), (-60, 60, -90), (0, 0, 100)])
+
+
+@EXPONENTS
+def test_decode_of_numbers_far_from_one(device, q_exp, k_exp, v_exp):
+    batch = Batch(device, [1, 70, 600], 4, 2, 32, seed=41)
+    at_scale(batch, k_exp, v_exp)
+    q = batch.queries(3, scale=2.0 ** q_exp)
+    check_decode(batch, q, batch.decode(q))
+
+
 @pytest.mark.parametrize("hq, hkv", [(2, 1), (16, 8), (12, 2)])
 def test_decode_beside_other_sequences(device, hq, hkv):
     """Contexts of up to 512 tokens give the same bits whatever runs beside them; of longer ones the cut, and with it the
@@ -509,6 +547,15 @@ def test_prefill_scores_far_apart(device, bound):
 
 
 @BOUNDS
+@EXPONENTS
+def test_prefill_of_numbers_far_from_one(device, q_exp, k_exp, v_exp, bound):
+    batch = Batch(device, [1, 70, 300], 4, 2, 32, seed=42)
+    at_scale(batch, k_exp, v_exp)
+    q = batch.queries(1 + 33 + 40, scale=2.0 ** q_exp)
+    check_prefill(batch, q, [1, 33, 40], batch.prefill(q, [1, 33, 40], max_q=bound))
+
+
+@BOUNDS
 def test_prefill_queries_with_outliers(device, bound):
     batch = Batch(device, [300, 70], 4, 1, 64, seed=15)
     slots = torch.cat(batch.slots)
@@ -681,6 +728,21 @@ def test_fused_step_has_the_bits_of_the_two_launches(device, hq, hkv, bs):
         assert torch.equal(got, want) and all(torch.equal(a, b) for a, b in zip(in_pages(batch), stored))
         assert all(torch.equal(a, b) for a, b in zip(args[:3], raw))
     assert _C.index_errors() == 0
+
+
+@pytest.mark.parametrize("hq, hkv, bs", [(16, 8, 128), (34, 2, 32), (1, 1, 16)])
+def test_fused_step_may_write_over_its_queries(device, hq, hkv, bs):
+    """out is q itself, a view into the projection's rows: k and v beside it stay as they are."""
+    batch = Batch(device, [1, 300, 0, 513, 4097], hq, hkv, bs, seed=37)
+    space = _C.alloc_paged_decode_workspace(5, hq, hkv, 4097, device)
+    args = step_of(batch, seed=38)
+    want = attend(batch, None, 4097, space, fused=args)
+    batch.upload()
+    q, k, v, *rest = step_of(batch, seed=38)
+    kv = k.clone(), v.clone()
+    got = _C.paged_decode_fused_fp4(q, q, k, v, *rest, batch.tables.to(device),
+                                    torch.tensor(batch.lens, dtype=torch.int32, device=device), SCALE, 4097, space)
+    assert got is q and torch.equal(q, want) and torch.equal(k, kv[0]) and torch.equal(v, kv[1])
 
 
 def test_fused_step_reports_what_it_skips_and_clamps(device):
