@@ -660,6 +660,14 @@ def _stream_of(device: int, *tensors: torch.Tensor) -> int:
     return _raw_stream(device) if _raw_stream is not None else _stream()
 
 
+def _int32(name: str, value) -> int:
+    """An int argument of the C ABI (ctypes would keep the lower half of a larger number)."""
+    value = int(value)
+    if not -(1 << 31) <= value < 1 << 31:
+        raise ValueError(f"{name} {value} is past 32 bits")
+    return value
+
+
 def _heads(name: str, t: torch.Tensor, rows: int, heads: int, d: int) -> int:
     """Checks a [T, heads, D] bf16 view of dense rows; returns its row stride."""
     if t.shape != (rows, heads, d):
@@ -817,10 +825,11 @@ def _fp4_attention_args(out, q, key_pages, value_pages, block_tables, seqs: int)
         raise ValueError("block_tables rows must be dense")
     if tables[0] > 1 and bt_stride[0] < width:
         raise ValueError(f"rows of block_tables overlap: {tuple(tables)} with a row stride of {bt_stride[0]}")
+    bt_row = _int32("the row stride of block_tables", bt_stride[0] if tables[0] > 1 else width)
     least = hq * d  # a single row's stride says nothing
     return (out.data_ptr(), out_stride[0] if t > 1 else max(out_stride[0], least), q.data_ptr(),
             q_stride[0] if t > 1 else max(q_stride[0], least), *pages, nb, bs, block_tables.data_ptr(),
-            max(bt_stride[0], width), width), (hq, hkv, d), device
+            bt_row, width), (hq, hkv, d), device
 
 
 def _fp4_decode_args(block_tables, context_lens, workspace, b: int) -> None:
@@ -847,9 +856,10 @@ def paged_decode_fp4(out: torch.Tensor | None, q: torch.Tensor, key_pages: Fp4Pa
     b = q.shape[0]
     args, heads, device = _fp4_attention_args(out, q, key_pages, value_pages, block_tables, b)
     _fp4_decode_args(block_tables, context_lens, workspace, b)
+    max_context_len = _int32("max_context_len", max_context_len)
     if _range_checks and _checking():
-        check_paged_context(block_tables, context_lens, args[8], args[9], int(max_context_len))
-    status = lib.nvamd_paged_decode_fp4(*args, context_lens.data_ptr(), b, *heads, float(scale), int(max_context_len),
+        check_paged_context(block_tables, context_lens, args[8], args[9], max_context_len)
+    status = lib.nvamd_paged_decode_fp4(*args, context_lens.data_ptr(), b, *heads, float(scale), max_context_len,
                                         workspace.data_ptr(), workspace.nbytes,
                                         _stream_of(device, q, out, block_tables, context_lens, workspace))
     if status:
@@ -875,17 +885,18 @@ def paged_decode_fused_fp4(out: torch.Tensor | None, q: torch.Tensor, k: torch.T
     b = q.shape[0]
     args, heads, device = _fp4_attention_args(out, q, key_pages, value_pages, block_tables, b)
     _fp4_decode_args(block_tables, context_lens, workspace, b)
+    max_context_len = _int32("max_context_len", max_context_len)
     nb, bs, (hq, hkv, d) = args[8], args[9], heads
     k_stride, v_stride = _heads("k", k, b, hkv, d), _heads("v", v, b, hkv, d)
     _rope_args(q_weight, k_weight, positions, cos_sin, b, d)
     slots = _page_slots(slot_mapping, b, nb * bs)
     if _range_checks and _checking():
         check_positions(positions, cos_sin.shape[0])
-        check_paged_context(block_tables, context_lens, nb, bs, int(max_context_len))
+        check_paged_context(block_tables, context_lens, nb, bs, max_context_len)
     status = lib.nvamd_paged_decode_fused_fp4(
         *args[:4], k.data_ptr(), k_stride, v.data_ptr(), v_stride, q_weight.data_ptr(), k_weight.data_ptr(),
         positions.data_ptr(), cos_sin.data_ptr(), cos_sin.shape[0], float(eps), *args[4:10], slots,
-        *args[10:], context_lens.data_ptr(), b, hq, hkv, d, float(scale), int(max_context_len), workspace.data_ptr(),
+        *args[10:], context_lens.data_ptr(), b, hq, hkv, d, float(scale), max_context_len, workspace.data_ptr(),
         workspace.nbytes,
         _stream_of(device, q, k, v, out, q_weight, k_weight, positions, cos_sin, slot_mapping, block_tables,
                    context_lens, workspace))
@@ -909,10 +920,10 @@ def paged_prefill_fp4(out: torch.Tensor, q: torch.Tensor, key_pages: Fp4Pages, v
     args, heads, device = _fp4_attention_args(out, q, key_pages, value_pages, block_tables, n)
     if n < 0 or kv_lens.dtype is not torch.int32 or kv_lens.numel() < n or not kv_lens.is_contiguous():
         raise ValueError("kv_lens must be contiguous int32, one per sequence")
+    max_q_len = _int32("max_q_len", max_q_len)
     if _range_checks and _checking():
         check_paged_context(block_tables[:n], kv_lens[:n], args[8], args[9])
     stream = _stream_of(device, q, out, block_tables, cu_seqlens_q, kv_lens)
-    max_q_len = int(max_q_len)
     need = lib.nvamd_paged_prefill_fp4_workspace_size(n, max_q_len, heads[0], heads[1], args[9], args[12])
     space = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None  # freed behind the call
     status = lib.nvamd_paged_prefill_fp4(*args, cu_seqlens_q.data_ptr(), kv_lens.data_ptr(), n, q.shape[0], max_q_len,

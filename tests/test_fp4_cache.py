@@ -336,6 +336,31 @@ def test_block_tables_whose_rows_overlap_are_refused():
             call(torch.zeros(12, dtype=torch.int32).as_strided((4, 3), (3, 1)))
 
 
+def test_numbers_past_32_bits_are_refused():
+    """The C ABI takes them as ints, and a conversion would keep their lower half."""
+    q, kv, w = heads(4, 16), heads(4, 8), torch.ones(128, dtype=torch.bfloat16)
+    lens, pos, ws = torch.ones(4, dtype=torch.int32), torch.arange(4), torch.zeros(64)
+    cu, table = torch.arange(5, dtype=torch.int32), torch.zeros(4, 3, dtype=torch.int32)
+    far = torch.empty(4, (1 << 32) + 3, dtype=torch.int32, device="meta")[:, :3]  # rows 2^32 + 3 apart
+
+    def decode(bt=table, bound=48):
+        _C.paged_decode_fp4(None, q, pages(), pages(), bt, lens, 0.1, bound, ws)
+
+    def fused(bt=table, bound=48):
+        _C.paged_decode_fused_fp4(None, q, kv, kv, w, w, pos, torch.zeros(64, 128), 1e-6, pages(), pages(), pos, bt, lens,
+                                  0.1, bound, ws)
+
+    def prefill(bt=table, bound=1):
+        _C.paged_prefill_fp4(q, q, pages(), pages(), bt, cu, lens, bound, 0.1)
+
+    for call in (decode, fused, prefill):
+        with pytest.raises(ValueError, match="row stride of block_tables .* 32 bits"):
+            call(bt=far)
+        for bound in ((1 << 32) + 48, 1 << 31, -(1 << 32) + 48):
+            with pytest.raises(ValueError, match="max_.*_len .* 32 bits"):
+                call(bound=bound)
+
+
 # -------------------------------------------------------------------------------------------- without csrc/calls.cpp
 CALLS = "nano_vllm_ascend_amd._calls"
 
