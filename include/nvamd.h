@@ -41,7 +41,7 @@ extern "C" {
 
 /* ABI version of this header; nvamd_version() returns the version the library was built
    with, for the loader's sanity check. */
-#define NVAMD_ABI_VERSION 4
+#define NVAMD_ABI_VERSION 5
 int nvamd_version(void);
 
 /* ------------------------------------------------------------------------- */
@@ -508,6 +508,125 @@ int nvamd_paged_prefill_fp4(void *out, int64_t out_stride,
 size_t nvamd_paged_prefill_fp4_workspace_size(int n_seqs, int max_q_len,
                                               int num_heads, int num_kv_heads,
                                               int block_size, int bt_width);
+
+/* ------------------------------------------------------------------------- */
+/* KV cache held in 8 bits.  No counterpart in the reference either: the same */
+/* path over a cache of 128 bytes per head vector, in e4m3 with a scale for   */
+/* each tile of 16 tokens of a head:                                          */
+/*   a tile's keys (values) share a scale 2^e, a byte e + 127.  Rows that     */
+/*   begin a tile set e to the least integer for which max|x| <= 448 * 2^e    */
+/*   over them, in [-117, 119]; rows that go behind others raise the tile's e */
+/*   to theirs if that is larger, and the codes of its other tokens are then  */
+/*   rounded to the new scale.  A value's code is x / 2^e in e4m3 (sign, 4    */
+/*   bits of exponent, 3 of fraction), to nearest, ties to the even code,     */
+/*   saturated at 448; an infinity or a NaN is held as a NaN (127 or 255) and */
+/*   does not count for the scale.                                            */
+/* So a tile is filled from its first token on: writing its first token       */
+/* starts it anew, and what its other tokens held is lost.                    */
+/* One layer's cache is four byte arrays, the codes 16-byte aligned:          */
+/*   k_codes, v_codes   [num_blocks, num_kv_heads, block_size, 128]           */
+/*   k_scales, v_scales [num_blocks, num_kv_heads, block_size / 16]           */
+/* Inside a page of a head every 16 tokens form a tile of 2048 bytes of codes; */
+/* with t = token % 16:                                                       */
+/*   k_codes  byte 1024 (d / 64) + 64 t + d % 64: dim d;                      */
+/*   v_codes  byte 16 d + t: dim d.                                           */
+/* Bytes that no write has filled may be anything: past a sequence's length   */
+/* they reach no result.                                                      */
+/* Attention sums weights of up to 2^8, and their products with v, in 32      */
+/* bits: |v| * 2^8 * (keys of the row) has to stay below 2^128.               */
+/* Slots, block tables, index errors, strides and alignments are as for the   */
+/* bf16 entry points; block_size a power of two >= 16.  A write or read of    */
+/* 2^27 rows or more, more than 32,767 kv heads, a prefill table of more than */
+/* 2^30 positions and a cache of 2^31 tiles or more return                    */
+/* NVAMD_EUNSUPPORTED.                                                        */
+/* ------------------------------------------------------------------------- */
+
+/* kv_cache_write_fp8: row t of k and v goes to slot_mapping[t] (-1: padding, */
+/* skipped).  The rows of a tile follow one another in the call, in the order */
+/* of their slots and with no padding row between them, as the tokens of a    */
+/* sequence do; those of different tiles come in any order.  (Else the tile   */
+/* holds none of them as a whole.)                                            */
+int nvamd_kv_cache_write_fp8(const void *k, int64_t k_stride,
+                             const void *v, int64_t v_stride,
+                             void *k_codes, void *k_scales,
+                             void *v_codes, void *v_scales,
+                             int num_blocks, int block_size,
+                             const int64_t *slot_mapping, int num_tokens,
+                             int num_kv_heads, int head_dim,
+                             hipStream_t stream);
+
+/* kv_cache_read_fp8: row t of k and v (bf16) = the values at                 */
+/* slot_mapping[t], in any order; zeros for -1 and (reported) for a slot      */
+/* outside the cache.  Exact.                                                 */
+int nvamd_kv_cache_read_fp8(void *k, int64_t k_stride,
+                            void *v, int64_t v_stride,
+                            const void *k_codes, const void *k_scales,
+                            const void *v_codes, const void *v_scales,
+                            int num_blocks, int block_size,
+                            const int64_t *slot_mapping, int num_tokens,
+                            int num_kv_heads, int head_dim,
+                            hipStream_t stream);
+
+/* qk_norm_rope_fp8: nvamd_qk_norm_rope_fp4 into the 8-bit cache (rows in the */
+/* order that nvamd_kv_cache_write_fp8 asks for).                             */
+int nvamd_qk_norm_rope_fp8(void *q_out, int64_t q_out_stride,
+                           void *k_out, int64_t k_out_stride,
+                           const void *q, int64_t q_stride,
+                           const void *k, int64_t k_stride,
+                           const void *v, int64_t v_stride,
+                           const void *q_weight, const void *k_weight,
+                           const int64_t *positions,
+                           const float *cos_sin, int max_positions,
+                           void *k_codes, void *k_scales,
+                           void *v_codes, void *v_scales,
+                           int num_blocks, int block_size,
+                           const int64_t *slot_mapping, int num_tokens,
+                           int num_heads, int num_kv_heads, int head_dim,
+                           float eps, hipStream_t stream);
+
+/* paged_decode_fp8: nvamd_paged_decode_fp4 over the 8-bit cache, workspace   */
+/* and the order of sums alike.                                               */
+int nvamd_paged_decode_fp8(void *out, int64_t out_stride,
+                           const void *q, int64_t q_stride,
+                           const void *k_codes, const void *k_scales,
+                           const void *v_codes, const void *v_scales,
+                           int num_blocks, int block_size,
+                           const int32_t *block_tables, int bt_stride,
+                           int bt_width, const int32_t *context_lens,
+                           int batch, int num_heads, int num_kv_heads,
+                           int head_dim, float scale, int max_context_len,
+                           void *workspace, size_t workspace_bytes,
+                           hipStream_t stream);
+
+/* paged_prefill_fp8: nvamd_paged_prefill_fp4 over the 8-bit cache, workspace, */
+/* reports and the order of sums alike.  A NaN of the cache reaches the rows  */
+/* that see its key and no others.                                            */
+int nvamd_paged_prefill_fp8(void *out, int64_t out_stride,
+                            const void *q, int64_t q_stride,
+                            const void *k_codes, const void *k_scales,
+                            const void *v_codes, const void *v_scales,
+                            int num_blocks, int block_size,
+                            const int32_t *block_tables, int bt_stride,
+                            int bt_width, const int32_t *cu_seqlens_q,
+                            const int32_t *kv_lens, int n_seqs, int num_tokens,
+                            int max_q_len, int num_heads, int num_kv_heads,
+                            int head_dim, float scale, void *workspace,
+                            size_t workspace_bytes, hipStream_t stream);
+size_t nvamd_paged_prefill_fp8_workspace_size(int n_seqs, int max_q_len,
+                                              int num_heads, int num_kv_heads,
+                                              int block_size, int bt_width);
+
+/* copy_blocks: pool[layer][targets[i]] = pool[layer][sources[i]] (device     */
+/* int32, i < count) for every layer of up to 8 pools [num_layers, num_blocks, */
+/* block_bytes[p]], in one launch.  `pools` and `block_bytes` are host arrays, */
+/* read during the call.  No block is a target twice, or a target and another */
+/* pair's source; a pair of the same block does nothing, and one that names a */
+/* block outside the pool is skipped and reported (NVAMD_ERR_BLOCK).  Up to   */
+/* 65,535 pairs, 65,535 layers and 4 GiB a block.                             */
+int nvamd_copy_blocks(void *const *pools, const int64_t *block_bytes,
+                      int num_pools, int num_layers, int num_blocks,
+                      const int32_t *sources, const int32_t *targets,
+                      int count, hipStream_t stream);
 
 #ifdef __cplusplus
 }

@@ -121,6 +121,35 @@ _SIGNATURES = {
          _c_ptr, _c_ptr, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_float, _c_ptr, _c_size, _c_ptr],
     ),
     "nvamd_paged_prefill_fp4_workspace_size": (_c_size, [_c_int, _c_int, _c_int, _c_int, _c_int, _c_int]),
+    "nvamd_kv_cache_write_fp8": (
+        _c_int,
+        [_c_ptr, _c_i64, _c_ptr, _c_i64, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_int, _c_ptr, _c_int, _c_int,
+         _c_int, _c_ptr],
+    ),
+    "nvamd_kv_cache_read_fp8": (
+        _c_int,
+        [_c_ptr, _c_i64, _c_ptr, _c_i64, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_int, _c_ptr, _c_int, _c_int,
+         _c_int, _c_ptr],
+    ),
+    "nvamd_qk_norm_rope_fp8": (
+        _c_int,
+        [_c_ptr, _c_i64, _c_ptr, _c_i64, _c_ptr, _c_i64, _c_ptr, _c_i64, _c_ptr, _c_i64, _c_ptr, _c_ptr, _c_ptr,
+         _c_ptr, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_int, _c_ptr, _c_int, _c_int, _c_int, _c_int,
+         _c_float, _c_ptr],
+    ),
+    "nvamd_paged_decode_fp8": (
+        _c_int,
+        [_c_ptr, _c_i64, _c_ptr, _c_i64, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_int, _c_ptr, _c_int, _c_int,
+         _c_ptr, _c_int, _c_int, _c_int, _c_int, _c_float, _c_int, _c_ptr, _c_size, _c_ptr],
+    ),
+    "nvamd_paged_prefill_fp8": (
+        _c_int,
+        [_c_ptr, _c_i64, _c_ptr, _c_i64, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_int, _c_ptr, _c_int, _c_int,
+         _c_ptr, _c_ptr, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_float, _c_ptr, _c_size, _c_ptr],
+    ),
+    "nvamd_paged_prefill_fp8_workspace_size": (_c_size, [_c_int, _c_int, _c_int, _c_int, _c_int, _c_int]),
+    "nvamd_copy_blocks": (
+        _c_int, [_c_ptr, _c_ptr, _c_int, _c_int, _c_int, _c_ptr, _c_ptr, _c_int, _c_ptr]),
     "nvamd_qk_norm_rope": (
         _c_int,
         [_c_ptr, _c_i64, _c_ptr, _c_i64, _c_ptr, _c_i64, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_ptr,
@@ -156,25 +185,27 @@ def load() -> ctypes.CDLL:
     return lib
 
 
-_calls = None  # csrc/calls.cpp: eager calls of the 4-bit cache, checked and made in one step; None: not usable here
+_calls = None  # csrc/calls.cpp: eager calls of the quantised caches, checked and made in one step; None: not usable here
 
 
 def _bind_calls(lib: ctypes.CDLL) -> None:
     """The library needs nothing of torch, the extension is tied to the torch that it was built with: without it the calls
     go through the checks in this file, with the same results."""
     global _calls
-    names = ("kv_cache_write_fp4", "kv_cache_read_fp4", "qk_norm_rope_fp4", "paged_decode_fp4",
-             "paged_decode_fused_fp4", "paged_prefill_fp4", "paged_prefill_fp4_workspace_size")
+    names = ("kv_cache_write_{}", "kv_cache_read_{}", "qk_norm_rope_{}", "paged_decode_{}", "paged_decode_fused_{}",
+             "paged_prefill_{}", "paged_prefill_{}_workspace_size")
     try:
         calls = importlib.import_module("._calls", __package__)
         if calls.ABI_VERSION != lib.nvamd_version():
             raise ImportError(f"built for version {calls.ABI_VERSION} of the C ABI, the library has {lib.nvamd_version()}")
     except ImportError as e:
         _calls = None
-        warnings.warn(f"eager calls of the 4-bit KV cache take some 5 us more each: {LIB_PATH.with_name('_calls.so')} cannot "
+        warnings.warn(f"eager calls of a quantised KV cache take some 5 us more each: {LIB_PATH.with_name('_calls.so')} cannot "
                       f"be used ({e}); `python -m nano_vllm_ascend_amd.build` builds it", RuntimeWarning, stacklevel=3)
         return
-    calls.bind(Fp4Pages, *(ctypes.cast(getattr(lib, f"nvamd_{n}"), ctypes.c_void_p).value for n in names))
+    for index, kind in enumerate((_FP4, _FP8)):
+        functions = (getattr(lib, "nvamd_" + n.format(kind.name), None) for n in names)
+        calls.bind(index, kind.pages, *(ctypes.cast(f, ctypes.c_void_p).value if f else 0 for f in functions))
     _calls = calls
 
 
@@ -604,10 +635,11 @@ def paged_prefill(out: torch.Tensor, q: torch.Tensor, key_cache: torch.Tensor, v
     return out
 
 
-# ------------------------------------------------------------------ KV cache held in 4 bits
-# The same path over pages of FP4 codes with a power-of-two scale per 32 dims (format and layout: nvamd.h).
+# ------------------------------------------------------------------ KV caches held in 4 and in 8 bits
+# The same path over pages of FP4 codes with a power-of-two scale per 32 dims, or of e4m3 codes with one per tile of 16
+# tokens (formats and layouts: nvamd.h).
 FP4_ROW_BYTES, FP4_ROW_SCALES = 64, 4  # of a head vector
-
+FP8_ROW_BYTES, FP8_TILE = 128, 16      # of a head vector; tokens that share a scale
 
 
 class Fp4Pages(NamedTuple):
@@ -624,18 +656,46 @@ class Fp4Pages(NamedTuple):
         return nb, bs, hkv, 2 * width
 
 
-def _fp4_pages(key_pages: Fp4Pages, value_pages: Fp4Pages):
+class Fp8Pages(NamedTuple):
+    """The keys or the values of one layer in 8 bits: ``codes`` uint8 [blocks, kv heads, block_size, 128] and ``scales``
+    uint8 [blocks, kv heads, block_size / 16], contiguous.  Pages are opaque (``kv_cache_read_fp8`` gives their values)."""
+
+    codes: torch.Tensor
+    scales: torch.Tensor
+
+    @property
+    def shape(self) -> tuple[int, int, int, int]:
+        """[blocks, block_size, kv heads, head_dim], as a bf16 cache of these pages has it."""
+        nb, hkv, bs, width = self.codes.shape
+        return nb, bs, hkv, width
+
+
+class _Kind(NamedTuple):
+    name: str        # of the entry points
+    pages: type
+    row_bytes: int   # codes of a head vector
+
+    def scales(self, nb: int, hkv: int, bs: int) -> tuple[int, ...]:
+        return (nb, hkv, bs, FP4_ROW_SCALES) if self.pages is Fp4Pages else (nb, hkv, bs // FP8_TILE)
+
+
+_FP4 = _Kind("fp4", Fp4Pages, FP4_ROW_BYTES)
+_FP8 = _Kind("fp8", Fp8Pages, FP8_ROW_BYTES)
+_HEAD_DIM = 128
+
+
+def _checked_pages(kind: _Kind, key_pages, value_pages):
     """Checks the pages of a layer; returns blocks, block_size, kv heads, their addresses and their device."""
-    if type(key_pages) is not Fp4Pages or type(value_pages) is not Fp4Pages:
-        raise ValueError("key and value pages must be Fp4Pages")
+    if type(key_pages) is not kind.pages or type(value_pages) is not kind.pages:
+        raise ValueError(f"key and value pages must be {kind.pages.__name__}")
     kc, ks = key_pages
     vc, vs = value_pages
     shape = kc.shape
-    if len(shape) != 4 or shape[3] != FP4_ROW_BYTES or vc.shape != shape:
-        raise ValueError(f"codes must be [blocks, kv heads, block_size, {FP4_ROW_BYTES}] for keys and values, got "
+    if len(shape) != 4 or shape[3] != kind.row_bytes or vc.shape != shape:
+        raise ValueError(f"codes must be [blocks, kv heads, block_size, {kind.row_bytes}] for keys and values, got "
                          f"{tuple(shape)} and {tuple(vc.shape)}")
     nb, hkv, bs, _ = shape
-    scales = (nb, hkv, bs, FP4_ROW_SCALES)
+    scales = kind.scales(nb, hkv, bs)
     if ks.shape != scales or vs.shape != scales:
         raise ValueError(f"scales must be {scales}, got {tuple(ks.shape)} and {tuple(vs.shape)}")
     u8 = torch.uint8
@@ -680,12 +740,25 @@ def _heads(name: str, t: torch.Tensor, rows: int, heads: int, d: int) -> int:
     return row if rows > 1 else max(row, heads * d)  # a single row's stride says nothing
 
 
-def _page_slots(slot_mapping: torch.Tensor, rows: int, num_slots: int) -> int:
+def check_tile_order(slot_mapping: torch.Tensor) -> None:
+    """Rows that go to one tile of the 8-bit cache follow one another, in the order of their slots, with no padding row
+    between them."""
+    sl = slot_mapping.detach().reshape(-1).cpu()
+    begins = sl >= 0
+    begins[1:] &= (sl[1:] != sl[:-1] + 1) | (sl[1:] % FP8_TILE == 0)
+    tiles = sl[begins] // FP8_TILE
+    if tiles.numel() != tiles.unique().numel():
+        raise IndexError("rows of a tile of 16 slots do not follow one another in the call, in the order of their slots")
+
+
+def _page_slots(slot_mapping: torch.Tensor, rows: int, num_slots: int, writes: _Kind | None = None) -> int:
     if (slot_mapping.dtype is not torch.int64 or slot_mapping.shape != (rows,) or not slot_mapping.is_contiguous()):
         raise ValueError(f"slot_mapping must be contiguous int64 [{rows}], got {slot_mapping.dtype} "
                          f"{tuple(slot_mapping.shape)}")
     if _range_checks and _checking():
         check_slots(slot_mapping, num_slots)
+        if writes is _FP8:
+            check_tile_order(slot_mapping)
     return slot_mapping.data_ptr()
 
 
@@ -699,36 +772,30 @@ def _made(answer, name: str) -> bool:
     return True
 
 
-def kv_cache_write_fp4(key_states: torch.Tensor, value_states: torch.Tensor, key_pages: Fp4Pages,
-                       value_pages: Fp4Pages, slot_mapping: torch.Tensor) -> None:
-    """Rows [T, Hkv, 128] of bf16 keys and values, quantised into the pages at their slots (-1: padding, skipped; no slot
-    twice in a call)."""
-    lib = _lib or load()
-    if _calls and not _range_checks and _made(
-            _calls.write(key_states, value_states, key_pages, value_pages, slot_mapping), "nvamd_kv_cache_write_fp4"):
+def _write(kind: _Kind, key_states, value_states, key_pages, value_pages, slot_mapping) -> None:
+    lib, name = _lib or load(), f"nvamd_kv_cache_write_{kind.name}"
+    if _calls and not _range_checks and type(key_pages) is kind.pages and _made(
+            _calls.write(key_states, value_states, key_pages, value_pages, slot_mapping), name):
         return
-    nb, bs, hkv, pages, device = _fp4_pages(key_pages, value_pages)
-    t, d = key_states.shape[0], 2 * FP4_ROW_BYTES
+    nb, bs, hkv, pages, device = _checked_pages(kind, key_pages, value_pages)
+    t, d = key_states.shape[0], _HEAD_DIM
     k_stride, v_stride = _heads("key_states", key_states, t, hkv, d), _heads("value_states", value_states, t, hkv, d)
-    slots = _page_slots(slot_mapping, t, nb * bs)
-    status = lib.nvamd_kv_cache_write_fp4(
+    slots = _page_slots(slot_mapping, t, nb * bs, kind)
+    status = getattr(lib, name)(
         key_states.data_ptr(), k_stride, value_states.data_ptr(), v_stride, *pages, nb, bs, slots, t, hkv, d,
         _stream_of(device, key_states, value_states, slot_mapping))
     if status:
-        _check(status, "nvamd_kv_cache_write_fp4")
+        _check(status, name)
 
 
-def kv_cache_read_fp4(key_pages: Fp4Pages, value_pages: Fp4Pages, slot_mapping: torch.Tensor,
-                      k_out: torch.Tensor | None = None,
-                      v_out: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
-    """The bf16 keys and values [T, Hkv, 128] that the pages hold at the slots (zeros for -1)."""
-    lib = _lib or load()
-    if _calls and not _range_checks and k_out is None and v_out is None:
+def _read(kind: _Kind, key_pages, value_pages, slot_mapping, k_out, v_out) -> tuple[torch.Tensor, torch.Tensor]:
+    lib, name = _lib or load(), f"nvamd_kv_cache_read_{kind.name}"
+    if _calls and not _range_checks and k_out is None and v_out is None and type(key_pages) is kind.pages:
         rows = _calls.read(key_pages, value_pages, slot_mapping)
-        if _made(rows, "nvamd_kv_cache_read_fp4"):
+        if _made(rows, name):
             return rows
-    nb, bs, hkv, pages, device = _fp4_pages(key_pages, value_pages)
-    t, d = slot_mapping.shape[0], 2 * FP4_ROW_BYTES
+    nb, bs, hkv, pages, device = _checked_pages(kind, key_pages, value_pages)
+    t, d = slot_mapping.shape[0], _HEAD_DIM
     slots = _page_slots(slot_mapping, t, nb * bs)
     k_stride = v_stride = hkv * d
     if k_out is None:
@@ -739,10 +806,10 @@ def kv_cache_read_fp4(key_pages: Fp4Pages, value_pages: Fp4Pages, slot_mapping: 
         v_out = torch.empty((t, hkv, d), dtype=torch.bfloat16, device=key_pages.codes.device)
     else:
         v_stride = _heads("v_out", v_out, t, hkv, d)
-    status = lib.nvamd_kv_cache_read_fp4(k_out.data_ptr(), k_stride, v_out.data_ptr(), v_stride, *pages, nb, bs, slots,
-                                         t, hkv, d, _stream_of(device, k_out, v_out, slot_mapping))
+    status = getattr(lib, name)(k_out.data_ptr(), k_stride, v_out.data_ptr(), v_stride, *pages, nb, bs, slots,
+                                t, hkv, d, _stream_of(device, k_out, v_out, slot_mapping))
     if status:
-        _check(status, "nvamd_kv_cache_read_fp4")
+        _check(status, name)
     return k_out, v_out
 
 
@@ -757,22 +824,16 @@ def _rope_args(q_weight, k_weight, positions, cos_sin, t: int, d: int) -> None:
         raise ValueError("cos_sin must be contiguous fp32 [max_positions, head_dim]")
 
 
-def qk_norm_rope_fp4(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_weight: torch.Tensor,
-                     k_weight: torch.Tensor, positions: torch.Tensor, cos_sin: torch.Tensor, eps: float,
-                     key_pages: Fp4Pages, value_pages: Fp4Pages, slot_mapping: torch.Tensor, *,
-                     q_out: torch.Tensor | None = None, k_out: torch.Tensor | None = None) -> torch.Tensor:
-    """RoPE(RMSNorm_head(x) * w) of q and k in one pass that also stores the rotated k and the raw v in the pages.
-
-    Returns the rotated q: ``q_out``, which may be q itself, or a new tensor.  The rotated k is written
-    only to the pages unless ``k_out`` (which may be k itself) asks for it.  64-bit arithmetic, one rounding to bf16."""
-    lib = _lib or load()
-    if _calls and not _range_checks:
+def _norm_rope(kind: _Kind, q, k, v, q_weight, k_weight, positions, cos_sin, eps, key_pages, value_pages, slot_mapping,
+               q_out, k_out) -> torch.Tensor:
+    lib, name = _lib or load(), f"nvamd_qk_norm_rope_{kind.name}"
+    if _calls and not _range_checks and type(key_pages) is kind.pages:
         rotated = _calls.rope(q, k, v, q_weight, k_weight, positions, cos_sin, eps, key_pages, value_pages, slot_mapping,
                               q_out, k_out)
-        if _made(rotated, "nvamd_qk_norm_rope_fp4"):
+        if _made(rotated, name):
             return rotated
-    nb, bs, hkv, pages, device = _fp4_pages(key_pages, value_pages)
-    d = 2 * FP4_ROW_BYTES
+    nb, bs, hkv, pages, device = _checked_pages(kind, key_pages, value_pages)
+    d = _HEAD_DIM
     if q.dim() != 3:
         raise ValueError(f"q must be [T, heads, D], got {tuple(q.shape)}")
     t, hq, _ = q.shape
@@ -787,24 +848,24 @@ def qk_norm_rope_fp4(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_weight
     if (qo_ptr == q_ptr and qo_stride != q_stride) or (ko_ptr == k_ptr and ko_stride != k_stride):
         raise ValueError("an output in place of its input must have the input's row stride")
     _rope_args(q_weight, k_weight, positions, cos_sin, t, d)
-    slots = _page_slots(slot_mapping, t, nb * bs)
+    slots = _page_slots(slot_mapping, t, nb * bs, kind)
     if _range_checks and _checking():
         check_positions(positions, cos_sin.shape[0])
-    status = lib.nvamd_qk_norm_rope_fp4(
+    status = getattr(lib, name)(
         qo_ptr, qo_stride, ko_ptr, ko_stride, q_ptr, q_stride, k_ptr, k_stride, v.data_ptr(), v_stride,
         q_weight.data_ptr(), k_weight.data_ptr(), positions.data_ptr(), cos_sin.data_ptr(), cos_sin.shape[0], *pages, nb,
         bs, slots, t, hq, hkv, d, float(eps),
         _stream_of(device, q, k, v, q_out, q if k_out is None else k_out, q_weight, k_weight, positions, cos_sin,
                    slot_mapping))
     if status:
-        _check(status, "nvamd_qk_norm_rope_fp4")
+        _check(status, name)
     return q_out
 
 
-def _fp4_attention_args(out, q, key_pages, value_pages, block_tables, seqs: int):
+def _attention_args(kind: _Kind, out, q, key_pages, value_pages, block_tables, seqs: int):
     """Checked arguments that decode and prefill share, up to the block tables; [heads, kv heads, head_dim]; the device."""
-    nb, bs, hkv, pages, device = _fp4_pages(key_pages, value_pages)
-    d = 2 * FP4_ROW_BYTES
+    nb, bs, hkv, pages, device = _checked_pages(kind, key_pages, value_pages)
+    d = _HEAD_DIM
     shape = q.shape
     if len(shape) != 3 or out.shape != shape:
         raise ValueError(f"q/out shape mismatch: {tuple(shape)} vs {tuple(out.shape)}")
@@ -832,7 +893,7 @@ def _fp4_attention_args(out, q, key_pages, value_pages, block_tables, seqs: int)
             bt_row, width), (hq, hkv, d), device
 
 
-def _fp4_decode_args(block_tables, context_lens, workspace, b: int) -> None:
+def _step_args(block_tables, context_lens, workspace, b: int) -> None:
     if block_tables.shape[0] != b:
         raise ValueError(f"block_tables must be int32 [{b}, W]")
     if context_lens.dtype is not torch.int32 or context_lens.shape != (b,) or not context_lens.is_contiguous():
@@ -841,30 +902,152 @@ def _fp4_decode_args(block_tables, context_lens, workspace, b: int) -> None:
         raise ValueError("workspace must be contiguous")
 
 
+def _decode(kind: _Kind, out, q, key_pages, value_pages, block_tables, context_lens, scale, max_context_len,
+            workspace) -> torch.Tensor:
+    lib, name = _lib or load(), f"nvamd_paged_decode_{kind.name}"
+    if _calls and not _range_checks and type(key_pages) is kind.pages:
+        made = _calls.decode(out, q, key_pages, value_pages, block_tables, context_lens, scale, max_context_len, workspace)
+        if _made(made, name):
+            return made
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    b = q.shape[0]
+    args, heads, device = _attention_args(kind, out, q, key_pages, value_pages, block_tables, b)
+    _step_args(block_tables, context_lens, workspace, b)
+    max_context_len = _int32("max_context_len", max_context_len)
+    if _range_checks and _checking():
+        check_paged_context(block_tables, context_lens, args[8], args[9], max_context_len)
+    status = getattr(lib, name)(*args, context_lens.data_ptr(), b, *heads, float(scale), max_context_len,
+                                workspace.data_ptr(), workspace.nbytes,
+                                _stream_of(device, q, out, block_tables, context_lens, workspace))
+    if status:
+        _check(status, name)
+    return out
+
+
+def _decode_fused(kind: _Kind, out, q, k, v, q_weight, k_weight, positions, cos_sin, eps, key_pages, value_pages,
+                  slot_mapping, block_tables, context_lens, scale, max_context_len, workspace) -> torch.Tensor:
+    lib, name = _lib or load(), f"nvamd_paged_decode_fused_{kind.name}"
+    if _calls and not _range_checks and type(key_pages) is kind.pages:
+        made = _calls.decode_fused(out, q, k, v, q_weight, k_weight, positions, cos_sin, eps, key_pages, value_pages,
+                                   slot_mapping, block_tables, context_lens, scale, max_context_len, workspace)
+        if _made(made, name):
+            return made
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    b = q.shape[0]
+    args, heads, device = _attention_args(kind, out, q, key_pages, value_pages, block_tables, b)
+    _step_args(block_tables, context_lens, workspace, b)
+    max_context_len = _int32("max_context_len", max_context_len)
+    nb, bs, (hq, hkv, d) = args[8], args[9], heads
+    k_stride, v_stride = _heads("k", k, b, hkv, d), _heads("v", v, b, hkv, d)
+    _rope_args(q_weight, k_weight, positions, cos_sin, b, d)
+    slots = _page_slots(slot_mapping, b, nb * bs, kind)
+    if _range_checks and _checking():
+        check_positions(positions, cos_sin.shape[0])
+        check_paged_context(block_tables, context_lens, nb, bs, max_context_len)
+    status = getattr(lib, name)(
+        *args[:4], k.data_ptr(), k_stride, v.data_ptr(), v_stride, q_weight.data_ptr(), k_weight.data_ptr(),
+        positions.data_ptr(), cos_sin.data_ptr(), cos_sin.shape[0], float(eps), *args[4:10], slots,
+        *args[10:], context_lens.data_ptr(), b, hq, hkv, d, float(scale), max_context_len, workspace.data_ptr(),
+        workspace.nbytes,
+        _stream_of(device, q, k, v, out, q_weight, k_weight, positions, cos_sin, slot_mapping, block_tables,
+                   context_lens, workspace))
+    if status:
+        _check(status, name)
+    return out
+
+
+def _prefill(kind: _Kind, out, q, key_pages, value_pages, block_tables, cu_seqlens_q, kv_lens, max_q_len,
+             scale) -> torch.Tensor:
+    lib, name = _lib or load(), f"nvamd_paged_prefill_{kind.name}"
+    if _calls and not _range_checks and type(key_pages) is kind.pages and _made(
+            _calls.prefill(out, q, key_pages, value_pages, block_tables, cu_seqlens_q, kv_lens, max_q_len, scale), name):
+        return out
+    if cu_seqlens_q.dtype is not torch.int32 or cu_seqlens_q.dim() != 1 or not cu_seqlens_q.is_contiguous():
+        raise ValueError("cu_seqlens_q must be contiguous int32 [n + 1]")
+    n = cu_seqlens_q.numel() - 1
+    args, heads, device = _attention_args(kind, out, q, key_pages, value_pages, block_tables, n)
+    if n < 0 or kv_lens.dtype is not torch.int32 or kv_lens.numel() < n or not kv_lens.is_contiguous():
+        raise ValueError("kv_lens must be contiguous int32, one per sequence")
+    max_q_len = _int32("max_q_len", max_q_len)
+    if _range_checks and _checking():
+        check_paged_context(block_tables[:n], kv_lens[:n], args[8], args[9])
+    stream = _stream_of(device, q, out, block_tables, cu_seqlens_q, kv_lens)
+    need = getattr(lib, f"{name}_workspace_size")(n, max_q_len, heads[0], heads[1], args[9], args[12])
+    space = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None  # freed behind the call
+    status = getattr(lib, name)(*args, cu_seqlens_q.data_ptr(), kv_lens.data_ptr(), n, q.shape[0], max_q_len,
+                                *heads, float(scale), space.data_ptr() if need else None, need, stream)
+    if status:
+        _check(status, name)
+    return out
+
+
+def kv_cache_write_fp4(key_states: torch.Tensor, value_states: torch.Tensor, key_pages: Fp4Pages,
+                       value_pages: Fp4Pages, slot_mapping: torch.Tensor) -> None:
+    """Rows [T, Hkv, 128] of bf16 keys and values, quantised into the pages at their slots (-1: padding, skipped; no slot
+    twice in a call)."""
+    _write(_FP4, key_states, value_states, key_pages, value_pages, slot_mapping)
+
+
+def kv_cache_write_fp8(key_states: torch.Tensor, value_states: torch.Tensor, key_pages: Fp8Pages,
+                       value_pages: Fp8Pages, slot_mapping: torch.Tensor) -> None:
+    """Rows [T, Hkv, 128] of bf16 keys and values, quantised into the pages at their slots (-1: padding, skipped).
+
+    The rows of a tile of 16 slots follow one another, in the order of their slots, as a sequence's tokens do; tiles come
+    in any order.  Rows that begin a tile set its scale and start it anew, others raise it where they need to and keep
+    what the tile holds."""
+    _write(_FP8, key_states, value_states, key_pages, value_pages, slot_mapping)
+
+
+def kv_cache_read_fp4(key_pages: Fp4Pages, value_pages: Fp4Pages, slot_mapping: torch.Tensor,
+                      k_out: torch.Tensor | None = None,
+                      v_out: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """The bf16 keys and values [T, Hkv, 128] that the pages hold at the slots (zeros for -1)."""
+    return _read(_FP4, key_pages, value_pages, slot_mapping, k_out, v_out)
+
+
+def kv_cache_read_fp8(key_pages: Fp8Pages, value_pages: Fp8Pages, slot_mapping: torch.Tensor,
+                      k_out: torch.Tensor | None = None,
+                      v_out: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """``kv_cache_read_fp4`` of pages of 8 bits (slots in any order)."""
+    return _read(_FP8, key_pages, value_pages, slot_mapping, k_out, v_out)
+
+
+def qk_norm_rope_fp4(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_weight: torch.Tensor,
+                     k_weight: torch.Tensor, positions: torch.Tensor, cos_sin: torch.Tensor, eps: float,
+                     key_pages: Fp4Pages, value_pages: Fp4Pages, slot_mapping: torch.Tensor, *,
+                     q_out: torch.Tensor | None = None, k_out: torch.Tensor | None = None) -> torch.Tensor:
+    """RoPE(RMSNorm_head(x) * w) of q and k in one pass that also stores the rotated k and the raw v in the pages.
+
+    Returns the rotated q: ``q_out``, which may be q itself, or a new tensor.  The rotated k is written
+    only to the pages unless ``k_out`` (which may be k itself) asks for it.  64-bit arithmetic, one rounding to bf16."""
+    return _norm_rope(_FP4, q, k, v, q_weight, k_weight, positions, cos_sin, eps, key_pages, value_pages, slot_mapping,
+                      q_out, k_out)
+
+
+def qk_norm_rope_fp8(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_weight: torch.Tensor,
+                     k_weight: torch.Tensor, positions: torch.Tensor, cos_sin: torch.Tensor, eps: float,
+                     key_pages: Fp8Pages, value_pages: Fp8Pages, slot_mapping: torch.Tensor, *,
+                     q_out: torch.Tensor | None = None, k_out: torch.Tensor | None = None) -> torch.Tensor:
+    """``qk_norm_rope_fp4`` into pages of 8 bits (rows in the order that ``kv_cache_write_fp8`` asks for)."""
+    return _norm_rope(_FP8, q, k, v, q_weight, k_weight, positions, cos_sin, eps, key_pages, value_pages, slot_mapping,
+                      q_out, k_out)
+
+
 def paged_decode_fp4(out: torch.Tensor | None, q: torch.Tensor, key_pages: Fp4Pages, value_pages: Fp4Pages,
                      block_tables: torch.Tensor, context_lens: torch.Tensor, scale: float, max_context_len: int,
                      workspace: torch.Tensor) -> torch.Tensor:
     """``paged_decode`` over pages of 4 bits; the workspace is the same (``alloc_paged_decode_workspace``).  Without
     ``out`` the result is a new tensor."""
-    lib = _lib or load()
-    if _calls and not _range_checks:
-        made = _calls.decode(out, q, key_pages, value_pages, block_tables, context_lens, scale, max_context_len, workspace)
-        if _made(made, "nvamd_paged_decode_fp4"):
-            return made
-    if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    b = q.shape[0]
-    args, heads, device = _fp4_attention_args(out, q, key_pages, value_pages, block_tables, b)
-    _fp4_decode_args(block_tables, context_lens, workspace, b)
-    max_context_len = _int32("max_context_len", max_context_len)
-    if _range_checks and _checking():
-        check_paged_context(block_tables, context_lens, args[8], args[9], max_context_len)
-    status = lib.nvamd_paged_decode_fp4(*args, context_lens.data_ptr(), b, *heads, float(scale), max_context_len,
-                                        workspace.data_ptr(), workspace.nbytes,
-                                        _stream_of(device, q, out, block_tables, context_lens, workspace))
-    if status:
-        _check(status, "nvamd_paged_decode_fp4")
-    return out
+    return _decode(_FP4, out, q, key_pages, value_pages, block_tables, context_lens, scale, max_context_len, workspace)
+
+
+def paged_decode_fp8(out: torch.Tensor | None, q: torch.Tensor, key_pages: Fp8Pages, value_pages: Fp8Pages,
+                     block_tables: torch.Tensor, context_lens: torch.Tensor, scale: float, max_context_len: int,
+                     workspace: torch.Tensor) -> torch.Tensor:
+    """``paged_decode_fp4`` over pages of 8 bits."""
+    return _decode(_FP8, out, q, key_pages, value_pages, block_tables, context_lens, scale, max_context_len, workspace)
 
 
 def paged_decode_fused_fp4(out: torch.Tensor | None, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
@@ -874,63 +1057,65 @@ def paged_decode_fused_fp4(out: torch.Tensor | None, q: torch.Tensor, k: torch.T
                            scale: float, max_context_len: int, workspace: torch.Tensor) -> torch.Tensor:
     """``qk_norm_rope_fp4`` and ``paged_decode_fp4`` in one launch, with the same bits: the step's k and v go to the slots
     of their sequences' last positions (-1: not stored), q, k and v stay as they are."""
-    lib = _lib or load()
-    if _calls and not _range_checks:
-        made = _calls.decode_fused(out, q, k, v, q_weight, k_weight, positions, cos_sin, eps, key_pages, value_pages,
-                                   slot_mapping, block_tables, context_lens, scale, max_context_len, workspace)
-        if _made(made, "nvamd_paged_decode_fused_fp4"):
-            return made
-    if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    b = q.shape[0]
-    args, heads, device = _fp4_attention_args(out, q, key_pages, value_pages, block_tables, b)
-    _fp4_decode_args(block_tables, context_lens, workspace, b)
-    max_context_len = _int32("max_context_len", max_context_len)
-    nb, bs, (hq, hkv, d) = args[8], args[9], heads
-    k_stride, v_stride = _heads("k", k, b, hkv, d), _heads("v", v, b, hkv, d)
-    _rope_args(q_weight, k_weight, positions, cos_sin, b, d)
-    slots = _page_slots(slot_mapping, b, nb * bs)
-    if _range_checks and _checking():
-        check_positions(positions, cos_sin.shape[0])
-        check_paged_context(block_tables, context_lens, nb, bs, max_context_len)
-    status = lib.nvamd_paged_decode_fused_fp4(
-        *args[:4], k.data_ptr(), k_stride, v.data_ptr(), v_stride, q_weight.data_ptr(), k_weight.data_ptr(),
-        positions.data_ptr(), cos_sin.data_ptr(), cos_sin.shape[0], float(eps), *args[4:10], slots,
-        *args[10:], context_lens.data_ptr(), b, hq, hkv, d, float(scale), max_context_len, workspace.data_ptr(),
-        workspace.nbytes,
-        _stream_of(device, q, k, v, out, q_weight, k_weight, positions, cos_sin, slot_mapping, block_tables,
-                   context_lens, workspace))
-    if status:
-        _check(status, "nvamd_paged_decode_fused_fp4")
-    return out
+    return _decode_fused(_FP4, out, q, k, v, q_weight, k_weight, positions, cos_sin, eps, key_pages, value_pages,
+                         slot_mapping, block_tables, context_lens, scale, max_context_len, workspace)
 
 
 def paged_prefill_fp4(out: torch.Tensor, q: torch.Tensor, key_pages: Fp4Pages, value_pages: Fp4Pages,
                       block_tables: torch.Tensor, cu_seqlens_q: torch.Tensor, kv_lens: torch.Tensor, max_q_len: int,
                       scale: float) -> torch.Tensor:
     """``paged_prefill`` over pages of 4 bits: queries are the last q_len of kv_len positions, all keys in the cache."""
+    return _prefill(_FP4, out, q, key_pages, value_pages, block_tables, cu_seqlens_q, kv_lens, max_q_len, scale)
+
+
+def paged_prefill_fp8(out: torch.Tensor, q: torch.Tensor, key_pages: Fp8Pages, value_pages: Fp8Pages,
+                      block_tables: torch.Tensor, cu_seqlens_q: torch.Tensor, kv_lens: torch.Tensor, max_q_len: int,
+                      scale: float) -> torch.Tensor:
+    """``paged_prefill`` over pages of 8 bits: queries are the last q_len of kv_len positions, all keys in the cache."""
+    return _prefill(_FP8, out, q, key_pages, value_pages, block_tables, cu_seqlens_q, kv_lens, max_q_len, scale)
+
+
+# ------------------------------------------------------------------ blocks of a cache
+COPY_MAX_POOLS = 8
+
+
+def check_block_pairs(sources: torch.Tensor, targets: torch.Tensor, num_blocks: int) -> None:
+    """Blocks of the pool, no target twice, none that another pair reads."""
+    src, dst = sources.detach().cpu().tolist(), targets.detach().cpu().tolist()
+    if any(not 0 <= b < num_blocks for b in src + dst):
+        raise IndexError(f"a block outside [0, {num_blocks}): {src} -> {dst}")
+    read = {s for s, d in zip(src, dst) if s != d}
+    if len(set(dst)) != len(dst) or read & set(dst):
+        raise IndexError(f"a block is a target twice, or a target and a source: {src} -> {dst}")
+
+
+def copy_blocks(pools, sources: torch.Tensor, targets: torch.Tensor) -> None:
+    """pool[:, targets[i]] = pool[:, sources[i]] of every pool, in one launch.
+
+    ``pools``: up to 8 contiguous tensors [layers, blocks, ...] of any type, with the same layers and blocks; sources and
+    targets: int32 [n] on the device.  No block is a target twice, or a target and another pair's source."""
     lib = _lib or load()
-    if _calls and not _range_checks and _made(
-            _calls.prefill(out, q, key_pages, value_pages, block_tables, cu_seqlens_q, kv_lens, max_q_len, scale),
-            "nvamd_paged_prefill_fp4"):
-        return out
-    if cu_seqlens_q.dtype is not torch.int32 or cu_seqlens_q.dim() != 1 or not cu_seqlens_q.is_contiguous():
-        raise ValueError("cu_seqlens_q must be contiguous int32 [n + 1]")
-    n = cu_seqlens_q.numel() - 1
-    args, heads, device = _fp4_attention_args(out, q, key_pages, value_pages, block_tables, n)
-    if n < 0 or kv_lens.dtype is not torch.int32 or kv_lens.numel() < n or not kv_lens.is_contiguous():
-        raise ValueError("kv_lens must be contiguous int32, one per sequence")
-    max_q_len = _int32("max_q_len", max_q_len)
+    pools = list(pools)
+    if not 0 < len(pools) <= COPY_MAX_POOLS:
+        raise ValueError(f"1 to {COPY_MAX_POOLS} pools, got {len(pools)}")
+    layers, blocks = pools[0].shape[:2] if pools[0].dim() > 2 else (0, 0)
+    device = pools[0].get_device()
+    for p in pools:
+        if p.dim() < 3 or p.shape[:2] != (layers, blocks) or not p.is_contiguous() or p.numel() == 0:
+            raise ValueError(f"pools must be contiguous [{layers}, {blocks}, ...] tensors, one is {tuple(p.shape)}")
+    n = sources.shape[0] if sources.dim() == 1 else -1
+    for name, t in (("sources", sources), ("targets", targets)):
+        if t.dtype is not torch.int32 or t.shape != (n,) or not t.is_contiguous():
+            raise ValueError(f"{name} must be contiguous int32 [n], got {t.dtype} {tuple(t.shape)}")
     if _range_checks and _checking():
-        check_paged_context(block_tables[:n], kv_lens[:n], args[8], args[9])
-    stream = _stream_of(device, q, out, block_tables, cu_seqlens_q, kv_lens)
-    need = lib.nvamd_paged_prefill_fp4_workspace_size(n, max_q_len, heads[0], heads[1], args[9], args[12])
-    space = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None  # freed behind the call
-    status = lib.nvamd_paged_prefill_fp4(*args, cu_seqlens_q.data_ptr(), kv_lens.data_ptr(), n, q.shape[0], max_q_len,
-                                         *heads, float(scale), space.data_ptr() if need else None, need, stream)
+        check_block_pairs(sources, targets, blocks)
+    stream = _stream_of(device, sources, targets, *pools)
+    at = (ctypes.c_void_p * len(pools))(*(p.data_ptr() for p in pools))
+    sizes = (ctypes.c_int64 * len(pools))(*(p.stride(1) * p.element_size() for p in pools))
+    status = lib.nvamd_copy_blocks(at, sizes, len(pools), layers, blocks, sources.data_ptr(), targets.data_ptr(), n,
+                                   stream)
     if status:
-        _check(status, "nvamd_paged_prefill_fp4")
-    return out
+        _check(status, "nvamd_copy_blocks")
 
 
 def add_rms_norm(delta: torch.Tensor | None, residual: torch.Tensor, weight: torch.Tensor, out: torch.Tensor,

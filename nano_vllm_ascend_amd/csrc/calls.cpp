@@ -1,4 +1,4 @@
-// The eager calls of the 4-bit cache from Python: arguments checked and read, outputs made and the C ABI called in one
+// The eager calls of the 4-bit and 8-bit caches from Python: arguments checked and read, outputs made and the C ABI called in one
 // step. A small batch's eager call is bound by the host: a launch costs it some 3.6 us, and checking 5 to 15 tensors
 // attribute by attribute from Python another 4 to 5, with 1 for ctypes (decode of 4 x U[1, 512] through the layer: 12.7
 // us, so 8.1; a row written and read back 18.5, 9.0).
@@ -19,16 +19,22 @@
 
 namespace {
 
-constexpr int64_t kHeadDim = 128, kRowBytes = 64, kRowScales = 4;
+constexpr int64_t kHeadDim = 128;
+constexpr int64_t kFp4RowBytes = 64, kFp4RowScales = 4, kFp8Tile = 16;
 
-decltype(&nvamd_kv_cache_write_fp4) f_write;
-decltype(&nvamd_kv_cache_read_fp4) f_read;
-decltype(&nvamd_qk_norm_rope_fp4) f_rope;
-decltype(&nvamd_paged_decode_fp4) f_decode;
-decltype(&nvamd_paged_decode_fused_fp4) f_fused;
-decltype(&nvamd_paged_prefill_fp4) f_prefill;
-decltype(&nvamd_paged_prefill_fp4_workspace_size) f_prefill_space;
-PyTypeObject *pages_type;  // _C.Fp4Pages
+// The entry points of a kind of pages; those of the 8-bit cache have the same signatures.
+struct Kind {
+  PyTypeObject *pages;  // _C.Fp4Pages, _C.Fp8Pages
+  decltype(&nvamd_kv_cache_write_fp4) write;
+  decltype(&nvamd_kv_cache_read_fp4) read;
+  decltype(&nvamd_qk_norm_rope_fp4) rope;
+  decltype(&nvamd_paged_decode_fp4) decode;
+  decltype(&nvamd_paged_decode_fused_fp4) fused;
+  decltype(&nvamd_paged_prefill_fp4) prefill;
+  decltype(&nvamd_paged_prefill_fp4_workspace_size) prefill_space;
+};
+constexpr int kFp4 = 0, kFp8 = 1;
+Kind kinds[2];  // by the bytes of a head vector: 64, 128
 
 struct Irregular {};  // thrown: answer None
 
@@ -54,6 +60,7 @@ const at::Tensor &dense(PyObject *o, int &device, at::ScalarType type) {
 struct Pages {
   void *kc, *ks, *vc, *vs;
   int64_t nb, bs, hkv;
+  const Kind &kind;
 };
 
 int narrow(int64_t v) {
@@ -62,15 +69,17 @@ int narrow(int64_t v) {
 }
 
 Pages pages(PyObject *keys, PyObject *values, int &device) {
-  need(Py_TYPE(keys) == pages_type && Py_TYPE(values) == pages_type);
+  const int is = Py_TYPE(keys) == kinds[kFp4].pages ? kFp4 : kFp8;
+  need(Py_TYPE(keys) == kinds[is].pages && Py_TYPE(values) == kinds[is].pages);
   const at::Tensor &kc = dense(PyTuple_GET_ITEM(keys, 0), device, at::kByte);
   const at::Tensor &ks = dense(PyTuple_GET_ITEM(keys, 1), device, at::kByte);
   const at::Tensor &vc = dense(PyTuple_GET_ITEM(values, 0), device, at::kByte);
   const at::Tensor &vs = dense(PyTuple_GET_ITEM(values, 1), device, at::kByte);
-  need(kc.dim() == 4 && kc.size(3) == kRowBytes && vc.sizes() == kc.sizes());
-  need(ks.dim() == 4 && ks.size(0) == kc.size(0) && ks.size(1) == kc.size(1) && ks.size(2) == kc.size(2) &&
-       ks.size(3) == kRowScales && vs.sizes() == ks.sizes());
-  return {kc.data_ptr(), ks.data_ptr(), vc.data_ptr(), vs.data_ptr(), kc.size(0), kc.size(2), kc.size(1)};
+  need(kc.dim() == 4 && kc.size(3) == (is == kFp4 ? kFp4RowBytes : kHeadDim) && vc.sizes() == kc.sizes());
+  need(ks.dim() == (is == kFp4 ? 4 : 3) && ks.size(0) == kc.size(0) && ks.size(1) == kc.size(1) &&
+       vs.sizes() == ks.sizes());
+  need(is == kFp4 ? ks.size(2) == kc.size(2) && ks.size(3) == kFp4RowScales : ks.size(2) * kFp8Tile == kc.size(2));
+  return {kc.data_ptr(), ks.data_ptr(), vc.data_ptr(), vs.data_ptr(), kc.size(0), kc.size(2), kc.size(1), kinds[is]};
 }
 
 struct Rows {
@@ -179,7 +188,7 @@ PyObject *write(PyObject *const *a) {
   const int nb = narrow(c.nb), bs = narrow(c.bs), t = narrow(k.rows), hkv = narrow(c.hkv);
   hipStream_t s = stream_on(dev);
   const int status = call([&] {
-    return f_write(k.p, k.stride, v.p, v.stride, c.kc, c.ks, c.vc, c.vs, nb, bs, slots, t, hkv, kHeadDim, s);
+    return c.kind.write(k.p, k.stride, v.p, v.stride, c.kc, c.ks, c.vc, c.vs, nb, bs, slots, t, hkv, kHeadDim, s);
   });
   return status ? PyLong_FromLong(status) : same(Py_True);
 }
@@ -195,7 +204,7 @@ PyObject *read(PyObject *const *a) {
   at::Tensor k = empty({t, c.hkv, kHeadDim}, at::kBFloat16, dev), v = empty({t, c.hkv, kHeadDim}, at::kBFloat16, dev);
   const int64_t stride = c.hkv * kHeadDim;
   const int status = call([&] {
-    return f_read(k.data_ptr(), stride, v.data_ptr(), stride, c.kc, c.ks, c.vc, c.vs, nb, bs, slots, n, hkv, kHeadDim, s);
+    return c.kind.read(k.data_ptr(), stride, v.data_ptr(), stride, c.kc, c.ks, c.vc, c.vs, nb, bs, slots, n, hkv, kHeadDim, s);
   });
   if (status) return PyLong_FromLong(status);
   return Py_BuildValue("(NN)", THPVariable_Wrap(std::move(k)), THPVariable_Wrap(std::move(v)));
@@ -220,7 +229,7 @@ PyObject *rope(PyObject *const *a) {
   const Rows qo = result(a[11], dev, q, made);
   need(qo.p != q.p || qo.stride == q.stride);
   const int status = call([&] {
-    return f_rope(qo.p, qo.stride, ko.p, ko.stride, q.p, q.stride, k.p, k.stride, v.p, v.stride, r.qw, r.kw,
+    return c.kind.rope(qo.p, qo.stride, ko.p, ko.stride, q.p, q.stride, k.p, k.stride, v.p, v.stride, r.qw, r.kw,
                   r.positions, r.table, r.rows, c.kc, c.ks, c.vc, c.vs, nb, bs, slots, t, hq, hkv, kHeadDim, r.eps, s);
   });
   if (status) return PyLong_FromLong(status);
@@ -244,7 +253,7 @@ PyObject *decode(PyObject *const *a) {
   at::Tensor made;
   const Rows out = result(a[0], dev, q, made);
   const int status = call([&] {
-    return f_decode(out.p, out.stride, q.p, q.stride, c.kc, c.ks, c.vc, c.vs, nb, bs, bt.p, bt.stride, bt.width, lens, t,
+    return c.kind.decode(out.p, out.stride, q.p, q.stride, c.kc, c.ks, c.vc, c.vs, nb, bs, bt.p, bt.stride, bt.width, lens, t,
                     hq, hkv, kHeadDim, scale, most, space.data_ptr(), space.nbytes(), s);
   });
   if (status) return PyLong_FromLong(status);
@@ -270,7 +279,7 @@ PyObject *decode_fused(PyObject *const *a) {
   at::Tensor made;
   const Rows out = result(a[0], dev, q, made);
   const int status = call([&] {
-    return f_fused(out.p, out.stride, q.p, q.stride, k.p, k.stride, v.p, v.stride, r.qw, r.kw, r.positions, r.table, r.rows,
+    return c.kind.fused(out.p, out.stride, q.p, q.stride, k.p, k.stride, v.p, v.stride, r.qw, r.kw, r.positions, r.table, r.rows,
                    r.eps, c.kc, c.ks, c.vc, c.vs, nb, bs, slots, bt.p, bt.stride, bt.width, lens, t, hq, hkv, kHeadDim,
                    scale, most, space.data_ptr(), space.nbytes(), s);
   });
@@ -291,12 +300,12 @@ PyObject *prefill(PyObject *const *a) {
   const float scale = number(a[8]);
   const int nb = narrow(c.nb), bs = narrow(c.bs), t = narrow(q.rows), hq = narrow(q.heads), hkv = narrow(c.hkv);
   hipStream_t s = stream_on(dev);
-  const size_t bytes = f_prefill_space(n, most, hq, hkv, bs, bt.width);
+  const size_t bytes = c.kind.prefill_space(n, most, hq, hkv, bs, bt.width);
   at::Tensor space;
   if (bytes) space = empty({(int64_t)bytes}, at::kByte, dev);  // freed behind the call on its stream
   void *p = bytes ? space.data_ptr() : nullptr;
   const int status = call([&] {
-    return f_prefill(out.p, out.stride, q.p, q.stride, c.kc, c.ks, c.vc, c.vs, nb, bs, bt.p, bt.stride, bt.width, cu, lens,
+    return c.kind.prefill(out.p, out.stride, q.p, q.stride, c.kc, c.ks, c.vc, c.vs, nb, bs, bt.p, bt.stride, bt.width, cu, lens,
                      n, t, most, hq, hkv, kHeadDim, scale, p, bytes, s);
   });
   return status ? PyLong_FromLong(status) : same(a[0]);
@@ -304,7 +313,7 @@ PyObject *prefill(PyObject *const *a) {
 
 template <PyObject *(*F)(PyObject *const *), Py_ssize_t N>
 PyObject *entry(PyObject *, PyObject *const *args, Py_ssize_t n) {
-  if (n != N || pages_type == nullptr) Py_RETURN_NONE;
+  if (n != N) Py_RETURN_NONE;
   try {
     return F(args);
   } catch (const Irregular &) {
@@ -315,22 +324,28 @@ PyObject *entry(PyObject *, PyObject *const *args, Py_ssize_t n) {
   }
 }
 
-// (Fp4Pages, addresses of the functions above)
+// (index, type of the pages, addresses of its entry points)
 PyObject *bind(PyObject *, PyObject *args) {
+  int index;
   PyObject *type;
   unsigned long long p[7];
-  if (!PyArg_ParseTuple(args, "O!KKKKKKK", &PyType_Type, &type, &p[0], &p[1], &p[2], &p[3], &p[4], &p[5], &p[6]))
+  if (!PyArg_ParseTuple(args, "iO!KKKKKKK", &index, &PyType_Type, &type, &p[0], &p[1], &p[2], &p[3], &p[4], &p[5], &p[6]))
     return nullptr;
-  f_write = reinterpret_cast<decltype(f_write)>(p[0]);
-  f_read = reinterpret_cast<decltype(f_read)>(p[1]);
-  f_rope = reinterpret_cast<decltype(f_rope)>(p[2]);
-  f_decode = reinterpret_cast<decltype(f_decode)>(p[3]);
-  f_fused = reinterpret_cast<decltype(f_fused)>(p[4]);
-  f_prefill = reinterpret_cast<decltype(f_prefill)>(p[5]);
-  f_prefill_space = reinterpret_cast<decltype(f_prefill_space)>(p[6]);
+  if (index != kFp4 && index != kFp8) {
+    PyErr_SetString(PyExc_ValueError, "no such kind of pages");
+    return nullptr;
+  }
+  Kind &k = kinds[index];
+  k.write = reinterpret_cast<decltype(k.write)>(p[0]);
+  k.read = reinterpret_cast<decltype(k.read)>(p[1]);
+  k.rope = reinterpret_cast<decltype(k.rope)>(p[2]);
+  k.decode = reinterpret_cast<decltype(k.decode)>(p[3]);
+  k.fused = reinterpret_cast<decltype(k.fused)>(p[4]);
+  k.prefill = reinterpret_cast<decltype(k.prefill)>(p[5]);
+  k.prefill_space = reinterpret_cast<decltype(k.prefill_space)>(p[6]);
   Py_INCREF(type);
-  Py_XDECREF(reinterpret_cast<PyObject *>(pages_type));
-  pages_type = reinterpret_cast<PyTypeObject *>(type);
+  Py_XDECREF(reinterpret_cast<PyObject *>(k.pages));
+  k.pages = reinterpret_cast<PyTypeObject *>(type);
   Py_RETURN_NONE;
 }
 

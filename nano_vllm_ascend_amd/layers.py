@@ -8,8 +8,8 @@ The ``Npu*`` names are kept as aliases so code written against the reference
 imports unchanged.  ``qk_norm_rope`` fuses q_norm, k_norm, RoPE and the KV
 store (nv/models/qwen3.py:83-96) into one kernel.
 
-Each takes either kind of cache: a PagedKVCache (bf16 tensors) or an
-Fp4PagedKVCache, whose layers are ``Fp4Pages`` of 4-bit codes and scales.
+Each takes any kind of cache: a PagedKVCache (bf16 tensors), an Fp4PagedKVCache or
+an Fp8PagedKVCache, whose layers are ``Fp4Pages`` or ``Fp8Pages`` of codes and scales.
 """
 from __future__ import annotations
 
@@ -69,6 +69,10 @@ def qk_norm_rope(q, k, v, q_norm: RMSNorm, k_norm: RMSNorm, rotary: RotaryEmbedd
             _C.qk_norm_rope_fp4(q, k, v, q_norm.weight, k_norm.weight, positions, rotary.cos_sin,
                                 q_norm.variance_epsilon, kc, vc, slot_mapping, q_out=q, k_out=k)
             return
+        if isinstance(kc, _C.Fp8Pages):
+            _C.qk_norm_rope_fp8(q, k, v, q_norm.weight, k_norm.weight, positions, rotary.cos_sin,
+                                q_norm.variance_epsilon, kc, vc, slot_mapping, q_out=q, k_out=k)
+            return
     _C.qk_norm_rope(q, k, q_norm.weight, k_norm.weight, positions, rotary.cos_sin, q_norm.variance_epsilon,
                     v=v if kc is not None else None, key_cache=kc, value_cache=vc,
                     slot_mapping=slot_mapping if kc is not None else None)
@@ -120,6 +124,9 @@ class HipPagedAttention(nn.Module):
         if isinstance(key_cache, _C.Fp4Pages):
             return _C.paged_decode_fp4(out, q, key_cache, value_cache, block_tables, context_lens, self.scale,
                                        max_context_len, workspace)
+        if isinstance(key_cache, _C.Fp8Pages):
+            return _C.paged_decode_fp8(out, q, key_cache, value_cache, block_tables, context_lens, self.scale,
+                                       max_context_len, workspace)
         out = torch.empty_like(q) if out is None else out
         return _C.paged_decode(out, q, key_cache, value_cache, block_tables, context_lens, self.scale,
                                max_context_len, workspace)
@@ -147,6 +154,11 @@ class HipPagedAttention(nn.Module):
             return _C.paged_decode_fused_fp4(out, q, k, v, q_norm.weight, k_norm.weight, positions, rotary.cos_sin,
                                              q_norm.variance_epsilon, key_cache, value_cache, slot_mapping,
                                              block_tables, context_lens, self.scale, max_context_len, workspace)
+        if isinstance(key_cache, _C.Fp8Pages):
+            rotated = _C.qk_norm_rope_fp8(q, k, v, q_norm.weight, k_norm.weight, positions, rotary.cos_sin,
+                                          q_norm.variance_epsilon, key_cache, value_cache, slot_mapping)
+            return _C.paged_decode_fp8(out, rotated, key_cache, value_cache, block_tables, context_lens, self.scale,
+                                       max_context_len, workspace)
         out = torch.empty_like(q) if out is None else out
         return _C.paged_decode_fused(out, q, k, v, q_norm.weight, k_norm.weight, positions, rotary.cos_sin,
                                      q_norm.variance_epsilon, key_cache, value_cache, slot_mapping, block_tables,
@@ -184,6 +196,9 @@ class HipBatchPrefillAttention(nn.Module):
                 raise ValueError("paged prefill requires physical key/value cache")
             if isinstance(key_cache, _C.Fp4Pages):
                 return _C.paged_prefill_fp4(out, q, key_cache, value_cache, attn_metadata.block_tables,
+                                            attn_metadata.cu_seqlens_q, attn_metadata.context_lens, max_q, self.scale)
+            if isinstance(key_cache, _C.Fp8Pages):
+                return _C.paged_prefill_fp8(out, q, key_cache, value_cache, attn_metadata.block_tables,
                                             attn_metadata.cu_seqlens_q, attn_metadata.context_lens, max_q, self.scale)
             return _C.paged_prefill(out, q, key_cache, value_cache, attn_metadata.block_tables,
                                     attn_metadata.cu_seqlens_q, attn_metadata.context_lens, max_q, self.scale)

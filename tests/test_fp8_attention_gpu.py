@@ -1,0 +1,665 @@
+"""Attention over the KV cache held in 8 bits, against the 64-bit oracle on the values that the pages hold.
+
+Tolerances are the bound that oracle.fp4_ref.attention derives for each element from the roundings that an evaluation with
+bf16 weights and results makes."""
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+from nano_vllm_ascend_amd import _C
+from nano_vllm_ascend_amd.layers import HipPagedAttention
+from nano_vllm_ascend_amd.paged_kv_cache import Fp8PagedKVCache
+from oracle import fp4_ref, fp8_ref
+
+pytestmark = pytest.mark.gpu
+SCALE = 128 ** -0.5
+
+
+@pytest.fixture(autouse=True)
+def clean_word(device):
+    _C.clear_index_errors()
+    yield
+    _C.clear_index_errors()
+    torch.cuda.synchronize()
+
+
+class Batch:
+    """Sequences of the given contexts in pages of a seeded order; rows past a context and pages of nobody hold stale bytes,
+    codes and scales of NaN among them."""
+
+    def __init__(self, device, lens, hq, hkv, bs, seed=0, spread=0.5, extra_width=0):
+        gen = torch.Generator().manual_seed(seed)
+        need = [-(-n // bs) for n in lens]
+        self.nb = sum(need) + 2
+        order = torch.randperm(self.nb, generator=gen)
+        self.tables = torch.zeros(len(lens), max(max(need), 1) + extra_width, dtype=torch.int32)
+        at = 0
+        for i, n in enumerate(need):
+            self.tables[i, :n] = order[at:at + n]
+            at += n
+        self.pages = tuple(torch.randint(0, 256, p.shape, generator=gen, dtype=torch.uint8)
+                           for p in fp8_ref.empty_pages(self.nb, hkv, bs))
+        for p in self.pages[1::2]:
+            p[p > 200] = 255
+        self.slots = [self.tables[i, torch.arange(n) // bs].long() * bs + torch.arange(n) % bs
+                      for i, n in enumerate(lens)]
+        slots = torch.cat(self.slots)
+        k, v = (torch.randn(len(slots), hkv, 128, generator=gen) for _ in range(2))
+        k = k * torch.exp(spread * torch.randn(len(slots), hkv, 1, generator=gen))
+        fp8_ref.write_sequences(self.pages, k.bfloat16(), v.bfloat16(), slots)
+        self.lens, self.hq, self.hkv, self.bs, self.device, self.gen = lens, hq, hkv, bs, device, gen
+        self.upload()
+
+    def upload(self):
+        kc, ks, vc, vs = (p.to(self.device) for p in self.pages)
+        self.keys, self.values = _C.Fp8Pages(kc, ks), _C.Fp8Pages(vc, vs)
+
+    def queries(self, t, scale=1.0):
+        return (scale * torch.randn(t, self.hq, 128, generator=self.gen)).bfloat16()
+
+    def want(self, i, q, scale=SCALE):
+        """The last len(q) positions of sequence i."""
+        k, v = fp8_ref.read_sequence(self.pages, self.slots[i])
+        return fp4_ref.attention(q, k, v, scale)
+
+    def decode(self, q, bound=None, scale=SCALE, out=None, workspace=None):
+        bound = bound or max(max(self.lens), 1)
+        if workspace is None:
+            workspace = _C.alloc_paged_decode_workspace(len(self.lens), self.hq, self.hkv, bound, self.device)
+        out = torch.full(q.shape, 7.0, dtype=torch.bfloat16, device=self.device) if out is None else out
+        return _C.paged_decode_fp8(out, q.to(self.device), self.keys, self.values, self.tables.to(self.device),
+                                   torch.tensor(self.lens, dtype=torch.int32, device=self.device), scale, bound,
+                                   workspace)
+
+    def prefill(self, q, q_lens, out=None, max_q=None, scale=SCALE):
+        cu = torch.tensor([0] + q_lens).cumsum(0).to(torch.int32).to(self.device)
+        out = torch.full(q.shape, 7.0, dtype=torch.bfloat16, device=self.device) if out is None else out
+        if max_q == "strips":
+            max_q = 65536 // (self.hq * len(self.lens))
+        return _C.paged_prefill_fp8(out, q.to(self.device), self.keys, self.values, self.tables.to(self.device), cu,
+                                    torch.tensor(self.lens, dtype=torch.int32, device=self.device),
+                                    max_q or max(q_lens), scale)
+
+
+def close(got, want, tol):
+    got = got.cpu().double()
+    assert torch.equal(got.isnan(), want.isnan())
+    off = ((got - want).abs() - tol).nan_to_num(-1.0)
+    assert off.max().item() <= 0, f"off by {off.max().item():.3g} over the bound at {off.argmax().item()}"
+
+
+def check_decode(batch, q, got, scale=SCALE):
+    for i, n in enumerate(batch.lens):
+        if n == 0:
+            assert not got[i].any()
+            continue
+        close(got[i:i + 1], *batch.want(i, q[i:i + 1], scale))
+
+
+# -------------------------------------------------------------------------------------------- decode
+@pytest.mark.parametrize("hq, hkv", [(1, 1), (2, 1), (16, 8), (6, 2), (4, 1), (5, 1), (16, 2), (15, 1), (16, 1), (17, 1),
+                                     (40, 2)])
+def test_decode_head_layouts(device, hq, hkv):
+    batch = Batch(device, [1, 300, 0, 77, 64], hq, hkv, 32, seed=hq)
+    q = batch.queries(5)
+    check_decode(batch, q, batch.decode(q))
+    assert _C.index_errors() == 0
+
+
+@pytest.mark.parametrize("bs", [16, 32, 64, 128, 256])
+def test_decode_contexts_around_tiles_pages_and_partitions(device, bs):
+    lens = [1, 2, 15, 16, 17, 31, 32, 33, 63, 64, 65, 127, 128, 129, 255, 256, 257, 511, 512, 513, 1023, 1024, 1025]
+    batch = Batch(device, lens, 4, 2, bs, seed=bs)
+    q = batch.queries(len(lens))
+    check_decode(batch, q, batch.decode(q))
+    check_decode(batch, q, batch.decode(q, bound=8192))  # a bound far past the contexts
+
+
+@pytest.mark.parametrize("lens, hq, hkv", [([5000, 3], 2, 1), ([9001, 1, 0, 4097], 4, 2), ([40960], 2, 1),
+                                           ([70000, 131072], 1, 1)])
+def test_decode_long_contexts(device, lens, hq, hkv):
+    batch = Batch(device, lens, hq, hkv, 128, seed=1)
+    q = batch.queries(len(lens))
+    check_decode(batch, q, batch.decode(q))
+
+
+def test_decode_many_sequences(device):
+    """More sequences than a wave's lanes, and enough partitions that they grow past the smallest."""
+    gen = torch.Generator().manual_seed(3)
+    lens = [int(x) for x in torch.randint(0, 700, (150,), generator=gen)]
+    batch = Batch(device, lens, 2, 2, 16, seed=4)
+    q = batch.queries(150)
+    check_decode(batch, q, batch.decode(q))
+    lens = [2600 + i for i in range(70)]
+    batch = Batch(device, lens, 4, 4, 128, seed=5)  # 70 x 11 x 4 partitions of 256 tokens, were they that small
+    q = batch.queries(70)
+    check_decode(batch, q, batch.decode(q, bound=4096))
+
+
+def test_decode_of_the_largest_batches(device):
+    """16,384 units of a sequence and a kv head: each sequence's bits are those of a small batch."""
+    gen = torch.Generator().manual_seed(39)
+    lens = [int(x) for x in torch.randint(0, 40, (2048,), generator=gen)]
+    batch = Batch(device, lens, 8, 8, 16, seed=40)
+    q = batch.queries(2048)
+    got = batch.decode(q, bound=4096)
+    tables, dq, n = batch.tables.to(device), q.to(device), torch.tensor(lens, dtype=torch.int32, device=device)
+    space = _C.alloc_paged_decode_workspace(100, 8, 8, 64, device)
+    for at in (0, 1000, 1948):
+        rows = slice(at, at + 100)
+        few = _C.paged_decode_fp8(None, dq[rows], batch.keys, batch.values, tables[rows], n[rows], SCALE, 64, space)
+        assert torch.equal(few, got[rows])
+    for i in (0, 1, 1023, 2047):
+        if lens[i]:
+            close(got[i:i + 1], *batch.want(i, q[i:i + 1]))
+    assert not got[n == 0].any() and _C.index_errors() == 0
+
+
+def at_scale(batch, k_exp, v_exp):
+    """The batch's rows with keys and values of about 2^k_exp and 2^v_exp."""
+    slots = torch.cat(batch.slots)
+    k, v = fp8_ref.read_sequence(batch.pages, slots)
+    fp8_ref.write_sequences(batch.pages, (k * 2.0 ** k_exp).bfloat16(), (v * 2.0 ** v_exp).bfloat16(), slots)
+    batch.upload()
+
+
+EXPONENTS = pytest.mark.parametrize("q_exp, k_exp, v_exp", [(100, -100, 0), (-90, 90, 90), (-60, 60, -90), (0, 0, 100)])
+
+
+@EXPONENTS
+def test_decode_of_numbers_far_from_one(device, q_exp, k_exp, v_exp):
+    batch = Batch(device, [1, 70, 600], 4, 2, 32, seed=41)
+    at_scale(batch, k_exp, v_exp)
+    q = batch.queries(3, scale=2.0 ** q_exp)
+    check_decode(batch, q, batch.decode(q))
+
+
+@pytest.mark.parametrize("hq, hkv", [(2, 1), (16, 8), (12, 2)])
+def test_decode_beside_other_sequences(device, hq, hkv):
+    """Contexts of up to 512 tokens give the same bits whatever runs beside them; of longer ones the cut, and with it the
+    order of the sums, follows from all contexts of the call, within the bound."""
+    lens = [512, 1, 3000, 200, 513, 5000] + [700] * 40
+    batch = Batch(device, lens, hq, hkv, 64, seed=36)
+    q = batch.queries(len(lens))
+    whole = batch.decode(q)
+    check_decode(batch, q, whole)
+    tables, dq = batch.tables.to(device), q.to(device)
+    for i in range(6):
+        n = torch.tensor(lens[i:i + 1], dtype=torch.int32, device=device)
+        space = _C.alloc_paged_decode_workspace(1, hq, hkv, 5000, device)
+        alone = _C.paged_decode_fp8(None, dq[i:i + 1], batch.keys, batch.values, tables[i:i + 1], n, SCALE, 5000, space)
+        close(alone, *batch.want(i, q[i:i + 1]))
+        if lens[i] <= 512:
+            assert torch.equal(alone[0], whole[i])
+
+
+def test_decode_scores_far_apart(device):
+    """A few keys carry all of the weight, in whichever partition they are; large and negative scales."""
+    batch = Batch(device, [1500, 700], 4, 1, 64, seed=6, spread=1.5)
+    q = batch.queries(2, scale=8.0)
+    check_decode(batch, q, batch.decode(q))
+    check_decode(batch, q, batch.decode(q, scale=-0.05), scale=-0.05)
+
+
+def outliers(q):
+    """A dim that is thousands of times the others, as some heads have."""
+    q = q.clone()
+    q[..., 5] *= 4000
+    q[..., 100] *= 70
+    return q
+
+
+def test_decode_queries_with_outliers(device):
+    """Keys without the outliers' dims: the scores come from what is left of the query."""
+    batch = Batch(device, [900, 70], 4, 1, 64, seed=16)
+    slots = torch.cat(batch.slots)
+    k, v = fp8_ref.read_sequence(batch.pages, slots)
+    k[..., 5] = k[..., 100] = 0
+    fp8_ref.write_sequences(batch.pages, k.bfloat16(), v.bfloat16(), slots)
+    batch.upload()
+    q = outliers(batch.queries(2))
+    check_decode(batch, q, batch.decode(q))
+
+
+def test_decode_scores_below_any_reference(device):
+    """Scores of about -1e31, all alike: every key weighs the same."""
+    batch = Batch(device, [700, 40], 2, 1, 16, seed=17)
+    slots = torch.cat(batch.slots)
+    _, v = fp8_ref.read_sequence(batch.pages, slots)
+    fp8_ref.write_sequences(batch.pages, torch.full((len(slots), 1, 128), -(2.0 ** 50)).bfloat16(), v.bfloat16(), slots)
+    batch.upload()
+    q = torch.full((2, 2, 128), 2.0 ** 50).bfloat16()
+    got = batch.decode(q).cpu().double()
+    for i, at in enumerate(batch.slots):
+        _, v = fp8_ref.read_sequence(batch.pages, at)
+        # equal weights are exact; 32-bit sums of up to 700 values, and one rounding
+        tol = 2.0 ** -8 * v.mean(0).abs() + 1e-4 * v.abs().mean(0)
+        assert ((got[i] - v.mean(0)).abs() <= tol).all()
+
+
+def test_decode_replays_from_a_graph(device):
+    """Contexts, tables and queries that change between the replays of a captured call."""
+    batch = Batch(device, [1500, 33, 700], 4, 2, 16, seed=18)
+    q = batch.queries(3).to(device)
+    lens, tables = torch.tensor(batch.lens, dtype=torch.int32, device=device), batch.tables.to(device)
+    out = torch.empty_like(q)
+    spaces = [_C.alloc_paged_decode_workspace(3, 4, 2, 1500, device) for _ in range(2)]
+
+    def call(out, space):
+        return _C.paged_decode_fp8(out, q, batch.keys, batch.values, tables, lens, SCALE, 1500, space)
+
+    call(out, spaces[0])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call(out, spaces[0])
+    for now in ([1500, 33, 700], [3, 0, 64], [512, 1, 1], [1400, 20, 513]):
+        q.copy_(batch.queries(3))
+        lens.copy_(torch.tensor(now, dtype=torch.int32))
+        for _ in range(2):
+            out.fill_(7.0)
+            graph.replay()
+            got = out.clone()
+            torch.cuda.synchronize()
+            assert torch.equal(got, call(torch.empty_like(q), spaces[1]))
+        batch.lens, full, slots = now, batch.lens, batch.slots
+        batch.slots = [s[:n] for s, n in zip(slots, now)]
+        check_decode(batch, q.cpu(), got)
+        batch.lens, batch.slots = full, slots
+
+
+def test_decode_layer_keeps_a_captured_workspace(device):
+    """A graph captured at a small batch replays right after the layer has served a larger one."""
+    batch = Batch(device, [2000, 33, 700, 1100], 4, 2, 16, seed=19)
+    layer = HipPagedAttention(4, 2, 128)
+    lens, tables = torch.tensor(batch.lens, dtype=torch.int32, device=device), batch.tables.to(device)
+    q = batch.queries(4).to(device)
+    out = torch.empty_like(q)
+
+    def call(n, out=None):
+        return layer(q[:n], batch.keys, batch.values, tables[:n], lens[:n], max_context_len=2000, out=out)
+
+    call(1)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call(1, out[:1])
+    for _ in range(3):
+        whole = call(4)
+        junk = [torch.full((1 << 20,), 255, dtype=torch.uint8, device=device) for _ in range(4)]  # takes what was freed
+        out.fill_(7.0)
+        graph.replay()
+        close(out[:1], *batch.want(0, q[:1].cpu()))
+        assert out[1:].eq(7).all()
+        del junk
+    check_decode(batch, q.cpu(), whole)
+
+
+def test_pages_past_32_bits(device):
+    """Pages whose codes lie past 4 GiB, and rows of them written, read and attended to."""
+    nb, bs, hkv = 2200, 256, 64
+    cache = Fp8PagedKVCache(1, nb, bs, hkv, 128, device)
+    assert cache.key_codes.nbytes > 1 << 32
+    gen = torch.Generator().manual_seed(20)
+    pages = torch.tensor([nb - 1, 0, nb // 2])
+    n = 600
+    slots = pages[torch.arange(n) // bs] * bs + torch.arange(n) % bs
+    k, v = (torch.randn(n, hkv, 128, generator=gen).bfloat16() for _ in range(2))
+    cache.write(0, k.to(device), v.to(device), slots.to(device))
+    small = fp8_ref.empty_pages(3, hkv, bs)
+    fp8_ref.write_sequences(small, k, v, torch.arange(n))
+    kk, vv = fp8_ref.read_sequence(small, torch.arange(n))
+    got = cache.read(0, slots.to(device))
+    assert torch.equal(got[0].cpu().double(), kk) and torch.equal(got[1].cpu().double(), vv)
+    q = torch.randn(n, hkv, 128, generator=gen).bfloat16()
+    tables = pages.to(torch.int32)[None].to(device)
+    lens = torch.tensor([n], dtype=torch.int32, device=device)
+    keys, values = cache.get_physical_cache(0)
+    for rows in (1, 20, 300):
+        want, tol = fp4_ref.attention(q[:rows], kk, vv, SCALE)
+        cu = torch.tensor([0, rows], dtype=torch.int32, device=device)
+        out = torch.empty(rows, hkv, 128, dtype=torch.bfloat16, device=device)
+        close(_C.paged_prefill_fp8(out, q[:rows].to(device), keys, values, tables, cu, lens, rows, SCALE), want, tol)
+    want, tol = fp4_ref.attention(q[:1], kk, vv, SCALE)
+    space = _C.alloc_paged_decode_workspace(1, hkv, hkv, n, device)
+    close(_C.paged_decode_fp8(out[:1], q[:1].to(device), keys, values, tables, lens, SCALE, n, space), want, tol)
+
+
+def test_decode_nan_reaches_only_its_sequence_and_dims(device):
+    batch = Batch(device, [200, 300, 100], 2, 1, 32, seed=7)
+    v = torch.ones(1, 1, 128, dtype=torch.bfloat16)
+    bad_v, bad_k = v.clone(), v.clone()
+    bad_v[0, 0, 70], bad_k[0, 0, 5] = math.inf, math.nan
+    fp8_ref.write(batch.pages, v, bad_v, batch.slots[0][17:18])      # a value
+    fp8_ref.write(batch.pages, bad_k, v, batch.slots[1][299:300])    # a key: every weight
+    batch.upload()
+    q = batch.queries(3)
+    got = batch.decode(q)
+    check_decode(batch, q, got)
+    nan = got.isnan().cpu()
+    assert nan[0, :, 70].all() and nan[0].sum() == 2
+    assert nan[1].all() and not nan[2].any()
+
+
+def test_a_nan_of_a_query_stays_in_its_row(device):
+    batch = Batch(device, [150, 400], 4, 1, 16, seed=27)
+    q = batch.queries(2)
+    clean = batch.decode(q)
+    q[1, 2, 77] = math.nan
+    got = batch.decode(q)
+    assert got[1, 2].isnan().all() and torch.equal(got[0], clean[0]) and torch.equal(got[1, :2], clean[1, :2])
+    assert torch.equal(got[1, 3], clean[1, 3])
+    q = batch.queries(200)
+    for bound in (None, "strips", 60_000):
+        clean = batch.prefill(q, [100, 100], max_q=bound)
+        bad = q.clone()
+        bad[130, 1, 3] = math.inf
+        got = batch.prefill(bad, [100, 100], max_q=bound)
+        assert got[130, 1].isnan().all()
+        got[130, 1] = clean[130, 1]
+        assert torch.equal(got, clean)
+
+
+def test_decode_views_and_rows_behind_the_batch(device):
+    batch = Batch(device, [40, 500], 6, 2, 16, seed=8, extra_width=3)
+    fused = torch.zeros(2, 10, 128, dtype=torch.bfloat16)
+    q = batch.queries(2)
+    fused[:, 1:7] = q
+    wide = torch.full((4, 9, 128), 7.0, dtype=torch.bfloat16, device=device)
+    got = batch.decode(fused.to(device)[:, 1:7], out=wide[:2, 2:8])
+    check_decode(batch, q, got)
+    assert wide[2:].eq(7).all() and wide[:, :2].eq(7).all() and wide[:, 8:].eq(7).all()
+
+
+def test_decode_bad_pages_and_contexts_stay_in_the_pool_and_are_reported(device):
+    batch = Batch(device, [40, 500, 100], 2, 1, 16, seed=9)
+    q = batch.queries(3)
+    good = batch.decode(q)
+    for entry in (batch.nb, -1, 1 << 30):
+        batch.tables[1, 3] = entry
+        got = batch.decode(q)
+        assert _C.index_errors() == _C.ERR_BLOCK
+        assert torch.equal(got[[0, 2]], good[[0, 2]])
+        _C.clear_index_errors()
+    batch.tables[1, 3] = 0
+    for n in (-1, 513, 1 << 30):  # the table holds 512 tokens
+        batch.lens[1] = n
+        got = batch.decode(q, bound=1024)
+        assert _C.index_errors() == _C.ERR_CONTEXT
+        assert torch.equal(got[[0, 2]], good[[0, 2]])
+        _C.clear_index_errors()
+    batch.lens[1] = 500
+    batch.decode(q, bound=400)  # the launch's bound holds less
+    assert _C.index_errors() == _C.ERR_CONTEXT
+
+
+def test_decode_is_the_same_whatever_runs_beside_it(device):
+    """A replayed graph, a workspace that served other calls and repeated calls give the same bits."""
+    batch = Batch(device, [40, 3000, 900], 8, 2, 64, seed=10)
+    q = batch.queries(3).to(device)
+    first = batch.decode(q)
+    ws = _C.alloc_paged_decode_workspace(8, 16, 2, 8192, device)
+    other = Batch(device, [700, 5000], 16, 2, 32, seed=11)
+    for _ in range(3):
+        other.decode(other.queries(2), workspace=ws)
+        assert torch.equal(batch.decode(q, bound=4096, workspace=ws), first)
+    tables, lens = batch.tables.to(device), torch.tensor(batch.lens, dtype=torch.int32, device=device)
+    out = torch.empty_like(q)
+    attn = HipPagedAttention(8, 2, 128)
+
+    def call():
+        return _C.paged_decode_fp8(out, q, batch.keys, batch.values, tables, lens, SCALE, 4096, ws)
+
+    call()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call()
+    for n in (3000, 0, 17, 2999):
+        lens[1] = n
+        out.fill_(7.0)
+        graph.replay()
+        got = out.clone()
+        torch.cuda.synchronize()
+        batch.lens[1] = n
+        assert torch.equal(got, attn(q, batch.keys, batch.values, tables, lens))
+        check_decode(Window(batch, n), q.cpu(), got)
+
+
+class Window:
+    """A batch whose sequence 1 is cut to n tokens."""
+
+    def __init__(self, batch, n):
+        self.batch, self.lens = batch, [batch.lens[0], n, batch.lens[2]]
+
+    def want(self, i, q, scale):
+        k, v = fp8_ref.read_sequence(self.batch.pages, self.batch.slots[i][: self.lens[i]])
+        return fp4_ref.attention(q, k, v, scale)
+
+
+# -------------------------------------------------------------------------------------------- prefill
+# The kernel follows the rows that a call's bounds allow: as many as there are, those of a middle size, of a large one.
+BOUNDS = pytest.mark.parametrize("bound", [None, "strips", 60_000], ids=["exact", "strips", "tiles"])
+
+
+def check_prefill(batch, q, q_lens, got, scale=SCALE):
+    at = 0
+    for i, n in enumerate(q_lens):
+        if n:
+            close(got[at:at + n], *batch.want(i, q[at:at + n], scale))
+        at += n
+
+
+@BOUNDS
+@pytest.mark.parametrize("hq, hkv", [(1, 1), (2, 1), (3, 1), (4, 1), (5, 1), (16, 8), (8, 1), (14, 2), (17, 1), (40, 1)])
+def test_prefill_head_layouts(device, hq, hkv, bound):
+    q_lens, cached = [1, 40, 0, 130], [200, 16, 33, 0]
+    batch = Batch(device, [a + b for a, b in zip(q_lens, cached)], hq, hkv, 32, seed=hq)
+    q = batch.queries(sum(q_lens))
+    check_prefill(batch, q, q_lens, batch.prefill(q, q_lens, max_q=bound))
+    assert _C.index_errors() == 0
+
+
+@BOUNDS
+@pytest.mark.parametrize("bs", [16, 32, 64, 128, 256])
+def test_prefill_lengths_around_tiles_and_pages(device, bs, bound):
+    q_lens = [1, 2, 15, 16, 17, 31, 32, 33, 63, 64, 65, 127, 128, 129, 255, 257]
+    cached = [0, 1, 16, 31, 32, 5, 64, 100, 0, 128, 129, 1, 16, 300, 0, 255]
+    batch = Batch(device, [a + b for a, b in zip(q_lens, cached)], 4, 2, bs, seed=bs)
+    q = batch.queries(sum(q_lens))
+    check_prefill(batch, q, q_lens, batch.prefill(q, q_lens, max_q=bound))
+
+
+@pytest.mark.parametrize("bs", [16, 64])
+def test_prefill_few_rows(device, bs):
+    """Each alone, so that no call has more than a few rows."""
+    for q_len, cached in ((1, 0), (1, 1), (2, 15), (3, 16), (15, 17), (16, 63), (17, 64), (31, 33), (33, 500), (64, 511),
+                          (65, 512), (127, 3000), (256, 0), (300, 1)):
+        batch = Batch(device, [q_len + cached], 4, 2, bs, seed=q_len)
+        q = batch.queries(q_len)
+        check_prefill(batch, q, [q_len], batch.prefill(q, [q_len]))
+
+
+def test_prefill_cut_replays_from_a_graph(device):
+    """Contexts that need one piece or many between the replays, and another call on another stream meanwhile."""
+    batch = Batch(device, [9000, 300], 4, 2, 16, seed=9)
+    q = batch.queries(40).to(device)
+    cu = torch.tensor([0, 30, 40], dtype=torch.int32, device=device)
+    lens, tables = torch.tensor(batch.lens, dtype=torch.int32, device=device), batch.tables.to(device)
+    out = torch.empty_like(q)
+
+    def call(out):
+        return _C.paged_prefill_fp8(out, q, batch.keys, batch.values, tables, cu, lens, 32, SCALE)
+
+    call(out)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call(out)
+    side = torch.cuda.Stream()
+    for now in ([9000, 300], [40, 10], [700, 200], [8999, 12]):
+        lens.copy_(torch.tensor(now, dtype=torch.int32))
+        torch.cuda.synchronize()
+        out.fill_(7.0)
+        graph.replay()
+        with torch.cuda.stream(side):
+            beside = call(torch.empty_like(q))
+        torch.cuda.synchronize()
+        assert torch.equal(out, beside)
+        for i, (n, rows) in enumerate(zip(now, (slice(0, 30), slice(30, 40)))):
+            k, v = fp8_ref.read_sequence(batch.pages, batch.slots[i][:n])
+            close(out[rows], *fp4_ref.attention(q[rows].cpu(), k, v, SCALE))
+
+
+@BOUNDS
+@pytest.mark.parametrize("q_len, cached", [(1, 9000), (600, 4096), (1500, 0)])
+def test_prefill_long(device, q_len, cached, bound):
+    batch = Batch(device, [q_len + cached, 1], 2, 1, 128, seed=2)
+    q = batch.queries(q_len + 1)
+    check_prefill(batch, q, [q_len, 1], batch.prefill(q, [q_len, 1], max_q=bound))
+
+
+@BOUNDS
+def test_prefill_scores_far_apart(device, bound):
+    """Maxima that rise along the keys, so that the running reference moves again and again."""
+    batch = Batch(device, [400, 90], 2, 1, 16, seed=3, spread=1.5)
+    q = batch.queries(300 + 90, scale=8.0)
+    check_prefill(batch, q, [300, 90], batch.prefill(q, [300, 90], max_q=bound))
+
+
+@BOUNDS
+@EXPONENTS
+def test_prefill_of_numbers_far_from_one(device, q_exp, k_exp, v_exp, bound):
+    batch = Batch(device, [1, 70, 300], 4, 2, 32, seed=42)
+    at_scale(batch, k_exp, v_exp)
+    q = batch.queries(1 + 33 + 40, scale=2.0 ** q_exp)
+    check_prefill(batch, q, [1, 33, 40], batch.prefill(q, [1, 33, 40], max_q=bound))
+
+
+@BOUNDS
+def test_prefill_queries_with_outliers(device, bound):
+    batch = Batch(device, [300, 70], 4, 1, 64, seed=15)
+    slots = torch.cat(batch.slots)
+    k, v = fp8_ref.read_sequence(batch.pages, slots)
+    k[..., 5] = k[..., 100] = 0
+    fp8_ref.write_sequences(batch.pages, k.bfloat16(), v.bfloat16(), slots)
+    batch.upload()
+    q = outliers(batch.queries(150))
+    check_prefill(batch, q, [100, 50], batch.prefill(q, [100, 50], max_q=bound))
+
+
+@BOUNDS
+def test_prefill_nan_reaches_the_rows_that_see_its_key_alone(device, bound):
+    batch = Batch(device, [150, 150], 2, 1, 16, seed=4)
+    one = torch.ones(1, 1, 128, dtype=torch.bfloat16)
+    bad_v, bad_k = one.clone(), one.clone()
+    bad_v[0, 0, 40], bad_k[0, 0, 100] = -math.inf, math.inf
+    for at in (109, 115):  # two of a tile, the first of them in a page's last
+        fp8_ref.write(batch.pages, one, bad_v, batch.slots[0][at:at + 1])
+    fp8_ref.write(batch.pages, bad_k, one, batch.slots[1][120:121])
+    batch.upload()
+    q = batch.queries(150)  # 50 rows of the first sequence, from position 100 on, and 100 of the second, from 50 on
+    got = batch.prefill(q, [50, 100], max_q=bound)
+    check_prefill(batch, q, [50, 100], got)
+    nan = got.isnan().cpu()
+    assert not nan[:9].any() and nan[9:50, :, 40].all() and nan[9:50].sum() == 41 * 2
+    assert not nan[50:120].any() and nan[120:].all()
+
+
+@BOUNDS
+def test_prefill_views_and_rows_behind_the_last_sequence(device, bound):
+    batch = Batch(device, [40, 70], 3, 1, 16, seed=5)
+    fused = torch.zeros(60, 5, 128, dtype=torch.bfloat16)
+    q = batch.queries(50)
+    fused[:50, 1:4] = q
+    wide = torch.full((60, 5, 128), 7.0, dtype=torch.bfloat16, device=device)
+    batch.prefill(fused.to(device)[:, 1:4], [20, 30], out=wide[:, 2:], max_q=bound)
+    check_prefill(batch, q, [20, 30], wide[:50, 2:])
+    assert wide[50:].eq(7).all() and wide[:, :2].eq(7).all()
+
+
+@BOUNDS
+def test_prefill_faults_are_reported_and_leave_the_others_alone(device, bound):
+    batch = Batch(device, [100, 60, 200], 2, 1, 16, seed=6)
+    q_lens = [20, 60, 100]
+    q = batch.queries(180)
+    good = batch.prefill(q, q_lens, max_q=bound)
+    others = torch.cat([torch.arange(20), torch.arange(80, 180)])
+    batch.tables[1, 2] = batch.nb
+    got = batch.prefill(q, q_lens, max_q=bound)
+    assert _C.index_errors() == _C.ERR_BLOCK and torch.equal(got[others], good[others])
+    _C.clear_index_errors()
+    batch.tables[1, 2] = 0
+    for n in (59, 0, -1, 1 << 20):  # fewer keys than rows; more than the table holds
+        batch.lens[1] = n
+        got = batch.prefill(q, q_lens, max_q=bound)
+        assert _C.index_errors() == _C.ERR_CONTEXT and torch.equal(got[others], good[others])
+        if n <= 0:
+            assert not got[20:80].any()  # rows that see no key
+        _C.clear_index_errors()
+    batch.lens[1] = 60
+    cu = torch.tensor([0, 20, 80, 181], dtype=torch.int32, device=device)  # one row past the last
+    out = torch.full((180, 2, 128), 7.0, dtype=torch.bfloat16, device=device)
+    args = (batch.keys, batch.values, batch.tables.to(device), cu,
+            torch.tensor(batch.lens, dtype=torch.int32, device=device))
+    _C.paged_prefill_fp8(out, q.to(device), *args, 65536 // 6 if bound == "strips" else bound or 101, SCALE)
+    assert _C.index_errors() == _C.ERR_CONTEXT
+    assert torch.equal(out[:20], good[:20]) and out[80:].eq(7).all()
+
+
+def test_prefill_bound_below_a_length_is_reported(device):
+    batch = Batch(device, [100], 2, 1, 16, seed=6)
+    q = batch.queries(50)
+    batch.prefill(q, [50], max_q=49)
+    assert _C.index_errors() == _C.ERR_CONTEXT
+
+
+def test_prefill_replays_from_a_graph(device):
+    batch = Batch(device, [100, 333], 4, 2, 16, seed=7)
+    q = batch.queries(130).to(device)
+    cu = torch.tensor([0, 30, 130], dtype=torch.int32, device=device)
+    lens, tables = torch.tensor(batch.lens, dtype=torch.int32, device=device), batch.tables.to(device)
+    out = torch.empty_like(q)
+
+    def call(out):
+        return _C.paged_prefill_fp8(out, q, batch.keys, batch.values, tables, cu, lens, 120, SCALE)  # 10 .. 120 rows
+
+    call(out)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call(out)
+    for seed in range(3):
+        q.copy_(batch.queries(130))
+        cu[1] = 10 + 20 * seed
+        graph.replay()
+        got = out.clone()
+        torch.cuda.synchronize()
+        assert torch.equal(got, call(torch.empty_like(q)))
+
+
+# -------------------------------------------------------------------------------------------- bytes that nobody wrote
+def with_stale_scales(batch, byte):
+    """The batch's rows in pages whose other scale bytes are all `byte`, over random codes."""
+    k, v = fp8_ref.read_sequence(batch.pages, torch.cat(batch.slots))
+    for p in batch.pages[1::2]:
+        p.fill_(byte)
+    fp8_ref.write_sequences(batch.pages, k.bfloat16(), v.bfloat16(), torch.cat(batch.slots))
+    batch.upload()
+
+
+@BOUNDS
+@pytest.mark.parametrize("byte", [0, 201, 252, 253, 254, 255])
+def test_prefill_reads_no_value_past_the_keys(device, byte, bound):
+    """Whatever scales unwritten tiles have; the codes behind a tile's tokens are random, NaNs among them."""
+    q_lens, cached = [1, 40, 130, 20], [200, 17, 1, 0]
+    batch = Batch(device, [a + b for a, b in zip(q_lens, cached)], 4, 2, 32, seed=28)
+    with_stale_scales(batch, byte)
+    q = batch.queries(sum(q_lens))
+    check_prefill(batch, q, q_lens, batch.prefill(q, q_lens, max_q=bound))
+
+
+@pytest.mark.parametrize("byte", [0, 201, 252, 253, 254, 255])
+def test_decode_reads_no_value_past_the_context(device, byte):
+    batch = Batch(device, [1, 40, 131, 530, 0, 65], 4, 2, 32, seed=29)
+    with_stale_scales(batch, byte)
+    q = batch.queries(6)
+    check_decode(batch, q, batch.decode(q))
