@@ -142,6 +142,12 @@ _SIGNATURES = {
         [_c_ptr, _c_i64, _c_ptr, _c_i64, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_int, _c_ptr, _c_int, _c_int,
          _c_ptr, _c_int, _c_int, _c_int, _c_int, _c_float, _c_int, _c_ptr, _c_size, _c_ptr],
     ),
+    "nvamd_paged_decode_fused_fp8": (
+        _c_int,
+        [_c_ptr, _c_i64, _c_ptr, _c_i64, _c_ptr, _c_i64, _c_ptr, _c_i64, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int,
+         _c_float, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_int, _c_ptr, _c_ptr, _c_int, _c_int, _c_ptr, _c_int,
+         _c_int, _c_int, _c_int, _c_float, _c_int, _c_ptr, _c_size, _c_ptr],
+    ),
     "nvamd_paged_prefill_fp8": (
         _c_int,
         [_c_ptr, _c_i64, _c_ptr, _c_i64, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_int, _c_ptr, _c_int, _c_int,
@@ -204,8 +210,8 @@ def _bind_calls(lib: ctypes.CDLL) -> None:
                       f"be used ({e}); `python -m nano_vllm_ascend_amd.build` builds it", RuntimeWarning, stacklevel=3)
         return
     for index, kind in enumerate((_FP4, _FP8)):
-        functions = (getattr(lib, "nvamd_" + n.format(kind.name), None) for n in names)
-        calls.bind(index, kind.pages, *(ctypes.cast(f, ctypes.c_void_p).value if f else 0 for f in functions))
+        functions = (getattr(lib, "nvamd_" + n.format(kind.name)) for n in names)
+        calls.bind(index, kind.pages, *(ctypes.cast(f, ctypes.c_void_p).value for f in functions))
     _calls = calls
 
 
@@ -1058,6 +1064,17 @@ def paged_decode_fused_fp4(out: torch.Tensor | None, q: torch.Tensor, k: torch.T
     """``qk_norm_rope_fp4`` and ``paged_decode_fp4`` in one launch, with the same bits: the step's k and v go to the slots
     of their sequences' last positions (-1: not stored), q, k and v stay as they are."""
     return _decode_fused(_FP4, out, q, k, v, q_weight, k_weight, positions, cos_sin, eps, key_pages, value_pages,
+                         slot_mapping, block_tables, context_lens, scale, max_context_len, workspace)
+
+
+def paged_decode_fused_fp8(out: torch.Tensor | None, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+                           q_weight: torch.Tensor, k_weight: torch.Tensor, positions: torch.Tensor,
+                           cos_sin: torch.Tensor, eps: float, key_pages: Fp8Pages, value_pages: Fp8Pages,
+                           slot_mapping: torch.Tensor, block_tables: torch.Tensor, context_lens: torch.Tensor,
+                           scale: float, max_context_len: int, workspace: torch.Tensor) -> torch.Tensor:
+    """``qk_norm_rope_fp8`` and ``paged_decode_fp8`` in one launch, with the same bits: the step's k and v go to the slots
+    of their sequences' last positions (-1: not stored), q, k and v stay as they are."""
+    return _decode_fused(_FP8, out, q, k, v, q_weight, k_weight, positions, cos_sin, eps, key_pages, value_pages,
                          slot_mapping, block_tables, context_lens, scale, max_context_len, workspace)
 
 

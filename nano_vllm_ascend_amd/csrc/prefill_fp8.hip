@@ -3,7 +3,6 @@
 // 16 keys (a tile) at a time: lane (t, part) takes 32 dims of key t, the four parts meet by exchanges, the softmax keeps
 // a running maximum and sum in 32 bits, and a lane adds up two dims of the values.
 #include "attention_tiles.h"
-#include "decode_workspace.h"
 #include "fp8.h"
 
 namespace nvamd {
@@ -130,31 +129,6 @@ int fill_args(AttentionArgs &a, void *out, int64_t out_stride, const void *q, in
 }  // namespace nvamd
 
 using namespace nvamd;
-
-extern "C" int nvamd_paged_decode_fp8(void *out, int64_t out_stride, const void *q, int64_t q_stride,
-                                      const void *k_codes, const void *k_scales, const void *v_codes,
-                                      const void *v_scales, int num_blocks, int block_size,
-                                      const int32_t *block_tables, int bt_stride, int bt_width,
-                                      const int32_t *context_lens, int batch, int num_heads, int num_kv_heads,
-                                      int head_dim, float scale, int max_context_len, void *workspace,
-                                      size_t workspace_bytes, hipStream_t stream) {
-  if (batch == 0) return NVAMD_OK;
-  AttentionArgs a;
-  const int st = fill_args(a, out, out_stride, q, q_stride, k_codes, k_scales, v_codes, v_scales, num_blocks, block_size,
-                           block_tables, bt_stride, bt_width, context_lens, num_heads, num_kv_heads, head_dim, scale);
-  if (st != NVAMD_OK) return st;
-  if (batch < 0 || max_context_len <= 0) return NVAMD_EINVAL;
-  if ((int64_t)batch * num_kv_heads > kCounterSlots || batch > 65535 || max_context_len > kMaxContext)
-    return NVAMD_EUNSUPPORTED;
-  if (!workspace || workspace_bytes < decode_workspace_bytes(batch, num_heads, num_kv_heads, max_context_len))
-    return NVAMD_EWORKSPACE;
-  if (!aligned16(workspace)) return NVAMD_EINVAL;
-  a.max_q_len = 1;
-  a.num_tokens = batch;
-  a.max_ctx = max_context_len;
-  hipLaunchKernelGGL(attention_fp8_kernel, dim3(num_heads, 1, batch), dim3(64), 0, stream, a);
-  return launch_status();
-}
 
 extern "C" size_t nvamd_paged_prefill_fp8_workspace_size(int n_seqs, int max_q_len, int num_heads, int num_kv_heads,
                                                          int block_size, int bt_width) {

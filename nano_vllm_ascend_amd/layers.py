@@ -155,10 +155,9 @@ class HipPagedAttention(nn.Module):
                                              q_norm.variance_epsilon, key_cache, value_cache, slot_mapping,
                                              block_tables, context_lens, self.scale, max_context_len, workspace)
         if isinstance(key_cache, _C.Fp8Pages):
-            rotated = _C.qk_norm_rope_fp8(q, k, v, q_norm.weight, k_norm.weight, positions, rotary.cos_sin,
-                                          q_norm.variance_epsilon, key_cache, value_cache, slot_mapping)
-            return _C.paged_decode_fp8(out, rotated, key_cache, value_cache, block_tables, context_lens, self.scale,
-                                       max_context_len, workspace)
+            return _C.paged_decode_fused_fp8(out, q, k, v, q_norm.weight, k_norm.weight, positions, rotary.cos_sin,
+                                             q_norm.variance_epsilon, key_cache, value_cache, slot_mapping,
+                                             block_tables, context_lens, self.scale, max_context_len, workspace)
         out = torch.empty_like(q) if out is None else out
         return _C.paged_decode_fused(out, q, k, v, q_norm.weight, k_norm.weight, positions, rotary.cos_sin,
                                      q_norm.variance_epsilon, key_cache, value_cache, slot_mapping, block_tables,

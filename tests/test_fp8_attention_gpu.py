@@ -5,12 +5,15 @@ bf16 weights and results makes."""
 from __future__ import annotations
 
 import math
+import random
 
 import pytest
 import torch
 
 from nano_vllm_ascend_amd import _C
-from nano_vllm_ascend_amd.layers import HipPagedAttention
+from nano_vllm_ascend_amd.block_manager import PagedKVCacheMetadata
+from nano_vllm_ascend_amd.layers import (HipBatchPrefillAttention, HipPagedAttention, RMSNorm, RotaryEmbedding,
+                                         qk_norm_rope)
 from nano_vllm_ascend_amd.paged_kv_cache import Fp8PagedKVCache
 from oracle import fp4_ref, fp8_ref
 
@@ -663,3 +666,336 @@ def test_decode_reads_no_value_past_the_context(device, byte):
     with_stale_scales(batch, byte)
     q = batch.queries(6)
     check_decode(batch, q, batch.decode(q))
+
+
+# -------------------------------------------------------------------------------------------- a whole decode step
+def step_of(batch, seed, slots=None):
+    """Projected rows of a new token for each sequence of the batch, whose last position is the token's."""
+    gen = torch.Generator().manual_seed(seed)
+    b = len(batch.lens)
+    qkv = torch.randn(b, batch.hq + 2 * batch.hkv, 128, generator=gen).bfloat16().to(batch.device)
+    q, k, v = qkv.split([batch.hq, batch.hkv, batch.hkv], 1)
+    weights = [(1 + 0.1 * torch.randn(128, generator=gen)).bfloat16().to(batch.device) for _ in range(2)]
+    angle = torch.rand(64, 64, generator=gen) * 7
+    table = torch.cat((angle.cos(), angle.sin()), 1).to(batch.device)
+    pos = torch.randint(0, 64, (b,), generator=gen).to(batch.device)
+    if slots is None:
+        slots = torch.stack([s[-1] if len(s) else torch.tensor(-1) for s in batch.slots])
+    return q, k, v, *weights, pos, table, 1e-6, batch.keys, batch.values, slots.to(batch.device)
+
+
+def attend(batch, q, bound, workspace, fused=None):
+    tables, lens = batch.tables.to(batch.device), torch.tensor(batch.lens, dtype=torch.int32, device=batch.device)
+    if fused is None:
+        return _C.paged_decode_fp8(None, q, batch.keys, batch.values, tables, lens, SCALE, bound, workspace)
+    return _C.paged_decode_fused_fp8(q, *fused, tables, lens, SCALE, bound, workspace)
+
+
+def in_pages(batch):
+    return [t.clone() for t in (*batch.keys, *batch.values)]
+
+
+@pytest.mark.parametrize("hq, hkv, bs", [(16, 8, 128), (1, 1, 16), (12, 4, 32), (8, 1, 64), (40, 8, 16), (17, 1, 256),
+                                         (34, 2, 128)])
+def test_fused_step_has_the_bits_of_the_two_launches(device, hq, hkv, bs):
+    batch = Batch(device, [1, 16, 17, 300, 0, 512, 513, 1100, 4097], hq, hkv, bs, seed=hq + bs)
+    space = _C.alloc_paged_decode_workspace(9, hq, hkv, 8192, device)
+    for bound in (4097, 8192):
+        batch.upload()
+        args = step_of(batch, seed=bound)
+        raw = [t.clone() for t in args[:3]]
+        want = attend(batch, _C.qk_norm_rope_fp8(*args), bound, space)
+        stored = in_pages(batch)
+        batch.upload()
+        got = attend(batch, None, bound, space, fused=step_of(batch, seed=bound))
+        assert torch.equal(got, want) and all(torch.equal(a, b) for a, b in zip(in_pages(batch), stored))
+        assert all(torch.equal(a, b) for a, b in zip(args[:3], raw))
+    assert _C.index_errors() == 0
+
+
+@pytest.mark.parametrize("hq, hkv, bs", [(16, 8, 128), (34, 2, 32), (1, 1, 16)])
+def test_fused_step_may_write_over_its_queries(device, hq, hkv, bs):
+    """out is q itself, a view into the projection's rows: k and v beside it stay as they are."""
+    batch = Batch(device, [1, 300, 0, 513, 4097], hq, hkv, bs, seed=37)
+    space = _C.alloc_paged_decode_workspace(5, hq, hkv, 4097, device)
+    args = step_of(batch, seed=38)
+    want = attend(batch, None, 4097, space, fused=args)
+    batch.upload()
+    q, k, v, *rest = step_of(batch, seed=38)
+    kv = k.clone(), v.clone()
+    got = _C.paged_decode_fused_fp8(q, q, k, v, *rest, batch.tables.to(device),
+                                    torch.tensor(batch.lens, dtype=torch.int32, device=device), SCALE, 4097, space)
+    assert got is q and torch.equal(q, want) and torch.equal(k, kv[0]) and torch.equal(v, kv[1])
+
+
+def test_fused_step_reports_what_it_skips_and_clamps(device):
+    batch = Batch(device, [30, 40, 50], 4, 2, 16, seed=24)
+    space = _C.alloc_paged_decode_workspace(3, 4, 2, 64, device)
+    slots = torch.stack([s[-1] for s in batch.slots])
+    before = in_pages(batch)
+    for bad, word in ((torch.tensor(-1), 0), (torch.tensor(-2), _C.ERR_SLOT), (torch.tensor(batch.nb * 16), _C.ERR_SLOT)):
+        attend(batch, None, 64, space, fused=step_of(batch, 25, slots=torch.stack([bad] * 3)))
+        assert _C.index_errors() == word and all(torch.equal(a, b) for a, b in zip(in_pages(batch), before))
+        _C.clear_index_errors()
+    args = list(step_of(batch, 26, slots=slots))
+    good = attend(batch, None, 64, space, fused=args)
+    args[5] = args[5].clone()
+    args[5][1] = 64
+    got = attend(batch, None, 64, space, fused=args)
+    assert _C.index_errors() == _C.ERR_POSITION and torch.equal(got[::2], good[::2])
+
+
+# -------------------------------------------------------------------------------------------- the two routes of a call
+def test_a_call_made_at_once_equals_one_that_python_checks(device):
+    """Range checks send the calls through the checks of _C.py; without them csrc/calls.cpp makes those that are plain."""
+    batch = Batch(device, [300, 5000, 20], 4, 2, 16, seed=21, extra_width=300)
+    gen = torch.Generator().manual_seed(22)
+    qkv = torch.randn(9, 8, 128, generator=gen).bfloat16().to(device)
+    q, k, v = qkv.split([4, 2, 2], 1)
+    weights = [torch.rand(128, generator=gen).bfloat16().to(device) for _ in range(2)]
+    table = torch.randn(64, 128, generator=gen).to(device)
+    pos = torch.arange(9, device=device)
+    slots = batch.slots[0][:9].to(device)
+    slots[8] = -1
+    lens = torch.tensor(batch.lens, dtype=torch.int32, device=device)
+    tables = batch.tables.to(device)
+    cu = torch.tensor([0, 4, 8, 9], dtype=torch.int32, device=device)
+    space = _C.alloc_paged_decode_workspace(3, 4, 2, 5000, device)
+
+    def results():
+        batch.upload()
+        pages = batch.keys, batch.values
+        got = [_C.paged_decode_fp8(None, q[:3], *pages, tables, lens, SCALE, 5000, space),
+               _C.paged_decode_fp8(torch.empty(3, 4, 128, dtype=torch.bfloat16, device=device), q[:3], *pages, tables, lens,
+                                   SCALE, 5000, space),
+               _C.paged_prefill_fp8(torch.empty(9, 4, 128, dtype=torch.bfloat16, device=device), q, *pages, tables, cu, lens,
+                                    4, SCALE)]
+        _C.kv_cache_write_fp8(k, v, *pages, slots)
+        got += [*pages[0], *pages[1], *_C.kv_cache_read_fp8(*pages, slots)]
+        k_out = torch.zeros(9, 2, 128, dtype=torch.bfloat16, device=device)
+        got.append(_C.qk_norm_rope_fp8(q, k, v, *weights, pos, table, 1e-6, *pages, slots, k_out=k_out))
+        got.append(_C.qk_norm_rope_fp8(q, k, v, *weights, pos, table, 1e-6, *pages, slots, q_out=torch.empty_like(got[-1])))
+        last = torch.stack([s[-1] for s in batch.slots]).to(device)
+        fused = q[:3], k[:3], v[:3], *weights, pos[:3], table, 1e-6, *pages, last, tables, lens, SCALE, 5000, space
+        got += [_C.paged_decode_fused_fp8(None, *fused), _C.paged_decode_fused_fp8(torch.empty_like(got[0]), *fused)]
+        return [t.clone() for t in (*got, k_out, *pages[0], *pages[1])]
+
+    at_once = results()
+    before = _C.set_range_checks(True)
+    try:
+        checked = results()
+    finally:
+        _C.set_range_checks(before)
+    assert len(at_once) == len(checked) and all(torch.equal(a, b) for a, b in zip(at_once, checked))
+
+
+def test_what_the_library_refuses_raises(device):
+    batch = Batch(device, [30], 2, 1, 16, seed=23)
+    q = batch.queries(1).to(device)
+    with pytest.raises(ValueError, match="workspace"):
+        batch.decode(q, workspace=torch.zeros(64, dtype=torch.uint8, device=device))
+    with pytest.raises(ValueError, match="invalid argument"):
+        batch.prefill(q, [1], scale=-1.0)
+    with pytest.raises(ValueError, match="invalid argument"):
+        _C.kv_cache_write_fp8(q[:, :1].expand(4, 1, 128), q[:, :1].expand(4, 1, 128), batch.keys, batch.values,
+                              torch.arange(4, device=device))
+    with pytest.raises(ValueError, match="on one device|GPU"):
+        _C.kv_cache_write_fp8(q[:, :1].cpu(), q[:, :1].cpu(), batch.keys, batch.values, torch.arange(1, device=device))
+
+
+def irregular(name, x):
+    """What an argument must not be: on the host, of another type, a row short, not dense."""
+    if isinstance(x, _C.Fp8Pages):
+        for i, t in enumerate(x):
+            for how, bad in irregular(name, t):
+                yield f"{x._fields[i]} {how}", x._replace(**{x._fields[i]: bad})
+        yield "a plain tuple", tuple(x)
+        return
+    yield "on the host", x.cpu()
+    if name != "workspace":
+        yield "of another type", x.to(torch.float64)
+        if name not in ("cos_sin", "cu_seqlens_q"):
+            yield "a row short", x[:-1]
+    if x.dim() == 1:
+        yield "with gaps", x.repeat_interleave(2)[::2]
+    else:
+        yield "with gaps", x.repeat_interleave(2, -1)[..., ::2]
+
+
+@pytest.mark.parametrize("name", ["write", "read", "rope", "decode", "decode_fused", "prefill"])
+def test_what_the_checks_refuse_is_not_called_at_once(device, name):
+    """csrc/calls.cpp leaves each call that _C.py refuses to it."""
+    batch = Batch(device, [40, 33, 20], 4, 2, 16, seed=34)
+    q, k, v, qw, kw, pos, table, eps, keys, values, slots = step_of(batch, 35)
+    lens = torch.tensor(batch.lens, dtype=torch.int32, device=device)
+    tables = batch.tables.to(device)
+    cu = torch.arange(4, dtype=torch.int32, device=device)
+    space = _C.alloc_paged_decode_workspace(3, 4, 2, 64, device)
+    out = torch.empty_like(q)
+    rope = dict(q=q, k=k, v=v, q_weight=qw, k_weight=kw, positions=pos, cos_sin=table, eps=eps)
+    pages = dict(key_pages=keys, value_pages=values)
+    where = dict(block_tables=tables, context_lens=lens, scale=SCALE, max_context_len=64, workspace=space)
+    call, args = {
+        "write": (_C.kv_cache_write_fp8, dict(key_states=k, value_states=v, **pages, slot_mapping=slots)),
+        "read": (_C.kv_cache_read_fp8, dict(**pages, slot_mapping=slots)),
+        "rope": (_C.qk_norm_rope_fp8, dict(**rope, **pages, slot_mapping=slots, q_out=out, k_out=torch.empty_like(k))),
+        "decode": (_C.paged_decode_fp8, dict(out=out, q=q, **pages, **where)),
+        "decode_fused": (_C.paged_decode_fused_fp8, dict(out=out, **rope, **pages, slot_mapping=slots, **where)),
+        "prefill": (_C.paged_prefill_fp8, dict(out=out, q=q, **pages, block_tables=tables, cu_seqlens_q=cu, kv_lens=lens,
+                                               max_q_len=1, scale=SCALE)),
+    }[name]
+    at_once = getattr(_C._calls, name)
+    assert type(at_once(*args.values())) not in (type(None), int)
+    for arg, x in args.items():
+        if name == "read" and arg == "slot_mapping":
+            cases = [c for c in irregular(arg, x) if c[0] != "a row short"]  # as many rows as there are slots
+        else:
+            cases = irregular(arg, x) if isinstance(x, (torch.Tensor, _C.Fp8Pages)) else ()
+        for how, bad in cases:
+            changed = {**args, arg: bad}
+            assert at_once(*changed.values()) is None, (arg, how)
+            with pytest.raises(ValueError):
+                call(**changed)
+    assert _C.index_errors() == 0
+
+
+def test_calls_without_the_extension(device, monkeypatch):
+    """Where csrc/calls.cpp cannot be used the same calls are made from Python."""
+    batch = Batch(device, [300, 20], 4, 2, 16, seed=32)
+    q = batch.queries(2)
+    step = step_of(batch, 33)
+    space = _C.alloc_paged_decode_workspace(2, 4, 2, 512, device)
+    slots = torch.stack([s[-1] for s in batch.slots]).to(device)
+
+    def results():
+        batch.upload()
+        args = (*step[:8], batch.keys, batch.values, slots)
+        got = [batch.decode(q, bound=512), batch.prefill(q, [1, 1]), attend(batch, None, 512, space, fused=args)]
+        batch.upload()
+        args = (*step[:8], batch.keys, batch.values, slots)
+        got.append(_C.qk_norm_rope_fp8(*args))
+        got += _C.kv_cache_read_fp8(batch.keys, batch.values, slots)
+        _C.kv_cache_write_fp8(step[1], step[2], batch.keys, batch.values, slots)
+        return got + in_pages(batch)
+
+    want = results()
+    monkeypatch.setattr(_C, "_calls", None)
+    assert all(torch.equal(a, b) for a, b in zip(results(), want))
+
+
+def test_block_tables_whose_rows_overlap_are_refused_on_either_route(device):
+    batch = Batch(device, [40, 33, 20], 4, 2, 16, seed=30)
+    q, step = batch.queries(3).to(device), step_of(batch, 31)
+    lens = torch.tensor(batch.lens, dtype=torch.int32, device=device)
+    cu = torch.arange(4, dtype=torch.int32, device=device)
+    space = _C.alloc_paged_decode_workspace(3, 4, 2, 64, device)
+    pages = batch.keys, batch.values
+    shared = batch.tables[:1].to(device).expand(3, -1)
+    calls = {
+        "decode": (_C.paged_decode_fp8, (None, q, *pages, shared, lens, SCALE, 64, space)),
+        "decode_fused": (_C.paged_decode_fused_fp8, (None, *step, shared, lens, SCALE, 64, space)),
+        "prefill": (_C.paged_prefill_fp8, (torch.empty_like(q), q, *pages, shared, cu, lens, 1, SCALE)),
+    }
+    for name, (call, args) in calls.items():
+        assert getattr(_C._calls, name)(*args) is None  # left to the checks, which name what is wrong
+        for checks in (False, True):
+            before = _C.set_range_checks(checks)
+            try:
+                with pytest.raises(ValueError, match="block_tables overlap"):
+                    call(*args)
+            finally:
+                _C.set_range_checks(before)
+    whole = _C.paged_decode_fp8(None, q, *pages, shared.contiguous(), lens, SCALE, 64, space)
+    one = batch.tables[0].to(device).expand(1, -1)  # a single row, whatever its stride
+    assert torch.equal(_C.paged_decode_fp8(None, q[:1], *pages, one, lens[:1], SCALE, 64, space), whole[:1])
+
+
+# -------------------------------------------------------------------------------------------- drawn calls
+HEADS = [(1, 1), (16, 8), (14, 2), (12, 4), (40, 8), (32, 4), (7, 7), (33, 1)]
+
+
+def some_length(rng, most):
+    return rng.choice([0, 1, 16, rng.randint(1, 40), int(2 ** rng.uniform(0, math.log2(most)))])
+
+
+@pytest.mark.parametrize("seed", range(10))
+def test_decode_of_a_drawn_batch(device, seed):
+    rng = random.Random(seed)
+    hq, hkv = rng.choice(HEADS)
+    batch = Batch(device, [some_length(rng, 6000) for _ in range(rng.randint(1, 20))], hq, hkv,
+                  rng.choice([16, 32, 64, 128, 256]), seed=seed, extra_width=rng.choice([0, 5]))
+    q = batch.queries(len(batch.lens))
+    check_decode(batch, q, batch.decode(q, bound=rng.choice([None, 8192, 131072])))
+    assert _C.index_errors() == 0
+
+
+@pytest.mark.parametrize("seed", range(12))
+def test_prefill_of_a_drawn_batch(device, seed):
+    rng = random.Random(100 + seed)
+    hq, hkv = rng.choice(HEADS)
+    most = 2000 // hq + 20
+    q_lens = [some_length(rng, most) for _ in range(rng.randint(1, 6))]
+    lens = [n + some_length(rng, 3000) for n in q_lens]
+    bs = rng.choice([16, 32, 64, 128, 256])
+    batch = Batch(device, lens, hq, hkv, bs, seed=seed, extra_width=rng.choice([0, 8192 // bs]))
+    q = batch.queries(sum(q_lens))
+    bound = max(max(q_lens), 1)
+    check_prefill(batch, q, q_lens, batch.prefill(q, q_lens, max_q=rng.choice([bound, bound, 4 * bound, bound + 1000, 20_000])))
+    assert _C.index_errors() == 0
+
+
+# -------------------------------------------------------------------------------------------- as they are used together
+def test_prompt_then_decode_steps(device):
+    """The layers as the model calls them: a prompt's rows are stored, a follow-up attends through the cache, decode steps
+    store their row and attend."""
+    hq, hkv, bs, nb = 8, 2, 16, 12
+    cache = Fp8PagedKVCache(2, nb, bs, hkv, 128, device)
+    pages = fp8_ref.empty_pages(nb, hkv, bs)
+    norms = [RMSNorm(128, 1e-6).to(device, torch.bfloat16) for _ in range(2)]
+    rotary = RotaryEmbedding(128, 512, 1e6).to(device)
+    prefill, decode = HipBatchPrefillAttention(hq, hkv, 128, bs, 512), HipPagedAttention(hq, hkv, 128)
+    gen = torch.Generator().manual_seed(1)
+    order = torch.randperm(nb, generator=gen)
+    tables = torch.stack([order[:6], order[6:]]).to(torch.int32)
+    done = [0, 0]
+
+    def step(new):
+        """The rows of `new[i]` more tokens of each sequence, as projected; returns what the oracle makes of them."""
+        pos = torch.cat([torch.arange(a, a + n) for a, n in zip(done, new)])
+        seq = torch.repeat_interleave(torch.arange(2), torch.tensor(new))
+        slots = tables[seq, pos // bs].long() * bs + pos % bs
+        qkv = torch.randn(sum(new), hq + 2 * hkv, 128, generator=gen).bfloat16()
+        q, k, v = qkv.split([hq, hkv, hkv], 1)
+        q, k = (fp4_ref.to_bf16(fp4_ref.norm_rope(x, m.weight.cpu(), pos, rotary.cos_sin.cpu(), 1e-6))
+                for x, m in zip((q, k), norms))
+        fp8_ref.write(pages, k, v, slots)
+        outs, tols, at = [], [], 0
+        for i, n in enumerate(new):
+            done[i] += n
+            seen = torch.arange(done[i])
+            kk, vv = fp8_ref.read_sequence(pages, tables[i, seen // bs].long() * bs + seen % bs)
+            out, tol = fp4_ref.attention(q[at:at + n], kk, vv, SCALE)
+            outs.append(out)
+            tols.append(tol)
+            at += n
+        return qkv.to(device).split([hq, hkv, hkv], 1), pos.to(device), slots.to(device), torch.cat(outs), torch.cat(tols)
+
+    for new in ([20, 37], [33, 5]):
+        (q, k, v), pos, slots, want, tol = step(new)
+        qk_norm_rope(q, k, v, *norms, rotary, pos, cache, 1, slots)
+        md = PagedKVCacheMetadata(block_tables=tables.to(device), slot_mapping=slots, max_query_len=max(new),
+                                  context_lens=torch.tensor(done, dtype=torch.int32, device=device),
+                                  cu_seqlens_q=torch.tensor([0, new[0], sum(new)], dtype=torch.int32, device=device),
+                                  use_paged_prefill=True)
+        close(prefill(q, k, v, md, *cache.get_physical_cache(1)), want, tol)
+    for _ in range(4):
+        (q, k, v), pos, slots, want, tol = step([1, 1])
+        raw = q.clone(), k.clone()
+        got = decode.decode_step(q, k, v, *norms, rotary, pos, *cache.get_physical_cache(1), slots, tables.to(device),
+                                 torch.tensor(done, dtype=torch.int32, device=device))
+        close(got, want, tol)
+        assert torch.equal(q, raw[0]) and torch.equal(k, raw[1])
+    for a, b in zip((cache.key_codes, cache.key_scales, cache.value_codes, cache.value_scales), pages):
+        assert torch.equal(a[1].cpu(), b)
+    assert not cache.key_codes[0].any()
+    assert _C.index_errors() == 0

@@ -153,6 +153,25 @@ def test_decode_argument_errors():
     assert call(ws_bytes=need - 1) == EWORKSPACE and call(ws=0) == EWORKSPACE and call(ws=A + 8) == EINVAL
 
 
+def test_fused_decode_argument_errors():
+    lib = _C.load()
+
+    def call(**over):
+        args = dict(out=A, out_stride=2048, q=A, q_stride=4096, k=A, k_stride=4096, v=A, v_stride=4096, qw=A, kw=A, pos=A,
+                    table=A, max_pos=4096, eps=1e-6, **CACHE, slots=A, bt=A, bt_stride=8, bt_width=8, lens=A, batch=4,
+                    hq=16, hkv=8, d=128, scale=128 ** -0.5, max_ctx=1024, ws=A, ws_bytes=1 << 24, stream=None)
+        args.update(over)
+        return lib.nvamd_paged_decode_fused_fp8(*args.values())
+
+    assert call(batch=0) == 0
+    for name in ("out", "q", "k", "v", "qw", "kw", "table", "kc", "vc"):
+        assert call(**{name: 0}) == EINVAL and call(**{name: A + 8}) == EINVAL, name
+    assert call(pos=0) == EINVAL and call(slots=0) == EINVAL and call(max_pos=0) == EINVAL and call(bt=0) == EINVAL
+    assert call(k_stride=1016) == EINVAL and call(v_stride=4092) == EINVAL
+    assert call(d=64) == EUNSUPPORTED and call(max_ctx=131073, ws_bytes=1 << 40) == EUNSUPPORTED
+    assert call(ws_bytes=100) == EWORKSPACE
+
+
 def test_prefill_argument_errors():
     lib = _C.load()
 
