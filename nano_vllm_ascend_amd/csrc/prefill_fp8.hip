@@ -1,128 +1,556 @@
-// Attention over the 8-bit paged KV cache, one wave for each query row and head: the formula as it stands.
+// Causal prefill attention over the 8-bit paged KV cache (the counterpart of prefill.hip's paged route): the queries are
+// the last q_len positions of a context of kv_len, query row r sees keys 0 .. kv_len - q_len + r, all of them in the
+// cache.  Rows, ways out and the choice of kernel are shared with the 4-bit cache's (prefill_quantised.h).
 //
-// 16 keys (a tile) at a time: lane (t, part) takes 32 dims of key t, the four parts meet by exchanges, the softmax keeps
-// a running maximum and sum in 32 bits, and a lane adds up two dims of the values.
-#include "attention_tiles.h"
-#include "fp8.h"
+// In all kernels
+//   S^T = K . Q^T   v_mfma_scale_f32_*_f8f6f4 on the codes as they lie in the cache, under their tiles' scales: a lane loads
+//        its dims of a key straight into the operand, and the row comes as two e4m3 numbers per value.  No expansion of
+//        K, and none of it in LDS;
+//   O^T += V^T . P^T   v_mfma_f32_*_bf16 on V expanded by v_cvt_scalef32_pk_bf16_fp8, exact.
+// The rows of K are taken in such an order that a lane's registers of S^T are the consecutive keys that its operand of
+// P^T needs: a repack in registers.  Three kernels, which differ in how many rows share an expansion of V:
+//
+// Tiles (the card is full).  Workgroup = 4 waves = 128 rows, a wave 32 of them, tiles of 32 keys.  The workgroup
+//   expands a tile of V once, to bf16 operands in LDS (every access is 64 lanes x 16 consecutive bytes): a wave takes 32
+//   dims, a lane a dim of 16 tokens.  Key 16a + 8b + 4c + x sits in row 16a + 8c + 4b + x of K.  K of the next tile loads
+//   as the scores have taken this one's, V's codes are two tiles ahead, V's operands one (two stages, one barrier a tile).
+// Strips (one long prompt, or several short ones).  Workgroup = 4 waves = 32 rows, a wave every fourth 32 keys; no
+//   barrier in the loop, the waves' results meet in LDS.  A lane expands 16 tokens of a dim straight into operands.
+// Few rows (a chat's next turn).  Workgroup = 8 waves = 16 rows, a wave every eighth 64 keys, as in
+//   paged_decode_fp8.hip with rows in the place of heads and a last key for each row.  On long contexts the keys are cut as
+//   well.
+//
+// Weights are rounded to bf16 once for the matrix cores, and the sums take the rounded values, as in the other caches'
+// prefill.
+//
+// A value that reads as NaN must reach the rows that see its key and no others, though masked rows multiply it by a weight
+// of zero.  Where every row of a workgroup sees every key of a tile the products do that; in the others, which cross the
+// diagonal, such values enter the products as zeros, and the rows that see the key get the NaN afterwards.
+#include "fp8_attention.h"
+#include "prefill_quantised.h"
 
 namespace nvamd {
 namespace {
 
-struct AttentionArgs {
-  u16 *out;
-  int64_t out_stride;
-  const u16 *q;
-  int64_t q_stride;
-  Fp8Cache cache;
-  const int32_t *block_tables;
-  const int32_t *cu_seqlens_q;  // or null: one row a sequence
-  const int32_t *kv_lens;
-  int bt_stride;
-  int bt_width;
-  int num_blocks;
-  int bs_log2;
-  int num_kv_heads;
-  int group;  // query heads of a kv head
-  int max_q_len;
-  int num_tokens;
-  int max_ctx;
-  float scale;
-  u32 *err;
-};
-
-__device__ __forceinline__ float code_value(const u8 *p, int64_t at, float scale) {
-  return bf16_lo(fp8_pair<false>((u32)p[at], scale));
+// 0x80 in the bytes that are codes of NaN (127 and 255).
+__device__ __forceinline__ u32 nan_bytes(u32 codes) { return ((codes & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
+__device__ __forceinline__ u32 without(u32 codes, u32 nans) { return codes & ~((nans >> 7) * 0xffu); }
+// Replaces a dim's NaNs by zeros and returns their tokens, a bit each.
+__device__ __forceinline__ u32 take_nans(u32x4 &codes) {
+  u32 tokens = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const u32 bad = nan_bytes(codes[i]);
+    codes[i] = without(codes[i], bad);
+    tokens |= ((bad >> 7 & 1u) | (bad >> 14 & 2u) | (bad >> 21 & 4u) | (bad >> 28 & 8u)) << (4 * i);
+  }
+  return tokens;
 }
 
-__global__ void __launch_bounds__(64)
-attention_fp8_kernel(AttentionArgs a) {
-  const int s = blockIdx.z, head = blockIdx.x, lane = threadIdx.x;
-  const int g = head / a.group;
-  const int q_start = a.cu_seqlens_q ? a.cu_seqlens_q[s] : s;
-  const int q_end = a.cu_seqlens_q ? a.cu_seqlens_q[s + 1] : s + 1;
-  const int q_len = (int)((unsigned)q_end - (unsigned)q_start);
-  const bool rows_in = q_start >= 0 && q_start <= q_end && q_end <= a.num_tokens;  // else no row is touched
-  const int cap = min(a.max_ctx, a.bt_width << a.bs_log2);
-  const int raw = a.kv_lens[s];
-  const bool short_of_rows = a.cu_seqlens_q != nullptr && raw < q_len;
-  if ((!rows_in || q_len > a.max_q_len || raw > cap || raw < 0 || short_of_rows) && head == 0 && blockIdx.y == 0 && lane == 0)
-    flag_index_error(a.err, NVAMD_ERR_CONTEXT);
-  const int token = blockIdx.y;
-  if (!rows_in || token >= q_len || token >= a.max_q_len) return;
-  const int kv_len = min(max(raw, 0), cap);
-  const int keys = a.cu_seqlens_q ? min(kv_len, kv_len - q_len + token + 1) : kv_len;  // that the row sees
-  const int t = lane & 15, part = lane >> 4;
-  float q[32];
-  const u16 *qp = a.q + (int64_t)(q_start + token) * a.q_stride + (int64_t)head * kHeadDim;
+// ------------------------------------------------------------------------------------------ tiles
+
+// 64 dims: lane (n, half) gives dims 16 half .. +15 and 32 + 16 half .. +15 of row and column n, the scale byte of its row
+// and that of block `half` of its column.
+__device__ __forceinline__ f32x16 mfma32_fp8_fp8(const u32x4 (&k)[2], u32 k_scale, i32x8 q, u32 q_scale, f32x16 c) {
+  const i32x8 codes = {(int)k[0][0], (int)k[0][1], (int)k[0][2], (int)k[0][3],
+                       (int)k[1][0], (int)k[1][1], (int)k[1][2], (int)k[1][3]};
+  return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(codes, q, c, 0, 0, 0, (int)k_scale, 0, (int)q_scale);
+}
+
+struct Stage {
+  u32x4 v[2][4][64];  // [16-key step][32-dim block][lane]
+  u32 any[4];         // on the diagonal, [wave that expanded them]: whether any of its values read as NaN,
+  u32 nan[4][32][2];  // and which: of each dim, a bit for each of the 16 tokens of a step
+};
+__global__ void __launch_bounds__(kTileWaves * 64) __attribute__((amdgpu_waves_per_eu(2)))
+prefill_fp8_kernel(PrefillArgs<Fp8Cache> a) {
+  __shared__ __attribute__((aligned(16))) u8 s_mem[2 * sizeof(Stage) > kTurnBytes ? 2 * sizeof(Stage) : kTurnBytes];
+  Stage *stages = reinterpret_cast<Stage *>(s_mem);
+
+  Rows rows;
+  if (!find_rows(a, kTileRows, blockIdx.y, rows)) return;
+  const int g = blockIdx.x;
+  const int lane = threadIdx.x & 63;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int half = lane >> 5, n = lane & 31;
+  const int kv_len = rows.kv_len;
+  const int r0 = rows.first + 32 * w;  // the wave's first row
+  int row = min(r0 + n, rows.rows - 1);
+  const int last_seen = min(rows.offset + row / a.group, kv_len - 1);  // by this lane's row
+  const int wave_first = rows.offset + r0 / a.group;           // the last key that the wave's first row sees
+  const int wave_last = rows.offset + min(r0 + 31, rows.rows - 1) / a.group;
+  const int end_row = min(rows.first + kTileRows, rows.rows) - 1;
+  const int keys = min(kv_len, rows.offset + end_row / a.group + 1);  // that the workgroup needs
+  const int n_tiles = keys > 0 ? ceil_div(keys, kBK) : 0;
+
+  i32x8 q_hi[2], q_lo[2];
+  u32 q_scale[2];
+  load_query(a, rows, row, g, half, q_hi, q_lo, q_scale);
+
+  f32x16 acc[4];
 #pragma unroll
-  for (int d = 0; d < 32; ++d) q[d] = bf16_to_f32(qp[32 * part + d]);
-  float m = kNoScore, l = 0.f, o0 = 0.f, o1 = 0.f;
-  for (int t0 = 0; t0 < keys; t0 += kFp8Tile) {
-    int entry = a.block_tables[(int64_t)s * a.bt_stride + (t0 >> a.bs_log2)];
-    if ((unsigned)entry >= (unsigned)a.num_blocks && lane == 0) flag_index_error(a.err, NVAMD_ERR_BLOCK);
-    entry = min(max(entry, 0), a.num_blocks - 1);  // never leave the pool
-    const int64_t tile = fp8_tile(entry, t0 & ((1 << a.bs_log2) - 1), g, a.num_kv_heads, a.bs_log2);
-    const u8 *kc = a.cache.k_codes + tile * kFp8TileBytes, *vc = a.cache.v_codes + tile * kFp8TileBytes;
-    const float ks = fp8_scale(a.cache.k_scales[tile]), vs = fp8_scale(a.cache.v_scales[tile]);
-    float score = 0.f;
+  for (int db = 0; db < 4; ++db)
 #pragma unroll
-    for (int d = 0; d < 32; ++d) score += q[d] * code_value(kc, fp8_key_at(t, 32 * part + d), ks);
-    score += __shfl_xor(score, 16);
-    score += __shfl_xor(score, 32);
-    score = t0 + t < keys ? score * a.scale * kLog2e : -INFINITY;
-    float top = score;
-    for (int x = 1; x < 16; x *= 2) top = fmaxf(top, __shfl_xor(top, x));
-    const float up = fmaxf(m, top), alpha = fast_exp2(m - up), p = fast_exp2(score - up);
-    float sum = p;
-    for (int x = 1; x < 16; x *= 2) sum += __shfl_xor(sum, x);
-    l = l * alpha + sum;
-    o0 *= alpha;
-    o1 *= alpha;
-    m = up;
-    for (int i = 0; i < kFp8Tile && t0 + i < keys; ++i) {
-      const float w = __shfl(p, i);
-      o0 += w * code_value(vc, fp8_value_at(i, 2 * lane), vs);
-      o1 += w * code_value(vc, fp8_value_at(i, 2 * lane + 1), vs);
+    for (int i = 0; i < 16; ++i) acc[db][i] = 0.f;
+  float neg_ref = -kNoScore, l_run = 0.f;  // minus the exponent's reference; the sum at that reference
+
+  // The two 16-token tiles of each tile of keys (past the keys: their last one), looked up a tile ahead.
+  const_i32 *bt = (const_i32 *)(a.block_tables + (int64_t)blockIdx.z * a.bt_stride);
+  const int last_tile = max(kv_len - 1, 0) & ~15;
+  int entry[2];
+  auto look_up = [&](int t) {
+#pragma unroll
+    for (int x = 0; x < 2; ++x) entry[x] = bt[min(t * kBK + 16 * x, last_tile) >> a.bs_log2];
+  };
+  int tile[2];  // of the latest tile that was located
+  auto locate = [&](int t) {
+#pragma unroll
+    for (int x = 0; x < 2; ++x)
+      tile[x] = tile_of(a, entry[x], min(t * kBK + 16 * x, last_tile), g, threadIdx.x == 0);
+  };
+  // K: key 16a + 8b + 4c + x of the tile in row n = 16a + 8c + 4b + x.
+  const int k_token = (n & 3) | ((n & 8) >> 1) | ((n & 4) << 1);  // of its 16-token tile, n / 16
+  u32x4 kc[2][2];
+  u32 ks;
+  auto load_k = [&](int t0, int t1) {
+    const int64_t t = n < 16 ? t0 : t1;
+    const u8 *kp = a.cache.k_codes + t * kFp8TileBytes + k_token * 64 + 16 * half;
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+      for (int x = 0; x < 2; ++x) kc[s][x] = *reinterpret_cast<const u32x4 *>(kp + s * (kFp8TileBytes / 2) + 32 * x);
+    ks = a.cache.k_scales[t];
+  };
+  // V: wave w expands dims 32 w .. +31, a lane the 16 tokens of tile `half` of one.
+  u32x4 vc;
+  u32 vs;
+  auto load_v = [&]() {
+    const int64_t t = half ? tile[1] : tile[0];
+    vc = *reinterpret_cast<const u32x4 *>(a.cache.v_codes + t * kFp8TileBytes + (32 * w + n) * kFp8Tile);
+    vs = a.cache.v_scales[t];
+  };
+  const int sees_all = rows.offset + rows.first / a.group;  // keys up to here every row of the workgroup sees
+  auto on_diagonal = [&](int t) { return t * kBK + kBK - 1 > sees_all; };
+  auto expand = [&](int t, Stage &st) {
+    if (__builtin_expect(t * kBK + kBK > kv_len, 0)) keep_tokens(vc, kv_len - t * kBK - 16 * half);  // stale rows
+    if (__builtin_expect(on_diagonal(t), 0)) {
+      const u32 tokens = take_nans(vc);
+      const bool some = __builtin_amdgcn_ballot_w64(tokens != 0) != 0;
+      if (some) st.nan[w][n][half] = tokens;
+      if (lane == 0) st.any[w] = some;
+    }
+    const float scale = fp8_scale(vs);
+    st.v[half][w][n] = expand8<0>(vc, scale);
+    st.v[half][w][32 + n] = expand8<2>(vc, scale);
+  };
+
+  f32x16 sc;
+  auto score = [&]() {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) sc[i] = 0.f;
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      sc = mfma32_fp8_fp8(kc[s], ks, q_hi[s], q_scale[s], sc);
+      sc = mfma32_fp8_fp8(kc[s], ks, q_lo[s], q_scale[s], sc);
+    }
+  };
+  auto weigh = [&](int t, const Stage &st) {
+    const int base = t * kBK;
+    // Key of register i: base + 16 (i / 8) + 8 half + i % 8.
+    if (__builtin_expect(base + kBK - 1 > wave_first || base + kBK > kv_len, 0)) {
+      const int lim = last_seen - base - 8 * half;
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if (16 * (i / 8) + (i % 8) > lim) sc[i] = -INFINITY;
+    }
+    float tmax = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) tmax = fmaxf(tmax, sc[i]);
+    tmax = max_xor32(tmax) * a.scale_log2e;
+    // Lazy rescale: the weights stay below 2^8, and O and l are scaled only where some row's reference moves.
+    const bool up = tmax + neg_ref > kRescaleLog2;
+    if (__builtin_amdgcn_ballot_w64(up) != 0) {
+      const float alpha = up ? fast_exp2(-neg_ref - tmax) : 1.f;
+      if (up) neg_ref = -tmax;
+      l_run *= alpha;
+#pragma unroll
+      for (int db = 0; db < 4; ++db)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[db][i] *= alpha;
+    }
+    u32x4 pf[2];
+#pragma unroll
+    for (int hh = 0; hh < 2; ++hh)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const u32 pr = pack_bf16x2(fast_exp2(fmaf(sc[8 * hh + 2 * e], a.scale_log2e, neg_ref)),
+                                   fast_exp2(fmaf(sc[8 * hh + 2 * e + 1], a.scale_log2e, neg_ref)));
+        l_run = dot2_bf16(pr, kBf16PairOne, l_run);  // both rounded values of the pair
+        pf[hh][e] = pr;
+      }
+#pragma unroll
+    for (int hh = 0; hh < 2; ++hh)
+#pragma unroll
+      for (int db = 0; db < 4; ++db) acc[db] = mfma32(st.v[hh][db][lane], pf[hh], acc[db]);
+    if (__builtin_expect(on_diagonal(t), 0)) {
+      const int seen = last_seen - base;  // the last key of the tile that this lane's row sees
+      const u32 mask = seen < 0 ? 0u : seen >= 31 ? 0xffffffffu : (2u << seen) - 1u;
+#pragma unroll
+      for (int db = 0; db < 4; ++db) {
+        if (__builtin_amdgcn_readfirstlane(st.any[db]) == 0) continue;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const u32 *tokens = st.nan[db][8 * (i >> 2) + 4 * half + (i & 3)];
+          acc[db][i] += ((tokens[0] | tokens[1] << 16) & mask) != 0 ? NAN : 0.f;
+        }
+      }
+    }
+  };
+
+  if (n_tiles > 0) {
+    look_up(0);
+    locate(0);
+    load_k(tile[0], tile[1]);
+    load_v();
+    look_up(1);
+    expand(0, stages[0]);
+    locate(1);
+    load_v();
+    look_up(2);
+    __syncthreads();
+    // Here K holds tile t, V's registers tile t + 1, stage t % 2 V's operands of tile t; `tile` is t + 1's, `entry` t +
+    // 2's.
+#pragma unroll 1
+    for (int t = 0; t < n_tiles; ++t) {
+      const bool visible = r0 < rows.rows && t * kBK <= wave_last;
+      const int2 next = {tile[0], tile[1]};
+      if (t + 1 < n_tiles) {
+        expand(t + 1, stages[(t + 1) & 1]);
+        locate(t + 2);
+        load_v();
+        look_up(t + 3);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      if (visible) score();
+      __builtin_amdgcn_sched_barrier(0);
+      if (t + 1 < n_tiles) load_k(next.x, next.y);
+      if (visible) weigh(t, stages[t & 1]);
+      __syncthreads();
     }
   }
-  const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;  // no key: zeros; a NaN stays one
-  reinterpret_cast<u32 *>(a.out + (int64_t)(q_start + token) * a.out_stride + (int64_t)head * kHeadDim)[lane] =
-      pack_bf16x2(o0 * inv, o1 * inv);
+
+  write_tile_rows(a, rows, g, r0, row, w, lane, acc, l_run, s_mem);
 }
 
-int fill_args(AttentionArgs &a, void *out, int64_t out_stride, const void *q, int64_t q_stride, const void *k_codes,
-              const void *k_scales, const void *v_codes, const void *v_scales, int num_blocks, int block_size,
-              const int32_t *block_tables, int bt_stride, int bt_width, const int32_t *kv_lens, int num_heads,
-              int num_kv_heads, int head_dim, float scale) {
-  const int bs_log2 = log2_exact(block_size);
-  if (head_dim != kHeadDim || bs_log2 < 4) return NVAMD_EUNSUPPORTED;
-  if (!out || !q || !fp8_cache_ok(k_codes, k_scales, v_codes, v_scales) || !block_tables || !kv_lens || num_blocks <= 0 ||
-      num_kv_heads <= 0 || num_heads <= 0 || num_heads % num_kv_heads != 0 || bt_width <= 0 || bt_stride < bt_width ||
-      !aligned16(q) || !aligned16(out) || q_stride % 8 || out_stride % 8 || q_stride < (int64_t)num_heads * head_dim ||
-      out_stride < (int64_t)num_heads * head_dim)
-    return NVAMD_EINVAL;
-  if (((int64_t)bt_width << bs_log2) > 1 << 30 || (((int64_t)num_blocks * num_kv_heads) << bs_log2) >> 4 > 0x7fffffff)
-    return NVAMD_EUNSUPPORTED;
-  a = {};
-  a.out = static_cast<u16 *>(out);
-  a.out_stride = out_stride;
-  a.q = static_cast<const u16 *>(q);
-  a.q_stride = q_stride;
-  a.cache = Fp8Cache{const_cast<u8 *>(static_cast<const u8 *>(k_codes)),
-                     const_cast<u8 *>(static_cast<const u8 *>(k_scales)),
-                     const_cast<u8 *>(static_cast<const u8 *>(v_codes)),
-                     const_cast<u8 *>(static_cast<const u8 *>(v_scales))};
-  a.block_tables = block_tables;
-  a.bt_stride = bt_stride;
-  a.bt_width = bt_width;
-  a.num_blocks = num_blocks;
-  a.bs_log2 = bs_log2;
-  a.kv_lens = kv_lens;
-  a.num_kv_heads = num_kv_heads;
-  a.group = num_heads / num_kv_heads;
-  a.scale = scale;
-  a.err = index_error_word();
-  return NVAMD_OK;
+// ------------------------------------------------------------------------------------------ strips
+__global__ void __launch_bounds__(kStripWaves * 64) __attribute__((amdgpu_waves_per_eu(2)))
+prefill_strip_fp8_kernel(PrefillArgs<Fp8Cache> a) {
+  __shared__ __attribute__((aligned(16))) float s_o[kStripWaves][kStripRows / 2][kRec];
+  __shared__ float s_m[kStripWaves][kStripRows];
+  __shared__ float s_l[kStripWaves][kStripRows];
+
+  Rows rows;
+  if (!find_rows(a, kStripRows, blockIdx.y, rows)) return;
+  const int piece = blockIdx.x / a.num_kv_heads, g = blockIdx.x - piece * a.num_kv_heads;
+  const Cut cut = find_cut(a, rows, kStripRows);
+  if (piece >= cut.pieces) return;
+  const int begin = piece * cut.length, end = min(begin + cut.length, cut.keys);
+  const int lane = threadIdx.x & 63;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int half = lane >> 5, n = lane & 31;
+  const int row = min(rows.first + n, rows.rows - 1);
+  const int last_seen = min(rows.offset + row / a.group, rows.kv_len - 1);
+  const int first_seen = rows.offset + rows.first / a.group;  // the last key that the first row sees
+
+  i32x8 q_hi[2], q_lo[2];
+  u32 q_scale[2];
+  load_query(a, rows, row, g, half, q_hi, q_lo, q_scale);
+
+  f32x16 acc[4];
+#pragma unroll
+  for (int db = 0; db < 4; ++db)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) acc[db][i] = 0.f;
+  float neg_ref = -kNoScore, l_run = 0.f;  // minus the exponent's reference; the sum at that reference
+
+  const_i32 *bt = (const_i32 *)(a.block_tables + (int64_t)blockIdx.z * a.bt_stride);
+  const int last_tile = max(rows.kv_len - 1, 0) & ~15;
+  int entry[2], tile[2];
+  auto look_up = [&](int t0) {
+#pragma unroll
+    for (int x = 0; x < 2; ++x) entry[x] = bt[min(t0 + 16 * x, last_tile) >> a.bs_log2];
+  };
+  auto locate = [&](int t0) {
+#pragma unroll
+    for (int x = 0; x < 2; ++x) tile[x] = tile_of(a, entry[x], min(t0 + 16 * x, last_tile), g, lane == 0);
+  };
+  // Byte `at` of the lane's one of the two tiles.
+  auto in_tile = [&](const u8 *base, int second, int tile_bytes, u32 at) {  // (second as a bool: 25 us for 14)
+    return base + (int64_t)(second ? tile[1] : tile[0]) * tile_bytes + at;
+  };
+  // Row n of K is token 4 (n / 8) + n % 4 of tile (n / 4) % 2: then register i of the scores is token i of tile `half`.
+  const int k_token = 4 * (n >> 3) + (n & 3);
+  const int k_second = (n & 4) ? -1 : 0, v_second = -half;
+  u32x4 kc[2][2], vc[4];
+  u32 ks, vs;
+  auto load_k = [&]() {
+    const u8 *kp = in_tile(a.cache.k_codes, k_second, kFp8TileBytes, k_token * 64 + 16 * half);
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+      for (int x = 0; x < 2; ++x) kc[s][x] = *reinterpret_cast<const u32x4 *>(kp + s * (kFp8TileBytes / 2) + 32 * x);
+    ks = *in_tile(a.cache.k_scales, k_second, 1, 0);
+  };
+  // Dims n, 32 + n .. of V, 16 tokens of tile `half` each.
+  auto load_v = [&]() {
+    const u8 *vp = in_tile(a.cache.v_codes, v_second, kFp8TileBytes, n * kFp8Tile);
+#pragma unroll
+    for (int db = 0; db < 4; ++db) vc[db] = *reinterpret_cast<const u32x4 *>(vp + 32 * kFp8Tile * db);
+    vs = *in_tile(a.cache.v_scales, v_second, 1, 0);
+  };
+  auto step = [&](const int t0, const int next) {
+    f32x16 sc;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) sc[i] = 0.f;
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      sc = mfma32_fp8_fp8(kc[s], ks, q_hi[s], q_scale[s], sc);
+      sc = mfma32_fp8_fp8(kc[s], ks, q_lo[s], q_scale[s], sc);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    if (next < end) {
+      locate(next);
+      load_k();
+      look_up(next + 32 * kStripWaves);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    if (t0 + 31 > first_seen || t0 + 32 > rows.kv_len) {
+      const int lim = last_seen - t0 - 16 * half;
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if (i > lim) sc[i] = -INFINITY;
+    }
+    float tmax = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) tmax = fmaxf(tmax, sc[i]);
+    tmax = max_xor32(tmax) * a.scale_log2e;
+    const bool up = tmax + neg_ref > kRescaleLog2;
+    if (__builtin_amdgcn_ballot_w64(up) != 0) {
+      const float alpha = up ? fast_exp2(-neg_ref - tmax) : 1.f;
+      if (up) neg_ref = -tmax;
+      l_run *= alpha;
+#pragma unroll
+      for (int db = 0; db < 4; ++db)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[db][i] *= alpha;
+    }
+    u32x4 pf[2];
+#pragma unroll
+    for (int hh = 0; hh < 2; ++hh)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const u32 pr = pack_bf16x2(fast_exp2(fmaf(sc[8 * hh + 2 * e], a.scale_log2e, neg_ref)),
+                                   fast_exp2(fmaf(sc[8 * hh + 2 * e + 1], a.scale_log2e, neg_ref)));
+        l_run = dot2_bf16(pr, kBf16PairOne, l_run);
+        pf[hh][e] = pr;
+      }
+    if (t0 + 31 > first_seen || t0 + 32 > rows.kv_len) {
+#pragma unroll
+      for (int db = 0; db < 4; ++db) {
+        keep_tokens(vc[db], rows.kv_len - t0 - 16 * half);  // stale rows past the keys
+        const u32 bad = take_nans(vc[db]);                  // tokens of tile `half` whose value of dim 32 db + n is NaN
+        if (__builtin_expect(__builtin_amdgcn_ballot_w64(bad != 0) == 0, 1)) continue;
+#pragma unroll 1
+        for (int x = 0; x < 64; ++x) {  // dim 32 db + x % 32, tile x / 32
+          const u32 tokens = (u32)__builtin_amdgcn_readlane((int)bad, x);
+          if (tokens == 0) continue;
+          const int at = t0 + 16 * (x >> 5) + __ffs((int)tokens) - 1;  // the first of them
+          const bool hit = last_seen >= at && half == ((x >> 2) & 1);
+          const int reg = 4 * ((x & 31) >> 3) + (x & 3);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) acc[db][i] += hit && i == reg ? NAN : 0.f;
+        }
+      }
+    }
+    const float v_scale = fp8_scale(vs);
+#pragma unroll
+    for (int db = 0; db < 4; ++db) {
+      acc[db] = mfma32(expand8<0>(vc[db], v_scale), pf[0], acc[db]);
+      acc[db] = mfma32(expand8<2>(vc[db], v_scale), pf[1], acc[db]);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    if (next < end) load_v();
+  };
+  if (int t0 = begin + 32 * w; t0 < end) {
+    look_up(t0);
+    locate(t0);
+    load_k();
+    load_v();
+    look_up(t0 + 32 * kStripWaves);
+#pragma unroll 1
+    do {
+      step(t0, t0 + 32 * kStripWaves);
+      t0 += 32 * kStripWaves;
+    } while (t0 < end);
+  }
+
+  write_strip(a, rows, cut, piece, g, w, lane, acc, neg_ref, l_run, s_o, s_m, s_l, [](int db, int i, int half) {
+    return 32 * db + 2 * i + 4 * half;
+  });
+}
+
+// ------------------------------------------------------------------------------------------ few rows
+__global__ void __launch_bounds__(kFewWaves * 64) __attribute__((amdgpu_waves_per_eu(2)))
+prefill_few_fp8_kernel(PrefillArgs<Fp8Cache> a) {
+  constexpr int D = kHeadDim;
+  __shared__ __attribute__((aligned(16))) float s_o[kFewWaves][kFewRows * kRec];
+  __shared__ float s_m[kFewWaves][kFewRows];
+  __shared__ float s_l[kFewWaves][kFewRows];
+
+  Rows rows;
+  if (!find_rows(a, kFewRows, blockIdx.y, rows)) return;
+  const int piece = blockIdx.x / a.num_kv_heads, g = blockIdx.x - piece * a.num_kv_heads;
+  const Cut cut = find_cut(a, rows, kFewRows);
+  if (piece >= cut.pieces) return;
+  const int begin = piece * cut.length, end = min(begin + cut.length, cut.keys);
+  const int lane = threadIdx.x & 63;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int n = lane & 15, gq = lane >> 4;
+  const int row = min(rows.first + n, rows.rows - 1);
+  const int token = row / a.group, head = g * a.group + row - token * a.group;
+  const int last_seen = min(rows.offset + token, rows.kv_len - 1);
+  const int first_seen = rows.offset + rows.first / a.group;  // the last key that the first row sees
+
+  i32x8 q_hi, q_lo;
+  u32 q_scale;
+  {
+    const u16 *qp = a.q + (int64_t)(rows.q_start + token) * a.q_stride + (int64_t)head * D + 16 * gq;
+    const u32x4 x[4] = {ld16(qp), ld16(qp + 8), ld16(qp + 64), ld16(qp + 72)};
+    q_scale = query_operand(x, gq, q_hi, q_lo);
+  }
+
+  float m = kNoScore, m_thr = kNoScore, l = 0.f;
+  f32x4 o[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) o[e] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+  const int32_t *bt = a.block_tables + (int64_t)blockIdx.z * a.bt_stride;
+  const int last_tile = max(rows.kv_len - 1, 0) & ~15;
+  int entry_k = 0, entry_v = 0;
+  auto look_up = [&](int t0) {
+    entry_k = bt[min(t0 + 16 * (n >> 2), last_tile) >> a.bs_log2];
+    entry_v = bt[min(t0 + 16 * gq, last_tile) >> a.bs_log2];
+  };
+  u32x4 kc[4][2], vc[8];
+  u32 ks, vs;
+  int k_tile, v_tile;
+  auto locate = [&](int t0) {
+    k_tile = tile_of(a, entry_k, min(t0 + 16 * (n >> 2), last_tile), g, true);
+    v_tile = tile_of(a, entry_v, min(t0 + 16 * gq, last_tile), g, true);
+  };
+  auto load_k = [&]() {
+    const u8 *kp = a.cache.k_codes + (int64_t)k_tile * kFp8TileBytes + (n & 3) * 64 + 16 * gq;
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+        kc[t][x] = *reinterpret_cast<const u32x4 *>(kp + 4 * t * 64 + x * (kFp8TileBytes / 2));
+    ks = a.cache.k_scales[k_tile];
+  };
+  auto load_v = [&]() {
+    const u8 *vp = a.cache.v_codes + (int64_t)v_tile * kFp8TileBytes + n * kFp8Tile;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) vc[e] = *reinterpret_cast<const u32x4 *>(vp + 16 * kFp8Tile * e);
+    vs = a.cache.v_scales[v_tile];
+  };
+  auto step = [&](const int t0, const int next) {
+    f32x4 s[4];
+    score(s[0], kc[0], ks, q_hi, q_lo, q_scale);
+    score(s[1], kc[1], ks, q_hi, q_lo, q_scale);
+    score(s[2], kc[2], ks, q_hi, q_lo, q_scale);
+    score(s[3], kc[3], ks, q_hi, q_lo, q_scale);
+    __builtin_amdgcn_sched_barrier(0);
+    if (next < end) {
+      locate(next);
+      load_k();
+      look_up(next + 64 * kFewWaves);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    float cm = kNoScore;
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s[t][i] *= a.scale_log2e;
+    if (t0 + 63 > first_seen || t0 + 64 > rows.kv_len) {
+      const int lim = last_seen - t0 - 16 * gq;  // token 4 t + i of tile gq
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (4 * t + i > lim) s[t][i] = -INFINITY;
+    }
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) cm = fmaxf(cm, s[t][i]);
+    cm = max_over_quarters(cm);
+    if (__builtin_amdgcn_ballot_w64(cm > m_thr) != 0) {
+      const bool up = cm > m_thr;
+      const float alpha = up ? fast_exp2(m - cm) : 1.f;
+      if (up) {
+        m = cm;
+        m_thr = cm + kRescaleLog2;
+      }
+      l *= alpha;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) o[e] *= alpha;
+    }
+    u32x4 pf[2];
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const u32 pr = pack_bf16x2(fast_exp2(s[t][2 * i] - m), fast_exp2(s[t][2 * i + 1] - m));
+        l = dot2_bf16(pr, kBf16PairOne, l);
+        pf[t >> 1][2 * (t & 1) + i] = pr;
+      }
+    if (t0 + 63 > first_seen || t0 + 64 > rows.kv_len) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        keep_tokens(vc[e], rows.kv_len - t0 - 16 * gq);  // stale rows past the keys
+        const u32 bad = take_nans(vc[e]);                // tokens of tile gq whose value of dim 16 e + n is NaN
+        if (__builtin_expect(__builtin_amdgcn_ballot_w64(bad != 0) == 0, 1)) continue;
+#pragma unroll 1
+        for (int x = 0; x < 64; ++x) {  // dim 16 e + x % 16, tile x / 16
+          const u32 tokens = (u32)__builtin_amdgcn_readlane((int)bad, x);
+          if (tokens == 0) continue;
+          const int at = t0 + 16 * (x >> 4) + __ffs((int)tokens) - 1;  // the first of them
+          const bool hit = last_seen >= at && gq == ((x & 15) >> 2);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) o[e][i] += hit && i == (x & 3) ? NAN : 0.f;
+        }
+      }
+    }
+    const float v_scale = fp8_scale(vs);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) add_values(o[e], vc[e], v_scale, pf);
+    __builtin_amdgcn_sched_barrier(0);
+    if (next < end) load_v();
+  };
+  if (int t0 = begin + 64 * w; t0 < end) {
+    look_up(t0);
+    locate(t0);
+    load_k();
+    load_v();
+    look_up(t0 + 64 * kFewWaves);
+#pragma unroll 1
+    do {
+      step(t0, t0 + 64 * kFewWaves);
+      t0 += 64 * kFewWaves;
+    } while (t0 < end);
+  }
+
+  write_few(a, rows, cut, piece, g, w, lane, o, m, l, s_o, s_m, s_l);
 }
 
 }  // namespace
@@ -132,7 +560,7 @@ using namespace nvamd;
 
 extern "C" size_t nvamd_paged_prefill_fp8_workspace_size(int n_seqs, int max_q_len, int num_heads, int num_kv_heads,
                                                          int block_size, int bt_width) {
-  return 0;
+  return prefill_workspace_bytes(n_seqs, max_q_len, num_heads, num_kv_heads, block_size, bt_width);
 }
 
 extern "C" int nvamd_paged_prefill_fp8(void *out, int64_t out_stride, const void *q, int64_t q_stride,
@@ -142,18 +570,12 @@ extern "C" int nvamd_paged_prefill_fp8(void *out, int64_t out_stride, const void
                                        const int32_t *cu_seqlens_q, const int32_t *kv_lens, int n_seqs, int num_tokens,
                                        int max_q_len, int num_heads, int num_kv_heads, int head_dim, float scale,
                                        void *workspace, size_t workspace_bytes, hipStream_t stream) {
-  if (n_seqs == 0 || max_q_len == 0 || num_tokens == 0) return NVAMD_OK;
-  AttentionArgs a;
-  const int st = fill_args(a, out, out_stride, q, q_stride, k_codes, k_scales, v_codes, v_scales, num_blocks, block_size,
-                           block_tables, bt_stride, bt_width, kv_lens, num_heads, num_kv_heads, head_dim, scale);
-  if (st != NVAMD_OK) return st;
-  if (!(scale > 0.f) || !cu_seqlens_q || n_seqs < 0 || num_tokens < 0 || max_q_len < 0 || n_seqs > 65535)
-    return NVAMD_EINVAL;
-  if (max_q_len > 65535) return NVAMD_EUNSUPPORTED;
-  a.cu_seqlens_q = cu_seqlens_q;
-  a.max_q_len = max_q_len;
-  a.num_tokens = num_tokens;
-  a.max_ctx = 0x7fffffff;
-  hipLaunchKernelGGL(attention_fp8_kernel, dim3(num_heads, max_q_len, n_seqs), dim3(64), 0, stream, a);
-  return launch_status();
+  const Fp8Cache cache = {const_cast<u8 *>(static_cast<const u8 *>(k_codes)),
+                          const_cast<u8 *>(static_cast<const u8 *>(k_scales)),
+                          const_cast<u8 *>(static_cast<const u8 *>(v_codes)),
+                          const_cast<u8 *>(static_cast<const u8 *>(v_scales))};
+  return prefill(prefill_few_fp8_kernel, prefill_strip_fp8_kernel, prefill_fp8_kernel, cache,
+                 fp8_cache_ok(k_codes, k_scales, v_codes, v_scales), out, out_stride, q, q_stride, num_blocks, block_size,
+                 block_tables, bt_stride, bt_width, cu_seqlens_q, kv_lens, n_seqs, num_tokens, max_q_len, num_heads,
+                 num_kv_heads, head_dim, scale, workspace, workspace_bytes, stream);
 }

@@ -483,6 +483,24 @@ def test_prefill_few_rows(device, bs):
         check_prefill(batch, q, [q_len], batch.prefill(q, [q_len]))
 
 
+@pytest.mark.parametrize("hq, hkv, q_lens, cached, bs", [
+    (16, 8, [20], [4096], 128),                    # few rows, 9 pieces
+    (2, 1, [1, 3], [40_000, 5], 128),              # 32 pieces, and a context of one piece beside it
+    (4, 1, [17, 0, 30], [5000, 100, 0], 16),       # a sequence without rows, one without cached keys
+    (5, 1, [3], [511], 16), (5, 1, [3], [509], 16),  # two pieces, one
+    (16, 8, [300], [4096], 128),                   # strips
+    (6, 2, [300, 10, 100], [3000, 9000, 0], 16),
+])
+def test_prefill_cut_along_the_keys(device, hq, hkv, q_lens, cached, bs):
+    batch = Batch(device, [a + b for a, b in zip(q_lens, cached)], hq, hkv, bs, seed=hq, extra_width=4096 // bs)
+    width = batch.tables.shape[1]
+    assert _C.load().nvamd_paged_prefill_fp8_workspace_size(len(q_lens), max(q_lens), hq, hkv, bs, width) > 0
+    q = batch.queries(sum(q_lens))
+    got = batch.prefill(q, q_lens)
+    check_prefill(batch, q, q_lens, got)
+    assert torch.equal(got, batch.prefill(q, q_lens)) and _C.index_errors() == 0
+
+
 def test_prefill_cut_replays_from_a_graph(device):
     """Contexts that need one piece or many between the replays, and another call on another stream meanwhile."""
     batch = Batch(device, [9000, 300], 4, 2, 16, seed=9)

@@ -190,6 +190,15 @@ def test_prefill_argument_errors():
     assert call(hq=12) == EINVAL and call(n=65536) == EINVAL and call(bt_width=16) == EINVAL
     assert call(d=64) == EUNSUPPORTED and call(bs=8) == EUNSUPPORTED
     assert call(bt_width=(1 << 23) + 1, bt_stride=1 << 25) == EUNSUPPORTED  # past 2^30 tokens
+    need = lib.nvamd_paged_prefill_fp8_workspace_size
+    size = need(2, 10, 16, 8, 128, 320)
+    # 2 x 8 units of 2 x 16 rows, the keys cut in 256 / 32 pieces, 528 bytes a row
+    assert size == 2 * 8 * 32 * 8 * 528
+    long = dict(max_q=10, bt_width=320, bt_stride=320)
+    assert call(**long, ws=A, ws_bytes=size - 1) == EWORKSPACE and call(**long, ws=A + 8, ws_bytes=size) == EINVAL
+    assert need(2, 10, 16, 8, 128, 31) == 0                        # short contexts
+    for bad in ((0, 10, 16, 8, 128, 320), (2, 0, 16, 8, 128, 320), (2, 10, 4, 8, 128, 320), (2, 10, 16, 0, 128, 320)):
+        assert need(*bad) == 0
 
 
 def test_copy_blocks_argument_errors():
