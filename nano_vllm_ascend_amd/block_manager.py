@@ -257,6 +257,21 @@ class BlockManager:
         if row is not None:
             self._free_rows.append(row)
 
+    def fork_slot(self, slot: int, new_slot: int) -> list[tuple[int, int]]:
+        """Give ``new_slot`` the context of ``slot`` (not in the reference).  Full blocks are shared: nobody writes to them
+        again.  A partly filled one gets a copy of its own; returns the (source, target) blocks to copy, one pair at
+        most.  Nothing changes if the pool has no block for it."""
+        if new_slot in self.block_tables:
+            raise ValueError(f"slot {new_slot} is in use")
+        n = self.seq_lens[slot]
+        full, rest = divmod(n, self.block_size)
+        if rest and not self._free:
+            raise RuntimeError("BlockManager out of free blocks")
+        table = self.block_tables[slot]
+        self._init_slot(new_slot, n, table[:full])
+        self.ensure_blocks(new_slot, n)
+        return [(table[full], self.block_tables[new_slot][full])] if rest else []
+
     def clear_prefix_cache(self) -> None:
         if self.block_tables or any(block.ref_count > 0 for block in self.blocks):
             raise RuntimeError("cannot clear prefix cache with active sequences")

@@ -61,9 +61,10 @@ class LLM:
     readable as ``runner.last_logits``, at one logits-sized copy per overlapped
     step.  ``kv_cache_dtype="fp4"`` (not in the reference) holds the KV cache in
     4 bits: 3.76 times the tokens in the same memory, at the precision of 4-bit
-    keys and values.  A prompt without a cached prefix attends to its own keys as
-    they are; one with a cached prefix, and every decode step, to what the cache
-    holds.  (Prompts of both kinds admitted together run as two batches.)
+    keys and values; ``kv_cache_dtype="fp8"`` in 8 bits: twice the tokens.  A prompt
+    without a cached prefix attends to its own keys as they are; one with a cached
+    prefix, and every decode step, to what the cache holds.  (Prompts of both kinds
+    admitted together run as two batches.)
     """
 
     def __init__(self, model_path, max_model_len: int = 2048, block_size: int = 128, num_blocks: int | None = None,
@@ -98,6 +99,30 @@ class LLM:
         """Queue one request (a string, tokenized with the chat template, or token ids); return its id."""
         params = _params(sampling_params, temperature, top_k, top_p)
         return self._new_request(prompt, max_new_tokens, params).seq_id
+
+    def fork(self, request_id: int, max_new_tokens: int | None = None, sampling_params: SamplingParams | None = None, *,
+             temperature: float | None = None, top_k: int | None = None, top_p: float | None = None) -> int:
+        """Branch a running request between two steps (not in the reference); return the new request's id.
+
+        The new one goes on from the present state: the same prompt and tokens so far, the last sampled one among them.
+        It shares the full blocks of the context; a partly filled block is copied.  Its budget ``max_new_tokens`` counts
+        the tokens that it starts with, and like its sampling is that of the request it branches from unless given.
+        RuntimeError if it does not fit now (``max_num_seqs``, or its blocks for its whole life)."""
+        seq = self.scheduler.running.get(request_id)
+        if seq is None or seq.next_token_id is None:
+            raise ValueError(f"request {request_id} is not running")
+        budget = seq.max_new_tokens if max_new_tokens is None else int(max_new_tokens)
+        if budget <= len(seq.generated_token_ids):
+            raise ValueError(f"max_new_tokens {budget} is spent: request {request_id} has "
+                             f"{len(seq.generated_token_ids)} tokens")
+        blocks = self.scheduler.compute_required_blocks(runtime_prompt_len=seq.prompt_len, max_new_tokens=budget)
+        if not self.scheduler.fits(blocks):
+            raise RuntimeError(f"no room for a fork of request {request_id} ({blocks} blocks)")
+        params = _params(sampling_params or seq.sampling_params, temperature, top_k, top_p)
+        child = seq.fork(self.scheduler.next_seq_id(), budget, params)
+        child.reserved_blocks = blocks
+        self.runner.fork(seq, child)
+        return self.scheduler.add_running(child).seq_id
 
     def _output(self, seq: Sequence) -> dict[str, object]:
         tokens = list(seq.generated_token_ids)

@@ -41,12 +41,13 @@ from .block_manager import BlockManager, PagedKVCacheMetadata
 from .config import load_config
 from .graph import DecodeGraphRunner
 from .layers import RotaryEmbedding, Sampler
-from .paged_kv_cache import Fp4PagedKVCache, PagedKVCache
+from .paged_kv_cache import Fp4PagedKVCache, Fp8PagedKVCache, PagedKVCache
 from .qwen3 import Qwen3ForCausalLM, load_safetensors_dir
 from .sequence import Sequence
 
 DEFAULT_DECODE_GRAPH_BATCH_SIZES = [1, 2, 4, 8, 16, 32]
-KV_CACHE_DTYPES = ("bf16", "fp4")
+KV_CACHE_DTYPES = ("bf16", "fp4", "fp8")
+_QUANTISED = {"fp4": Fp4PagedKVCache, "fp8": Fp8PagedKVCache}
 
 
 class _TokenFetch:
@@ -136,8 +137,8 @@ class ModelRunner:
                                           max_blocks_per_seq=max(1, -(-max_model_len // block_size)))
         cfg = self.config
         pool = cfg.num_hidden_layers, self.num_blocks, block_size, cfg.num_key_value_heads, cfg.head_dim
-        self.kv_cache = (Fp4PagedKVCache(*pool, self.device) if kv_cache_dtype == "fp4"
-                         else PagedKVCache(*pool, self.dtype, self.device))
+        quantised = _QUANTISED.get(kv_cache_dtype)
+        self.kv_cache = quantised(*pool, self.device) if quantised else PagedKVCache(*pool, self.dtype, self.device)
         self.decode_graph_runner = None
         if enable_decode_graph:
             self.decode_graph_runner = DecodeGraphRunner(
@@ -192,7 +193,7 @@ class ModelRunner:
         free, total = torch.cuda.mem_get_info(self.device)
         budget = int(total * utilization) - (total - free)
         cfg = self.config
-        kind = Fp4PagedKVCache if self.kv_cache_dtype == "fp4" else PagedKVCache
+        kind = _QUANTISED.get(self.kv_cache_dtype, PagedKVCache)
         per_block = kind.bytes_per_block(cfg.num_hidden_layers, self.block_size, cfg.num_key_value_heads,
                                          cfg.head_dim)
         return max(1, budget // per_block)
@@ -289,11 +290,11 @@ class ModelRunner:
 
     def _by_route(self, seqs: list[Sequence]) -> list[list[Sequence]]:
         """The batches that prompts run in.  A batch takes one route: the paged one, over what the cache holds, if any of
-        its prompts has a cached prefix, else the dense one, over the prompts' own keys.  In a 4-bit cache the two differ by
-        the precision of the cache, and prompts with a prefix run apart from those without, so that none of them
+        its prompts has a cached prefix, else the dense one, over the prompts' own keys.  In a cache of 4 or 8 bits the two
+        differ by the precision of the cache, and prompts with a prefix run apart from those without, so that none of them
         depends on what the others hit.  (Those with a prefix first: new prompts may take unused cached blocks.)"""
         hits = [s for s in seqs if s.cached_prefix_len > 0]
-        if not isinstance(self.kv_cache, Fp4PagedKVCache) or len(hits) in (0, len(seqs)):
+        if not isinstance(self.kv_cache, tuple(_QUANTISED.values())) or len(hits) in (0, len(seqs)):
             return [seqs]
         return [hits, [s for s in seqs if s.cached_prefix_len == 0]]
 
@@ -416,6 +417,13 @@ class ModelRunner:
 
     def decode_graph_stats(self) -> dict[str, int]:
         return {} if self.decode_graph_runner is None else self.decode_graph_runner.stats_dict()
+
+    def fork(self, seq: Sequence, child: Sequence) -> None:
+        """The child's context: the full blocks of seq's, and a copy of a partly filled one."""
+        self._drop_in_flight()  # the next batch is another one
+        pairs = self.block_manager.fork_slot(seq.seq_id, child.seq_id)
+        if pairs:
+            self.kv_cache.copy_blocks(*zip(*pairs))
 
     def free_seq(self, seq: Sequence) -> None:
         self._drop_in_flight()  # a finishing sequence was in the launched batch

@@ -91,6 +91,17 @@ class MiniScheduler:
         return (len(self.waiting) > 0 and len(self.running) < self.max_num_seqs
                 and self.budget.fits(self.waiting[0].reserved_blocks))
 
+    def fits(self, blocks: int) -> bool:
+        """Whether one more running request with this reservation fits."""
+        return len(self.running) < self.max_num_seqs and self.budget.fits(blocks)
+
+    def add_running(self, seq: Sequence) -> Sequence:
+        """A request that runs already (a fork): it reserves its blocks and joins the next plan."""
+        self.seqs[seq.seq_id] = seq
+        self.budget.take(seq.reserved_blocks)
+        self.running[seq.seq_id] = seq
+        return seq
+
     def retire(self, seq: Sequence, reason: str) -> None:
         """Move a running request to ``finished`` and return its reservation."""
         self.running.pop(seq.seq_id)

@@ -100,6 +100,16 @@ class Sequence:
         self._decode_steps += 1
         self._pending = next_token_id
 
+    def fork(self, seq_id: int, max_new_tokens: int, sampling_params: Any) -> "Sequence":
+        """A request of its own that goes on from this one's state: the same tokens so far, the pending one among them."""
+        child = Sequence(seq_id, self.prompt, max_new_tokens, self.prompt_token_ids, sampling_params)
+        for name in ("status", "estimated_prompt_len", "cached_prefix_len", "runtime_prompt_token_ids",
+                     "runtime_prompt_len", "prompt_len", "_pending", "_decode_steps"):
+            setattr(child, name, getattr(self, name))
+        child.cached_block_ids = list(self.cached_block_ids)
+        child.generated_token_ids = list(self.generated_token_ids)
+        return child
+
     def finish(self, reason: str | None = None) -> None:
         self.status = SequenceStatus.FINISHED
         self.finish_reason = reason
