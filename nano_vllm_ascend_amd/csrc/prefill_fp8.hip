@@ -62,7 +62,7 @@ struct Stage {
   u32 any[4];         // on the diagonal, [wave that expanded them]: whether any of its values read as NaN,
   u32 nan[4][32][2];  // and which: of each dim, a bit for each of the 16 tokens of a step
 };
-__global__ void __launch_bounds__(kTileWaves * 64) __attribute__((amdgpu_waves_per_eu(2)))
+__global__ void __launch_bounds__(kTileWaves * 64) __attribute__((amdgpu_waves_per_eu(3)))
 prefill_fp8_kernel(PrefillArgs<Fp8Cache> a) {
   __shared__ __attribute__((aligned(16))) u8 s_mem[2 * sizeof(Stage) > kTurnBytes ? 2 * sizeof(Stage) : kTurnBytes];
   Stage *stages = reinterpret_cast<Stage *>(s_mem);
@@ -76,7 +76,11 @@ prefill_fp8_kernel(PrefillArgs<Fp8Cache> a) {
   const int kv_len = rows.kv_len;
   const int r0 = rows.first + 32 * w;  // the wave's first row
   int row = min(r0 + n, rows.rows - 1);
-  const int last_seen = min(rows.offset + row / a.group, kv_len - 1);  // by this lane's row
+  auto last_seen = [&]() {  // by this lane's row; made anew where it is needed: it would hold a register through the loop
+    int r = row;
+    asm volatile("" : "+v"(r));
+    return min(rows.offset + r / a.group, kv_len - 1);
+  };
   const int wave_first = rows.offset + r0 / a.group;           // the last key that the wave's first row sees
   const int wave_last = rows.offset + min(r0 + 31, rows.rows - 1) / a.group;
   const int end_row = min(rows.first + kTileRows, rows.rows) - 1;
@@ -158,7 +162,7 @@ prefill_fp8_kernel(PrefillArgs<Fp8Cache> a) {
     const int base = t * kBK;
     // Key of register i: base + 16 (i / 8) + 8 half + i % 8.
     if (__builtin_expect(base + kBK - 1 > wave_first || base + kBK > kv_len, 0)) {
-      const int lim = last_seen - base - 8 * half;
+      const int lim = last_seen() - base - 8 * half;
 #pragma unroll
       for (int i = 0; i < 16; ++i)
         if (16 * (i / 8) + (i % 8) > lim) sc[i] = -INFINITY;
@@ -193,15 +197,17 @@ prefill_fp8_kernel(PrefillArgs<Fp8Cache> a) {
 #pragma unroll
       for (int db = 0; db < 4; ++db) acc[db] = mfma32(st.v[hh][db][lane], pf[hh], acc[db]);
     if (__builtin_expect(on_diagonal(t), 0)) {
-      const int seen = last_seen - base;  // the last key of the tile that this lane's row sees
+      const int seen = last_seen() - base;  // the last key of the tile that this lane's row sees
       const u32 mask = seen < 0 ? 0u : seen >= 31 ? 0xffffffffu : (2u << seen) - 1u;
 #pragma unroll
       for (int db = 0; db < 4; ++db) {
         if (__builtin_amdgcn_readfirstlane(st.any[db]) == 0) continue;
+#pragma unroll 1
+        for (int x = 0; x < 16; ++x) {  // a register at a time: unrolled, the loads would take registers from the loop
+          const u32 *tokens = st.nan[db][8 * (x >> 2) + 4 * half + (x & 3)];
+          const float poison = ((tokens[0] | tokens[1] << 16) & mask) != 0 ? NAN : 0.f;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const u32 *tokens = st.nan[db][8 * (i >> 2) + 4 * half + (i & 3)];
-          acc[db][i] += ((tokens[0] | tokens[1] << 16) & mask) != 0 ? NAN : 0.f;
+          for (int i = 0; i < 16; ++i) acc[db][i] += i == x ? poison : 0.f;
         }
       }
     }
