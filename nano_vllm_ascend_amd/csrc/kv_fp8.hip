@@ -5,6 +5,11 @@
 // that follow one another, as their slots do.  It finds the runs that begin among its own rows by itself, from the
 // slots.  A key's row is 8 lanes of 16 dims (the rotation then needs no lane exchange); of the values a lane takes two
 // dims of all tokens, so that what it writes, 16 tokens of a dim in consecutive bytes, needs no transpose.
+//
+// All three are bound by memory: per head vector 256 bytes of bf16 and 128 of the cache, once.  12,345 tokens of 8 kv
+// heads written and read back 152 MB in 30 us (5.0 TB/s); 36,488 tokens of prompts, 16 query heads, rotated and stored with
+// the keys returned 598 MB in 139 us (4.3 TB/s: the 64-bit arithmetic is 40% of its time and hides behind four waves a
+// SIMD; at two it took 164), read back 243 MB in 38 us (6.4).  One token: 3 us, the launch.
 #include "fp8_rows.h"
 #include "norm_rope64.h"
 
@@ -45,6 +50,8 @@ struct RowsArgs {
   const float *cos_sin;
   int max_positions;
   int num_heads;  // 0: rows are only stored
+  int q_heads;    // of a wave
+  int k_heads;
   float eps;
 };
 
@@ -63,6 +70,14 @@ __device__ __forceinline__ void rope_row(const RowsArgs &a, int64_t t, int c, bo
     cs[e] = e < 4 ? c0[e & 3] : c1[e & 3];
     sn[e] = e < 4 ? s0[e & 3] : s1[e & 3];
   }
+}
+
+// Keeps the conversions of a row's 16 numbers and of the weights inside a loop over heads: hoisted, they would hold 64
+// registers and with them half of the waves.
+__device__ __forceinline__ void keep_here(float (&cs)[8], float (&sn)[8], u32x4 &w_lo, u32x4 &w_hi) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) asm volatile("" : "+v"(cs[e]), "+v"(sn[e]));
+  asm volatile("" : "+v"(w_lo), "+v"(w_hi));
 }
 
 // Runs among rows base .. base + ROWS - 1: calls body(first row, its slot, rows).  A run is rows whose slots follow one
@@ -90,25 +105,30 @@ __device__ __forceinline__ void for_runs(const RowsArgs &a, int64_t base, int la
 }
 
 // Heads that a wave of the rotation takes one after another: the table's rows and the weights are read once for them.
-constexpr int kRopeHeads = 8;
+// Fewer where that leaves less than four waves for each SIMD of 256 CUs.  us, with the rows read back, of 36,488 tokens at
+// query / key heads of 8 / 8, 8 / 4, 8 / 2, 4 / 4, 1 / 1: 183, 176, 179, 188, 201; of 2,600 tokens 47 (8 / 8), 20 (1 / 1).
+constexpr int kQueryHeads = 8, kKeyHeads = 4;
+constexpr int kWantedWaves = 4096;
 
 // blockIdx.y: groups of query heads, groups of key heads (of one without the rotation), value heads.  ROWS rows of the
 // call to a wave: 16, or 1 where there are few.
 template <bool ROPE, int ROWS>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(4)))
 rows_fp8_kernel(RowsArgs a) {
+  // A lane's own numbers of the table for its two tokens of a run: kept in registers they take 32, and with them one wave
+  // of four.
+  __shared__ f32x4 s_turn[ROPE ? kWaves : 1][2][4][ROPE ? 64 : 1];
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int c = lane & 7, tok = lane >> 3;
   const int64_t base = ((int64_t)blockIdx.x * kWaves + w) * ROWS;
   if (base >= a.num_tokens) return;
   const int hkv = a.num_kv_heads;
-  constexpr int kHeads = ROPE && ROWS > 1 ? kRopeHeads : 1;  // key heads of a wave
   int y = blockIdx.y;
   if constexpr (ROPE) {
-    const int q_groups = (a.num_heads + kRopeHeads - 1) / kRopeHeads;
+    const int q_groups = (a.num_heads + a.q_heads - 1) / a.q_heads;
     if (y < q_groups) {
-      const int h0 = y * kRopeHeads, h1 = min(h0 + kRopeHeads, a.num_heads);
-      const u32x4 w_lo = ld16(a.q_w + 8 * c), w_hi = ld16(a.q_w + 64 + 8 * c);
+      const int h0 = y * a.q_heads, h1 = min(h0 + a.q_heads, a.num_heads);
+      u32x4 w_lo = ld16(a.q_w + 8 * c), w_hi = ld16(a.q_w + 64 + 8 * c);
       // 16 rows: 8 at a time, head after head; one row: its heads at a time.
 #pragma unroll 1
       for (int p = 0; p < (ROWS + 7) / 8; ++p) {
@@ -117,14 +137,22 @@ rows_fp8_kernel(RowsArgs a) {
         const int64_t tt = exists ? t : base;
         float cs[8], sn[8];
         rope_row(a, tt, c, y == 0 && c == 0 && (ROWS > 1 || tok == 0), cs, sn);
+        auto head_of = [&](int i) { return ROWS == 1 ? min(h0 + tok, h1 - 1) : i; };
+        auto source = [&](int i) { return a.q + tt * a.q_stride + head_of(i) * kHeadDim + 8 * c; };
+        const int end = ROWS == 1 ? h0 + 1 : h1;
+        u32x4 next_lo = ld16(source(h0)), next_hi = ld16(source(h0) + 64);
 #pragma unroll 1
-        for (int i = h0; i < (ROWS == 1 ? h0 + 1 : h1); ++i) {
-          const int h = ROWS == 1 ? min(h0 + tok, h1 - 1) : i;
-          const u16 *src = a.q + tt * a.q_stride + h * kHeadDim + 8 * c;
-          u32x4 lo = ld16(src), hi = ld16(src + 64);
+        for (int i = h0; i < end; ++i) {
+          u32x4 lo = next_lo, hi = next_hi;
+          if (i + 1 < end) {  // the next head's row is on its way during this one's work
+            next_lo = ld16(source(i + 1));
+            next_hi = ld16(source(i + 1) + 64);
+          }
+          keep_here(cs, sn, w_lo, w_hi);
           const double rstd = norm_factor(dpp_sum8(sum_squares(lo, hi)), (double)a.eps);
+          asm volatile("" : "+v"(lo), "+v"(hi));  // the row's 64-bit numbers are made anew
           norm_rope_f64(lo, hi, w_lo, w_hi, cs, sn, rstd);
-          u16 *dst = a.q_out + tt * a.q_out_stride + h * kHeadDim + 8 * c;
+          u16 *dst = a.q_out + tt * a.q_out_stride + head_of(i) * kHeadDim + 8 * c;
           if (exists && (ROWS > 1 || h0 + tok < h1)) {
             st16(dst, lo);
             st16(dst + 64, hi);
@@ -135,14 +163,13 @@ rows_fp8_kernel(RowsArgs a) {
     }
     y -= q_groups;
   }
-  const int k_groups = (hkv + kHeads - 1) / kHeads;
+  const int k_groups = (hkv + a.k_heads - 1) / a.k_heads;
   if (y < k_groups) {
-    const int h0 = y * kHeads, h1 = min(h0 + kHeads, hkv);
+    const int h0 = y * a.k_heads, h1 = min(h0 + a.k_heads, hkv);
     for_runs<ROWS>(a, base, lane, y == 0, ROPE && a.k_out != nullptr, [&](int64_t row, int64_t slot, int n) {
       const int o = slot < 0 ? 0 : (int)(slot & (kFp8Tile - 1));
       const int64_t block = slot < 0 ? 0 : slot >> a.bs_log2;
       const int token = slot < 0 ? 0 : (int)(slot & ((1 << a.bs_log2) - 1));
-      float cs[2][8], sn[2][8];
       u32x4 w_lo, w_hi;
       int64_t at[2];  // of the lane's two tokens; lanes without one read the first row's
       bool in[2];
@@ -156,7 +183,15 @@ rows_fp8_kernel(RowsArgs a) {
         w_lo = ld16(a.k_w + 8 * c);
         w_hi = ld16(a.k_w + 64 + 8 * c);
 #pragma unroll
-        for (int p = 0; p < 2; ++p) rope_row(a, at[p], c, false, cs[p], sn[p]);
+        for (int p = 0; p < 2; ++p) {
+          float cs[8], sn[8];
+          rope_row(a, at[p], c, false, cs, sn);
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            s_turn[w][p][x][lane] = f32x4{cs[4 * x], cs[4 * x + 1], cs[4 * x + 2], cs[4 * x + 3]};
+            s_turn[w][p][2 + x][lane] = f32x4{sn[4 * x], sn[4 * x + 1], sn[4 * x + 2], sn[4 * x + 3]};
+          }
+        }
       }
 #pragma unroll 1
       for (int h = h0; h < h1; ++h) {
@@ -168,8 +203,17 @@ rows_fp8_kernel(RowsArgs a) {
           const u16 *src = a.k + at[p] * a.k_stride + h * kHeadDim + 8 * c;
           u32x4 lo = ld16(src), hi = ld16(src + 64);
           if constexpr (ROPE) {
+            asm volatile("" ::: "memory");  // read anew for each head
+            float cs[8], sn[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              cs[e] = s_turn[w][p][e >> 2][lane][e & 3];
+              sn[e] = s_turn[w][p][2 + (e >> 2)][lane][e & 3];
+            }
+            keep_here(cs, sn, w_lo, w_hi);
             const double rstd = norm_factor(dpp_sum8(sum_squares(lo, hi)), (double)a.eps);
-            norm_rope_f64(lo, hi, w_lo, w_hi, cs[p], sn[p], rstd);
+            asm volatile("" : "+v"(lo), "+v"(hi));
+            norm_rope_f64(lo, hi, w_lo, w_hi, cs, sn, rstd);
             if (a.k_out != nullptr && in[p]) {
               u16 *dst = a.k_out + at[p] * a.k_out_stride + h * kHeadDim + 8 * c;
               st16(dst, lo);
@@ -290,16 +334,25 @@ kv_read_fp8_kernel(ReadArgs a) {
   }
 }
 
-// Rows of a wave: 16 where that leaves enough waves.
-constexpr int kFewTokens = 2048;
+// A wave looks after the runs that begin in one row up to here, in 16 rows from there on.  us, one / 16: 300 rows written
+// and read back 9.1 / 11.8, 1,000 11.8 / 11.6 (the host's time), 2,000 16.4 / 11.1, 4,000 26 / 12; 500 prompt rows rotated
+// and stored 10.7 / 12.0.
+constexpr int kFewTokens = 512;
 
 template <bool ROPE>
-int launch_rows(const RowsArgs &a, hipStream_t stream) {
+int launch_rows(RowsArgs &a, hipStream_t stream) {
   const bool few = a.num_tokens <= kFewTokens;
-  const int heads = ROPE && !few ? kRopeHeads : 1;
-  const int y = (ROPE ? ceil_div(a.num_heads, kRopeHeads) : 0) + ceil_div(a.num_kv_heads, heads) + a.num_kv_heads;
+  const int64_t windows = ceil_div(a.num_tokens, few ? 1 : 16);
+  // one row: its query heads side by side in a wave; else and of keys one after another
+  a.q_heads = kQueryHeads;
+  a.k_heads = ROPE && !few ? kKeyHeads : 1;
+  if (ROPE && !few) {
+    while (a.q_heads > 1 && windows * ceil_div(a.num_heads, a.q_heads) < kWantedWaves) a.q_heads /= 2;
+    while (a.k_heads > 1 && windows * ceil_div(a.num_kv_heads, a.k_heads) < kWantedWaves) a.k_heads /= 2;
+  }
+  const int y = (ROPE ? ceil_div(a.num_heads, a.q_heads) : 0) + ceil_div(a.num_kv_heads, a.k_heads) + a.num_kv_heads;
   if (y > 65535) return NVAMD_EUNSUPPORTED;
-  const dim3 grid((unsigned)ceil_div(a.num_tokens, kWaves * (few ? 1 : 16)), (unsigned)y);
+  const dim3 grid((unsigned)((windows + kWaves - 1) / kWaves), (unsigned)y);
   if (few)
     hipLaunchKernelGGL((rows_fp8_kernel<ROPE, 1>), grid, dim3(kThreads), 0, stream, a);
   else

@@ -76,7 +76,7 @@ def some_slots(t, nb, bs, order, seed):
 
 
 SIZES = [(1, 8, 128), (1, 1, 16), (2, 3, 16), (11, 2, 32), (15, 8, 32), (16, 8, 128), (17, 5, 16), (33, 8, 64), (100, 1, 256),
-         (257, 4, 128), (2049, 1, 64), (2100, 2, 16)]  # one row to a wave up to 2,048
+         (257, 4, 128), (512, 1, 32), (513, 2, 64), (2049, 1, 64), (2100, 2, 16)]  # one row to a wave up to 512
 
 
 @pytest.mark.parametrize("order", ["page", "odd", "short"])
@@ -226,7 +226,8 @@ def table_of(positions):
 @pytest.mark.parametrize("t, hq, hkv, bs, order", [(1, 16, 8, 128, "page"), (1, 1, 1, 16, "odd"), (7, 16, 8, 16, "short"),
                                                    (33, 40, 8, 64, "odd"), (130, 16, 8, 128, "page"),
                                                    (300, 2, 1, 32, "odd"), (65, 24, 3, 256, "short"),
-                                                   (2060, 9, 2, 128, "odd"), (2049, 3, 1, 16, "page")])
+                                                   (2060, 9, 2, 128, "odd"), (2049, 3, 1, 16, "page"),
+                                                   (512, 9, 5, 32, "odd"), (513, 17, 5, 32, "short")])
 def test_norm_rope_stores_the_code_of_the_exact_key(device, t, hq, hkv, bs, order, keys):
     nb, table = (-(-(t + 5) // bs) + 1 if order != "short" else t), table_of(40960)
     gen = torch.Generator().manual_seed(t)
