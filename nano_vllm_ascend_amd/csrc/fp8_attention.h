@@ -29,6 +29,10 @@ __device__ __forceinline__ u32x4 expand8(u32x4 codes, float scale) {
   return u32x4{fp8_pair<false>(codes[I], scale), fp8_pair<true>(codes[I], scale), fp8_pair<false>(codes[I + 1], scale),
                fp8_pair<true>(codes[I + 1], scale)};
 }
+__device__ __forceinline__ u32x4 expand8(u32x2 codes, float scale) {
+  return u32x4{fp8_pair<false>(codes[0], scale), fp8_pair<true>(codes[0], scale), fp8_pair<false>(codes[1], scale),
+               fp8_pair<true>(codes[1], scale)};
+}
 // o += V^T P^T for 16 dims and the 64 tokens of a wave's step: lane (n, gq) has the codes of dim n, the 16 tokens of tile
 // gq, and that tile's scale.
 __device__ __forceinline__ void add_values(f32x4 &o, u32x4 codes, float scale, const u32x4 (&p)[2]) {

@@ -33,6 +33,7 @@ namespace nvamd {
 namespace {
 
 constexpr int kWaves = 8;
+constexpr int kLeastPart = 64 * kWaves;  // tokens of the smallest partition: one step of each wave
 
 // The new token's k (normed and rotated) and v of a kv head into its slot: lanes 0 .. 7 of a wave the key, 8 .. 15 the
 // value, whose bytes go through 512 bytes of LDS.
@@ -81,7 +82,7 @@ paged_decode_fp4_kernel(DecodeArgs<Fp4Cache> a, std::conditional_t<FUSED, StepAr
 
   u32 err_bits = 0;
   Part part;
-  if (!find_part(a, blockIdx.x, lane, kLeastPart<kWaves>, err_bits, part)) return;
+  if (!find_part(a, blockIdx.x, lane, kLeastPart, err_bits, part)) return;
   const int b = part.b, g = part.g, p = part.p, ctx = part.ctx, part_tokens = part.tokens;
   const int n = lane & 15, gq = lane >> 4;
   const int head0 = g * a.q_group + a.q_head0;
@@ -272,6 +273,8 @@ paged_decode_fp4_kernel(DecodeArgs<Fp4Cache> a, std::conditional_t<FUSED, StepAr
   }
 
   report(a.err, err_bits, lane);
+  if constexpr (GP <= 4) l += dpp<kRowRor4>(l);
+  if constexpr (GP <= 8) l += dpp<kDppRowRor8>(l);
   finish<kWaves, GP>(a, part, head0, tid, w, o, m, l, s_o, s_m, s_l, s_last);
 }
 
@@ -308,7 +311,7 @@ extern "C" int nvamd_paged_decode_fp4(void *out, int64_t out_stride, const void 
                                       size_t workspace_bytes, hipStream_t stream) {
   if (batch == 0) return NVAMD_OK;
   DecodeArgs<Fp4Cache> a;
-  const int st = fill_decode_args<kWaves>(a, out, out_stride, q, q_stride, cache_of(k_codes, k_scales, v_codes, v_scales),
+  const int st = fill_decode_args<kLeastPart>(a, out, out_stride, q, q_stride, cache_of(k_codes, k_scales, v_codes, v_scales),
                                     fp4_cache_ok(k_codes, k_scales, v_codes, v_scales), num_blocks, block_size,
                                     block_tables, bt_stride, bt_width, context_lens, batch, num_heads, num_kv_heads,
                                     head_dim, scale, max_context_len, workspace, workspace_bytes);
@@ -328,7 +331,7 @@ extern "C" int nvamd_paged_decode_fused_fp4(void *out, int64_t out_stride, const
                                             hipStream_t stream) {
   if (batch == 0) return NVAMD_OK;
   DecodeArgs<Fp4Cache> a;
-  int st = fill_decode_args<kWaves>(a, out, out_stride, q, q_stride, cache_of(k_codes, k_scales, v_codes, v_scales),
+  int st = fill_decode_args<kLeastPart>(a, out, out_stride, q, q_stride, cache_of(k_codes, k_scales, v_codes, v_scales),
                                     fp4_cache_ok(k_codes, k_scales, v_codes, v_scales), num_blocks, block_size,
                                     block_tables, bt_stride, bt_width, context_lens, batch, num_heads, num_kv_heads,
                                     head_dim, scale, max_context_len, workspace, workspace_bytes);

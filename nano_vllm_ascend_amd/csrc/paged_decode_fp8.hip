@@ -25,6 +25,8 @@ namespace nvamd {
 namespace {
 
 constexpr int kWaves = 8;
+constexpr int kStep = 32;                   // tokens of a wave
+constexpr int kLeastPart = 64 * kWaves;     // of the smallest partition: two steps of each wave
 
 // The new token's k (normed and rotated) into its slot, by a wave: every 8 lanes make the row, those of the token keep it.
 __device__ __forceinline__ void store_key_row(const Fp8Cache &cache, const StepArgs &s, int b, int g, int64_t slot,
@@ -74,7 +76,7 @@ __device__ __forceinline__ void store_value_row(const Fp8Cache &cache, const Ste
 // key, another the value) and waits for it, so that its loads find it.  Bits as of nvamd_qk_norm_rope_fp8 and this kernel
 // after it.
 template <int GP, bool WIDE, bool FUSED>
-__global__ void __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(2)))
+__global__ void __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(4)))
 paged_decode_fp8_kernel(DecodeArgs<Fp8Cache> a, std::conditional_t<FUSED, StepArgs, Nothing> step_args) {
   __shared__ __attribute__((aligned(16))) float s_o[kWaves][GP * kPartFloats];
   __shared__ float s_m[kWaves][GP];
@@ -87,7 +89,7 @@ paged_decode_fp8_kernel(DecodeArgs<Fp8Cache> a, std::conditional_t<FUSED, StepAr
 
   u32 err_bits = 0;
   Part part;
-  if (!find_part(a, blockIdx.x, lane, kLeastPart<kWaves>, err_bits, part)) return;
+  if (!find_part(a, blockIdx.x, lane, kLeastPart, err_bits, part)) return;
   const int b = part.b, g = part.g, p = part.p, ctx = part.ctx, part_tokens = part.tokens;
   const int n = lane & 15, gq = lane >> 4;
   const int head0 = g * a.q_group + a.q_head0;
@@ -122,114 +124,92 @@ paged_decode_fp8_kernel(DecodeArgs<Fp8Cache> a, std::conditional_t<FUSED, StepAr
 #pragma unroll
   for (int e = 0; e < 8; ++e) o[e] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-  // A step's 64 tokens are the four tiles t0 .. t0+63.  The tile of each 16 lanes, as row owners of K (tile n / 4) and
-  // as token owners of V (tile gq); tiles past the context repeat its last one.
+  // A step's 32 tokens are two tiles: a lane owns a row of K in tile n / 8 and tokens of V in tile gq / 2.  Tiles past the
+  // context repeat its last one.
   typedef const __attribute__((address_space(4))) int32_t const_i32;  // nothing writes the table: scalar loads
   const_i32 *bt = (const_i32 *)bt_row;
   const int t_end = min((p + 1) * part_tokens, ctx);
   const int last = (ctx - 1) & ~15;
   // The table's entries are asked for a step before their tiles.
-  int entry_k = 0, entry_v = 0;
+  int entry[2];
   auto look_up = [&](int t0) {
-    if constexpr (WIDE) {
-      entry_k = bt[min(t0, last) >> a.bs_log2];
-    } else {
-      entry_k = bt_row[min(t0 + 16 * (n >> 2), last) >> a.bs_log2];
-      entry_v = bt_row[min(t0 + 16 * gq, last) >> a.bs_log2];
-    }
+    entry[0] = bt[min(t0, last) >> a.bs_log2];
+    if constexpr (!WIDE) entry[1] = bt[min(t0 + 16, last) >> a.bs_log2];
   };
-  // Where the next tiles lie: a tile that the lanes share (a scalar, WIDE) and each lane's tiles past it.
-  int tile0 = 0;
-  u32 k_tile = 0, v_tile = 0;
+  int tile[2];  // of the pool, scalars
   auto locate = [&](int t0) {
     auto page = [&](int t, int e) {
       if ((unsigned)e >= (unsigned)a.num_blocks) err_bits |= NVAMD_ERR_BLOCK;
       return (int)fp8_tile(min(max(e, 0), a.num_blocks - 1), t & bs_mask, g, hkv, a.bs_log2);  // never leave the pool
     };
-    if constexpr (WIDE) {
-      tile0 = page(t0, entry_k);
-      const int tiles = (last - t0) >> 4;  // 0 .. 3, or more: the last tile that exists
-      k_tile = min(n >> 2, tiles);
-      v_tile = min(gq, tiles);
-    } else {
-      k_tile = page(min(t0 + 16 * (n >> 2), last), entry_k);
-      v_tile = page(min(t0 + 16 * gq, last), entry_v);
-    }
+    tile[0] = page(t0, entry[0]);
+    tile[1] = WIDE ? tile[0] + (t0 + 16 <= last ? 1 : 0) : page(min(t0 + 16, last), entry[1]);
   };
-  // Byte `at` of tile `tile0 + tile`: a 32-bit offset from a scalar address where the tiles lie in one page.
-  auto in_tiles = [&](const u8 *base, u32 tile, int tile_bytes, u32 at) {
-    if constexpr (WIDE) return base + (int64_t)tile0 * tile_bytes + (tile * tile_bytes + at);
-    else return base + (int64_t)tile * tile_bytes + at;
+  // Byte `at` of the lane's one of the two tiles: a 32-bit offset from a scalar address where they lie in one page.
+  auto in_tile = [&](const u8 *base, bool second, int tile_bytes, u32 at) {
+    if constexpr (WIDE) return base + (int64_t)tile[0] * tile_bytes + ((second ? (tile[1] - tile[0]) * tile_bytes : 0) + at);
+    else return base + (int64_t)(second ? tile[1] : tile[0]) * tile_bytes + at;
   };
-  u32x4 kc[4][2], vc[8];
-  u32 ks, vs;  // scale bytes of the tile that the lane owns a row of K in, and of tile gq
+  u32x4 kc[2][2];
+  u32x4 vc[4];  // 16 tokens of dims 64 (gq % 2) + 16 j + n
+  u32 ks, vs;  // scale bytes of the tile that the lane owns a row of K in, and of its tile of V
   auto load_k = [&]() {
-    const u8 *kp = in_tiles(a.cache.k_codes, k_tile, kFp8TileBytes, (n & 3) * 64 + 16 * gq);
+    const u8 *kp = in_tile(a.cache.k_codes, n >= 8, kFp8TileBytes, (2 * (n & 4) + (n & 3)) * 64 + 16 * gq);
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
+    for (int t = 0; t < 2; ++t) {
       kc[t][0] = load16(kp + 4 * t * 64);
       kc[t][1] = load16(kp + 4 * t * 64 + kFp8TileBytes / 2);
     }
-    ks = *in_tiles(a.cache.k_scales, k_tile, 1, 0);
+    ks = *in_tile(a.cache.k_scales, n >= 8, 1, 0);
   };
   auto load_v = [&]() {
-    const u8 *vp = in_tiles(a.cache.v_codes, v_tile, kFp8TileBytes, n * kFp8Tile);
+    const u8 *vp = in_tile(a.cache.v_codes, gq >= 2, kFp8TileBytes, (64 * (gq & 1) + n) * kFp8Tile);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) vc[e] = load16(vp + 16 * kFp8Tile * e);
-    vs = *in_tiles(a.cache.v_scales, v_tile, 1, 0);
+    for (int j = 0; j < 4; ++j) vc[j] = load16(vp + 16 * kFp8Tile * j);
+    vs = *in_tile(a.cache.v_scales, gq >= 2, 1, 0);
   };
 
   // K of the next step is asked for as soon as the scores have taken this step's, V as soon as the products have: each
   // is in flight during the other half of the step, without registers of its own.
   auto step = [&](const int t0, const int next) {
-    constexpr int NP = GP <= 4 ? 1 : GP <= 8 ? 2 : 4;  // accumulators that hold all scores once packed
-    f32x4 s[4];
+    constexpr int NP = GP <= 8 ? 1 : 2;  // accumulators that hold all scores once packed
+    f32x4 s[2];
     score(s[0], kc[0], ks, q_hi, q_lo, q_scale);
     score(s[1], kc[1], ks, q_hi, q_lo, q_scale);
-    score(s[2], kc[2], ks, q_hi, q_lo, q_scale);
-    score(s[3], kc[3], ks, q_hi, q_lo, q_scale);
     __builtin_amdgcn_sched_barrier(0);
     if (next < t_end) {
       locate(next);
       load_k();
-      look_up(next + 64 * kWaves);
+      look_up(next + kStep * kWaves);
     }
     __builtin_amdgcn_sched_barrier(0);
 
-    // Score x * 4 + i of a lane: token 16 gq + 4 (x + NP * its column group) + i, the group being n / (4 NP).
+    // Score x * 4 + i of a lane: token 8 gq + 4 (x + n / 8) + i where packed, else 8 gq + 4 x + i.
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if constexpr (NP == 1) {
-        s[0][i] = dpp_into<kRowShr4, 0x2>(s[0][i], s[1][i]);
-        s[0][i] = dpp_into<kRowShr8, 0x4>(s[0][i], s[2][i]);
-        s[0][i] = dpp_into<kRowShr12, 0x8>(s[0][i], s[3][i]);
-      } else if constexpr (NP == 2) {
-        s[0][i] = dpp_into<kRowShr8, 0xC>(s[0][i], s[2][i]);
-        s[1][i] = dpp_into<kRowShr8, 0xC>(s[1][i], s[3][i]);
-      }
-    }
-    const int group = NP == 4 ? 0 : n / (4 * NP);
-    const int live = t_end - t0 - 16 * gq;  // this lane's tile's tokens that the partition holds
+    for (int i = 0; i < 4; ++i)
+      if constexpr (NP == 1) s[0][i] = dpp_into<kRowShr8, 0xC>(s[0][i], s[1][i]);
+    const int group = NP == 1 ? n >> 3 : 0;
+    const int live = t_end - t0 - 8 * gq;  // this lane's tokens that the partition holds
     float cm = kNoScore;
 #pragma unroll
     for (int x = 0; x < NP; ++x)
 #pragma unroll
       for (int i = 0; i < 4; ++i) s[x][i] *= a.scale_log2e;
-    if (t0 + 64 > t_end) {
+    if (t0 + kStep > t_end) {
 #pragma unroll
       for (int x = 0; x < NP; ++x)
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          if (4 * (x + NP * group) + i >= live) s[x][i] = -INFINITY;
+          if (4 * (x + group) + i >= live) s[x][i] = -INFINITY;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) keep_tokens(vc[e], live);  // values past the end weigh nothing, NaNs of stale rows too
+      for (int j = 0; j < 4; ++j)  // values past the end weigh nothing, NaNs of stale rows too
+        keep_tokens(vc[j], t_end - t0 - 16 * (gq >> 1));
     }
 #pragma unroll
     for (int x = 0; x < NP; ++x)
 #pragma unroll
       for (int i = 0; i < 4; ++i) cm = fmaxf(cm, s[x][i]);
-    if constexpr (NP == 1) cm = fmaxf(cm, dpp<kRowRor4>(cm));
-    if constexpr (NP <= 2) cm = fmaxf(cm, dpp<kDppRowRor8>(cm));
+    if constexpr (NP == 1) cm = fmaxf(cm, dpp<kDppRowRor8>(cm));
     cm = max_over_quarters(cm);
     // Lazy rescale: the weights stay below 2^8 and the numerators are scaled only where some head's reference moves.
     if (__builtin_amdgcn_ballot_w64(cm > m_thr) != 0) {
@@ -245,42 +225,43 @@ paged_decode_fp8_kernel(DecodeArgs<Fp8Cache> a, std::conditional_t<FUSED, StepAr
     }
     // P rounded to bf16 for the matrix cores; the sum takes the same rounded values.  Back in the order of the products,
     // the columns past the heads hold weights of other tokens and give numerators that are never read.
-    u32x4 pf[2];
+    u32x4 pf;
 #pragma unroll
     for (int x = 0; x < NP; ++x)
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const u32 pr = pack_bf16x2(fast_exp2(s[x][2 * i] - m), fast_exp2(s[x][2 * i + 1] - m));
         l = dot2_bf16(pr, kBf16PairOne, l);
-        pf[x >> 1][2 * (x & 1) + i] = pr;
-        if constexpr (NP == 1) {
-          pf[0][2 + i] = dpp_u32<kRowShl4>(pr);
-          pf[1][i] = dpp_u32<kRowShl8>(pr);
-          pf[1][2 + i] = dpp_u32<kRowShl12>(pr);
-        } else if constexpr (NP == 2) {
-          pf[1][2 * x + i] = dpp_u32<kRowShl8>(pr);
-        }
+        pf[2 * x + i] = pr;
+        if constexpr (NP == 1) pf[2 + i] = dpp_u32<kRowShl8>(pr);
       }
     const float v_scale = fp8_scale(vs);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) add_values(o[e], vc[e], v_scale, pf);
+    for (int j = 0; j < 4; ++j) {
+      // Lanes gq and gq ^ 1 hold 64 dims each of 16 tokens; they swap for all dims of 8 tokens.
+      const auto x = __builtin_amdgcn_permlane16_swap(vc[j][0], vc[j][2], false, false);
+      const auto y = __builtin_amdgcn_permlane16_swap(vc[j][1], vc[j][3], false, false);
+      o[j] = mfma16(expand8(u32x2{(u32)x[0], (u32)y[0]}, v_scale), pf, o[j]);
+      o[4 + j] = mfma16(expand8(u32x2{(u32)x[1], (u32)y[1]}, v_scale), pf, o[4 + j]);
+    }
     __builtin_amdgcn_sched_barrier(0);
     if (next < t_end) load_v();
   };
-  if (int t0 = p * part_tokens + 64 * w; t0 < t_end) {
+  if (int t0 = p * part_tokens + kStep * w; t0 < t_end) {
     look_up(t0);
     locate(t0);
     load_k();
     load_v();
-    look_up(t0 + 64 * kWaves);
+    look_up(t0 + kStep * kWaves);
 #pragma unroll 1
     do {
-      step(t0, t0 + 64 * kWaves);
-      t0 += 64 * kWaves;
+      step(t0, t0 + kStep * kWaves);
+      t0 += kStep * kWaves;
     } while (t0 < t_end);
   }
 
   report(a.err, err_bits, lane);
+  if constexpr (GP <= 8) l += dpp<kDppRowRor8>(l);
   finish<kWaves, GP>(a, part, head0, tid, w, o, m, l, s_o, s_m, s_l, s_last);
 }
 
@@ -290,7 +271,7 @@ int launch(DecodeArgs<Fp8Cache> &a, const Step &s, hipStream_t stream) {
   return launch_groups(a, [&](auto heads) {
     constexpr int GP = decltype(heads)::value;
     const dim3 grid(decode_items(a)), block(kWaves * 64);
-    if (a.bs_log2 >= 6)
+    if (a.bs_log2 >= 5)
       hipLaunchKernelGGL((paged_decode_fp8_kernel<GP, true, FUSED>), grid, block, 0, stream, a, s);
     else
       hipLaunchKernelGGL((paged_decode_fp8_kernel<GP, false, FUSED>), grid, block, 0, stream, a, s);
@@ -317,7 +298,7 @@ extern "C" int nvamd_paged_decode_fp8(void *out, int64_t out_stride, const void 
                                       size_t workspace_bytes, hipStream_t stream) {
   if (batch == 0) return NVAMD_OK;
   DecodeArgs<Fp8Cache> a;
-  const int st = fill_decode_args<kWaves>(a, out, out_stride, q, q_stride, cache_of(k_codes, k_scales, v_codes, v_scales),
+  const int st = fill_decode_args<kLeastPart>(a, out, out_stride, q, q_stride, cache_of(k_codes, k_scales, v_codes, v_scales),
                                     fp8_cache_ok(k_codes, k_scales, v_codes, v_scales), num_blocks, block_size,
                                     block_tables, bt_stride, bt_width, context_lens, batch, num_heads, num_kv_heads,
                                     head_dim, scale, max_context_len, workspace, workspace_bytes);
@@ -337,7 +318,7 @@ extern "C" int nvamd_paged_decode_fused_fp8(void *out, int64_t out_stride, const
                                             hipStream_t stream) {
   if (batch == 0) return NVAMD_OK;
   DecodeArgs<Fp8Cache> a;
-  int st = fill_decode_args<kWaves>(a, out, out_stride, q, q_stride, cache_of(k_codes, k_scales, v_codes, v_scales),
+  int st = fill_decode_args<kLeastPart>(a, out, out_stride, q, q_stride, cache_of(k_codes, k_scales, v_codes, v_scales),
                                     fp8_cache_ok(k_codes, k_scales, v_codes, v_scales), num_blocks, block_size,
                                     block_tables, bt_stride, bt_width, context_lens, batch, num_heads, num_kv_heads,
                                     head_dim, scale, max_context_len, workspace, workspace_bytes);
