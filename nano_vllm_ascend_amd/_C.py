@@ -191,7 +191,7 @@ def load() -> ctypes.CDLL:
     return lib
 
 
-_calls = None  # csrc/calls.cpp: eager calls of the quantised caches, checked and made in one step; None: not usable here
+_calls = None  # csrc/calls.cpp: eager calls of the quantised caches and of copies, checked and made in one step; None: not usable
 
 
 def _bind_calls(lib: ctypes.CDLL) -> None:
@@ -212,6 +212,7 @@ def _bind_calls(lib: ctypes.CDLL) -> None:
     for index, kind in enumerate((_FP4, _FP8)):
         functions = (getattr(lib, "nvamd_" + n.format(kind.name)) for n in names)
         calls.bind(index, kind.pages, *(ctypes.cast(f, ctypes.c_void_p).value for f in functions))
+    calls.bind_copy(ctypes.cast(lib.nvamd_copy_blocks, ctypes.c_void_p).value)
     _calls = calls
 
 
@@ -1112,6 +1113,8 @@ def copy_blocks(pools, sources: torch.Tensor, targets: torch.Tensor) -> None:
     ``pools``: up to 8 contiguous tensors [layers, blocks, ...] of any type, with the same layers and blocks; sources and
     targets: int32 [n] on the device.  No block is a target twice, or a target and another pair's source."""
     lib = _lib or load()
+    if _calls and not _range_checks and _made(_calls.copy(pools, sources, targets), "nvamd_copy_blocks"):
+        return
     pools = list(pools)
     if not 0 < len(pools) <= COPY_MAX_POOLS:
         raise ValueError(f"1 to {COPY_MAX_POOLS} pools, got {len(pools)}")

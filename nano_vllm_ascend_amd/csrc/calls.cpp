@@ -1,7 +1,7 @@
-// The eager calls of the 4-bit and 8-bit caches from Python: arguments checked and read, outputs made and the C ABI called in one
-// step. A small batch's eager call is bound by the host: a launch costs it some 3.6 us, and checking 5 to 15 tensors
-// attribute by attribute from Python another 4 to 5, with 1 for ctypes (decode of 4 x U[1, 512] through the layer: 12.7
-// us, so 8.1; a row written and read back 18.5, 9.0).
+// The eager calls of the 4-bit and 8-bit caches, and of copies of blocks, from Python: arguments checked and read, outputs
+// made and the C ABI called in one step.  A small batch's eager call is bound by the host: a launch costs it some 3.6 us,
+// and checking 5 to 15 tensors attribute by attribute from Python another 4 to 5, with 1 for ctypes (decode of 4 x U[1,
+// 512] through the layer: 12.7 us, so 8.1; a row written and read back 18.5, 9.0; a block copied in 28 layers 9.8, 5.1).
 //
 // Every function answers
 //   its result   the call was made;
@@ -34,7 +34,9 @@ struct Kind {
   decltype(&nvamd_paged_prefill_fp4_workspace_size) prefill_space;
 };
 constexpr int kFp4 = 0, kFp8 = 1;
-Kind kinds[2];  // by the bytes of a head vector: 64, 128
+Kind kinds[2];
+decltype(&nvamd_copy_blocks) f_copy;
+constexpr Py_ssize_t kMaxPools = 8;
 
 struct Irregular {};  // thrown: answer None
 
@@ -311,6 +313,32 @@ PyObject *prefill(PyObject *const *a) {
   return status ? PyLong_FromLong(status) : same(a[0]);
 }
 
+// (pools, sources, targets) -> True; pools a list or a tuple
+PyObject *copy(PyObject *const *a) {
+  need(PyList_CheckExact(a[0]) || PyTuple_CheckExact(a[0]));
+  PyObject *const *pools = PySequence_Fast_ITEMS(a[0]);
+  const Py_ssize_t n_pools = PySequence_Fast_GET_SIZE(a[0]);
+  need(n_pools > 0 && n_pools <= kMaxPools);
+  int dev = -1;
+  void *at[kMaxPools];
+  int64_t bytes[kMaxPools], layers = 0, blocks = 0;
+  for (Py_ssize_t i = 0; i < n_pools; ++i) {
+    const at::Tensor &t = tensor(pools[i], dev);
+    need(t.dim() >= 3 && t.is_contiguous() && t.numel() > 0);
+    if (i == 0) layers = t.size(0), blocks = t.size(1);
+    need(t.size(0) == layers && t.size(1) == blocks);
+    at[i] = t.data_ptr();
+    bytes[i] = t.stride(1) * (int64_t)t.element_size();
+  }
+  const int32_t *sources = lengths(a[1], dev, 0, false);
+  const int64_t n = THPVariable_Unpack(a[1]).size(0);
+  const int32_t *targets = lengths(a[2], dev, n, true);
+  const int l = narrow(layers), nb = narrow(blocks), count = narrow(n);
+  hipStream_t s = stream_on(dev);
+  const int status = call([&] { return f_copy(at, bytes, (int)n_pools, l, nb, sources, targets, count, s); });
+  return status ? PyLong_FromLong(status) : same(Py_True);
+}
+
 template <PyObject *(*F)(PyObject *const *), Py_ssize_t N>
 PyObject *entry(PyObject *, PyObject *const *args, Py_ssize_t n) {
   if (n != N) Py_RETURN_NONE;
@@ -322,6 +350,14 @@ PyObject *entry(PyObject *, PyObject *const *args, Py_ssize_t n) {
     torch::translate_exception_to_python(std::current_exception());
     return nullptr;
   }
+}
+
+// (address of nvamd_copy_blocks)
+PyObject *bind_copy(PyObject *, PyObject *arg) {
+  const unsigned long long p = PyLong_AsUnsignedLongLong(arg);
+  if (PyErr_Occurred()) return nullptr;
+  f_copy = reinterpret_cast<decltype(f_copy)>(p);
+  Py_RETURN_NONE;
 }
 
 // (index, type of the pages, addresses of its entry points)
@@ -353,8 +389,9 @@ PyObject *bind(PyObject *, PyObject *args) {
   { #name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&entry<name, args>)), METH_FASTCALL, nullptr }
 PyMethodDef methods[] = {
     {"bind", bind, METH_VARARGS, nullptr},
+    {"bind_copy", bind_copy, METH_O, nullptr},
     ENTRY(write, 5), ENTRY(read, 3), ENTRY(rope, 13), ENTRY(decode, 9), ENTRY(decode_fused, 17),
-    ENTRY(prefill, 9),
+    ENTRY(prefill, 9), ENTRY(copy, 3),
     {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_calls", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

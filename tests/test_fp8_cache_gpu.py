@@ -459,3 +459,24 @@ def test_copy_blocks_replays_from_a_graph_and_follows_the_stream(device):
             graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(p, w) for p, w in zip(pools, want))
+
+
+def test_copies_are_made_at_once_only_if_they_are_plain(device, monkeypatch):
+    """csrc/calls.cpp leaves what _C.py refuses to it; without it the same copies are made from Python."""
+    pools = [torch.empty(2, 6, 40, dtype=torch.uint8, device=device), torch.empty(2, 6, 3, 2, device=device)]
+    ids = torch.arange(3, dtype=torch.int32, device=device)
+    for bad in (([], ids, ids), (pools * 5, ids, ids), ([pools[0].cpu()], ids, ids), ([pools[0][:, :5]], ids, ids),
+                ([pools[0], pools[1][:1]], ids, ids), ([pools[0][0]], ids, ids), (pools, ids.long(), ids),
+                (pools, ids, ids[:2]), (pools, ids.cpu(), ids), (pools, ids, ids.repeat_interleave(2)[::2])):
+        assert _C._calls.copy(*bad) is None
+        with pytest.raises(ValueError):
+            _C.copy_blocks(*bad)
+    results = []
+    for at_once in (True, False):
+        if not at_once:
+            monkeypatch.setattr(_C, "_calls", None)
+        for i, p in enumerate(pools):
+            random_bytes(p, i)
+        _C.copy_blocks(iter(pools) if not at_once else tuple(pools), ids, ids + 3)
+        results.append([p.clone() for p in pools])
+    assert all(torch.equal(a, b) for a, b in zip(*results)) and torch.equal(results[0][0][:, :3], results[0][0][:, 3:])
