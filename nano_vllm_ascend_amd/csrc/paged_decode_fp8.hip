@@ -3,19 +3,25 @@
 // For a query token of each sequence and its heads h of kv head g: out = softmax(q . K^T * scale) V over the cached
 // context.
 //
-// Work: partitions of a (sequence, kv head), a workgroup of kWaves waves each (decode_quantised.h).  A wave takes 64
-// tokens at a time, four 16-token tiles, one per 16 lanes (gq = lane / 16):
+// Work: partitions of a (sequence, kv head), a workgroup of kWaves waves each (decode_quantised.h).  A wave takes 32
+// tokens at a time, two 16-token tiles (n = lane % 16, gq = lane / 16):
 //   S^T = K . Q^T  v_mfma_scale_f32_16x16x128_f8f6f4 on the codes as they lie in the cache, A = 16 rows of K under their
 //        tiles' scales, B = the heads as 16 columns, in e4m3 twice: a bf16 query is the sum of two e4m3 numbers under a
-//        scale for each block (QueryScale), so two products give the scores.  Row 4a + i of product t is token 4t + i
-//        of tile a: lane (h, gq) then finds the scores of tile gq's tokens 4t .. 4t+3 of head h in its accumulator of
-//        product t, that is of all 16 tokens in the four products;
-//   softmax  on up to 4 (8) heads the accumulators' 16 columns are mostly repeats: products 1..3 (2, 3) move into the
-//        idle columns by DPP, and one lane does 4 (8) scores instead of 16;
+//        scale for each block (QueryScale), so two products give the scores.  Row 4a + i of product t is token
+//        8a + 4t + i of the step: lane (h, gq) then finds the scores of tokens 8 gq + 4t + i of head h in its accumulator
+//        of product t;
+//   softmax  on up to 8 heads the accumulators' 16 columns are repeats: product 1 moves into the idle columns by DPP, and
+//        one lane does 4 scores instead of 8;
 //   O^T += V^T . P^T  v_mfma_f32_16x16x32_bf16, A = 16 dims of V^T expanded by v_cvt_scalef32_pk_bf16_fp8 (two tokens of
-//        a dim and the tile's scale in one instruction, exact), B = P^T, whose 8 k-slots per lane are tokens 0..7
-//        (8..15) of tile gq: just what the lane holds.  The cache keeps the 16 tokens of a dim in consecutive bytes, so
-//        the lane's 16 bytes give both products' operands of a dim: no lane movement.
+//        a dim and the tile's scale in one instruction, exact), B = P^T, whose 8 k-slots per lane are tokens 8 gq .. + 7:
+//        just what the lane holds.  The cache keeps the 16 tokens of a dim in consecutive bytes: lanes gq and gq ^ 1 load
+//        16 bytes each of different dims of the same tile and swap halves, so that every load is whole.
+//
+// Bound by memory on long contexts, by latency on short ones: a token of a head is 256 bytes and 2 scales.  Measured
+// (8 kv heads, 16 query heads unless said): 4 contexts of up to 512 tokens 5.5 us; 32 of 256..2304 20.3 us (4.3 TB/s);
+// 100 of 2048..4096 105 us (5.9 TB/s); 4 of 8192..40960, 64 query heads, 35 us (4.9 TB/s); 16 of 512..4096, 64 query
+// heads, 16.3 us.  Steps of 64 tokens, a tile to 16 lanes, need registers for two waves a SIMD; four waves with half the
+// step hide more of the loads' latency: those 32 contexts took 23.7 us, the 100 as long, the 4 longest 2% less.
 // The score of a token past the context is replaced by -inf and its values by zero, whatever bytes it holds.
 #include "decode_quantised.h"
 #include "fp8_attention.h"
@@ -25,8 +31,8 @@ namespace nvamd {
 namespace {
 
 constexpr int kWaves = 8;
-constexpr int kStep = 32;                   // tokens of a wave
-constexpr int kLeastPart = 64 * kWaves;     // of the smallest partition: two steps of each wave
+constexpr int kStep = 32;                // tokens of a wave
+constexpr int kLeastPart = 64 * kWaves;  // of the smallest partition: two steps of each wave
 
 // The new token's k (normed and rotated) into its slot, by a wave: every 8 lanes make the row, those of the token keep it.
 __device__ __forceinline__ void store_key_row(const Fp8Cache &cache, const StepArgs &s, int b, int g, int64_t slot,
@@ -70,8 +76,45 @@ __device__ __forceinline__ void store_value_row(const Fp8Cache &cache, const Ste
   store_values(cache, tile, o, 1, held, old, lane, x);
 }
 
-// GP: heads that the registers and LDS are laid out for.  WIDE: pages of 64 tokens or more, so that the 64 tokens of a
-// wave's step lie in one page, whose id is a scalar.  FUSED: the norm, the rotation and the store of the step's rows
+// The query's operand, for every wave of the workgroup: each of the first four makes a quarter, and they meet in LDS.
+// (Made whole by every wave, a call takes 0.3 us more: 5.8 us, so 5.5, for 4 contexts of 384..512 tokens.)
+struct SharedQuery {
+  u32x2 words[2][4][64];  // [hi, lo][8 dims of a lane][lane]
+  u32 scale[2][64];       // of the blocks of a lane's dims 16 gq .. and 64 + 16 gq ..
+};
+__device__ __forceinline__ void shared_query(const DecodeArgs<Fp8Cache> &a, int b, int head0, int w, int lane, SharedQuery &s, i32x8 &q_hi,
+                                             i32x8 &q_lo, u32 &q_scale) {
+  const int n = lane & 15, gq = lane >> 4;
+  if (w < 4) {
+    const u16 *qp = a.q + (int64_t)b * a.q_stride + (int64_t)(head0 + min(n, a.q_sub - 1)) * kHeadDim + 16 * gq +
+                    64 * (w >> 1);
+    const u32x4 x[2] = {ld16(qp), ld16(qp + 8)};
+    const u32 top = max(largest(x[0]), largest(x[1]));
+    const auto r = __builtin_amdgcn_permlane16_swap(top, top, false, false);  // lanes gq and gq ^ 1 hold a block
+    const QueryScale scale = query_scale(max((u32)r[0], (u32)r[1]));
+    const u32x4 mine = w & 1 ? x[1] : x[0];
+    int hi[2], lo[2];
+    split4(mine[0], mine[1], scale.up, hi[0], lo[0]);
+    split4(mine[2], mine[3], scale.up, hi[1], lo[1]);
+    s.words[0][w][lane] = u32x2{(u32)hi[0], (u32)hi[1]};
+    s.words[1][w][lane] = u32x2{(u32)lo[0], (u32)lo[1]};
+    if ((w & 1) == 0) s.scale[w >> 1][lane] = scale.byte;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const u32x2 h = s.words[0][j][lane], l = s.words[1][j][lane];
+    q_hi[2 * j] = (int)h[0];
+    q_hi[2 * j + 1] = (int)h[1];
+    q_lo[2 * j] = (int)l[0];
+    q_lo[2 * j + 1] = (int)l[1];
+  }
+  q_scale = s.scale[gq >> 1][(gq & 1) * 32 + n];  // block gq's: of the lanes that hold it
+}
+
+// GP: heads that the registers and LDS are laid out for.  WIDE: pages of 32 tokens or more, so that the 32 tokens of a
+// wave's step lie in one page, and one entry of the table finds both tiles (on pages of 16: 22.2 us against 21.6 for 32
+// contexts of 1000..2000).  FUSED: the norm, the rotation and the store of the step's rows
 // first: every workgroup makes its own queries; the one whose partition ends the context stores the new row (one wave the
 // key, another the value) and waits for it, so that its loads find it.  Bits as of nvamd_qk_norm_rope_fp8 and this kernel
 // after it.
@@ -113,9 +156,8 @@ paged_decode_fp8_kernel(DecodeArgs<Fp8Cache> a, std::conditional_t<FUSED, StepAr
                  __builtin_amdgcn_s_waitcnt(0);  // before this workgroup's loads of the row
                });
   } else {
-    u32x4 x[4];
-    load_query(a, b, head0, n, gq, x);
-    q_scale = query_operand(x, gq, q_hi, q_lo);
+    __shared__ __attribute__((aligned(16))) SharedQuery s_q;
+    shared_query(a, b, head0, w, lane, s_q, q_hi, q_lo, q_scale);
   }
 
   // The exponent's reference, the threshold above which it moves; the sum and the numerators at that reference.

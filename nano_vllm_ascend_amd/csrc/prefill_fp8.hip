@@ -20,6 +20,13 @@
 //   paged_decode_fp8.hip with rows in the place of heads and a last key for each row.  On long contexts the keys are cut as
 //   well.
 //
+// Bounds and figures (16 query heads on 8 kv heads unless said).  Tiles: bound by the issue of instructions, since a wave's
+// matrix products and its softmax (a tile of 32 keys: 12 products, some 90 vector instructions, 16 of them exponentials)
+// do not overlap, only those of different waves do: 3 waves a SIMD, 700 us for 32 prompts of 512..2,048 tokens on
+// 1,152 cached (881 TFLOP/s), 842 at two.  40 query heads, 2 x U[3000, 4000] on 4,096 cached: 1,003 us (991 TFLOP/s).
+// Strips: 1 x 4,000 on 4,096 222 us, 8 x 1..64 on 1,040 12.6 us.  Strips and few rows wait for loads; the registers of
+// their 8-bit operands leave room for two waves a SIMD, and they take as long as the 4-bit cache's kernels at three.
+//
 // Weights are rounded to bf16 once for the matrix cores, and the sums take the rounded values, as in the other caches'
 // prefill.
 //
