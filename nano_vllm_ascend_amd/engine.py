@@ -89,10 +89,13 @@ class LLM:
         seq = Sequence(seq_id=self.scheduler.next_seq_id(), prompt=prompt if isinstance(prompt, str) else "",
                        max_new_tokens=max_new_tokens, prompt_token_ids=self.runner.tokenize_prompts([prompt])[0],
                        sampling_params=params)
-        self.runner.prepare_sequences([seq])  # prefix lookup happens here, at submit time
-        seq.reserved_blocks = self.scheduler.compute_required_blocks(runtime_prompt_len=seq.runtime_prompt_len,
-                                                                     max_new_tokens=max_new_tokens)
+        self._plan_prompt(seq)  # prefix lookup happens here, at submit time
         return self.scheduler.add_request(seq)
+
+    def _plan_prompt(self, seq: Sequence) -> None:
+        self.runner.prepare_sequences([seq])
+        seq.reserved_blocks = self.scheduler.compute_required_blocks(runtime_prompt_len=seq.runtime_prompt_len,
+                                                                     max_new_tokens=seq.max_new_tokens)
 
     def submit(self, prompt, max_new_tokens: int = 128, sampling_params: SamplingParams | None = None, *,
                temperature: float | None = None, top_k: int | None = None, top_p: float | None = None) -> int:
@@ -121,7 +124,10 @@ class LLM:
         params = _params(sampling_params or seq.sampling_params, temperature, top_k, top_p)
         child = seq.fork(self.scheduler.next_seq_id(), budget, params)
         child.reserved_blocks = blocks
-        self.runner.fork(seq, child)
+        taken = self.runner.fork(seq, child) or ()
+        for waiting in self.scheduler.waiting:  # whose cached prefix lay in the block that the copy took
+            if not set(waiting.cached_block_ids).isdisjoint(taken):
+                self._plan_prompt(waiting)
         return self.scheduler.add_running(child).seq_id
 
     def _output(self, seq: Sequence) -> dict[str, object]:

@@ -4,6 +4,7 @@ from __future__ import annotations
 import sys
 from dataclasses import replace
 from pathlib import Path
+from types import SimpleNamespace
 
 import pytest
 import torch
@@ -14,6 +15,7 @@ from test_continuous_batching import ScriptedRunner, engine  # noqa: E402
 
 from nano_vllm_ascend_amd import LLM, SamplingParams  # noqa: E402
 from nano_vllm_ascend_amd.config import QWEN3_0_6B  # noqa: E402
+from nano_vllm_ascend_amd.model_runner import ModelRunner  # noqa: E402
 
 
 def manager(num_blocks=8, block_size=4):
@@ -126,6 +128,51 @@ def test_forks_that_are_refused():
     run(llm)
     with pytest.raises(ValueError, match="not running"):
         llm.fork(a)
+
+
+class PoolRunner(ScriptedRunner):
+    """Whose prompts and forks take blocks of a real pool of 8, in which requests find their prefixes."""
+
+    def __init__(self):
+        super().__init__()
+        self.block_size, self.enable_prefix_cache = 4, True
+        self.block_manager = manager(num_blocks=8)
+        self.copied = []
+        self.kv_cache = SimpleNamespace(copy_blocks=lambda sources, targets: self.copied.append((sources, targets)))
+
+    prepare_sequences = ModelRunner.prepare_sequences
+    fork = ModelRunner.fork
+
+    def _drop_in_flight(self):
+        pass
+
+    def prefill(self, seqs):
+        super().prefill(seqs)
+        for seq in seqs:
+            prefill(self.block_manager, seq.seq_id, seq.estimated_prompt_len)
+
+
+def test_a_fork_that_takes_a_cached_block_leaves_no_request_waiting_for_it():
+    llm = engine(max_num_seqs=2)
+    llm.runner = PoolRunner()
+    llm.engine_core.runner = llm.runner
+    m = llm.runner.block_manager
+    prefill(m, "before", 4)  # its block, 0, stays cached behind the other free ones
+    m.cache_full_blocks("before", torch.arange(1, 5))
+    a = llm.submit("a" * 10, max_new_tokens=3)
+    llm.scheduler.waiting[0].cached_block_ids, llm.scheduler.waiting[0].cached_prefix_len = [], 0
+    llm.step()
+    m.free_slot("before")
+    prefill(m, "other", 16)
+    assert m.free_block_ids == [0]
+    b = llm.submit("b" * 11, max_new_tokens=3)
+    (waiting,) = llm.scheduler.waiting
+    assert waiting.seq_id == b and waiting.cached_block_ids == [0] and waiting.runtime_prompt_len == 7
+    reserved = waiting.reserved_blocks
+    llm.fork(a)
+    assert llm.runner.copied == [((3,), (0,))]
+    assert waiting.cached_block_ids == [] and waiting.cached_prefix_len == 0 and waiting.runtime_prompt_len == 11
+    assert waiting.runtime_prompt_token_ids.tolist() == list(range(1, 12)) and waiting.reserved_blocks == reserved + 1
 
 
 # -------------------------------------------------------------------------------------------- on the GPU
