@@ -21,9 +21,12 @@
 //   well.
 //
 // Bounds and figures (16 query heads on 8 kv heads unless said).  Tiles: bound by the issue of instructions, since a wave's
-// matrix products and its softmax (a tile of 32 keys: 12 products, some 90 vector instructions, 16 of them exponentials)
-// do not overlap, only those of different waves do: 3 waves a SIMD, 700 us for 32 prompts of 512..2,048 tokens on
-// 1,152 cached (881 TFLOP/s), 842 at two.  40 query heads, 2 x U[3000, 4000] on 4,096 cached: 1,003 us (991 TFLOP/s).
+// matrix products and its softmax (a tile of 32 keys: 12 products, some 75 vector instructions, 16 of them exponentials)
+// do not overlap, only those of different waves do: 32 prompts of 512..2,048 tokens on 1,152 cached take 655 us (941
+// TFLOP/s) at 3 waves a SIMD, 842 at two; 40 query heads, 2 x U[3000, 4000] on 4,096 cached 940 us (1,057 TFLOP/s).  Of the
+// first, 12 us are the maximum that is only looked for where it matters (weigh_scores), 25 V's operands, which are on
+// their way from LDS before they are needed, and 10 the fewer registers and instructions of the pages' bookkeeping.  One
+// barrier for two tiles, with four stages: 654.
 // Strips: 1 x 4,000 on 4,096 222 us, 8 x 1..64 on 1,040 12.6 us.  Strips and few rows wait for loads; the registers of
 // their 8-bit operands leave room for two waves a SIMD, and they take as long as the 4-bit cache's kernels at three.
 //
@@ -54,14 +57,59 @@ __device__ __forceinline__ u32 take_nans(u32x4 &codes) {
   return tokens;
 }
 
+// Weights of a row's 16 keys as bf16 pairs, in the order of the scores; their sum joins l_run.  The exponent's reference is
+// 2^kHeadroom above a maximum of the row, so that a weight of 2 or more, that is a set top bit of its exponent, says that a
+// score exceeds that maximum by 2^8: the maximum is looked for only then, and the reference, the numerators and the sum
+// follow it.  (An infinity or a NaN is one of these; so is the first score that a row sees.)
+constexpr float kHeadroom = kRescaleLog2 - 1.f;
+__device__ __forceinline__ void weigh_scores(const f32x16 &sc, float scale, f32x16 (&acc)[4], float &neg_ref, float &l_run,
+                                             u32x4 (&pf)[2]) {
+  auto weights = [&]() {
+#pragma unroll
+    for (int hh = 0; hh < 2; ++hh)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        pf[hh][e] = pack_bf16x2(fast_exp2(fmaf(sc[8 * hh + 2 * e], scale, neg_ref)),
+                                fast_exp2(fmaf(sc[8 * hh + 2 * e + 1], scale, neg_ref)));
+  };
+  weights();
+  u32 seen = 0;
+#pragma unroll
+  for (int hh = 0; hh < 2; ++hh)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) seen |= pf[hh][e];
+  seen &= 0x40004000u;
+  if (__builtin_expect(__builtin_amdgcn_ballot_w64(seen != 0) != 0, 0)) {
+    const auto both = __builtin_amdgcn_permlane32_swap(seen, seen, false, false);  // lanes l and l ^ 32 hold a row
+    const bool up = ((u32)both[0] | (u32)both[1]) != 0;                            // whatever the other rows do
+    float tmax = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) tmax = fmaxf(tmax, sc[i]);
+    tmax = max_xor32(tmax) * scale;
+    const float alpha = up ? fast_exp2(-neg_ref - tmax - kHeadroom) : 1.f;
+    if (up) neg_ref = -tmax - kHeadroom;
+    l_run *= alpha;
+#pragma unroll
+    for (int db = 0; db < 4; ++db)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) acc[db][i] *= alpha;
+    weights();
+  }
+#pragma unroll
+  for (int hh = 0; hh < 2; ++hh)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) l_run = dot2_bf16(pf[hh][e], kBf16PairOne, l_run);  // both rounded values of the pair
+}
+
 // ------------------------------------------------------------------------------------------ tiles
 
 // 64 dims: lane (n, half) gives dims 16 half .. +15 and 32 + 16 half .. +15 of row and column n, the scale byte of its row
 // and that of block `half` of its column.
+template <int BYTE = 0>  // of q_scale
 __device__ __forceinline__ f32x16 mfma32_fp8_fp8(const u32x4 (&k)[2], u32 k_scale, i32x8 q, u32 q_scale, f32x16 c) {
   const i32x8 codes = {(int)k[0][0], (int)k[0][1], (int)k[0][2], (int)k[0][3],
                        (int)k[1][0], (int)k[1][1], (int)k[1][2], (int)k[1][3]};
-  return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(codes, q, c, 0, 0, 0, (int)k_scale, 0, (int)q_scale);
+  return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(codes, q, c, 0, 0, 0, (int)k_scale, BYTE, (int)q_scale);
 }
 
 struct Stage {
@@ -82,10 +130,11 @@ prefill_fp8_kernel(PrefillArgs<Fp8Cache> a) {
   const int half = lane >> 5, n = lane & 31;
   const int kv_len = rows.kv_len;
   const int r0 = rows.first + 32 * w;  // the wave's first row
-  int row = min(r0 + n, rows.rows - 1);
+  const int row = min(r0 + n, rows.rows - 1);
   auto last_seen = [&]() {  // by this lane's row; made anew where it is needed: it would hold a register through the loop
-    int r = row;
-    asm volatile("" : "+v"(r));
+    u32 lanes = ~0u;
+    asm volatile("" : "+s"(lanes));
+    const int r = min(r0 + (int)(__builtin_amdgcn_mbcnt_hi(lanes, __builtin_amdgcn_mbcnt_lo(lanes, 0)) & 31), rows.rows - 1);
     return min(rows.offset + r / a.group, kv_len - 1);
   };
   const int wave_first = rows.offset + r0 / a.group;           // the last key that the wave's first row sees
@@ -97,6 +146,7 @@ prefill_fp8_kernel(PrefillArgs<Fp8Cache> a) {
   i32x8 q_hi[2], q_lo[2];
   u32 q_scale[2];
   load_query(a, rows, row, g, half, q_hi, q_lo, q_scale);
+  const u32 q_scales = q_scale[0] | q_scale[1] << 8;
 
   f32x16 acc[4];
 #pragma unroll
@@ -114,10 +164,13 @@ prefill_fp8_kernel(PrefillArgs<Fp8Cache> a) {
     for (int x = 0; x < 2; ++x) entry[x] = bt[min(t * kBK + 16 * x, last_tile) >> a.bs_log2];
   };
   int tile[2];  // of the latest tile that was located
+  bool outside = false;  // some page; reported at the end
   auto locate = [&](int t) {
 #pragma unroll
-    for (int x = 0; x < 2; ++x)
-      tile[x] = tile_of(a, entry[x], min(t * kBK + 16 * x, last_tile), g, threadIdx.x == 0);
+    for (int x = 0; x < 2; ++x) {
+      outside |= (unsigned)entry[x] >= (unsigned)a.num_blocks;
+      tile[x] = tile_of(a, entry[x], min(t * kBK + 16 * x, last_tile), g, false);
+    }
   };
   // K: key 16a + 8b + 4c + x of the tile in row n = 16a + 8c + 4b + x.
   const int k_token = (n & 3) | ((n & 8) >> 1) | ((n & 4) << 1);  // of its 16-token tile, n / 16
@@ -142,6 +195,8 @@ prefill_fp8_kernel(PrefillArgs<Fp8Cache> a) {
   };
   const int sees_all = rows.offset + rows.first / a.group;  // keys up to here every row of the workgroup sees
   auto on_diagonal = [&](int t) { return t * kBK + kBK - 1 > sees_all; };
+  int v_at = ((half * 4 + w) * 64 + n) * (int)sizeof(u32x4);  // of the lane's operands in a stage
+  asm volatile("" : "+v"(v_at));
   auto expand = [&](int t, Stage &st) {
     if (__builtin_expect(t * kBK + kBK > kv_len, 0)) keep_tokens(vc, kv_len - t * kBK - 16 * half);  // stale rows
     if (__builtin_expect(on_diagonal(t), 0)) {
@@ -151,21 +206,20 @@ prefill_fp8_kernel(PrefillArgs<Fp8Cache> a) {
       if (lane == 0) st.any[w] = some;
     }
     const float scale = fp8_scale(vs);
-    st.v[half][w][n] = expand8<0>(vc, scale);
-    st.v[half][w][32 + n] = expand8<2>(vc, scale);
+    u32x4 *at = reinterpret_cast<u32x4 *>(reinterpret_cast<u8 *>(&st.v) + v_at);
+    at[0] = expand8<0>(vc, scale);
+    at[32] = expand8<2>(vc, scale);
   };
 
-  f32x16 sc;
-  auto score = [&]() {
+  auto score = [&](f32x16 &sc) {
 #pragma unroll
     for (int i = 0; i < 16; ++i) sc[i] = 0.f;
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      sc = mfma32_fp8_fp8(kc[s], ks, q_hi[s], q_scale[s], sc);
-      sc = mfma32_fp8_fp8(kc[s], ks, q_lo[s], q_scale[s], sc);
-    }
+    sc = mfma32_fp8_fp8<0>(kc[0], ks, q_hi[0], q_scales, sc);
+    sc = mfma32_fp8_fp8<0>(kc[0], ks, q_lo[0], q_scales, sc);
+    sc = mfma32_fp8_fp8<1>(kc[1], ks, q_hi[1], q_scales, sc);
+    sc = mfma32_fp8_fp8<1>(kc[1], ks, q_lo[1], q_scales, sc);
   };
-  auto weigh = [&](int t, const Stage &st) {
+  auto weigh = [&](int t, const Stage &st, f32x16 &sc) {
     const int base = t * kBK;
     // Key of register i: base + 16 (i / 8) + 8 half + i % 8.
     if (__builtin_expect(base + kBK - 1 > wave_first || base + kBK > kv_len, 0)) {
@@ -174,35 +228,24 @@ prefill_fp8_kernel(PrefillArgs<Fp8Cache> a) {
       for (int i = 0; i < 16; ++i)
         if (16 * (i / 8) + (i % 8) > lim) sc[i] = -INFINITY;
     }
-    float tmax = -INFINITY;
+    // V's operands are on their way from LDS two ahead of their products.
+    u32x4 v[2];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) tmax = fmaxf(tmax, sc[i]);
-    tmax = max_xor32(tmax) * a.scale_log2e;
-    // Lazy rescale: the weights stay below 2^8, and O and l are scaled only where some row's reference moves.
-    const bool up = tmax + neg_ref > kRescaleLog2;
-    if (__builtin_amdgcn_ballot_w64(up) != 0) {
-      const float alpha = up ? fast_exp2(-neg_ref - tmax) : 1.f;
-      if (up) neg_ref = -tmax;
-      l_run *= alpha;
-#pragma unroll
-      for (int db = 0; db < 4; ++db)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) acc[db][i] *= alpha;
-    }
+    for (int i = 0; i < 2; ++i) v[i] = st.v[0][i][lane];
+    __builtin_amdgcn_sched_barrier(0);
     u32x4 pf[2];
+    weigh_scores(sc, a.scale_log2e, acc, neg_ref, l_run, pf);
 #pragma unroll
-    for (int hh = 0; hh < 2; ++hh)
+    for (int i = 0; i < 8; ++i) {
+      acc[i % 4] = mfma32(v[i % 2], pf[i / 4], acc[i % 4]);
+      if (i + 2 < 8) v[i % 2] = st.v[(i + 2) / 4][(i + 2) % 4][lane];
+    }
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const u32 pr = pack_bf16x2(fast_exp2(fmaf(sc[8 * hh + 2 * e], a.scale_log2e, neg_ref)),
-                                   fast_exp2(fmaf(sc[8 * hh + 2 * e + 1], a.scale_log2e, neg_ref)));
-        l_run = dot2_bf16(pr, kBf16PairOne, l_run);  // both rounded values of the pair
-        pf[hh][e] = pr;
-      }
-#pragma unroll
-    for (int hh = 0; hh < 2; ++hh)
-#pragma unroll
-      for (int db = 0; db < 4; ++db) acc[db] = mfma32(st.v[hh][db][lane], pf[hh], acc[db]);
+    for (int i = 0; i < 6; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // a product
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
     if (__builtin_expect(on_diagonal(t), 0)) {
       const int seen = last_seen() - base;  // the last key of the tile that this lane's row sees
       const u32 mask = seen < 0 ? 0u : seen >= 31 ? 0xffffffffu : (2u << seen) - 1u;
@@ -244,14 +287,16 @@ prefill_fp8_kernel(PrefillArgs<Fp8Cache> a) {
         look_up(t + 3);
       }
       __builtin_amdgcn_sched_barrier(0);
-      if (visible) score();
+      f32x16 sc;  // of this tile alone: its registers are free while V is added
+      if (visible) score(sc);
       __builtin_amdgcn_sched_barrier(0);
       if (t + 1 < n_tiles) load_k(next.x, next.y);
-      if (visible) weigh(t, stages[t & 1]);
+      if (visible) weigh(t, stages[t & 1], sc);
       __syncthreads();
     }
   }
 
+  if (outside && threadIdx.x == 0) flag_index_error(a.err, NVAMD_ERR_BLOCK);
   write_tile_rows(a, rows, g, r0, row, w, lane, acc, l_run, s_mem);
 }
 
@@ -343,30 +388,8 @@ prefill_strip_fp8_kernel(PrefillArgs<Fp8Cache> a) {
       for (int i = 0; i < 16; ++i)
         if (i > lim) sc[i] = -INFINITY;
     }
-    float tmax = -INFINITY;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) tmax = fmaxf(tmax, sc[i]);
-    tmax = max_xor32(tmax) * a.scale_log2e;
-    const bool up = tmax + neg_ref > kRescaleLog2;
-    if (__builtin_amdgcn_ballot_w64(up) != 0) {
-      const float alpha = up ? fast_exp2(-neg_ref - tmax) : 1.f;
-      if (up) neg_ref = -tmax;
-      l_run *= alpha;
-#pragma unroll
-      for (int db = 0; db < 4; ++db)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) acc[db][i] *= alpha;
-    }
     u32x4 pf[2];
-#pragma unroll
-    for (int hh = 0; hh < 2; ++hh)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const u32 pr = pack_bf16x2(fast_exp2(fmaf(sc[8 * hh + 2 * e], a.scale_log2e, neg_ref)),
-                                   fast_exp2(fmaf(sc[8 * hh + 2 * e + 1], a.scale_log2e, neg_ref)));
-        l_run = dot2_bf16(pr, kBf16PairOne, l_run);
-        pf[hh][e] = pr;
-      }
+    weigh_scores(sc, a.scale_log2e, acc, neg_ref, l_run, pf);
     if (t0 + 31 > first_seen || t0 + 32 > rows.kv_len) {
 #pragma unroll
       for (int db = 0; db < 4; ++db) {

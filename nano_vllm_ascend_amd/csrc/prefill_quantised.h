@@ -85,12 +85,12 @@ __device__ __forceinline__ float *record(const Args &a, int per_group, int g, in
   return a.partials + (unit * (a.max_tiles * per_group) + row) * kRec;
 }
 
-// Index of the 16-token tile of the pool that holds a token whose page is `entry`.
+// Index of the 16-token tile of the pool that holds a token whose page is `entry`.  (A pool has less than 2^31.)
 template <typename Args>
 __device__ __forceinline__ int tile_of(const Args &a, int entry, int token, int g, bool report) {
   if ((unsigned)entry >= (unsigned)a.num_blocks && report) flag_index_error(a.err, NVAMD_ERR_BLOCK);
   entry = min(max(entry, 0), a.num_blocks - 1);  // never leave the pool
-  return (int)(((((int64_t)entry * a.num_kv_heads + g) << a.bs_log2) + (token & ((1 << a.bs_log2) - 1))) >> 4);
+  return (int)((((u32)entry * (u32)a.num_kv_heads + (u32)g) << (a.bs_log2 - 4)) + ((u32)(token & ((1 << a.bs_log2) - 1)) >> 4));
 }
 
 __device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
