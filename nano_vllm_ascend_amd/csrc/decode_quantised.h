@@ -103,9 +103,9 @@ __device__ __forceinline__ void norm_rope_row(u32x4 (&x)[4], const u16 *weight, 
 //     Anything between one and two workgroups per CU has half of the CUs do double the work;
 //   many units: twice the mean context.  Units then go round by themselves, and only contexts far longer than the
 //     others are cut.
-// Measured (us, 4-bit cache): 4 x U[8192, 40960] at 8 kv heads 20.9 with one workgroup per CU, 22.8 with two, 25.8 where the length
-// was the next power of two; 16 x U[512, 4096] at 8 groups of 8 heads 13.9 either way (16.4); 32 x U[256, 2304] at 8 kv
-// heads 21.7 uncut, 16.0 with two (16.7); 100 x U[2048, 4096] 63 uncut, 76 cut in two.
+// Measured (us, 4-bit cache): 4 x U[8192, 40960] at 8 kv heads 20.9 with one workgroup per CU, 22.8 with two, 25.8 where
+// the length was the next power of two; 16 x U[512, 4096] at 8 groups of 8 heads 13.9 either way (16.4); 32 x U[256, 2304]
+// at 8 kv heads 21.7 uncut, 16.0 with two (16.7); 100 x U[2048, 4096] 63 uncut, 76 cut in two.
 __host__ __device__ constexpr int partition_share(int units) {
   const int slots = units * 2 <= kCus ? kCus : 2 * kCus;
   return slots - units / 2 > units / 2 ? slots - units / 2 : units / 2;

@@ -46,9 +46,9 @@ __device__ __forceinline__ double norm_factor(double squares, double eps) {
 }
 
 // y = x * rsqrt(mean(x^2) + eps) * w, then the rotation out[d] = y[d] cos[d] - y[d+64] sin[d], out[d+64] = y[d+64]
-// cos[d] + y[d] sin[d], in 64 bits with one rounding to bf16 at the end.  A code's step is a
-// third to a half of the value in 4 bits (an eighth in 8), so a key that 32-bit arithmetic puts on the other side of a
-// rounding border is that far off; in 64 bits the code is that of the exact value.  x w is exact in 64 bits (in 32 its bits would fit, its exponent not
+// cos[d] + y[d] sin[d], in 64 bits with one rounding to bf16 at the end.  A code's step is a third to a half of the value
+// in 4 bits (an eighth in 8), so a key that 32-bit arithmetic puts on the other side of a rounding border is that far off;
+// in 64 bits the code is that of the exact value.  x w is exact in 64 bits (in 32 its bits would fit, its exponent not
 // always), and the reciprocal root comes last: one multiplication for each result.
 __device__ __forceinline__ void norm_rope_f64(u32x4 &lo, u32x4 &hi, const u32x4 w_lo, const u32x4 w_hi,
                                               const float (&cs)[8], const float (&sn)[8], double rstd) {

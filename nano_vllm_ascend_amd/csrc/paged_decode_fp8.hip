@@ -82,8 +82,8 @@ struct SharedQuery {
   u32x2 words[2][4][64];  // [hi, lo][8 dims of a lane][lane]
   u32 scale[2][64];       // of the blocks of a lane's dims 16 gq .. and 64 + 16 gq ..
 };
-__device__ __forceinline__ void shared_query(const DecodeArgs<Fp8Cache> &a, int b, int head0, int w, int lane, SharedQuery &s, i32x8 &q_hi,
-                                             i32x8 &q_lo, u32 &q_scale) {
+__device__ __forceinline__ void shared_query(const DecodeArgs<Fp8Cache> &a, int b, int head0, int w, int lane,
+                                             SharedQuery &s, i32x8 &q_hi, i32x8 &q_lo, u32 &q_scale) {
   const int n = lane & 15, gq = lane >> 4;
   if (w < 4) {
     const u16 *qp = a.q + (int64_t)b * a.q_stride + (int64_t)(head0 + min(n, a.q_sub - 1)) * kHeadDim + 16 * gq +

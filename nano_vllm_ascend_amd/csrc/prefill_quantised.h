@@ -332,12 +332,14 @@ prefill_join_kernel(Args a, int per_group) {
 }
 
 // Which kernel, by the workgroups that the bounds of a call allow (few sequences are as long as the longest).  us, few
-// rows / strips / tiles, 16 query and 8 kv heads unless given:
+// rows / strips / tiles, 4-bit cache, 16 query and 8 kv heads unless given:
 //   1 x 20 rows on 4,096 cached   20 /  32 / 132        1 x 1,000 on 4,096    87 /  60 / 163
 //   1 x 100 on 4,096              21 /  32 / 135        1 x 4,000 on none    171 /  96 / 151
 //   the same, 40 and 8 heads      21 /  34 / 134        4 x 2,000 on 1,152     - / 194 / 194 (1,000 workgroups of tiles)
 //   1 x 300 on none               10 / 8.7 /  16        3 x 3,000 on none      - / 163 / 146 (1,128)
 //   8 x 64 on 1,040               19 /  15 /  41        16 x 2,000 on 1,152    - / 698 / 642 (4,096)
+// The 8-bit cache has the same borders: 1 x 20 on 4,096 11.3 / 13.9, 8 x 64 on 1,040 19.8 / 13.5, 4 x 2,000 on 1,152
+// - / 177 / 200, 8 x 2,000 on none - / 214 / 195 (with slower tiles than now).
 // Few rows: while one round over the CUs takes them all.  Tiles: from four workgroups a CU on; before, whole CUs wait
 // for the longest rows.
 constexpr int64_t kFewGroups = 256;
