@@ -548,6 +548,19 @@ def test_prefill_scores_far_apart(device, bound):
 
 
 @BOUNDS
+def test_prefill_rows_do_not_follow_their_neighbours(device, bound):
+    """A row whose reference moves often, or whose scores overflow, leaves the bits of those beside it as they are."""
+    batch = Batch(device, [200, 700], 4, 2, 16, seed=31, spread=1.5)
+    q = batch.queries(300)
+    clean = batch.prefill(q, [100, 200], max_q=bound)
+    loud = q.clone()
+    loud[1::4] *= 40
+    loud[3::8] = 3e38
+    got = batch.prefill(loud, [100, 200], max_q=bound)
+    assert torch.equal(got[0::2], clean[0::2]) and not torch.equal(got[1::4], clean[1::4])
+
+
+@BOUNDS
 @EXPONENTS
 def test_prefill_of_numbers_far_from_one(device, q_exp, k_exp, v_exp, bound):
     batch = Batch(device, [1, 70, 300], 4, 2, 32, seed=42)
