@@ -1131,7 +1131,7 @@ def copy_blocks(pools, sources: torch.Tensor, targets: torch.Tensor) -> None:
         check_block_pairs(sources, targets, blocks)
     stream = _stream_of(device, sources, targets, *pools)
     at = (ctypes.c_void_p * len(pools))(*(p.data_ptr() for p in pools))
-    sizes = (ctypes.c_int64 * len(pools))(*(p.stride(1) * p.element_size() for p in pools))
+    sizes = (ctypes.c_int64 * len(pools))(*(p.nbytes // (layers * blocks) for p in pools))
     status = lib.nvamd_copy_blocks(at, sizes, len(pools), layers, blocks, sources.data_ptr(), targets.data_ptr(), n,
                                    stream)
     if status:

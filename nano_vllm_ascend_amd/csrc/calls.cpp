@@ -328,7 +328,7 @@ PyObject *copy(PyObject *const *a) {
     if (i == 0) layers = t.size(0), blocks = t.size(1);
     need(t.size(0) == layers && t.size(1) == blocks);
     at[i] = t.data_ptr();
-    bytes[i] = t.stride(1) * (int64_t)t.element_size();
+    bytes[i] = (int64_t)t.nbytes() / (layers * blocks);  // a single block's stride says nothing
   }
   const int32_t *sources = lengths(a[1], dev, 0, false);
   const int64_t n = THPVariable_Unpack(a[1]).size(0);
