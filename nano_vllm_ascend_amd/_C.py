@@ -198,8 +198,6 @@ def _bind_calls(lib: ctypes.CDLL) -> None:
     """The library needs nothing of torch, the extension is tied to the torch that it was built with: without it the calls
     go through the checks in this file, with the same results."""
     global _calls
-    names = ("kv_cache_write_{}", "kv_cache_read_{}", "qk_norm_rope_{}", "paged_decode_{}", "paged_decode_fused_{}",
-             "paged_prefill_{}", "paged_prefill_{}_workspace_size")
     try:
         calls = importlib.import_module("._calls", __package__)
         if calls.ABI_VERSION != lib.nvamd_version():
@@ -210,8 +208,9 @@ def _bind_calls(lib: ctypes.CDLL) -> None:
                       f"be used ({e}); `python -m nano_vllm_ascend_amd.build` builds it", RuntimeWarning, stacklevel=3)
         return
     for index, kind in enumerate((_FP4, _FP8)):
-        functions = (getattr(lib, "nvamd_" + n.format(kind.name)) for n in names)
-        calls.bind(index, kind.pages, *(ctypes.cast(f, ctypes.c_void_p).value for f in functions))
+        functions = (kind.write, kind.read, kind.norm_rope, kind.decode, kind.decode_fused, kind.prefill,
+                     kind.prefill_workspace)
+        calls.bind(index, kind.pages, *(ctypes.cast(getattr(lib, f), ctypes.c_void_p).value for f in functions))
     calls.bind_copy(ctypes.cast(lib.nvamd_copy_blocks, ctypes.c_void_p).value)
     _calls = calls
 
@@ -677,10 +676,16 @@ class Fp8Pages(NamedTuple):
         return nb, bs, hkv, width
 
 
-class _Kind(NamedTuple):
-    name: str        # of the entry points
-    pages: type
-    row_bytes: int   # codes of a head vector
+class _Kind:
+    """A quantised cache: its pages, the bytes of a head vector's codes, the names of its entry points (put together here: in
+    a call they would take 0.1 us of its 4)."""
+
+    def __init__(self, name: str, pages: type, row_bytes: int):
+        self.name, self.pages, self.row_bytes = name, pages, row_bytes
+        self.write, self.read = f"nvamd_kv_cache_write_{name}", f"nvamd_kv_cache_read_{name}"
+        self.norm_rope = f"nvamd_qk_norm_rope_{name}"
+        self.decode, self.decode_fused = f"nvamd_paged_decode_{name}", f"nvamd_paged_decode_fused_{name}"
+        self.prefill, self.prefill_workspace = (f"nvamd_paged_prefill_{name}{s}" for s in ("", "_workspace_size"))
 
     def scales(self, nb: int, hkv: int, bs: int) -> tuple[int, ...]:
         return (nb, hkv, bs, FP4_ROW_SCALES) if self.pages is Fp4Pages else (nb, hkv, bs // FP8_TILE)
@@ -780,10 +785,11 @@ def _made(answer, name: str) -> bool:
 
 
 def _write(kind: _Kind, key_states, value_states, key_pages, value_pages, slot_mapping) -> None:
-    lib, name = _lib or load(), f"nvamd_kv_cache_write_{kind.name}"
-    if _calls and not _range_checks and type(key_pages) is kind.pages and _made(
-            _calls.write(key_states, value_states, key_pages, value_pages, slot_mapping), name):
-        return
+    lib, name = _lib or load(), kind.write
+    if _calls and not _range_checks and type(key_pages) is kind.pages:
+        made = _calls.write(key_states, value_states, key_pages, value_pages, slot_mapping)
+        if made is True or _made(made, name):
+            return
     nb, bs, hkv, pages, device = _checked_pages(kind, key_pages, value_pages)
     t, d = key_states.shape[0], _HEAD_DIM
     k_stride, v_stride = _heads("key_states", key_states, t, hkv, d), _heads("value_states", value_states, t, hkv, d)
@@ -796,10 +802,10 @@ def _write(kind: _Kind, key_states, value_states, key_pages, value_pages, slot_m
 
 
 def _read(kind: _Kind, key_pages, value_pages, slot_mapping, k_out, v_out) -> tuple[torch.Tensor, torch.Tensor]:
-    lib, name = _lib or load(), f"nvamd_kv_cache_read_{kind.name}"
+    lib, name = _lib or load(), kind.read
     if _calls and not _range_checks and k_out is None and v_out is None and type(key_pages) is kind.pages:
         rows = _calls.read(key_pages, value_pages, slot_mapping)
-        if _made(rows, name):
+        if type(rows) is tuple or _made(rows, name):
             return rows
     nb, bs, hkv, pages, device = _checked_pages(kind, key_pages, value_pages)
     t, d = slot_mapping.shape[0], _HEAD_DIM
@@ -833,11 +839,11 @@ def _rope_args(q_weight, k_weight, positions, cos_sin, t: int, d: int) -> None:
 
 def _norm_rope(kind: _Kind, q, k, v, q_weight, k_weight, positions, cos_sin, eps, key_pages, value_pages, slot_mapping,
                q_out, k_out) -> torch.Tensor:
-    lib, name = _lib or load(), f"nvamd_qk_norm_rope_{kind.name}"
+    lib, name = _lib or load(), kind.norm_rope
     if _calls and not _range_checks and type(key_pages) is kind.pages:
         rotated = _calls.rope(q, k, v, q_weight, k_weight, positions, cos_sin, eps, key_pages, value_pages, slot_mapping,
                               q_out, k_out)
-        if _made(rotated, name):
+        if type(rotated) is torch.Tensor or _made(rotated, name):
             return rotated
     nb, bs, hkv, pages, device = _checked_pages(kind, key_pages, value_pages)
     d = _HEAD_DIM
@@ -911,10 +917,10 @@ def _step_args(block_tables, context_lens, workspace, b: int) -> None:
 
 def _decode(kind: _Kind, out, q, key_pages, value_pages, block_tables, context_lens, scale, max_context_len,
             workspace) -> torch.Tensor:
-    lib, name = _lib or load(), f"nvamd_paged_decode_{kind.name}"
+    lib, name = _lib or load(), kind.decode
     if _calls and not _range_checks and type(key_pages) is kind.pages:
         made = _calls.decode(out, q, key_pages, value_pages, block_tables, context_lens, scale, max_context_len, workspace)
-        if _made(made, name):
+        if type(made) is torch.Tensor or _made(made, name):
             return made
     if out is None:
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
@@ -934,11 +940,11 @@ def _decode(kind: _Kind, out, q, key_pages, value_pages, block_tables, context_l
 
 def _decode_fused(kind: _Kind, out, q, k, v, q_weight, k_weight, positions, cos_sin, eps, key_pages, value_pages,
                   slot_mapping, block_tables, context_lens, scale, max_context_len, workspace) -> torch.Tensor:
-    lib, name = _lib or load(), f"nvamd_paged_decode_fused_{kind.name}"
+    lib, name = _lib or load(), kind.decode_fused
     if _calls and not _range_checks and type(key_pages) is kind.pages:
         made = _calls.decode_fused(out, q, k, v, q_weight, k_weight, positions, cos_sin, eps, key_pages, value_pages,
                                    slot_mapping, block_tables, context_lens, scale, max_context_len, workspace)
-        if _made(made, name):
+        if type(made) is torch.Tensor or _made(made, name):
             return made
     if out is None:
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
@@ -967,10 +973,11 @@ def _decode_fused(kind: _Kind, out, q, k, v, q_weight, k_weight, positions, cos_
 
 def _prefill(kind: _Kind, out, q, key_pages, value_pages, block_tables, cu_seqlens_q, kv_lens, max_q_len,
              scale) -> torch.Tensor:
-    lib, name = _lib or load(), f"nvamd_paged_prefill_{kind.name}"
-    if _calls and not _range_checks and type(key_pages) is kind.pages and _made(
-            _calls.prefill(out, q, key_pages, value_pages, block_tables, cu_seqlens_q, kv_lens, max_q_len, scale), name):
-        return out
+    lib, name = _lib or load(), kind.prefill
+    if _calls and not _range_checks and type(key_pages) is kind.pages:
+        made = _calls.prefill(out, q, key_pages, value_pages, block_tables, cu_seqlens_q, kv_lens, max_q_len, scale)
+        if made is out or _made(made, name):
+            return out
     if cu_seqlens_q.dtype is not torch.int32 or cu_seqlens_q.dim() != 1 or not cu_seqlens_q.is_contiguous():
         raise ValueError("cu_seqlens_q must be contiguous int32 [n + 1]")
     n = cu_seqlens_q.numel() - 1
@@ -981,7 +988,7 @@ def _prefill(kind: _Kind, out, q, key_pages, value_pages, block_tables, cu_seqle
     if _range_checks and _checking():
         check_paged_context(block_tables[:n], kv_lens[:n], args[8], args[9])
     stream = _stream_of(device, q, out, block_tables, cu_seqlens_q, kv_lens)
-    need = getattr(lib, f"{name}_workspace_size")(n, max_q_len, heads[0], heads[1], args[9], args[12])
+    need = getattr(lib, kind.prefill_workspace)(n, max_q_len, heads[0], heads[1], args[9], args[12])
     space = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None  # freed behind the call
     status = getattr(lib, name)(*args, cu_seqlens_q.data_ptr(), kv_lens.data_ptr(), n, q.shape[0], max_q_len,
                                 *heads, float(scale), space.data_ptr() if need else None, need, stream)
