@@ -403,8 +403,10 @@ class BlockManager:
         if not (len(slots) == len(seq_lens) == len(start_positions) == len(prefix_block_ids)):
             raise ValueError("slots, seq_lens, start_positions and prefix_block_ids length mismatch")
         q_cum, kv_cum, tq, tkv = [], [], 0, 0
-        for slot, n, start, prefix in zip(slots, seq_lens, start_positions, prefix_block_ids):
+        # every prefix is kept first, so that no prompt's new blocks are the cached ones of another
+        for slot, start, prefix in zip(slots, start_positions, prefix_block_ids):
             self._init_slot(slot, start, prefix)
+        for slot, n, start in zip(slots, seq_lens, start_positions):
             end = start + n
             self.ensure_blocks(slot, end)
             self.seq_lens[slot] = max(self.seq_lens[slot], end)
