@@ -230,6 +230,17 @@ class BlockManager:
             parent = kid
         return found
 
+    def holds_prefix(self, token_ids, block_ids: list[int]) -> bool:
+        """Whether these blocks still hold the first tokens, as they did when ``find_longest_prefix_blocks`` gave them: one
+        that nobody used meanwhile may have been handed out since (not in the reference, which does not look)."""
+        parent: int | None = None
+        bs = self.block_size
+        for i, block_id in enumerate(block_ids):
+            parent = self._key_id(parent, self._token_tuple(token_ids, i * bs, (i + 1) * bs), create=False)
+            if parent is None or self.blocks[block_id].block_hash != parent:
+                return False
+        return True
+
     def cache_full_blocks(self, slot: int, token_ids, num_cached_blocks: int = 0,
                           num_full_blocks: int | None = None) -> None:
         table = self.block_tables[slot]

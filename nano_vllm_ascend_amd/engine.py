@@ -23,9 +23,9 @@ class EngineCore:
         self.runner = runner
         self.scheduler = scheduler
 
-    def step(self, eos_token_id: int) -> list[Sequence]:
-        """Run one step; return the requests that finished in it."""
-        plan = self.scheduler.plan_next_step(eos_token_id)
+    def step(self, eos_token_id: int, replan=None) -> list[Sequence]:
+        """Run one step; return the requests that finished in it.  ``replan``: of ``plan_next_step``."""
+        plan = self.scheduler.plan_next_step(eos_token_id, replan)
         for seq in plan.retired:
             self.runner.free_seq(seq)
         if plan.admitted:
@@ -97,6 +97,14 @@ class LLM:
         seq.reserved_blocks = self.scheduler.compute_required_blocks(runtime_prompt_len=seq.runtime_prompt_len,
                                                                      max_new_tokens=seq.max_new_tokens)
 
+    def _replan(self, seq: Sequence) -> bool:
+        """Plan a queued request anew if its cached prefix is gone (a block that nobody used when it was planned may have
+        been handed out since); whether it was."""
+        if not seq.cached_block_ids or self.runner.block_manager.holds_prefix(seq.prompt_token_ids, seq.cached_block_ids):
+            return False
+        self._plan_prompt(seq)
+        return True
+
     def submit(self, prompt, max_new_tokens: int = 128, sampling_params: SamplingParams | None = None, *,
                temperature: float | None = None, top_k: int | None = None, top_p: float | None = None) -> int:
         """Queue one request (a string, tokenized with the chat template, or token ids); return its id."""
@@ -124,10 +132,9 @@ class LLM:
         params = _params(sampling_params or seq.sampling_params, temperature, top_k, top_p)
         child = seq.fork(self.scheduler.next_seq_id(), budget, params)
         child.reserved_blocks = blocks
-        taken = self.runner.fork(seq, child) or ()
-        for waiting in self.scheduler.waiting:  # whose cached prefix lay in the block that the copy took
-            if not set(waiting.cached_block_ids).isdisjoint(taken):
-                self._plan_prompt(waiting)
+        self.runner.fork(seq, child)
+        for waiting in self.scheduler.waiting:  # the copy may have taken a cached block
+            self._replan(waiting)
         return self.scheduler.add_running(child).seq_id
 
     def _output(self, seq: Sequence) -> dict[str, object]:
@@ -138,7 +145,7 @@ class LLM:
 
     def step(self) -> list[dict[str, object]]:
         """Advance every request by one engine step; return the outputs of those that finished."""
-        finished = self.engine_core.step(int(self.runner.tokenizer.eos_token_id))
+        finished = self.engine_core.step(int(self.runner.tokenizer.eos_token_id), self._replan)
         return [self._output(seq) for seq in finished]
 
     def generate(self, prompts: list, max_new_tokens: int = 128, sampling_params: SamplingParams | None = None, *,

@@ -418,13 +418,12 @@ class ModelRunner:
     def decode_graph_stats(self) -> dict[str, int]:
         return {} if self.decode_graph_runner is None else self.decode_graph_runner.stats_dict()
 
-    def fork(self, seq: Sequence, child: Sequence) -> list[int]:
-        """The child's context: the full blocks of seq's, and a copy of a partly filled one.  Returns the blocks taken."""
+    def fork(self, seq: Sequence, child: Sequence) -> None:
+        """The child's context: the full blocks of seq's, and a copy of a partly filled one."""
         self._drop_in_flight()  # the next batch is another one
         pairs = self.block_manager.fork_slot(seq.seq_id, child.seq_id)
         if pairs:
             self.kv_cache.copy_blocks(*zip(*pairs))
-        return [target for _, target in pairs]
 
     def free_seq(self, seq: Sequence) -> None:
         self._drop_in_flight()  # a finishing sequence was in the launched batch

@@ -116,7 +116,9 @@ class MiniScheduler:
             return "eos"
         return "max_new_tokens" if seq.reach_max_tokens() else None
 
-    def plan_next_step(self, eos_token_id: int) -> StepPlan:
+    def plan_next_step(self, eos_token_id: int, replan=None) -> StepPlan:
+        """``replan(request)``: asked before a request is admitted; True if its cached prefix was gone and it has been
+        planned anew, with another reservation."""
         plan = StepPlan()
         verdicts = [(seq, self._finish_reason(seq, eos_token_id)) for seq in self.running.values()]
         for seq, reason in verdicts:
@@ -128,6 +130,8 @@ class MiniScheduler:
             head = self.waiting[0]
             if len(self.running) >= self.max_num_seqs or not self.budget.fits(head.reserved_blocks):
                 break
+            if replan is not None and replan(head):
+                continue
             self.waiting.popleft()
             head.status = SequenceStatus.RUNNING
             self.budget.take(head.reserved_blocks)
