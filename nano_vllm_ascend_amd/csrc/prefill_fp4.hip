@@ -282,7 +282,8 @@ __device__ __forceinline__ void add_strip(f32x16 (&acc)[4], u32x4 codes, u32 v_s
   }
 }
 
-__global__ void __launch_bounds__(kStripWaves * 64) __attribute__((amdgpu_waves_per_eu(3)))
+constexpr int kStripsOnCu = 3;  // a wave of the workgroup on each SIMD
+__global__ void __launch_bounds__(kStripWaves * 64) __attribute__((amdgpu_waves_per_eu(kStripsOnCu)))
 prefill_strip_fp4_kernel(PrefillArgs<Fp4Cache> a) {
   __shared__ __attribute__((aligned(16))) float s_o[kStripWaves][kStripRows / 2][kRec];
   __shared__ float s_m[kStripWaves][kStripRows];
@@ -594,7 +595,7 @@ using namespace nvamd;
 
 extern "C" size_t nvamd_paged_prefill_fp4_workspace_size(int n_seqs, int max_q_len, int num_heads, int num_kv_heads,
                                                          int block_size, int bt_width) {
-  return prefill_workspace_bytes(n_seqs, max_q_len, num_heads, num_kv_heads, block_size, bt_width);
+  return prefill_workspace_bytes<kStripsOnCu>(n_seqs, max_q_len, num_heads, num_kv_heads, block_size, bt_width);
 }
 
 extern "C" int nvamd_paged_prefill_fp4(void *out, int64_t out_stride, const void *q, int64_t q_stride,
@@ -608,7 +609,7 @@ extern "C" int nvamd_paged_prefill_fp4(void *out, int64_t out_stride, const void
                           const_cast<u8 *>(static_cast<const u8 *>(k_scales)),
                           const_cast<u8 *>(static_cast<const u8 *>(v_codes)),
                           const_cast<u8 *>(static_cast<const u8 *>(v_scales))};
-  return prefill(prefill_few_fp4_kernel, prefill_strip_fp4_kernel, prefill_fp4_kernel, cache,
+  return prefill<kStripsOnCu>(prefill_few_fp4_kernel, prefill_strip_fp4_kernel, prefill_fp4_kernel, cache,
                  fp4_cache_ok(k_codes, k_scales, v_codes, v_scales), out, out_stride, q, q_stride, num_blocks, block_size,
                  block_tables, bt_stride, bt_width, cu_seqlens_q, kv_lens, n_seqs, num_tokens, max_q_len, num_heads,
                  num_kv_heads, head_dim, scale, workspace, workspace_bytes, stream);

@@ -338,8 +338,9 @@ prefill_join_kernel(Args a, int per_group) {
 //   the same, 40 and 8 heads      21 /  34 / 134        4 x 2,000 on 1,152     - / 194 / 194 (1,000 workgroups of tiles)
 //   1 x 300 on none               10 / 8.7 /  16        3 x 3,000 on none      - / 163 / 146 (1,128)
 //   8 x 64 on 1,040               19 /  15 /  41        16 x 2,000 on 1,152    - / 698 / 642 (4,096)
-// The 8-bit cache has the same borders: 1 x 20 on 4,096 11.3 / 13.9, 8 x 64 on 1,040 19.8 / 13.5, 4 x 2,000 on 1,152
-// - / 177 / 200, 8 x 2,000 on none - / 214 / 195 (with slower tiles than now).
+// The 8-bit cache has the same borders: 1 x 20 on 4,096 11.0 / 13.9, 8 x 64 on 1,040 20.3 / 14.0, 1 x 4,000 on none - / 85
+// / 120, 4 x 2,000 on 1,152 (1,024) - / 172 / 172, 5 x 2,000 on 1,152 (1,280) - / 214 / 209, 3 x 3,000 on none - / 150 /
+// 129, 8 x 2,000 on none (2,048) - / 207 / 166, 16 x 2,000 on 1,152 - / 695 / 584.
 // Few rows: while one round over the CUs takes them all.  Tiles: from four workgroups a CU on; before, whole CUs wait
 // for the longest rows.
 constexpr int64_t kFewGroups = 256;
@@ -348,8 +349,13 @@ constexpr int64_t kStripGroups = 1024;  // of the tile kernel
 // Where few rows or strips leave the card idle and contexts may be long, the keys are cut until the workgroups fill it
 // once, at most kMaxSplits times, and a second kernel joins the pieces (some 3 us).  us, uncut / cut: 1 x 20 rows on
 // 4,096 keys 20 / 12.4, 2 x 20 on 8,192 35 / 17.6, 1 x 300 on 8,192 61 / 44, 1 x 600 on 8,192 93 / 79.  Few rows take a
-// CU each, strips a third of one (with half: 45 and 93).
-constexpr int kSplitFrom = 4096;  // keys that the block tables hold
+// CU each; of strips a CU holds STRIPS_ON_CU: three of the 4-bit cache's (cut for two: 45 and 93), two of the 8-bit
+// cache's (cut for two / for three: 1 x 300 on 4,096 24.5 / 31.0, on 8,192 37.8 / 43.2, on 16,384 57.7 / 67.3; 3 x 100 on
+// 4,096 25.8 / 33.6).
+// Between one and two whole strips a CU, halves in a round and a half take less than one uneven round, but only of long
+// contexts (8-bit cache, uncut / halves: 1 x 600 on 8,192 69.5 / 72.4, on 16,384 127.6 / 123.4, on 30,000 224.7 / 207.6).
+constexpr int kSplitFrom = 4096;    // keys that the block tables hold
+constexpr int kHalvesFrom = 16384;
 constexpr int kMaxSplits = 32;
 
 struct Plan {
@@ -358,7 +364,8 @@ struct Plan {
   int splits;
   size_t workspace;
 };
-inline Plan plan_prefill(int64_t n_seqs, int64_t max_rows, int64_t num_kv_heads, int64_t cap) {
+template <int STRIPS_ON_CU>
+Plan plan_prefill(int64_t n_seqs, int64_t max_rows, int64_t num_kv_heads, int64_t cap) {
   const int64_t units = n_seqs * num_kv_heads;
   const auto tiles_of = [&](int rows) { return (max_rows + rows - 1) / rows; };
   Plan p;
@@ -368,29 +375,31 @@ inline Plan plan_prefill(int64_t n_seqs, int64_t max_rows, int64_t num_kv_heads,
     slots = 256;
   } else if (tiles_of(kTileRows) * units <= kStripGroups) {
     p.rows = kStripRows;
-    slots = 3 * 256;
+    slots = STRIPS_ON_CU * 256;
   } else {
     p.rows = kTileRows;
   }
   p.tiles = tiles_of(p.rows);
   const int64_t wanted = cap < kSplitFrom ? 1 : min(slots / (p.tiles * units), min(cap / kMinSplit, (int64_t)kMaxSplits));
   p.splits = (int)max(wanted, (int64_t)1);
+  if (p.rows == kStripRows && cap >= kHalvesFrom && 2 * p.tiles * units <= 3 * 256) p.splits = max(p.splits, 2);
   p.workspace = p.splits == 1 ? 0 : (size_t)(units * p.splits * p.tiles * p.rows) * kRec * sizeof(float);
   return p;
 }
 
 // ------------------------------------------------------------------------------------------ a call
-inline size_t prefill_workspace_bytes(int n_seqs, int max_q_len, int num_heads, int num_kv_heads, int block_size,
+template <int STRIPS_ON_CU>
+size_t prefill_workspace_bytes(int n_seqs, int max_q_len, int num_heads, int num_kv_heads, int block_size,
                                       int bt_width) {
   if (n_seqs <= 0 || max_q_len <= 0 || num_kv_heads <= 0 || num_heads < num_kv_heads || block_size <= 0 || bt_width <= 0)
     return 0;
-  return plan_prefill(n_seqs, (int64_t)max_q_len * (num_heads / num_kv_heads), num_kv_heads,
+  return plan_prefill<STRIPS_ON_CU>(n_seqs, (int64_t)max_q_len * (num_heads / num_kv_heads), num_kv_heads,
                       (int64_t)bt_width * block_size)
       .workspace;
 }
 
 // Checks and launches; few, strip and tiles are the kernels.
-template <typename Cache>
+template <int STRIPS_ON_CU, typename Cache>
 int prefill(void (*few)(PrefillArgs<Cache>), void (*strip)(PrefillArgs<Cache>), void (*tiles)(PrefillArgs<Cache>),
             const Cache &cache, bool cache_ok, void *out, int64_t out_stride, const void *q, int64_t q_stride,
             int num_blocks, int block_size, const int32_t *block_tables, int bt_stride, int bt_width,
@@ -430,7 +439,7 @@ int prefill(void (*few)(PrefillArgs<Cache>), void (*strip)(PrefillArgs<Cache>), 
   a.group = num_heads / num_kv_heads;
   const int64_t max_rows = (int64_t)max_q_len * a.group;
   if (max_rows > 0x7fffffff) return NVAMD_EUNSUPPORTED;
-  const Plan plan = plan_prefill(n_seqs, max_rows, num_kv_heads, (int64_t)bt_width << bs_log2);
+  const Plan plan = plan_prefill<STRIPS_ON_CU>(n_seqs, max_rows, num_kv_heads, (int64_t)bt_width << bs_log2);
   if (plan.tiles > 65535) return NVAMD_EUNSUPPORTED;
   a.max_tiles = (int)plan.tiles;
   a.splits = 1;
