@@ -41,7 +41,7 @@ extern "C" {
 
 /* ABI version of this header; nvamd_version() returns the version the library was built
    with, for the loader's sanity check. */
-#define NVAMD_ABI_VERSION 5
+#define NVAMD_ABI_VERSION 6
 int nvamd_version(void);
 
 /* ------------------------------------------------------------------------- */
@@ -566,6 +566,30 @@ int nvamd_kv_cache_read_fp8(void *k, int64_t k_stride,
                             const int64_t *slot_mapping, int num_tokens,
                             int num_kv_heads, int head_dim,
                             hipStream_t stream);
+
+/* kv_cache_keep_fp8, kv_cache_restore_fp8: a row that goes behind others may */
+/* raise its tile's scale, which rounds their codes again; a caller that may  */
+/* have to take such rows back (a step run ahead of its time) keeps the tiles */
+/* first.  keep copies, of every layer [num_layers, num_blocks, ...], the     */
+/* tiles that rows at slot_mapping would go behind (none for a slot that      */
+/* begins a tile, -1, or one outside the cache) to `kept`, 16-byte aligned,   */
+/* of nvamd_kv_cache_kept_size_fp8 bytes; restore puts them back: the tokens  */
+/* before those rows are again as they were.                                  */
+size_t nvamd_kv_cache_kept_size_fp8(int num_layers, int num_tokens,
+                                    int num_kv_heads);
+int nvamd_kv_cache_keep_fp8(void *kept, size_t kept_bytes,
+                            const void *k_codes, const void *k_scales,
+                            const void *v_codes, const void *v_scales,
+                            int num_layers, int num_blocks, int block_size,
+                            const int64_t *slot_mapping, int num_tokens,
+                            int num_kv_heads, int head_dim,
+                            hipStream_t stream);
+int nvamd_kv_cache_restore_fp8(const void *kept, size_t kept_bytes,
+                               void *k_codes, void *k_scales,
+                               void *v_codes, void *v_scales,
+                               int num_layers, int num_blocks, int block_size,
+                               int num_tokens, int num_kv_heads, int head_dim,
+                               hipStream_t stream);
 
 /* qk_norm_rope_fp8: nvamd_qk_norm_rope_fp4 into the 8-bit cache (rows in the */
 /* order that nvamd_kv_cache_write_fp8 asks for).                             */

@@ -131,6 +131,15 @@ _SIGNATURES = {
         [_c_ptr, _c_i64, _c_ptr, _c_i64, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_int, _c_ptr, _c_int, _c_int,
          _c_int, _c_ptr],
     ),
+    "nvamd_kv_cache_kept_size_fp8": (_c_size, [_c_int, _c_int, _c_int]),
+    "nvamd_kv_cache_keep_fp8": (
+        _c_int,
+        [_c_ptr, _c_size, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_int, _c_int, _c_ptr, _c_int, _c_int, _c_int, _c_ptr],
+    ),
+    "nvamd_kv_cache_restore_fp8": (
+        _c_int,
+        [_c_ptr, _c_size, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_ptr],
+    ),
     "nvamd_qk_norm_rope_fp8": (
         _c_int,
         [_c_ptr, _c_i64, _c_ptr, _c_i64, _c_ptr, _c_i64, _c_ptr, _c_i64, _c_ptr, _c_i64, _c_ptr, _c_ptr, _c_ptr,
@@ -1026,6 +1035,42 @@ def kv_cache_read_fp8(key_pages: Fp8Pages, value_pages: Fp8Pages, slot_mapping: 
                       v_out: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """``kv_cache_read_fp4`` of pages of 8 bits (slots in any order)."""
     return _read(_FP8, key_pages, value_pages, slot_mapping, k_out, v_out)
+
+
+def _layers_fp8(pools):
+    """Checks the tensors of a cache of 8 bits [layers, ...]; layers, blocks, block_size, kv heads, addresses, device."""
+    kc, ks, vc, vs = pools
+    if any(t.dim() < 2 or t.shape[0] != kc.shape[0] or t.shape[0] == 0 or not t.is_contiguous() for t in pools):
+        raise ValueError("codes and scales must be contiguous tensors of as many layers")
+    nb, bs, hkv, _, device = _checked_pages(_FP8, Fp8Pages(kc[0], ks[0]), Fp8Pages(vc[0], vs[0]))
+    return kc.shape[0], nb, bs, hkv, [t.data_ptr() for t in pools], device
+
+
+def kv_cache_keep_fp8(pools, slot_mapping: torch.Tensor) -> torch.Tensor:
+    """The tiles of 16 slots, of every layer, that rows at these slots would go behind, as they are now.
+
+    ``pools``: key codes, key scales, value codes and value scales of an ``Fp8PagedKVCache`` [layers, ...].  Such rows may
+    raise a tile's scale, which rounds the codes of the others again; ``kv_cache_restore_fp8`` undoes it."""
+    lib = _lib or load()
+    layers, nb, bs, hkv, at, device = _layers_fp8(pools)
+    t = slot_mapping.shape[0] if slot_mapping.dim() == 1 else -1
+    slots = _page_slots(slot_mapping, t, nb * bs)
+    stream = _stream_of(device, slot_mapping)
+    kept = torch.empty((t, lib.nvamd_kv_cache_kept_size_fp8(layers, 1, hkv)), dtype=torch.uint8, device=pools[0].device)
+    _check(lib.nvamd_kv_cache_keep_fp8(kept.data_ptr(), kept.nbytes, *at, layers, nb, bs, slots, t, hkv, _HEAD_DIM, stream),
+           "nvamd_kv_cache_keep_fp8")
+    return kept
+
+
+def kv_cache_restore_fp8(pools, kept: torch.Tensor) -> None:
+    """Puts back what ``kv_cache_keep_fp8`` kept: the tokens before those rows are again as they were."""
+    lib = _lib or load()
+    layers, nb, bs, hkv, at, device = _layers_fp8(pools)
+    if (kept.dtype is not torch.uint8 or kept.dim() != 2 or not kept.is_contiguous()
+            or kept.shape[1] != lib.nvamd_kv_cache_kept_size_fp8(layers, 1, hkv)):
+        raise ValueError(f"kept must be what was kept of {layers} layers of {hkv} heads, got {tuple(kept.shape)}")
+    _check(lib.nvamd_kv_cache_restore_fp8(kept.data_ptr(), kept.nbytes, *at, layers, nb, bs, kept.shape[0], hkv, _HEAD_DIM,
+                                          _stream_of(device, kept)), "nvamd_kv_cache_restore_fp8")
 
 
 def qk_norm_rope_fp4(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_weight: torch.Tensor,

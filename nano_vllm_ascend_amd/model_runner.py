@@ -27,7 +27,9 @@ Differences from the reference, all on the hot path:
     discarded step wrote K/V only into rows no live sequence has reached and
     into free blocks that carry no prefix-cache key (others are never packed
     ahead), and every later write to those rows is ordered after it on the
-    stream.
+    stream.  In an 8-bit cache such a row may also have raised the scale that
+    it shares with up to 15 tokens before it, and their codes were rounded
+    again: the tiles are kept before the launch and put back.
 """
 from __future__ import annotations
 
@@ -74,7 +76,7 @@ class _TokenFetch:
 class _InFlightStep:
     """A decode step launched ahead of the call that asks for it (not yet applied to the pool)."""
 
-    def __init__(self, seqs, positions, taken, entry, fetch: _TokenFetch, logits: torch.Tensor, snapshot=None):
+    def __init__(self, seqs, positions, taken, entry, fetch: _TokenFetch, logits: torch.Tensor, snapshot=None, kept=None):
         self.seqs = list(seqs)
         self.slots = [seq.seq_id for seq in seqs]
         self.positions = positions
@@ -83,6 +85,7 @@ class _InFlightStep:
         self.fetch = fetch
         self.logits = logits
         self.snapshot = snapshot    # host copy of its metadata, kept only for a metadata hook
+        self.kept = kept            # tiles of an 8-bit cache that its rows go behind, as they were
 
     def matches(self, seqs, positions) -> bool:
         return (len(seqs) == len(self.seqs) and all(a is b for a, b in zip(seqs, self.seqs))
@@ -253,9 +256,11 @@ class ModelRunner:
     # ------------------------------------------------------------- forward
     def _drop_in_flight(self) -> None:
         """Forget a step launched ahead: the batch it assumed is not the next one."""
-        if self._in_flight is not None:
-            self._in_flight = None
+        ahead, self._in_flight = self._in_flight, None
+        if ahead is not None:
             self.overlap_stats["discarded"] += 1
+            if ahead.kept is not None:
+                self.kv_cache.restore_tiles(ahead.kept)
 
     @staticmethod
     def _host_metadata(md) -> PagedKVCacheMetadata:
@@ -352,10 +357,12 @@ class ModelRunner:
         slots = [seq.seq_id for seq in seqs]
         b = len(seqs)
         graph = self.decode_graph_runner
+        if self._in_flight is not None and not self._in_flight.matches(seqs, positions):
+            self._drop_in_flight()
         ahead, self._in_flight = self._in_flight, None
         entry = fetch = logits = None
         reported = False
-        if ahead is not None and ahead.matches(seqs, positions):
+        if ahead is not None:
             # launched by the previous call: apply it to the pool now that the batch is confirmed
             self.block_manager.commit_decode_ahead(ahead.slots, ahead.positions, ahead.taken)
             entry, fetch, logits = ahead.entry, ahead.fetch, ahead.logits
@@ -363,8 +370,6 @@ class ModelRunner:
             if ahead.snapshot is not None:
                 self._report("decode", slots, ahead.snapshot, is_host_copy=True)
         else:
-            if ahead is not None:
-                self.overlap_stats["discarded"] += 1
             if graph is not None and graph.supports(b):
                 entry = graph.entry_for(b, 1, self.device, self.block_size)
                 md = self.block_manager.prepare_decode_metadata(slots, positions, 1, token_ids=tokens,
@@ -409,9 +414,12 @@ class ModelRunner:
         md, taken = packed
         kept = self._keep_logits(b, logits) if self.retain_logits else None
         snapshot = self._host_metadata(md) if self.metadata_hook is not None else None
+        # its rows may raise the scales of tiles with live tokens, and that has to be undone if it is dropped
+        keep = getattr(self.kv_cache, "keep_tiles", None)
+        tiles = keep(entry.buffers["slot_mapping"]) if keep else None
         nxt_logits = self.decode_graph_runner.replay(entry)  # its input ids: step N's argmax, in place
         self._in_flight = _InFlightStep(seqs, nxt, taken, entry, self._fetch_tokens(b, entry.buffers["greedy_ids"]),
-                                        nxt_logits, snapshot)
+                                        nxt_logits, snapshot, tiles)
         self.overlap_stats["launched"] += 1
         return kept
 

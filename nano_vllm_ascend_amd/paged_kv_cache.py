@@ -99,10 +99,13 @@ class _QuantisedKVCache:
     def get_physical_cache(self, layer_idx: int):
         return self._pages[layer_idx]
 
+    @property
+    def _pools(self) -> tuple[torch.Tensor, ...]:
+        return self.key_codes, self.key_scales, self.value_codes, self.value_scales
+
     def copy_blocks(self, sources, targets) -> None:
         """Blocks sources[i] to targets[i], in every layer (``_copy_blocks``)."""
-        _copy_blocks((self.key_codes, self.key_scales, self.value_codes, self.value_scales), self.num_blocks, sources,
-                     targets)
+        _copy_blocks(self._pools, self.num_blocks, sources, targets)
 
 
 class Fp4PagedKVCache(_QuantisedKVCache):
@@ -165,3 +168,11 @@ class Fp8PagedKVCache(_QuantisedKVCache):
     def read(self, layer_idx: int, slot_mapping: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
         """The bf16 keys and values [T, kv heads, head_dim] that the layer holds at the slots (zeros for -1)."""
         return _C.kv_cache_read_fp8(*self.get_physical_cache(layer_idx), self._slots(slot_mapping))
+
+    def keep_tiles(self, slot_mapping: torch.Tensor) -> torch.Tensor:
+        """The tiles that rows at the slots would go behind, in every layer: such rows may raise a tile's scale, which
+        rounds its other tokens again.  ``restore_tiles`` takes them back."""
+        return _C.kv_cache_keep_fp8(self._pools, self._slots(slot_mapping))
+
+    def restore_tiles(self, kept: torch.Tensor) -> None:
+        _C.kv_cache_restore_fp8(self._pools, kept)
