@@ -64,6 +64,8 @@ int nvamd_version(void);
 #define NVAMD_ERR_POSITION 2u /* position < 0 or >= the RoPE table's rows    */
 #define NVAMD_ERR_CONTEXT 4u  /* context < 0 or past its table row / bound   */
 #define NVAMD_ERR_BLOCK 8u    /* block-table entry < 0 or >= num_blocks      */
+#define NVAMD_ERR_ORDER 16u   /* rows of an 8-bit tile that do not follow one */
+                              /* another (nvamd_kv_cache_write_fp8)          */
 int nvamd_errors_fetch(unsigned *host, hipStream_t stream);
 int nvamd_errors_clear(hipStream_t stream);
 
@@ -544,8 +546,11 @@ size_t nvamd_paged_prefill_fp4_workspace_size(int n_seqs, int max_q_len,
 /* kv_cache_write_fp8: row t of k and v goes to slot_mapping[t] (-1: padding, */
 /* skipped).  The rows of a tile follow one another in the call, in the order */
 /* of their slots and with no padding row between them, as the tokens of a    */
-/* sequence do; those of different tiles come in any order.  (Else the tile   */
-/* holds none of them as a whole.)                                            */
+/* sequence do; those of different tiles come in any order.  Rows in the tile */
+/* of one of the NVAMD_FP8_ORDER_ROWS rows before them that do not follow it  */
+/* are skipped and reported (NVAMD_ERR_ORDER); where they are farther apart,  */
+/* the tile holds neither as a whole.                                         */
+#define NVAMD_FP8_ORDER_ROWS 32
 int nvamd_kv_cache_write_fp8(const void *k, int64_t k_stride,
                              const void *v, int64_t v_stride,
                              void *k_codes, void *k_scales,

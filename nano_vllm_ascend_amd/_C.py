@@ -278,12 +278,13 @@ def version() -> int:
 # lookup, the block-table gather), the kernels skip or clamp the access and set a bit in a
 # per-device error word.  The runner copies the word to the host with each step's tokens (no extra
 # synchronisation) and raises IndexError there.
-ERR_SLOT, ERR_POSITION, ERR_CONTEXT, ERR_BLOCK = 1, 2, 4, 8  # NVAMD_ERR_*
+ERR_SLOT, ERR_POSITION, ERR_CONTEXT, ERR_BLOCK, ERR_ORDER = 1, 2, 4, 8, 16  # NVAMD_ERR_*
 _ERR_TEXT = {
     ERR_SLOT: "a slot_mapping entry outside the KV cache (index_copy_, nv/npu/paged_kv_cache.py:68-69)",
     ERR_POSITION: "a position outside the RoPE table (nv/layers/rotary_embedding.py:49-50)",
     ERR_CONTEXT: "a context length its block-table row or the launch's bound cannot hold",
     ERR_BLOCK: "a block-table entry outside the block pool",
+    ERR_ORDER: "rows of a 16-slot tile of an 8-bit cache that do not follow one another in the order of their slots",
 }
 
 
@@ -1018,7 +1019,8 @@ def kv_cache_write_fp8(key_states: torch.Tensor, value_states: torch.Tensor, key
     """Rows [T, Hkv, 128] of bf16 keys and values, quantised into the pages at their slots (-1: padding, skipped).
 
     The rows of a tile of 16 slots follow one another, in the order of their slots, as a sequence's tokens do; tiles come
-    in any order.  Rows that begin a tile set its scale and start it anew, others raise it where they need to and keep
+    in any order.  Rows in the tile of one of the 32 before them that do not follow it are not stored and reported
+    (``ERR_ORDER`` in the error word); ``set_range_checks(True)`` refuses all other orders, too.  Rows that begin a tile set its scale and start it anew, others raise it where they need to and keep
     what the tile holds."""
     _write(_FP8, key_states, value_states, key_pages, value_pages, slot_mapping)
 

@@ -82,25 +82,34 @@ __device__ __forceinline__ void keep_here(float (&cs)[8], float (&sn)[8], u32x4 
 
 // Runs among rows base .. base + ROWS - 1: calls body(first row, its slot, rows).  A run is rows whose slots follow one
 // another inside a tile; it may go on past the wave's own rows.  Rows without a slot come as runs of one, slot -1, if
-// asked for.
+// asked for.  So does a run in a tile that an earlier row of the wave's window lies in (two waves would write the tile at
+// once): it is reported, and stored by nobody.
 template <int ROWS, typename Body>
 __device__ __forceinline__ void for_runs(const RowsArgs &a, int64_t base, int lane, bool report, bool slotless,
                                          Body &&body) {
-  const int64_t r = base - 1 + lane;  // lane 0: the row before
-  const bool exists = lane < ROWS + kFp8Tile && r >= 0 && r < a.num_tokens;
+  constexpr int kBefore = 64 - ROWS - (kFp8Tile - 1);  // rows of the window before the wave's own; those that a run needs
+  static_assert(kBefore >= 1 && kBefore >= NVAMD_FP8_ORDER_ROWS, "behind them end the window");
+  const int64_t r = base - kBefore + lane;
+  const bool exists = r >= 0 && r < a.num_tokens;
   int64_t slot = exists ? a.slots[r] : -1;
   if (slot >= a.num_slots || slot < -1) {  // skip the row, report it once
-    if (report && lane >= 1 && lane <= ROWS) flag_index_error(a.err, NVAMD_ERR_SLOT);
+    if (report && lane >= kBefore && lane < kBefore + ROWS) flag_index_error(a.err, NVAMD_ERR_SLOT);
     slot = -1;
   }
   const int64_t before = __shfl_up(slot, 1);
   const bool follows = lane > 0 && slot >= 0 && (slot & (kFp8Tile - 1)) != 0 && before + 1 == slot;
   const uint64_t go_on = __ballot(follows);
-  uint64_t begins = __ballot(exists && !follows && (slot >= 0 || slotless)) & (((1ull << ROWS) - 1) << 1);
+  uint64_t begins = __ballot(exists && !follows && (slot >= 0 || slotless)) & (((1ull << ROWS) - 1) << kBefore);
   while (begins != 0) {
     const int j = __ffsll((unsigned long long)begins) - 1;
     begins &= begins - 1;
-    body(base - 1 + j, lane_value(slot, j), __ffsll((unsigned long long)~(go_on >> (j + 1))));
+    int64_t first = lane_value(slot, j);
+    if (first >= 0 && __ballot(lane < j && slot >= 0 && (slot ^ first) < kFp8Tile) != 0) {
+      if (report && lane == 0) flag_index_error(a.err, NVAMD_ERR_ORDER);
+      if (!slotless) continue;
+      first = -1;
+    }
+    body(base - kBefore + j, first, __ffsll((unsigned long long)~(go_on >> (j + 1))));
   }
 }
 

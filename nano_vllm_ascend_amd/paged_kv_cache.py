@@ -162,6 +162,7 @@ class Fp8PagedKVCache(_QuantisedKVCache):
 
     def write(self, layer_idx: int, key_states: torch.Tensor, value_states: torch.Tensor,
               slot_mapping: torch.Tensor) -> None:
+        """Unlike the other caches' this asks for an order: the rows of a tile follow one another in that of their slots."""
         self._check_rows(key_states, slot_mapping)
         _C.kv_cache_write_fp8(key_states, value_states, *self.get_physical_cache(layer_idx), self._slots(slot_mapping))
 
