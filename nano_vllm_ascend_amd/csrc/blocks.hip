@@ -21,7 +21,6 @@ struct CopyArgs {
   int pieces[kMaxPools + 1];  // of a block: those of pool p are pieces[p] .. pieces[p + 1] - 1
   const int32_t *sources;
   const int32_t *targets;
-  int num_pools;
   int num_blocks;
   u32 *err;
 };
@@ -86,7 +85,6 @@ extern "C" int nvamd_copy_blocks(void *const *pools, const int64_t *block_bytes,
   }
   a.sources = sources;
   a.targets = targets;
-  a.num_pools = num_pools;
   a.num_blocks = num_blocks;
   a.err = index_error_word();
   hipLaunchKernelGGL(copy_blocks_kernel, dim3(a.pieces[num_pools], count, num_layers), dim3(kThreads), 0, stream, a);
