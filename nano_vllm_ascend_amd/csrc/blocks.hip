@@ -3,9 +3,9 @@
 // pool[layer][target[i]] = pool[layer][source[i]] for every layer of every pool, in one launch.  Bound by memory: each
 // byte is read once and written once.  A workgroup copies 16 KiB of a block's layer, a lane 64 bytes whose loads are on
 // their way together; the stores pass the caches by.  One block of 128 tokens of 8 heads in 28 layers of the 8-bit cache
-// (15 MB read and written): 3.0 us, 4.0 with ordinary stores, one load at a time; 8 blocks 21.8 us (5.4 TB/s), 26.2; 48
-// blocks of the bf16 cache, 1.4 GB, 271 us (5.2 TB/s, the rate of one large copy), 272.  Pieces of 8 KiB: 4.1, 24.5 and
-// 262 us, of 32: 3.3, 23.0 and 267.
+// (15 MB read and written): 3.0 us from a graph (4.1 to 4.4 eager, where the launch takes the host 3.6), 4.0 with ordinary
+// stores, one load at a time; 8 blocks 21.8 us (5.4 TB/s), 26.2; 48 blocks of the bf16 cache, 1.4 GB, 268 to 271 us (5.2
+// TB/s, the rate of one large copy), 272.  Pieces of 8 KiB: 4.1, 24.5 and 262 us, of 32: 3.3, 23.0 and 267.
 #include "common.h"
 
 namespace nvamd {

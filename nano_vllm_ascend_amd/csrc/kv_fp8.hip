@@ -438,9 +438,11 @@ int launch_kept(u8 *kept, size_t kept_bytes, void *k_codes, void *k_scales, void
   return launch_status();
 }
 
-// A wave looks after the runs that begin in one row up to here, in 16 rows from there on.  us, one / 16: 300 rows written
-// and read back 9.1 / 11.8, 1,000 11.8 / 11.6 (the host's time), 2,000 16.4 / 11.1, 4,000 26 / 12; 500 prompt rows rotated
-// and stored 10.7 / 12.0.
+// A wave looks after the runs that begin in one row up to here, in 16 rows from there on: the rows of a decode step have a
+// tile each, whose runs a wave takes one after another, those of a long prompt share tiles.  us from a graph, one / 16,
+// written: rows of a tile each, 32 3.2 / 17.7, 512 7.1 / 20.1, 1,000 11.8 / 20.8; of one run, 300 3.7 / 3.5, 500 4.4 / 3.4,
+// 1,000 6.6 / 3.6.  Rotated and stored, 16 query heads: of a tile each, 32 4.8 / 39.5, 512 13.5 / 42.4; of one run, 500 6.8 /
+// 5.2, 1,000 12.2 / 6.6.
 constexpr int kFewTokens = 512;
 
 template <bool ROPE>
@@ -528,8 +530,8 @@ extern "C" int nvamd_kv_cache_read_fp8(void *k, int64_t k_stride, void *v, int64
   a.k_stride = k_stride;
   a.v = static_cast<u16 *>(v);
   a.v_stride = v_stride;
-  // us, one / 16 rows to a wave, from a graph: 32 rows of 32 tiles 2.2 / 10.1, 512 of 500 tiles 3.9 / 12.7; 512 rows of a
-  // run 3.6 / 2.6, 1,000 5.5 / 2.8.
+  // us, one / 16 rows to a wave, from a graph: rows of a tile each, 32 2.5 / 10.3, 512 3.8 / 10.5, 1,000 5.5 / 10.5; of one
+  // run, 500 3.9 / 2.9, 1,000 5.8 / 3.0.
   const bool few = num_tokens <= kFewTokens;
   const dim3 grid((unsigned)ceil_div(num_tokens, few ? kWaves : kWaves * 16), 2u * num_kv_heads);
   if (few)

@@ -17,11 +17,12 @@
 //        just what the lane holds.  The cache keeps the 16 tokens of a dim in consecutive bytes: lanes gq and gq ^ 1 load
 //        16 bytes each of different dims of the same tile and swap halves, so that every load is whole.
 //
-// Bound by memory on long contexts, by latency on short ones: a token of a head is 256 bytes and 2 scales.  Measured
-// (8 kv heads, 16 query heads unless said): 4 contexts of up to 512 tokens 5.5 us; 32 of 256..2304 20.3 us (4.3 TB/s);
-// 100 of 2048..4096 105 us (5.9 TB/s); 4 of 8192..40960, 64 query heads, 35 us (4.9 TB/s); 16 of 512..4096, 64 query
-// heads, 16.3 us.  Steps of 64 tokens, a tile to 16 lanes, need registers for two waves a SIMD; four waves with half the
-// step hide more of the loads' latency: those 32 contexts took 23.7 us, the 100 as long, the 4 longest 2% less.
+// Bound by memory on long contexts, by latency on short ones: a token of a head is 256 bytes and 2 scales.  Measured (8
+// kv heads, 16 query heads unless said; the first and the last from a graph): 4 contexts of up to 512 tokens 5.6 us; 32
+// of 256..2304 19.3 to 19.7 us (4.4 TB/s); 100 of 2048..4096 102 us (6.1 TB/s); 4 of 8192..40960, 64 query heads, 31.2
+// to 31.7 us (5.5 TB/s); 16 of 512..4096, 64 query heads, 15.9 us.  Steps of 64 tokens, a tile to 16 lanes, need
+// registers for two waves a SIMD; four waves with half the step hide more of the loads' latency: those 32 contexts took
+// 23.7 us, the 100 as long, the 4 longest 2% less.
 // The score of a token past the context is replaced by -inf and its values by zero, whatever bytes it holds.
 #include "decode_quantised.h"
 #include "fp8_attention.h"

@@ -20,14 +20,15 @@
 //   paged_decode_fp8.hip with rows in the place of heads and a last key for each row.  On long contexts the keys are cut as
 //   well.
 //
-// Bounds and figures (16 query heads on 8 kv heads unless said).  Tiles: bound by the issue of instructions, since matrix
-// products and softmax (a tile of 32 keys: 12 products, some 75 vector instructions, 16 of them exponentials) do not
-// overlap, neither a wave's own nor, by the counters, those of different waves.  32 prompts of 512..2,048 tokens on 1,152
-// cached take 655 us (941 TFLOP/s) at three waves a SIMD, 842 at two; 40 query heads, 2 x U[3000, 4000] on 4,096 cached
-// 940 us (1,057 TFLOP/s).  Of the first, 12 us are the maximum that is only looked for where it matters (weigh_scores), 25
-// V's operands, which are on their way from LDS before they are needed, and 10 the fewer registers and instructions of the
-// pages' bookkeeping.  One barrier for two tiles, with four stages, gives 654: not worth it.
-// Strips: 1 x 4,000 on 4,096 220 us (911 TFLOP/s), 8 x 1..64 on 1,040 13.5 us.  Few short rows are bound by one step after
+// Bounds and figures (16 query heads on 8 kv heads unless said).  Tiles: bound by the issue of instructions, since
+// matrix products and softmax (a tile of 32 keys: 12 products, some 75 vector instructions, 16 of them exponentials) do
+// not overlap, neither a wave's own nor, by the counters, those of different waves.  32 prompts of 512..2,048 tokens on
+// 1,152 cached take 655 to 664 us (929 to 941 TFLOP/s) at three waves a SIMD, 842 at two; 40 query heads, 2 x U[3000,
+// 4000] on 4,096 cached 940 to 947 us (1,057 TFLOP/s).  Of the first, 12 us are the maximum that is only looked for
+// where it matters (weigh_scores), 25 V's operands, which are on their way from LDS before they are needed, and 10 the
+// fewer registers and instructions of the pages' bookkeeping.  One barrier for two tiles, with four stages, gives 654:
+// not worth it.
+// Strips: 1 x 4,000 on 4,096 217 us (925 TFLOP/s), 8 x 1..64 on 1,040 13.4 us.  Few short rows are bound by one step after
 // another in a wave, some 0.6 us, whose products, softmax and expansion wait for one another: loads two steps ahead (14.5)
 // and eight waves to a strip (13.6) gain nothing.  The registers of the 8-bit operands leave room for two waves a SIMD, and
 // strips and few rows take as long as the 4-bit cache's kernels at three.

@@ -118,7 +118,8 @@ class LLM:
         The new one goes on from the present state: the same prompt and tokens so far, the last sampled one among them.
         It shares the full blocks of the context; a partly filled block is copied.  Its budget ``max_new_tokens`` counts
         the tokens that it starts with, and like its sampling is that of the request it branches from unless given.
-        RuntimeError if it does not fit now (``max_num_seqs``, or its blocks for its whole life)."""
+        RuntimeError if it does not fit now (``max_num_seqs``, or its blocks for its whole life: the shared ones count for
+        each branch, so that any of them may end first)."""
         seq = self.scheduler.running.get(request_id)
         if seq is None or seq.next_token_id is None:
             raise ValueError(f"request {request_id} is not running")
