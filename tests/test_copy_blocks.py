@@ -25,6 +25,7 @@ def test_a_blocks_size_is_that_of_its_values(monkeypatch):
         called.append((list(sizes), n_pools, layers, blocks, n))
         return 0
 
+    _C.load()  # binds _calls
     monkeypatch.setattr(_C, "_lib", SimpleNamespace(nvamd_copy_blocks=copy))
     monkeypatch.setattr(_C, "_calls", None)
     monkeypatch.setattr(_C, "_stream_of", lambda *a: None)
@@ -40,6 +41,7 @@ def test_a_blocks_size_is_that_of_its_values(monkeypatch):
 @pytest.mark.parametrize("at_once", [False, True])
 def test_a_pool_of_one_block_is_left_alone(device, monkeypatch, at_once):
     """Its only pair is the block itself, which is no copy; with another size of a block, a pair in a pool of two."""
+    _C.load()  # binds _calls
     if not at_once:
         monkeypatch.setattr(_C, "_calls", None)
     pool, memory = one_block_pool(5, 16, 3, device=device)
