@@ -87,8 +87,9 @@ __device__ __forceinline__ void keep_here(float (&cs)[8], float (&sn)[8], u32x4 
 template <int ROWS, typename Body>
 __device__ __forceinline__ void for_runs(const RowsArgs &a, int64_t base, int lane, bool report, bool slotless,
                                          Body &&body) {
-  constexpr int kBefore = 64 - ROWS - (kFp8Tile - 1);  // rows of the window before the wave's own; those that a run needs
-  static_assert(kBefore >= 1 && kBefore >= NVAMD_FP8_ORDER_ROWS, "behind them end the window");
+  // Of the window's 64 rows these lie before the wave's own, and behind those the ones that a run may go on in.
+  constexpr int kBefore = 64 - ROWS - (kFp8Tile - 1);
+  static_assert(kBefore >= NVAMD_FP8_ORDER_ROWS);
   const int64_t r = base - kBefore + lane;
   const bool exists = r >= 0 && r < a.num_tokens;
   int64_t slot = exists ? a.slots[r] : -1;
