@@ -322,7 +322,7 @@ prefill_strip_fp4_kernel(PrefillArgs<Fp4Cache> a) {
   };
   auto locate = [&](int t0) {
 #pragma unroll
-    for (int x = 0; x < 2; ++x) tile[x] = tile_of(a, entry[x], min(t0 + 16 * x, last_tile), g, lane == 0);
+    for (int x = 0; x < 2; ++x) tile[x] = tile_of<true>(a, entry[x], min(t0 + 16 * x, last_tile), g, lane == 0);
   };
   // Byte `at` of the lane's one of the two tiles.
   auto in_tile = [&](const u8 *base, int second, int tile_bytes, u32 at) {  // (second as a bool: 25 us for 14)
