@@ -162,8 +162,11 @@ class Fp8PagedKVCache(_QuantisedKVCache):
 
     def write(self, layer_idx: int, key_states: torch.Tensor, value_states: torch.Tensor,
               slot_mapping: torch.Tensor) -> None:
-        """Unlike the other caches' this asks for an order: the rows of a tile follow one another in that of their slots."""
+        """Unlike the other caches' this asks for an order: the rows of a tile follow one another in that of their slots.
+        Slots on the host are checked for it; of slots on the device see ``_C.kv_cache_write_fp8``."""
         self._check_rows(key_states, slot_mapping)
+        if not slot_mapping.is_cuda:
+            _C.check_tile_order(slot_mapping)
         _C.kv_cache_write_fp8(key_states, value_states, *self.get_physical_cache(layer_idx), self._slots(slot_mapping))
 
     def read(self, layer_idx: int, slot_mapping: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:

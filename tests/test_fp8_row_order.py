@@ -38,6 +38,18 @@ def test_the_rule():
     assert "follow one another" in _C.describe_index_errors(_C.ERR_ORDER)
 
 
+def test_host_slots_are_refused_however_far_apart():
+    cache = Fp8PagedKVCache(1, 64, 32, 1, 128, "cpu")
+    far_apart = torch.cat([torch.tensor([64]), 16 * torch.arange(10, 110), torch.tensor([65])])
+    for slots in (torch.tensor([1, 0]), far_apart, far_apart.int(), far_apart[:, None]):
+        k = torch.zeros(slots.numel(), 1, 128, dtype=torch.bfloat16)
+        with pytest.raises(IndexError, match="do not follow one another"):
+            cache.write(0, k, k, slots)
+    k = torch.zeros(3, 1, 128, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="on the GPU"):  # checked, and then refused for where the rows are
+        cache.write(0, k, k, torch.tensor([15, 16, 17]))
+
+
 def rows(t, heads, seed):
     gen = torch.Generator().manual_seed(seed)
     return (torch.randn(t, heads, 128, generator=gen) * torch.exp(torch.randn(t, heads, 1, generator=gen))).bfloat16()
